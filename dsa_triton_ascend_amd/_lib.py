@@ -156,6 +156,44 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32,               # sparse_mode, layout_q, dtype, w_dtype
         _vp,                                  # stream
     ]),
+    "dsa_rope": (_c.c_int, [
+        _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,  # query, out, 6 strides, heads, d, start
+        _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,  # key, likewise
+        _vp, _i32, _i32, _vp,                 # positions, positions_64, positions_per_sequence, inv_freq
+        _i64, _i64, _i64,                     # batch, s1, rotary_dim
+        _i32, _i32, _i32, _f32, _vp,          # interleaved, inverse, dtype, attention_scale, stream
+    ]),
+    "dsa_paged_cache_write": (_c.c_int, [
+        _i64, _vp, _vp, _vp, _vp, _vp,        # n_caches, rows, caches, row_bytes, row_batch_stride, row_token_stride
+        _i32p, _i32p, _i32p,                  # block_table, seq_lengths, row_lengths
+        _i64, _i64, _i64, _i64, _i64, _i64,   # batch, s1, tokens, max_blocks, num_pages, page_size
+        _i32, _vp,                            # layout, stream
+    ]),
+    "dsa_paged_cache_fork_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "dsa_paged_cache_fork": (_c.c_int, [
+        _i64, _vp, _vp,                       # n_caches, caches, row_bytes
+        _i32p, _i32p, _i32p, _i32p,           # block_table, seq_lengths, page_refs, parents
+        _i32p, _i32p, _i32p,                  # new_block_table, new_seq_lengths, new_page_refs
+        _i64, _i64, _i64, _i64, _i64, _i64,   # rows, new_rows, max_blocks, new_max_blocks, num_pages, page_size
+        _i64, _vp, _sz, _vp,                  # new_tokens, workspace, workspace_bytes, stream
+    ]),
+    "dsa_paged_cache_compact_workspace_size": (_sz, [_i64]),
+    "dsa_paged_cache_compact": (_c.c_int, [
+        _i64, _vp, _vp,                       # n_caches, caches, row_bytes
+        _i32p, _i32p, _i32p, _i32p, _i32p,    # block_table, page_refs, new_block_table, new_page_refs, page_map
+        _i64, _i64, _i64, _i64,               # rows, max_blocks, num_pages, page_size
+        _vp, _sz, _vp,                        # workspace, workspace_bytes, stream
+    ]),
+    "dsa_paged_attn_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i64, _i64]),
+    "dsa_paged_attn": (_c.c_int, [
+        _vp, _vp, _vp, _vp, _vp,              # query, query_rope, key, key_rope, value
+        _vp, _vp, _vp,                        # attention_out, softmax_max, softmax_sum
+        _i32p, _i32p, _i32p,                  # actual_seq_q, actual_seq_kv, block_table
+        _i64, _i64, _i64, _i64, _i64, _i64,   # batch, s1, n1, n2, d, d_rope
+        _i64, _i64, _i64,                     # num_blocks, page_size, max_blocks
+        _i32, _i64, _i64, _i32, _f32, _i32,   # sparse_mode, pre_tokens, next_tokens, dtype, scale_value, return_lse
+        _vp, _sz, _vp,                        # workspace, workspace_bytes, stream
+    ]),
 }
 
 _lib = None
@@ -207,6 +245,27 @@ def stream_handle(device):
             idx = device if isinstance(device, int) else torch.device(device).index
         return _raw_stream(torch.cuda.current_device() if idx is None else idx)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class on_device:
+    """The device of a call's tensors, made current while the library plans
+    and launches (sizes such as the CU count and the launch itself go to the
+    current device).  Nothing is done where it is current already."""
+
+    __slots__ = ("idx", "prev")
+
+    def __init__(self, device):
+        self.idx = device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.idx)
+
+    def __exit__(self, *exc):
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.prev)
+        return False
 
 
 def dtype_code(dt):

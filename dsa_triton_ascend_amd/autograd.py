@@ -23,9 +23,12 @@ computes the loss and its gradients for ``query_index``, ``key_index`` and
 gradients; the backward scales them by the incoming gradient. The teacher
 side (query, key, rope and the SFA statistics) carries no gradient, as in
 DSA indexer training, where the KL loss trains only the indexer.
+
+``RotaryEmbeddingFunction`` is the differentiable form of ``rotary_embedding``.
 """
 import torch
 
+from .rotary_embedding import _rotate
 from .sparse_flash_attention import INT64_MAX, sparse_flash_attention_triton
 from .sparse_flash_attention_grad import _sfa_grad
 from .sparse_lightning_indexer_grad_kl_loss import sparse_lightning_indexer_grad_kl_loss_triton
@@ -124,5 +127,33 @@ def sparse_lightning_indexer_kl_loss(query_index, key_index, weights, query, key
         actual_seq_qlen, actual_seq_klen, scale_value, sparse_mode)
 
 
-__all__ = ["SparseFlashAttentionFunction", "sparse_flash_attention_train",
+class RotaryEmbeddingFunction(torch.autograd.Function):
+    """Differentiable rotary positions of a query and an optional key: a
+    rotation's gradient is the rotation by the opposite angles, with the same
+    scale, so nothing of the forward but the positions is kept."""
+
+    @staticmethod
+    def forward(ctx, query, key, positions, inv_freq, interleaved, q_start, k_start, scale, layout, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.args = (interleaved, q_start, k_start, scale, layout)
+        ctx.inverse = inverse
+        ctx.set_materialize_grads(False)
+        return tuple(_rotate(query, key, positions, inv_freq, *ctx.args, inverse, False))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_query, d_key):
+        positions, inv_freq = ctx.saved_tensors
+        interleaved, q_start, k_start, scale, layout = ctx.args
+        d_q = d_query if ctx.needs_input_grad[0] else None
+        d_k = d_key if ctx.needs_input_grad[1] else None
+        if d_q is not None:
+            d_q, d_k = _rotate(d_q, d_k, positions, inv_freq, *ctx.args, not ctx.inverse, False)
+        elif d_k is not None:
+            d_k, _ = _rotate(d_k, None, positions, inv_freq, interleaved, k_start, 0, scale, layout, not ctx.inverse,
+                             False)
+        return (d_q, d_k) + (None,) * 8
+
+
+__all__ = ["RotaryEmbeddingFunction", "SparseFlashAttentionFunction", "sparse_flash_attention_train",
            "SparseLightningIndexerKLLossFunction", "sparse_lightning_indexer_kl_loss", "INT64_MAX"]

@@ -27,6 +27,11 @@ SOURCES = [
     "kl_generic.hip",
     "dense_kl.hip",
     "calib.hip",
+    "capi_decode.cpp",
+    "rope.hip",
+    "paged_cache.hip",
+    "paged_attn.hip",
+    "paged_attn_latent.hip",
 ]
 
 ARCH = os.environ.get("DSA_OFFLOAD_ARCH", "gfx950")
@@ -62,6 +67,8 @@ VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]
 PER_SOURCE_FLAGS = {
     "sfa_fwd.hip": VGPR_FORM,
     "li_fwd.hip": VGPR_FORM,
+    "paged_attn.hip": VGPR_FORM,
+    "paged_attn_latent.hip": VGPR_FORM,
 }
 
 

@@ -20,6 +20,8 @@ void set_error(const char* fmt, ...) {
   va_end(ap);
 }
 
+void clear_error() { g_err[0] = '\0'; }
+
 static std::atomic<int> g_test_flags{0};
 int test_flags() { return g_test_flags.load(std::memory_order_relaxed); }
 

@@ -151,6 +151,7 @@ __device__ __forceinline__ int rope_swz(int tok) { return (tok >> 1) & 7; }
 // ---------------------------------------------------------------------------
 namespace dsa {
 void set_error(const char* fmt, ...);
+void clear_error();
 int hip_fail(hipError_t e, const char* what);
 // CUs of the current device (cached per device; 256 when it cannot be queried)
 int device_cu_count();

@@ -1,0 +1,486 @@
+// Attention of the newest tokens over paged key and value caches with grouped
+// heads, and the join of the runs of a sequence (both described in
+// paged_attn.h).
+//
+//   S^T = K Q^T,  P = 2^(S - ref),  O^T = V^T P^T
+//
+// Bound by the bytes of K and V: 2 (G / 2) flops per byte at G query heads
+// per key head.  So every wave works alone, on its own run of tokens of one
+// key head, with no LDS and no barrier; what it needs in flight sits in
+// registers.  Neighbouring waves take neighbouring key heads of the same
+// tokens, so that the rows of a page are read whole.
+//
+// Per tile of 32 tokens: K goes straight into the A operand of 16x16x32
+// (lane l: token l % 16, 16 bytes of 8 columns).  V is read a row at a time
+// across 16 lanes, each lane 8 tokens x D/16 columns, and turned in the lane
+// by byte permutes into V^T operands: the column a lane's MFMA row stands
+// for, and the token its k slot stands for, are free to choose, and are
+// chosen so that nothing crosses lanes.  Token 16 st + 4 g + r is k slot
+// 8 g + 4 st + r of lane group g, which is also where S^T leaves its score,
+// so P needs no shuffle either.  K of the next tile is loaded as soon as the
+// scores are done, V of the next as soon as the output is.
+//
+// P is multiplied as a sum of two values of the input type (the MFMAs are
+// idle otherwise), so the weights keep 16 bits and more.
+#include "paged_attn.h"
+
+namespace dsa {
+
+__device__ __attribute__((aligned(16))) unsigned char g_paged_zero_row[1024];
+
+constexpr int kPaTile = 32;
+constexpr int kPaThreads = 256;
+
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(kPaThreads, (D * MT <= 128 ? 3 : (D * MT <= 256 ? 2 : 1))) void paged_attn_kernel(
+    PagedAttnParams p) {
+  using E = Elem<T>;
+  using V8 = typename E::v8;
+  constexpr int KS = D / 32;   // k-steps of the scores
+  constexpr int NJ = D / 16;   // output tiles
+  constexpr int VC = D >= 128 ? D / 128 : 1;  // 16-byte pieces of a lane's V row
+  constexpr int EPL = D / 16;  // V columns of a lane
+  const int lane = threadIdx.x & 63;
+  const int li = lane & 15, lg = lane >> 4;
+  const int64_t wid = (int64_t)blockIdx.x * (kPaThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int worker = (int)(wid / p.groups), ng = (int)(wid - (int64_t)worker * p.groups);
+  if (worker >= p.workers) return;
+  const int kvh = ng / p.row_groups, rg = ng - kvh * p.row_groups;
+
+  PagedPlan plan;
+  plan.make(p, kPaTile, lane);
+  int64_t at = (int64_t)worker * plan.per;
+  const int64_t end = min(at + plan.per, plan.total);
+  if (at >= end) return;
+  int64_t before;
+  int b = plan.find(p, kPaTile, lane, at, &before);
+  const int64_t row_bytes = (int64_t)p.n2 * D * 2;
+  const unsigned char* kbase = (const unsigned char*)p.k + (int64_t)kvh * D * 2;
+  const unsigned char* vbase = (const unsigned char*)p.v + (int64_t)kvh * D * 2;
+
+  bool first_segment = true;
+  while (at < end) {
+    b = __builtin_amdgcn_readfirstlane(b);
+    PagedSeq seq = paged_seq(p, b);
+    seq.lo = __builtin_amdgcn_readfirstlane(seq.lo);
+    seq.hi = __builtin_amdgcn_readfirstlane(seq.hi);
+    const int nt = paged_tiles(seq, kPaTile);
+    if (nt == 0) {
+      ++b;
+      continue;
+    }
+    const int t0 = (int)(at - before), t1 = (int)min(end - before, (int64_t)nt);
+    const int tok0 = seq.lo + t0 * kPaTile, tok1 = min(seq.hi, seq.lo + t1 * kPaTile);
+    const int32_t* tab = p.table + (int64_t)b * p.max_blocks;
+
+    // rows of this lane's MFMA column: query head kvh * group + r % group of
+    // token r / group
+    V8 qf[MT][KS];
+    int lo[MT], hi[MT];
+    int64_t orow[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r = rg * p.group_rows + mt * 16 + li;
+      const bool live = r < p.rows;
+      const int s = live ? r / p.group : 0;
+      orow[mt] = live ? ((int64_t)b * p.s1 + s) * p.n1 + kvh * p.group + (r - s * p.group) : -1;
+      paged_bounds(p, seq.act_q, seq.act_k, s, &lo[mt], &hi[mt]);
+      if (!live) hi[mt] = 0;
+      const u32x4 z = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        qf[mt][ks] = as_v8<V8>(live ? *(const u32x4*)((const T*)p.q + orow[mt] * D + ks * 32 + lg * 8) : z);
+    }
+
+    f32x4 acc[MT][NJ];
+    float ref[MT], top[MT], sum[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      ref[mt] = top[mt] = -INFINITY;
+      sum[mt] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[mt][j] = {0.f, 0.f, 0.f, 0.f};
+    }
+
+    // cache row of token tile0 + lane % 32, -1 past the run's end or where
+    // the table names no page
+    auto page_of = [&](int tile0) {
+      const int t = tile0 + (lane & 31);
+      unsigned off;
+      return t < tok1 ? tab[paged_split(p, (unsigned)t, &off)] : -1;
+    };
+    auto row_of = [&](int tile0, int blk) {
+      unsigned off;
+      paged_split(p, (unsigned)(tile0 + (lane & 31)), &off);
+      const int64_t r = (int64_t)blk * p.page + (int)off;
+      return blk < 0 || r >= p.kv_rows ? -1 : (int)r;
+    };
+    u32x4 kf[2][KS];
+    auto load_k = [&](int row) {
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const int r = __shfl(row, st * 16 + li);
+        const unsigned char* src = r >= 0 ? kbase + r * row_bytes : g_paged_zero_row;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kf[st][ks] = *(const u32x4*)(src + ks * 64 + lg * 16);
+      }
+    };
+    typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+    unsigned vf[8][EPL / 2];
+    auto load_v = [&](int row) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = __shfl(row, (i >> 2) * 16 + lg * 4 + (i & 3));
+        const unsigned char* src = r >= 0 ? vbase + r * row_bytes : g_paged_zero_row;
+        if constexpr (D == 64) {
+          const u32x2 x = *(const u32x2*)(src + li * 8);
+          vf[i][0] = x[0], vf[i][1] = x[1];
+        } else {
+#pragma unroll
+          for (int c = 0; c < VC; ++c) {
+            const u32x4 x = *(const u32x4*)(src + c * 256 + li * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vf[i][c * 4 + e] = x[e];
+          }
+        }
+      }
+    };
+
+    int row = row_of(tok0, page_of(tok0));
+    load_k(row);
+    load_v(row);
+    int blk = page_of(tok0 + kPaTile);
+    for (int tk = tok0; tk < tok1; tk += kPaTile) {
+      const int next = row_of(tk + kPaTile, blk);
+      blk = page_of(tk + 2 * kPaTile);
+      f32x4 s[MT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          s[mt][st] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) s[mt][st] = E::mfma(as_v8<V8>(kf[st][ks]), qf[mt][ks], s[mt][st]);
+        }
+      const bool more = tk + kPaTile < tok1;
+      if (more) load_k(next);
+
+      V8 ph[MT], pl[MT];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float v[8], mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int t = tk + (i >> 2) * 16 + lg * 4 + (i & 3);
+          v[i] = t >= lo[mt] && t < hi[mt] ? s[mt][i >> 2][i & 3] * p.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, v[i]);
+        }
+        mx = xgroup_max(mx);
+        top[mt] = fmaxf(top[mt], mx);
+        if (__any(mx > ref[mt] + kPaAbove)) {
+          const float nref = mx > ref[mt] + kPaAbove ? mx - kPaBelow : ref[mt];
+          const float f = ref[mt] == -INFINITY ? 0.f : fast_exp2(ref[mt] - nref);
+          ref[mt] = nref;
+          sum[mt] *= f;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[mt][j] *= f;
+        }
+        const float from = ref[mt] == -INFINITY ? 0.f : ref[mt];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float e = fast_exp2(v[i] - from);
+          sum[mt] += e;
+          ph[mt][i] = E::from_f32(e);
+          pl[mt][i] = E::from_f32(e - E::to_f32(ph[mt][i]));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        // columns EPL-major: piece j / 8 (or j / 4 at D = 64), element j % 8
+        const int dw = j / 2;
+        u32x4 w;
+#pragma unroll
+        for (int q2 = 0; q2 < 4; ++q2)
+          w[q2] = __builtin_amdgcn_perm(vf[2 * q2 + 1][dw], vf[2 * q2][dw], j & 1 ? 0x07060302u : 0x05040100u);
+        const V8 a = as_v8<V8>(w);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          acc[mt][j] = E::mfma(a, ph[mt], acc[mt][j]);
+          acc[mt][j] = E::mfma(a, pl[mt], acc[mt][j]);
+        }
+      }
+      if (more) load_v(next);
+    }
+
+    // MFMA j, register r of lane group g: column 8 (4 g + r) + j % 8 of piece
+    // j / 8 (4 (4 g + r) + j at D = 64), so a lane holds whole chunks
+    const bool whole = t0 == 0 && t1 == nt;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const float l = xgroup_sum(sum[mt]);
+      constexpr int EC = D == 64 ? 4 : 8;  // elements of a chunk
+      if (whole) {
+        if (orow[mt] >= 0) {
+          const float inv = l > 0.f ? 1.f / l : 0.f;
+          typedef T TC __attribute__((ext_vector_type(EC)));
+#pragma unroll
+          for (int c = 0; c < NJ / EC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              TC o;
+#pragma unroll
+              for (int e = 0; e < EC; ++e) o[e] = E::from_f32(acc[mt][c * EC + e][r] * inv);
+              *(TC*)((T*)p.out + orow[mt] * D + c * 128 + (lg * 4 + r) * EC) = o;
+            }
+          if (lg == 0 && p.smax) {
+            // statistics are [B, N2, S1, G]
+            const int rr = rg * p.group_rows + mt * 16 + li;
+            const int64_t at2 = ((int64_t)b * p.n2 + kvh) * p.rows + rr;
+            const bool any = p.return_lse && l > 0.f;
+            p.smax[at2] = any ? top[mt] * kLn2 : 0.f;
+            p.ssum[at2] = any ? l * fast_exp2(ref[mt] - top[mt]) : 0.f;
+          }
+        }
+      } else {
+        const int64_t slot = (((int64_t)worker * 2 + (first_segment ? 0 : 1)) * p.groups + ng) * p.group_rows +
+                             mt * 16 + li;
+        float* dst = p.part_o + slot * D;
+#pragma unroll
+        for (int c = 0; c < NJ / EC; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < EC; e += 4) {
+              const f32x4 o = {acc[mt][c * EC + e][r], acc[mt][c * EC + e + 1][r], acc[mt][c * EC + e + 2][r],
+                               acc[mt][c * EC + e + 3][r]};
+              *(f32x4*)(dst + c * 128 + (lg * 4 + r) * EC + e) = o;
+            }
+        if (lg == 0) p.part_ml[slot] = {ref[mt], l, top[mt], l};
+      }
+    }
+    first_segment = false;
+    at = before + t1;
+    if (t1 == nt) {
+      before += nt;
+      ++b;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// join: one workgroup per (sequence, row).  A row of D floats is read by
+// D / 4 lanes, so 256 / (D / 4) runs are read side by side, four deep.
+// Sequences without a visible token get their zeros here.
+// ---------------------------------------------------------------------------
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, int tile) {
+  using E = Elem<T>;
+  constexpr int LPR = D / 4;
+  constexpr int PAR = 256 / LPR;
+  __shared__ f32x4 s_o[256];
+  __shared__ float s_l[PAR], s_n[PAR];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int per_seq = p.n2 * p.rows;
+  const int b = blockIdx.x / per_seq;
+  const int rest = blockIdx.x - b * per_seq;
+  const int kvh = rest / p.rows, rr = rest - kvh * p.rows;  // row rr = s * group + head
+  const int rg = rr / p.group_rows, ng = kvh * p.row_groups + rg;
+  const int s = rr / p.group;
+  const int64_t orow = ((int64_t)b * p.s1 + s) * p.n1 + kvh * p.group + (rr - s * p.group);
+  const int64_t srow = ((int64_t)b * p.n2 + kvh) * p.rows + rr;
+
+  PagedPlan plan;
+  plan.make(p, tile, lane);
+  const int nt = paged_tiles(paged_seq(p, b), tile);
+  const int64_t first = plan.start(p, tile, lane, b), last = first + nt - 1;
+  const int64_t w0 = nt ? first / plan.per : 0, w1 = nt ? last / plan.per : -1;
+  if (nt && w0 == w1) return;  // written whole by its worker
+
+  const int c = tid % LPR, part = tid / LPR;
+  auto slot = [&](int64_t w) {
+    const int k = w == w0 && first != w * plan.per ? 1 : 0;
+    return ((w * 2 + k) * p.groups + ng) * p.group_rows + (rr - rg * p.group_rows);
+  };
+  float big = -INFINITY, top = -INFINITY;
+  for (int64_t w = w0 + lane; w <= w1; w += 64) {
+    const f32x4 ml = p.part_ml[slot(w)];
+    big = fmaxf(big, ml[0]);
+    top = fmaxf(top, ml[2]);
+  }
+  big = wave_max(big);
+  top = wave_max(top);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f, norm = 0.f;
+  if (big != -INFINITY) {
+#pragma unroll 4
+    for (int64_t w = w0 + part; w <= w1; w += PAR) {
+      const int64_t at = slot(w);
+      const f32x4 ml = p.part_ml[at];
+      const f32x4 x = *(const f32x4*)(p.part_o + at * D + c * 4);
+      const float f = fast_exp2(ml[0] - big);
+      o += x * f;
+      l += ml[1] * f;
+      norm += ml[3] * f;
+    }
+  }
+  s_o[tid] = o;
+  if (c == 0) s_l[part] = l, s_n[part] = norm;
+  __syncthreads();
+  if (part == 0) {
+    l = s_l[0];
+    norm = s_n[0];
+#pragma unroll
+    for (int i = 1; i < PAR; ++i) {
+      o += s_o[i * LPR + c];
+      l += s_l[i];
+      norm += s_n[i];
+    }
+    const float inv = norm > 0.f ? 1.f / norm : 0.f;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const T4 r = {E::from_f32(o[0] * inv), E::from_f32(o[1] * inv), E::from_f32(o[2] * inv), E::from_f32(o[3] * inv)};
+    *(T4*)((T*)p.out + orow * D + c * 4) = r;
+    if (c == 0 && p.smax) {
+      const bool any = p.return_lse && l > 0.f;
+      p.smax[srow] = any ? top * kLn2 : 0.f;
+      p.ssum[srow] = any ? l * fast_exp2(big - top) : 0.f;
+    }
+  }
+}
+
+template <typename T>
+static void paged_combine_d(const PagedAttnParams& p, int tile, int64_t d, unsigned grid, hipStream_t stream) {
+  if (d == 64) paged_combine_kernel<T, 64><<<grid, 256, 0, stream>>>(p, tile);
+  else if (d == 128) paged_combine_kernel<T, 128><<<grid, 256, 0, stream>>>(p, tile);
+  else if (d == 256) paged_combine_kernel<T, 256><<<grid, 256, 0, stream>>>(p, tile);
+  else paged_combine_kernel<T, 512><<<grid, 256, 0, stream>>>(p, tile);
+}
+
+int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream) {
+  const unsigned grid = (unsigned)((int64_t)p.batch * p.n2 * p.rows);
+  if (dtype == DSA_DTYPE_BF16) paged_combine_d<bf16>(p, tile, d, grid, stream);
+  else paged_combine_d<f16>(p, tile, d, grid, stream);
+  DSA_HIP(hipGetLastError());
+  return DSA_OK;
+}
+
+size_t paged_part_bytes(const PagedShape& s, int64_t d) {
+  return (size_t)s.workers * 2 * s.groups * s.group_rows * (d * sizeof(float) + sizeof(f32x4));
+}
+
+// Workers of a lane group for `slots` workers resident at once.  As many as
+// fill the slots once; where the lane groups alone come near that, so many
+// that the last round of them is nearly full too.  Never more than the
+// longest lengths keep busy.
+int paged_workers(int64_t slots, int64_t groups, int64_t tiles, int min_tiles) {
+  int64_t best = slots / groups;
+  if (best < 8) {
+    double best_fill = 0;
+    const int64_t from = best < 1 ? 1 : best;
+    for (int64_t w = from; w < from + 8; ++w) {
+      const int64_t all = w * groups, rounds = (all + slots - 1) / slots;
+      const double fill = (double)all / ((double)rounds * slots);
+      if (fill > best_fill + 0.02) best = w, best_fill = fill;
+    }
+  }
+  const int64_t most = (tiles + min_tiles - 1) / min_tiles;
+  return (int)(best > most ? (most < 1 ? 1 : most) : best);
+}
+
+static PagedShape paged_grouped_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d,
+                                      int64_t max_blocks, int64_t page) {
+  PagedShape s;
+  s.tile = kPaTile;
+  const int64_t rows = s1 * (n1 / n2);
+  int mt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+  if (d * mt > 512) mt = 2;
+  s.group_rows = mt * 16;
+  s.row_groups = (int)((rows + s.group_rows - 1) / s.group_rows);
+  s.groups = (int)n2 * s.row_groups;
+  s.min_tiles = 4;
+  const int waves = d * mt <= 128 ? 12 : (d * mt <= 256 ? 8 : 4);  // of a CU, as many as registers allow
+  s.workers = paged_workers((int64_t)device_cu_count() * waves, s.groups,
+                            batch * ((max_blocks * page + kPaTile - 1) / kPaTile), s.min_tiles);
+  return s;
+}
+
+static PagedShape paged_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
+                              int64_t max_blocks, int64_t page) {
+  return latent ? paged_latent_shape(batch, s1, n1, d, max_blocks, page)
+                : paged_grouped_shape(batch, s1, n1, n2, d, max_blocks, page);
+}
+
+size_t paged_attn_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
+                                  int64_t max_blocks, int64_t page) {
+  return paged_part_bytes(paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page), d);
+}
+
+template <typename T, int D>
+static void paged_launch_mt(const PagedAttnParams& p, unsigned grid, hipStream_t stream) {
+  if (p.group_rows == 16) paged_attn_kernel<T, D, 1><<<grid, kPaThreads, 0, stream>>>(p);
+  else if (p.group_rows == 32) paged_attn_kernel<T, D, 2><<<grid, kPaThreads, 0, stream>>>(p);
+  else if constexpr (D <= 128) paged_attn_kernel<T, D, 4><<<grid, kPaThreads, 0, stream>>>(p);
+}
+
+template <typename T>
+static void paged_launch(const PagedAttnParams& p, int64_t d, unsigned grid, hipStream_t stream) {
+  if (d == 64) paged_launch_mt<T, 64>(p, grid, stream);
+  else if (d == 128) paged_launch_mt<T, 128>(p, grid, stream);
+  else paged_launch_mt<T, 256>(p, grid, stream);
+}
+
+int paged_attn_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
+                   const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
+                   const int32_t* act_k, const int32_t* table, int64_t batch, int64_t s1, int64_t n1, int64_t n2,
+                   int64_t d, int64_t num_blocks, int64_t page, int64_t max_blocks, int32_t mode, int64_t pre_tokens,
+                   int64_t next_tokens, int32_t dtype, float scale, int32_t return_lse, void* workspace,
+                   hipStream_t stream) {
+  const bool latent = value == nullptr;
+  const PagedShape s = paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
+  PagedAttnParams p = {};
+  p.q = query;
+  p.qr = query_rope;
+  p.k = key;
+  p.kr = key_rope;
+  p.v = value;
+  p.out = out;
+  p.smax = smax;
+  p.ssum = ssum;
+  p.act_q = act_q;
+  p.act_k = act_k;
+  p.table = table;
+  p.part_o = (float*)workspace;
+  p.part_ml = (f32x4*)(p.part_o + (int64_t)s.workers * 2 * s.groups * s.group_rows * d);
+  p.kv_rows = num_blocks * page;
+  p.band_pre = band_clamp(pre_tokens);
+  p.band_next = band_clamp(next_tokens);
+  p.batch = (int)batch;
+  p.s1 = (int)s1;
+  p.n1 = (int)n1;
+  p.n2 = (int)n2;
+  p.group = (int)(n1 / n2);
+  p.rows = (int)(s1 * p.group);
+  p.max_blocks = (int)max_blocks;
+  p.page = (int)page;
+  p.mode = mode;
+  p.return_lse = return_lse;
+  p.workers = s.workers;
+  p.min_tiles = s.min_tiles;
+  p.groups = s.groups;
+  p.row_groups = s.row_groups;
+  p.group_rows = s.group_rows;
+  p.page_magic = 0xffffffffu / (unsigned)page;
+  p.scale_log2 = scale * kLog2e;
+  if (latent) {
+    const int st = paged_latent_launch(p, d, dtype, stream);
+    if (st != DSA_OK) return st;
+  } else {
+    const int64_t waves = (int64_t)s.workers * s.groups;
+    const unsigned grid = (unsigned)((waves + kPaThreads / 64 - 1) / (kPaThreads / 64));
+    if (dtype == DSA_DTYPE_BF16) paged_launch<bf16>(p, d, grid, stream);
+    else paged_launch<f16>(p, d, grid, stream);
+    DSA_HIP(hipGetLastError());
+  }
+  return paged_combine_launch(p, s.tile, d, dtype, stream);
+}
+
+}  // namespace dsa

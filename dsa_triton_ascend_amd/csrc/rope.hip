@@ -1,0 +1,199 @@
+// Rotary positions: the pairs (a, b) of a head's rotary slice turned by the
+// angle position * inv_freq[i],
+//   a' = s (a cos - b sin),  b' = s (a sin + b cos),
+// with pairs of adjacent columns (interleaved) or of columns i and i + R/2
+// (half).  The backward is the rotation by the opposite angle, the same
+// kernel with the sine negated.
+//
+// The angle is formed in 64 bits, as turns: position * inv_freq / 2 pi less
+// its nearest integer is exact to 2^-33 of a turn at position 2^20, where a
+// 32-bit product is off by 0.06 rad.  The sine and cosine of what is left
+// are taken in 32 bits, once per token and frequency, into LDS; all heads of
+// the token share them.  No table of positions is read or kept.
+//
+// Bound by memory (3 flops per element), or by the launch for one decoding
+// step.  A thread moves 16 bytes (two times 16 for pairs in the half layout),
+// neighbouring threads neighbouring chunks of a head; heads and tokens are
+// flattened, so that no lane idles at any head count.  Query and key go in
+// one launch.
+#include "common.h"
+
+namespace dsa {
+
+struct RopeTensor {
+  const void* in;
+  void* out;
+  int64_t in_sb, in_ss, in_sh;     // strides in elements: batch, token, head
+  int64_t out_sb, out_ss, out_sh;
+  int heads, d, start;             // head columns, first rotated column
+  int units;                       // work units of a head
+  int total;                       // heads * units
+};
+
+struct RopeParams {
+  RopeTensor t[2];
+  const void* pos;
+  const double* inv_freq;
+  int64_t tokens;
+  int s;               // tokens of a sequence (BSND); tokens for packed rows
+  int pos64, pos_per_seq;
+  int rot, rot_units, interleaved;
+  int tok_wg, parts, per_part;     // tokens of a workgroup; unit ranges they are cut into
+  float scale, sign;
+};
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeTab = 4096;  // cos and sin values of a workgroup's tokens
+
+template <typename T> struct RopeIo {
+  static __device__ __forceinline__ float get(T x) { return Elem<T>::to_f32(x); }
+  static __device__ __forceinline__ T put(float x) { return Elem<T>::from_f32(x); }
+};
+template <> struct RopeIo<float> {
+  static __device__ __forceinline__ float get(float x) { return x; }
+  static __device__ __forceinline__ float put(float x) { return x; }
+};
+
+// VEC elements per chunk: 16 bytes, or 1 where sizes, strides or addresses
+// do not allow it (a unit is then one pair, or one column that is copied).
+template <typename T, int VEC>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeParams p) {
+  typedef T Vec __attribute__((ext_vector_type(VEC)));
+  using Io = RopeIo<T>;
+  __shared__ float s_tab[kRopeTab];
+  const int half = p.rot / 2;
+  const int64_t tok0 = (int64_t)(blockIdx.x / p.parts) * p.tok_wg;
+  const int ntok = (int)min((int64_t)p.tok_wg, p.tokens - tok0);
+  for (int i = threadIdx.x; i < ntok * half; i += kRopeThreads) {
+    const int tk = i / half, f = i - tk * half;
+    const int64_t t = tok0 + tk;
+    const int64_t pi = p.pos_per_seq ? t : t % p.s;
+    const double pos = p.pos64 ? (double)((const int64_t*)p.pos)[pi] : (double)((const int32_t*)p.pos)[pi];
+    const double turns = pos * (p.inv_freq[f] * 0.15915494309189533577);  // 1 / (2 pi)
+    float sn, cs;
+    sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+    s_tab[2 * i] = cs * p.scale;
+    s_tab[2 * i + 1] = sn * p.scale * p.sign;
+  }
+  __syncthreads();
+  const int all = p.t[0].total + p.t[1].total;
+  const int u0 = (blockIdx.x % p.parts) * p.per_part;
+  const int u1 = min(u0 + p.per_part, all * ntok);
+  for (int u = u0 + threadIdx.x; u < u1; u += kRopeThreads) {
+    const int tk = ntok == 1 ? 0 : u / all;
+    int r = u - tk * all;
+    const int which = r >= p.t[0].total;
+    const RopeTensor& x = p.t[which];
+    r -= which ? p.t[0].total : 0;
+    const int h = r / x.units, c = r - h * x.units;
+    const int64_t t = tok0 + tk, b = t / p.s, s = t - b * p.s;
+    const T* in = (const T*)x.in + b * x.in_sb + s * x.in_ss + h * x.in_sh;
+    T* out = (T*)x.out + b * x.out_sb + s * x.out_ss + h * x.out_sh;
+    const float* tab = s_tab + tk * p.rot;
+    if (c >= p.rot_units) {  // a column chunk outside the rotary slice
+      int col = (c - p.rot_units) * VEC;
+      if (col >= x.start) col += p.rot;
+      *(Vec*)(out + col) = *(const Vec*)(in + col);
+    } else if (VEC > 1 && p.interleaved) {
+      const int col = x.start + c * VEC;
+      const Vec v = *(const Vec*)(in + col);
+      Vec w;
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) {
+        const float cs = tab[c * VEC + 2 * j], sn = tab[c * VEC + 2 * j + 1];
+        const float a = Io::get(v[2 * j]), bb = Io::get(v[VEC > 1 ? 2 * j + 1 : 0]);
+        w[2 * j] = Io::put(a * cs - bb * sn);
+        w[VEC > 1 ? 2 * j + 1 : 0] = Io::put(a * sn + bb * cs);
+      }
+      *(Vec*)(out + col) = w;
+    } else {
+      // pairs c * VEC ..: columns i and i + R/2, or (VEC = 1) 2i and 2i + 1
+      const int ca = x.start + (p.interleaved ? 2 * c : c * VEC);
+      const int cb = p.interleaved ? ca + 1 : ca + half;
+      const Vec va = *(const Vec*)(in + ca), vb = *(const Vec*)(in + cb);
+      Vec wa, wb;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float cs = tab[2 * (c * VEC + j)], sn = tab[2 * (c * VEC + j) + 1];
+        const float a = Io::get(va[j]), bb = Io::get(vb[j]);
+        wa[j] = Io::put(a * cs - bb * sn);
+        wb[j] = Io::put(a * sn + bb * cs);
+      }
+      *(Vec*)(out + ca) = wa;
+      *(Vec*)(out + cb) = wb;
+    }
+  }
+}
+
+template <typename T>
+static void rope_launch(const RopeParams& p, int vec, int64_t grid, hipStream_t stream) {
+  if (vec > 1)
+    rope_kernel<T, 16 / (int)sizeof(T)><<<dim3((unsigned)grid), kRopeThreads, 0, stream>>>(p);
+  else
+    rope_kernel<T, 1><<<dim3((unsigned)grid), kRopeThreads, 0, stream>>>(p);
+}
+
+// strides: in (batch, token, head) then out, in elements
+int rope_run(const void* const in[2], void* const out[2], const int64_t* const strides[2], const int64_t heads[2],
+             const int64_t d[2], const int64_t start[2], int n, const void* positions, int32_t pos64,
+             int32_t pos_per_seq, const double* inv_freq, int64_t tokens, int64_t s, int64_t rot, int32_t interleaved,
+             int32_t inverse, int32_t dtype, float scale, hipStream_t stream) {
+  const int es = dtype == DSA_DTYPE_FP32 ? 4 : 2;
+  const int full = 16 / es;
+  // 16-byte chunks: every column count, offset, stride and address a whole
+  // number of them
+  bool wide = (interleaved ? rot : rot / 2) % full == 0;
+  for (int i = 0; i < n; ++i) {
+    wide &= d[i] % full == 0 && start[i] % full == 0;
+    wide &= (((uintptr_t)in[i] | (uintptr_t)out[i]) & 15) == 0;
+    for (int j = 0; j < 6; ++j) wide &= strides[i][j] % full == 0;
+  }
+  const int vec = wide ? full : 1;
+  RopeParams p = {};
+  p.rot = (int)rot;
+  p.interleaved = interleaved;
+  p.rot_units = (int)(wide ? (interleaved ? rot : rot / 2) / vec : rot / 2);
+  int64_t all = 0;
+  for (int i = 0; i < n; ++i) {
+    RopeTensor& x = p.t[i];
+    x.in = in[i];
+    x.out = out[i];
+    x.in_sb = strides[i][0], x.in_ss = strides[i][1], x.in_sh = strides[i][2];
+    x.out_sb = strides[i][3], x.out_ss = strides[i][4], x.out_sh = strides[i][5];
+    x.heads = (int)heads[i];
+    x.d = (int)d[i];
+    x.start = (int)start[i];
+    // in place, the columns outside the slice stay as they are
+    x.units = p.rot_units + (in[i] == out[i] ? 0 : (int)((d[i] - rot) / vec));
+    x.total = x.heads * x.units;
+    all += x.total;
+  }
+  p.pos = positions;
+  p.inv_freq = inv_freq;
+  p.tokens = tokens;
+  p.s = (int)s;
+  p.pos64 = pos64;
+  p.pos_per_seq = pos_per_seq;
+  p.scale = scale;
+  p.sign = inverse ? -1.f : 1.f;
+  // tokens of few units share a workgroup; tokens of many are cut into parts
+  // where they alone would not give every CU a few workgroups
+  p.tok_wg = 1;
+  while (p.tok_wg < 16 && p.tok_wg * all < kRopeThreads && 2 * p.tok_wg * rot <= kRopeTab) p.tok_wg *= 2;
+  const int64_t groups = (tokens + p.tok_wg - 1) / p.tok_wg;
+  const int64_t units = p.tok_wg * all;
+  int64_t parts = 4ll * device_cu_count() / groups;
+  const int64_t most = (units + kRopeThreads - 1) / kRopeThreads;
+  parts = parts < 1 ? 1 : (parts > most ? most : parts);
+  p.per_part = (int)(((units + parts - 1) / parts + kRopeThreads - 1) / kRopeThreads * kRopeThreads);
+  p.parts = (int)((units + p.per_part - 1) / p.per_part);
+  const int64_t grid = groups * p.parts;
+  DSA_CHECK_SUPPORTED(grid < (1ll << 31), "too many tokens");
+  if (dtype == DSA_DTYPE_BF16) rope_launch<bf16>(p, vec, grid, stream);
+  else if (dtype == DSA_DTYPE_FP16) rope_launch<f16>(p, vec, grid, stream);
+  else rope_launch<float>(p, vec, grid, stream);
+  DSA_HIP(hipGetLastError());
+  return DSA_OK;
+}
+
+}  // namespace dsa

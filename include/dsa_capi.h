@@ -398,6 +398,117 @@ int dsa_li_scores_paged(const void* query, const void* key_cache, const void* we
                         int64_t page_size, int64_t max_blocks, int32_t sparse_mode,
                         int32_t layout_query, int32_t dtype, int32_t weights_dtype, void* stream);
 
+/*
+ * Rotary positions of a query and, in the same launch, a key (no reference
+ * counterpart: the reference takes rotated query_rope / key_rope).  Every
+ * head's columns [start, start + rotary_dim) are turned, pair i by the angle
+ * position * inv_freq[i], and multiplied by attention_scale:
+ *   a' = s (a cos - b sin), b' = s (a sin + b cos)
+ * on columns (2i, 2i + 1) (interleaved) or (i, i + rotary_dim / 2); inverse
+ * turns the other way, which is the gradient.  The other columns are copied,
+ * or left alone where the output is the input.  query [B, S1, heads, d] with
+ * element strides sb / ss / sh (batch, token, head; a packed [T, heads, d]
+ * has batch 1 and s1 = T) and columns next to each other, likewise key and
+ * the outputs.  An output is its input exactly, with the same strides, or
+ * does not overlap it.  positions: int32, or int64 (positions_64), one per token of
+ * every sequence (positions_per_sequence: [B, S1]) or shared by all ([S1]);
+ * inv_freq: rotary_dim / 2 doubles on the device.  Angles are formed in 64
+ * bits.  dtype BF16, FP16 or FP32; rotary_dim even, up to 1024.
+ */
+int dsa_rope(const void* query, void* query_out, int64_t q_in_sb, int64_t q_in_ss, int64_t q_in_sh, int64_t q_out_sb,
+             int64_t q_out_ss, int64_t q_out_sh, int64_t q_heads, int64_t q_d, int64_t q_start, const void* key,
+             void* key_out, int64_t k_in_sb, int64_t k_in_ss, int64_t k_in_sh, int64_t k_out_sb, int64_t k_out_ss,
+             int64_t k_out_sh, int64_t k_heads, int64_t k_d, int64_t k_start, const void* positions,
+             int32_t positions_64, int32_t positions_per_sequence, const double* inv_freq, int64_t batch, int64_t s1,
+             int64_t rotary_dim, int32_t interleaved, int32_t inverse, int32_t dtype, float attention_scale,
+             void* stream);
+
+/*
+ * Pages of a cache.  A cache is [num_pages, page_size, row] with rows of
+ * row_bytes[i] bytes next to each other; the n_caches caches of a call (host
+ * arrays of device pointers) share block_table, int32 [rows, max_blocks].
+ * No reference counterpart (the reference reads paged caches only).
+ *
+ * Write: token s of sequence b (layout BSND: rows [B, S1] with byte strides
+ * row_batch_stride / row_token_stride, the first row_lengths[b] of them, all
+ * if NULL; TND: packed rows [tokens], row_lengths cumulative) goes to position
+ * seq_lengths[b] + s of the sequence.  Tokens without a page (past the
+ * table's width, a -1 entry) and packed rows behind the last sequence are
+ * dropped.  No page may be written through two rows of the table in one call.
+ */
+int dsa_paged_cache_write(int64_t n_caches, const void* const* rows, void* const* caches, const int64_t* row_bytes,
+                          const int64_t* row_batch_stride, const int64_t* row_token_stride, const int32_t* block_table,
+                          const int32_t* seq_lengths, const int32_t* row_lengths, int64_t batch, int64_t s1,
+                          int64_t tokens, int64_t max_blocks, int64_t num_pages, int64_t page_size, int32_t layout,
+                          void* stream);
+
+/*
+ * Fork: the block table of the next step.  New row c continues row parents[c]
+ * (negative or out of range: an empty row; parents NULL: row c continues row
+ * c), with pages for new_tokens more tokens.  Rows that nobody continues are
+ * released.  Full pages are shared.  The last page, where partly filled, is
+ * kept by the first row that continues its sequence, if page_refs counts
+ * nobody else on it, and is copied, up to its last token, for every other.
+ * Pages are taken from those with page_refs 0 before the call, in ascending
+ * order, for rows in ascending order; a row for which they do not last (or
+ * that outgrows new_max_blocks) gets an empty row with length -1.  Entries of
+ * the old table past a sequence's last token are released.  new_page_refs is
+ * page_refs changed by the entries of the new and the old table.  A negative
+ * length counts as 0.  The new arrays are not the old ones; only the copied
+ * pages of the caches are written (n_caches may be 0: tables only).
+ */
+size_t dsa_paged_cache_fork_workspace_size(int64_t rows, int64_t new_rows, int64_t num_pages);
+int dsa_paged_cache_fork(int64_t n_caches, void* const* caches, const int64_t* row_bytes, const int32_t* block_table,
+                         const int32_t* seq_lengths, const int32_t* page_refs, const int32_t* parents,
+                         int32_t* new_block_table, int32_t* new_seq_lengths, int32_t* new_page_refs, int64_t rows,
+                         int64_t new_rows, int64_t max_blocks, int64_t new_max_blocks, int64_t num_pages,
+                         int64_t page_size, int64_t new_tokens, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/*
+ * Compact: the n pages with page_refs > 0 go to the ids below n.  Pages
+ * already there stay; the k-th of the others, in ascending order, moves to
+ * the k-th free id.  page_map [num_pages] gets each page's new id (-1: was
+ * free); table and counts follow (entries that name a free page become -1).
+ * new_block_table may be block_table.
+ */
+size_t dsa_paged_cache_compact_workspace_size(int64_t num_pages);
+int dsa_paged_cache_compact(int64_t n_caches, void* const* caches, const int64_t* row_bytes,
+                            const int32_t* block_table, const int32_t* page_refs, int32_t* new_block_table,
+                            int32_t* new_page_refs, int32_t* page_map, int64_t rows, int64_t max_blocks,
+                            int64_t num_pages, int64_t page_size, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/*
+ * Attention of the newest tokens of each sequence over every cached token
+ * that they see (the dense counterpart of dsa_sfa_fwd's paged decode; no
+ * reference counterpart).  Two forms:
+ *   grouped  key, value [num_blocks, page_size, N2, D], D in {64, 128, 256},
+ *            query head n uses key head n / (N1 / N2); query_rope, key_rope
+ *            NULL and d_rope 0
+ *   latent   value NULL: N2 = 1, value = key, D in {128, 256, 512}, with
+ *            query_rope / key_rope of 64 columns, as in dsa_sfa_fwd
+ * query [B, S1, N1, D], dtype BF16 or FP16.  actual_seq_kv [B]: tokens in the
+ * cache, the new ones among them (required; negative counts as 0, more than
+ * the table holds as that); actual_seq_q [B]: new tokens (NULL: S1), the rows
+ * after them give zeros.  sparse_mode, pre_tokens and next_tokens as in
+ * dsa_sfa_fwd (mode 3: new token s1 sees act_kv - act_q + s1 + 1 tokens).
+ * Block-table entries outside the cache read as zero rows.  Writes
+ * attention_out [B, S1, N1, D] and, where given, softmax_max / softmax_sum
+ * [B, N2, S1, N1 / N2] (zeros unless return_lse); rows that see nothing give
+ * zeros.  Tensors are 16-byte aligned.  The workspace size depends on sizes
+ * alone (lengths are read on the device).
+ */
+size_t dsa_paged_attn_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, int32_t latent,
+                                     int64_t max_blocks, int64_t page_size);
+int dsa_paged_attn(const void* query, const void* query_rope, const void* key, const void* key_rope,
+                   const void* value, void* attention_out, float* softmax_max, float* softmax_sum,
+                   const int32_t* actual_seq_q, const int32_t* actual_seq_kv, const int32_t* block_table,
+                   int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, int64_t d_rope, int64_t num_blocks,
+                   int64_t page_size, int64_t max_blocks, int32_t sparse_mode, int64_t pre_tokens,
+                   int64_t next_tokens, int32_t dtype, float scale_value, int32_t return_lse, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
