@@ -100,22 +100,22 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   const bool rope_wave = wave < 4;
   const unsigned char* const kbase = (const unsigned char*)p.k;
   const unsigned char* const rbase = (const unsigned char*)p.kr;
-  // this lane's part in the two products
-  const int g1b = nope_off(li, 0) + ((lg ^ nope_swz(li)) * 16);
-  const int g1rb = rope_off(li, 0) + ((lg ^ rope_swz(li)) * 16);
+  // this lane's addresses in the two products, made anew from the lane's
+  // number in every step: kept, they would push Q or the output out of the
+  // registers
+  auto fresh_lane = []() {
+    int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(ln));
+    return ln;
+  };
   constexpr int G1_TT = ((16 / TPI) * NBUF) * 1024;
   constexpr int G1R_TT = 2 * NBUF * 1024;
-  const int r1 = lg * 4 + (li >> 2);
-  const int g2b = nope_off(r1, 0) + ((((li & 3) >> 1) ^ nope_swz(r1)) * 16) + (li & 1) * 8;
-  const int pb = li * PROW + ((lg ^ ((li >> 2) & 3)) * 16);
-  const int pw = (hq * 16 + li) * PROW + ((lg ^ ((li >> 2) & 3)) * 16);
-  auto a1 = [&](int buf, int ks, int tt) -> V8 {
-    if (ks < KSN)
-      return as_v8<V8>(*(const u32x4*)(smem + ((g1b ^ ((ks & 3) << 6)) + tt * G1_TT + buf * 1024 + (ks >> 2) * 256)));
-    return as_v8<V8>(*(const u32x4*)(smem + ((g1rb ^ ((ks - KSN) << 6)) + tt * G1R_TT + buf * 1024)));
+  auto a1 = [&](int g1b, int g1rb, int ks, int tt) -> V8 {
+    if (ks < KSN) return as_v8<V8>(*(const u32x4*)(smem + ((g1b ^ ((ks & 3) << 6)) + tt * G1_TT + (ks >> 2) * 256)));
+    return as_v8<V8>(*(const u32x4*)(smem + ((g1rb ^ ((ks - KSN) << 6)) + tt * G1R_TT)));
   };
-  auto a2 = [&](int buf, int dt) -> V8 {
-    const unsigned char* pp = smem + ((g2b ^ ((dt & 7) << 5)) + buf * 1024 + (dt >> 3) * 256);
+  auto a2 = [&](int g2b, int dt) -> V8 {
+    const unsigned char* pp = smem + ((g2b ^ ((dt & 7) << 5)) + (dt >> 3) * 256);
     const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)pp);
     const bf16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(pp + G1_TT));
     const i16x4 w1 = __builtin_bit_cast(i16x4, v1), w2 = __builtin_bit_cast(i16x4, v2);
@@ -146,12 +146,12 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     {
       const int s = live ? rr / p.n1 : 0;
       const int64_t qrow = (int64_t)b * p.rows + (live ? rr : 0);
-      const u32x4 z = {0u, 0u, 0u, 0u};
+      // (rows that do not exist read row 0; what they compute is not stored)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const T* src = ks < KSN ? (const T*)p.q + qrow * D + ks * 32 + lg * 8
                                 : (const T*)p.qr + qrow * DR + (ks - KSN) * 32 + lg * 8;
-        qf[ks] = as_v8<V8>(live ? *(const u32x4*)src : z);
+        qf[ks] = as_v8<V8>(*(const u32x4*)src);
       }
       if (live) paged_bounds(p, seq.act_q, seq.act_k, s, &lo, &hi);
     }
@@ -159,8 +159,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     // would be one for the tiles in flight too
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
-    // tokens that all of the wave's rows see need no mask (rows that do not
-    // exist compute what is never stored)
+    // tokens that all of the wave's rows see need no mask
     int all_lo = live ? lo : 0, all_hi = live ? hi : 0x7fffffff;
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) {
@@ -190,6 +189,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       const int n_tiles = (tb - ta + TILE - 1) / TILE;
 
       auto issue = [&](int t, int buf) {
+        const int lane = fresh_lane();
         // lane l < 32 finds token l's row, -1 past the end or without a page
         const int tok = ta + t * TILE + (lane & 31);
         int row = -1;
@@ -219,9 +219,24 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       f32x4 s[NTT];
       auto gemm1 = [&](int buf) {
         f32x4 a[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        // two accumulators, so that neighbouring MFMAs are independent
+        // (sub-tiles, or even and odd k-steps); PF fragments read ahead, and
+        // no more (the accumulators leave few registers)
+        constexpr int NS = KS * NTT, PF = 4;
+        const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
+        const int g1b = nope_off(l, 0) + ((g ^ nope_swz(l)) * 16) + buf * 1024;
+        const int g1rb = rope_off(l, 0) + ((g ^ rope_swz(l)) * 16) + buf * 1024;
+        auto read = [&](int st) { return a1(g1b, g1rb, st / NTT, NTT == 1 ? th : st % NTT); };
+        V8 fa[PF];
 #pragma unroll
-        for (int st = 0; st < KS * NTT; ++st)
-          a[st & 1] = E::mfma(a1(buf, st / NTT, NTT == 1 ? th : st % NTT), qf[st / NTT], a[st & 1]);
+        for (int i = 0; i < PF; ++i) fa[i] = read(i);
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+          const V8 f = fa[st % PF];
+          if (st + PF < NS) fa[st % PF] = read(st + PF);
+          a[st & 1] = E::mfma(f, qf[st / NTT], a[st & 1]);
+          if constexpr (HG == 128) __builtin_amdgcn_sched_barrier(0);
+        }
         if constexpr (NTT == 1) s[0] = a[0] + a[1];
         else s[0] = a[0], s[1] = a[1];
       };
@@ -246,39 +261,51 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       };
       auto numerators = [&](int par) {
         const float from = ref == -INFINITY ? 0.f : ref;
-        unsigned char* dst = s_p + par * (NPB * HG * PROW) + pw;
+        const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
+        unsigned char* dst = s_p + par * (NPB * HG * PROW) + (hq * 16 + l) * PROW + ((g ^ ((l >> 2) & 3)) * 16);
         es = 0.f;
         eps = 0.f;
 #pragma unroll
         for (int u = 0; u < NTT; ++u) {
-          T4 h, l;
+          T4 h, lw;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float e = fast_exp2(v[u * 4 + r] - from);
             es += e;
             h[r] = E::from_f32(e);
-            if constexpr (kLo) l[r] = E::from_f32(e - E::to_f32(h[r]));
+            if constexpr (kLo) lw[r] = E::from_f32(e - E::to_f32(h[r]));
             else eps += E::to_f32(h[r]);
           }
           *(T4*)(dst + (NTT == 1 ? th : u) * 8) = h;
-          if constexpr (kLo) *(T4*)(dst + HG * PROW + (NTT == 1 ? th : u) * 8) = l;
+          if constexpr (kLo) *(T4*)(dst + HG * PROW + (NTT == 1 ? th : u) * 8) = lw;
         }
       };
       auto gemm2 = [&](int buf, int par) {
+        const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
+        const int r1 = g * 4 + (l >> 2);
+        const int g2b = nope_off(r1, 0) + ((((l & 3) >> 1) ^ nope_swz(r1)) * 16) + (l & 1) * 8 + buf * 1024;
         V8 va[NDW];
 #pragma unroll
-        for (int j = 0; j < NDW; ++j) va[j] = a2(buf, wave * NDW + j);
+        for (int j = 0; j < NDW; ++j) va[j] = a2(g2b, wave * NDW + j);
+        const unsigned char* src = s_p + par * (NPB * HG * PROW) + l * PROW + ((g ^ ((l >> 2) & 3)) * 16);
+        auto read = [&](int ht, int part) {
+          return as_v8<V8>(*(const u32x4*)(src + part * HG * PROW + ht * 16 * PROW));
+        };
+        V8 nh = read(0, 0), nl = kLo ? read(0, 1) : nh;
 #pragma unroll
         for (int ht = 0; ht < HGT; ++ht) {
-          const unsigned char* src = s_p + par * (NPB * HG * PROW) + pb + ht * 16 * PROW;
-          const V8 ph = as_v8<V8>(*(const u32x4*)src);
+          const V8 ph = nh, pl = nl;
+          if (ht + 1 < HGT) {
+            nh = read(ht + 1, 0);
+            if constexpr (kLo) nl = read(ht + 1, 1);
+          }
 #pragma unroll
           for (int j = 0; j < NDW; ++j) acc[j][ht] = E::mfma(va[j], ph, acc[j][ht]);
           if constexpr (kLo) {
-            const V8 pl = as_v8<V8>(*(const u32x4*)(src + HG * PROW));
 #pragma unroll
             for (int j = 0; j < NDW; ++j) acc[j][ht] = E::mfma(va[j], pl, acc[j][ht]);
           }
+          if constexpr (HG == 128) __builtin_amdgcn_sched_barrier(0);
         }
       };
 
@@ -295,13 +322,17 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
         const bool more = t + 1 < n_tiles;
         const bool loads = t >= 0 && t + NBUF - 1 < n_tiles;
         if (loads) issue(t + NBUF - 1, buf == 0 ? NBUF - 1 : buf - 1);
-        if (more && scores) gemm1(next);
-        if (t >= 0) gemm2(buf, t & 1);
-        if (more && scores) {
+        auto score_tile = [&]() {
+          gemm1(next);
           scale_mask(t + 1);
           numerators((t + 1) & 1);
           if (__any(tmax > ref + kPaAbove) && lane == 0) s_flag[flag] = 1;
-        }
+        };
+        // of the two waves of a SIMD one starts with the scores and one with
+        // the output, so that one's MFMAs run beside the other's softmax
+        if (more && scores && wave < 4) score_tile();
+        if (t >= 0) gemm2(buf, t & 1);
+        if (more && scores && wave >= 4) score_tile();
         // tile t + 2's flag, last read a barrier ago
         const int flag2 = flag == 2 ? 0 : flag + 1;
         if (tid == 0) s_flag[flag2] = 0;
@@ -347,6 +378,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     }
 
     // ---- the run's output ----
+    const int ln = fresh_lane(), li = ln & 15, lg = ln >> 4;
     {
       const float l = xgroup_sum(sum), lp = xgroup_sum(kLo ? sum : sum_p);
       if (scores && lg == 0) {
