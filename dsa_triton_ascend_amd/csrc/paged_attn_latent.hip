@@ -18,21 +18,24 @@
 //  * O^T: a wave owns D / 8 columns of all HG rows, so each V^T fragment is
 //    read by one wave and serves all rows.
 //  * The scores of tile t + 1 are computed in the same stretch as the output
-//    of tile t, with two P buffers and one barrier per tile, so that a SIMD's
-//    two waves can be in different products.
+//    of tile t, so that a SIMD's two waves can be in different products: one
+//    barrier per tile with two P buffers; at 128 rows of 512 columns, where the
+//    LDS holds one, the numerators wait in registers for a second barrier.
 // The references (paged_attn.h) are looked at once per tile: a wave that
 // sees a score too far above its row's raises a flag, and behind the barrier
 // everyone takes the slow way for that tile (exchange of the maxima, new
 // numerators, rescaled output).  That happens on a run's first tile and
 // seldom after it.
 //
-// Up to 64 rows P is multiplied as a sum of two values of the input type.  At
-// 128 rows the second product would take half of the time again, so P is
-// rounded once there, and the output is divided by the sum of the rounded
+// Up to 32 rows P is multiplied as a sum of two values of the input type.
+// With more the second product costs time (64 rows: 1.6 instead of 1.1 us of
+// MFMAs and LDS reads per tile), so P is rounded once there, and the output is divided by the sum of the rounded
 // values: the weights still add up to one, and what is left is the rounding
 // of single weights, below the rounding of the output.
 #include "paged_attn.h"
 #include "sfa_fwd.h"
+
+#include <type_traits>
 
 namespace dsa {
 
@@ -40,7 +43,7 @@ __device__ __attribute__((aligned(16))) unsigned char g_latent_zero_row[1024];
 
 constexpr int kPlTile = 32;
 constexpr int kPlThreads = 512;
-constexpr int kPlPages = 1024;  // block-table entries held in LDS
+constexpr int kPlPages = 512;  // block-table entries held in LDS
 
 template <int D, typename T, int HG>
 __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnParams p) {
@@ -48,40 +51,49 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   using V8 = typename E::v8;
   typedef T T4 __attribute__((ext_vector_type(4)));
   constexpr int NW = kPlThreads / 64;
-  constexpr int HGT = HG / 16;         // row tiles
-  constexpr int TW = HG == 128 ? 1 : 2;  // waves that share a row tile's tokens
-  constexpr int NTT = 2 / TW;          // 16-token sub-tiles of a wave's scores
-  constexpr int NG1 = HGT * TW;        // waves that compute scores
-  constexpr bool kLo = HG <= 64;       // P as two values
+  constexpr int HW = HG / 16;            // waves that compute scores, 16 rows each
+  constexpr int NTT = 2;                 // 16-token sub-tiles
+  constexpr bool kLo = HG <= 32;         // P as two values
   constexpr int NPB = kLo ? 2 : 1;
   constexpr int DR = 64;
   constexpr int KS = (D + DR) / 32, KSN = D / 32;
-  constexpr int NDW = D / NW / 16;     // output column tiles of a wave
+  constexpr int NDW = D / NW / 16;       // output column tiles of a wave
   constexpr int TILE = kPlTile;
   constexpr int NOPE_BYTES = TILE * D * 2;
   constexpr int BUF_BYTES = NOPE_BYTES + TILE * DR * 2;
-  constexpr int NBUF = HG <= 32 ? 4 : 3;  // what fits beside P
-  constexpr int CPT = D / 8;           // 16-byte chunks of a token
-  constexpr int TPI = 64 / CPT;        // tokens of one DMA
-  constexpr int NIW = TILE / TPI / NW;  // DMAs of a wave per tile, beside the rope rows' (waves 0..3)
+  // at 128 rows of 512 columns the output takes half of the registers and Q
+  // would take most of the rest: QL k-steps of it are kept in LDS, in the
+  // place of a ring buffer
+  constexpr int QL = HG == 128 && D == 512 ? 4 : 0;
+  constexpr int KQR = KS - QL;
+  constexpr int NBUF = QL ? 3 : 4, RBUF = 3;  // ring buffers: a tile's rope rows serve the scores only
+  constexpr int CPT = D / 8;             // 16-byte chunks of a token
+  constexpr int TPI = 64 / CPT;          // tokens of one DMA
+  // waves that fetch: those without scores, where four are
+  constexpr int NL = HW <= 4 ? 4 : 8;
+  constexpr int NIW = TILE / TPI / NL;   // DMAs of a fetching wave per tile; four waves one more for rope rows
   constexpr int ROPE0 = NBUF * NOPE_BYTES;
   constexpr int PROW = TILE * 2;
-  static_assert(NG1 <= NW && NIW * TPI * NW == TILE && NDW * 16 * NW == D, "tile split");
+  static_assert(HW <= NW && NIW * TPI * NL == TILE && NDW * 16 * NW == D, "tile split");
   // a token's row of buffer b; buffers alternate per DMA
   auto nope_off = [](int tk, int b) { return ((tk / TPI) * NBUF + b) * 1024 + (tk % TPI) * (D * 2); };
-  auto rope_off = [](int tk, int b) { return ROPE0 + ((tk >> 3) * NBUF + b) * 1024 + (tk & 7) * (DR * 2); };
+  auto rope_off = [](int tk, int b) { return ROPE0 + ((tk >> 3) * RBUF + b) * 1024 + (tk & 7) * (DR * 2); };
 
-  __shared__ __attribute__((aligned(16))) unsigned char smem[NBUF * BUF_BYTES];
+  __shared__ __attribute__((aligned(16))) unsigned char smem[NBUF * NOPE_BYTES + RBUF * TILE * DR * 2];
   __shared__ __attribute__((aligned(16))) unsigned char s_p[2 * NPB * HG * PROW];
+  __shared__ __attribute__((aligned(16))) unsigned char s_q[QL ? HG * QL * 64 : 16];
   __shared__ int s_tab[kPlPages];
-  __shared__ float s_mx[TW * HG], s_l[TW * HG], s_f[HG];
-  __shared__ int s_flag[3];  // of a tile: its number modulo 3
+  __shared__ float s_f[2 * HG];  // by a tile's parity: factors of the rows whose reference moved
+  __shared__ int s_flag[3];  // by a tile's number modulo 3: bits of the waves whose rows moved
+  float* const s_n = (float*)s_p;  // of a finished run, in place of P: the rows' divisors
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const bool scores = wave < NG1;
-  const int hq = wave % HGT, th = scores ? wave / HGT : 0;
+  const bool scores = wave < HW;
+  const bool fetches = NL == NW || wave >= NW - NL;
+  const int lw = wave - (NW - NL);  // among the fetching waves
+  const bool rope_wave = lw >= 0 && lw < 4;
 
   // the row groups of a worker read the same tokens: they share an XCD
   const int jj = blockIdx.x >> 3;
@@ -96,20 +108,23 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   int64_t before;
   int b = plan.find(p, TILE, lane, at, &before);
 
+  // scores in log2 units are s * scale - ref, one operation each; for that
+  // the scale is positive (Q takes its sign) and not zero (masked scores are
+  // -inf before it)
+  const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
+  const unsigned flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
   const unsigned smem_base = (unsigned)(uintptr_t)smem;
-  const bool rope_wave = wave < 4;
   const unsigned char* const kbase = (const unsigned char*)p.k;
   const unsigned char* const rbase = (const unsigned char*)p.kr;
-  // this lane's addresses in the two products, made anew from the lane's
-  // number in every step: kept, they would push Q or the output out of the
-  // registers
+  // a lane's addresses in the two products are made anew from its number in
+  // every step: kept, they would push Q or the output out of the registers
   auto fresh_lane = []() {
     int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
     asm volatile("" : "+v"(ln));
     return ln;
   };
   constexpr int G1_TT = ((16 / TPI) * NBUF) * 1024;
-  constexpr int G1R_TT = 2 * NBUF * 1024;
+  constexpr int G1R_TT = 2 * RBUF * 1024;
   auto a1 = [&](int g1b, int g1rb, int ks, int tt) -> V8 {
     if (ks < KSN) return as_v8<V8>(*(const u32x4*)(smem + ((g1b ^ ((ks & 3) << 6)) + tt * G1_TT + (ks >> 2) * 256)));
     return as_v8<V8>(*(const u32x4*)(smem + ((g1rb ^ ((ks - KSN) << 6)) + tt * G1R_TT)));
@@ -122,6 +137,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     const i16x8 w = {w1[0], w1[1], w1[2], w1[3], w2[0], w2[1], w2[2], w2[3]};
     return __builtin_bit_cast(V8, w);
   };
+  using Off = std::integral_constant<bool, false>;
 
   bool first_segment = true;
   while (at < end) {
@@ -138,29 +154,30 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     const int tok0 = seq.lo + t0 * TILE, tok1 = min(seq.hi, seq.lo + t1 * TILE);
     const int32_t* tab = p.table + (int64_t)b * p.max_blocks;
 
-    // row of this lane's column of the scores: head rr % n1 of new token rr / n1
-    const int rr = rg * HG + hq * 16 + li;
-    const bool live = scores && rr < p.rows;
-    int lo = 0, hi = 0;
-    V8 qf[KS];
+    // rows of this lane's score columns: head rr % n1 of new token rr / n1
+    // (rows that do not exist read row 0; what they compute is not stored)
+    const int row = rg * HG + wave * 16 + li;
+    const bool live = scores && row < p.rows;
+    int all_lo = 0, all_hi = 0x7fffffff;
+    V8 qf[KQR];
     {
-      const int s = live ? rr / p.n1 : 0;
-      const int64_t qrow = (int64_t)b * p.rows + (live ? rr : 0);
-      // (rows that do not exist read row 0; what they compute is not stored)
+      const int64_t qrow = (int64_t)b * p.rows + (live ? row : 0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const T* src = ks < KSN ? (const T*)p.q + qrow * D + ks * 32 + lg * 8
                                 : (const T*)p.qr + qrow * DR + (ks - KSN) * 32 + lg * 8;
-        qf[ks] = as_v8<V8>(*(const u32x4*)src);
+        const u32x4 x = *(const u32x4*)src ^ flip;
+        if (ks < KQR) qf[ks < KQR ? ks : 0] = as_v8<V8>(x);
+        else if constexpr (QL > 0)
+          *(u32x4*)(s_q + (((wave * 16 + li) * (QL * 64) + ((lg ^ nope_swz(li)) * 16)) ^ ((ks - KQR) << 6))) = x;
       }
-      if (live) paged_bounds(p, seq.act_q, seq.act_k, s, &lo, &hi);
+      if (live) paged_bounds(p, seq.act_q, seq.act_k, row / p.n1, &all_lo, &all_hi);
     }
     // the loads end here, not inside the tile loop, where a wait for them
     // would be one for the tiles in flight too
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
+    for (int ks = 0; ks < KQR; ++ks) asm volatile("" : "+v"(qf[ks]));
     // tokens that all of the wave's rows see need no mask
-    int all_lo = live ? lo : 0, all_hi = live ? hi : 0x7fffffff;
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) {
       all_lo = max(all_lo, __shfl_xor(all_lo, o));
@@ -169,11 +186,11 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     all_lo = __builtin_amdgcn_readfirstlane(all_lo);
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
 
-    f32x4 acc[NDW][HGT];
+    f32x4 acc[NDW][HW];
 #pragma unroll
     for (int j = 0; j < NDW; ++j)
 #pragma unroll
-      for (int ht = 0; ht < HGT; ++ht) acc[j][ht] = {0.f, 0.f, 0.f, 0.f};
+      for (int ht = 0; ht < HW; ++ht) acc[j][ht] = {0.f, 0.f, 0.f, 0.f};
     float ref = -INFINITY, top = -INFINITY, sum = 0.f, sum_p = 0.f;
 
     for (int ta = tok0; ta < tok1;) {
@@ -188,244 +205,293 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       lds_barrier();
       const int n_tiles = (tb - ta + TILE - 1) / TILE;
 
-      auto issue = [&](int t, int buf) {
-        const int lane = fresh_lane();
-        // lane l < 32 finds token l's row, -1 past the end or without a page
-        const int tok = ta + t * TILE + (lane & 31);
-        int row = -1;
-        if (tok < tb) {
-          unsigned off;
-          const unsigned pg = paged_split(p, (unsigned)tok, &off);
-          const int blk = s_tab[(int)pg - pg0];
-          const int64_t r = (int64_t)blk * p.page + (int)off;
-          row = blk < 0 || r >= p.kv_rows ? -1 : (int)r;
-        }
-#pragma unroll
-        for (int j = 0; j < NIW; ++j) {
-          const int tk = (j * NW + wave) * TPI + lane / CPT;
-          const int ch = (lane % CPT) ^ nope_swz(tk);
-          const int r = TPI == 1 ? __builtin_amdgcn_readlane(row, j * NW + wave) : __shfl(row, tk);
-          dma_glb16(smem_base + nope_off((j * NW + wave) * TPI, buf),
-                    r >= 0 ? kbase + (int64_t)r * (D * 2) + ch * 16 : g_latent_zero_row + ch * 16);
-        }
-        if (rope_wave) {
-          const int tk = wave * 8 + (lane >> 3);
-          const int ch = (lane & 7) ^ rope_swz(tk);
-          const int r = __shfl(row, tk);
-          dma_glb16(smem_base + rope_off(wave * 8, buf),
+      // cache row of token lane % 32 of tile t, -1 past the end or without a
+      // page (both are read as zeros)
+      auto tile_rows = [&](int t) -> int {
+        const int tok = ta + t * TILE + (fresh_lane() & 31);
+        if (tok >= tb) return -1;
+        unsigned off;
+        const unsigned pg = paged_split(p, (unsigned)tok, &off);
+        const int blk = s_tab[(int)pg - pg0];
+        const int64_t r = (int64_t)blk * p.page + (int)off;
+        return blk < 0 || r >= p.kv_rows ? -1 : (int)r;
+      };
+      // the wave's DMA j of a tile into buffers buf and rbuf
+      auto dma = [&](int j, int rows, int buf, int rbuf) {
+        const int ln = fresh_lane();
+        if (j < NIW) {
+          const unsigned dst = smem_base + nope_off((j * NL + lw) * TPI, buf);
+          if constexpr (TPI == 1) {
+            // one row: its address goes into the descriptor, of no bytes
+            // where there is no row
+            const int r = __builtin_amdgcn_readlane(rows, j * NL + lw);
+            const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)(kbase + (int64_t)(r < 0 ? 0 : r) * (D * 2)), (short)0, r < 0 ? 0 : D * 2, 0x00020000);
+            dma_buf16(dst, (ln ^ nope_swz(j * NL + lw)) * 16, rsrc);
+          } else {
+            const int tk = (j * NL + lw) * TPI + ((unsigned)ln / CPT);
+            const int ch = ((unsigned)ln % CPT) ^ nope_swz(tk);
+            const int r = __shfl(rows, tk);
+            dma_glb16(dst, r >= 0 ? kbase + (int64_t)r * (D * 2) + ch * 16 : g_latent_zero_row + ch * 16);
+          }
+        } else if (rope_wave) {
+          const int tk = lw * 8 + (ln >> 3);
+          const int ch = (ln & 7) ^ rope_swz(tk);
+          const int r = __shfl(rows, tk);
+          dma_glb16(smem_base + rope_off(lw * 8, rbuf),
                     r >= 0 ? rbase + (int64_t)r * (DR * 2) + ch * 16 : g_latent_zero_row + ch * 16);
         }
       };
+
+      // all but the last K tiles that this wave asked for have landed
+      auto landed = [&](auto k) {
+        constexpr int K = decltype(k)::value;
+        if (rope_wave) wait_vmcnt<K * (NIW + 1)>();
+        else wait_vmcnt<K * NIW>();
+      };
+
+      // ---- scores of a tile, with the DMAs of another between the MFMAs ----
       f32x4 s[NTT];
-      auto gemm1 = [&](int buf) {
-        f32x4 a[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        // two accumulators, so that neighbouring MFMAs are independent
-        // (sub-tiles, or even and odd k-steps); PF fragments read ahead, and
-        // no more (the accumulators leave few registers)
-        constexpr int NS = KS * NTT, PF = 4;
-        const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
-        const int g1b = nope_off(l, 0) + ((g ^ nope_swz(l)) * 16) + buf * 1024;
-        const int g1rb = rope_off(l, 0) + ((g ^ rope_swz(l)) * 16) + buf * 1024;
-        auto read = [&](int st) { return a1(g1b, g1rb, st / NTT, NTT == 1 ? th : st % NTT); };
-        V8 fa[PF];
-#pragma unroll
-        for (int i = 0; i < PF; ++i) fa[i] = read(i);
-#pragma unroll
-        for (int st = 0; st < NS; ++st) {
-          const V8 f = fa[st % PF];
-          if (st + PF < NS) fa[st % PF] = read(st + PF);
-          a[st & 1] = E::mfma(f, qf[st / NTT], a[st & 1]);
-          if constexpr (HG == 128) __builtin_amdgcn_sched_barrier(0);
-        }
-        if constexpr (NTT == 1) s[0] = a[0] + a[1];
-        else s[0] = a[0], s[1] = a[1];
-      };
-      // numerators of the wave's scores into P buffer `par`; their sums
-      float v[NTT * 4], tmax, es, eps;
-      auto scale_mask = [&](int t) {
-        const int tk = ta + t * TILE;
-        tmax = -INFINITY;
-        if (tk >= all_lo && tk + TILE <= min(all_hi, tb)) {
-#pragma unroll
-          for (int i = 0; i < NTT * 4; ++i) v[i] = s[i >> 2][i & 3] * p.scale_log2;
-        } else {
-#pragma unroll
-          for (int i = 0; i < NTT * 4; ++i) {
-            const int tok = tk + (NTT == 1 ? th : i >> 2) * 16 + lg * 4 + (i & 3);
-            v[i] = tok >= lo && tok < min(hi, tb) ? s[i >> 2][i & 3] * p.scale_log2 : -INFINITY;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NTT * 4; ++i) tmax = fmaxf(tmax, v[i]);
-        tmax = xgroup_max(tmax);
-      };
-      auto numerators = [&](int par) {
-        const float from = ref == -INFINITY ? 0.f : ref;
-        const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
-        unsigned char* dst = s_p + par * (NPB * HG * PROW) + (hq * 16 + l) * PROW + ((g ^ ((l >> 2) & 3)) * 16);
-        es = 0.f;
-        eps = 0.f;
-#pragma unroll
-        for (int u = 0; u < NTT; ++u) {
-          T4 h, lw;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float e = fast_exp2(v[u * 4 + r] - from);
-            es += e;
-            h[r] = E::from_f32(e);
-            if constexpr (kLo) lw[r] = E::from_f32(e - E::to_f32(h[r]));
-            else eps += E::to_f32(h[r]);
-          }
-          *(T4*)(dst + (NTT == 1 ? th : u) * 8) = h;
-          if constexpr (kLo) *(T4*)(dst + HG * PROW + (NTT == 1 ? th : u) * 8) = lw;
-        }
-      };
-      auto gemm2 = [&](int buf, int par) {
+      V8 va[NDW];
+      auto read_v = [&](int buf) {
         const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
         const int r1 = g * 4 + (l >> 2);
         const int g2b = nope_off(r1, 0) + ((((l & 3) >> 1) ^ nope_swz(r1)) * 16) + (l & 1) * 8 + buf * 1024;
-        V8 va[NDW];
 #pragma unroll
         for (int j = 0; j < NDW; ++j) va[j] = a2(g2b, wave * NDW + j);
-        const unsigned char* src = s_p + par * (NPB * HG * PROW) + l * PROW + ((g ^ ((l >> 2) & 3)) * 16);
+      };
+      auto gemm1 = [&](int kbuf, int krbuf, auto with_dma, int rows, int dbuf, int drbuf) {
+        constexpr int PF = QL ? 2 : 4;  // k-steps read ahead
+        const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
+        const int g1b = nope_off(l, 0) + ((g ^ nope_swz(l)) * 16) + kbuf * 1024;
+        const int g1rb = rope_off(l, 0) + ((g ^ rope_swz(l)) * 16) + krbuf * 1024;
+        const int qb = ((wave * 16 + l) * (QL * 64)) + ((g ^ nope_swz(l)) * 16);
+        V8 fa[PF][NTT], ql[2];  // Q of a k-step in LDS is read two ahead
+#pragma unroll
+        for (int i = 0; i < PF; ++i)
+#pragma unroll
+          for (int u = 0; u < NTT; ++u) fa[i][u] = a1(g1b, g1rb, i, u);
+#pragma unroll
+        for (int u = 0; u < NTT; ++u) s[u] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          V8 f[NTT];
+#pragma unroll
+          for (int u = 0; u < NTT; ++u) {
+            f[u] = fa[ks % PF][u];
+            if (ks + PF < KS) fa[ks % PF][u] = a1(g1b, g1rb, ks + PF, u);
+          }
+          const V8 q = ks < KQR ? qf[ks < KQR ? ks : 0] : ql[ks & 1];
+          if (QL > 0 && ks + 2 >= KQR && ks + 2 < KS)
+            ql[ks & 1] = as_v8<V8>(*(const u32x4*)(s_q + (qb ^ ((ks + 2 - KQR) << 6))));
+#pragma unroll
+          for (int u = 0; u < NTT; ++u) s[u] = E::mfma(f[u], q, s[u]);
+          if constexpr (decltype(with_dma)::value) {
+            constexpr int kStep = KS / (NIW + 1);
+            if (ks % kStep == 0 && ks / kStep <= NIW) dma(ks / kStep, rows, dbuf, drbuf);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+
+      // ---- softmax of the scores in eight stages, which go between the
+      // groups of output MFMAs ----
+      float es, eps;
+      T4 ph[NTT], pl[NTT];
+      auto stage = [&](int k, int t, int flag) {
+        if (k == 0) {
+          const int tk = ta + t * TILE;
+          if (tk < all_lo || tk + TILE > min(all_hi, tb)) {
+            const int ln = fresh_lane();
+            int lo, hi;
+            const int r = min(rg * HG + wave * 16 + (ln & 15), p.rows - 1);
+            paged_bounds(p, seq.act_q, seq.act_k, r / p.n1, &lo, &hi);
+            hi = min(hi, tb);
+#pragma unroll
+            for (int i = 0; i < NTT * 4; ++i) {
+              const int tok = tk + (i >> 2) * 16 + (ln >> 4) * 4 + (i & 3);
+              s[i >> 2][i & 3] = tok >= lo && tok < hi ? s[i >> 2][i & 3] : -INFINITY;
+            }
+          }
+        } else if (k == 1) {
+          float m = s[0][0];
+#pragma unroll
+          for (int i = 1; i < NTT * 4; ++i) m = fmaxf(m, s[i >> 2][i & 3]);
+          const float tmax = xgroup_max(m) * scale;
+          top = fmaxf(top, tmax);
+          es = eps = 0.f;
+          const bool moves = tmax > ref + kPaAbove;
+          if (__any(moves)) {
+            // new references; whoever multiplies this tile's numerators
+            // first scales these rows of its output
+            const int ln = fresh_lane();
+            const float nref = moves ? tmax - kPaBelow : ref;
+            const float f = ref == -INFINITY ? 0.f : fast_exp2(ref - nref);
+            ref = nref;
+            sum *= f;
+            sum_p *= f;
+            if (ln < 16) s_f[(t & 1) * HG + wave * 16 + ln] = f;
+            if (ln == 0) atomicOr(&s_flag[flag], 1 << wave);
+          }
+        } else if (k < 6) {
+          // a quarter of the numerators
+          const float from = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+          for (int i = (k - 2) * NTT; i < (k - 1) * NTT; ++i) {
+            const float e = fast_exp2(__builtin_fmaf(s[i >> 2][i & 3], scale, -from));
+            es += e;
+            ph[i >> 2][i & 3] = E::from_f32(e);
+            if constexpr (kLo) pl[i >> 2][i & 3] = E::from_f32(e - E::to_f32(ph[i >> 2][i & 3]));
+            else eps += E::to_f32(ph[i >> 2][i & 3]);
+          }
+        } else if (k == 6) {
+          sum += es;
+          sum_p += eps;
+        } else {
+          const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
+          unsigned char* dst = s_p + (t & 1) * (NPB * HG * PROW) + (wave * 16 + l) * PROW + ((g ^ ((l >> 2) & 3)) * 16);
+#pragma unroll
+          for (int u = 0; u < NTT; ++u) {
+            *(T4*)(dst + u * 8) = ph[u];
+            if constexpr (kLo) *(T4*)(dst + HG * PROW + u * 8) = pl[u];
+          }
+        }
+      };
+
+      // ---- output of tile t (V^T fragments in va), with the softmax of tile
+      // t + 1 between the MFMAs ----
+      auto gemm2 = [&](int t, int flag) {
+        const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
+        const unsigned char* src = s_p + (t & 1) * (NPB * HG * PROW) + l * PROW + ((g ^ ((l >> 2) & 3)) * 16);
         auto read = [&](int ht, int part) {
           return as_v8<V8>(*(const u32x4*)(src + part * HG * PROW + ht * 16 * PROW));
         };
         V8 nh = read(0, 0), nl = kLo ? read(0, 1) : nh;
 #pragma unroll
-        for (int ht = 0; ht < HGT; ++ht) {
-          const V8 ph = nh, pl = nl;
-          if (ht + 1 < HGT) {
+        for (int ht = 0; ht < HW; ++ht) {
+          const V8 bh = nh, bl = nl;
+          if (ht + 1 < HW) {
             nh = read(ht + 1, 0);
             if constexpr (kLo) nl = read(ht + 1, 1);
           }
 #pragma unroll
-          for (int j = 0; j < NDW; ++j) acc[j][ht] = E::mfma(va[j], ph, acc[j][ht]);
+          for (int j = 0; j < NDW; ++j) acc[j][ht] = E::mfma(va[j], bh, acc[j][ht]);
           if constexpr (kLo) {
 #pragma unroll
-            for (int j = 0; j < NDW; ++j) acc[j][ht] = E::mfma(va[j], pl, acc[j][ht]);
+            for (int j = 0; j < NDW; ++j) acc[j][ht] = E::mfma(va[j], bl, acc[j][ht]);
           }
-          if constexpr (HG == 128) __builtin_amdgcn_sched_barrier(0);
+          if (scores) {
+#pragma unroll
+            for (int k = ht * 8 / HW; k < (ht + 1) * 8 / HW; ++k) stage(k, t + 1, flag);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       };
 
+      // the first tiles (those past the end, here and below, read zeros, so
+      // that the number of DMAs in flight is known)
+      if (fetches) {
 #pragma unroll
-      for (int t = 0; t < NBUF - 1; ++t)
-        if (t < n_tiles) issue(t, t);
-      wait_vmcnt<0>();
-      lds_barrier();
-      // step t: scores of tile t + 1, output of tile t
-      int buf = NBUF - 1;  // buffer of tile t
-      int flag = 0;        // of tile t + 1
-      for (int t = -1; t < n_tiles; ++t) {
-        const int next = buf + 1 == NBUF ? 0 : buf + 1;
-        const bool more = t + 1 < n_tiles;
-        const bool loads = t >= 0 && t + NBUF - 1 < n_tiles;
-        if (loads) issue(t + NBUF - 1, buf == 0 ? NBUF - 1 : buf - 1);
-        auto score_tile = [&]() {
-          gemm1(next);
-          scale_mask(t + 1);
-          numerators((t + 1) & 1);
-          if (__any(tmax > ref + kPaAbove) && lane == 0) s_flag[flag] = 1;
-        };
-        // of the two waves of a SIMD one starts with the scores and one with
-        // the output, so that one's MFMAs run beside the other's softmax
-        if (more && scores && wave < 4) score_tile();
-        if (t >= 0) gemm2(buf, t & 1);
-        if (more && scores && wave >= 4) score_tile();
-        // tile t + 2's flag, last read a barrier ago
-        const int flag2 = flag == 2 ? 0 : flag + 1;
-        if (tid == 0) s_flag[flag2] = 0;
-        // tile t + 2 has landed: with four buffers the one after it may be
-        // in flight
-        if (NBUF == 3 || !loads) wait_vmcnt<0>();
-        else if (rope_wave) wait_vmcnt<NIW + 1>();
-        else wait_vmcnt<NIW>();
-        lds_barrier();
-        if (!more) break;
-        const bool moved = __builtin_amdgcn_readfirstlane(s_flag[flag]) != 0;
-        flag = flag2;
-        if (moved) {
-          if (scores && lg == 0) s_mx[th * HG + hq * 16 + li] = tmax;
-          lds_barrier();
-          if (scores) {
-            float mx = s_mx[hq * 16 + li];
-            if constexpr (TW == 2) mx = fmaxf(mx, s_mx[HG + hq * 16 + li]);
-            const float nref = mx > ref + kPaAbove ? mx - kPaBelow : ref;
-            const float f = ref == -INFINITY ? 0.f : fast_exp2(ref - nref);
-            if (th == 0 && lg == 0) s_f[hq * 16 + li] = f;
-            ref = nref;
-            sum *= f;
-            sum_p *= f;
-            numerators((t + 1) & 1);
-          }
-          lds_barrier();
+        for (int t = 0; t < NBUF - 1; ++t) {
+          const int rows = tile_rows(t);
 #pragma unroll
-          for (int ht = 0; ht < HGT; ++ht) {
-            const float f = s_f[ht * 16 + li];
-#pragma unroll
-            for (int j = 0; j < NDW; ++j) acc[j][ht] *= f;
-          }
+          for (int j = 0; j <= NIW; ++j) dma(j, rows, t, t);
         }
-        if (scores) {
-          sum += es;
-          sum_p += eps;
-          top = fmaxf(top, tmax);
-        }
-        buf = next;
       }
+      landed(std::integral_constant<int, NBUF - 2>{});
+      lds_barrier();
+      if (scores) {
+        gemm1(0, 0, Off{}, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) stage(k, 0, 0);
+      }
+      landed(std::integral_constant<int, NBUF - 3>{});
+      lds_barrier();
+      // step t: scores of tile t + 1 (of no visible token after the last),
+      // output of tile t, DMAs of tile t + NBUF - 1
+      int buf = 0, rbuf = 0;  // buffers and flags of tile t
+      for (int t = 0; t < n_tiles; ++t) {
+        const int next = buf + 1 == NBUF ? 0 : buf + 1;
+        const int rnext = rbuf + 1 == RBUF ? 0 : rbuf + 1;
+        const int rlast = rnext + 1 == RBUF ? 0 : rnext + 1;  // of tile t + 2, and of tile t - 1
+        const int dbuf = buf == 0 ? NBUF - 1 : buf - 1, drbuf = NBUF == 3 ? rlast : rbuf;
+        const int moved_v = s_flag[rbuf];
+        // flags of tile t + 2, last read a step ago
+        if (tid == 0) s_flag[rlast] = 0;
+        const int rows = fetches ? tile_rows(t + NBUF - 1) : -1;
+        if (NL < NW && fetches) {
+#pragma unroll
+          for (int j = 0; j <= NIW; ++j) dma(j, rows, dbuf, drbuf);
+        }
+        if (scores) gemm1(next, rnext, std::integral_constant<bool, NL == NW>{}, rows, dbuf, drbuf);
+        read_v(buf);
+        const int moved = __builtin_amdgcn_readfirstlane(moved_v);
+        if (moved) {
+          const int l = fresh_lane() & 15;
+#pragma unroll
+          for (int w = 0; w < HW; ++w)
+            if (moved >> w & 1) {
+              const float f = s_f[(t & 1) * HG + w * 16 + l];
+#pragma unroll
+              for (int j = 0; j < NDW; ++j) acc[j][w] *= f;
+            }
+        }
+        gemm2(t, rnext);
+        landed(std::integral_constant<int, NBUF - 3>{});  // tile t + 2 has
+        lds_barrier();
+        buf = next;
+        rbuf = rnext;
+      }
+      wait_vmcnt<0>();  // of the DMAs past the end too: the ring is theirs until then
       ta = tb;
     }
 
     // ---- the run's output ----
     const int ln = fresh_lane(), li = ln & 15, lg = ln >> 4;
-    {
-      const float l = xgroup_sum(sum), lp = xgroup_sum(kLo ? sum : sum_p);
-      if (scores && lg == 0) {
-        s_l[th * HG + hq * 16 + li] = l;
-        s_mx[th * HG + hq * 16 + li] = top;
-        if (th == 0) s_f[hq * 16 + li] = kLo ? 0.f : lp;
-      }
-    }
-    lds_barrier();
     const bool whole = t0 == 0 && t1 == nt;
     const int64_t slot0 =
         (((int64_t)worker * 2 + (first_segment ? 0 : 1)) * p.groups + rg) * p.group_rows;
-    // the statistics, by the waves that hold a row's reference
-    if (scores && th == 0 && lg == 0 && live) {
-      const int h = hq * 16 + li;
-      float l = s_l[h], m = s_mx[h];
-      if constexpr (TW == 2) l += s_l[HG + h], m = fmaxf(m, s_mx[HG + h]);
-      if (whole) {
-        if (p.smax) {
-          const int64_t o = (int64_t)b * p.rows + rr;
-          const bool any = p.return_lse && l > 0.f;
-          // [B, 1, S1, N1], the order of the rows
-          p.smax[o] = any ? m * kLn2 : 0.f;
-          p.ssum[o] = any ? l * fast_exp2(ref - m) : 0.f;
+    {
+      const float l = xgroup_sum(sum), n = xgroup_sum(kLo ? sum : sum_p);
+      const int r = wave * 16 + li, rr = rg * HG + r;
+      if (scores && lg == 0) {
+        s_n[r] = n;
+        if (rr < p.rows) {
+          if (!whole) {
+            p.part_ml[slot0 + r] = {ref, l, top, n};
+          } else if (p.smax) {
+            const int64_t o = (int64_t)b * p.rows + rr;  // [B, 1, S1, N1], the order of the rows
+            const bool any = p.return_lse && l > 0.f;
+            p.smax[o] = any ? top * kLn2 : 0.f;
+            p.ssum[o] = any ? l * fast_exp2(ref - top) : 0.f;
+          }
         }
-      } else {
-        p.part_ml[slot0 + h] = {ref, l, m, kLo ? l : s_f[h]};
       }
     }
+    lds_barrier();
+    const int col = wave * NDW * 16 + lg * 4;
+    if (whole) {
 #pragma unroll
-    for (int ht = 0; ht < HGT; ++ht) {
-      const int h = ht * 16 + li;
-      const int64_t r = (int64_t)rg * HG + h;
-      float l = s_l[h];
-      if constexpr (TW == 2) l += s_l[HG + h];
-      if constexpr (!kLo) l = s_f[h];
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      if (r >= p.rows) continue;
+      for (int ht = 0; ht < HW; ++ht) {
+        const int r = rg * HG + ht * 16 + li;
+        const float n = s_n[ht * 16 + li];
+        const float inv = n > 0.f ? 1.f / n : 0.f;
+        if (r < p.rows) {
+          T* dst = (T*)p.out + ((int64_t)b * p.rows + r) * D + col;
 #pragma unroll
-      for (int j = 0; j < NDW; ++j) {
-        const int col = (wave * NDW + j) * 16 + lg * 4;
-        if (whole) {
-          const f32x4 x = acc[j][ht] * inv;
-          const T4 o = {E::from_f32(x[0]), E::from_f32(x[1]), E::from_f32(x[2]), E::from_f32(x[3])};
-          *(T4*)((T*)p.out + ((int64_t)b * p.rows + r) * D + col) = o;
-        } else {
-          *(f32x4*)(p.part_o + (slot0 + h) * D + col) = acc[j][ht];
+          for (int j = 0; j < NDW; ++j) {
+            const f32x4 x = acc[j][ht] * inv;
+            *(T4*)(dst + j * 16) = (T4){E::from_f32(x[0]), E::from_f32(x[1]), E::from_f32(x[2]), E::from_f32(x[3])};
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int ht = 0; ht < HW; ++ht) {
+        if (rg * HG + ht * 16 + li < p.rows) {
+          float* dst = p.part_o + (slot0 + ht * 16 + li) * D + col;
+#pragma unroll
+          for (int j = 0; j < NDW; ++j) *(f32x4*)(dst + j * 16) = acc[j][ht];
         }
       }
     }
@@ -435,7 +501,6 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       before += nt;
       ++b;
     }
-    lds_barrier();  // s_l, s_mx and s_f are read
   }
 }
 

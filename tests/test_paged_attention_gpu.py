@@ -7,7 +7,7 @@ most ds = (columns + 4) 2^-24 sum |q k| scale (products and sums of 32 bits,
 scale, exponent), a weight by 2 ds (its own and the sum's), by the rounding u
 of the numerator to the type (twice: its own and the divisor's), and by 2^-20
 for exponential, sums and joins; the output rounds by eps / 2.  u is eps / 2
-where the numerators are rounded once (latent form, more than 64 rows) and
+where the numerators are rounded once (latent form, more than 32 rows) and
 (eps / 2)^2 where they are kept as two values.  Largest score: off by ds and
 2^-22 of itself; sum: 2 ds + 2^-20 relative.
 """
@@ -86,7 +86,7 @@ def _compare(args, data, lens, act_q=None):
     G = N1 // N2
     dtype = q.dtype
     half = torch.finfo(dtype).eps / 2
-    u = half if latent and S1 * N1 > 64 else half * half
+    u = half if latent and S1 * N1 > 32 else half * half
     cols = D + 64 if latent else D
     for b, n in enumerate(lens):
         q_b = S1 if act_q is None else act_q[b]
