@@ -247,25 +247,38 @@ def stream_handle(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-class on_device:
-    """The device of a call's tensors, made current while the library plans
-    and launches (sizes such as the CU count and the launch itself go to the
-    current device).  Nothing is done where it is current already."""
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
-    __slots__ = ("idx", "prev")
 
-    def __init__(self, device):
-        self.idx = device.index
+def call_on(index, fn, *args):
+    """``fn(*args)`` with GPU ``index`` current: the library plans for and
+    launches on the current device, which need not be the tensors'."""
+    if _current_device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
 
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.idx)
 
-    def __exit__(self, *exc):
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.prev)
-        return False
+def raw_stream(index):
+    """The current stream of GPU ``index`` as a raw handle."""
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def same_device(first, *others):
+    """Index of the GPU that all the tensors (None: absent) are on; ValueError
+    if one is elsewhere.  A call of the paged decoding operators takes a few
+    microseconds, so this compares plain integers."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError("this operator requires tensors on a ROCm GPU device (it has no CPU path)")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            if t.get_device() < 0:
+                raise ValueError("this operator requires tensors on a ROCm GPU device (it has no CPU path)")
+            raise ValueError("all tensors must be on the same device")
+    return index
 
 
 def dtype_code(dt):

@@ -133,26 +133,24 @@ class RotaryEmbeddingFunction(torch.autograd.Function):
     scale, so nothing of the forward but the positions is kept."""
 
     @staticmethod
-    def forward(ctx, query, key, positions, inv_freq, interleaved, q_start, k_start, scale, layout, inverse):
+    def forward(ctx, query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.args = (interleaved, q_start, k_start, scale, layout)
-        ctx.inverse = inverse
+        ctx.args = (interleaved, q_start, k_start, scale, not inverse)
         ctx.set_materialize_grads(False)
-        return tuple(_rotate(query, key, positions, inv_freq, *ctx.args, inverse, False))
+        return _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_query, d_key):
         positions, inv_freq = ctx.saved_tensors
-        interleaved, q_start, k_start, scale, layout = ctx.args
+        interleaved, q_start, k_start, scale, inverse = ctx.args
         d_q = d_query if ctx.needs_input_grad[0] else None
         d_k = d_key if ctx.needs_input_grad[1] else None
         if d_q is not None:
-            d_q, d_k = _rotate(d_q, d_k, positions, inv_freq, *ctx.args, not ctx.inverse, False)
+            d_q, d_k = _rotate(d_q, d_k, positions, inv_freq, *ctx.args, False)
         elif d_k is not None:
-            d_k, _ = _rotate(d_k, None, positions, inv_freq, interleaved, k_start, 0, scale, layout, not ctx.inverse,
-                             False)
-        return (d_q, d_k) + (None,) * 8
+            d_k, _ = _rotate(d_k, None, positions, inv_freq, interleaved, k_start, 0, scale, inverse, False)
+        return (d_q, d_k) + (None,) * 7
 
 
 __all__ = ["RotaryEmbeddingFunction", "SparseFlashAttentionFunction", "sparse_flash_attention_train",

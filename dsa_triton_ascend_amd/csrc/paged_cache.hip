@@ -62,7 +62,7 @@ struct PcWriteParams {
 
 __global__ __launch_bounds__(kPcThreads) void pc_write_kernel(PcWriteParams p) {
   const int64_t i = (int64_t)blockIdx.x * kPcThreads + threadIdx.x;
-  const int64_t t = i / p.units;
+  const int64_t t = i >> 32 ? i / p.units : (int64_t)((unsigned)i / (unsigned)p.units);
   if (t >= p.tokens) return;
   const int u = (int)(i - t * p.units);
   int b, s;
@@ -402,6 +402,8 @@ int pc_fork_run(int64_t n, void* const* caches, const int64_t* row_bytes, const 
 // of n or above moves to the k-th free id below n, so no page is both read
 // and written and the moves need no order.
 // ---------------------------------------------------------------------------
+constexpr int64_t kPcCountsHere = 16384;
+
 struct PcCompactParams {
   PcCopySet set;
   const int32_t *table, *refs;
@@ -410,6 +412,7 @@ struct PcCompactParams {
   int64_t pages, entries;
   int chunks;                          // chunks of kPcPlanThreads pages
   int table_blocks, copy_blocks;
+  int counts_here;                     // the ranks are found without a launch that counts first
 };
 
 __global__ __launch_bounds__(kPcPlanThreads) void pc_count_kernel(PcCompactParams p) {
@@ -434,18 +437,33 @@ __device__ __forceinline__ void pc_live(const PcCompactParams& p, int upto, int*
 __global__ __launch_bounds__(kPcPlanThreads) void pc_rank_kernel(PcCompactParams p) {
   constexpr int W = kPcPlanThreads / 64;
   __shared__ int s_part[W];
-  int before, n, total;
-  pc_live<W>(p, blockIdx.x, s_part, &before, &n);
-  // live pages below id n: the chunks before n's, and that chunk's own part
-  const int nc = n / kPcPlanThreads;
-  int low, dummy;
-  pc_live<W>(p, nc, s_part, &low, &dummy);
-  const int64_t in = (int64_t)nc * kPcPlanThreads + threadIdx.x;
-  pc_block_scan<W>(in < n && p.refs[in] > 0, s_part, &dummy);
-  low += dummy;
+  int before, n, low, total, dummy;
+  if (p.counts_here) {
+    // few pages: every block counts them all
+    int a = 0, b = 0;
+    for (int64_t i = threadIdx.x; i < p.pages; i += kPcPlanThreads) {
+      const int v = p.refs[i] > 0;
+      b += v;
+      a += i < (int64_t)blockIdx.x * kPcPlanThreads ? v : 0;
+    }
+    pc_block_scan<W>(a, s_part, &before);
+    pc_block_scan<W>(b, s_part, &n);
+    int c = 0;
+    for (int64_t i = threadIdx.x; i < n; i += kPcPlanThreads) c += p.refs[i] > 0;
+    pc_block_scan<W>(c, s_part, &low);
+  } else {
+    pc_live<W>(p, blockIdx.x, s_part, &before, &n);
+    // live pages below id n: the chunks before n's, and that chunk's own part
+    const int nc = n / kPcPlanThreads;
+    pc_live<W>(p, nc, s_part, &low, &dummy);
+    const int64_t in = (int64_t)nc * kPcPlanThreads + threadIdx.x;
+    pc_block_scan<W>(in < n && p.refs[in] > 0, s_part, &dummy);
+    low += dummy;
+  }
   const int64_t i = (int64_t)blockIdx.x * kPcPlanThreads + threadIdx.x;
   const int lv = i < p.pages && p.refs[i] > 0;
   const int at = before + pc_block_scan<W>(lv, s_part, &total) - lv;  // live pages before i
+  if (p.counts_here && threadIdx.x == 0) p.live[blockIdx.x] = total;
   if (i >= p.pages) return;
   int k = -1;
   if (lv && i >= n) {
@@ -517,6 +535,7 @@ int pc_compact_run(int64_t n, void* const* caches, const int64_t* row_bytes, con
   p.hole = p.high + pages;
   p.pages = pages;
   p.entries = entries;
+  p.counts_here = pages <= kPcCountsHere;
   int64_t tb = ((entries > pages ? entries : pages) + 4 * kPcThreads - 1) / (4 * kPcThreads);
   tb = tb < 1 ? 1 : (tb > 512 ? 512 : tb);
   bool first = true;
@@ -529,7 +548,7 @@ int pc_compact_run(int64_t n, void* const* caches, const int64_t* row_bytes, con
     const int64_t cap = 16ll * device_cu_count();
     p.copy_blocks = (int)(most < cap ? most : cap);
     if (first) {
-      pc_count_kernel<<<dim3((unsigned)p.chunks), kPcPlanThreads, 0, stream>>>(p);
+      if (!p.counts_here) pc_count_kernel<<<dim3((unsigned)p.chunks), kPcPlanThreads, 0, stream>>>(p);
       pc_rank_kernel<<<dim3((unsigned)p.chunks), kPcPlanThreads, 0, stream>>>(p);
     }
     const int64_t grid = p.table_blocks + p.copy_blocks;

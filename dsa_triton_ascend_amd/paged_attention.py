@@ -11,7 +11,7 @@ names, masks, zero rows and the return triple are those of
 import torch
 
 from . import _lib
-from .sparse_flash_attention import (INT64_MAX, _band_args, _check_device, _expect_shape, _seq_tensor)
+from .sparse_flash_attention import INT64_MAX, _band_args, _expect_shape, _seq_tensor
 
 _GROUPED_D = (64, 128, 256)
 _LATENT_D = (128, 256, 512)
@@ -49,67 +49,88 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
         raise ValueError("the latent form (value=None) needs query_rope and key_rope")
     if not latent and (query_rope is not None or key_rope is not None):
         raise ValueError("the grouped form takes no rope parts: rotate query and key instead")
-    if query.dim() != 4 or key.dim() != 4:
-        raise ValueError(f"query must be [B, S1, N1, D] and key [pages, page_size, N2, D], got {tuple(query.shape)} "
-                         f"and {tuple(key.shape)}")
-    B, S1, N1, D = query.shape
-    pages, page, N2, kd = key.shape
+    q_shape, k_shape = query.shape, key.shape
+    if len(q_shape) != 4 or len(k_shape) != 4:
+        raise ValueError(f"query must be [B, S1, N1, D] and key [pages, page_size, N2, D], got {tuple(q_shape)} "
+                         f"and {tuple(k_shape)}")
+    B, S1, N1, D = q_shape
+    pages, page, N2, kd = k_shape
     if kd != D:
         raise ValueError(f"key must have the query's {D} columns, got {kd}")
-    valid = _LATENT_D if latent else _GROUPED_D
-    if D not in valid:
-        raise ValueError(f"D must be one of {valid}, got {D}")
+    if D not in (_LATENT_D if latent else _GROUPED_D):
+        raise ValueError(f"D must be one of {_LATENT_D if latent else _GROUPED_D}, got {D}")
     if latent and N2 != 1:
         raise ValueError(f"the latent form has one key head, got {N2}")
     if N1 < 1 or N2 < 1 or N1 % N2:
         raise ValueError(f"query heads ({N1}) must be a multiple of key heads ({N2})")
-    if query.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"query dtype must be bfloat16 or float16, got {query.dtype}")
-    if latent:
-        _expect_shape(query_rope, (B, S1, N1, _D_ROPE), "query_rope")
-        _expect_shape(key_rope, (pages, page, 1, _D_ROPE), "key_rope")
+    dtype = query.dtype
+    if dtype is torch.bfloat16:
+        code = _lib.DTYPE_BF16
+    elif dtype is torch.float16:
+        code = _lib.DTYPE_FP16
     else:
-        _expect_shape(value, key.shape, "value")
-    for name, t in (("key", key), ("value", value), ("query_rope", query_rope), ("key_rope", key_rope)):
-        if t is not None and t.dtype != query.dtype:
-            raise ValueError(f"{name} dtype {t.dtype} differs from query dtype {query.dtype}")
+        raise ValueError(f"query dtype must be bfloat16 or float16, got {dtype}")
+    if latent:
+        if query_rope.shape[:-1] != q_shape[:-1] or query_rope.shape[-1] != _D_ROPE:
+            _expect_shape(query_rope, (B, S1, N1, _D_ROPE), "query_rope")
+        if key_rope.shape[:-1] != k_shape[:-1] or key_rope.shape[-1] != _D_ROPE:
+            _expect_shape(key_rope, (pages, page, 1, _D_ROPE), "key_rope")
+        others = (("key", key), ("query_rope", query_rope), ("key_rope", key_rope))
+    else:
+        if value.shape != k_shape:
+            _expect_shape(value, k_shape, "value")
+        others = (("key", key), ("value", value))
+    for name, t in others:
+        if t.dtype != dtype:
+            raise ValueError(f"{name} dtype {t.dtype} differs from query dtype {dtype}")
     if block_table is None or actual_seq_lengths_kv is None:
         raise ValueError("block_table and actual_seq_lengths_kv are required")
     if block_table.dim() != 2 or block_table.shape[0] < B:
         raise ValueError(f"block_table must be [B, max_blocks] with B={B} rows, got {tuple(block_table.shape)}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (query, key, value, query_rope, key_rope)):
+    if torch.is_grad_enabled() and (query.requires_grad or any(t.requires_grad for _, t in others)):
         raise ValueError("paged_attention has no backward: call it under torch.no_grad()")
-    dev = _check_device(query, key, value, query_rope, key_rope, block_table)
-    act_k = _seq_tensor(actual_seq_lengths_kv, dev)
-    act_q = _seq_tensor(actual_seq_lengths_query, dev)
+    index = _lib.same_device(query, key, value, query_rope, key_rope, block_table)
+    dev = query.device
+    act_k = _lengths(actual_seq_lengths_kv, dev)
+    act_q = None if actual_seq_lengths_query is None else _lengths(actual_seq_lengths_query, dev)
     if act_k.numel() != B or (act_q is not None and act_q.numel() != B):
         raise ValueError("actual sequence length arrays must have one entry per batch")
-    for name, t in (("key", key), ("value", value), ("key_rope", key_rope)):
-        if t is not None and not t.is_contiguous():
+    for name, t in others:
+        if name != "query_rope" and not t.is_contiguous():
             raise ValueError(f"the {name} cache must be contiguous (a copy of it would be made at every call)")
-    table = block_table.to(dtype=torch.int32).contiguous()
-    q = query.contiguous()
-    qr = query_rope.contiguous() if latent else None
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    smax = torch.empty(B, N2, S1, N1 // N2, dtype=torch.float32, device=dev)
+    table = block_table if block_table.dtype is torch.int32 else block_table.to(dtype=torch.int32)
+    if not table.is_contiguous():
+        table = table.contiguous()
+    q = query if query.is_contiguous() else query.contiguous()
+    qr = query_rope
+    if latent and not qr.is_contiguous():
+        qr = qr.contiguous()
+    out = q.new_empty(q_shape)
+    smax = torch.empty((B, N2, S1, N1 // N2), dtype=torch.float32, device=dev)
     ssum = torch.empty_like(smax)
     if q.numel() == 0:
         return out, smax, ssum
-    if key.numel() == 0 or table.shape[1] == 0:  # no page at all: no row sees a token
+    wide = table.shape[1]
+    if key.numel() == 0 or wide == 0:  # no page at all: no row sees a token
         return out.zero_(), smax.zero_(), ssum.zero_()
     lib = _lib.load()
-    with _lib.on_device(dev):
-        nbytes = lib.dsa_paged_attn_workspace_size(B, S1, N1, N2, D, 1 if latent else 0, table.shape[1], page)
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-        status = lib.dsa_paged_attn(
-            q.data_ptr(), _lib.ptr(qr), key.data_ptr(), _lib.ptr(key_rope), _lib.ptr(value), out.data_ptr(),
-            smax.data_ptr(), ssum.data_ptr(), _lib.ptr(act_q), act_k.data_ptr(), table.data_ptr(), B, S1, N1, N2, D,
-            _D_ROPE if latent else 0, pages, page, table.shape[1], sparse_mode, pre_tokens, next_tokens,
-            _lib.dtype_code(q.dtype), float(scale_value), 1 if return_softmax_lse else 0, ws.data_ptr(), nbytes,
-            _lib.stream_handle(dev))
-    _lib.check(status, "dsa_paged_attn")
+    nbytes = _lib.call_on(index, lib.dsa_paged_attn_workspace_size, B, S1, N1, N2, D, latent, wide, page)
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    status = _lib.call_on(
+        index, lib.dsa_paged_attn, q.data_ptr(), qr.data_ptr() if latent else None, key.data_ptr(),
+        key_rope.data_ptr() if latent else None, None if latent else value.data_ptr(), out.data_ptr(),
+        smax.data_ptr(), ssum.data_ptr(), None if act_q is None else act_q.data_ptr(), act_k.data_ptr(),
+        table.data_ptr(), B, S1, N1, N2, D, _D_ROPE if latent else 0, pages, page, wide, sparse_mode, pre_tokens,
+        next_tokens, code, float(scale_value), bool(return_softmax_lse), ws.data_ptr(), nbytes, _lib.raw_stream(index))
+    if status:
+        _lib.check(status, "dsa_paged_attn")
     return out, smax, ssum
+
+
+def _lengths(x, device):
+    if isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.device == device and x.is_contiguous():
+        return x
+    return _seq_tensor(x, device)
 
 
 class PagedAttention(torch.nn.Module):

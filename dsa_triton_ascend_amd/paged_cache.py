@@ -21,48 +21,48 @@ One decoding step:
     out, _, _ = paged_attention(q, latent_cache, None, table, lens + 1, ...)                 # per layer
     lens = lens + 1
 """
-import ctypes
+from array import array
 
 import torch
 
 from . import _lib
-from .sparse_flash_attention import _check_device
 
 _INT = torch.int32
 
 
 def _list(x, name):
     if isinstance(x, torch.Tensor):
-        x = [x]
-    x = list(x)
+        return [x]
     for t in x:
         if not isinstance(t, torch.Tensor):
             raise ValueError(f"{name} must be tensors")
     return x
 
 
-def _check_caches(caches, pages=None):
-    """Number of pages and page size of caches that share a table."""
-    size = None
+def _check_caches(caches):
+    """(pages, page size, addresses, bytes of a token's row) of caches that
+    share a table; (None, None, [], []) without caches."""
+    pages = page = None
+    addresses, row_bytes = [], []
     for t in caches:
-        if t.dim() < 3:
-            raise ValueError(f"a cache must be [pages, page_size, heads, columns], got {tuple(t.shape)}")
+        shape = t.shape
+        if len(shape) < 3:
+            raise ValueError(f"a cache must be [pages, page_size, heads, columns], got {tuple(shape)}")
         if not t.is_contiguous():
             raise ValueError("caches must be contiguous (they are changed in place)")
-        if size is None:
-            size = (t.shape[0], t.shape[1])
-        elif (t.shape[0], t.shape[1]) != size:
-            raise ValueError(f"all caches must have the same pages and page size, got {size} and {tuple(t.shape[:2])}")
-        if t.numel() == 0:
-            raise ValueError(f"a cache must not be empty, got {tuple(t.shape)}")
-    if pages is not None and size is not None and size[0] != pages:
-        raise ValueError(f"page_refs must have one entry per page ({size[0]}), got {pages}")
-    seen = {}
-    for t in caches:
-        if t.data_ptr() in seen:
-            raise ValueError("the same cache is given twice")
-        seen[t.data_ptr()] = True
-    return size
+        if pages is None:
+            pages, page = shape[0], shape[1]
+        elif shape[0] != pages or shape[1] != page:
+            raise ValueError("all caches must have the same pages and page size, got "
+                             f"{(pages, page)} and {tuple(shape[:2])}")
+        n = t.numel()
+        if n == 0:
+            raise ValueError(f"a cache must not be empty, got {tuple(shape)}")
+        addresses.append(t.data_ptr())
+        row_bytes.append(n // (pages * page) * t.element_size())
+    if len(set(addresses)) != len(addresses):
+        raise ValueError("the same cache is given twice")
+    return pages, page, addresses, row_bytes
 
 
 def _ints(t, name, dim):
@@ -70,19 +70,18 @@ def _ints(t, name, dim):
         raise ValueError(f"{name} must be int32, got {t.dtype}")
     if t.dim() != dim or t.numel() == 0:
         raise ValueError(f"{name} must have {dim} dimension(s) and not be empty, got {tuple(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _pointers(tensors):
-    return (ctypes.c_void_p * max(1, len(tensors)))(*[t.data_ptr() for t in tensors])
-
-
-def _longs(values):
-    return (ctypes.c_int64 * max(1, len(values)))(*values)
-
-
-def _row_bytes(t):
-    return t[0, 0].numel() * t.element_size()
+def _longs(*lists):
+    """The lists as arrays of 64-bit integers in one allocation: the owner,
+    which has to live until the call returns, and their addresses."""
+    a = array("q", [x for values in lists for x in values])
+    at, out = a.buffer_info()[0], []
+    for values in lists:
+        out.append(at)
+        at += 8 * len(values)
+    return a, out
 
 
 def paged_cache_write(caches, rows, block_table, seq_lengths, row_lengths=None, layout="BSND"):
@@ -101,11 +100,15 @@ def paged_cache_write(caches, rows, block_table, seq_lengths, row_lengths=None, 
     caches, rows = _list(caches, "caches"), _list(rows, "rows")
     if len(caches) != len(rows) or not caches:
         raise ValueError(f"one tensor of rows per cache is needed, got {len(rows)} for {len(caches)}")
-    if layout not in ("BSND", "TND"):
+    if layout == "BSND":
+        lead = 2
+    elif layout == "TND":
+        lead = 1
+    else:
         raise ValueError(f"layout must be BSND or TND, got {layout}")
-    pages, page = _check_caches(caches)
+    pages, page, addresses, sizes = _check_caches(caches)
     table = _ints(block_table, "block_table", 2)
-    batch = table.shape[0]
+    batch, wide = table.shape
     lens = _ints(seq_lengths, "seq_lengths", 1)
     if lens.shape[0] != batch:
         raise ValueError(f"seq_lengths must have one entry per row of block_table ({batch}), got {lens.shape[0]}")
@@ -113,36 +116,43 @@ def paged_cache_write(caches, rows, block_table, seq_lengths, row_lengths=None, 
         row_lengths = _ints(row_lengths, "row_lengths", 1)
         if row_lengths.shape[0] != batch:
             raise ValueError(f"row_lengths must have one entry per sequence ({batch}), got {row_lengths.shape[0]}")
-    elif layout == "TND":
+    elif lead == 1:
         raise ValueError("TND layout requires row_lengths (cumulative)")
-    lead = 1 if layout == "TND" else 2
-    tokens = tuple(rows[0].shape[:lead])
-    sizes, sb, st, kept = [], [], [], []
+    tokens = rows[0].shape[:lead]
+    if lead == 2 and tokens and tokens[0] != batch:
+        raise ValueError(f"rows must be [B={batch}, S, ...], got {tuple(rows[0].shape)}")
+    sources, sb, st, kept = [], [], [], []
     for r, c in zip(rows, caches):
-        if r.dim() != c.dim() - 2 + lead or tuple(r.shape[lead:]) != tuple(c.shape[2:]):
-            raise ValueError(f"rows {tuple(r.shape)} do not fit a cache {tuple(c.shape)}")
-        if tuple(r.shape[:lead]) != tokens or (lead == 2 and tokens[0] != batch):
-            raise ValueError(f"rows must be [{'T' if lead == 1 else f'B={batch}, S'}, ...], alike for all caches, "
-                             f"got {tuple(r.shape)}")
+        shape, inner = r.shape, c.shape[2:]
+        if shape[lead:] != inner:
+            raise ValueError(f"rows {tuple(shape)} do not fit a cache {tuple(c.shape)}")
+        if shape[:lead] != tokens:
+            raise ValueError(f"rows must have the same tokens for all caches, got {tuple(tokens)} and {tuple(shape)}")
         if r.dtype != c.dtype:
             raise ValueError(f"rows dtype {r.dtype} differs from cache dtype {c.dtype}")
-        if r.numel() and not r[(0,) * lead].is_contiguous():
-            r = r.contiguous()
-        kept.append(r)
+        stride, step = r.stride(), 1
+        for i in range(len(shape) - 1, lead - 1, -1):  # a token's row has to be in one piece
+            if stride[i] != step and shape[i] != 1:
+                r = r.contiguous()
+                stride = r.stride()
+                break
+            step *= shape[i]
         es = r.element_size()
-        sizes.append(_row_bytes(c))
-        sb.append(r.stride(0) * es if lead == 2 else 0)
-        st.append(r.stride(lead - 1) * es)
-    _check_device(*caches, *kept, table, lens, row_lengths)
+        kept.append(r)
+        sources.append(r.data_ptr())
+        sb.append(stride[0] * es if lead == 2 else 0)
+        st.append(stride[lead - 1] * es)
+    index = _lib.same_device(table, lens, row_lengths, *caches, *kept)
     n_tok = tokens[0] if lead == 1 else tokens[0] * tokens[1]
     if n_tok == 0:
         return
-    with _lib.on_device(table.device):
-        status = _lib.load().dsa_paged_cache_write(
-            len(caches), _pointers(kept), _pointers(caches), _longs(sizes), _longs(sb), _longs(st), table.data_ptr(),
-            lens.data_ptr(), _lib.ptr(row_lengths), batch, 0 if lead == 1 else tokens[1], n_tok, table.shape[1], pages,
-            page, _lib.LAYOUT[layout], _lib.stream_handle(table.device))
-    _lib.check(status, "dsa_paged_cache_write")
+    owner, (a_src, a_dst, a_size, a_sb, a_st) = _longs(sources, addresses, sizes, sb, st)
+    status = _lib.call_on(
+        index, _lib.load().dsa_paged_cache_write, len(caches), a_src, a_dst, a_size, a_sb, a_st, table.data_ptr(),
+        lens.data_ptr(), None if row_lengths is None else row_lengths.data_ptr(), batch,
+        0 if lead == 1 else tokens[1], n_tok, wide, pages, page, 2 - lead, _lib.raw_stream(index))
+    if status:
+        _lib.check(status, "dsa_paged_cache_write")
 
 
 def paged_cache_fork(caches, block_table, seq_lengths, page_refs, parents=None, new_tokens=0, page_size=None):
@@ -165,38 +175,43 @@ def paged_cache_fork(caches, block_table, seq_lengths, page_refs, parents=None, 
     Returns ``(block_table [C, max_blocks], seq_lengths [C], page_refs)``.
     """
     caches = _list(caches, "caches")
+    pages, page, addresses, sizes = _check_caches(caches)
     refs = _ints(page_refs, "page_refs", 1)
-    size = _check_caches(caches, refs.shape[0])
-    if size is None:
+    n_pages = refs.shape[0]
+    if pages is not None and pages != n_pages:
+        raise ValueError(f"page_refs must have one entry per page ({pages}), got {n_pages}")
+    if page is None:
         if page_size is None:
             raise ValueError("page_size is required without caches")
-    elif page_size is not None and page_size != size[1]:
-        raise ValueError(f"page_size ({page_size}) must equal the caches' ({size[1]})")
-    page = size[1] if size is not None else int(page_size)
+        page = int(page_size)
+    elif page_size is not None and page_size != page:
+        raise ValueError(f"page_size ({page_size}) must equal the caches' ({page})")
     table = _ints(block_table, "block_table", 2)
     rows, wide = table.shape
     lens = _ints(seq_lengths, "seq_lengths", 1)
     if lens.shape[0] != rows:
         raise ValueError(f"seq_lengths must have one entry per row of block_table ({rows}), got {lens.shape[0]}")
+    children = rows
     if parents is not None:
         parents = _ints(parents, "parents", 1)
+        children = parents.shape[0]
     if int(new_tokens) != new_tokens or not 0 <= new_tokens < 2 ** 31:
         raise ValueError(f"new_tokens must be an integer in [0, 2^31), got {new_tokens}")
-    _check_device(table, *caches, lens, refs, parents)
-    children = rows if parents is None else parents.shape[0]
-    dev = table.device
-    new_table = torch.empty(children, wide, dtype=_INT, device=dev)
-    new_lens = torch.empty(children, dtype=_INT, device=dev)
+    index = _lib.same_device(table, lens, refs, parents, *caches)
+    new_table = table.new_empty((children, wide))
+    new_lens = lens.new_empty(children)
     new_refs = torch.empty_like(refs)
     lib = _lib.load()
-    nbytes = lib.dsa_paged_cache_fork_workspace_size(rows, children, refs.shape[0])
-    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        status = lib.dsa_paged_cache_fork(
-            len(caches), _pointers(caches), _longs([_row_bytes(c) for c in caches]), table.data_ptr(), lens.data_ptr(),
-            refs.data_ptr(), _lib.ptr(parents), new_table.data_ptr(), new_lens.data_ptr(), new_refs.data_ptr(), rows,
-            children, wide, wide, refs.shape[0], page, int(new_tokens), ws.data_ptr(), nbytes, _lib.stream_handle(dev))
-    _lib.check(status, "dsa_paged_cache_fork")
+    nbytes = lib.dsa_paged_cache_fork_workspace_size(rows, children, n_pages)
+    ws = refs.new_empty((nbytes + 3) // 4)
+    owner, (a_caches, a_sizes) = _longs(addresses, sizes)
+    status = _lib.call_on(
+        index, lib.dsa_paged_cache_fork, len(caches), a_caches, a_sizes, table.data_ptr(), lens.data_ptr(),
+        refs.data_ptr(), None if parents is None else parents.data_ptr(), new_table.data_ptr(), new_lens.data_ptr(),
+        new_refs.data_ptr(), rows, children, wide, wide, n_pages, page, int(new_tokens), ws.data_ptr(), nbytes,
+        _lib.raw_stream(index))
+    if status:
+        _lib.check(status, "dsa_paged_cache_fork")
     return new_table, new_lens, new_refs
 
 
@@ -209,22 +224,25 @@ def paged_cache_compact(caches, block_table, page_refs, page_size=None):
     old page's new id (-1: it was free).
     """
     caches = _list(caches, "caches")
+    pages, page, addresses, sizes = _check_caches(caches)
     refs = _ints(page_refs, "page_refs", 1)
-    size = _check_caches(caches, refs.shape[0])
-    if size is not None and page_size is not None and page_size != size[1]:
-        raise ValueError(f"page_size ({page_size}) must equal the caches' ({size[1]})")
+    n_pages = refs.shape[0]
+    if pages is not None and pages != n_pages:
+        raise ValueError(f"page_refs must have one entry per page ({pages}), got {n_pages}")
+    if page is not None and page_size is not None and page_size != page:
+        raise ValueError(f"page_size ({page_size}) must equal the caches' ({page})")
     table = _ints(block_table, "block_table", 2)
     rows, wide = table.shape
-    _check_device(table, *caches, refs)
-    dev = table.device
+    index = _lib.same_device(table, refs, *caches)
     new_table, new_refs, page_map = torch.empty_like(table), torch.empty_like(refs), torch.empty_like(refs)
     lib = _lib.load()
-    nbytes = lib.dsa_paged_cache_compact_workspace_size(refs.shape[0])
-    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        status = lib.dsa_paged_cache_compact(
-            len(caches), _pointers(caches), _longs([_row_bytes(c) for c in caches]), table.data_ptr(), refs.data_ptr(),
-            new_table.data_ptr(), new_refs.data_ptr(), page_map.data_ptr(), rows, wide, refs.shape[0],
-            size[1] if size is not None else 1, ws.data_ptr(), nbytes, _lib.stream_handle(dev))
-    _lib.check(status, "dsa_paged_cache_compact")
+    nbytes = lib.dsa_paged_cache_compact_workspace_size(n_pages)
+    ws = refs.new_empty((nbytes + 3) // 4)
+    owner, (a_caches, a_sizes) = _longs(addresses, sizes)
+    status = _lib.call_on(
+        index, lib.dsa_paged_cache_compact, len(caches), a_caches, a_sizes, table.data_ptr(), refs.data_ptr(),
+        new_table.data_ptr(), new_refs.data_ptr(), page_map.data_ptr(), rows, wide, n_pages,
+        1 if page is None else page, ws.data_ptr(), nbytes, _lib.raw_stream(index))
+    if status:
+        _lib.check(status, "dsa_paged_cache_compact")
     return new_table, new_refs, page_map

@@ -14,7 +14,6 @@ import math
 import torch
 
 from . import _lib
-from .sparse_flash_attention import _check_device, _expect_shape
 
 SCALINGS = ("none", "linear", "ntk", "yarn")
 
@@ -75,20 +74,8 @@ def rotary_frequencies(dim, base=10000.0, scaling="none", factor=1.0, original_m
     return torch.tensor(freq, dtype=torch.float64, device=device), scale
 
 
-def _heads(t, layout, name):
-    """(batch, tokens, heads, columns) of a BSND or TND tensor."""
-    if t.dim() != (3 if layout == "TND" else 4):
-        raise ValueError(f"{name} must be {'[T, N, D]' if layout == 'TND' else '[B, S, N, D]'}, got {tuple(t.shape)}")
-    return (1,) + tuple(t.shape) if layout == "TND" else tuple(t.shape)
-
-
-def _strides(t):
-    """Batch, token and head strides in elements; None if the columns of a
-    head are not next to each other."""
-    s = t.stride()
-    if s[-1] != 1 and t.shape[-1] != 1:
-        return None
-    return (0,) + s[:2] if t.dim() == 3 else s[:3]
+_RANK = {"BSND": 4, "TND": 3}
+_DTYPE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
 
 
 def _overlaps_itself(t):
@@ -101,33 +88,41 @@ def _overlaps_itself(t):
     return False
 
 
-def _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, layout, inverse, inplace):
+def _side(t, start, inplace):
+    """Output and C arguments of one rotated tensor [(B,) S, N, D]."""
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] != 1:  # columns apart
+        t = t.contiguous()
+        st = t.stride()
+    shape = t.shape
+    out = t if inplace else torch.empty(shape, dtype=t.dtype, device=t.device)
+    so = out.stride()
+    if len(shape) == 4:
+        return t, out, (t.data_ptr(), out.data_ptr(), st[0], st[1], st[2], so[0], so[1], so[2], shape[2], shape[3], start)
+    return t, out, (t.data_ptr(), out.data_ptr(), 0, st[0], st[1], 0, so[0], so[1], shape[1], shape[2], start)
+
+
+_NO_KEY = (None, None) + (0,) * 9
+
+
+def _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, inplace):
     """Launch on checked arguments; returns the rotated query and key."""
-    outs, args = [], []
-    for t, start in ((query, q_start), (key, k_start)):
-        if t is None:
-            outs.append(None)
-            args += [None, None] + [0] * 9
-            continue
-        b, s, n, d = _heads(t, layout, "tensor")
-        st = _strides(t)
-        if st is None:
-            t = t.contiguous()
-            st = _strides(t)
-        out = t if inplace else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        outs.append(out)
-        args += [t.data_ptr(), out.data_ptr(), *st, *_strides(out), n, d, start]
-    b, s = _heads(query, layout, "query")[:2]
-    if query.numel() == 0:
-        return outs
-    per_seq = layout == "TND" or positions.dim() == 2
-    with _lib.on_device(query.device):
-        status = _lib.load().dsa_rope(
-            *args, positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0, 1 if per_seq else 0,
-            inv_freq.data_ptr(), b, s, 2 * inv_freq.numel(), 1 if interleaved else 0, 1 if inverse else 0,
-            _lib.dtype_code(query.dtype), scale, _lib.stream_handle(query.device))
-    _lib.check(status, "dsa_rope")
-    return outs
+    query, q_out, q_args = _side(query, q_start, inplace)
+    k_out, k_args = None, _NO_KEY
+    if key is not None:
+        key, k_out, k_args = _side(key, k_start, inplace)
+    shape = query.shape
+    b, s = (shape[0], shape[1]) if len(shape) == 4 else (1, shape[0])
+    if b == 0 or s == 0:
+        return q_out, k_out
+    index = query.get_device()
+    status = _lib.call_on(
+        index, _lib.load().dsa_rope, *q_args, *k_args, positions.data_ptr(), positions.dtype == torch.int64,
+        len(shape) == 3 or positions.dim() == 2, inv_freq.data_ptr(), b, s, 2 * inv_freq.shape[0], interleaved, inverse,
+        _DTYPE[query.dtype], scale, _lib.raw_stream(index))
+    if status:
+        _lib.check(status, "dsa_rope")
+    return q_out, k_out
 
 
 def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved=False, rotary_offset=0,
@@ -149,54 +144,58 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     views are read as they are if a head's columns are next to each other.
     Differentiable in query and key (not in place).
     """
-    if layout not in ("BSND", "TND"):
+    rank = _RANK.get(layout)
+    if rank is None:
         raise ValueError(f"layout must be BSND or TND, got {layout}")
     if positions is None or inv_freq is None:
         raise ValueError("positions and inv_freq are required")
-    b, s, n, d = _heads(query, layout, "query")
-    if query.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    shape = query.shape
+    if len(shape) != rank:
+        raise ValueError(f"query must be {'[T, N, D]' if rank == 3 else '[B, S, N, D]'}, got {tuple(shape)}")
+    lead = shape[:rank - 2]
+    if query.dtype not in _DTYPE:
         raise ValueError(f"query dtype must be bfloat16, float16 or float32, got {query.dtype}")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-    if inv_freq.dim() != 1 or inv_freq.numel() < 1:
+    if inv_freq.dim() != 1 or inv_freq.shape[0] < 1:
         raise ValueError(f"inv_freq must be a vector, got {tuple(inv_freq.shape)}")
-    rot = 2 * inv_freq.numel()
-    if positions.dim() != 1 or positions.shape[0] != s:
-        _expect_shape(positions, (s,) if layout == "TND" else (b, s), "positions")
+    rot = 2 * inv_freq.shape[0]
+    if positions.shape != lead and positions.shape != lead[-1:]:
+        raise ValueError(f"positions must have shape {tuple(lead)}, or {tuple(lead[-1:])} for all sequences, "
+                         f"got {tuple(positions.shape)}")
     if key_rotary_offset is None:
         key_rotary_offset = rotary_offset
-    checks = [("query", query, d, rotary_offset)]
     if key is not None:
-        kb, ks, _, kd = _heads(key, layout, "key")
-        if (kb, ks) != (b, s):
+        if key.dim() != rank or key.shape[:rank - 2] != lead:
             raise ValueError(f"key must have the query's batch and tokens, got {tuple(key.shape)}")
         if key.dtype != query.dtype:
             raise ValueError(f"key dtype {key.dtype} differs from query dtype {query.dtype}")
-        checks.append(("key", key, kd, key_rotary_offset))
-    for name, t, cols, start in checks:
-        if int(start) != start or not 0 <= start <= cols - rot:
-            raise ValueError(f"the {rot} rotary columns from {start} do not lie inside the {cols} of {name}")
+    for name, t, start in (("query", query, rotary_offset), ("key", key, key_rotary_offset)):
+        if t is not None and (int(start) != start or not 0 <= start <= t.shape[-1] - rot):
+            raise ValueError(f"the {rot} rotary columns from {start} do not lie inside the {t.shape[-1]} of {name}")
     grad = torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))
     if inplace:
         if grad:
             raise ValueError("inplace is for inference: the inputs require grad")
-        for name, t, _, _ in checks:
-            if _strides(t) is None or _overlaps_itself(t):
+        for name, t in (("query", query), ("key", key)):
+            if t is not None and ((t.stride(-1) != 1 and t.shape[-1] != 1) or _overlaps_itself(t)):
                 raise ValueError(f"inplace needs a {name} whose head columns are next to each other and whose "
                                  "elements do not share memory")
         if key is not None and key.numel() and query.numel() and key.data_ptr() == query.data_ptr():
             raise ValueError("inplace needs a key and a query of their own")
-    _check_device(query, key, positions, inv_freq)
-    positions = positions.contiguous()
-    inv_freq = inv_freq.to(torch.float64).contiguous()
+    _lib.same_device(query, key, positions, inv_freq)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.to(torch.float64).contiguous()
     args = (positions, inv_freq, bool(interleaved), int(rotary_offset), int(key_rotary_offset),
-            float(attention_scale), layout)
+            float(attention_scale), bool(inverse))
     if grad:
         from .autograd import RotaryEmbeddingFunction
-        return RotaryEmbeddingFunction.apply(query, key, *args, bool(inverse))
-    out = tuple(_rotate(query, key, *args, bool(inverse), inplace))
+        return RotaryEmbeddingFunction.apply(query, key, *args)
+    out = _rotate(query, key, *args, inplace)
     if inplace:
-        torch.autograd.graph.increment_version([t for _, t, _, _ in checks])
+        torch.autograd.graph.increment_version([t for t in out if t is not None])
     return out
 
 
