@@ -93,58 +93,93 @@ __device__ __forceinline__ int64_t wave_first(int64_t v) {
 }
 
 // inclusive sum over the lanes of a wave
-__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
+__device__ __forceinline__ int wave_scan(int v, int lane) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(v, o);
+    const int y = __shfl_up(v, o);
     if (lane >= o) v += y;
   }
   return v;
 }
 
 // The tiles of all sequences end to end, as a wave sees them (every lane
-// gets the same results).
+// gets the same results).  Lane l keeps sequence l of the first 64, so that
+// up to 64 sequences are read once.  (64 sequences have fewer than 2^31
+// tiles.)
 struct PagedPlan {
   int64_t total, per;  // tiles, tiles of a worker
+  PagedSeq seq;        // of this lane
+  int tiles, incl;     // its tiles, and those of the lanes up to it
 
   __device__ __forceinline__ void make(const PagedAttnParams& p, int tile, int lane) {
-    total = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 64) {
-      const int b = b0 + lane;
-      int64_t n = b < p.batch ? paged_tiles(paged_seq(p, b), tile) : 0;
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o);
-      total += wave_first(n);
+    tiles = 0;
+    if (lane < p.batch) {
+      seq = paged_seq(p, lane);
+      tiles = paged_tiles(seq, tile);
     }
-    per = max((total + p.workers - 1) / p.workers, (int64_t)p.min_tiles);
+    incl = wave_scan(tiles, lane);
+    total = __builtin_amdgcn_readlane(incl, 63);
+    for (int b0 = 64; b0 < p.batch; b0 += 64) {
+      const int b = b0 + lane;
+      const int n = wave_scan(b < p.batch ? paged_tiles(paged_seq(p, b), tile) : 0, lane);
+      total += __builtin_amdgcn_readlane(n, 63);
+    }
+    // (the quotient in 32 bits wherever it fits: a 64-bit one takes a microsecond)
+    const int64_t sum = total + p.workers - 1;
+    per = sum >> 32 ? sum / p.workers : (int64_t)((unsigned)sum / (unsigned)p.workers);
+    per = max(per, (int64_t)p.min_tiles);
   }
 
   // sequence that holds tile `at` (< total), and the tiles before it
-  __device__ __forceinline__ int find(const PagedAttnParams& p, int tile, int lane, int64_t at, int64_t* before) {
+  __device__ __forceinline__ int find(const PagedAttnParams& p, int tile, int lane, int64_t at, int64_t* before) const {
     int64_t base = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
       const int b = b0 + lane;
-      const int64_t n = b < p.batch ? paged_tiles(paged_seq(p, b), tile) : 0;
-      const int64_t incl = base + wave_scan(n, lane);
-      const unsigned long long m = __ballot(b < p.batch && incl > at);
+      int n = tiles, in = incl;
+      if (b0) {
+        n = b < p.batch ? paged_tiles(paged_seq(p, b), tile) : 0;
+        in = wave_scan(n, lane);
+      }
+      const unsigned long long m = __ballot(base + in > at);
       if (m) {
         const int first = __ffsll(m) - 1;
-        *before = wave_first(__shfl(incl - n, first));
+        *before = base + __builtin_amdgcn_readlane(in - n, first);
         return b0 + first;
       }
-      base = wave_first(__shfl(incl, 63));
+      base += __builtin_amdgcn_readlane(in, 63);
     }
     *before = base;
     return p.batch;
   }
 
-  // tiles before sequence `seq`
-  __device__ __forceinline__ int64_t start(const PagedAttnParams& p, int tile, int lane, int seq) {
+  // sequence b (the same on all lanes)
+  __device__ __forceinline__ PagedSeq sequence(const PagedAttnParams& p, int b) const {
+    PagedSeq s;
+    if (b < 64) {
+      s.act_q = __builtin_amdgcn_readlane(seq.act_q, b);
+      s.act_k = __builtin_amdgcn_readlane(seq.act_k, b);
+      s.lo = __builtin_amdgcn_readlane(seq.lo, b);
+      s.hi = __builtin_amdgcn_readlane(seq.hi, b);
+    } else {
+      s = paged_seq(p, b);
+      s.lo = __builtin_amdgcn_readfirstlane(s.lo);
+      s.hi = __builtin_amdgcn_readfirstlane(s.hi);
+    }
+    return s;
+  }
+
+  __device__ __forceinline__ int64_t worker_of(int64_t at) const {
+    return (at | per) >> 32 ? at / per : (int64_t)((unsigned)at / (unsigned)per);
+  }
+
+  // tiles before sequence b
+  __device__ __forceinline__ int64_t start(const PagedAttnParams& p, int tile, int lane, int b) const {
+    if (b < 64) return b ? __builtin_amdgcn_readlane(incl, b - 1) : 0;
     int64_t n = 0;
-    for (int b = lane; b < seq; b += 64) n += paged_tiles(paged_seq(p, b), tile);
+    for (int i = lane; i < b; i += 64) n += paged_tiles(paged_seq(p, i), tile);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o);
-    return n;
+    return wave_first(n);
   }
 };
 

@@ -31,9 +31,17 @@ __device__ __attribute__((aligned(16))) unsigned char g_paged_zero_row[1024];
 constexpr int kPaTile = 32;
 constexpr int kPaThreads = 256;
 
-template <typename T, int D, int MT>
-__global__ __launch_bounds__(kPaThreads, (D * MT <= 128 ? 3 : (D * MT <= 256 ? 2 : 1))) void paged_attn_kernel(
-    PagedAttnParams p) {
+// Waves of a SIMD: as many as keep everything in registers, at most two.  At
+// 128 columns three waves spill 12 registers, and each reload waits for the
+// tile on its way too (32 x 32K tokens of eight key heads: 711 us against 663
+// with two, 1350 with four); at 64 columns three fit and are slower (32 x 8K
+// tokens of four key heads: 55 to 62 us against 51).
+constexpr int pa_waves(int d, int mt) { return d <= 128 && mt <= 2 ? 2 : 1; }
+
+// STREAM: loads that keep nothing in the caches, for more K and V than the
+// caches hold from one call to the next.
+template <typename T, int D, int MT, bool STREAM>
+__global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel(PagedAttnParams p) {
   using E = Elem<T>;
   using V8 = typename E::v8;
   constexpr int KS = D / 32;   // k-steps of the scores
@@ -61,9 +69,7 @@ __global__ __launch_bounds__(kPaThreads, (D * MT <= 128 ? 3 : (D * MT <= 256 ? 2
   bool first_segment = true;
   while (at < end) {
     b = __builtin_amdgcn_readfirstlane(b);
-    PagedSeq seq = paged_seq(p, b);
-    seq.lo = __builtin_amdgcn_readfirstlane(seq.lo);
-    seq.hi = __builtin_amdgcn_readfirstlane(seq.hi);
+    const PagedSeq seq = plan.sequence(p, b);
     const int nt = paged_tiles(seq, kPaTile);
     if (nt == 0) {
       ++b;
@@ -115,6 +121,10 @@ __global__ __launch_bounds__(kPaThreads, (D * MT <= 128 ? 3 : (D * MT <= 256 ? 2
       const int64_t r = (int64_t)blk * p.page + (int)off;
       return blk < 0 || r >= p.kv_rows ? -1 : (int)r;
     };
+    auto load = [](auto* at) {
+      if constexpr (STREAM) return __builtin_nontemporal_load(at);
+      else return *at;
+    };
     u32x4 kf[2][KS];
     auto load_k = [&](int row) {
 #pragma unroll
@@ -122,7 +132,7 @@ __global__ __launch_bounds__(kPaThreads, (D * MT <= 128 ? 3 : (D * MT <= 256 ? 2
         const int r = __shfl(row, st * 16 + li);
         const unsigned char* src = r >= 0 ? kbase + r * row_bytes : g_paged_zero_row;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kf[st][ks] = *(const u32x4*)(src + ks * 64 + lg * 16);
+        for (int ks = 0; ks < KS; ++ks) kf[st][ks] = load((const u32x4*)(src + ks * 64 + lg * 16));
       }
     };
     typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
@@ -133,12 +143,12 @@ __global__ __launch_bounds__(kPaThreads, (D * MT <= 128 ? 3 : (D * MT <= 256 ? 2
         const int r = __shfl(row, (i >> 2) * 16 + lg * 4 + (i & 3));
         const unsigned char* src = r >= 0 ? vbase + r * row_bytes : g_paged_zero_row;
         if constexpr (D == 64) {
-          const u32x2 x = *(const u32x2*)(src + li * 8);
+          const u32x2 x = load((const u32x2*)(src + li * 8));
           vf[i][0] = x[0], vf[i][1] = x[1];
         } else {
 #pragma unroll
           for (int c = 0; c < VC; ++c) {
-            const u32x4 x = *(const u32x4*)(src + c * 256 + li * 16);
+            const u32x4 x = load((const u32x4*)(src + c * 256 + li * 16));
 #pragma unroll
             for (int e = 0; e < 4; ++e) vf[i][c * 4 + e] = x[e];
           }
@@ -291,9 +301,9 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, i
 
   PagedPlan plan;
   plan.make(p, tile, lane);
-  const int nt = paged_tiles(paged_seq(p, b), tile);
+  const int nt = paged_tiles(plan.sequence(p, b), tile);
   const int64_t first = plan.start(p, tile, lane, b), last = first + nt - 1;
-  const int64_t w0 = nt ? first / plan.per : 0, w1 = nt ? last / plan.per : -1;
+  const int64_t w0 = nt ? plan.worker_of(first) : 0, w1 = nt ? plan.worker_of(last) : -1;
   if (nt && w0 == w1) return;  // written whole by its worker
 
   const int c = tid % LPR, part = tid / LPR;
@@ -397,8 +407,7 @@ static PagedShape paged_grouped_shape(int64_t batch, int64_t s1, int64_t n1, int
   s.row_groups = (int)((rows + s.group_rows - 1) / s.group_rows);
   s.groups = (int)n2 * s.row_groups;
   s.min_tiles = 4;
-  const int waves = d * mt <= 128 ? 12 : (d * mt <= 256 ? 8 : 4);  // of a CU, as many as registers allow
-  s.workers = paged_workers((int64_t)device_cu_count() * waves, s.groups,
+  s.workers = paged_workers((int64_t)device_cu_count() * 4 * pa_waves((int)d, mt), s.groups,
                             batch * ((max_blocks * page + kPaTile - 1) / kPaTile), s.min_tiles);
   return s;
 }
@@ -414,18 +423,24 @@ size_t paged_attn_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t
   return paged_part_bytes(paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page), d);
 }
 
+template <typename T, int D, int MT>
+static void paged_launch_one(const PagedAttnParams& p, bool streaming, unsigned grid, hipStream_t stream) {
+  if (streaming) paged_attn_kernel<T, D, MT, true><<<grid, kPaThreads, 0, stream>>>(p);
+  else paged_attn_kernel<T, D, MT, false><<<grid, kPaThreads, 0, stream>>>(p);
+}
+
 template <typename T, int D>
-static void paged_launch_mt(const PagedAttnParams& p, unsigned grid, hipStream_t stream) {
-  if (p.group_rows == 16) paged_attn_kernel<T, D, 1><<<grid, kPaThreads, 0, stream>>>(p);
-  else if (p.group_rows == 32) paged_attn_kernel<T, D, 2><<<grid, kPaThreads, 0, stream>>>(p);
-  else if constexpr (D <= 128) paged_attn_kernel<T, D, 4><<<grid, kPaThreads, 0, stream>>>(p);
+static void paged_launch_mt(const PagedAttnParams& p, bool streaming, unsigned grid, hipStream_t stream) {
+  if (p.group_rows == 16) paged_launch_one<T, D, 1>(p, streaming, grid, stream);
+  else if (p.group_rows == 32) paged_launch_one<T, D, 2>(p, streaming, grid, stream);
+  else if constexpr (D <= 128) paged_launch_one<T, D, 4>(p, streaming, grid, stream);
 }
 
 template <typename T>
-static void paged_launch(const PagedAttnParams& p, int64_t d, unsigned grid, hipStream_t stream) {
-  if (d == 64) paged_launch_mt<T, 64>(p, grid, stream);
-  else if (d == 128) paged_launch_mt<T, 128>(p, grid, stream);
-  else paged_launch_mt<T, 256>(p, grid, stream);
+static void paged_launch(const PagedAttnParams& p, int64_t d, bool streaming, unsigned grid, hipStream_t stream) {
+  if (d == 64) paged_launch_mt<T, 64>(p, streaming, grid, stream);
+  else if (d == 128) paged_launch_mt<T, 128>(p, streaming, grid, stream);
+  else paged_launch_mt<T, 256>(p, streaming, grid, stream);
 }
 
 int paged_attn_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
@@ -476,8 +491,12 @@ int paged_attn_run(const void* query, const void* query_rope, const void* key, c
   } else {
     const int64_t waves = (int64_t)s.workers * s.groups;
     const unsigned grid = (unsigned)((waves + kPaThreads / 64 - 1) / (kPaThreads / 64));
-    if (dtype == DSA_DTYPE_BF16) paged_launch<bf16>(p, d, grid, stream);
-    else paged_launch<f16>(p, d, grid, stream);
+    // K and V that the caches could hold until the next call are kept there
+    // (134 MB: 38 us, streaming 41; 537 MB: 115 us, streaming 104)
+    const int64_t tokens = p.kv_rows < batch * max_blocks * page ? p.kv_rows : batch * max_blocks * page;
+    const bool streaming = tokens * n2 * d * 4 > (256ll << 20);
+    if (dtype == DSA_DTYPE_BF16) paged_launch<bf16>(p, d, streaming, grid, stream);
+    else paged_launch<f16>(p, d, streaming, grid, stream);
     DSA_HIP(hipGetLastError());
   }
   return paged_combine_launch(p, s.tile, d, dtype, stream);

@@ -142,9 +142,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   bool first_segment = true;
   while (at < end) {
     b = __builtin_amdgcn_readfirstlane(b);
-    PagedSeq seq = paged_seq(p, b);
-    seq.lo = __builtin_amdgcn_readfirstlane(seq.lo);
-    seq.hi = __builtin_amdgcn_readfirstlane(seq.hi);
+    const PagedSeq seq = plan.sequence(p, b);
     const int nt = paged_tiles(seq, TILE);
     if (nt == 0) {
       ++b;

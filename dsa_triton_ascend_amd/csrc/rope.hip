@@ -41,11 +41,10 @@ struct RopeParams {
   int rot, rot_units, interleaved;
   int tok_wg, parts, per_part;     // tokens of a workgroup; unit ranges they are cut into
   float scale, sign;
-  int stream;                      // the output does not fit the caches: stores that do not keep it there
 };
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeDeep = 4;
+constexpr int kRopeDeep = 3;
 constexpr int kRopeTab = 4096;  // cos and sin values of a workgroup's tokens
 
 template <typename T> struct RopeIo {
@@ -71,9 +70,13 @@ __device__ __forceinline__ int fast_div(unsigned n, unsigned d, unsigned magic) 
 // the lanes active in every second load and store, 117 against 99 us for 4096
 // tokens of 128 heads of 128 + 64 columns).  In place and with VEC = 1 a unit
 // is what one lane can turn alone: a pair of chunks or columns, or a copy.
-template <typename T, int VEC, bool INPLACE>
+template <typename T, int VEC, bool INPLACE, bool STREAM>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeParams p) {
   typedef T Vec __attribute__((ext_vector_type(VEC)));
+  // (a choice of two tensors' addresses is a flat address unless it is said
+  // that both are global; flat accesses wait for LDS too)
+  typedef __attribute__((address_space(1))) T GT;
+  typedef __attribute__((address_space(1))) Vec GVec;
   using Io = RopeIo<T>;
   constexpr bool kPairs = INPLACE || VEC == 1;
   __shared__ float s_tab[kRopeTab];
@@ -95,17 +98,17 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeParams p) {
   const int all = p.t[0].total + p.t[1].total;
   const int u0 = (blockIdx.x % p.parts) * p.per_part;
   const int u1 = min(u0 + p.per_part, all * ntok);
-  auto put = [&](T* at, Vec x) {
-    if (p.stream) __builtin_nontemporal_store(x, (Vec*)at);
-    else *(Vec*)at = x;
+  auto put = [&](GT* at, Vec x) {
+    if constexpr (STREAM) __builtin_nontemporal_store(x, (GVec*)at);
+    else *(GVec*)at = x;
   };
   // kRopeDeep units of a thread at a time: all their loads go out before the
   // first is used
   for (int ub = u0 + threadIdx.x; ub < u1; ub += kRopeThreads * kRopeDeep) {
     Vec va[kRopeDeep], vb[kRopeDeep];
-    T* dst[kRopeDeep];
+    GT* dst[kRopeDeep];
     int unit[kRopeDeep];  // chunk of the head; -1: none
-    const float* tab[kRopeDeep];
+    int tab[kRopeDeep];   // its token's sines and cosines
     int start[kRopeDeep];
 #pragma unroll
     for (int j = 0; j < kRopeDeep; ++j) {
@@ -119,12 +122,12 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeParams p) {
       const unsigned units = key ? p.t[1].units : p.t[0].units;
       const int h = fast_div((unsigned)r, units, key ? p.t[1].magic : p.t[0].magic), c = r - h * (int)units;
       const int64_t t = tok0 + tk, b = p.s == p.tokens ? 0 : t / p.s, s = t - b * p.s;
-      const T* in = (const T*)(key ? p.t[1].in : p.t[0].in) + b * (key ? p.t[1].in_sb : p.t[0].in_sb) +
+      const GT* in = (const GT*)(key ? p.t[1].in : p.t[0].in) + b * (key ? p.t[1].in_sb : p.t[0].in_sb) +
                     s * (key ? p.t[1].in_ss : p.t[0].in_ss) + h * (key ? p.t[1].in_sh : p.t[0].in_sh);
-      dst[j] = (T*)(key ? p.t[1].out : p.t[0].out) + b * (key ? p.t[1].out_sb : p.t[0].out_sb) +
+      dst[j] = (GT*)(key ? p.t[1].out : p.t[0].out) + b * (key ? p.t[1].out_sb : p.t[0].out_sb) +
                s * (key ? p.t[1].out_ss : p.t[0].out_ss) + h * (key ? p.t[1].out_sh : p.t[0].out_sh);
       unit[j] = c;
-      tab[j] = s_tab + tk * p.rot;
+      tab[j] = tk * p.rot;
       start[j] = key ? p.t[1].start : p.t[0].start;
       if constexpr (kPairs) {
         // pairs c * VEC ..: columns i and i + R/2, or (VEC = 1) 2i and 2i + 1
@@ -132,72 +135,72 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeParams p) {
           int col = (c - p.rot_units) * VEC;
           if (col >= start[j]) col += p.rot;
           dst[j] += col;
-          va[j] = *(const Vec*)(in + col);
+          va[j] = *(const GVec*)(in + col);
         } else {
           const int ca = start[j] + (p.interleaved ? (VEC > 1 ? c * VEC : 2 * c) : c * VEC);
           dst[j] += ca;
-          va[j] = *(const Vec*)(in + ca);
-          if (VEC == 1 || !p.interleaved) vb[j] = *(const Vec*)(in + ca + (p.interleaved ? 1 : half));
+          va[j] = *(const GVec*)(in + ca);
+          if (VEC == 1 || !p.interleaved) vb[j] = *(const GVec*)(in + ca + (p.interleaved ? 1 : half));
         }
       } else {
         // chunk c of the head; unit: its place in the rotary slice, or past it
         const int col = c * VEC, i = col - start[j];
         dst[j] += col;
-        va[j] = *(const Vec*)(in + col);
+        va[j] = *(const GVec*)(in + col);
         unit[j] = i >= 0 && i < p.rot ? i / VEC : p.rot_units;
-        if (!p.interleaved && unit[j] < p.rot_units) vb[j] = *(const Vec*)(in + col + (i < half ? half : -half));
+        if (!p.interleaved && unit[j] < p.rot_units) vb[j] = *(const GVec*)(in + col + (i < half ? half : -half));
       }
     }
 #pragma unroll
     for (int j = 0; j < kRopeDeep; ++j) {
       const int c = unit[j];
       if (c < 0) continue;
-      if (c >= p.rot_units) {
-        put(dst[j], va[j]);
-      } else if (VEC > 1 && p.interleaved) {
-        Vec w;
+      // one store for all lanes, turned or copied (stores of their own for
+      // each took 10 us more of 94)
+      Vec w = va[j];
+      if (c < p.rot_units) {
+        if (VEC > 1 && p.interleaved) {
 #pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) {
-          const float cs = tab[j][c * VEC + 2 * i], sn = tab[j][c * VEC + 2 * i + 1];
-          const float a = Io::get(va[j][2 * i]), bb = Io::get(va[j][VEC > 1 ? 2 * i + 1 : 0]);
-          w[2 * i] = Io::put(a * cs - bb * sn);
-          w[VEC > 1 ? 2 * i + 1 : 0] = Io::put(a * sn + bb * cs);
-        }
-        put(dst[j], w);
-      } else if (!kPairs) {
-        // the other member of each pair is in vb
-        const bool first = c * VEC < half;
-        const float* t2 = tab[j] + 2 * (c * VEC - (first ? 0 : half));
-        Vec w;
+          for (int i = 0; i < VEC / 2; ++i) {
+            const float cs = s_tab[tab[j] + c * VEC + 2 * i], sn = s_tab[tab[j] + c * VEC + 2 * i + 1];
+            const float a = Io::get(va[j][2 * i]), bb = Io::get(va[j][VEC > 1 ? 2 * i + 1 : 0]);
+            w[2 * i] = Io::put(a * cs - bb * sn);
+            w[VEC > 1 ? 2 * i + 1 : 0] = Io::put(a * sn + bb * cs);
+          }
+        } else if constexpr (!kPairs) {
+          // the other member of each pair is in vb
+          const bool first = c * VEC < half;
+          const int t2 = tab[j] + 2 * (c * VEC - (first ? 0 : half));
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float cs = t2[2 * i], sn = first ? -t2[2 * i + 1] : t2[2 * i + 1];
-          w[i] = Io::put(Io::get(va[j][i]) * cs + Io::get(vb[j][i]) * sn);
-        }
-        put(dst[j], w);
-      } else {
-        Vec wa, wb;
+          for (int i = 0; i < VEC; ++i) {
+            const float cs = s_tab[t2 + 2 * i], s1 = s_tab[t2 + 2 * i + 1], sn = first ? -s1 : s1;
+            w[i] = Io::put(Io::get(va[j][i]) * cs + Io::get(vb[j][i]) * sn);
+          }
+        } else {
+          Vec wb;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float cs = tab[j][2 * (c * VEC + i)], sn = tab[j][2 * (c * VEC + i) + 1];
-          const float a = Io::get(va[j][i]), bb = Io::get(vb[j][i]);
-          wa[i] = Io::put(a * cs - bb * sn);
-          wb[i] = Io::put(a * sn + bb * cs);
+          for (int i = 0; i < VEC; ++i) {
+            const float cs = s_tab[tab[j] + 2 * (c * VEC + i)], sn = s_tab[tab[j] + 2 * (c * VEC + i) + 1];
+            const float a = Io::get(va[j][i]), bb = Io::get(vb[j][i]);
+            w[i] = Io::put(a * cs - bb * sn);
+            wb[i] = Io::put(a * sn + bb * cs);
+          }
+          put(dst[j] + (p.interleaved ? 1 : half), wb);
         }
-        put(dst[j], wa);
-        put(dst[j] + (p.interleaved ? 1 : half), wb);
       }
+      put(dst[j], w);
     }
   }
 }
 
 template <typename T>
-static void rope_launch(const RopeParams& p, int vec, bool inplace, int64_t grid, hipStream_t stream) {
+static void rope_launch(const RopeParams& p, int vec, bool inplace, bool streaming, int64_t grid, hipStream_t stream) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const dim3 g((unsigned)grid);
-  if (vec == 1) rope_kernel<T, 1, true><<<g, kRopeThreads, 0, stream>>>(p);
-  else if (inplace) rope_kernel<T, VEC, true><<<g, kRopeThreads, 0, stream>>>(p);
-  else rope_kernel<T, VEC, false><<<g, kRopeThreads, 0, stream>>>(p);
+  if (vec == 1) rope_kernel<T, 1, true, false><<<g, kRopeThreads, 0, stream>>>(p);
+  else if (inplace) rope_kernel<T, VEC, true, false><<<g, kRopeThreads, 0, stream>>>(p);
+  else if (streaming) rope_kernel<T, VEC, false, true><<<g, kRopeThreads, 0, stream>>>(p);
+  else rope_kernel<T, VEC, false, false><<<g, kRopeThreads, 0, stream>>>(p);
 }
 
 // strides: in (batch, token, head) then out, in elements
@@ -257,7 +260,7 @@ int rope_run(const void* const in[2], void* const out[2], const int64_t* const s
   // interleaved 81.9 and 87.1)
   int64_t bytes = 0;
   for (int i = 0; i < n; ++i) bytes += tokens * heads[i] * d[i] * es;
-  p.stream = bytes > (64ll << 20);
+  const bool streaming = bytes > (64ll << 20);  // more than the caches hold for whoever reads it
   const int64_t groups = (tokens + p.tok_wg - 1) / p.tok_wg;
   const int64_t units = p.tok_wg * all;
   int64_t parts = 4ll * device_cu_count() / groups;
@@ -267,9 +270,9 @@ int rope_run(const void* const in[2], void* const out[2], const int64_t* const s
   p.parts = (int)((units + p.per_part - 1) / p.per_part);
   const int64_t grid = groups * p.parts;
   DSA_CHECK_SUPPORTED(grid < (1ll << 31), "too many tokens");
-  if (dtype == DSA_DTYPE_BF16) rope_launch<bf16>(p, vec, inplace, grid, stream);
-  else if (dtype == DSA_DTYPE_FP16) rope_launch<f16>(p, vec, inplace, grid, stream);
-  else rope_launch<float>(p, vec, inplace, grid, stream);
+  if (dtype == DSA_DTYPE_BF16) rope_launch<bf16>(p, vec, inplace, streaming, grid, stream);
+  else if (dtype == DSA_DTYPE_FP16) rope_launch<f16>(p, vec, inplace, streaming, grid, stream);
+  else rope_launch<float>(p, vec, inplace, streaming, grid, stream);
   DSA_HIP(hipGetLastError());
   return DSA_OK;
 }
