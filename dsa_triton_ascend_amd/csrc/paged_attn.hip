@@ -24,6 +24,8 @@
 // idle otherwise), so the weights keep 16 bits and more.
 #include "paged_attn.h"
 
+#include <type_traits>
+
 namespace dsa {
 
 __device__ __attribute__((aligned(16))) unsigned char g_paged_zero_row[1024];
@@ -254,7 +256,7 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
       } else {
         const int64_t slot = (((int64_t)worker * 2 + (first_segment ? 0 : 1)) * p.groups + ng) * p.group_rows +
                              mt * 16 + li;
-        float* dst = p.part_o + slot * D;
+        float* dst = (float*)p.part_o + slot * D;
 #pragma unroll
         for (int c = 0; c < NJ / EC; ++c)
 #pragma unroll
@@ -278,103 +280,157 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
 }
 
 // ---------------------------------------------------------------------------
-// join: one workgroup per (sequence, row).  A row of D floats is read by
-// D / 4 lanes, so 256 / (D / 4) runs are read side by side, four deep.
-// Sequences without a visible token get their zeros here.
+// join: a workgroup takes `wg_rows` rows of a sequence.  With up to 64 runs a
+// wave takes a row; with more (one row per workgroup, where the host expects
+// them) the four waves share them.  A lane holds D / 64 columns and, for the
+// weights, one run of 64.  Sequences without a visible token get their zeros
+// here.
 // ---------------------------------------------------------------------------
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, int tile) {
+constexpr int kPcFewRuns = 64;
+
+template <typename T, int D, bool HALF>
+__global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, int tile, int wg_rows) {
   using E = Elem<T>;
-  constexpr int LPR = D / 4;
-  constexpr int PAR = 256 / LPR;
-  __shared__ f32x4 s_o[256];
-  __shared__ float s_l[PAR], s_n[PAR];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int per_seq = p.n2 * p.rows;
-  const int b = blockIdx.x / per_seq;
-  const int rest = blockIdx.x - b * per_seq;
-  const int kvh = rest / p.rows, rr = rest - kvh * p.rows;  // row rr = s * group + head
-  const int rg = rr / p.group_rows, ng = kvh * p.row_groups + rg;
-  const int s = rr / p.group;
-  const int64_t orow = ((int64_t)b * p.s1 + s) * p.n1 + kvh * p.group + (rr - s * p.group);
-  const int64_t srow = ((int64_t)b * p.n2 + kvh) * p.rows + rr;
+  constexpr int EPL = D / 64;
+  typedef T TV __attribute__((ext_vector_type(EPL)));
+  typedef float FV __attribute__((ext_vector_type(EPL)));
+  typedef f16 HV __attribute__((ext_vector_type(EPL)));
+  __shared__ FV s_o[4][64];
+  __shared__ float s_l[4], s_n[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int per_seq = p.n2 * p.rows, groups = (per_seq + wg_rows - 1) / wg_rows;
+  const int b = blockIdx.x / groups, row0 = (blockIdx.x - b * groups) * wg_rows;
 
   PagedPlan plan;
   plan.make(p, tile, lane);
   const int nt = paged_tiles(plan.sequence(p, b), tile);
   const int64_t first = plan.start(p, tile, lane, b), last = first + nt - 1;
-  const int64_t w0 = nt ? plan.worker_of(first) : 0, w1 = nt ? plan.worker_of(last) : -1;
-  if (nt && w0 == w1) return;  // written whole by its worker
+  const int64_t w0 = nt ? plan.worker_of(first) : 0;
+  const int runs = nt ? (int)(plan.worker_of(last) - w0) + 1 : 0;
+  if (runs == 1) return;  // written whole by its worker
+  const int slot0 = first != w0 * plan.per ? 1 : 0;  // of the first worker; the others' is 0
 
-  const int c = tid % LPR, part = tid / LPR;
-  auto slot = [&](int64_t w) {
-    const int k = w == w0 && first != w * plan.per ? 1 : 0;
-    return ((w * 2 + k) * p.groups + ng) * p.group_rows + (rr - rg * p.group_rows);
-  };
-  float big = -INFINITY, top = -INFINITY;
-  for (int64_t w = w0 + lane; w <= w1; w += 64) {
-    const f32x4 ml = p.part_ml[slot(w)];
-    big = fmaxf(big, ml[0]);
-    top = fmaxf(top, ml[2]);
-  }
-  big = wave_max(big);
-  top = wave_max(top);
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f, norm = 0.f;
-  if (big != -INFINITY) {
-#pragma unroll 4
-    for (int64_t w = w0 + part; w <= w1; w += PAR) {
-      const int64_t at = slot(w);
-      const f32x4 ml = p.part_ml[at];
-      const f32x4 x = *(const f32x4*)(p.part_o + at * D + c * 4);
-      const float f = fast_exp2(ml[0] - big);
-      o += x * f;
-      l += ml[1] * f;
-      norm += ml[3] * f;
+  // the runs i0 .. i1 of a row, summed relative to the largest reference of all
+  auto row_of = [&](int row, int i0, int i1, float* big, float* top, FV* o, float* l, float* n) {
+    const int kvh = row / p.rows, rr = row - kvh * p.rows;  // row rr = s * group + head
+    const int rg = rr / p.group_rows;
+    const int64_t in_group = (int64_t)(kvh * p.row_groups + rg) * p.group_rows + (rr - rg * p.group_rows);
+    const int64_t span = (int64_t)p.groups * p.group_rows;
+    auto slot = [&](int i) { return ((w0 + i) * 2 + (i == 0 ? slot0 : 0)) * span + in_group; };
+    float m = -INFINITY, t = -INFINITY;
+    for (int i = lane; i < runs; i += 64) {
+      const f32x4 ml = p.part_ml[slot(i)];
+      m = fmaxf(m, ml[0]);
+      t = fmaxf(t, ml[2]);
     }
-  }
-  s_o[tid] = o;
-  if (c == 0) s_l[part] = l, s_n[part] = norm;
-  __syncthreads();
-  if (part == 0) {
-    l = s_l[0];
-    norm = s_n[0];
+    *big = m = wave_max(m);
+    *top = wave_max(t);
+    FV acc = {};
+    float la = 0.f, na = 0.f;
+    if (m != -INFINITY)
+      for (int c = i0; c < i1; c += 64) {
+        const int mine = c + lane;
+        float f = 0.f;
+        if (mine < i1) {
+          const int64_t at = slot(mine);
+          const f32x4 ml = p.part_ml[at];
+          f = fast_exp2(ml[0] - m);
+          la += ml[1] * f;
+          na += ml[3] * f;
+          if constexpr (HALF) f *= ml[3] * p.part_scale[at];
+        }
+        const int cnt = min(64, i1 - c);
+        for (int i = 0; i < cnt; i += 8) {
+          // eight rows in flight (those past the last read it again, times zero)
+          std::conditional_t<HALF, HV, FV> x[8];
 #pragma unroll
-    for (int i = 1; i < PAR; ++i) {
-      o += s_o[i * LPR + c];
-      l += s_l[i];
-      norm += s_n[i];
-    }
-    const float inv = norm > 0.f ? 1.f / norm : 0.f;
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    const T4 r = {E::from_f32(o[0] * inv), E::from_f32(o[1] * inv), E::from_f32(o[2] * inv), E::from_f32(o[3] * inv)};
-    *(T4*)((T*)p.out + orow * D + c * 4) = r;
-    if (c == 0 && p.smax) {
+          for (int u = 0; u < 8; ++u)
+            x[u] = *((const std::conditional_t<HALF, HV, FV>*)p.part_o + slot(c + min(i + u, cnt - 1)) * 64 + lane);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const float g =
+                i + u < cnt ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (i + u) & 63)) : 0.f;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) acc[e] += i + u < cnt ? (float)x[u][e] * g : 0.f;
+          }
+        }
+      }
+    *o = acc;
+    *l = wave_sum(la);
+    *n = wave_sum(na);
+  };
+  auto write = [&](int row, FV o, float big, float top, float l, float n) {
+    const int kvh = row / p.rows, rr = row - kvh * p.rows;
+    const int s = rr / p.group;
+    const int64_t orow = ((int64_t)b * p.s1 + s) * p.n1 + kvh * p.group + (rr - s * p.group);
+    const float inv = n > 0.f ? 1.f / n : 0.f;
+    TV r;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) r[e] = E::from_f32(o[e] * inv);
+    *(TV*)((T*)p.out + orow * D + lane * EPL) = r;
+    if (lane == 0 && p.smax) {
+      const int64_t srow = (int64_t)b * per_seq + row;
       const bool any = p.return_lse && l > 0.f;
       p.smax[srow] = any ? top * kLn2 : 0.f;
       p.ssum[srow] = any ? l * fast_exp2(big - top) : 0.f;
     }
+  };
+  FV o;
+  float big, top, l, n;
+  if (runs <= kPcFewRuns && wg_rows > 1) {
+    if (row0 + wave < per_seq) {
+      row_of(row0 + wave, 0, runs, &big, &top, &o, &l, &n);
+      write(row0 + wave, o, big, top, l, n);
+    }
+    return;
+  }
+  const int part = (runs + 3) / 4;
+  for (int row = row0; row < min(row0 + wg_rows, per_seq); ++row) {
+    row_of(row, min(wave * part, runs), min((wave + 1) * part, runs), &big, &top, &o, &l, &n);
+    s_o[wave][lane] = o;
+    if (lane == 0) s_l[wave] = l, s_n[wave] = n;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        o += s_o[w][lane];
+        l += s_l[w];
+        n += s_n[w];
+      }
+      write(row, o, big, top, l, n);
+    }
+    __syncthreads();
   }
 }
 
+template <typename T, int D>
+static void paged_combine_one(const PagedAttnParams& p, int tile, int wg_rows, unsigned grid, hipStream_t stream) {
+  if (p.half_parts) paged_combine_kernel<T, D, true><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
+  else paged_combine_kernel<T, D, false><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
+}
+
 template <typename T>
-static void paged_combine_d(const PagedAttnParams& p, int tile, int64_t d, unsigned grid, hipStream_t stream) {
-  if (d == 64) paged_combine_kernel<T, 64><<<grid, 256, 0, stream>>>(p, tile);
-  else if (d == 128) paged_combine_kernel<T, 128><<<grid, 256, 0, stream>>>(p, tile);
-  else if (d == 256) paged_combine_kernel<T, 256><<<grid, 256, 0, stream>>>(p, tile);
-  else paged_combine_kernel<T, 512><<<grid, 256, 0, stream>>>(p, tile);
+static void paged_combine_d(const PagedAttnParams& p, int tile, int wg_rows, int64_t d, unsigned grid, hipStream_t stream) {
+  if (d == 64) paged_combine_kernel<T, 64, false><<<grid, 256, 0, stream>>>(p, tile, wg_rows);  // grouped form only
+  else if (d == 128) paged_combine_one<T, 128>(p, tile, wg_rows, grid, stream);
+  else if (d == 256) paged_combine_one<T, 256>(p, tile, wg_rows, grid, stream);
+  else paged_combine_one<T, 512>(p, tile, wg_rows, grid, stream);
 }
 
 int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream) {
-  const unsigned grid = (unsigned)((int64_t)p.batch * p.n2 * p.rows);
-  if (dtype == DSA_DTYPE_BF16) paged_combine_d<bf16>(p, tile, d, grid, stream);
-  else paged_combine_d<f16>(p, tile, d, grid, stream);
+  // rows of a workgroup: four, one per wave, unless the average sequence has
+  // so many runs that the waves had better share them
+  const int wg_rows = p.workers > 32ll * p.batch ? 1 : 4;
+  const unsigned grid = (unsigned)(p.batch * (((int64_t)p.n2 * p.rows + wg_rows - 1) / wg_rows));
+  if (dtype == DSA_DTYPE_BF16) paged_combine_d<bf16>(p, tile, wg_rows, d, grid, stream);
+  else paged_combine_d<f16>(p, tile, wg_rows, d, grid, stream);
   DSA_HIP(hipGetLastError());
   return DSA_OK;
 }
 
 size_t paged_part_bytes(const PagedShape& s, int64_t d) {
-  return (size_t)s.workers * 2 * s.groups * s.group_rows * (d * sizeof(float) + sizeof(f32x4));
+  const size_t rows = (size_t)s.workers * 2 * s.groups * s.group_rows;
+  return rows * (sizeof(f32x4) + (s.half_parts ? d * sizeof(f16) + sizeof(float) : d * sizeof(float)));
 }
 
 // Workers of a lane group for `slots` workers resident at once.  As many as
@@ -399,6 +455,7 @@ int paged_workers(int64_t slots, int64_t groups, int64_t tiles, int min_tiles) {
 static PagedShape paged_grouped_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d,
                                       int64_t max_blocks, int64_t page) {
   PagedShape s;
+  s.half_parts = 0;
   s.tile = kPaTile;
   const int64_t rows = s1 * (n1 / n2);
   int mt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
@@ -463,8 +520,11 @@ int paged_attn_run(const void* query, const void* query_rope, const void* key, c
   p.act_q = act_q;
   p.act_k = act_k;
   p.table = table;
-  p.part_o = (float*)workspace;
-  p.part_ml = (f32x4*)(p.part_o + (int64_t)s.workers * 2 * s.groups * s.group_rows * d);
+  const int64_t part_rows = (int64_t)s.workers * 2 * s.groups * s.group_rows;
+  p.half_parts = s.half_parts;
+  p.part_ml = (f32x4*)workspace;
+  p.part_o = p.part_ml + part_rows;
+  p.part_scale = (float*)((f16*)p.part_o + part_rows * d);  // with half_parts
   p.kv_rows = num_blocks * page;
   p.band_pre = band_clamp(pre_tokens);
   p.band_next = band_clamp(next_tokens);

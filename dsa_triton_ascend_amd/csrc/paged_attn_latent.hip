@@ -85,7 +85,9 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   __shared__ int s_tab[kPlPages];
   __shared__ float s_f[2 * HG];  // by a tile's parity: factors of the rows whose reference moved
   __shared__ int s_flag[3];  // by a tile's number modulo 3: bits of the waves whose rows moved
-  float* const s_n = (float*)s_p;  // of a finished run, in place of P: the rows' divisors
+  // of a finished run, in place of P: the rows' divisors, and largest outputs as bits
+  float* const s_n = (float*)s_p;
+  int* const s_am = (int*)s_p + HG;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int li = lane & 15, lg = lane >> 4;
@@ -142,7 +144,11 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   bool first_segment = true;
   while (at < end) {
     b = __builtin_amdgcn_readfirstlane(b);
-    const PagedSeq seq = plan.sequence(p, b);
+    // (where the output fills the registers, what the plan keeps of the
+    // sequences would not stay in them)
+    PagedSeq seq = HG == 128 ? paged_seq(p, b) : plan.sequence(p, b);
+    seq.lo = __builtin_amdgcn_readfirstlane(seq.lo);
+    seq.hi = __builtin_amdgcn_readfirstlane(seq.hi);
     const int nt = paged_tiles(seq, TILE);
     if (nt == 0) {
       ++b;
@@ -454,6 +460,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       const int r = wave * 16 + li, rr = rg * HG + r;
       if (scores && lg == 0) {
         s_n[r] = n;
+        s_am[r] = 0;
         if (rr < p.rows) {
           if (!whole) {
             p.part_ml[slot0 + r] = {ref, l, top, n};
@@ -483,13 +490,44 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
           }
         }
       }
-    } else {
+    } else if constexpr (kLo) {
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
         if (rg * HG + ht * 16 + li < p.rows) {
-          float* dst = p.part_o + (slot0 + ht * 16 + li) * D + col;
+          float* dst = (float*)p.part_o + (slot0 + ht * 16 + li) * D + col;
 #pragma unroll
           for (int j = 0; j < NDW; ++j) *(f32x4*)(dst + j * 16) = acc[j][ht];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int ht = 0; ht < HW; ++ht) {
+        float a = 0.f;
+#pragma unroll
+        for (int j = 0; j < NDW; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) a = fmaxf(a, fabsf(acc[j][ht][r]));
+        a = xgroup_max(a);
+        if (lg == 0) atomicMax(s_am + ht * 16 + li, __float_as_int(a));  // (not negative: ordered as integers)
+      }
+      lds_barrier();
+#pragma unroll
+      for (int ht = 0; ht < HW; ++ht) {
+        const float n = s_n[ht * 16 + li], a = __int_as_float(s_am[ht * 16 + li]);
+        const float inv = n > 0.f ? 1.f / n : 0.f;
+        int ex = 0;
+        if (a * inv > 0.f) (void)frexpf(a * inv, &ex);  // a / n < 2^ex
+        ex = max(ex, -100);
+        const float mul = ldexpf(inv, -ex);
+        if (rg * HG + ht * 16 + li < p.rows) {
+          const int64_t slot = slot0 + ht * 16 + li;
+          if (wave == 0 && lg == 0) p.part_scale[slot] = ldexpf(1.f, ex);
+          f16* dst = (f16*)p.part_o + slot * D + col;
+#pragma unroll
+          for (int j = 0; j < NDW; ++j) {
+            const f32x4 x = acc[j][ht] * mul;
+            *(f16x4*)(dst + j * 16) = (f16x4){(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3]};
+          }
         }
       }
     }
@@ -505,8 +543,10 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
 PagedShape paged_latent_shape(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t max_blocks, int64_t page) {
   PagedShape s;
   s.tile = kPlTile;
+  s.half_parts = 0;
   const int64_t rows = s1 * n1;
   s.group_rows = rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 ? 64 : 128));
+  s.half_parts = s.group_rows > 32;  // as P is rounded once there
   s.row_groups = (int)((rows + s.group_rows - 1) / s.group_rows);
   s.groups = s.row_groups;
   s.min_tiles = 8;
