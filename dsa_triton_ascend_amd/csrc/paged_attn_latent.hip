@@ -177,10 +177,6 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       }
       if (live) paged_bounds(p, seq.act_q, seq.act_k, row / p.n1, &all_lo, &all_hi);
     }
-    // the loads end here, not inside the tile loop, where a wait for them
-    // would be one for the tiles in flight too
-#pragma unroll
-    for (int ks = 0; ks < KQR; ++ks) asm volatile("" : "+v"(qf[ks]));
     // tokens that all of the wave's rows see need no mask
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) {
@@ -208,6 +204,11 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       for (int i = tid; i < npg; i += kPlThreads) s_tab[i] = tab[pg0 + i];
       lds_barrier();
       const int n_tiles = (tb - ta + TILE - 1) / TILE;
+      // Q's loads, on their way beside the table's, end here and not inside
+      // the tile loop, where a wait for them would be one for the tiles in
+      // flight too
+#pragma unroll
+      for (int ks = 0; ks < KQR; ++ks) asm volatile("" : "+v"(qf[ks]));
 
       // cache row of token lane % 32 of tile t, -1 past the end or without a
       // page (both are read as zeros)
