@@ -42,10 +42,27 @@ namespace dsa {
 __device__ __attribute__((aligned(16))) unsigned char g_latent_zero_row[1024];
 
 constexpr int kPlTile = 32;
+
+// The LDS-DMAs of sfa_fwd.h, and the same with loads that keep nothing in
+// the caches.
+template <bool STREAM>
+__device__ __forceinline__ void pl_dma_buf(unsigned lds_base, int voff, __amdgpu_buffer_rsrc_t rsrc) {
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+                 :: "s"(lds_base), "v"(voff), "s"(rsrc) : "memory");
+  else dma_buf16(lds_base, voff, rsrc);
+}
+template <bool STREAM>
+__device__ __forceinline__ void pl_dma_glb(unsigned lds_base, const void* gaddr) {
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+                 :: "s"(lds_base), "v"(gaddr) : "memory");
+  else dma_glb16(lds_base, gaddr);
+}
 constexpr int kPlThreads = 512;
 constexpr int kPlPages = 512;  // block-table entries held in LDS
 
-template <int D, typename T, int HG>
+template <int D, typename T, int HG, bool STREAM>
 __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnParams p) {
   using E = Elem<T>;
   using V8 = typename E::v8;
@@ -232,18 +249,18 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
             const int r = __builtin_amdgcn_readlane(rows, j * NL + lw);
             const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
                 (void*)(kbase + (int64_t)(r < 0 ? 0 : r) * (D * 2)), (short)0, r < 0 ? 0 : D * 2, 0x00020000);
-            dma_buf16(dst, (ln ^ nope_swz(j * NL + lw)) * 16, rsrc);
+            pl_dma_buf<STREAM>(dst, (ln ^ nope_swz(j * NL + lw)) * 16, rsrc);
           } else {
             const int tk = (j * NL + lw) * TPI + ((unsigned)ln / CPT);
             const int ch = ((unsigned)ln % CPT) ^ nope_swz(tk);
             const int r = __shfl(rows, tk);
-            dma_glb16(dst, r >= 0 ? kbase + (int64_t)r * (D * 2) + ch * 16 : g_latent_zero_row + ch * 16);
+            pl_dma_glb<STREAM>(dst, r >= 0 ? kbase + (int64_t)r * (D * 2) + ch * 16 : g_latent_zero_row + ch * 16);
           }
         } else if (rope_wave) {
           const int tk = lw * 8 + (ln >> 3);
           const int ch = (ln & 7) ^ rope_swz(tk);
           const int r = __shfl(rows, tk);
-          dma_glb16(smem_base + rope_off(lw * 8, rbuf),
+          pl_dma_glb<STREAM>(smem_base + rope_off(lw * 8, rbuf),
                     r >= 0 ? rbase + (int64_t)r * (DR * 2) + ch * 16 : g_latent_zero_row + ch * 16);
         }
       };
@@ -556,19 +573,26 @@ PagedShape paged_latent_shape(int64_t batch, int64_t s1, int64_t n1, int64_t d, 
   return s;
 }
 
-template <int D, typename T>
+template <int D, typename T, bool STREAM>
 static void paged_latent_hg(const PagedAttnParams& p, unsigned grid, hipStream_t stream) {
-  if (p.group_rows == 16) paged_latent_kernel<D, T, 16><<<grid, kPlThreads, 0, stream>>>(p);
-  else if (p.group_rows == 32) paged_latent_kernel<D, T, 32><<<grid, kPlThreads, 0, stream>>>(p);
-  else if (p.group_rows == 64) paged_latent_kernel<D, T, 64><<<grid, kPlThreads, 0, stream>>>(p);
-  else paged_latent_kernel<D, T, 128><<<grid, kPlThreads, 0, stream>>>(p);
+  if (p.group_rows == 16) paged_latent_kernel<D, T, 16, STREAM><<<grid, kPlThreads, 0, stream>>>(p);
+  else if (p.group_rows == 32) paged_latent_kernel<D, T, 32, STREAM><<<grid, kPlThreads, 0, stream>>>(p);
+  else if (p.group_rows == 64) paged_latent_kernel<D, T, 64, STREAM><<<grid, kPlThreads, 0, stream>>>(p);
+  else paged_latent_kernel<D, T, 128, STREAM><<<grid, kPlThreads, 0, stream>>>(p);
 }
 
 template <typename T>
 static void paged_latent_d(const PagedAttnParams& p, int64_t d, unsigned grid, hipStream_t stream) {
-  if (d == 128) paged_latent_hg<128, T>(p, grid, stream);
-  else if (d == 256) paged_latent_hg<256, T>(p, grid, stream);
-  else paged_latent_hg<512, T>(p, grid, stream);
+  // rows that the caches cannot hold until the next call, read by one row
+  // group only, are not kept there (512 columns; 1.2 GB at 16 heads: 222 us,
+  // streaming 192; 300 MB at 32 rows: 85 and 79; 75 MB at 16: 28 and 29)
+  const int64_t tokens = p.kv_rows < (int64_t)p.batch * p.max_blocks * p.page
+                             ? p.kv_rows : (int64_t)p.batch * p.max_blocks * p.page;
+  const bool streaming = p.row_groups == 1 && tokens * (d + 64) * 2 > (256ll << 20);
+  if (d == 128) paged_latent_hg<128, T, false>(p, grid, stream);
+  else if (d == 256) paged_latent_hg<256, T, false>(p, grid, stream);
+  else if (streaming) paged_latent_hg<512, T, true>(p, grid, stream);
+  else paged_latent_hg<512, T, false>(p, grid, stream);
 }
 
 int paged_latent_launch(const PagedAttnParams& p, int64_t d, int32_t dtype, hipStream_t stream) {
