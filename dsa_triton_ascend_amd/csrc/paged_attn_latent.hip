@@ -128,10 +128,9 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   int b = plan.find(p, TILE, lane, at, &before);
 
   // scores in log2 units are s * scale - ref, one operation each; for that
-  // the scale is positive (Q takes its sign) and not zero (masked scores are
-  // -inf before it)
-  const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
-  const unsigned flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+  // the scale is positive: Q takes its sign, and is zero where it is
+  const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  const unsigned flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
   const unsigned smem_base = (unsigned)(uintptr_t)smem;
   const unsigned char* const kbase = (const unsigned char*)p.k;
   const unsigned char* const rbase = (const unsigned char*)p.kr;
@@ -187,7 +186,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       for (int ks = 0; ks < KS; ++ks) {
         const T* src = ks < KSN ? (const T*)p.q + qrow * D + ks * 32 + lg * 8
                                 : (const T*)p.qr + qrow * DR + (ks - KSN) * 32 + lg * 8;
-        const u32x4 x = *(const u32x4*)src ^ flip;
+        const u32x4 x = (*(const u32x4*)src & keep) ^ flip;
         if (ks < KQR) qf[ks < KQR ? ks : 0] = as_v8<V8>(x);
         else if constexpr (QL > 0)
           *(u32x4*)(s_q + (((wave * 16 + li) * (QL * 64) + ((lg ^ nope_swz(li)) * 16)) ^ ((ks - KQR) << 6))) = x;

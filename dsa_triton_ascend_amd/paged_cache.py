@@ -19,7 +19,7 @@ One decoding step:
     table, lens, refs = paged_cache_fork(caches, table, lens, refs, parents, new_tokens=1)   # once
     paged_cache_write([latent, k_rope, k_index], [...], table, lens)                         # per layer
     out, _, _ = paged_attention(q, latent_cache, None, table, lens + 1, ...)                 # per layer
-    lens = lens + 1
+    lens = lens + 1                                                                          # of rows in use
 """
 from array import array
 
@@ -159,9 +159,9 @@ def paged_cache_fork(caches, block_table, seq_lengths, page_refs, parents=None, 
     """The block table of the next step: rows forked, reordered, released and
     given room.
 
-    New row c continues row ``parents[c]`` (int32; negative: an empty row;
-    None: every row continues itself) and has pages for ``new_tokens`` more
-    tokens.  Rows that nobody continues are released.  Full pages are shared;
+    New row c continues row ``parents[c]`` (int32; negative: an empty row,
+    length 0 and no pages; None: every row continues itself) and has pages for
+    ``new_tokens`` more tokens.  Rows that nobody continues are released.  Full pages are shared;
     a partly filled last page stays with the first row that continues it if
     nobody else refers to it, and is copied in all ``caches`` for every other.
     Pages come from those free before the call, lowest first, to rows in

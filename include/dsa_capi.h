@@ -444,8 +444,8 @@ int dsa_paged_cache_write(int64_t n_caches, const void* const* rows, void* const
 
 /*
  * Fork: the block table of the next step.  New row c continues row parents[c]
- * (negative or out of range: an empty row; parents NULL: row c continues row
- * c), with pages for new_tokens more tokens.  Rows that nobody continues are
+ * (negative or out of range: an empty row of length 0 without pages; parents
+ * NULL: row c continues row c), with pages for new_tokens more tokens.  Rows that nobody continues are
  * released.  Full pages are shared.  The last page, where partly filled, is
  * kept by the first row that continues its sequence, if page_refs counts
  * nobody else on it, and is copied, up to its last token, for every other.

@@ -343,3 +343,59 @@ def test_matches_sparse_flash_attention_where_all_tokens_are_selected():
         # each off by at most 2^-8 of the value and twice 2^-8 of the mean |v|
         assert (out[b].double() - ref[b].double()).abs().max() <= 2 * 3 * 2.0 ** -8 * v
     assert torch.allclose(mx, rmax, rtol=2.0 ** -20, atol=1e-4) and torch.allclose(sm, rsum, rtol=1e-3)
+
+
+@pytest.mark.parametrize("latent,N1,N2,D", [(False, 16, 8, 128), (False, 40, 2, 64), (False, 6, 3, 256), (True, 16, 1, 512),
+                                            (True, 32, 1, 512), (True, 64, 1, 512), (True, 128, 1, 512)])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_streaming_loads(latent, N1, N2, D, dt):
+    """A pool and a table for more tokens than the caches hold, whose loads
+    stream, with short sequences in it (one of them without a page in the
+    middle)."""
+    page, lens = 64, [400, 131, 0, 64]
+    args, data = _make(4, 1, N1, N2, D, page, lens, DTYPES[dt], latent, seed=23, hole=(0, 2, -1))
+    cols = N2 * (D + 64 if latent else 2 * D)
+    pool = (300 << 20) // (page * cols * 2) + 1
+    table = torch.full((4, pool), -1, dtype=torch.int32, device="cuda")
+    ids = torch.randperm(pool, device="cuda")[:16].int()
+    for name in ("key", "key_rope" if latent else "value"):
+        small = args[name]
+        big = torch.full((pool, *small.shape[1:]), float("nan"), dtype=small.dtype, device="cuda")
+        at = 0
+        for b, n in enumerate(lens):
+            for i in range(-(-n // page)):
+                old = int(args["block_table"][b, i])
+                if old >= 0:
+                    table[b, i] = ids[at]
+                    big[int(ids[at])] = small[old]
+                at += 1
+        args[name] = big
+    args["block_table"] = table
+    _compare(args, data, lens)
+
+
+def test_negative_and_zero_scale():
+    lens = [100, 333]
+    for latent in (False, True):
+        for scale in (-0.07, 0.0):
+            args, data = _make(2, 2, 16, 1 if latent else 4, 512 if latent else 128, 16, lens, torch.bfloat16, latent,
+                               seed=61)
+            args["scale_value"] = scale
+            _compare(args, data, lens)
+
+
+def test_lengths_past_the_table_and_negative():
+    """More tokens than the table holds count as those it holds, fewer than none as none."""
+    import dsa_triton_ascend_amd as dsa
+    lens = [128, 64, 0]
+    for latent in (False, True):
+        args, data = _make(3, 1, 8, 1 if latent else 2, 512 if latent else 128, 64, lens, torch.bfloat16, latent,
+                           seed=71)
+        for name in ("key", "value", "key_rope"):
+            if args[name] is not None:
+                args[name].nan_to_num_(0.25)
+        args["actual_seq_lengths_kv"] = torch.tensor([128, 64, 0], dtype=torch.int32, device="cuda")
+        want = dsa.paged_attention(**args)
+        args["actual_seq_lengths_kv"] = torch.tensor([2 ** 31 - 1, 64, -7], dtype=torch.int32, device="cuda")
+        got = dsa.paged_attention(**args)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
