@@ -68,13 +68,15 @@ static int check_workspace(const void* workspace, size_t bytes, size_t need) {
   return DSA_OK;
 }
 
+constexpr int64_t kMaxTableTokens = 1ll << 35;  // of a block table: the kernels count its 32-token tiles in 32 bits
+
 static bool paged_attn_sizes_ok(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
                                 int64_t max_blocks, int64_t page) {
   return batch >= 1 && batch <= (1 << 24) && s1 >= 1 && n2 >= 1 && n1 >= n2 && n1 % n2 == 0 &&
          within(s1, n1, 1ll << 24) && within(batch * s1, n1, (1ll << 31) - 1) &&
          (latent ? n2 == 1 && (d == 128 || d == 256 || d == 512) : d == 64 || d == 128 || d == 256) &&
          page >= 1 && page <= (1 << 20) && max_blocks >= 1 && max_blocks <= (1 << 20) &&
-         within(max_blocks, page, 65535ll * 1024);
+         within(max_blocks, page, 65535ll * 1024) && within(batch, max_blocks * page, kMaxTableTokens);
 }
 
 }  // namespace dsa
@@ -244,6 +246,8 @@ int dsa_paged_attn(const void* query, const void* query_rope, const void* key, c
   DSA_CHECK_ARG(within(s1, n1, 1ll << 24) && within(batch * s1, n1, (1ll << 31) - 1), "too many query rows");
   int st = check_pages(num_blocks, page_size, max_blocks);
   if (st != DSA_OK) return st;
+  DSA_CHECK_SUPPORTED(within(batch, max_blocks * page_size, kMaxTableTokens),
+                      "batch * max_blocks * page size must be <= 2^35");
   // 16-byte loads of rows
   DSA_CHECK_ARG((((uintptr_t)query | (uintptr_t)key | (uintptr_t)value | (uintptr_t)query_rope | (uintptr_t)key_rope |
                   (uintptr_t)attention_out) & 15) == 0, "tensors must be 16-byte aligned");

@@ -5,6 +5,8 @@
 // sequences are laid end to end, and every worker (a wave or a workgroup)
 // takes an equal run of them, whatever the lengths: no worker waits for a
 // long sequence while others idle, and the host need not know the lengths.
+// Where the workers suffice for it, each sequence starts a run of its own: a
+// run that crosses from one sequence into the next fills its pipeline twice.
 // A run that covers a sequence whole writes its output; every other run
 // leaves its softmax sums and unnormalised output in the workspace, and
 // paged_combine_kernel joins the runs of a sequence.
@@ -90,33 +92,53 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
   return s;
 }
 
+// sequence b, the same on all lanes (nothing past the last)
+__device__ __forceinline__ PagedSeq paged_seq_uniform(const PagedAttnParams& p, int b) {
+  PagedSeq s = paged_seq(p, min(b, p.batch - 1));
+  s.lo = __builtin_amdgcn_readfirstlane(s.lo);
+  s.hi = b < p.batch ? __builtin_amdgcn_readfirstlane(s.hi) : s.lo;
+  return s;
+}
+
 __device__ __forceinline__ int paged_tiles(const PagedSeq& s, int tile) { return (s.hi - s.lo + tile - 1) / tile; }
 
-// the first lane's value, for all (a scalar to the compiler)
-__device__ __forceinline__ int64_t wave_first(int64_t v) {
-  const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)v);
-  const int hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
-  return ((int64_t)hi << 32) | lo;
-}
-
-// inclusive sum over the lanes of a wave
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(v, o);
-    if (lane >= o) v += y;
-  }
+// inclusive sum over the lanes of a wave (in registers: six exchanges by LDS
+// take half a microsecond)
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15: lane 15's to 16.., 47's to 48..
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: lane 31's to 32..
   return v;
 }
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
 // The tiles of all sequences end to end, as a wave sees them (every lane
-// gets the same results).  Lane l keeps sequence l of the first 64, so that
-// up to 64 sequences are read once.  (64 sequences have fewer than 2^31
-// tiles.)
+// gets the same results); the tiles of a sequence are counted as a multiple
+// of `grain`, what is behind its last tile is nobody's work.  grain is the
+// length of a run, so that sequences start runs, if there are workers enough
+// for runs of the balanced length or kPaSlack tiles more, and 1 otherwise.
+// Lane l keeps sequence l of the first 64, so that up to 64 sequences are
+// read once.  (The entry point refuses tables of more than 2^30 tiles, so all
+// of this is in 32 bits: 64-bit quotients take a microsecond each.)
+//
+// A sequence more in a run costs some 2 to 4 tiles (its rows, pages and first
+// tiles have to arrive, its output leaves): 4 sequences of 40 tokens at 128
+// heads took 86 us in one run, 27 in four; one tile too many is cheaper.
+constexpr int kPaSlack = 2;
+constexpr int kPaMinTiles = 2;
+
 struct PagedPlan {
-  int64_t total, per;  // tiles, tiles of a worker
-  PagedSeq seq;        // of this lane
-  int tiles, incl;     // its tiles, and those of the lanes up to it
+  int total, per;   // tiles, tiles of a worker
+  int grain;
+  PagedSeq seq;     // of this lane
+  int tiles, incl;  // its tiles, and those of the lanes up to it
+
+  __device__ __forceinline__ int padded(int n) const {
+    return grain == 1 ? n : (int)((unsigned)(n + grain - 1) / (unsigned)grain) * grain;
+  }
 
   __device__ __forceinline__ void make(const PagedAttnParams& p, int tile, int lane) {
     tiles = 0;
@@ -124,29 +146,39 @@ struct PagedPlan {
       seq = paged_seq(p, lane);
       tiles = paged_tiles(seq, tile);
     }
-    incl = wave_scan(tiles, lane);
+    incl = wave_scan(tiles);
     total = __builtin_amdgcn_readlane(incl, 63);
-    for (int b0 = 64; b0 < p.batch; b0 += 64) {
-      const int b = b0 + lane;
-      const int n = wave_scan(b < p.batch ? paged_tiles(paged_seq(p, b), tile) : 0, lane);
-      total += __builtin_amdgcn_readlane(n, 63);
+    if (p.batch > 64) {
+      int n = 0;
+#pragma unroll 4
+      for (int b = 64 + lane; b < p.batch; b += 64) n += paged_tiles(paged_seq(p, b), tile);
+      total += wave_total(n);
     }
-    // (the quotient in 32 bits wherever it fits: a 64-bit one takes a microsecond)
-    const int64_t sum = total + p.workers - 1;
-    per = sum >> 32 ? sum / p.workers : (int64_t)((unsigned)sum / (unsigned)p.workers);
-    per = max(per, (int64_t)p.min_tiles);
+    per = max((int)((unsigned)(total + p.workers - 1) / (unsigned)p.workers), p.min_tiles);
+    grain = 1;
+    if (p.batch > p.workers) return;
+    for (int g = per; g <= per + kPaSlack; g += kPaSlack) {
+      int n = (int)((unsigned)(tiles + g - 1) / (unsigned)g);
+#pragma unroll 4
+      for (int b = 64 + lane; b < p.batch; b += 64)
+        n += (int)((unsigned)(paged_tiles(paged_seq(p, b), tile) + g - 1) / (unsigned)g);
+      const int runs = wave_total(n);
+      if (runs <= p.workers) {
+        grain = per = g;
+        total = runs * g;
+        tiles = padded(tiles);
+        incl = wave_scan(tiles);
+        break;
+      }
+    }
   }
 
   // sequence that holds tile `at` (< total), and the tiles before it
-  __device__ __forceinline__ int find(const PagedAttnParams& p, int tile, int lane, int64_t at, int64_t* before) const {
-    int64_t base = 0;
+  __device__ __forceinline__ int find(const PagedAttnParams& p, int tile, int lane, int at, int* before) const {
+    int base = 0, n = tiles, in = incl;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
-      const int b = b0 + lane;
-      int n = tiles, in = incl;
-      if (b0) {
-        n = b < p.batch ? paged_tiles(paged_seq(p, b), tile) : 0;
-        in = wave_scan(n, lane);
-      }
+      const int b = b0 + 64 + lane;
+      const int next = b < p.batch ? padded(paged_tiles(paged_seq(p, b), tile)) : 0;
       const unsigned long long m = __ballot(base + in > at);
       if (m) {
         const int first = __ffsll(m) - 1;
@@ -154,6 +186,8 @@ struct PagedPlan {
         return b0 + first;
       }
       base += __builtin_amdgcn_readlane(in, 63);
+      n = next;
+      in = wave_scan(n);
     }
     *before = base;
     return p.batch;
@@ -175,18 +209,15 @@ struct PagedPlan {
     return s;
   }
 
-  __device__ __forceinline__ int64_t worker_of(int64_t at) const {
-    return (at | per) >> 32 ? at / per : (int64_t)((unsigned)at / (unsigned)per);
-  }
+  __device__ __forceinline__ int worker_of(int at) const { return (int)((unsigned)at / (unsigned)per); }
 
   // tiles before sequence b
-  __device__ __forceinline__ int64_t start(const PagedAttnParams& p, int tile, int lane, int b) const {
+  __device__ __forceinline__ int start(const PagedAttnParams& p, int tile, int lane, int b) const {
     if (b < 64) return b ? __builtin_amdgcn_readlane(incl, b - 1) : 0;
-    int64_t n = 0;
-    for (int i = lane; i < b; i += 64) n += paged_tiles(paged_seq(p, i), tile);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o);
-    return wave_first(n);
+    int n = 0;
+#pragma unroll 4
+    for (int i = lane; i < b; i += 64) n += padded(paged_tiles(paged_seq(p, i), tile));
+    return wave_total(n);
   }
 };
 
@@ -195,7 +226,7 @@ struct PagedShape {
   int workers, min_tiles, groups, row_groups, group_rows, tile, half_parts;
 };
 size_t paged_part_bytes(const PagedShape& s, int64_t d);
-int paged_workers(int64_t slots, int64_t groups, int64_t tiles, int min_tiles);
+int paged_workers(int64_t slots, int64_t groups, int64_t batch, int64_t tiles, int min_tiles);
 int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream);
 PagedShape paged_latent_shape(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t max_blocks, int64_t page);
 int paged_latent_launch(const PagedAttnParams& p, int64_t d, int32_t dtype, hipStream_t stream);

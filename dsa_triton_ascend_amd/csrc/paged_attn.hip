@@ -59,25 +59,25 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
 
   PagedPlan plan;
   plan.make(p, kPaTile, lane);
-  int64_t at = (int64_t)worker * plan.per;
-  const int64_t end = min(at + plan.per, plan.total);
-  if (at >= end) return;
-  int64_t before;
+  if (worker >= (plan.total + plan.per - 1) / plan.per) return;
+  int at = worker * plan.per;
+  const int end = min(at + plan.per, plan.total);
+  int before;
   int b = plan.find(p, kPaTile, lane, at, &before);
   const int64_t row_bytes = (int64_t)p.n2 * D * 2;
   const unsigned char* kbase = (const unsigned char*)p.k + (int64_t)kvh * D * 2;
   const unsigned char* vbase = (const unsigned char*)p.v + (int64_t)kvh * D * 2;
 
   bool first_segment = true;
+  b = __builtin_amdgcn_readfirstlane(b);
+  PagedSeq seq = plan.sequence(p, b);  // (later ones are read again: the plan's do not stay in registers)
   while (at < end) {
-    b = __builtin_amdgcn_readfirstlane(b);
-    const PagedSeq seq = plan.sequence(p, b);
     const int nt = paged_tiles(seq, kPaTile);
     if (nt == 0) {
-      ++b;
+      seq = paged_seq_uniform(p, ++b);
       continue;
     }
-    const int t0 = (int)(at - before), t1 = (int)min(end - before, (int64_t)nt);
+    const int t0 = at - before, t1 = min(end - before, nt);
     const int tok0 = seq.lo + t0 * kPaTile, tok1 = min(seq.hi, seq.lo + t1 * kPaTile);
     const int32_t* tab = p.table + (int64_t)b * p.max_blocks;
 
@@ -273,8 +273,8 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
     first_segment = false;
     at = before + t1;
     if (t1 == nt) {
-      before += nt;
-      ++b;
+      at = before += plan.padded(nt);
+      if (at < end) seq = paged_seq_uniform(p, ++b);
     }
   }
 }
@@ -304,9 +304,9 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, i
   PagedPlan plan;
   plan.make(p, tile, lane);
   const int nt = paged_tiles(plan.sequence(p, b), tile);
-  const int64_t first = plan.start(p, tile, lane, b), last = first + nt - 1;
-  const int64_t w0 = nt ? plan.worker_of(first) : 0;
-  const int runs = nt ? (int)(plan.worker_of(last) - w0) + 1 : 0;
+  const int first = plan.start(p, tile, lane, b), last = first + nt - 1;
+  const int w0 = nt ? plan.worker_of(first) : 0;
+  const int runs = nt ? plan.worker_of(last) - w0 + 1 : 0;
   if (runs == 1) return;  // written whole by its worker
   const int slot0 = first != w0 * plan.per ? 1 : 0;  // of the first worker; the others' is 0
 
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, i
     const int rg = rr / p.group_rows;
     const int64_t in_group = (int64_t)(kvh * p.row_groups + rg) * p.group_rows + (rr - rg * p.group_rows);
     const int64_t span = (int64_t)p.groups * p.group_rows;
-    auto slot = [&](int i) { return ((w0 + i) * 2 + (i == 0 ? slot0 : 0)) * span + in_group; };
+    auto slot = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i == 0 ? slot0 : 0)) * span + in_group; };
     float m = -INFINITY, t = -INFINITY;
     for (int i = lane; i < runs; i += 64) {
       const f32x4 ml = p.part_ml[slot(i)];
@@ -435,9 +435,9 @@ size_t paged_part_bytes(const PagedShape& s, int64_t d) {
 
 // Workers of a lane group for `slots` workers resident at once.  As many as
 // fill the slots once; where the lane groups alone come near that, so many
-// that the last round of them is nearly full too.  Never more than the
-// longest lengths keep busy.
-int paged_workers(int64_t slots, int64_t groups, int64_t tiles, int min_tiles) {
+// that the last round of them is nearly full too.  Never more than sequences
+// of the longest length, `tiles`, keep busy.
+int paged_workers(int64_t slots, int64_t groups, int64_t batch, int64_t tiles, int min_tiles) {
   int64_t best = slots / groups;
   if (best < 8) {
     double best_fill = 0;
@@ -448,7 +448,7 @@ int paged_workers(int64_t slots, int64_t groups, int64_t tiles, int min_tiles) {
       if (fill > best_fill + 0.02) best = w, best_fill = fill;
     }
   }
-  const int64_t most = (tiles + min_tiles - 1) / min_tiles;
+  const int64_t most = batch * ((tiles + min_tiles - 1) / min_tiles);
   return (int)(best > most ? (most < 1 ? 1 : most) : best);
 }
 
@@ -463,9 +463,9 @@ static PagedShape paged_grouped_shape(int64_t batch, int64_t s1, int64_t n1, int
   s.group_rows = mt * 16;
   s.row_groups = (int)((rows + s.group_rows - 1) / s.group_rows);
   s.groups = (int)n2 * s.row_groups;
-  s.min_tiles = 4;
-  s.workers = paged_workers((int64_t)device_cu_count() * 4 * pa_waves((int)d, mt), s.groups,
-                            batch * ((max_blocks * page + kPaTile - 1) / kPaTile), s.min_tiles);
+  s.min_tiles = kPaMinTiles;
+  s.workers = paged_workers((int64_t)device_cu_count() * 4 * pa_waves((int)d, mt), s.groups, batch,
+                            (max_blocks * page + kPaTile - 1) / kPaTile, s.min_tiles);
   return s;
 }
 

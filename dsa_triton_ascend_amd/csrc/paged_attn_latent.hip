@@ -59,6 +59,11 @@ __device__ __forceinline__ void pl_dma_glb(unsigned lds_base, const void* gaddr)
                  :: "s"(lds_base), "v"(gaddr) : "memory");
   else dma_glb16(lds_base, gaddr);
 }
+template <typename O>
+__device__ __forceinline__ O from_f32_as(float x) {
+  if constexpr (std::is_same<O, float>::value) return x;
+  else return Elem<O>::from_f32(x);
+}
 constexpr int kPlThreads = 512;
 constexpr int kPlPages = 512;  // block-table entries held in LDS
 
@@ -121,10 +126,10 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   if (worker >= p.workers) return;
   PagedPlan plan;
   plan.make(p, TILE, lane);
-  int64_t at = (int64_t)worker * plan.per;
-  const int64_t end = min(at + plan.per, plan.total);
-  if (at >= end) return;
-  int64_t before;
+  if (worker >= (plan.total + plan.per - 1) / plan.per) return;
+  int at = worker * plan.per;
+  const int end = min(at + plan.per, plan.total);
+  int before;
   int b = plan.find(p, TILE, lane, at, &before);
 
   // scores in log2 units are s * scale - ref, one operation each; for that
@@ -158,50 +163,65 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   using Off = std::integral_constant<bool, false>;
 
   bool first_segment = true;
+  // (what the plan keeps of the sequences does not stay in the registers
+  // through the tiles: later ones are read again)
+  b = __builtin_amdgcn_readfirstlane(b);
+  PagedSeq seq = plan.sequence(p, b);
   while (at < end) {
-    b = __builtin_amdgcn_readfirstlane(b);
-    // (where the output fills the registers, what the plan keeps of the
-    // sequences would not stay in them)
-    PagedSeq seq = HG == 128 ? paged_seq(p, b) : plan.sequence(p, b);
-    seq.lo = __builtin_amdgcn_readfirstlane(seq.lo);
-    seq.hi = __builtin_amdgcn_readfirstlane(seq.hi);
+    const int ln = fresh_lane(), li = ln & 15, lg = ln >> 4, tid = wave * 64 + ln;
     const int nt = paged_tiles(seq, TILE);
     if (nt == 0) {
-      ++b;
+      seq = paged_seq_uniform(p, ++b);
       continue;
     }
-    const int t0 = (int)(at - before), t1 = (int)min(end - before, (int64_t)nt);
+    const int t0 = at - before, t1 = min(end - before, nt);
     const int tok0 = seq.lo + t0 * TILE, tok1 = min(seq.hi, seq.lo + t1 * TILE);
     const int32_t* tab = p.table + (int64_t)b * p.max_blocks;
 
-    // rows of this lane's score columns: head rr % n1 of new token rr / n1
-    // (rows that do not exist read row 0; what they compute is not stored)
-    const int row = rg * HG + wave * 16 + li;
-    const bool live = scores && row < p.rows;
+    // the run's pages, as many as the LDS holds at a time, a thread's each
+    int ta = tok0, tb, pg0, page_entry;
+    auto read_pages = [&]() {
+      unsigned off0;
+      pg0 = (int)paged_split(p, (unsigned)ta, &off0);
+      tb = (int)min((int64_t)tok1, (int64_t)(pg0 + kPlPages) * p.page);
+      const int npg = (int)(((int64_t)tb - 1) / p.page) - pg0 + 1;
+      page_entry = tid < npg ? tab[pg0 + tid] : 0;
+    };
+    read_pages();
+
+    // rows of the wave's scores: head rr % n1 of new token rr / n1 (those
+    // that do not exist compute something, which is not stored).  Tokens that
+    // all of them see need no mask; a row's bounds rise with its token.
     int all_lo = 0, all_hi = 0x7fffffff;
+    const int first_row = rg * HG + wave * 16;
+    if (scores && first_row < p.rows) {
+      int l, h;
+      paged_bounds(p, seq.act_q, seq.act_k, min(first_row + 15, p.rows - 1) / p.n1, &all_lo, &h);
+      paged_bounds(p, seq.act_q, seq.act_k, first_row / p.n1, &l, &all_hi);
+      all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+      all_hi = __builtin_amdgcn_readfirstlane(min(all_hi, h));
+    }
     V8 qf[KQR];
+    u32x4 ql_in[QL ? QL : 1];
     {
-      const int64_t qrow = (int64_t)b * p.rows + (live ? row : 0);
+      // (bounds in the descriptors: rows that do not exist and waves without
+      // scores read zeros, without a branch around what then fills registers)
+      const int rows_here = scores ? min(p.rows - rg * HG, HG) : 0;
+      const int64_t row0 = (int64_t)b * p.rows + rg * HG;
+      const __amdgpu_buffer_rsrc_t q_src =
+          __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)p.q + row0 * D), (short)0, rows_here * D * 2, 0x00020000);
+      const __amdgpu_buffer_rsrc_t qr_src = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)((const T*)p.qr + row0 * DR), (short)0, rows_here * DR * 2, 0x00020000);
+      const int r = wave * 16 + li;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const T* src = ks < KSN ? (const T*)p.q + qrow * D + ks * 32 + lg * 8
-                                : (const T*)p.qr + qrow * DR + (ks - KSN) * 32 + lg * 8;
-        const u32x4 x = (*(const u32x4*)src & keep) ^ flip;
+        const u32x4 x = ks < KSN ? __builtin_amdgcn_raw_buffer_load_b128(q_src, r * (D * 2) + lg * 16 + ks * 64, 0, 0)
+                                 : __builtin_amdgcn_raw_buffer_load_b128(qr_src, r * (DR * 2) + lg * 16 + (ks - KSN) * 64, 0, 0);
         if (ks < KQR) qf[ks < KQR ? ks : 0] = as_v8<V8>(x);
-        else if constexpr (QL > 0)
-          *(u32x4*)(s_q + (((wave * 16 + li) * (QL * 64) + ((lg ^ nope_swz(li)) * 16)) ^ ((ks - KQR) << 6))) = x;
+        else ql_in[ks < KQR ? 0 : ks - KQR] = x;
       }
-      if (live) paged_bounds(p, seq.act_q, seq.act_k, row / p.n1, &all_lo, &all_hi);
+      __builtin_amdgcn_sched_barrier(0);  // all on their way before the first is waited for
     }
-    // tokens that all of the wave's rows see need no mask
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) {
-      all_lo = max(all_lo, __shfl_xor(all_lo, o));
-      all_hi = min(all_hi, __shfl_xor(all_hi, o));
-    }
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-
     f32x4 acc[NDW][HW];
 #pragma unroll
     for (int j = 0; j < NDW; ++j)
@@ -209,23 +229,28 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       for (int ht = 0; ht < HW; ++ht) acc[j][ht] = {0.f, 0.f, 0.f, 0.f};
     float ref = -INFINITY, top = -INFINITY, sum = 0.f, sum_p = 0.f;
 
-    for (int ta = tok0; ta < tok1;) {
-      // the run's pages, as many as the LDS holds at a time
-      unsigned off0;
-      const int pg0 = (int)paged_split(p, (unsigned)ta, &off0);
-      const int tb = (int)min((int64_t)tok1, (int64_t)(pg0 + kPlPages) * p.page);
-      const int npg = (int)(((int64_t)tb - 1) / p.page) - pg0 + 1;
-      lds_barrier();  // the pages, tiles and numerators of the stretch before are read
+    auto share_pages = [&]() {
+      lds_barrier();  // the pages, tiles and numerators before are read
       if (tid < 3) s_flag[tid] = 0;
-      for (int i = tid; i < npg; i += kPlThreads) s_tab[i] = tab[pg0 + i];
+      s_tab[tid] = page_entry;
       lds_barrier();
-      const int n_tiles = (tb - ta + TILE - 1) / TILE;
-      // Q's loads, on their way beside the table's, end here and not inside
-      // the tile loop, where a wait for them would be one for the tiles in
-      // flight too
+    };
+    share_pages();
+    // Q's loads, on their way beside the pages', end here and not inside the
+    // tile loop, where a wait for them would be one for the tiles in flight too
+    {
 #pragma unroll
-      for (int ks = 0; ks < KQR; ++ks) asm volatile("" : "+v"(qf[ks]));
+      for (int ks = 0; ks < KQR; ++ks) {
+        qf[ks] = as_v8<V8>((__builtin_bit_cast(u32x4, qf[ks]) & keep) ^ flip);
+        asm volatile("" : "+v"(qf[ks]));
+      }
+#pragma unroll
+      for (int i = 0; i < QL; ++i)
+        *(u32x4*)(s_q + (((wave * 16 + li) * (QL * 64) + ((lg ^ nope_swz(li)) * 16)) ^ (i << 6))) = (ql_in[i] & keep) ^ flip;
+    }
 
+    for (;;) {
+      const int n_tiles = (tb - ta + TILE - 1) / TILE;
       // cache row of token lane % 32 of tile t, -1 past the end or without a
       // page (both are read as zeros)
       auto tile_rows = [&](int t) -> int {
@@ -272,7 +297,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       };
 
       // ---- scores of a tile, with the DMAs of another between the MFMAs ----
-      f32x4 s[NTT];
+      f32x4 s[NTT] = {};  // (these are set to something so that they do not stay alive from run to run)
       V8 va[NDW];
       auto read_v = [&](int buf) {
         const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
@@ -282,7 +307,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
         for (int j = 0; j < NDW; ++j) va[j] = a2(g2b, wave * NDW + j);
       };
       auto gemm1 = [&](int kbuf, int krbuf, auto with_dma, int rows, int dbuf, int drbuf) {
-        constexpr int PF = QL ? 2 : 4;  // k-steps read ahead
+        constexpr int PF = QL ? 2 : HG <= 32 && KS >= 8 ? 8 : 4;  // k-steps read ahead
         const int ln = fresh_lane(), l = ln & 15, g = ln >> 4;
         const int g1b = nope_off(l, 0) + ((g ^ nope_swz(l)) * 16) + kbuf * 1024;
         const int g1rb = rope_off(l, 0) + ((g ^ rope_swz(l)) * 16) + krbuf * 1024;
@@ -317,8 +342,8 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
 
       // ---- softmax of the scores in eight stages, which go between the
       // groups of output MFMAs ----
-      float es, eps;
-      T4 ph[NTT], pl[NTT];
+      float es = 0.f, eps = 0.f;
+      T4 ph[NTT] = {}, pl[NTT] = {};
       auto stage = [&](int k, int t, int flag) {
         if (k == 0) {
           const int tk = ta + t * TILE;
@@ -465,10 +490,15 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       }
       wait_vmcnt<0>();  // of the DMAs past the end too: the ring is theirs until then
       ta = tb;
+      if (ta >= tok1) break;
+      read_pages();
+      share_pages();
     }
 
     // ---- the run's output ----
-    const int ln = fresh_lane(), li = ln & 15, lg = ln >> 4;
+    // (a scope of its own: the lane's numbers are made anew here)
+    [&](int ln) __attribute__((always_inline)) {
+    const int li = ln & 15, lg = ln >> 4;
     const bool whole = t0 == 0 && t1 == nt;
     const int64_t slot0 =
         (((int64_t)worker * 2 + (first_segment ? 0 : 1)) * p.groups + rg) * p.group_rows;
@@ -491,31 +521,49 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       }
     }
     lds_barrier();
-    const int col = wave * NDW * 16 + lg * 4;
-    if (whole) {
+    // By columns, as the waves hold it, the output would leave in pieces of
+    // 32 bytes (9 to 19 thousand cycles at 128 rows of 512): it goes through
+    // the ring, which is free by now, and leaves as whole rows, which follow
+    // each other in memory.
+    auto put = [&](auto zero, void* to, auto value) {
+      using O = decltype(zero);
+      typedef O O4 __attribute__((ext_vector_type(4)));
+      constexpr int RP = HG < 64 ? HG : 64;              // rows of a pass
+      constexpr int ROW = D * (int)sizeof(O), PITCH = ROW + 16;  // (16 rows' chunks lie in 64 different banks)
+      constexpr int CHUNKS = RP * ROW / 16;
+      static_assert(RP * PITCH <= (int)sizeof(smem), "output stage");
+      const int col = (wave * NDW * 16 + lg * 4) * (int)sizeof(O);
 #pragma unroll
-      for (int ht = 0; ht < HW; ++ht) {
-        const int r = rg * HG + ht * 16 + li;
-        const float n = s_n[ht * 16 + li];
-        const float inv = n > 0.f ? 1.f / n : 0.f;
-        if (r < p.rows) {
-          T* dst = (T*)p.out + ((int64_t)b * p.rows + r) * D + col;
+      for (int h0 = 0; h0 < HW; h0 += RP / 16) {
+        if (h0) lds_barrier();
+#pragma unroll
+        for (int h = 0; h < RP / 16; ++h)
 #pragma unroll
           for (int j = 0; j < NDW; ++j) {
-            const f32x4 x = acc[j][ht] * inv;
-            *(T4*)(dst + j * 16) = (T4){E::from_f32(x[0]), E::from_f32(x[1]), E::from_f32(x[2]), E::from_f32(x[3])};
+            const f32x4 x = value(h0 + h, j);
+            *(O4*)(smem + (h * 16 + li) * PITCH + col + j * 16 * (int)sizeof(O)) =
+                (O4){from_f32_as<O>(x[0]), from_f32_as<O>(x[1]), from_f32_as<O>(x[2]), from_f32_as<O>(x[3])};
           }
+        lds_barrier();
+        const int bytes = min(p.rows - rg * HG - h0 * 16, RP) * ROW;  // (not positive without rows)
+        unsigned char* const dst = (unsigned char*)to + h0 * 16 * ROW;
+#pragma unroll
+        for (int i = 0; i < (CHUNKS + kPlThreads - 1) / kPlThreads; ++i) {
+          const int c = i * kPlThreads + wave * 64 + ln;
+          if (c * 16 < bytes) *(u32x4*)(dst + c * 16) = *(const u32x4*)(smem + c * 16 / ROW * PITCH + c * 16 % ROW);
         }
       }
-    } else if constexpr (kLo) {
+    };
+    if (whole) {
+      float inv[HW];
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
-        if (rg * HG + ht * 16 + li < p.rows) {
-          float* dst = (float*)p.part_o + (slot0 + ht * 16 + li) * D + col;
-#pragma unroll
-          for (int j = 0; j < NDW; ++j) *(f32x4*)(dst + j * 16) = acc[j][ht];
-        }
+        const float n = s_n[ht * 16 + li];
+        inv[ht] = n > 0.f ? 1.f / n : 0.f;
       }
+      put(T{}, (T*)p.out + ((int64_t)b * p.rows + rg * HG) * D, [&](int ht, int j) { return acc[j][ht] * inv[ht]; });
+    } else if constexpr (kLo) {
+      put(0.f, (float*)p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht]; });
     } else {
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
@@ -528,6 +576,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
         if (lg == 0) atomicMax(s_am + ht * 16 + li, __float_as_int(a));  // (not negative: ordered as integers)
       }
       lds_barrier();
+      float mul[HW];
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
         const float n = s_n[ht * 16 + li], a = __int_as_float(s_am[ht * 16 + li]);
@@ -535,24 +584,18 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
         int ex = 0;
         if (a * inv > 0.f) (void)frexpf(a * inv, &ex);  // a / n < 2^ex
         ex = max(ex, -100);
-        const float mul = ldexpf(inv, -ex);
-        if (rg * HG + ht * 16 + li < p.rows) {
-          const int64_t slot = slot0 + ht * 16 + li;
-          if (wave == 0 && lg == 0) p.part_scale[slot] = ldexpf(1.f, ex);
-          f16* dst = (f16*)p.part_o + slot * D + col;
-#pragma unroll
-          for (int j = 0; j < NDW; ++j) {
-            const f32x4 x = acc[j][ht] * mul;
-            *(f16x4*)(dst + j * 16) = (f16x4){(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3]};
-          }
-        }
+        mul[ht] = ldexpf(inv, -ex);
+        if (wave == 0 && lg == 0 && rg * HG + ht * 16 + li < p.rows)
+          p.part_scale[slot0 + ht * 16 + li] = ldexpf(1.f, ex);
       }
+      put(f16{}, (f16*)p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht] * mul[ht]; });
     }
+    }(fresh_lane());
     first_segment = false;
     at = before + t1;
     if (t1 == nt) {
-      before += nt;
-      ++b;
+      at = before += plan.padded(nt);
+      if (at < end) seq = paged_seq_uniform(p, ++b);
     }
   }
 }
@@ -566,8 +609,8 @@ PagedShape paged_latent_shape(int64_t batch, int64_t s1, int64_t n1, int64_t d, 
   s.half_parts = s.group_rows > 32;  // as P is rounded once there
   s.row_groups = (int)((rows + s.group_rows - 1) / s.group_rows);
   s.groups = s.row_groups;
-  s.min_tiles = 8;
-  s.workers = paged_workers(device_cu_count(), s.groups, batch * ((max_blocks * page + s.tile - 1) / s.tile),
+  s.min_tiles = kPaMinTiles;
+  s.workers = paged_workers(device_cu_count(), s.groups, batch, (max_blocks * page + s.tile - 1) / s.tile,
                             s.min_tiles);
   return s;
 }
