@@ -140,17 +140,23 @@ class RotaryEmbeddingFunction(torch.autograd.Function):
         return _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_query, d_key):
         positions, inv_freq = ctx.saved_tensors
         interleaved, q_start, k_start, scale, inverse = ctx.args
         d_q = d_query if ctx.needs_input_grad[0] else None
         d_k = d_key if ctx.needs_input_grad[1] else None
+        if d_q is None and d_k is not None:
+            d_q, k_start, q_start = d_k, 0, k_start
+            d_k, swapped = None, True
+        else:
+            swapped = False
         if d_q is not None:
-            d_q, d_k = _rotate(d_q, d_k, positions, inv_freq, *ctx.args, False)
-        elif d_k is not None:
-            d_k, _ = _rotate(d_k, None, positions, inv_freq, interleaved, k_start, 0, scale, inverse, False)
-        return (d_q, d_k) + (None,) * 7
+            if torch.is_grad_enabled():  # the gradient of this one will be asked for
+                d_q, d_k = RotaryEmbeddingFunction.apply(d_q, d_k, positions, inv_freq, interleaved, q_start, k_start,
+                                                         scale, inverse)
+            else:
+                d_q, d_k = _rotate(d_q, d_k, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False)
+        return ((None, d_q) if swapped else (d_q, d_k)) + (None,) * 7
 
 
 __all__ = ["RotaryEmbeddingFunction", "SparseFlashAttentionFunction", "sparse_flash_attention_train",

@@ -142,7 +142,7 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     Returns ``(query_out, key_out)`` (key_out is None without a key), new
     contiguous tensors, or with ``inplace`` the inputs themselves.  Strided
     views are read as they are if a head's columns are next to each other.
-    Differentiable in query and key (not in place).
+    Differentiable in query and key, any number of times (not in place).
     """
     rank = _RANK.get(layout)
     if rank is None:

@@ -101,6 +101,26 @@ def test_gradient_against_differences():
         assert abs(left - right) <= 2 * 6 * 40 * 2 * 2 * 16 * 2.0 ** -20
 
 
+@pytest.mark.parametrize("sides", ["both", "query", "key"])
+def test_second_gradient(sides):
+    """<grad, h> as a function of the outputs' gradients d is <d, f(h)>: its gradient is f(h)."""
+    import dsa_triton_ascend_amd as dsa
+    g = torch.Generator(device="cuda").manual_seed(7)
+    q = torch.randn(2, 5, 3, 48, generator=g, device="cuda", requires_grad=sides != "key")
+    k = torch.randn(2, 5, 1, 32, generator=g, device="cuda", requires_grad=sides != "query")
+    pos = torch.arange(5, device="cuda") + 77
+    inv, _ = dsa.rotary_frequencies(16)
+    outs = dsa.rotary_embedding(q, k, pos, inv, rotary_offset=8, key_rotary_offset=16, attention_scale=0.5)
+    some = [i for i, t in enumerate((q, k)) if t.requires_grad]
+    d = [torch.randn(outs[i].shape, generator=g, device="cuda", requires_grad=True) for i in some]
+    h = [torch.randn(outs[i].shape, generator=g, device="cuda") for i in some]
+    first = torch.autograd.grad([outs[i] for i in some], [(q, k)[i] for i in some], d, create_graph=True)
+    second = torch.autograd.grad(first, d, h)
+    for i, got, x in zip(some, second, h):
+        want, mag = _turn(x, pos, inv, (8, 16)[i], False, 0.5)
+        _check(got, want, mag, torch.float32, sides)
+
+
 def test_only_one_side_differentiable():
     import dsa_triton_ascend_amd as dsa
     q = torch.randn(1, 3, 2, 32, device="cuda")
