@@ -75,6 +75,7 @@ __global__ __launch_bounds__(kPcThreads) void pc_write_kernel(PcWriteParams p) {
     if (lo == p.batch) return;  // rows behind the last sequence
     b = lo;
     s = (int)(t - (b ? p.rows[b - 1] : 0));
+    if (s < 0) return;  // (a count of -2^31 before it)
   } else {
     b = (int)(t / p.s);
     s = (int)(t - (int64_t)b * p.s);

@@ -285,3 +285,23 @@ def test_graph_replays():
         eager = step(mine)
         assert all(torch.equal(a, b) for a, b in zip(got, eager))
         assert all(torch.equal(a, b) for a, b in zip(caches, mine))
+
+
+def test_write_counts_that_do_not_rise():
+    """Whatever the cumulative counts are, what lies around the pages keeps its values."""
+    import dsa_triton_ascend_amd as dsa
+    pool = torch.full((6, 4, 1, 8), 7.0, device="cuda")
+    cache = pool[2:4]  # two pages, with two before and two behind them
+    table = torch.tensor([[0], [1], [1]], dtype=torch.int32, device="cuda")
+    lens = torch.zeros(3, dtype=torch.int32, device="cuda")
+    rows = torch.arange(6 * 8, device="cuda", dtype=torch.float32).view(6, 1, 8)
+    counts = torch.tensor([2, 30, 4], dtype=torch.int32, device="cuda")
+    dsa.paged_cache_write(cache, rows, table, lens, row_lengths=counts, layout="TND")
+    assert (pool[:2] == 7).all() and (pool[4:] == 7).all()
+    assert torch.equal(pool[2, :2], rows[:2]) and (pool[2, 2:] == 7).all()
+    assert torch.equal(pool[3], rows[2:6])
+    for counts in ([5, 1, 6], [-2 ** 31, 4, 6], [-1, -2 ** 31, 6]):
+        pool.fill_(7.0)
+        dsa.paged_cache_write(cache, rows, table, lens, layout="TND",
+                              row_lengths=torch.tensor(counts, dtype=torch.int32, device="cuda"))
+        assert (pool[:2] == 7).all() and (pool[4:] == 7).all()
