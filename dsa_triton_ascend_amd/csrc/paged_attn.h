@@ -71,6 +71,14 @@ struct PagedSeq {
   int act_q, act_k, lo, hi;  // lo <= t < hi: tokens that any row sees
 };
 
+// A row's output times the factor f, which is 0 where the row saw no token of
+// the run: then the output is 0 too, also where another row's value beside it
+// is not finite.
+__device__ __forceinline__ float paged_scaled(float x, float f) { return f == 0.f ? 0.f : x * f; }
+__device__ __forceinline__ f32x4 paged_scaled(f32x4 x, float f) {
+  return f == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : x * f;
+}
+
 // bounds of row s1
 __device__ __forceinline__ void paged_bounds(const PagedAttnParams& p, int act_q, int act_k, int s1, int* lo, int* hi) {
   const int64_t diag = p.mode == 0 ? (int64_t)s1 : (int64_t)act_k - act_q + s1;

@@ -230,10 +230,10 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const float l = xgroup_sum(sum[mt]);
+      const float inv = l != 0.f ? 1.f / l : 0.f;
       constexpr int EC = D == 64 ? 4 : 8;  // elements of a chunk
       if (whole) {
         if (orow[mt] >= 0) {
-          const float inv = l > 0.f ? 1.f / l : 0.f;
           typedef T TC __attribute__((ext_vector_type(EC)));
 #pragma unroll
           for (int c = 0; c < NJ / EC; ++c)
@@ -241,14 +241,14 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
             for (int r = 0; r < 4; ++r) {
               TC o;
 #pragma unroll
-              for (int e = 0; e < EC; ++e) o[e] = E::from_f32(acc[mt][c * EC + e][r] * inv);
+              for (int e = 0; e < EC; ++e) o[e] = E::from_f32(paged_scaled(acc[mt][c * EC + e][r], inv));
               *(TC*)((T*)p.out + orow[mt] * D + c * 128 + (lg * 4 + r) * EC) = o;
             }
           if (lg == 0 && p.smax) {
             // statistics are [B, N2, S1, G]
             const int rr = rg * p.group_rows + mt * 16 + li;
             const int64_t at2 = ((int64_t)b * p.n2 + kvh) * p.rows + rr;
-            const bool any = p.return_lse && l > 0.f;
+            const bool any = p.return_lse && l != 0.f;
             p.smax[at2] = any ? top[mt] * kLn2 : 0.f;
             p.ssum[at2] = any ? l * fast_exp2(ref[mt] - top[mt]) : 0.f;
           }
@@ -257,6 +257,7 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
         const int64_t slot = (((int64_t)worker * 2 + (first_segment ? 0 : 1)) * p.groups + ng) * p.group_rows +
                              mt * 16 + li;
         float* dst = (float*)p.part_o + slot * D;
+        const float seen = l != 0.f ? 1.f : 0.f;
 #pragma unroll
         for (int c = 0; c < NJ / EC; ++c)
 #pragma unroll
@@ -265,7 +266,7 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
             for (int e = 0; e < EC; e += 4) {
               const f32x4 o = {acc[mt][c * EC + e][r], acc[mt][c * EC + e + 1][r], acc[mt][c * EC + e + 2][r],
                                acc[mt][c * EC + e + 3][r]};
-              *(f32x4*)(dst + c * 128 + (lg * 4 + r) * EC + e) = o;
+              *(f32x4*)(dst + c * 128 + (lg * 4 + r) * EC + e) = paged_scaled(o, seen);
             }
         if (lg == 0) p.part_ml[slot] = {ref[mt], l, top[mt], l};
       }
@@ -363,14 +364,14 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, i
     const int kvh = row / p.rows, rr = row - kvh * p.rows;
     const int s = rr / p.group;
     const int64_t orow = ((int64_t)b * p.s1 + s) * p.n1 + kvh * p.group + (rr - s * p.group);
-    const float inv = n > 0.f ? 1.f / n : 0.f;
+    const float inv = n != 0.f ? 1.f / n : 0.f;
     TV r;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) r[e] = E::from_f32(o[e] * inv);
+    for (int e = 0; e < EPL; ++e) r[e] = E::from_f32(paged_scaled(o[e], inv));
     *(TV*)((T*)p.out + orow * D + lane * EPL) = r;
     if (lane == 0 && p.smax) {
       const int64_t srow = (int64_t)b * per_seq + row;
-      const bool any = p.return_lse && l > 0.f;
+      const bool any = p.return_lse && l != 0.f;
       p.smax[srow] = any ? top * kLn2 : 0.f;
       p.ssum[srow] = any ? l * fast_exp2(big - top) : 0.f;
     }

@@ -513,7 +513,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
             p.part_ml[slot0 + r] = {ref, l, top, n};
           } else if (p.smax) {
             const int64_t o = (int64_t)b * p.rows + rr;  // [B, 1, S1, N1], the order of the rows
-            const bool any = p.return_lse && l > 0.f;
+            const bool any = p.return_lse && l != 0.f;
             p.smax[o] = any ? top * kLn2 : 0.f;
             p.ssum[o] = any ? l * fast_exp2(ref - top) : 0.f;
           }
@@ -559,11 +559,14 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
         const float n = s_n[ht * 16 + li];
-        inv[ht] = n > 0.f ? 1.f / n : 0.f;
+        inv[ht] = n != 0.f ? 1.f / n : 0.f;
       }
-      put(T{}, (T*)p.out + ((int64_t)b * p.rows + rg * HG) * D, [&](int ht, int j) { return acc[j][ht] * inv[ht]; });
+      put(T{}, (T*)p.out + ((int64_t)b * p.rows + rg * HG) * D, [&](int ht, int j) { return paged_scaled(acc[j][ht], inv[ht]); });
     } else if constexpr (kLo) {
-      put(0.f, (float*)p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht]; });
+      float keep_row[HW];
+#pragma unroll
+      for (int ht = 0; ht < HW; ++ht) keep_row[ht] = s_n[ht * 16 + li] != 0.f ? 1.f : 0.f;
+      put(0.f, (float*)p.part_o + slot0 * D, [&](int ht, int j) { return paged_scaled(acc[j][ht], keep_row[ht]); });
     } else {
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
@@ -571,7 +574,10 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
 #pragma unroll
         for (int j = 0; j < NDW; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) a = fmaxf(a, fabsf(acc[j][ht][r]));
+          for (int r = 0; r < 4; ++r) {
+            const float y = fabsf(acc[j][ht][r]);
+            a = y < INFINITY ? fmaxf(a, y) : a;
+          }
         a = xgroup_max(a);
         if (lg == 0) atomicMax(s_am + ht * 16 + li, __float_as_int(a));  // (not negative: ordered as integers)
       }
@@ -580,7 +586,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
         const float n = s_n[ht * 16 + li], a = __int_as_float(s_am[ht * 16 + li]);
-        const float inv = n > 0.f ? 1.f / n : 0.f;
+        const float inv = n != 0.f ? 1.f / n : 0.f;
         int ex = 0;
         if (a * inv > 0.f) (void)frexpf(a * inv, &ex);  // a / n < 2^ex
         ex = max(ex, -100);
@@ -588,7 +594,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
         if (wave == 0 && lg == 0 && rg * HG + ht * 16 + li < p.rows)
           p.part_scale[slot0 + ht * 16 + li] = ldexpf(1.f, ex);
       }
-      put(f16{}, (f16*)p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht] * mul[ht]; });
+      put(f16{}, (f16*)p.part_o + slot0 * D, [&](int ht, int j) { return paged_scaled(acc[j][ht], mul[ht]); });
     }
     }(fresh_lane());
     first_segment = false;

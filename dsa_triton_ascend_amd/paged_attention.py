@@ -28,14 +28,17 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
     rope parts.  Latent form: ``value`` None, key [pages, page_size, 1, D], D
     in (128, 256, 512), query_rope [B, S1, N1, 64] and key_rope [pages,
     page_size, 1, 64].  ``block_table`` [B, max_blocks]; entries outside the
-    cache read as zero rows.  ``actual_seq_lengths_kv`` [B]: cached tokens, the
+    cache read as zero rows; all of it may name up to 2^35 tokens.  ``actual_seq_lengths_kv`` [B]: cached tokens, the
     new ones included.  ``actual_seq_lengths_query`` [B]: new tokens (S1 by
     default); later rows give zeros.
 
     sparse_mode 3: new token s1 sees the first act_kv - act_q + s1 + 1 tokens;
     0: all act_kv.  ``pre_tokens`` / ``next_tokens`` select a band around the
     diagonal, as in ``sparse_flash_attention`` (a sliding window of w tokens:
-    pre_tokens = w - 1); tokens outside every row's band are not read.
+    pre_tokens = w - 1); tokens outside every row's band are not read.  A value
+    that one new token of a sequence sees and another does not has weight zero
+    for the latter, so it must be finite there; rows that see no token are zero
+    whatever the values.
 
     Returns ``(attention_out, softmax_max, softmax_sum)``: the output in the
     query's shape and dtype, the statistics [B, N2, S1, N1 / N2] in float32,

@@ -60,8 +60,13 @@ def _check_caches(caches):
             raise ValueError(f"a cache must not be empty, got {tuple(shape)}")
         addresses.append(t.data_ptr())
         row_bytes.append(n // (pages * page) * t.element_size())
-    if len(set(addresses)) != len(addresses):
-        raise ValueError("the same cache is given twice")
+    if len(addresses) > 1:
+        spans = sorted(zip(addresses, row_bytes))
+        end = 0
+        for at, size in spans:
+            if at < end:
+                raise ValueError("the same cache is given twice, or two caches overlap")
+            end = at + size * pages * page
     return pages, page, addresses, row_bytes
 
 
@@ -89,7 +94,7 @@ def paged_cache_write(caches, rows, block_table, seq_lengths, row_lengths=None, 
 
     ``rows[i]`` [B, S, ...] (layout "BSND") or [T, ...] ("TND", packed) holds the new
     rows of ``caches[i]`` [pages, page_size, ...], of its dtype and trailing
-    sizes; batch and token strides are free.  The first new token of sequence b
+    sizes, outside the caches; batch and token strides are free.  The first new token of sequence b
     goes to position ``seq_lengths[b]`` (tokens before the call).
     ``row_lengths``: new tokens of each sequence (BSND; all S by default), or
     cumulative (TND, required).  Tokens that have no page (past the table, a -1

@@ -493,7 +493,8 @@ int dsa_paged_cache_compact(int64_t n_caches, void* const* caches, const int64_t
  * the table holds as that); actual_seq_q [B]: new tokens (NULL: S1), the rows
  * after them give zeros.  sparse_mode, pre_tokens and next_tokens as in
  * dsa_sfa_fwd (mode 3: new token s1 sees act_kv - act_q + s1 + 1 tokens).
- * Block-table entries outside the cache read as zero rows.  Writes
+ * Block-table entries outside the cache read as zero rows; the table may name
+ * up to 2^35 tokens in all.  Writes
  * attention_out [B, S1, N1, D] and, where given, softmax_max / softmax_sum
  * [B, N2, S1, N1 / N2] (zeros unless return_lse); rows that see nothing give
  * zeros.  Tensors are 16-byte aligned.  The workspace size depends on sizes

@@ -310,3 +310,17 @@ def test_workspace_sizes():
     assert lib.dsa_paged_cache_fork_workspace_size(2, 3, 8) == 4 * (2 + 6 + 8)
     assert lib.dsa_paged_cache_compact_workspace_size(0) == 0
     assert lib.dsa_paged_cache_compact_workspace_size(1025) == 4 * (2 + 3 * 1025)
+
+
+def test_tables_that_name_too_many_tokens_are_refused():
+    lib = _lib()
+    big = dict(b=1 << 11, blocks=1 << 20, page=32)  # 2^36
+    assert lib.dsa_paged_attn(*_c(ATTN, big)) == 2 and b"2^35" in lib.dsa_last_error()
+    assert lib.dsa_paged_attn_workspace_size(1 << 11, 1, 8, 2, 128, 0, 1 << 20, 32) == 0
+
+
+def test_caches_that_overlap_are_refused():
+    pool = torch.zeros(8, 4, 1, 8, dtype=BF)
+    rows = [torch.zeros(2, 3, 1, 8, dtype=BF)] * 2
+    with pytest.raises(ValueError, match="overlap"):
+        _write(caches=[pool[3:8], pool[0:5]], rows=rows)

@@ -399,3 +399,36 @@ def test_lengths_past_the_table_and_negative():
         args["actual_seq_lengths_kv"] = torch.tensor([2 ** 31 - 1, 64, -7], dtype=torch.int32, device="cuda")
         got = dsa.paged_attention(**args)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("N1,D,latent", [(16, 128, True), (64, 128, True), (8, 64, False)])
+@pytest.mark.parametrize("lens", [
+    [96] * 3,                                             # every sequence three tiles, runs of two
+    [1 + 37 * i % 211 for i in range(300)],               # more sequences than workgroups
+    [40] * 520,                                           # two of them in a run
+    [0] * 70 + [33] + [0] * 70 + [4000, 0, 1],            # long empty stretches
+    [2500] * 9,                                           # runs a little longer than an equal share
+])
+def test_runs_over_many_shapes_of_batches(N1, D, latent, lens):
+    args, data = _make(len(lens), 1, N1, 1 if latent else 2, D, 16, lens, torch.bfloat16, latent, seed=81)
+    _compare(args, data, lens)
+
+
+@pytest.mark.parametrize("latent,N1,D", [(False, 8, 64), (False, 4, 256), (True, 8, 512), (True, 16, 512),
+                                         (True, 128, 512), (True, 64, 128)])
+@pytest.mark.parametrize("n", [70, 3000])
+def test_rows_that_see_nothing_beside_values_that_are_not_finite(latent, N1, D, n):
+    """Padding rows are zero next to a token of infinities; a row that sees a NaN says so."""
+    import dsa_triton_ascend_amd as dsa
+    args, _ = _make(2, 3, N1, 1 if latent else 2, D, 64, [n, n], torch.bfloat16, latent, seed=83, act_q=[1, 2])
+    last = int(args["block_table"][0, (n - 1) // 64]), (n - 1) % 64
+    want = dsa.paged_attention(**args)
+    for value in (float("inf"), float("nan")):
+        args["key" if latent else "value"][last] = value
+        out, mx, sm = dsa.paged_attention(**args)
+        assert not torch.isfinite(out[0, 0]).any()
+        assert (out[0, 1:] == 0).all() and (mx[0, :, 1:] == 0).all() and (sm[0, :, 1:] == 0).all()
+        assert all(torch.equal(a[1], b[1]) for a, b in zip((out, mx, sm), want))  # the other sequence
+    args["key"][last] = float("nan")
+    out, mx, sm = dsa.paged_attention(**args)
+    assert torch.isnan(out[0, 0]).all() and torch.isnan(sm[0, :, 0]).all() and (out[0, 1:] == 0).all()
