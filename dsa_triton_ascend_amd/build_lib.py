@@ -1,4 +1,6 @@
-"""Build libdsa_hip.so (the C-ABI HIP library) in-tree for gfx950.
+"""Build libdsa_hip.so (the C-ABI HIP library) in-tree for gfx950, and
+_torch_calls.so, the host-only module by which torch reaches the operators of
+a decoding step without Python's cost per argument.
 
     python -m dsa_triton_ascend_amd.build_lib
 
@@ -15,6 +17,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(PKG, "libdsa_hip.so")
+CALLS_OUT = os.path.join(PKG, "_torch_calls.so")
 BUILD_DIR = os.path.join(ROOT, "_build")
 
 SOURCES = [
@@ -90,6 +93,29 @@ def _compile(src, extra):
     return src, obj, r.returncode, _filter(r.stdout + r.stderr), cmd
 
 
+def build_calls():
+    """Compile _torch_calls.so against the installed torch (no device code)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    includes = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(rocm, "include")]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = CALLS_OUT + ".tmp"
+    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+            "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+           + [x for i in includes for x in ("-isystem", i)]
+           + [os.path.join(CSRC, "torch_calls.cpp"), "-o", tmp, "-L" + lib, "-ltorch_python", "-ltorch_cpu",
+              "-lc10", "-lc10_hip"])
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for torch_calls.cpp:\n{' '.join(cmd)}\n{r.stdout + r.stderr}")
+    os.replace(tmp, CALLS_OUT)
+    return CALLS_OUT
+
+
 def build(verbose=False, jobs=None, extra_flags=()):
     os.makedirs(BUILD_DIR, exist_ok=True)
     jobs = jobs or min(8, len(SOURCES))
@@ -107,8 +133,9 @@ def build(verbose=False, jobs=None, extra_flags=()):
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{_filter(r.stdout + r.stderr)}")
     os.replace(tmp, OUT)
+    build_calls()
     if verbose:
-        print(f"built {OUT}")
+        print(f"built {OUT} and {CALLS_OUT}")
     return OUT
 
 

@@ -1,0 +1,422 @@
+// Short way from torch tensors into the C-ABI entry points of the paged
+// decoding operators.  A decoding step makes several such calls per layer,
+// and at its sizes the kernels take 5 us where the checks and conversions of
+// a call in Python take 10.
+//
+// Each function checks that its call is an ordinary one (plain tensors of the
+// documented shapes and types on the current GPU, nothing to convert, no
+// gradient wanted) and makes it; for anything else, an entry point that
+// refuses included, it returns None and the Python function goes its own way,
+// which converts what may be converted and raises the errors.
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <ATen/ATen.h>
+#include <c10/core/Allocator.h>
+#include <c10/core/GradMode.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
+
+#include <algorithm>
+#include <climits>
+#include <utility>
+#include <vector>
+
+#include "../../include/dsa_capi.h"
+
+namespace {
+
+struct Entries {
+  decltype(&dsa_rope) rope;
+  decltype(&dsa_paged_cache_write) write;
+  decltype(&dsa_paged_cache_fork_workspace_size) fork_bytes;
+  decltype(&dsa_paged_cache_fork) fork;
+  decltype(&dsa_paged_cache_compact_workspace_size) compact_bytes;
+  decltype(&dsa_paged_cache_compact) compact;
+  decltype(&dsa_paged_attn_workspace_size) attn_bytes;
+  decltype(&dsa_paged_attn) attn;
+} entry;
+
+// an entry point's status; other Python threads run meanwhile, since a launch
+// may wait for room in its queue
+template <typename F, typename... Args>
+bool launched(F f, Args... args) {
+  PyThreadState* state = PyEval_SaveThread();
+  const int status = f(args...);
+  PyEval_RestoreThread(state);
+  return status == DSA_OK;
+}
+
+constexpr int64_t kMaxCaches = 512;
+
+// A plain tensor of the GPU of the call (the first tensor's; index -1 before
+// it), else null.
+const at::Tensor* tensor(PyObject* o, int* index) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.is_conj() || t.is_neg()) return nullptr;
+  if (*index < 0) *index = (int)t.get_device();
+  return t.get_device() == *index ? &t : nullptr;
+}
+
+const at::Tensor* ints(PyObject* o, int* index, int64_t dim) {
+  const at::Tensor* t = tensor(o, index);
+  return t && t->scalar_type() == at::kInt && t->dim() == dim && t->numel() > 0 && t->is_contiguous() ? t : nullptr;
+}
+
+bool integer(PyObject* o, int64_t* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  int overflow = 0;
+  *v = PyLong_AsLongLongAndOverflow(o, &overflow);
+  return !overflow;
+}
+
+bool number(PyObject* o, double* v) {
+  if (PyFloat_CheckExact(o)) *v = PyFloat_AS_DOUBLE(o);
+  else if (PyLong_CheckExact(o)) *v = PyLong_AsDouble(o);
+  else return false;
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+
+bool flag(PyObject* o, bool* v) {
+  *v = o == Py_True;
+  return PyBool_Check(o);
+}
+
+// "BSND" 0, "TND" 1, else -1
+int layout(PyObject* o) {
+  if (!PyUnicode_CheckExact(o)) return -1;
+  if (PyUnicode_CompareWithASCIIString(o, "BSND") == 0) return 0;
+  return PyUnicode_CompareWithASCIIString(o, "TND") == 0 ? 1 : -1;
+}
+
+// items of a tensor, list or tuple
+bool items(PyObject* o, PyObject*** first, PyObject** self, int64_t* n) {
+  if (PyList_CheckExact(o) || PyTuple_CheckExact(o)) {
+    *n = PySequence_Fast_GET_SIZE(o);
+    *first = PySequence_Fast_ITEMS(o);
+    return *n <= kMaxCaches;
+  }
+  *self = o;
+  *first = self;
+  *n = 1;
+  return true;
+}
+
+struct Caches {
+  std::vector<const at::Tensor*> t;
+  std::vector<void*> at;
+  std::vector<int64_t> row_bytes;
+  int64_t pages = 0, page = 0;
+
+  bool read(PyObject* o, int* index) {
+    PyObject **list, *self;
+    int64_t n;
+    if (!items(o, &list, &self, &n)) return false;
+    t.reserve(n), at.reserve(n), row_bytes.reserve(n);
+    for (int64_t i = 0; i < n; ++i) {
+      const at::Tensor* c = tensor(list[i], index);
+      if (!c || c->dim() < 3 || !c->is_contiguous() || c->numel() == 0) return false;
+      if (i == 0) pages = c->size(0), page = c->size(1);
+      if (c->size(0) != pages || c->size(1) != page) return false;
+      t.push_back(c);
+      at.push_back(c->data_ptr());
+      row_bytes.push_back(c->numel() / (pages * page) * (int64_t)c->element_size());
+    }
+    std::vector<int64_t> order(n);
+    for (int64_t i = 0; i < n; ++i) order[i] = i;
+    std::sort(order.begin(), order.end(), [&](int64_t a, int64_t b) { return at[a] < at[b]; });
+    for (int64_t i = 1; i < n; ++i)
+      if ((char*)at[order[i - 1]] + row_bytes[order[i - 1]] * pages * page > (char*)at[order[i]]) return false;
+    return true;
+  }
+};
+
+bool current(int index) { return index >= 0 && c10::hip::current_device() == index; }
+void* stream_of(int index) { return c10::hip::getCurrentHIPStream((c10::DeviceIndex)index).stream(); }
+const int32_t* data(const at::Tensor* t) { return t ? (const int32_t*)t->data_ptr() : nullptr; }
+
+// (caches, rows, block_table, seq_lengths, row_lengths, layout) -> True
+PyObject* write(PyObject* const* a) {
+  const int tnd = layout(a[5]);
+  int index = -1;
+  Caches c;
+  if (tnd < 0 || !c.read(a[0], &index) || c.t.empty()) return nullptr;
+  const at::Tensor *table = ints(a[2], &index, 2), *lens = ints(a[3], &index, 1), *counts = nullptr;
+  if (!table || !lens || !current(index)) return nullptr;
+  const int64_t batch = table->size(0);
+  if (a[4] != Py_None && (!(counts = ints(a[4], &index, 1)) || counts->size(0) != batch)) return nullptr;
+  if (lens->size(0) != batch || (tnd && !counts)) return nullptr;
+  PyObject **list, *self;
+  int64_t n;
+  if (!items(a[1], &list, &self, &n) || n != (int64_t)c.t.size()) return nullptr;
+  const int64_t lead = tnd ? 1 : 2;
+  std::vector<const void*> src(n);
+  std::vector<int64_t> sb(n), st(n);
+  int64_t t0 = 0, t1 = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    const at::Tensor* r = tensor(list[i], &index);
+    const at::Tensor& k = *c.t[i];
+    if (!r || r->dim() != lead + k.dim() - 2 || r->scalar_type() != k.scalar_type()) return nullptr;
+    if (i == 0) t0 = r->size(0), t1 = tnd ? 1 : r->size(1);
+    if (r->size(0) != t0 || (!tnd && (r->size(1) != t1 || t0 != batch))) return nullptr;
+    int64_t step = 1;
+    for (int64_t d = r->dim() - 1; d >= lead; --d) {
+      if (r->size(d) != k.size(d - lead + 2) || (r->stride(d) != step && r->size(d) != 1)) return nullptr;
+      step *= r->size(d);
+    }
+    const int64_t es = (int64_t)r->element_size();
+    src[i] = r->data_ptr();
+    sb[i] = tnd ? 0 : r->stride(0) * es;
+    st[i] = r->stride(lead - 1) * es;
+  }
+  if (t0 * t1 == 0) return nullptr;
+  if (!launched(entry.write, n, src.data(), c.at.data(), c.row_bytes.data(), sb.data(), st.data(), data(table), data(lens),
+                  data(counts), batch, tnd ? 0 : t1, t0 * t1, table->size(1), c.pages, c.page,
+                  tnd ? DSA_LAYOUT_TND : DSA_LAYOUT_BSND, stream_of(index)))
+    return nullptr;
+  Py_RETURN_TRUE;
+}
+
+PyObject* triple(at::Tensor x, at::Tensor y, at::Tensor z) {
+  PyObject* r = PyTuple_New(3);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(x)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(y)));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(z)));
+  return r;
+}
+
+// memory of torch's allocator for a workspace: returned to it with the value,
+// in the order of the current stream
+c10::DataPtr workspace(size_t n) { return c10::GetAllocator(c10::kCUDA)->allocate(std::max<size_t>(n, 1)); }
+
+// (caches, block_table, seq_lengths, page_refs, parents, new_tokens, page_size) -> triple
+PyObject* fork(PyObject* const* a) {
+  int index = -1;
+  Caches c;
+  int64_t more, page;
+  if (!c.read(a[0], &index) || c.t.empty() || !integer(a[5], &more) || more < 0 || more > INT_MAX) return nullptr;
+  if (a[6] != Py_None && (!integer(a[6], &page) || page != c.page)) return nullptr;
+  const at::Tensor *table = ints(a[1], &index, 2), *lens = ints(a[2], &index, 1), *refs = ints(a[3], &index, 1);
+  const at::Tensor* parents = nullptr;
+  if (!table || !lens || !refs || !current(index)) return nullptr;
+  if (a[4] != Py_None && !(parents = ints(a[4], &index, 1))) return nullptr;
+  const int64_t rows = table->size(0), wide = table->size(1), children = parents ? parents->size(0) : rows;
+  if (lens->size(0) != rows || refs->size(0) != c.pages) return nullptr;
+  const auto kind = table->options();
+  at::Tensor new_table = at::empty({children, wide}, kind), new_lens = at::empty({children}, kind);
+  at::Tensor new_refs = at::empty({c.pages}, kind);
+  const size_t bytes = entry.fork_bytes(rows, children, c.pages);
+  c10::DataPtr ws = workspace(bytes);
+  if (!launched(entry.fork, (int64_t)c.t.size(), c.at.data(), c.row_bytes.data(), data(table), data(lens), data(refs),
+                 data(parents), (int32_t*)new_table.data_ptr(), (int32_t*)new_lens.data_ptr(),
+                 (int32_t*)new_refs.data_ptr(), rows, children, wide, wide, c.pages, c.page, more, ws.get(),
+                 bytes, stream_of(index)))
+    return nullptr;
+  return triple(std::move(new_table), std::move(new_lens), std::move(new_refs));
+}
+
+// (caches, block_table, page_refs, page_size) -> triple
+PyObject* compact(PyObject* const* a) {
+  int index = -1;
+  Caches c;
+  int64_t page;
+  if (!c.read(a[0], &index) || c.t.empty()) return nullptr;
+  if (a[3] != Py_None && (!integer(a[3], &page) || page != c.page)) return nullptr;
+  const at::Tensor *table = ints(a[1], &index, 2), *refs = ints(a[2], &index, 1);
+  if (!table || !refs || !current(index) || refs->size(0) != c.pages) return nullptr;
+  const auto kind = table->options();
+  at::Tensor new_table = at::empty(table->sizes(), kind), new_refs = at::empty({c.pages}, kind);
+  at::Tensor map = at::empty({c.pages}, kind);
+  const size_t bytes = entry.compact_bytes(c.pages);
+  c10::DataPtr ws = workspace(bytes);
+  if (!launched(entry.compact, (int64_t)c.t.size(), c.at.data(), c.row_bytes.data(), data(table), data(refs),
+                    (int32_t*)new_table.data_ptr(), (int32_t*)new_refs.data_ptr(), (int32_t*)map.data_ptr(),
+                    table->size(0), table->size(1), c.pages, c.page, ws.get(), bytes, stream_of(index)))
+    return nullptr;
+  return triple(std::move(new_table), std::move(new_refs), std::move(map));
+}
+
+// (query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
+// actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse) -> triple
+PyObject* attention(PyObject* const* a) {
+  int index = -1;
+  const at::Tensor *q = tensor(a[0], &index), *k = tensor(a[1], &index), *v = nullptr, *qr = nullptr, *kr = nullptr;
+  const at::Tensor *table = ints(a[3], &index, 2), *act_k = ints(a[4], &index, 1), *act_q = nullptr;
+  const bool latent = a[2] == Py_None;
+  double scale;
+  int64_t mode, pre, next;
+  bool lse;
+  if (!q || !k || !table || !act_k || !current(index) || q->dim() != 4 || k->dim() != 4) return nullptr;
+  if (!number(a[5], &scale) || !integer(a[9], &mode) || !integer(a[10], &pre) || !integer(a[11], &next) ||
+      !flag(a[12], &lse))
+    return nullptr;
+  const auto kind = q->scalar_type();
+  auto cache = [&](const at::Tensor* t) {
+    return t && t->scalar_type() == kind && t->is_contiguous() && t->numel() > 0 && !t->requires_grad();
+  };
+  if ((kind != at::kBFloat16 && kind != at::kHalf) || !cache(q) || !cache(k)) return nullptr;
+  const int64_t b = q->size(0), s1 = q->size(1), n1 = q->size(2), d = q->size(3);
+  const int64_t pages = k->size(0), page = k->size(1), n2 = k->size(2);
+  if (k->size(3) != d || n1 % n2 || table->size(0) < b || act_k->size(0) != b) return nullptr;
+  if (latent) {
+    qr = tensor(a[6], &index), kr = tensor(a[7], &index);
+    if (!cache(qr) || !cache(kr) || n2 != 1 || qr->sizes() != at::IntArrayRef({b, s1, n1, 64}) ||
+        kr->sizes() != at::IntArrayRef({pages, page, 1, 64}))
+      return nullptr;
+  } else {
+    v = tensor(a[2], &index);
+    if (!cache(v) || a[6] != Py_None || a[7] != Py_None || v->sizes() != k->sizes()) return nullptr;
+  }
+  if (a[8] != Py_None && (!(act_q = ints(a[8], &index, 1)) || act_q->size(0) != b)) return nullptr;
+  const int64_t wide = table->size(1);
+  const size_t bytes = entry.attn_bytes(b, s1, n1, n2, d, latent, wide, page);
+  if (!bytes) return nullptr;
+  const auto f32 = q->options().dtype(at::kFloat);
+  at::Tensor out = at::empty(q->sizes(), q->options()), mx = at::empty({b, n2, s1, n1 / n2}, f32);
+  at::Tensor sm = at::empty({b, n2, s1, n1 / n2}, f32);
+  c10::DataPtr ws = workspace(bytes);
+  if (!launched(entry.attn, q->data_ptr(), latent ? qr->data_ptr() : nullptr, k->data_ptr(), latent ? kr->data_ptr() : nullptr,
+                 latent ? nullptr : v->data_ptr(), out.data_ptr(), (float*)mx.data_ptr(), (float*)sm.data_ptr(),
+                 data(act_q), data(act_k), data(table), b, s1, n1, n2, d, latent ? 64 : 0, pages, page, wide,
+                 (int32_t)mode, pre, next, kind == at::kHalf ? DSA_DTYPE_FP16 : DSA_DTYPE_BF16, (float)scale, lse,
+                 ws.get(), bytes, stream_of(index)))
+    return nullptr;
+  return triple(std::move(out), std::move(mx), std::move(sm));
+}
+
+// whether two elements of a strided tensor may share an address
+bool overlaps_itself(const at::Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> d;  // stride, size
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) d.emplace_back(t.stride(i), t.size(i));
+  std::sort(d.begin(), d.end());
+  int64_t reach = 0;
+  for (const auto& x : d) {
+    if (x.first <= reach) return true;
+    reach += (x.second - 1) * x.first;
+  }
+  return false;
+}
+
+// (query, key, positions, inv_freq, interleaved, rotary_offset, key_rotary_offset, attention_scale, layout,
+// inverse, inplace) -> (query_out, key_out)
+PyObject* rotate(PyObject* const* a) {
+  const int tnd = layout(a[8]);
+  int index = -1;
+  const at::Tensor *q = tensor(a[0], &index), *k = nullptr, *pos = tensor(a[2], &index), *freq = tensor(a[3], &index);
+  if (tnd < 0 || !q || !pos || !freq || !current(index)) return nullptr;
+  if (a[1] != Py_None && !(k = tensor(a[1], &index))) return nullptr;
+  bool interleaved, inverse, inplace;
+  int64_t start[2] = {0, 0};
+  double scale;
+  if (!flag(a[4], &interleaved) || !integer(a[5], &start[0]) || !number(a[7], &scale) || !flag(a[9], &inverse) ||
+      !flag(a[10], &inplace))
+    return nullptr;
+  start[1] = start[0];
+  if (a[6] != Py_None && !integer(a[6], &start[1])) return nullptr;
+  const bool grad = c10::GradMode::is_enabled();
+  const int64_t rank = tnd ? 3 : 4, lead = rank - 2;
+  const auto kind = q->scalar_type();
+  const int dtype = kind == at::kBFloat16 ? DSA_DTYPE_BF16
+                    : kind == at::kHalf   ? DSA_DTYPE_FP16
+                    : kind == at::kFloat  ? DSA_DTYPE_FP32
+                                          : -1;
+  if (dtype < 0 || freq->scalar_type() != at::kDouble || freq->dim() != 1 || freq->size(0) < 1 ||
+      !freq->is_contiguous())
+    return nullptr;
+  if ((pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong) || !pos->is_contiguous()) return nullptr;
+  const int64_t rot = 2 * freq->size(0);
+  const at::Tensor* in[2] = {q, k};
+  at::Tensor out[2];
+  int64_t si[2][3] = {}, so[2][3] = {}, heads[2] = {}, cols[2] = {};
+  void *from[2] = {}, *to[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor* t = in[i];
+    if (!t) continue;
+    if (t->dim() != rank || t->scalar_type() != kind || (grad && t->requires_grad()) || t->numel() == 0) return nullptr;
+    for (int64_t j = 0; j < lead; ++j)
+      if (t->size(j) != q->size(j)) return nullptr;
+    cols[i] = t->size(rank - 1), heads[i] = t->size(lead);
+    if ((t->stride(rank - 1) != 1 && cols[i] != 1) || start[i] < 0 || start[i] > cols[i] - rot) return nullptr;
+    if (inplace && (t->stride(rank - 1) != 1 || t->is_inference() || overlaps_itself(*t))) return nullptr;
+    out[i] = inplace ? *t : at::empty(t->sizes(), t->options());
+    for (int64_t j = 0; j < lead + 1; ++j) {
+      si[i][j + tnd] = t->stride(j);
+      so[i][j + tnd] = out[i].stride(j);
+    }
+    from[i] = t->data_ptr(), to[i] = out[i].data_ptr();
+  }
+  if (inplace && from[0] == from[1]) return nullptr;
+  const int64_t b = tnd ? 1 : q->size(0), s = q->size(lead - 1);
+  const bool full = pos->dim() == lead && (tnd || pos->size(0) == b) && pos->size(lead - 1) == s;
+  const bool shared = !tnd && pos->dim() == 1 && pos->size(0) == s;
+  if (!full && !shared) return nullptr;
+  if (!launched(entry.rope, from[0], to[0], si[0][0], si[0][1], si[0][2], so[0][0], so[0][1], so[0][2], heads[0], cols[0],
+                 start[0], from[1], to[1], si[1][0], si[1][1], si[1][2], so[1][0], so[1][1], so[1][2], heads[1],
+                 cols[1], k ? start[1] : 0, pos->data_ptr(), pos->scalar_type() == at::kLong, full,
+                 (const double*)freq->data_ptr(), b, s, rot, interleaved, inverse, dtype, (float)scale,
+                 stream_of(index)))
+    return nullptr;
+  if (inplace)
+    for (auto& t : out)
+      if (t.defined()) t.unsafeGetTensorImpl()->bump_version();
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(out[0])));
+  if (!k) Py_INCREF(Py_None);
+  PyTuple_SET_ITEM(r, 1, k ? THPVariable_Wrap(std::move(out[1])) : Py_None);
+  return r;
+}
+
+// A call that is not an ordinary one, and one that torch refuses (no memory),
+// is left to the Python function.
+template <PyObject* (*F)(PyObject* const*), int N>
+PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  PyObject* r = nullptr;
+  if (n == N && entry.attn) {
+    try {
+      r = F(args);
+    } catch (...) {
+      r = nullptr;
+    }
+  }
+  if (r) return r;
+  if (PyErr_Occurred()) PyErr_Clear();
+  Py_RETURN_NONE;
+}
+
+// addresses of the entry points, in the order of Entries
+PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  constexpr int kEntries = sizeof(Entries) / sizeof(void*);
+  if (n != kEntries) {
+    PyErr_SetString(PyExc_TypeError, "one address per entry point expected");
+    return nullptr;
+  }
+  void* at[kEntries];
+  for (int i = 0; i < kEntries; ++i) {
+    at[i] = PyLong_AsVoidPtr(args[i]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  std::copy(at, at + kEntries, (void**)&entry);
+  Py_RETURN_NONE;
+}
+
+#define FAST(f) ((PyCFunction)(void (*)(void))(f))
+PyMethodDef methods[] = {
+    {"bind", FAST(bind), METH_FASTCALL, nullptr},
+    {"write", FAST((call<write, 6>)), METH_FASTCALL, nullptr},
+    {"fork", FAST((call<fork, 7>)), METH_FASTCALL, nullptr},
+    {"compact", FAST((call<compact, 4>)), METH_FASTCALL, nullptr},
+    {"attention", FAST((call<attention, 13>)), METH_FASTCALL, nullptr},
+    {"rotate", FAST((call<rotate, 11>)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, methods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__torch_calls() { return PyModule_Create(&module); }

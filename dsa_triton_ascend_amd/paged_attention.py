@@ -44,6 +44,11 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
     query's shape and dtype, the statistics [B, N2, S1, N1 / N2] in float32,
     zeros unless ``return_softmax_lse``.  Inference only.
     """
+    result = _lib.calls().attention(query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope,
+                                    key_rope, actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens,
+                                    return_softmax_lse)
+    if result is not None:
+        return result
     pre_tokens, next_tokens = _band_args(pre_tokens, next_tokens)
     if sparse_mode not in (0, 3):
         raise ValueError("Only sparse_mode 0 (full) / 3 (rightDownCausal) supported")

@@ -102,6 +102,8 @@ def paged_cache_write(caches, rows, block_table, seq_lengths, row_lengths=None, 
     that several sequences share is not to be written: fork first.  Returns
     None.
     """
+    if _lib.calls().write(caches, rows, block_table, seq_lengths, row_lengths, layout):
+        return
     caches, rows = _list(caches, "caches"), _list(rows, "rows")
     if len(caches) != len(rows) or not caches:
         raise ValueError(f"one tensor of rows per cache is needed, got {len(rows)} for {len(caches)}")
@@ -179,6 +181,9 @@ def paged_cache_fork(caches, block_table, seq_lengths, page_refs, parents=None, 
 
     Returns ``(block_table [C, max_blocks], seq_lengths [C], page_refs)``.
     """
+    state = _lib.calls().fork(caches, block_table, seq_lengths, page_refs, parents, new_tokens, page_size)
+    if state is not None:
+        return state
     caches = _list(caches, "caches")
     pages, page, addresses, sizes = _check_caches(caches)
     refs = _ints(page_refs, "page_refs", 1)
@@ -228,6 +233,9 @@ def paged_cache_compact(caches, block_table, page_refs, page_size=None):
     page_refs, page_map)``: the table and the counts for the new ids, and each
     old page's new id (-1: it was free).
     """
+    state = _lib.calls().compact(caches, block_table, page_refs, page_size)
+    if state is not None:
+        return state
     caches = _list(caches, "caches")
     pages, page, addresses, sizes = _check_caches(caches)
     refs = _ints(page_refs, "page_refs", 1)

@@ -107,6 +107,10 @@ _NO_KEY = (None, None) + (0,) * 9
 
 def _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, inplace):
     """Launch on checked arguments; returns the rotated query and key."""
+    result = _lib.calls().rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale,
+                                 "BSND" if query.dim() == 4 else "TND", inverse, inplace)
+    if result is not None:
+        return result
     query, q_out, q_args = _side(query, q_start, inplace)
     k_out, k_args = None, _NO_KEY
     if key is not None:
@@ -122,6 +126,8 @@ def _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scal
         _DTYPE[query.dtype], scale, _lib.raw_stream(index))
     if status:
         _lib.check(status, "dsa_rope")
+    if inplace:
+        torch.autograd.graph.increment_version([t for t in (q_out, k_out) if t is not None])
     return q_out, k_out
 
 
@@ -144,6 +150,10 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     views are read as they are if a head's columns are next to each other.
     Differentiable in query and key, any number of times (not in place).
     """
+    result = _lib.calls().rotate(query, key, positions, inv_freq, interleaved, rotary_offset, key_rotary_offset,
+                                 attention_scale, layout, inverse, inplace)
+    if result is not None:
+        return result
     rank = _RANK.get(layout)
     if rank is None:
         raise ValueError(f"layout must be BSND or TND, got {layout}")
@@ -193,10 +203,7 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     if grad:
         from .autograd import RotaryEmbeddingFunction
         return RotaryEmbeddingFunction.apply(query, key, *args)
-    out = _rotate(query, key, *args, inplace)
-    if inplace:
-        torch.autograd.graph.increment_version([t for t in out if t is not None])
-    return out
+    return _rotate(query, key, *args, inplace)
 
 
 class RotaryEmbedding(torch.nn.Module):

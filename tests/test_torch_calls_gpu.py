@@ -1,0 +1,185 @@
+"""Ordinary calls of the paged decoding operators by way of _torch_calls and
+by way of Python: the same results, bit for bit; what is not an ordinary call
+is left to Python."""
+import threading
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+I32 = torch.int32
+
+
+def _state(dtype=torch.bfloat16, heads=1, cols=64):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    caches = [torch.randn(9, 16, heads, c, generator=g, device="cuda").to(dtype) for c in (cols, 64)]
+    table = torch.tensor([[3, 1, -1], [5, 8, 0]], dtype=I32, device="cuda")
+    lens = torch.tensor([20, 40], dtype=I32, device="cuda")
+    refs = torch.zeros(9, dtype=I32, device="cuda")
+    refs[[3, 1, 5, 8, 0]] = 1
+    return caches, table, lens, refs
+
+
+def _both(monkeypatch, f):
+    """f() with and without the module; whether the module took it is in _taken."""
+    from dsa_triton_ascend_amd import _lib
+    assert _lib.calls() is not _lib._NoCalls
+    a = f()
+    monkeypatch.setattr(_lib, "_calls", _lib._NoCalls)
+    b = f()
+    monkeypatch.undo()
+    for x, y in zip(a, b):
+        assert (x is None) == (y is None)
+        if x is not None:
+            assert x.shape == y.shape and x.dtype == y.dtype and x.stride() == y.stride() and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("layout,key,shared", [("BSND", True, False), ("BSND", False, True), ("TND", True, False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rotary(monkeypatch, layout, key, shared, dtype):
+    import dsa_triton_ascend_amd as dsa
+    lead = (3, 5) if layout == "BSND" else (7,)
+    q = torch.randn(*lead, 6, 96, device="cuda").to(dtype)[..., :5, 16:]  # strided
+    k = torch.randn(*lead, 2, 64, device="cuda").to(dtype) if key else None
+    pos = torch.arange(5, device="cuda") + 9 if shared else torch.randint(0, 9999, lead, device="cuda", dtype=I32)
+    inv, _ = dsa.rotary_frequencies(32)
+    _both(monkeypatch, lambda: dsa.rotary_embedding(q, k, pos, inv, interleaved=key, rotary_offset=32,
+                                                    attention_scale=1.25, layout=layout, inverse=shared))
+
+    def in_place():
+        packed = torch.cat([q] * 2, -1)
+        x, y = packed[..., :80], None if k is None else k.clone()
+        return dsa.rotary_embedding(x, y, pos, inv, rotary_offset=32, layout=layout, inplace=True) + (packed,)
+
+    _both(monkeypatch, in_place)
+
+
+@pytest.mark.parametrize("layout", ["BSND", "TND"])
+def test_cache(monkeypatch, layout):
+    import dsa_triton_ascend_amd as dsa
+    caches, table, lens, refs = _state()
+    keep = [c.clone() for c in caches]
+    if layout == "BSND":
+        rows = [torch.randn(2, 4, 1, 64, device="cuda").bfloat16(), torch.randn(2, 4, 3, 64, device="cuda").bfloat16()[:, :, 1:2]]
+        counts = None
+    else:
+        rows = [torch.randn(9, 1, 64, device="cuda").bfloat16() for _ in range(2)]
+        counts = torch.tensor([3, 8], dtype=I32, device="cuda")
+
+    def write():
+        for c, x in zip(caches, keep):
+            c.copy_(x)
+        dsa.paged_cache_write(caches, rows, table, lens, row_lengths=counts, layout=layout)
+        return [c.clone() for c in caches]
+
+    def fork():
+        for c, x in zip(caches, keep):
+            c.copy_(x)
+        parents = torch.tensor([1, 0, 1], dtype=I32, device="cuda")
+        return (*dsa.paged_cache_fork(caches, table, lens, refs, parents, new_tokens=2), *[c.clone() for c in caches])
+
+    def compact():
+        for c, x in zip(caches, keep):
+            c.copy_(x)
+        return (*dsa.paged_cache_compact(caches, table, refs), *[c.clone() for c in caches])
+
+    for f in (write, fork, compact, lambda: dsa.paged_cache_fork(caches[0], table, lens, refs)):
+        _both(monkeypatch, f)
+
+
+@pytest.mark.parametrize("latent", [False, True])
+def test_attention(monkeypatch, latent):
+    import dsa_triton_ascend_amd as dsa
+    caches, table, lens, _ = _state(heads=1, cols=128 if latent else 64)
+    q = torch.randn(2, 2, 8, 128 if latent else 64, device="cuda").bfloat16()
+    qr = torch.randn(2, 2, 8, 64, device="cuda").bfloat16() if latent else None
+    new = torch.tensor([2, 1], dtype=I32, device="cuda")
+    table = table.clamp(min=0)
+    for lse in (True, False):
+        _both(monkeypatch, lambda: dsa.paged_attention(
+            q, caches[0], None if latent else caches[1], table, lens, scale_value=0.125, query_rope=qr,
+            key_rope=caches[1] if latent else None, actual_seq_lengths_query=new if lse else None, sparse_mode=3,
+            pre_tokens=30 if lse else 2 ** 63 - 1, return_softmax_lse=lse)[:3 if lse else 1])
+
+
+def test_what_is_taken_and_what_is_left():
+    from dsa_triton_ascend_amd import _lib, rotary_frequencies
+    c = _lib.calls()
+    caches, table, lens, refs = _state()
+    inv, _ = rotary_frequencies(32)
+    q = torch.randn(2, 3, 4, 64, device="cuda")
+    pos = torch.arange(3, device="cuda")
+    ok = (q, None, pos, inv, False, 0, None, 1.0, "BSND", False, False)
+    assert c.rotate(*ok) is not None
+    for i, x in ((0, q.double()), (0, q.cpu()), (0, q[:0]), (0, q.clone().requires_grad_()), (0, q.transpose(2, 3)),
+                 (2, pos.float()), (2, pos[:2]), (2, None), (3, inv.float()), (5, 40), (5, -1), (5, 2 ** 70), (5, 0.0),
+                 (7, "1"), (8, "SBND"), (9, 0), (1, q[:, :2]), (1, q.bfloat16())):
+        assert c.rotate(*ok[:i], x, *ok[i + 1:]) is None, (i, x)
+    with torch.no_grad():
+        assert c.rotate(q.clone().requires_grad_(), *ok[1:]) is not None
+    x = q.clone()
+    out, _ = c.rotate(x, *ok[1:10], True)
+    assert out is x and x._version == 1 and torch.equal(x, c.rotate(*ok)[0])
+    for t in (q[:, :1].expand(2, 3, 4, 64), q[..., ::2], q.clone().requires_grad_()):
+        assert c.rotate(t, None, pos, inv[:8].contiguous(), *ok[4:10], True) is None
+    assert c.rotate(x, x, *ok[2:10], True) is None
+    rows = [torch.randn(2, 4, 1, 64, device="cuda").bfloat16()] * 2
+    ok = (caches, rows, table, lens, None, "BSND")
+    assert c.write(*ok) is True
+    for i, x in ((0, caches[:1]), (0, [caches[0], caches[0]]), (0, [caches[0], caches[0][1:]]), (0, []),
+                 (0, [caches[0], caches[1].cpu()]), (1, rows[:1]), (1, [r.float() for r in rows]),
+                 (1, [r[:, :, :, ::2] for r in rows]), (1, [r[:1] for r in rows]), (1, [rows[0], rows[0][:, :2]]),
+                 (2, table.long()), (2, table[0]), (2, table.t()), (3, lens[:1]), (4, lens[:1]), (5, "TND"), (5, None),
+                 (0, None), (1, None)):
+        assert c.write(*ok[:i], x, *ok[i + 1:]) is None, (i, x)
+    ok = (caches, table, lens, refs, None, 1, None)
+    assert c.fork(*ok) is not None and c.fork(*ok[:6], 16) is not None
+    for i, x in ((0, []), (1, table.long()), (2, lens[:1]), (3, refs[:5]), (4, lens.long()), (5, -1), (5, 2 ** 31),
+                 (5, 1.0), (6, 8)):
+        assert c.fork(*ok[:i], x, *ok[i + 1:]) is None, (i, x)
+    ok = (caches, table, refs, None)
+    assert c.compact(*ok) is not None
+    for i, x in ((0, []), (1, table.long()), (2, refs[:5]), (3, 8)):
+        assert c.compact(*ok[:i], x, *ok[i + 1:]) is None, (i, x)
+    q = torch.randn(2, 1, 8, 64, device="cuda").bfloat16()
+    ok = (q, caches[0], caches[1], table, lens, 0.1, None, None, None, 3, 2 ** 63 - 1, 2 ** 63 - 1, False)
+    assert c.attention(*ok) is not None
+    for i, x in ((0, q.float()), (0, q[:, :, :3, :48]), (0, q[:, :, ::2]), (1, caches[0].half()), (1, caches[0][:, ::2]),
+                 (2, caches[1][:5]), (2, None), (3, table.long()), (3, table[:1]), (4, [20, 40]), (4, lens.long()),
+                 (5, None), (6, q), (8, lens[:1]), (9, 1), (9, True), (10, 2 ** 63), (11, None), (12, 1)):
+        assert c.attention(*ok[:i], x, *ok[i + 1:]) is None, (i, x)
+    assert c.attention(*ok[:12]) is None  # too few arguments
+    torch.cuda.synchronize()
+
+
+def test_two_threads_and_a_graph():
+    import dsa_triton_ascend_amd as dsa
+    caches, table, lens, _ = _state()
+    q = torch.randn(2, 1, 8, 64, device="cuda").bfloat16()
+    table = table.clamp(min=0)
+    want = dsa.paged_attention(q, caches[0], caches[1], table, lens)[0]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                out = dsa.paged_attention(q, caches[0], caches[1], table, lens)[0]
+                if not torch.equal(out, want):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = dsa.paged_attention(q, caches[0], caches[1], table, lens)[0]
+    for scale in (1.0, 0.5, 2.0):
+        q.mul_(scale)
+        graph.replay()
+        eager = dsa.paged_attention(q, caches[0], caches[1], table, lens)[0]
+        assert torch.equal(out, eager)
