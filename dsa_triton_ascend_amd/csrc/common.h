@@ -90,6 +90,19 @@ __device__ __forceinline__ float relu_bits(float x) { return __int_as_float(max(
 // Hardware exp2 (v_exp_f32); callers keep arguments <= 0 or -inf.
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// inclusive sum over the lanes of a wave (in registers: six exchanges by LDS
+// take half a microsecond)
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15: lane 15's to 16.., 47's to 48..
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: lane 31's to 32..
+  return v;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
 // Butterfly max/sum across the four 16-lane groups that share lane%16, on
 // the VALU lane-swap instructions of gfx950: v_permlane16_swap with both
 // operands v returns (v[l], v[l ^ 16]) on every lane and v_permlane32_swap

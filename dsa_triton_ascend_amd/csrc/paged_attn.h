@@ -110,19 +110,6 @@ __device__ __forceinline__ PagedSeq paged_seq_uniform(const PagedAttnParams& p, 
 
 __device__ __forceinline__ int paged_tiles(const PagedSeq& s, int tile) { return (s.hi - s.lo + tile - 1) / tile; }
 
-// inclusive sum over the lanes of a wave (in registers: six exchanges by LDS
-// take half a microsecond)
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15: lane 15's to 16.., 47's to 48..
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: lane 31's to 32..
-  return v;
-}
-__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
-
 // The tiles of all sequences end to end, as a wave sees them (every lane
 // gets the same results); the tiles of a sequence are counted as a multiple
 // of `grain`, what is behind its last tile is nobody's work.  grain is the

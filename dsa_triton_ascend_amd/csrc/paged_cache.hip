@@ -81,17 +81,21 @@ __global__ __launch_bounds__(kPcThreads) void pc_write_kernel(PcWriteParams p) {
     s = (int)(t - (int64_t)b * p.s);
     if (p.rows && s >= p.rows[b]) return;
   }
-  const int64_t pos = (int64_t)max(p.lens[b], 0) + s;
-  const int64_t slot = pos / p.page;
-  if (slot >= p.max_blocks) return;
-  const int blk = p.table[(int64_t)b * p.max_blocks + slot];
-  if (blk < 0 || blk >= p.pages) return;
+  const unsigned pos = (unsigned)max(p.lens[b], 0) + (unsigned)s;  // both are below 2^31
+  const unsigned slot = pos / (unsigned)p.page;
   int ci = 0;
   while (ci + 1 < p.n && u >= p.c[ci + 1].unit0) ++ci;
   const PcCache& c = p.c[ci];
   const int64_t off = (int64_t)(u - c.unit0) << c.shift;
-  const unsigned char* src = p.tnd ? c.src + t * c.src_st : c.src + b * c.src_sb + s * c.src_st;
-  pc_move(c.dst + blk * c.page_bytes + (pos - slot * p.page) * c.row_bytes + off, src + off, c.shift);
+  const unsigned char* src = (p.tnd ? c.src + t * c.src_st : c.src + b * c.src_sb + s * c.src_st) + off;
+  // (the row is read beside the table, not behind it)
+  const u32x4 wide = c.shift == 4 ? *(const u32x4*)src : u32x4{0, 0, 0, 0};
+  if (slot >= (unsigned)p.max_blocks) return;
+  const int blk = p.table[(int64_t)b * p.max_blocks + slot];
+  if (blk < 0 || blk >= p.pages) return;
+  unsigned char* dst = c.dst + blk * c.page_bytes + (int64_t)(pos - slot * (unsigned)p.page) * c.row_bytes + off;
+  if (c.shift == 4) *(u32x4*)dst = wide;
+  else pc_move(dst, src, c.shift);
 }
 
 int pc_write_run(int64_t n, const void* const* rows, void* const* caches, const int64_t* row_bytes,
@@ -191,12 +195,7 @@ static int64_t pc_copy_set(PcCopySet& s, int64_t c0, int64_t n, void* const* cac
 template <int W>
 __device__ __forceinline__ int pc_block_scan(int v, int* s_part, int* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
+  const int x = wave_scan(v);
   __syncthreads();  // s_part of the scan before is read
   if (lane == 63) s_part[wave] = x;
   __syncthreads();
@@ -237,9 +236,10 @@ __device__ __forceinline__ PcChild pc_child(const PcForkParams& p, int c) {
   // a length past the table's end is the table's end
   const int64_t room = (int64_t)p.max_blocks * p.page;
   k.len = (int)min((int64_t)max(p.lens[k.parent], 0), room);
-  k.held = (int)(((int64_t)k.len + p.page - 1) / p.page);
-  const int64_t w = ((int64_t)k.len + p.new_tokens + p.page - 1) / p.page;
-  k.want = (int)min(w, (int64_t)0x7fffffff);
+  // (below 2^26 tokens, 2^31 new ones, 2^20 of a page: the sums fit 32 bits)
+  const unsigned page = (unsigned)p.page;
+  k.held = (int)(((unsigned)k.len + page - 1) / page);
+  k.want = (int)(((unsigned)k.len + (unsigned)p.new_tokens + page - 1) / page);
   return k;
 }
 
@@ -325,7 +325,8 @@ __global__ __launch_bounds__(kPcThreads) void pc_fork_kernel(PcForkParams p) {
       if (e >= 0 && e < p.pages) atomicSub(p.new_refs + e, 1);
     }
     for (int64_t i = me; i < (int64_t)p.children * p.new_blocks; i += stride) {
-      const int c = (int)(i / p.new_blocks), col = (int)(i - (int64_t)c * p.new_blocks);
+      const int c = i >> 32 ? (int)(i / p.new_blocks) : (int)((unsigned)i / (unsigned)p.new_blocks);
+      const int col = (int)(i - (int64_t)c * p.new_blocks);
       const PcChild k = pc_child(p, c);
       const bool served = k.parent >= 0 && p.flags[c];
       int e = -1;
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(kPcThreads) void pc_fork_kernel(PcForkParams p) {
     return;
   }
   const int64_t w = (int64_t)blockIdx.x - p.table_blocks;
-  const int c = (int)(w / p.set.chunks);
+  const int c = (int)((unsigned)w / (unsigned)p.set.chunks);  // (the grid is below 2^31)
   const PcChild k = pc_child(p, c);
   const int src = pc_copied_page(p, k, c);
   if (src < 0 || !p.flags[c]) return;
