@@ -8,7 +8,9 @@
 // per key head.  So every wave works alone, on its own run of tokens of one
 // key head, with no LDS and no barrier; what it needs in flight sits in
 // registers.  Neighbouring waves take neighbouring key heads of the same
-// tokens, so that the rows of a page are read whole.
+// tokens, so that the rows of a page are read whole.  32 x 32K tokens of eight
+// key heads of 128 columns, 4.3 GB: 650 us, 6.6 TB/s (a streaming read alone:
+// 7.1); the join behind it takes 6 us.
 //
 // Per tile of 32 tokens: K goes straight into the A operand of 16x16x32
 // (lane l: token l % 16, 16 bytes of 8 columns).  V is read a row at a time

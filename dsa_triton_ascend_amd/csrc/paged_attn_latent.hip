@@ -3,35 +3,43 @@
 //
 //   S^T = K Q^T,  P = 2^(S - ref),  O^T = V^T P^T,  V = K[:, :D]
 //
-// At 128 heads a token is 242 flops per byte, so bytes, matrix rate and LDS
-// reads are all near their limits; below that the bytes are.  A token is
-// read from memory once per workgroup and serves both products and every
-// row (head, new token) of the workgroup.
+// A token of 576 columns is 1152 bytes and 2176 flops a row.  Up to 32 rows
+// the bytes bound it (16 heads, 32 x 32K tokens, 1.2 GB: 191 us, 6.3 TB/s in
+// all and 7.4 TB/s between 16K and 32K); at 64 rows bytes and LDS reads are
+// near each other (231 us); at 128 it is the LDS reads: 416 KB a tile of 32
+// tokens (288 of them K, which each of eight waves reads for its 16 rows),
+// 3250 of a tile's 5400 cycles, beside 2180 of MFMAs (346 us, 0.84 PFLOP/s,
+// 40 % of the matrix pipes' cycles at the 2.05 GHz that the card holds).
 //
-// One workgroup of eight waves per CU owns a run of tokens for HG rows.
-//  * Tiles of 32 tokens come by LDS-DMA into a ring, chunks swizzled so that
-//    both products read them without bank conflicts.
-//  * S^T: a wave takes 16 rows and all 32 tokens (HG = 128) or 16 of them.
-//    Its Q stays in registers.
+// One workgroup of eight waves per CU owns a run of tokens for HG rows; a
+// token is read from memory once and serves both products and every row
+// (head, new token) of the workgroup.
+//  * Tiles of 32 tokens come by LDS-DMA into a ring of four (of three at 128
+//    rows of 512 columns), 16-byte chunks swizzled so that both products read
+//    them without bank conflicts.  Up to 64 rows the four waves without scores
+//    fetch; at 128 all do, a DMA between every few score MFMAs.
+//  * S^T: wave w < HG / 16 takes 16 rows and all 32 tokens, so a row's softmax
+//    stays in one wave.  Its Q stays in registers, but for four k-steps at 128
+//    rows of 512 columns, where the output takes half of the registers.
 //  * P goes through LDS, 64 bytes per row: token 16 tt + 4 g + r in slot
 //    8 g + 4 tt + r, chunk g at g ^ (row / 4 % 4).
 //  * O^T: a wave owns D / 8 columns of all HG rows, so each V^T fragment is
-//    read by one wave and serves all rows.
-//  * The scores of tile t + 1 are computed in the same stretch as the output
-//    of tile t, so that a SIMD's two waves can be in different products: one
-//    barrier per tile with two P buffers; at 128 rows of 512 columns, where the
-//    LDS holds one, the numerators wait in registers for a second barrier.
-// The references (paged_attn.h) are looked at once per tile: a wave that
-// sees a score too far above its row's raises a flag, and behind the barrier
-// everyone takes the slow way for that tile (exchange of the maxima, new
-// numerators, rescaled output).  That happens on a run's first tile and
-// seldom after it.
+//    read by one wave (transposed on its way out of the LDS) and serves all
+//    rows.
+//  * A step computes the scores of tile t + 1, then the output of tile t with
+//    the softmax of tile t + 1 between its MFMAs; P has two buffers and a step
+//    one barrier.
+// A row's reference (paged_attn.h) is moved by the wave that owns the row: it
+// leaves the factor in LDS and raises its bit of the tile's flags, and every
+// wave scales that row's output before it multiplies the tile.  That happens on
+// a run's first tile and seldom after it.
 //
-// Up to 32 rows P is multiplied as a sum of two values of the input type.
-// With more the second product costs time (64 rows: 1.6 instead of 1.1 us of
-// MFMAs and LDS reads per tile), so P is rounded once there, and the output is divided by the sum of the rounded
-// values: the weights still add up to one, and what is left is the rounding
-// of single weights, below the rounding of the output.
+// Up to 32 rows P is multiplied as a sum of two values of the input type,
+// which is free where the bytes bound.  With more rows the MFMAs and LDS reads
+// of the second value are not, so P is rounded once there, and the output is
+// divided by the sum of the rounded values: the weights still add up to one,
+// and what is left is the rounding of single weights, below the rounding of
+// the output.
 #include "paged_attn.h"
 #include "sfa_fwd.h"
 
@@ -522,7 +530,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     }
     lds_barrier();
     // By columns, as the waves hold it, the output would leave in pieces of
-    // 32 bytes (9 to 19 thousand cycles at 128 rows of 512): it goes through
+    // 32 bytes (9 to 19 thousand cycles at 128 rows of 512; a tile is 5): it goes through
     // the ring, which is free by now, and leaves as whole rows, which follow
     // each other in memory.
     auto put = [&](auto zero, void* to, auto value) {
