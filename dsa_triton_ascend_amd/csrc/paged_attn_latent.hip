@@ -67,11 +67,6 @@ __device__ __forceinline__ void pl_dma_glb(unsigned lds_base, const void* gaddr)
                  :: "s"(lds_base), "v"(gaddr) : "memory");
   else dma_glb16(lds_base, gaddr);
 }
-template <typename O>
-__device__ __forceinline__ O from_f32_as(float x) {
-  if constexpr (std::is_same<O, float>::value) return x;
-  else return Elem<O>::from_f32(x);
-}
 constexpr int kPlThreads = 512;
 constexpr int kPlPages = 512;  // block-table entries held in LDS
 
@@ -192,7 +187,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       unsigned off0;
       pg0 = (int)paged_split(p, (unsigned)ta, &off0);
       tb = (int)min((int64_t)tok1, (int64_t)(pg0 + kPlPages) * p.page);
-      const int npg = (int)(((int64_t)tb - 1) / p.page) - pg0 + 1;
+      const int npg = (int)paged_split(p, (unsigned)tb - 1u, &off0) - pg0 + 1;
       page_entry = tid < npg ? tab[pg0 + tid] : 0;
     };
     read_pages();
@@ -204,8 +199,10 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     const int first_row = rg * HG + wave * 16;
     if (scores && first_row < p.rows) {
       int l, h;
-      paged_bounds(p, seq.act_q, seq.act_k, min(first_row + 15, p.rows - 1) / p.n1, &all_lo, &h);
-      paged_bounds(p, seq.act_q, seq.act_k, first_row / p.n1, &l, &all_hi);
+      const int s_first = p.s1 == 1 ? 0 : first_row / p.n1;
+      const int s_last = p.s1 == 1 ? 0 : min(first_row + 15, p.rows - 1) / p.n1;
+      paged_bounds(p, seq.act_q, seq.act_k, s_last, &all_lo, &h);
+      paged_bounds(p, seq.act_q, seq.act_k, s_first, &l, &all_hi);
       all_lo = __builtin_amdgcn_readfirstlane(all_lo);
       all_hi = __builtin_amdgcn_readfirstlane(min(all_hi, h));
     }
@@ -550,7 +547,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
           for (int j = 0; j < NDW; ++j) {
             const f32x4 x = value(h0 + h, j);
             *(O4*)(smem + (h * 16 + li) * PITCH + col + j * 16 * (int)sizeof(O)) =
-                (O4){from_f32_as<O>(x[0]), from_f32_as<O>(x[1]), from_f32_as<O>(x[2]), from_f32_as<O>(x[3])};
+                __builtin_convertvector(x, O4);
           }
         lds_barrier();
         const int bytes = min(p.rows - rg * HG - h0 * 16, RP) * ROW;  // (not positive without rows)
@@ -562,30 +559,52 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
         }
       }
     };
+    // rows that saw no token of the run: their output is zero, also where
+    // another row's value beside it was not finite
+    float n_row[HW];
+    bool none = false;
+#pragma unroll
+    for (int ht = 0; ht < HW; ++ht) {
+      n_row[ht] = s_n[ht * 16 + li];
+      none |= n_row[ht] == 0.f;
+    }
+    if (__any(none)) {
+#pragma unroll
+      for (int ht = 0; ht < HW; ++ht)
+#pragma unroll
+        for (int j = 0; j < NDW; ++j)
+          if (n_row[ht] == 0.f) acc[j][ht] = {0.f, 0.f, 0.f, 0.f};
+    }
     if (whole) {
       float inv[HW];
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
-        const float n = s_n[ht * 16 + li];
-        inv[ht] = n != 0.f ? 1.f / n : 0.f;
+        inv[ht] = n_row[ht] != 0.f ? 1.f / n_row[ht] : 0.f;
       }
-      put(T{}, (T*)p.out + ((int64_t)b * p.rows + rg * HG) * D, [&](int ht, int j) { return paged_scaled(acc[j][ht], inv[ht]); });
+      put(T{}, (T*)p.out + ((int64_t)b * p.rows + rg * HG) * D, [&](int ht, int j) { return acc[j][ht] * inv[ht]; });
     } else if constexpr (kLo) {
-      float keep_row[HW];
-#pragma unroll
-      for (int ht = 0; ht < HW; ++ht) keep_row[ht] = s_n[ht * 16 + li] != 0.f ? 1.f : 0.f;
-      put(0.f, (float*)p.part_o + slot0 * D, [&](int ht, int j) { return paged_scaled(acc[j][ht], keep_row[ht]); });
+      put(0.f, (float*)p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht]; });
     } else {
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
-        float a = 0.f;
+        // (magnitudes as integers, which are ordered alike and need no
+        // canonical form; infinities and NaN, above all others, do not count)
+        unsigned m = 0;
 #pragma unroll
         for (int j = 0; j < NDW; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float y = fabsf(acc[j][ht][r]);
-            a = y < INFINITY ? fmaxf(a, y) : a;
-          }
+          for (int r = 0; r < 4; ++r) m = max(m, __float_as_uint(acc[j][ht][r]) & 0x7fffffffu);
+        if (__any(m >= 0x7f800000u)) {
+          m = 0;
+#pragma unroll
+          for (int j = 0; j < NDW; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const unsigned y = __float_as_uint(acc[j][ht][r]) & 0x7fffffffu;
+              m = y < 0x7f800000u ? max(m, y) : m;
+            }
+        }
+        float a = __uint_as_float(m);
         a = xgroup_max(a);
         if (lg == 0) atomicMax(s_am + ht * 16 + li, __float_as_int(a));  // (not negative: ordered as integers)
       }
@@ -593,8 +612,8 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       float mul[HW];
 #pragma unroll
       for (int ht = 0; ht < HW; ++ht) {
-        const float n = s_n[ht * 16 + li], a = __int_as_float(s_am[ht * 16 + li]);
-        const float inv = n != 0.f ? 1.f / n : 0.f;
+        const float a = __int_as_float(s_am[ht * 16 + li]);
+        const float inv = n_row[ht] != 0.f ? 1.f / n_row[ht] : 0.f;
         int ex = 0;
         if (a * inv > 0.f) (void)frexpf(a * inv, &ex);  // a / n < 2^ex
         ex = max(ex, -100);
@@ -602,7 +621,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
         if (wave == 0 && lg == 0 && rg * HG + ht * 16 + li < p.rows)
           p.part_scale[slot0 + ht * 16 + li] = ldexpf(1.f, ex);
       }
-      put(f16{}, (f16*)p.part_o + slot0 * D, [&](int ht, int j) { return paged_scaled(acc[j][ht], mul[ht]); });
+      put(f16{}, (f16*)p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht] * mul[ht]; });
     }
     }(fresh_lane());
     first_segment = false;
