@@ -209,9 +209,8 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     V8 qf[KQR];
     u32x4 ql_in[QL ? QL : 1];
     {
-      // (bounds in the descriptors: rows that do not exist and waves without
-      // scores read zeros, without a branch around what then fills registers)
-      const int rows_here = scores ? min(p.rows - rg * HG, HG) : 0;
+      // (bounds in the descriptors: rows that do not exist read zeros)
+      const int rows_here = min(p.rows - rg * HG, HG);
       const int64_t row0 = (int64_t)b * p.rows + rg * HG;
       const __amdgpu_buffer_rsrc_t q_src =
           __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)p.q + row0 * D), (short)0, rows_here * D * 2, 0x00020000);
@@ -220,8 +219,13 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       const int r = wave * 16 + li;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 x = ks < KSN ? __builtin_amdgcn_raw_buffer_load_b128(q_src, r * (D * 2) + lg * 16 + ks * 64, 0, 0)
-                                 : __builtin_amdgcn_raw_buffer_load_b128(qr_src, r * (DR * 2) + lg * 16 + (ks - KSN) * 64, 0, 0);
+        // (the empty asm gives waves without scores something in these registers:
+        // left undefined, they cost 60 spilled ones)
+        u32x4 x;
+        asm volatile("" : "=v"(x));
+        if (NL == NW || scores)
+          x = ks < KSN ? __builtin_amdgcn_raw_buffer_load_b128(q_src, r * (D * 2) + lg * 16 + ks * 64, 0, 0)
+                       : __builtin_amdgcn_raw_buffer_load_b128(qr_src, r * (DR * 2) + lg * 16 + (ks - KSN) * 64, 0, 0);
         if (ks < KQR) qf[ks < KQR ? ks : 0] = as_v8<V8>(x);
         else ql_in[ks < KQR ? 0 : ks - KQR] = x;
       }
