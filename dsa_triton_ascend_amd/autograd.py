@@ -128,7 +128,8 @@ def sparse_lightning_indexer_kl_loss(query_index, key_index, weights, query, key
 
 
 class RotaryEmbeddingFunction(torch.autograd.Function):
-    """Differentiable rotary positions of a query and an optional key: a
+    """Differentiable rotary positions of a query and an optional key, for
+    calls that ``_torch_calls`` leaves to Python (it has the same node): a
     rotation's gradient is the rotation by the opposite angles, with the same
     scale, so nothing of the forward but the positions is kept."""
 

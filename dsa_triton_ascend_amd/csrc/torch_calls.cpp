@@ -4,11 +4,16 @@
 // a call in Python take 10.
 //
 // Each function checks that its call is an ordinary one (plain tensors of the
-// documented shapes and types on the current GPU, nothing to convert, no
-// gradient wanted) and makes it; for anything else, an entry point that
+// documented shapes and types on the current GPU, nothing to convert) and makes it; for anything else, an entry point that
 // refuses included, it returns None and the Python function goes its own way,
 // which converts what may be converted and raises the errors.
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/Allocator.h>
@@ -40,6 +45,7 @@ struct Entries {
 // may wait for room in its queue
 template <typename F, typename... Args>
 bool launched(F f, Args... args) {
+  if (!PyGILState_Check()) return f(args...) == DSA_OK;  // (a thread of the autograd engine)
   PyThreadState* state = PyEval_SaveThread();
   const int status = f(args...);
   PyEval_RestoreThread(state);
@@ -303,6 +309,115 @@ bool overlaps_itself(const at::Tensor& t) {
   return false;
 }
 
+struct Rotation {
+  int64_t start[2];  // of the query's and the key's rotated columns
+  double scale;
+  bool tnd, interleaved, inverse;
+};
+
+// Rotates in[0] and, if defined, in[1] into out; false if the call is not an
+// ordinary one.
+bool rotated(const Rotation& r, const at::Tensor in[2], const at::Tensor& pos, const at::Tensor& freq, bool inplace,
+             at::Tensor out[2]) {
+  const at::Tensor& q = in[0];
+  const int64_t rank = r.tnd ? 3 : 4, lead = rank - 2;
+  const auto kind = q.scalar_type();
+  const int dtype = kind == at::kBFloat16 ? DSA_DTYPE_BF16
+                    : kind == at::kHalf   ? DSA_DTYPE_FP16
+                    : kind == at::kFloat  ? DSA_DTYPE_FP32
+                                          : -1;
+  if (dtype < 0 || freq.scalar_type() != at::kDouble || freq.dim() != 1 || freq.size(0) < 1 || !freq.is_contiguous())
+    return false;
+  if ((pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong) || !pos.is_contiguous()) return false;
+  const int64_t rot = 2 * freq.size(0);
+  int64_t si[2][3] = {}, so[2][3] = {}, heads[2] = {}, cols[2] = {};
+  void *from[2] = {}, *to[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor& t = in[i];
+    if (!t.defined()) continue;
+    if (t.dim() != rank || t.scalar_type() != kind || t.numel() == 0) return false;
+    for (int64_t j = 0; j < lead; ++j)
+      if (t.size(j) != q.size(j)) return false;
+    cols[i] = t.size(rank - 1), heads[i] = t.size(lead);
+    if ((t.stride(rank - 1) != 1 && cols[i] != 1) || r.start[i] < 0 || r.start[i] > cols[i] - rot) return false;
+    if (inplace && (t.stride(rank - 1) != 1 || t.is_inference() || overlaps_itself(t))) return false;
+    out[i] = inplace ? t : at::empty(t.sizes(), t.options());
+    for (int64_t j = 0; j < lead + 1; ++j) {
+      si[i][j + r.tnd] = t.stride(j);
+      so[i][j + r.tnd] = out[i].stride(j);
+    }
+    from[i] = t.data_ptr(), to[i] = out[i].data_ptr();
+  }
+  if (inplace && from[0] == from[1]) return false;
+  const int64_t b = r.tnd ? 1 : q.size(0), s = q.size(lead - 1);
+  const bool full = pos.dim() == lead && (r.tnd || pos.size(0) == b) && pos.size(lead - 1) == s;
+  const bool shared = !r.tnd && pos.dim() == 1 && pos.size(0) == s;
+  if (!full && !shared) return false;
+  return launched(entry.rope, from[0], to[0], si[0][0], si[0][1], si[0][2], so[0][0], so[0][1], so[0][2], heads[0],
+                  cols[0], r.start[0], from[1], to[1], si[1][0], si[1][1], si[1][2], so[1][0], so[1][1], so[1][2],
+                  heads[1], cols[1], in[1].defined() ? r.start[1] : 0, pos.data_ptr(), pos.scalar_type() == at::kLong,
+                  full, (const double*)freq.data_ptr(), b, s, rot, r.interleaved, r.inverse, dtype, (float)r.scale,
+                  stream_of((int)q.get_device()));
+}
+
+bool rotated_with_gradient(const Rotation& r, const at::Tensor in[2], const at::Tensor& pos, const at::Tensor& freq,
+                           at::Tensor out[2]);
+
+// The gradient of a rotation is the rotation by the opposite angles, with the
+// same scale; nothing of the forward but the positions is kept.
+struct RotaryBackward : torch::autograd::Node {
+  Rotation r;
+  torch::autograd::SavedVariable pos, freq;
+
+  std::string name() const override { return "RotaryEmbeddingBackward"; }
+
+  void release_variables() override {
+    pos.reset_data();
+    freq.reset_data();
+  }
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const at::Tensor p = pos.unpack(), f = freq.unpack();
+    const size_t n = num_outputs();
+    at::Tensor in[2], out[2];
+    int place[2];  // whose gradient in[i] is
+    int count = 0;
+    Rotation back = r;
+    back.inverse = !r.inverse;
+    for (int i = 0; i < (int)n; ++i)
+      if (grads[i].defined() && task_should_compute_output(i)) {
+        in[count] = grads[i].stride(-1) == 1 ? grads[i] : grads[i].contiguous();
+        back.start[count] = r.start[i];
+        place[count++] = i;
+      }
+    torch::autograd::variable_list result(n);
+    if (!count) return result;
+    const bool ok = c10::GradMode::is_enabled() ? rotated_with_gradient(back, in, p, f, out)
+                                                : rotated(back, in, p, f, false, out);
+    TORCH_CHECK(ok, "the backward of rotary_embedding could not be launched");
+    for (int i = 0; i < count; ++i) result[place[i]] = out[i];
+    return result;
+  }
+};
+
+bool rotated_with_gradient(const Rotation& r, const at::Tensor in[2], const at::Tensor& pos, const at::Tensor& freq,
+                           at::Tensor out[2]) {
+  {
+    c10::AutoGradMode off(false);
+    if (!rotated(r, in, pos, freq, false, out)) return false;
+  }
+  const bool two = in[1].defined();
+  if (!in[0].requires_grad() && !(two && in[1].requires_grad())) return true;
+  std::shared_ptr<RotaryBackward> node(new RotaryBackward(), torch::autograd::deleteNode);
+  node->r = r;
+  node->pos = torch::autograd::SavedVariable(pos, false);
+  node->freq = torch::autograd::SavedVariable(freq, false);
+  node->set_next_edges(two ? torch::autograd::collect_next_edges(in[0], in[1])
+                           : torch::autograd::collect_next_edges(in[0]));
+  for (int i = 0; i < 1 + two; ++i) torch::autograd::set_history(out[i], node);
+  return true;
+}
+
 // (query, key, positions, inv_freq, interleaved, rotary_offset, key_rotary_offset, attention_scale, layout,
 // inverse, inplace) -> (query_out, key_out)
 PyObject* rotate(PyObject* const* a) {
@@ -311,66 +426,29 @@ PyObject* rotate(PyObject* const* a) {
   const at::Tensor *q = tensor(a[0], &index), *k = nullptr, *pos = tensor(a[2], &index), *freq = tensor(a[3], &index);
   if (tnd < 0 || !q || !pos || !freq || !current(index)) return nullptr;
   if (a[1] != Py_None && !(k = tensor(a[1], &index))) return nullptr;
-  bool interleaved, inverse, inplace;
-  int64_t start[2] = {0, 0};
-  double scale;
-  if (!flag(a[4], &interleaved) || !integer(a[5], &start[0]) || !number(a[7], &scale) || !flag(a[9], &inverse) ||
-      !flag(a[10], &inplace))
+  Rotation r;
+  bool inplace;
+  r.tnd = tnd;
+  if (!flag(a[4], &r.interleaved) || !integer(a[5], &r.start[0]) || !number(a[7], &r.scale) ||
+      !flag(a[9], &r.inverse) || !flag(a[10], &inplace))
     return nullptr;
-  start[1] = start[0];
-  if (a[6] != Py_None && !integer(a[6], &start[1])) return nullptr;
-  const bool grad = c10::GradMode::is_enabled();
-  const int64_t rank = tnd ? 3 : 4, lead = rank - 2;
-  const auto kind = q->scalar_type();
-  const int dtype = kind == at::kBFloat16 ? DSA_DTYPE_BF16
-                    : kind == at::kHalf   ? DSA_DTYPE_FP16
-                    : kind == at::kFloat  ? DSA_DTYPE_FP32
-                                          : -1;
-  if (dtype < 0 || freq->scalar_type() != at::kDouble || freq->dim() != 1 || freq->size(0) < 1 ||
-      !freq->is_contiguous())
-    return nullptr;
-  if ((pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong) || !pos->is_contiguous()) return nullptr;
-  const int64_t rot = 2 * freq->size(0);
-  const at::Tensor* in[2] = {q, k};
+  r.start[1] = r.start[0];
+  if (a[6] != Py_None && !integer(a[6], &r.start[1])) return nullptr;
+  const bool grad = c10::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()));
+  if (grad && (inplace || pos->requires_grad() || freq->requires_grad())) return nullptr;
+  const at::Tensor in[2] = {*q, k ? *k : at::Tensor()};
   at::Tensor out[2];
-  int64_t si[2][3] = {}, so[2][3] = {}, heads[2] = {}, cols[2] = {};
-  void *from[2] = {}, *to[2] = {};
-  for (int i = 0; i < 2; ++i) {
-    const at::Tensor* t = in[i];
-    if (!t) continue;
-    if (t->dim() != rank || t->scalar_type() != kind || (grad && t->requires_grad()) || t->numel() == 0) return nullptr;
-    for (int64_t j = 0; j < lead; ++j)
-      if (t->size(j) != q->size(j)) return nullptr;
-    cols[i] = t->size(rank - 1), heads[i] = t->size(lead);
-    if ((t->stride(rank - 1) != 1 && cols[i] != 1) || start[i] < 0 || start[i] > cols[i] - rot) return nullptr;
-    if (inplace && (t->stride(rank - 1) != 1 || t->is_inference() || overlaps_itself(*t))) return nullptr;
-    out[i] = inplace ? *t : at::empty(t->sizes(), t->options());
-    for (int64_t j = 0; j < lead + 1; ++j) {
-      si[i][j + tnd] = t->stride(j);
-      so[i][j + tnd] = out[i].stride(j);
-    }
-    from[i] = t->data_ptr(), to[i] = out[i].data_ptr();
-  }
-  if (inplace && from[0] == from[1]) return nullptr;
-  const int64_t b = tnd ? 1 : q->size(0), s = q->size(lead - 1);
-  const bool full = pos->dim() == lead && (tnd || pos->size(0) == b) && pos->size(lead - 1) == s;
-  const bool shared = !tnd && pos->dim() == 1 && pos->size(0) == s;
-  if (!full && !shared) return nullptr;
-  if (!launched(entry.rope, from[0], to[0], si[0][0], si[0][1], si[0][2], so[0][0], so[0][1], so[0][2], heads[0], cols[0],
-                 start[0], from[1], to[1], si[1][0], si[1][1], si[1][2], so[1][0], so[1][1], so[1][2], heads[1],
-                 cols[1], k ? start[1] : 0, pos->data_ptr(), pos->scalar_type() == at::kLong, full,
-                 (const double*)freq->data_ptr(), b, s, rot, interleaved, inverse, dtype, (float)scale,
-                 stream_of(index)))
+  if (grad ? !rotated_with_gradient(r, in, *pos, *freq, out) : !rotated(r, in, *pos, *freq, inplace, out))
     return nullptr;
   if (inplace)
     for (auto& t : out)
       if (t.defined()) t.unsafeGetTensorImpl()->bump_version();
-  PyObject* r = PyTuple_New(2);
-  if (!r) return nullptr;
-  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(out[0])));
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out[0])));
   if (!k) Py_INCREF(Py_None);
-  PyTuple_SET_ITEM(r, 1, k ? THPVariable_Wrap(std::move(out[1])) : Py_None);
-  return r;
+  PyTuple_SET_ITEM(pair, 1, k ? THPVariable_Wrap(std::move(out[1])) : Py_None);
+  return pair;
 }
 
 // A call that is not an ordinary one, and one that torch refuses (no memory),
@@ -381,6 +459,11 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n == N && entry.attn) {
     try {
       r = F(args);
+    } catch (python_error& e) {
+      // raised by Python code on the way (a hook on saved tensors, which
+      // checkpoints stop their recomputation by): the caller's
+      e.restore();
+      return nullptr;
     } catch (...) {
       r = nullptr;
     }

@@ -55,6 +55,70 @@ def test_rotary(monkeypatch, layout, key, shared, dtype):
     _both(monkeypatch, in_place)
 
 
+@pytest.mark.parametrize("sides", ["both", "query", "key", "query alone"])
+@pytest.mark.parametrize("how", ["dense", "strided", "broadcast", "missing"])
+def test_rotary_gradients(monkeypatch, sides, how):
+    import dsa_triton_ascend_amd as dsa
+    pos = torch.randint(0, 9999, (2, 5), device="cuda")
+    inv, _ = dsa.rotary_frequencies(32)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    base = [torch.randn(2, 5, n, 64, generator=g, device="cuda") for n in (4, 2)]
+    up = [torch.randn(2, 5, n, 64, generator=g, device="cuda") for n in (4, 2)]
+    if how == "strided":
+        up = [x.transpose(2, 3).contiguous().transpose(2, 3) for x in up]  # columns apart
+    elif how == "broadcast":
+        up = [x[:, :1, :, :1].expand_as(x) for x in up]
+
+    def run():
+        q, k = (x.clone().requires_grad_(sides != other) for x, other in zip(base, ("key", "query")))
+        out = dsa.rotary_embedding(q, None if sides == "query alone" else k, pos, inv, rotary_offset=16,
+                                   key_rotary_offset=32, attention_scale=0.75)
+        outs = [t for t in out if t is not None]
+        assert all(t.requires_grad for t in outs)
+        keep = slice(0, 1) if how == "missing" else slice(None)
+        leaves = [t for t in (q, k) if t.requires_grad and not (t is k and sides == "query alone")]
+        return torch.autograd.grad(outs[keep], leaves, up[:len(outs)][keep], allow_unused=how == "missing")
+
+    _both(monkeypatch, run)
+
+
+def test_rotary_gradients_in_a_graph_on_a_stream_and_after_a_change():
+    import dsa_triton_ascend_amd as dsa
+    q = torch.randn(2, 5, 4, 64, device="cuda", requires_grad=True)
+    pos = torch.arange(5, device="cuda")
+    inv, _ = dsa.rotary_frequencies(64)
+    up = torch.randn_like(q)
+
+    def step():
+        out, _ = dsa.rotary_embedding(q, None, pos, inv)
+        return out, torch.autograd.grad(out, q, up)[0]
+
+    assert dsa.rotary_embedding(q, None, pos, inv)[0].grad_fn.name() == "RotaryEmbeddingBackward"
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = step()
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for scale in (1.0, 2.0, 0.25):
+        up.mul_(scale)
+        with torch.no_grad():
+            q.mul_(scale)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+    out, _ = dsa.rotary_embedding(q, None, pos, inv)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    from torch.utils.checkpoint import checkpoint
+    pos.sub_(1)
+    checkpoint(lambda x: dsa.rotary_embedding(x, None, pos, inv)[0] * 2, q, use_reentrant=False).backward(up)
+    assert torch.equal(q.grad, torch.autograd.grad(dsa.rotary_embedding(q, None, pos, inv)[0] * 2, q, up)[0])
+
+
 @pytest.mark.parametrize("layout", ["BSND", "TND"])
 def test_cache(monkeypatch, layout):
     import dsa_triton_ascend_amd as dsa
@@ -112,7 +176,7 @@ def test_what_is_taken_and_what_is_left():
     pos = torch.arange(3, device="cuda")
     ok = (q, None, pos, inv, False, 0, None, 1.0, "BSND", False, False)
     assert c.rotate(*ok) is not None
-    for i, x in ((0, q.double()), (0, q.cpu()), (0, q[:0]), (0, q.clone().requires_grad_()), (0, q.transpose(2, 3)),
+    for i, x in ((0, q.double()), (0, q.cpu()), (0, q[:0]), (0, q.transpose(2, 3)),
                  (2, pos.float()), (2, pos[:2]), (2, None), (3, inv.float()), (5, 40), (5, -1), (5, 2 ** 70), (5, 0.0),
                  (7, "1"), (8, "SBND"), (9, 0), (1, q[:, :2]), (1, q.bfloat16())):
         assert c.rotate(*ok[:i], x, *ok[i + 1:]) is None, (i, x)
