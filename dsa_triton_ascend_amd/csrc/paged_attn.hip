@@ -76,7 +76,8 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
   while (at < end) {
     const int nt = paged_tiles(seq, kPaTile);
     if (nt == 0) {
-      seq = paged_seq_uniform(p, ++b);
+      if (++b >= p.batch) break;
+      seq = paged_seq_uniform(p, b);
       continue;
     }
     const int t0 = at - before, t1 = min(end - before, nt);

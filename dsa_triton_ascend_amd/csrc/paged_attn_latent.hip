@@ -174,7 +174,8 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     const int ln = fresh_lane(), li = ln & 15, lg = ln >> 4, tid = wave * 64 + ln;
     const int nt = paged_tiles(seq, TILE);
     if (nt == 0) {
-      seq = paged_seq_uniform(p, ++b);
+      if (++b >= p.batch) break;
+      seq = paged_seq_uniform(p, b);
       continue;
     }
     const int t0 = at - before, t1 = min(end - before, nt);

@@ -242,7 +242,7 @@ __device__ __forceinline__ PcChild pc_child(const PcForkParams& p, int c) {
   // (below 2^26 tokens, 2^31 new ones, 2^20 of a page: the sums fit 32 bits)
   const unsigned page = (unsigned)p.page;
   k.held = (int)(((unsigned)k.len + page - 1) / page);
-  k.want = (int)(((unsigned)k.len + (unsigned)p.new_tokens + page - 1) / page);
+  k.want = (int)min(((unsigned)k.len + (unsigned)p.new_tokens + page - 1) / page, 0x7fffffffu);
   return k;
 }
 

@@ -305,3 +305,15 @@ def test_write_counts_that_do_not_rise():
         dsa.paged_cache_write(cache, rows, table, lens, layout="TND",
                               row_lengths=torch.tensor(counts, dtype=torch.int32, device="cuda"))
         assert (pool[:2] == 7).all() and (pool[4:] == 7).all()
+
+
+@pytest.mark.parametrize("page", [1, 16])
+def test_fork_for_more_tokens_than_any_table_holds(page):
+    import dsa_triton_ascend_amd as dsa
+    cache = torch.zeros(8, page, 1, 8, device="cuda")
+    table = torch.tensor([[2, 5], [-1, -1]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([2, 0], dtype=torch.int32, device="cuda")
+    refs = torch.zeros(8, dtype=torch.int32, device="cuda")
+    refs[2] = refs[5] = 1
+    new_table, new_lens, new_refs = dsa.paged_cache_fork(cache, table, lens, refs, new_tokens=2 ** 31 - 1)
+    assert (new_table == -1).all() and (new_lens == -1).all() and (new_refs == 0).all()
