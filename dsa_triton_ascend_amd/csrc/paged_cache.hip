@@ -11,7 +11,7 @@
 // are handed out in ascending order to rows in ascending order, integer
 // counts are the only atomics, so results do not depend on timing.
 //
-// Bound by the launches for one step's tables (a fork of 16 rows: 4.5 + 5.2 us
+// Bound by the launches for one step's tables (a fork of 16 rows: 3.8 + 4.8 us
 // for its two kernels, a write of 32 rows 3.9, of 8192 rows 8.4), by memory
 // where pages move (half of a 740 MB pool in use: 369 MB read and written in
 // 76.5 us, 4.8 TB/s; a large copy reaches 4.9).
@@ -220,7 +220,7 @@ struct PcForkParams {
   PcCopySet set;
   const int32_t *table, *lens, *refs, *parents;  // parents null: row c continues row c
   int32_t *new_table, *new_lens, *new_refs;
-  int32_t *first, *start, *flags, *freelist;     // workspace
+  int32_t *first, *start, *flags, *freelist;     // workspace (first: for more rows than kPcRowsHere)
   int64_t pages, new_tokens;
   int rows, children, max_blocks, new_blocks, page;
   int table_blocks;                              // blocks of the tables in the second launch
@@ -249,13 +249,14 @@ __device__ __forceinline__ PcChild pc_child(const PcForkParams& p, int c) {
 // Last page of the child's tokens where it is partly filled and has to be
 // copied, else -1: the first child of a row keeps the row's own page, where
 // nothing else refers to it.
-__device__ __forceinline__ int pc_copied_page(const PcForkParams& p, const PcChild& k, int c) {
+__device__ __forceinline__ int pc_copied_page(const PcForkParams& p, const PcChild& k, int c, int first) {
   if (k.parent < 0 || k.len % p.page == 0) return -1;
   const int e = p.table[(int64_t)k.parent * p.max_blocks + k.held - 1];
   if (e < 0 || e >= p.pages) return -1;
-  const int first = __hip_atomic_load(p.first + k.parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   return first == c && p.refs[e] == 1 ? -1 : e;
 }
+
+constexpr int kPcRowsHere = 4096;  // rows whose first children the plan finds in LDS
 
 // Block 0 plans: which rows need how many pages, and which free ones those
 // are.  The other blocks copy the counts for the second launch to change.
@@ -268,14 +269,33 @@ __global__ __launch_bounds__(kPcPlanThreads) void pc_fork_plan_kernel(PcForkPara
     return;
   }
   __shared__ int s_part[kPcPlanThreads / 64];
-  for (int b = tid; b < p.rows; b += kPcPlanThreads)
-    __hip_atomic_store(p.first + b, 0x7fffffff, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __shared__ int s_first[kPcRowsHere];
+  // (the first counts are on their way beside what follows)
+  int early[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) early[j] = 4 * tid + j < p.pages ? p.refs[4 * tid + j] : 1;
+  // the first child of each row
+  const bool here = p.rows <= kPcRowsHere;
+  if (here) {
+    for (int b = tid; b < p.rows; b += kPcPlanThreads) s_first[b] = 0x7fffffff;
+  } else {
+    for (int b = tid; b < p.rows; b += kPcPlanThreads)
+      __hip_atomic_store(p.first + b, 0x7fffffff, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
   __syncthreads();
   for (int c = tid; c < p.children; c += kPcPlanThreads) {
     const int par = p.parents ? p.parents[c] : c;
-    if (par >= 0 && par < p.rows) atomicMin(p.first + par, c);
+    if (par >= 0 && par < p.rows) {
+      if (here) atomicMin(s_first + par, c);
+      else atomicMin(p.first + par, c);
+    }
   }
   __syncthreads();
+  auto first_of = [&](int row) {
+    if (row < 0) return -1;
+    if (here) return s_first[row];
+    return __hip_atomic_load(p.first + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
   // pages that the rows before each row take; a row that does not fit the
   // new table takes none and is marked
   int64_t taken = 0;
@@ -284,9 +304,13 @@ __global__ __launch_bounds__(kPcPlanThreads) void pc_fork_plan_kernel(PcForkPara
     int need = 0;
     if (c < p.children) {
       const PcChild k = pc_child(p, c);
+      int copies = 0;
       if (k.want > p.new_blocks) need = -1;
-      else if (k.parent >= 0) need = (pc_copied_page(p, k, c) >= 0) + k.want - k.held;
-      p.flags[c] = need;
+      else if (k.parent >= 0) {
+        copies = pc_copied_page(p, k, c, first_of(k.parent)) >= 0;
+        need = copies + k.want - k.held;
+      }
+      p.flags[c] = need * 2 + copies;
     }
     int total;
     const int mine = max(need, 0);
@@ -301,7 +325,7 @@ __global__ __launch_bounds__(kPcPlanThreads) void pc_fork_plan_kernel(PcForkPara
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t i = i0 + 4 * tid + j;
-      fr[j] = i < p.pages ? p.refs[i] == 0 : 0;
+      fr[j] = i0 == 0 ? early[j] == 0 : (i < p.pages ? p.refs[i] == 0 : 0);
       n += fr[j];
     }
     int total;
@@ -312,10 +336,11 @@ __global__ __launch_bounds__(kPcPlanThreads) void pc_fork_plan_kernel(PcForkPara
     found += total;
   }
   // a row is served if it needs nothing, or if the free pages last for it
-  // and all before it; flags: 1 served, 0 not
+  // and all before it; flags: bit 0 served, bit 1 its last page is a copy
   for (int c = tid; c < p.children; c += kPcPlanThreads) {
-    const int need = p.flags[c];
-    p.flags[c] = need == 0 || (need > 0 && (int64_t)p.start[c] + need <= found);
+    const int f = p.flags[c], need = f >> 1;
+    const int served = need == 0 || (need > 0 && (int64_t)p.start[c] + need <= found);
+    p.flags[c] = served | (f & 1) << 1;
   }
 }
 
@@ -331,10 +356,11 @@ __global__ __launch_bounds__(kPcThreads) void pc_fork_kernel(PcForkParams p) {
       const int c = i >> 32 ? (int)(i / p.new_blocks) : (int)((unsigned)i / (unsigned)p.new_blocks);
       const int col = (int)(i - (int64_t)c * p.new_blocks);
       const PcChild k = pc_child(p, c);
-      const bool served = k.parent >= 0 && p.flags[c];
+      const int flags = p.flags[c];
+      const bool served = k.parent >= 0 && (flags & 1);
       int e = -1;
       if (served && col < k.want) {
-        const bool copies = pc_copied_page(p, k, c) >= 0;
+        const int copies = flags >> 1;
         if (col >= k.held) e = p.freelist[p.start[c] + copies + col - k.held];
         else if (copies && col == k.held - 1) e = p.freelist[p.start[c]];
         else e = p.table[(int64_t)k.parent * p.max_blocks + col];
@@ -345,15 +371,15 @@ __global__ __launch_bounds__(kPcThreads) void pc_fork_kernel(PcForkParams p) {
     }
     for (int64_t c = me; c < p.children; c += stride) {
       const PcChild k = pc_child(p, (int)c);
-      p.new_lens[c] = k.parent < 0 ? 0 : (p.flags[c] ? k.len : -1);
+      p.new_lens[c] = k.parent < 0 ? 0 : (p.flags[c] & 1 ? k.len : -1);
     }
     return;
   }
   const int64_t w = (int64_t)blockIdx.x - p.table_blocks;
   const int c = (int)((unsigned)w / (unsigned)p.set.chunks);  // (the grid is below 2^31)
+  if (p.flags[c] != 3) return;
   const PcChild k = pc_child(p, c);
-  const int src = pc_copied_page(p, k, c);
-  if (src < 0 || !p.flags[c]) return;
+  const int src = p.table[(int64_t)k.parent * p.max_blocks + k.held - 1];
   pc_copy_chunk(p.set, (int)(w - (int64_t)c * p.set.chunks), src, p.freelist[p.start[c]], k.len % p.page);
 }
 

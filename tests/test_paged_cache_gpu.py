@@ -317,3 +317,23 @@ def test_fork_for_more_tokens_than_any_table_holds(page):
     refs[2] = refs[5] = 1
     new_table, new_lens, new_refs = dsa.paged_cache_fork(cache, table, lens, refs, new_tokens=2 ** 31 - 1)
     assert (new_table == -1).all() and (new_lens == -1).all() and (new_refs == 0).all()
+
+
+@pytest.mark.parametrize("rows,kids", [(4096, 5000), (4097, 4500), (9000, 3)])
+def test_fork_of_many_rows(rows, kids):
+    import dsa_triton_ascend_amd as dsa
+    rng = random.Random(rows)
+    page = 8
+    table, lens, refs = _pool(rng, rows, page, 20, 1500)
+    parents = [rng.randint(-1, rows) for _ in range(kids)]
+    caches = _caches(len(refs), page, ROWS[0], TYPES[0])
+    w_table, w_lens, w_refs, moves = _fork(table, lens, refs, parents, 1, page)
+    want = [c.clone() for c in caches]
+    moved = torch.tensor(moves, device="cuda").view(-1, 3)
+    for w in want:
+        for k in moved[:, 2].unique().tolist():
+            m = moved[moved[:, 2] == k]
+            w[m[:, 1], :k] = w[m[:, 0], :k]
+    t, l, r = dsa.paged_cache_fork(caches, _ints(table), _ints(lens), _ints(refs), parents=_ints(parents), new_tokens=1)
+    assert t.tolist() == w_table and l.tolist() == w_lens and r.tolist() == w_refs
+    assert all(torch.equal(c, w) for c, w in zip(caches, want))
