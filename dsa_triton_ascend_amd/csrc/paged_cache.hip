@@ -434,7 +434,7 @@ int pc_fork_run(int64_t n, void* const* caches, const int64_t* row_bytes, const 
 // and written and the moves need no order.
 // ---------------------------------------------------------------------------
 // Up to this many pages every block of the rank kernel counts the live pages by
-// itself: a block's 1024 threads read 16 counts each.  8192 pages: 6.9 us, and
+// itself: a block's 1024 threads read 16 counts each.  8192 pages: 5.1 us, and
 // 3.3 + 4.2 us with a launch that counts first, which pays where the counts
 // no longer come from the L2 (64 KB of them here, by 16 blocks).
 constexpr int64_t kPcCountsHere = 16384;
@@ -443,7 +443,8 @@ struct PcCompactParams {
   PcCopySet set;
   const int32_t *table, *refs;
   int32_t *new_table, *new_refs, *page_map;
-  int32_t *live, *rank, *high, *hole;  // workspace: live pages of each chunk, ranks, moved pages and their places
+  // workspace: live pages of each chunk (where they are counted first), ranks, moved pages and their places
+  int32_t *live, *rank, *high, *hole;
   int64_t pages, entries;
   int chunks;                          // chunks of kPcPlanThreads pages
   int table_blocks, copy_blocks;
@@ -476,15 +477,18 @@ __global__ __launch_bounds__(kPcPlanThreads) void pc_rank_kernel(PcCompactParams
   if (p.counts_here) {
     // few pages: every block counts them all
     int a = 0, b = 0;
-    for (int64_t i = threadIdx.x; i < p.pages; i += kPcPlanThreads) {
+    const int pages = (int)p.pages, mine = (int)blockIdx.x * kPcPlanThreads;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < pages; i += kPcPlanThreads) {
       const int v = p.refs[i] > 0;
       b += v;
-      a += i < (int64_t)blockIdx.x * kPcPlanThreads ? v : 0;
+      a += i < mine ? v : 0;
     }
     pc_block_scan<W>(a, s_part, &before);
     pc_block_scan<W>(b, s_part, &n);
     int c = 0;
-    for (int64_t i = threadIdx.x; i < n; i += kPcPlanThreads) c += p.refs[i] > 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += kPcPlanThreads) c += p.refs[i] > 0;
     pc_block_scan<W>(c, s_part, &low);
   } else {
     pc_live<W>(p, blockIdx.x, s_part, &before, &n);
@@ -498,7 +502,12 @@ __global__ __launch_bounds__(kPcPlanThreads) void pc_rank_kernel(PcCompactParams
   const int64_t i = (int64_t)blockIdx.x * kPcPlanThreads + threadIdx.x;
   const int lv = i < p.pages && p.refs[i] > 0;
   const int at = before + pc_block_scan<W>(lv, s_part, &total) - lv;  // live pages before i
-  if (p.counts_here && threadIdx.x == 0) p.live[blockIdx.x] = total;
+  // live pages and moved ones, for the next launch: at most half the pages
+  // move, so the lists' last places are free
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.high[p.pages - 1] = n;
+    p.hole[p.pages - 1] = n - low;
+  }
   if (i >= p.pages) return;
   int k = -1;
   if (lv && i >= n) {
@@ -517,11 +526,8 @@ __device__ __forceinline__ int pc_place(const PcCompactParams& p, int64_t i, int
 }
 
 __global__ __launch_bounds__(kPcThreads) void pc_compact_kernel(PcCompactParams p) {
-  constexpr int W = kPcThreads / 64;
-  __shared__ int s_part[W];
   const int tid = threadIdx.x;
-  int low, n;
-  pc_live<W>(p, 0, s_part, &low, &n);
+  const int n = p.high[p.pages - 1];
   if ((int)blockIdx.x < p.table_blocks) {
     const int64_t stride = (int64_t)p.table_blocks * kPcThreads, me = (int64_t)blockIdx.x * kPcThreads + tid;
     for (int64_t i = me; i < p.entries; i += stride) {
@@ -535,13 +541,7 @@ __global__ __launch_bounds__(kPcThreads) void pc_compact_kernel(PcCompactParams 
     }
     return;
   }
-  // moved pages: as many as free ids below n
-  const int nc = n / kPcPlanThreads;
-  int dummy, part = 0, more;
-  pc_live<W>(p, nc, s_part, &low, &dummy);
-  for (int64_t i = (int64_t)nc * kPcPlanThreads + tid; i < n; i += kPcThreads) part += p.refs[i] > 0;
-  pc_block_scan<W>(part, s_part, &more);
-  const int64_t work = (int64_t)(n - low - more) * p.set.chunks;
+  const int64_t work = (int64_t)p.hole[p.pages - 1] * p.set.chunks;
   for (int64_t w = (int64_t)blockIdx.x - p.table_blocks; w < work; w += p.copy_blocks) {
     const int k = (int)(w / p.set.chunks);
     const int64_t src = p.high[k], dst = p.hole[k];
