@@ -108,7 +108,7 @@ def build_calls():
             "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
            + [x for i in includes for x in ("-isystem", i)]
            + [os.path.join(CSRC, "torch_calls.cpp"), "-o", tmp, "-L" + lib, "-ltorch_python", "-ltorch_cpu",
-              "-lc10", "-lc10_hip"])
+              "-ltorch_hip", "-lc10", "-lc10_hip"])
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for torch_calls.cpp:\n{' '.join(cmd)}\n{r.stdout + r.stderr}")

@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/Allocator.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
@@ -196,6 +197,12 @@ PyObject* triple(at::Tensor x, at::Tensor y, at::Tensor z) {
   return r;
 }
 
+// a new contiguous tensor beside t (what at::empty comes down to)
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor& t, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, t.device(), std::nullopt));
+}
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor& t) { return fresh(sizes, t, t.scalar_type()); }
+
 // memory of torch's allocator for a workspace: returned to it with the value,
 // in the order of the current stream
 c10::DataPtr workspace(size_t n) { return c10::GetAllocator(c10::kCUDA)->allocate(std::max<size_t>(n, 1)); }
@@ -213,9 +220,8 @@ PyObject* fork(PyObject* const* a) {
   if (a[4] != Py_None && !(parents = ints(a[4], &index, 1))) return nullptr;
   const int64_t rows = table->size(0), wide = table->size(1), children = parents ? parents->size(0) : rows;
   if (lens->size(0) != rows || refs->size(0) != c.pages) return nullptr;
-  const auto kind = table->options();
-  at::Tensor new_table = at::empty({children, wide}, kind), new_lens = at::empty({children}, kind);
-  at::Tensor new_refs = at::empty({c.pages}, kind);
+  at::Tensor new_table = fresh({children, wide}, *table), new_lens = fresh({children}, *table);
+  at::Tensor new_refs = fresh({c.pages}, *table);
   const size_t bytes = entry.fork_bytes(rows, children, c.pages);
   c10::DataPtr ws = workspace(bytes);
   if (!launched(entry.fork, (int64_t)c.t.size(), c.at.data(), c.row_bytes.data(), data(table), data(lens), data(refs),
@@ -235,9 +241,8 @@ PyObject* compact(PyObject* const* a) {
   if (a[3] != Py_None && (!integer(a[3], &page) || page != c.page)) return nullptr;
   const at::Tensor *table = ints(a[1], &index, 2), *refs = ints(a[2], &index, 1);
   if (!table || !refs || !current(index) || refs->size(0) != c.pages) return nullptr;
-  const auto kind = table->options();
-  at::Tensor new_table = at::empty(table->sizes(), kind), new_refs = at::empty({c.pages}, kind);
-  at::Tensor map = at::empty({c.pages}, kind);
+  at::Tensor new_table = fresh(table->sizes(), *table), new_refs = fresh({c.pages}, *table);
+  at::Tensor map = fresh({c.pages}, *table);
   const size_t bytes = entry.compact_bytes(c.pages);
   c10::DataPtr ws = workspace(bytes);
   if (!launched(entry.compact, (int64_t)c.t.size(), c.at.data(), c.row_bytes.data(), data(table), data(refs),
@@ -282,9 +287,8 @@ PyObject* attention(PyObject* const* a) {
   const int64_t wide = table->size(1);
   const size_t bytes = entry.attn_bytes(b, s1, n1, n2, d, latent, wide, page);
   if (!bytes) return nullptr;
-  const auto f32 = q->options().dtype(at::kFloat);
-  at::Tensor out = at::empty(q->sizes(), q->options()), mx = at::empty({b, n2, s1, n1 / n2}, f32);
-  at::Tensor sm = at::empty({b, n2, s1, n1 / n2}, f32);
+  at::Tensor out = fresh(q->sizes(), *q), mx = fresh({b, n2, s1, n1 / n2}, *q, at::kFloat);
+  at::Tensor sm = fresh({b, n2, s1, n1 / n2}, *q, at::kFloat);
   c10::DataPtr ws = workspace(bytes);
   if (!launched(entry.attn, q->data_ptr(), latent ? qr->data_ptr() : nullptr, k->data_ptr(), latent ? kr->data_ptr() : nullptr,
                  latent ? nullptr : v->data_ptr(), out.data_ptr(), (float*)mx.data_ptr(), (float*)sm.data_ptr(),
@@ -341,7 +345,7 @@ bool rotated(const Rotation& r, const at::Tensor in[2], const at::Tensor& pos, c
     cols[i] = t.size(rank - 1), heads[i] = t.size(lead);
     if ((t.stride(rank - 1) != 1 && cols[i] != 1) || r.start[i] < 0 || r.start[i] > cols[i] - rot) return false;
     if (inplace && (t.stride(rank - 1) != 1 || t.is_inference() || overlaps_itself(t))) return false;
-    out[i] = inplace ? t : at::empty(t.sizes(), t.options());
+    out[i] = inplace ? t : fresh(t.sizes(), t);
     for (int64_t j = 0; j < lead + 1; ++j) {
       si[i][j + r.tnd] = t.stride(j);
       so[i][j + r.tnd] = out[i].stride(j);
