@@ -264,7 +264,7 @@ PyObject* attention(PyObject* const* a) {
   bool lse;
   if (!q || !k || !table || !act_k || !current(index) || q->dim() != 4 || k->dim() != 4) return nullptr;
   if (!number(a[5], &scale) || !integer(a[9], &mode) || !integer(a[10], &pre) || !integer(a[11], &next) ||
-      !flag(a[12], &lse))
+      !flag(a[12], &lse) || (mode != 0 && mode != 3))
     return nullptr;
   const auto kind = q->scalar_type();
   auto cache = [&](const at::Tensor* t) {

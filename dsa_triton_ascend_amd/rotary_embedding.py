@@ -6,8 +6,8 @@ launch, of a key; ``rotary_frequencies`` gives its frequencies, plain or
 scaled for contexts longer than the trained one.  The reference has no such
 operator: it takes rotated inputs.
 
-Angles ``position * inv_freq`` are formed in 64 bits inside the kernel, so any
-position of an int32 or int64 tensor is exact to fp32 and no table is kept.
+Angles ``position * inv_freq`` are formed in 64 bits inside the kernel, so
+positions up to 2^31 are exact to fp32 and no table is kept.
 """
 import math
 

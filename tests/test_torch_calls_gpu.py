@@ -211,7 +211,7 @@ def test_what_is_taken_and_what_is_left():
     assert c.attention(*ok) is not None
     for i, x in ((0, q.float()), (0, q[:, :, :3, :48]), (0, q[:, :, ::2]), (1, caches[0].half()), (1, caches[0][:, ::2]),
                  (2, caches[1][:5]), (2, None), (3, table.long()), (3, table[:1]), (4, [20, 40]), (4, lens.long()),
-                 (5, None), (6, q), (8, lens[:1]), (9, 1), (9, True), (10, 2 ** 63), (11, None), (12, 1)):
+                 (5, None), (6, q), (8, lens[:1]), (9, 1), (9, True), (9, 2 ** 32 + 3), (10, 2 ** 63), (11, None), (12, 1)):
         assert c.attention(*ok[:i], x, *ok[i + 1:]) is None, (i, x)
     assert c.attention(*ok[:12]) is None  # too few arguments
     torch.cuda.synchronize()
