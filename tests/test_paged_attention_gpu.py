@@ -432,3 +432,16 @@ def test_rows_that_see_nothing_beside_values_that_are_not_finite(latent, N1, D, 
     args["key"][last] = float("nan")
     out, mx, sm = dsa.paged_attention(**args)
     assert torch.isnan(out[0, 0]).all() and torch.isnan(sm[0, :, 0]).all() and (out[0, 1:] == 0).all()
+
+
+@pytest.mark.parametrize("latent,N1,N2,D,S1,page,lens,act_q", [
+    (False, 4, 2, 64, 100, 1000, [100, 1500, 70], [100, 100, 70]),
+    (False, 6, 1, 256, 33, 24, [33, 400, 0], None),
+    (True, 4, 1, 128, 100, 24, [100, 130, 900], [100, 1, 64]),
+    (True, 40, 1, 512, 17, 64, [17, 333, 5], [17, 17, 5]),
+])
+@pytest.mark.parametrize("mode,pre", [(3, INT64_MAX), (3, 40), (0, INT64_MAX)])
+def test_many_new_tokens(latent, N1, N2, D, S1, page, lens, act_q, mode, pre):
+    args, data = _make(len(lens), S1, N1, N2, D, page, lens, torch.bfloat16, latent, seed=91, act_q=act_q, mode=mode,
+                       pre=pre)
+    _compare(args, data, lens, act_q=act_q)
