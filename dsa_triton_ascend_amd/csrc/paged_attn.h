@@ -36,18 +36,16 @@ struct PagedAttnParams {
   void* out;
   float *smax, *ssum;
   const int32_t *act_q, *act_k, *table;
-  // Outputs of runs, [worker][2][lane group][rows][D]: unnormalised in 32
-  // bits, or (half_parts) divided by their divisor and by a power of two above
-  // their row's largest, in 16.  The latter are off by 2^-12 of the row's
-  // largest value, a sixteenth of what the bf16 output rounds and as much as
-  // the fp16 output does; they halve 134 MB written and read at 128 heads.
-  void* part_o;
-  float* part_scale;  // [worker][2][lane group][rows] those powers of two
+  // Outputs of runs, unnormalised, [worker][2][lane group][rows][D], in 32
+  // bits.  16 bits with a power of two per row would halve what is written and
+  // read (134 MB at 128 heads, 352 us in place of 358 for 32 x 32K tokens), but
+  // a column much larger than its row's others would take their bits: at 2^24
+  // times their size they were off by a tenth of their values.
+  float* part_o;
   f32x4* part_ml;  // [worker][2][lane group][rows] {ref, sum, largest score, divisor of the output}
   int64_t kv_rows, band_pre, band_next;
   int batch, s1, n1, n2, group, rows;  // group = n1 / n2 query heads of a key head; rows = s1 * group
   int max_blocks, page, mode, return_lse;
-  int half_parts;
   int workers, min_tiles;              // workers of one lane group; fewest tiles of a worker
   int groups, row_groups, group_rows;  // lane groups (key head, row group); rows of a row group
   unsigned page_magic;                 // floor((2^32 - 1) / page)
@@ -222,7 +220,7 @@ struct PagedPlan {
 
 // workspace and launches of the two kernels (paged_attn.hip, paged_attn_latent.hip)
 struct PagedShape {
-  int workers, min_tiles, groups, row_groups, group_rows, tile, half_parts;
+  int workers, min_tiles, groups, row_groups, group_rows, tile;
 };
 size_t paged_part_bytes(const PagedShape& s, int64_t d);
 int paged_workers(int64_t slots, int64_t groups, int64_t batch, int64_t tiles, int min_tiles);

@@ -26,8 +26,6 @@
 // idle otherwise), so the weights keep 16 bits and more.
 #include "paged_attn.h"
 
-#include <type_traits>
-
 namespace dsa {
 
 __device__ __attribute__((aligned(16))) unsigned char g_paged_zero_row[1024];
@@ -259,7 +257,7 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
       } else {
         const int64_t slot = (((int64_t)worker * 2 + (first_segment ? 0 : 1)) * p.groups + ng) * p.group_rows +
                              mt * 16 + li;
-        float* dst = (float*)p.part_o + slot * D;
+        float* dst = p.part_o + slot * D;
         const float seen = l != 0.f ? 1.f : 0.f;
 #pragma unroll
         for (int c = 0; c < NJ / EC; ++c)
@@ -292,13 +290,12 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
 // ---------------------------------------------------------------------------
 constexpr int kPcFewRuns = 64;
 
-template <typename T, int D, bool HALF>
+template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, int tile, int wg_rows) {
   using E = Elem<T>;
   constexpr int EPL = D / 64;
   typedef T TV __attribute__((ext_vector_type(EPL)));
   typedef float FV __attribute__((ext_vector_type(EPL)));
-  typedef f16 HV __attribute__((ext_vector_type(EPL)));
   __shared__ FV s_o[4][64];
   __shared__ float s_l[4], s_n[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -336,26 +333,23 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, i
         const int mine = c + lane;
         float f = 0.f;
         if (mine < i1) {
-          const int64_t at = slot(mine);
-          const f32x4 ml = p.part_ml[at];
+          const f32x4 ml = p.part_ml[slot(mine)];
           f = fast_exp2(ml[0] - m);
           la += ml[1] * f;
           na += ml[3] * f;
-          if constexpr (HALF) f *= ml[3] * p.part_scale[at];
         }
         const int cnt = min(64, i1 - c);
         for (int i = 0; i < cnt; i += 8) {
           // eight rows in flight (those past the last read it again, times zero)
-          std::conditional_t<HALF, HV, FV> x[8];
+          FV x[8];
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            x[u] = *((const std::conditional_t<HALF, HV, FV>*)p.part_o + slot(c + min(i + u, cnt - 1)) * 64 + lane);
+          for (int u = 0; u < 8; ++u) x[u] = *((const FV*)p.part_o + slot(c + min(i + u, cnt - 1)) * 64 + lane);
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
             const float g =
                 i + u < cnt ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (i + u) & 63)) : 0.f;
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) acc[e] += i + u < cnt ? (float)x[u][e] * g : 0.f;
+            for (int e = 0; e < EPL; ++e) acc[e] += i + u < cnt ? x[u][e] * g : 0.f;
           }
         }
       }
@@ -407,18 +401,12 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, i
   }
 }
 
-template <typename T, int D>
-static void paged_combine_one(const PagedAttnParams& p, int tile, int wg_rows, unsigned grid, hipStream_t stream) {
-  if (p.half_parts) paged_combine_kernel<T, D, true><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
-  else paged_combine_kernel<T, D, false><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
-}
-
 template <typename T>
 static void paged_combine_d(const PagedAttnParams& p, int tile, int wg_rows, int64_t d, unsigned grid, hipStream_t stream) {
-  if (d == 64) paged_combine_kernel<T, 64, false><<<grid, 256, 0, stream>>>(p, tile, wg_rows);  // grouped form only
-  else if (d == 128) paged_combine_one<T, 128>(p, tile, wg_rows, grid, stream);
-  else if (d == 256) paged_combine_one<T, 256>(p, tile, wg_rows, grid, stream);
-  else paged_combine_one<T, 512>(p, tile, wg_rows, grid, stream);
+  if (d == 64) paged_combine_kernel<T, 64><<<grid, 256, 0, stream>>>(p, tile, wg_rows);  // grouped form only
+  else if (d == 128) paged_combine_kernel<T, 128><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
+  else if (d == 256) paged_combine_kernel<T, 256><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
+  else paged_combine_kernel<T, 512><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
 }
 
 int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream) {
@@ -434,7 +422,7 @@ int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t 
 
 size_t paged_part_bytes(const PagedShape& s, int64_t d) {
   const size_t rows = (size_t)s.workers * 2 * s.groups * s.group_rows;
-  return rows * (sizeof(f32x4) + (s.half_parts ? d * sizeof(f16) + sizeof(float) : d * sizeof(float)));
+  return rows * (sizeof(f32x4) + d * sizeof(float));
 }
 
 // Workers of a lane group for `slots` workers resident at once.  As many as
@@ -459,7 +447,6 @@ int paged_workers(int64_t slots, int64_t groups, int64_t batch, int64_t tiles, i
 static PagedShape paged_grouped_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d,
                                       int64_t max_blocks, int64_t page) {
   PagedShape s;
-  s.half_parts = 0;
   s.tile = kPaTile;
   const int64_t rows = s1 * (n1 / n2);
   int mt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
@@ -525,10 +512,8 @@ int paged_attn_run(const void* query, const void* query_rope, const void* key, c
   p.act_k = act_k;
   p.table = table;
   const int64_t part_rows = (int64_t)s.workers * 2 * s.groups * s.group_rows;
-  p.half_parts = s.half_parts;
   p.part_ml = (f32x4*)workspace;
-  p.part_o = p.part_ml + part_rows;
-  p.part_scale = (float*)((f16*)p.part_o + part_rows * d);  // with half_parts
+  p.part_o = (float*)(p.part_ml + part_rows);
   p.kv_rows = num_blocks * page;
   p.band_pre = band_clamp(pre_tokens);
   p.band_next = band_clamp(next_tokens);

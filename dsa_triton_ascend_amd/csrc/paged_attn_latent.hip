@@ -110,9 +110,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   __shared__ int s_tab[kPlPages];
   __shared__ float s_f[2 * HG];  // by a tile's parity: factors of the rows whose reference moved
   __shared__ int s_flag[3];  // by a tile's number modulo 3: bits of the waves whose rows moved
-  // of a finished run, in place of P: the rows' divisors, and largest outputs as bits
-  float* const s_n = (float*)s_p;
-  int* const s_am = (int*)s_p + HG;
+  float* const s_n = (float*)s_p;  // of a finished run, in place of P: the rows' divisors
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int li = lane & 15, lg = lane >> 4;
@@ -517,7 +515,6 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
       const int r = wave * 16 + li, rr = rg * HG + r;
       if (scores && lg == 0) {
         s_n[r] = n;
-        s_am[r] = 0;
         if (rr < p.rows) {
           if (!whole) {
             p.part_ml[slot0 + r] = {ref, l, top, n};
@@ -538,8 +535,9 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     auto put = [&](auto zero, void* to, auto value) {
       using O = decltype(zero);
       typedef O O4 __attribute__((ext_vector_type(4)));
-      constexpr int RP = HG < 64 ? HG : 64;              // rows of a pass
       constexpr int ROW = D * (int)sizeof(O), PITCH = ROW + 16;  // (16 rows' chunks lie in 64 different banks)
+      constexpr int FIT = 64 * PITCH <= (int)sizeof(smem) ? 64 : 32;
+      constexpr int RP = HG < FIT ? HG : FIT;                    // rows of a pass
       constexpr int CHUNKS = RP * ROW / 16;
       static_assert(RP * PITCH <= (int)sizeof(smem), "output stage");
       const int col = (wave * NDW * 16 + lg * 4) * (int)sizeof(O);
@@ -587,46 +585,8 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
         inv[ht] = n_row[ht] != 0.f ? 1.f / n_row[ht] : 0.f;
       }
       put(T{}, (T*)p.out + ((int64_t)b * p.rows + rg * HG) * D, [&](int ht, int j) { return acc[j][ht] * inv[ht]; });
-    } else if constexpr (kLo) {
-      put(0.f, (float*)p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht]; });
     } else {
-#pragma unroll
-      for (int ht = 0; ht < HW; ++ht) {
-        // (magnitudes as integers, which are ordered alike and need no
-        // canonical form; infinities and NaN, above all others, do not count)
-        unsigned m = 0;
-#pragma unroll
-        for (int j = 0; j < NDW; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) m = max(m, __float_as_uint(acc[j][ht][r]) & 0x7fffffffu);
-        if (__any(m >= 0x7f800000u)) {
-          m = 0;
-#pragma unroll
-          for (int j = 0; j < NDW; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const unsigned y = __float_as_uint(acc[j][ht][r]) & 0x7fffffffu;
-              m = y < 0x7f800000u ? max(m, y) : m;
-            }
-        }
-        float a = __uint_as_float(m);
-        a = xgroup_max(a);
-        if (lg == 0) atomicMax(s_am + ht * 16 + li, __float_as_int(a));  // (not negative: ordered as integers)
-      }
-      lds_barrier();
-      float mul[HW];
-#pragma unroll
-      for (int ht = 0; ht < HW; ++ht) {
-        const float a = __int_as_float(s_am[ht * 16 + li]);
-        const float inv = n_row[ht] != 0.f ? 1.f / n_row[ht] : 0.f;
-        int ex = 0;
-        if (a * inv > 0.f) (void)frexpf(a * inv, &ex);  // a / n < 2^ex
-        ex = max(ex, -100);
-        mul[ht] = ldexpf(inv, -ex);
-        if (wave == 0 && lg == 0 && rg * HG + ht * 16 + li < p.rows)
-          p.part_scale[slot0 + ht * 16 + li] = ldexpf(1.f, ex);
-      }
-      put(f16{}, (f16*)p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht] * mul[ht]; });
+      put(0.f, p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht]; });
     }
     }(fresh_lane());
     first_segment = false;
@@ -641,10 +601,8 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
 PagedShape paged_latent_shape(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t max_blocks, int64_t page) {
   PagedShape s;
   s.tile = kPlTile;
-  s.half_parts = 0;
   const int64_t rows = s1 * n1;
   s.group_rows = rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 ? 64 : 128));
-  s.half_parts = s.group_rows > 32;  // as P is rounded once there
   s.row_groups = (int)((rows + s.group_rows - 1) / s.group_rows);
   s.groups = s.row_groups;
   s.min_tiles = kPaMinTiles;

@@ -445,3 +445,19 @@ def test_many_new_tokens(latent, N1, N2, D, S1, page, lens, act_q, mode, pre):
     args, data = _make(len(lens), S1, N1, N2, D, page, lens, torch.bfloat16, latent, seed=91, act_q=act_q, mode=mode,
                        pre=pre)
     _compare(args, data, lens, act_q=act_q)
+
+
+@pytest.mark.parametrize("latent,N1,D", [(False, 8, 128), (True, 16, 512), (True, 64, 512), (True, 128, 512),
+                                         (True, 128, 128), (True, 40, 256)])
+@pytest.mark.parametrize("dt,large,small", [("bf16", 2.0 ** 12, 2.0 ** -12), ("fp16", 2.0 ** 14, 2.0 ** -8)])
+def test_small_columns_beside_a_large_one(latent, N1, D, dt, large, small):
+    """A column of values 2^22 or 2^24 times the others': the others keep their
+    own precision, also where a sequence is joined from many runs."""
+    lens = [4000, 130, 3]
+    args, data = _make(3, 1, N1, 1, D, 64, lens, DTYPES[dt], latent, seed=95)
+    args["query"][..., 0] = 0
+    i = 0 if latent else 1
+    for x in [args["key" if latent else "value"]] + [d[i] for d in data]:
+        x *= small
+        x[..., 0] = large
+    _compare(args, data, lens)
