@@ -221,7 +221,7 @@ def load():
 
 _ENTRIES = ("dsa_rope", "dsa_paged_cache_write", "dsa_paged_cache_fork_workspace_size", "dsa_paged_cache_fork",
             "dsa_paged_cache_compact_workspace_size", "dsa_paged_cache_compact", "dsa_paged_attn_workspace_size",
-            "dsa_paged_attn")  # in the order in which _torch_calls takes them
+            "dsa_paged_attn", "dsa_last_error")  # in the order in which _torch_calls takes them
 _calls = None
 
 

@@ -6,7 +6,10 @@
 // Each function checks that its call is an ordinary one (plain tensors of the
 // documented shapes and types on the current GPU, nothing to convert) and makes it; for anything else, an entry point that
 // refuses included, it returns None and the Python function goes its own way,
-// which converts what may be converted and raises the errors.
+// which converts what may be converted and raises the errors.  An error of the
+// HIP runtime is raised here: the kernels may have run by then (an error that
+// another call left behind is reported by the next launch), and a rotation in
+// place must not be made twice.
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <torch/csrc/Exceptions.h>
@@ -24,6 +27,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <stdexcept>
 #include <utility>
 #include <vector>
 
@@ -40,16 +44,27 @@ struct Entries {
   decltype(&dsa_paged_cache_compact) compact;
   decltype(&dsa_paged_attn_workspace_size) attn_bytes;
   decltype(&dsa_paged_attn) attn;
+  decltype(&dsa_last_error) error;
 } entry;
 
-// an entry point's status; other Python threads run meanwhile, since a launch
-// may wait for room in its queue
+// the HIP runtime reported an error at or before a launch
+struct HipError : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+
+// Whether an entry point made its launches; other Python threads run
+// meanwhile, since a launch may wait for room in its queue.
 template <typename F, typename... Args>
 bool launched(F f, Args... args) {
-  if (!PyGILState_Check()) return f(args...) == DSA_OK;  // (a thread of the autograd engine)
-  PyThreadState* state = PyEval_SaveThread();
-  const int status = f(args...);
-  PyEval_RestoreThread(state);
+  int status;
+  if (!PyGILState_Check()) {  // (a thread of the autograd engine)
+    status = f(args...);
+  } else {
+    PyThreadState* state = PyEval_SaveThread();
+    status = f(args...);
+    PyEval_RestoreThread(state);
+  }
+  if (status == DSA_ERR_HIP) throw HipError(entry.error());
   return status == DSA_OK;
 }
 
@@ -467,6 +482,9 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
       // raised by Python code on the way (a hook on saved tensors, which
       // checkpoints stop their recomputation by): the caller's
       e.restore();
+      return nullptr;
+    } catch (const HipError& e) {
+      PyErr_SetString(PyExc_RuntimeError, e.what());
       return nullptr;
     } catch (...) {
       r = nullptr;

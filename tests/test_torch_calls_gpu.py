@@ -247,3 +247,31 @@ def test_two_threads_and_a_graph():
         graph.replay()
         eager = dsa.paged_attention(q, caches[0], caches[1], table, lens)[0]
         assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_an_error_left_behind_is_raised_and_no_rotation_made_twice(monkeypatch, compiled):
+    """An error that an earlier HIP call left behind (here: no such device) is
+    reported by the next launch, whose kernel has run by then."""
+    import ctypes
+
+    import dsa_triton_ascend_amd as dsa
+    from dsa_triton_ascend_amd import _lib
+    if not compiled:
+        monkeypatch.setattr(_lib, "_calls", _lib._NoCalls)
+    q = torch.randn(2, 3, 4, 64, device="cuda")
+    pos = torch.arange(3, device="cuda")
+    inv, _ = dsa.rotary_frequencies(64)
+    once, _ = dsa.rotary_embedding(q, None, pos, inv)
+    hip = ctypes.CDLL("libamdhip64.so")
+    x = q.clone()
+    torch.cuda.synchronize()
+    hip.hipGetLastError()
+    assert hip.hipSetDevice(10 ** 6) != 0
+    try:
+        with pytest.raises(RuntimeError, match="HIP error"):
+            dsa.rotary_embedding(x, None, pos, inv, inplace=True)
+    finally:
+        hip.hipGetLastError()
+    assert torch.equal(x, once)
+    assert torch.equal(dsa.rotary_embedding(q, None, pos, inv)[0], once)  # and the next call is an ordinary one
