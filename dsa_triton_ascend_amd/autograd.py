@@ -27,6 +27,7 @@ DSA indexer training, where the KL loss trains only the indexer.
 ``RotaryEmbeddingFunction`` is the differentiable form of ``rotary_embedding``.
 """
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .rotary_embedding import _rotate
 from .sparse_flash_attention import INT64_MAX, sparse_flash_attention_triton
@@ -131,12 +132,15 @@ class RotaryEmbeddingFunction(torch.autograd.Function):
     """Differentiable rotary positions of a query and an optional key, for
     calls that ``_torch_calls`` leaves to Python (it has the same node): a
     rotation's gradient is the rotation by the opposite angles, with the same
-    scale, so nothing of the forward but the positions is kept."""
+    scale, so nothing of the forward but the positions is kept.  The rotation
+    is linear, so a tangent turns as its input does."""
 
     @staticmethod
     def forward(ctx, query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse):
         ctx.save_for_backward(positions, inv_freq)
+        ctx.save_for_forward(positions, inv_freq)
         ctx.args = (interleaved, q_start, k_start, scale, not inverse)
+        ctx.shapes = query.shape, None if key is None else key.shape
         ctx.set_materialize_grads(False)
         return _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False)
 
@@ -146,18 +150,29 @@ class RotaryEmbeddingFunction(torch.autograd.Function):
         interleaved, q_start, k_start, scale, inverse = ctx.args
         d_q = d_query if ctx.needs_input_grad[0] else None
         d_k = d_key if ctx.needs_input_grad[1] else None
-        if d_q is None and d_k is not None:
-            d_q, k_start, q_start = d_k, 0, k_start
-            d_k, swapped = None, True
-        else:
-            swapped = False
-        if d_q is not None:
-            if torch.is_grad_enabled():  # the gradient of this one will be asked for
-                d_q, d_k = RotaryEmbeddingFunction.apply(d_q, d_k, positions, inv_freq, interleaved, q_start, k_start,
-                                                         scale, inverse)
-            else:
-                d_q, d_k = _rotate(d_q, d_k, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False)
-        return ((None, d_q) if swapped else (d_q, d_k)) + (None,) * 7
+        return _rotate_linear(d_q, d_k, positions, inv_freq, interleaved, q_start, k_start, scale, inverse) + (None,) * 7
+
+    @staticmethod
+    def jvp(ctx, t_query, t_key, *_):
+        positions, inv_freq = ctx.saved_tensors
+        interleaved, q_start, k_start, scale, inverse = ctx.args
+        out = _rotate_linear(t_query, t_key, positions, inv_freq, interleaved, q_start, k_start, scale, not inverse)
+        some = t_key if t_query is None else t_query
+        # (an output's tangent may not be absent)
+        return tuple(some.new_zeros(shape) if o is None and shape is not None else o for o, shape in zip(out, ctx.shapes))
+
+
+def _rotate_linear(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse):
+    """Rotated gradients or tangents, either of which may be absent, with
+    whatever derivatives they carry themselves."""
+    if query is None and key is None:
+        return None, None
+    if query is None:
+        return _rotate_linear(key, None, positions, inv_freq, interleaved, k_start, 0, scale, inverse)[::-1]
+    if torch.is_grad_enabled() or any(t is not None and unpack_dual(t).tangent is not None for t in (query, key)):
+        return RotaryEmbeddingFunction.apply(query, key, positions, inv_freq, interleaved, q_start, k_start, scale,
+                                             inverse)
+    return _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False)
 
 
 __all__ = ["RotaryEmbeddingFunction", "SparseFlashAttentionFunction", "sparse_flash_attention_train",

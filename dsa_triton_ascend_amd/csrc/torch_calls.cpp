@@ -80,6 +80,9 @@ const at::Tensor* tensor(PyObject* o, int* index) {
   return t.get_device() == *index ? &t : nullptr;
 }
 
+// the tangent of a dual tensor (forward-mode derivatives), else undefined
+const at::Tensor& tangent(const at::Tensor& t) { return t._fw_grad(/*level=*/0); }
+
 const at::Tensor* ints(PyObject* o, int* index, int64_t dim) {
   const at::Tensor* t = tensor(o, index);
   return t && t->scalar_type() == at::kInt && t->dim() == dim && t->numel() > 0 && t->is_contiguous() ? t : nullptr;
@@ -354,7 +357,7 @@ bool rotated(const Rotation& r, const at::Tensor in[2], const at::Tensor& pos, c
   for (int i = 0; i < 2; ++i) {
     const at::Tensor& t = in[i];
     if (!t.defined()) continue;
-    if (t.dim() != rank || t.scalar_type() != kind || t.numel() == 0) return false;
+    if (t.dim() != rank || t.scalar_type() != kind || t.numel() == 0 || t._is_zerotensor()) return false;
     for (int64_t j = 0; j < lead; ++j)
       if (t.size(j) != q.size(j)) return false;
     cols[i] = t.size(rank - 1), heads[i] = t.size(lead);
@@ -396,6 +399,21 @@ struct RotaryBackward : torch::autograd::Node {
   }
 
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    torch::autograd::variable_list result = turned(grads);
+    // the tangent of a gradient turns as the gradient does
+    torch::autograd::variable_list tangents(grads.size());
+    bool dual = false;
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (grads[i].defined() && tangent(grads[i]).defined()) tangents[i] = tangent(grads[i]), dual = true;
+    if (dual) {
+      tangents = turned(tangents);
+      for (size_t i = 0; i < result.size(); ++i)
+        if (result[i].defined() && tangents[i].defined()) result[i]._set_fw_grad(tangents[i], /*level=*/0, false);
+    }
+    return result;
+  }
+
+  torch::autograd::variable_list turned(const torch::autograd::variable_list& grads) {
     const at::Tensor p = pos.unpack(), f = freq.unpack();
     const size_t n = num_outputs();
     at::Tensor in[2], out[2];
@@ -404,7 +422,7 @@ struct RotaryBackward : torch::autograd::Node {
     Rotation back = r;
     back.inverse = !r.inverse;
     for (int i = 0; i < (int)n; ++i)
-      if (grads[i].defined() && task_should_compute_output(i)) {
+      if (grads[i].defined() && !grads[i]._is_zerotensor() && task_should_compute_output(i)) {
         in[count] = grads[i].stride(-1) == 1 ? grads[i] : grads[i].contiguous();
         back.start[count] = r.start[i];
         place[count++] = i;
@@ -445,6 +463,7 @@ PyObject* rotate(PyObject* const* a) {
   const at::Tensor *q = tensor(a[0], &index), *k = nullptr, *pos = tensor(a[2], &index), *freq = tensor(a[3], &index);
   if (tnd < 0 || !q || !pos || !freq || !current(index)) return nullptr;
   if (a[1] != Py_None && !(k = tensor(a[1], &index))) return nullptr;
+  if (tangent(*q).defined() || (k && tangent(*k).defined())) return nullptr;
   Rotation r;
   bool inplace;
   r.tnd = tnd;

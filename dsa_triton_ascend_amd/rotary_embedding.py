@@ -12,6 +12,7 @@ positions up to 2^31 are exact to fp32 and no table is kept.
 import math
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 
@@ -90,6 +91,8 @@ def _overlaps_itself(t):
 
 def _side(t, start, inplace):
     """Output and C arguments of one rotated tensor [(B,) S, N, D]."""
+    if t._is_zerotensor():  # (a gradient without memory)
+        t = torch.zeros(t.shape, dtype=t.dtype, device=t.device)
     st = t.stride()
     if st[-1] != 1 and t.shape[-1] != 1:  # columns apart
         t = t.contiguous()
@@ -148,7 +151,8 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     Returns ``(query_out, key_out)`` (key_out is None without a key), new
     contiguous tensors, or with ``inplace`` the inputs themselves.  Strided
     views are read as they are if a head's columns are next to each other.
-    Differentiable in query and key, any number of times (not in place).
+    Differentiable in query and key, any number of times, in both modes (not
+    in place; ``inv_freq`` gets no gradient).
     """
     result = _lib.calls().rotate(query, key, positions, inv_freq, interleaved, rotary_offset, key_rotary_offset,
                                  attention_scale, layout, inverse, inplace)
@@ -183,10 +187,11 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     for name, t, start in (("query", query, rotary_offset), ("key", key, key_rotary_offset)):
         if t is not None and (int(start) != start or not 0 <= start <= t.shape[-1] - rot):
             raise ValueError(f"the {rot} rotary columns from {start} do not lie inside the {t.shape[-1]} of {name}")
-    grad = torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))
+    grad = (torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))
+            or any(t is not None and unpack_dual(t).tangent is not None for t in (query, key)))
     if inplace:
         if grad:
-            raise ValueError("inplace is for inference: the inputs require grad")
+            raise ValueError("inplace is for inference: the inputs require grad or carry tangents")
         for name, t in (("query", query), ("key", key)):
             if t is not None and ((t.stride(-1) != 1 and t.shape[-1] != 1) or _overlaps_itself(t)):
                 raise ValueError(f"inplace needs a {name} whose head columns are next to each other and whose "

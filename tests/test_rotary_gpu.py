@@ -263,3 +263,66 @@ def test_frequencies():
     assert yarn[0] == plain[0] and math.isclose(float(yarn[-1] * 40), float(plain[-1]), rel_tol=1e-12)
     assert (yarn <= plain).all() and (yarn * 40 >= plain * (1 - 1e-12)).all()
     assert dsa.rotary_frequencies(64, scaling="yarn", factor=40.0, mscale=0.7, mscale_all_dim=0.7)[1] == 1.0
+
+
+@pytest.mark.parametrize("sides", ["both", "query", "key", "query alone"])
+@pytest.mark.parametrize("compiled", [True, False])
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode(monkeypatch, sides, compiled, requires_grad):
+    """The rotation is linear: a tangent turns as its input does, whether or not
+    a gradient is asked for too, and a gradient's tangent as the gradient."""
+    import torch.autograd.forward_ad as fwad
+
+    import dsa_triton_ascend_amd as dsa
+    from dsa_triton_ascend_amd import _lib
+    if not compiled:
+        monkeypatch.setattr(_lib, "_calls", _lib._NoCalls)
+    pos = torch.randint(0, 9999, (2, 5), device="cuda")
+    inv, _ = dsa.rotary_frequencies(32)
+    args = dict(positions=pos, inv_freq=inv, rotary_offset=16, key_rotary_offset=32, attention_scale=0.75)
+    x, t, up, up_t = ([torch.randn(2, 5, n, 64, device="cuda") for n in (4, 2)] for _ in range(4))
+    with_key = sides != "query alone"
+    has = (sides != "key", sides in ("both", "key"))
+
+    def turn(q, k, **kw):
+        return [o for o in dsa.rotary_embedding(q, k if with_key else None, **args, **kw) if o is not None]
+
+    plain, turned, back, back_t = turn(*x), turn(*t), turn(*up, inverse=True), turn(*up_t, inverse=True)
+    with fwad.dual_level():
+        leaves = [a.clone().requires_grad_(requires_grad) for a in x]
+        ins = [fwad.make_dual(a, b) if h else a for a, b, h in zip(leaves, t, has)]
+        outs = turn(*ins)
+        for i, o in enumerate(outs):
+            got = fwad.unpack_dual(o)
+            assert torch.equal(got.primal, plain[i])
+            if has[i]:
+                assert torch.equal(got.tangent, turned[i])
+            else:
+                assert got.tangent is None or not got.tangent.any()
+        if requires_grad:
+            grads = torch.autograd.grad(outs, ins[:len(outs)], [fwad.make_dual(a, b) for a, b in zip(up, up_t)][:len(outs)])
+            for g, a, b in zip(grads, back, back_t):
+                g = fwad.unpack_dual(g)
+                assert torch.equal(g.primal, a) and torch.equal(g.tangent, b)
+        with torch.no_grad(), pytest.raises(ValueError, match="tangents"):
+            dsa.rotary_embedding(fwad.make_dual(x[0].clone(), t[0]), None, **args, inplace=True)
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_a_gradient_s_tangent_where_the_input_has_none(monkeypatch, compiled):
+    import torch.autograd.forward_ad as fwad
+
+    import dsa_triton_ascend_amd as dsa
+    from dsa_triton_ascend_amd import _lib
+    if not compiled:
+        monkeypatch.setattr(_lib, "_calls", _lib._NoCalls)
+    pos = torch.arange(5, device="cuda")
+    inv, _ = dsa.rotary_frequencies(64)
+    q = torch.randn(1, 5, 2, 64, device="cuda", requires_grad=True)
+    k = torch.randn(1, 5, 1, 64, device="cuda", requires_grad=True)
+    w, t = torch.randn(1, 5, 2, 64, device="cuda"), torch.randn(1, 5, 2, 64, device="cuda")
+    with fwad.dual_level():
+        qo, ko = dsa.rotary_embedding(q, k, pos, inv)
+        g = fwad.unpack_dual(torch.autograd.grad((qo * fwad.make_dual(w, t)).sum(), q)[0])
+    assert torch.equal(g.primal, dsa.rotary_embedding(w, None, pos, inv, inverse=True)[0])
+    assert torch.equal(g.tangent, dsa.rotary_embedding(t, None, pos, inv, inverse=True)[0])
