@@ -9,7 +9,8 @@ import ctypes
 import os
 import warnings
 
-import torch  # noqa: F401  (must be loaded before the HIP library)
+import torch  # (must be loaded before the HIP library)
+from torch.autograd.forward_ad import unpack_dual
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DSA_HIP_LIB", os.path.join(_PKG, "libdsa_hip.so"))
@@ -314,6 +315,14 @@ def same_device(first, *others):
                 raise ValueError("this operator requires tensors on a ROCm GPU device (it has no CPU path)")
             raise ValueError("all tensors must be on the same device")
     return index
+
+
+def no_derivatives(what, *tensors):
+    """ValueError where a derivative of one of the tensors would be lost."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError(f"{what} has no backward: call it under torch.no_grad()")
+    if any(unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} has no forward-mode derivative, but its inputs carry tangents")
 
 
 def dtype_code(dt):

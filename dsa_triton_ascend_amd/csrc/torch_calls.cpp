@@ -83,6 +83,11 @@ const at::Tensor* tensor(PyObject* o, int* index) {
 // the tangent of a dual tensor (forward-mode derivatives), else undefined
 const at::Tensor& tangent(const at::Tensor& t) { return t._fw_grad(/*level=*/0); }
 
+// whether a derivative would be lost in an operator that has none
+bool differentiable(const at::Tensor& t) {
+  return (t.requires_grad() && c10::GradMode::is_enabled()) || tangent(t).defined();
+}
+
 const at::Tensor* ints(PyObject* o, int* index, int64_t dim) {
   const at::Tensor* t = tensor(o, index);
   return t && t->scalar_type() == at::kInt && t->dim() == dim && t->numel() > 0 && t->is_contiguous() ? t : nullptr;
@@ -146,7 +151,7 @@ struct Caches {
       const at::Tensor* c = tensor(list[i], index);
       if (!c || c->dim() < 3 || !c->is_contiguous() || c->numel() == 0) return false;
       if (i == 0) pages = c->size(0), page = c->size(1);
-      if (c->size(0) != pages || c->size(1) != page) return false;
+      if (c->size(0) != pages || c->size(1) != page || differentiable(*c)) return false;
       t.push_back(c);
       at.push_back(c->data_ptr());
       row_bytes.push_back(c->numel() / (pages * page) * (int64_t)c->element_size());
@@ -185,7 +190,7 @@ PyObject* write(PyObject* const* a) {
   for (int64_t i = 0; i < n; ++i) {
     const at::Tensor* r = tensor(list[i], &index);
     const at::Tensor& k = *c.t[i];
-    if (!r || r->dim() != lead + k.dim() - 2 || r->scalar_type() != k.scalar_type()) return nullptr;
+    if (!r || r->dim() != lead + k.dim() - 2 || r->scalar_type() != k.scalar_type() || differentiable(*r)) return nullptr;
     if (i == 0) t0 = r->size(0), t1 = tnd ? 1 : r->size(1);
     if (r->size(0) != t0 || (!tnd && (r->size(1) != t1 || t0 != batch))) return nullptr;
     int64_t step = 1;
@@ -286,7 +291,7 @@ PyObject* attention(PyObject* const* a) {
     return nullptr;
   const auto kind = q->scalar_type();
   auto cache = [&](const at::Tensor* t) {
-    return t && t->scalar_type() == kind && t->is_contiguous() && t->numel() > 0 && !t->requires_grad();
+    return t && t->scalar_type() == kind && t->is_contiguous() && t->numel() > 0 && !differentiable(*t);
   };
   if ((kind != at::kBFloat16 && kind != at::kHalf) || !cache(q) || !cache(k)) return nullptr;
   const int64_t b = q->size(0), s1 = q->size(1), n1 = q->size(2), d = q->size(3);

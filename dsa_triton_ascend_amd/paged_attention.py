@@ -95,8 +95,7 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
         raise ValueError("block_table and actual_seq_lengths_kv are required")
     if block_table.dim() != 2 or block_table.shape[0] < B:
         raise ValueError(f"block_table must be [B, max_blocks] with B={B} rows, got {tuple(block_table.shape)}")
-    if torch.is_grad_enabled() and (query.requires_grad or any(t.requires_grad for _, t in others)):
-        raise ValueError("paged_attention has no backward: call it under torch.no_grad()")
+    _lib.no_derivatives("paged_attention", query, *(t for _, t in others))
     index = _lib.same_device(query, key, value, query_rope, key_rope, block_table)
     dev = query.device
     act_k = _lengths(actual_seq_lengths_kv, dev)

@@ -12,7 +12,8 @@ lengths ``[B]`` and ``page_refs [pages]``, how often each page is referred to
 in ``page_refs``.  Everything is decided on the device from these tensors,
 without reading them on the host; the functions return new ones and leave the
 given ones as they are, so a call can be captured and replayed.  The caches
-are changed in place.
+are changed in place.  None of the functions has derivatives: caches and rows
+that require grad are refused outside ``torch.no_grad()``.
 
 One decoding step:
 
@@ -149,6 +150,7 @@ def paged_cache_write(caches, rows, block_table, seq_lengths, row_lengths=None, 
         sources.append(r.data_ptr())
         sb.append(stride[0] * es if lead == 2 else 0)
         st.append(stride[lead - 1] * es)
+    _lib.no_derivatives("paged_cache_write", *caches, *rows)
     index = _lib.same_device(table, lens, row_lengths, *caches, *kept)
     n_tok = tokens[0] if lead == 1 else tokens[0] * tokens[1]
     if n_tok == 0:
@@ -207,6 +209,7 @@ def paged_cache_fork(caches, block_table, seq_lengths, page_refs, parents=None, 
         children = parents.shape[0]
     if int(new_tokens) != new_tokens or not 0 <= new_tokens < 2 ** 31:
         raise ValueError(f"new_tokens must be an integer in [0, 2^31), got {new_tokens}")
+    _lib.no_derivatives("paged_cache_fork", *caches)
     index = _lib.same_device(table, lens, refs, parents, *caches)
     new_table = table.new_empty((children, wide))
     new_lens = lens.new_empty(children)
@@ -246,6 +249,7 @@ def paged_cache_compact(caches, block_table, page_refs, page_size=None):
         raise ValueError(f"page_size ({page_size}) must equal the caches' ({page})")
     table = _ints(block_table, "block_table", 2)
     rows, wide = table.shape
+    _lib.no_derivatives("paged_cache_compact", *caches)
     index = _lib.same_device(table, refs, *caches)
     new_table, new_refs, page_map = torch.empty_like(table), torch.empty_like(refs), torch.empty_like(refs)
     lib = _lib.load()

@@ -324,3 +324,42 @@ def test_caches_that_overlap_are_refused():
     rows = [torch.zeros(2, 3, 1, 8, dtype=BF)] * 2
     with pytest.raises(ValueError, match="overlap"):
         _write(caches=[pool[3:8], pool[0:5]], rows=rows)
+
+
+# ---- derivatives ----
+
+@pytest.mark.parametrize("which", ["caches", "rows"])
+def test_write_refuses_what_requires_grad(which):
+    c, r = torch.zeros(5, 4, 1, 8), torch.zeros(2, 3, 1, 8)
+    a = dict(caches=[c, c.clone()], rows=[r, r.clone()])
+    a[which][1].requires_grad_()
+    with pytest.raises(ValueError, match="paged_cache_write has no backward"):
+        _write(**a)
+    with torch.no_grad(), pytest.raises(ValueError, match="ROCm GPU device"):
+        _write(**a)
+
+
+def test_fork_and_compact_refuse_caches_that_require_grad():
+    c = torch.zeros(5, 4, 1, 8, requires_grad=True)
+    for f in (lambda: dsa.paged_cache_fork([c], _i(2, 3), _i(2), _i(5)),
+              lambda: dsa.paged_cache_compact([c * 2], _i(2, 3), _i(5))):
+        with pytest.raises(ValueError, match="has no backward"):
+            f()
+        with torch.no_grad(), pytest.raises(ValueError, match="ROCm GPU device"):
+            f()
+
+
+def test_operators_without_derivatives_refuse_tangents():
+    import torch.autograd.forward_ad as fwad
+    with fwad.dual_level(), torch.no_grad():
+        def dual(*shape, dtype=torch.float32):
+            return fwad.make_dual(torch.zeros(*shape, dtype=dtype), torch.ones(*shape, dtype=dtype))
+
+        for f in (lambda: _write(caches=[torch.zeros(5, 4, 1, 8)], rows=[dual(2, 3, 1, 8)]),
+                  lambda: _write(caches=[dual(5, 4, 1, 8)], rows=[torch.zeros(2, 3, 1, 8)]),
+                  lambda: dsa.paged_cache_fork([dual(5, 4, 1, 8)], _i(2, 3), _i(2), _i(5)),
+                  lambda: dsa.paged_cache_compact([dual(5, 4, 1, 8)], _i(2, 3), _i(5)),
+                  lambda: _attn(query=dual(2, 1, 8, 128, dtype=BF)),
+                  lambda: _attn(latent=True, key_rope=dual(5, 4, 1, 64, dtype=BF))):
+            with pytest.raises(ValueError, match="tangents"):
+                f()

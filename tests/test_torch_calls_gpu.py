@@ -275,3 +275,32 @@ def test_an_error_left_behind_is_raised_and_no_rotation_made_twice(monkeypatch, 
         hip.hipGetLastError()
     assert torch.equal(x, once)
     assert torch.equal(dsa.rotary_embedding(q, None, pos, inv)[0], once)  # and the next call is an ordinary one
+
+
+def test_derivatives_are_left_to_python():
+    """Where a derivative would be lost the module takes no call; under no_grad it does."""
+    import torch.autograd.forward_ad as fwad
+
+    from dsa_triton_ascend_amd import _lib
+    c = _lib.calls()
+    caches, table, lens, refs = _state()
+    rows = [torch.randn(2, 4, 1, 64, device="cuda").bfloat16() for _ in range(2)]
+    q = torch.randn(2, 1, 8, 64, device="cuda").bfloat16()
+    inf = 2 ** 63 - 1
+
+    def calls(caches, rows, q):
+        return [c.write(caches, rows, table, lens, None, "BSND"), c.fork(caches, table, lens, refs, None, 1, None),
+                c.compact(caches, table, refs, None),
+                c.attention(q, caches[0], caches[1], table, lens, 0.1, None, None, None, 3, inf, inf, False)]
+
+    assert all(x is not None for x in calls(caches, rows, q))
+    leaf = [caches[0], caches[1].clone().requires_grad_()]
+    assert all(x is None for x in calls(leaf, rows, q))
+    assert calls(caches, [rows[0], rows[1].clone().requires_grad_()], q)[0] is None
+    assert calls(caches, rows, q.clone().requires_grad_())[3] is None
+    with torch.no_grad():
+        assert all(x is not None for x in calls(leaf, [r.clone().requires_grad_() for r in rows], q.clone().requires_grad_()))
+    with fwad.dual_level():
+        assert all(x is None for x in calls([caches[0], fwad.make_dual(caches[1], caches[0])], rows, q))
+        assert calls(caches, [fwad.make_dual(rows[0], rows[1]), rows[1]], q)[0] is None
+        assert calls(caches, rows, fwad.make_dual(q, q.clone()))[3] is None
