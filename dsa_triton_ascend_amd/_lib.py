@@ -317,6 +317,12 @@ def same_device(first, *others):
     return index
 
 
+def changed(*tensors):
+    """Tells autograd that the tensors were changed in place: a backward that
+    saved one of them raises instead of using the new values."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def no_derivatives(what, *tensors):
     """ValueError where a derivative of one of the tensors would be lost."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):

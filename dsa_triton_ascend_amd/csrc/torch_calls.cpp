@@ -165,6 +165,16 @@ struct Caches {
   }
 };
 
+// Tells autograd that a tensor was changed in place: a backward that saved it
+// raises instead of using the new values.  (Inference tensors are not saved.)
+// Before the call: while it runs, another thread may drop the caller's tensors.
+void changed(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void changed(const Caches& c) {
+  for (const at::Tensor* t : c.t) changed(*t);
+}
+
 bool current(int index) { return index >= 0 && c10::hip::current_device() == index; }
 void* stream_of(int index) { return c10::hip::getCurrentHIPStream((c10::DeviceIndex)index).stream(); }
 const int32_t* data(const at::Tensor* t) { return t ? (const int32_t*)t->data_ptr() : nullptr; }
@@ -204,6 +214,7 @@ PyObject* write(PyObject* const* a) {
     st[i] = r->stride(lead - 1) * es;
   }
   if (t0 * t1 == 0) return nullptr;
+  changed(c);
   if (!launched(entry.write, n, src.data(), c.at.data(), c.row_bytes.data(), sb.data(), st.data(), data(table), data(lens),
                   data(counts), batch, tnd ? 0 : t1, t0 * t1, table->size(1), c.pages, c.page,
                   tnd ? DSA_LAYOUT_TND : DSA_LAYOUT_BSND, stream_of(index)))
@@ -247,6 +258,7 @@ PyObject* fork(PyObject* const* a) {
   at::Tensor new_refs = fresh({c.pages}, *table);
   const size_t bytes = entry.fork_bytes(rows, children, c.pages);
   c10::DataPtr ws = workspace(bytes);
+  changed(c);
   if (!launched(entry.fork, (int64_t)c.t.size(), c.at.data(), c.row_bytes.data(), data(table), data(lens), data(refs),
                  data(parents), (int32_t*)new_table.data_ptr(), (int32_t*)new_lens.data_ptr(),
                  (int32_t*)new_refs.data_ptr(), rows, children, wide, wide, c.pages, c.page, more, ws.get(),
@@ -268,6 +280,7 @@ PyObject* compact(PyObject* const* a) {
   at::Tensor map = fresh({c.pages}, *table);
   const size_t bytes = entry.compact_bytes(c.pages);
   c10::DataPtr ws = workspace(bytes);
+  changed(c);
   if (!launched(entry.compact, (int64_t)c.t.size(), c.at.data(), c.row_bytes.data(), data(table), data(refs),
                     (int32_t*)new_table.data_ptr(), (int32_t*)new_refs.data_ptr(), (int32_t*)map.data_ptr(),
                     table->size(0), table->size(1), c.pages, c.page, ws.get(), bytes, stream_of(index)))
@@ -485,7 +498,7 @@ PyObject* rotate(PyObject* const* a) {
     return nullptr;
   if (inplace)
     for (auto& t : out)
-      if (t.defined()) t.unsafeGetTensorImpl()->bump_version();
+      if (t.defined()) changed(t);
   PyObject* pair = PyTuple_New(2);
   if (!pair) return nullptr;
   PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out[0])));

@@ -162,6 +162,7 @@ def paged_cache_write(caches, rows, block_table, seq_lengths, row_lengths=None, 
         0 if lead == 1 else tokens[1], n_tok, wide, pages, page, 2 - lead, _lib.raw_stream(index))
     if status:
         _lib.check(status, "dsa_paged_cache_write")
+    _lib.changed(*caches)
 
 
 def paged_cache_fork(caches, block_table, seq_lengths, page_refs, parents=None, new_tokens=0, page_size=None):
@@ -225,6 +226,7 @@ def paged_cache_fork(caches, block_table, seq_lengths, page_refs, parents=None, 
         _lib.raw_stream(index))
     if status:
         _lib.check(status, "dsa_paged_cache_fork")
+    _lib.changed(*caches)
     return new_table, new_lens, new_refs
 
 
@@ -262,4 +264,5 @@ def paged_cache_compact(caches, block_table, page_refs, page_size=None):
         1 if page is None else page, ws.data_ptr(), nbytes, _lib.raw_stream(index))
     if status:
         _lib.check(status, "dsa_paged_cache_compact")
+    _lib.changed(*caches)
     return new_table, new_refs, page_map

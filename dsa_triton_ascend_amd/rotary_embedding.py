@@ -130,7 +130,7 @@ def _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scal
     if status:
         _lib.check(status, "dsa_rope")
     if inplace:
-        torch.autograd.graph.increment_version([t for t in (q_out, k_out) if t is not None])
+        _lib.changed(*(t for t in (q_out, k_out) if t is not None))
     return q_out, k_out
 
 

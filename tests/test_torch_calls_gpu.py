@@ -304,3 +304,32 @@ def test_derivatives_are_left_to_python():
         assert all(x is None for x in calls([caches[0], fwad.make_dual(caches[1], caches[0])], rows, q))
         assert calls(caches, [fwad.make_dual(rows[0], rows[1]), rows[1]], q)[0] is None
         assert calls(caches, rows, fwad.make_dual(q, q.clone()))[3] is None
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_caches_are_marked_as_changed(monkeypatch, compiled):
+    """A backward that saved a cache before a write, a fork or a compaction
+    raises, as after torch's own operations in place."""
+    import dsa_triton_ascend_amd as dsa
+    from dsa_triton_ascend_amd import _lib
+    if not compiled:
+        monkeypatch.setattr(_lib, "_calls", _lib._NoCalls)
+    caches, table, lens, refs = _state(dtype=torch.float32)
+    rows = [torch.randn(2, 4, 1, 64, device="cuda") for _ in range(2)]
+    w = torch.randn(64, device="cuda", requires_grad=True)
+    for change in (lambda c: dsa.paged_cache_write(c, rows, table, lens),
+                   lambda c: dsa.paged_cache_fork(c, table, lens, refs, new_tokens=1),
+                   lambda c: dsa.paged_cache_compact(c, table, refs)):
+        loss = (caches[1] * w).sum()
+        before = [c._version for c in caches]
+        change(caches)
+        assert [c._version for c in caches] == [v + 1 for v in before]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with torch.inference_mode():
+            mine = [c.clone() for c in caches]
+        change(mine)  # tensors without a version
+    views = [caches[0][:9], caches[1][:9]]
+    before = caches[0]._version
+    dsa.paged_cache_write(views, rows, table, lens)
+    assert caches[0]._version == before + 1
