@@ -349,6 +349,50 @@ bool overlaps_itself(const at::Tensor& t) {
   return false;
 }
 
+// Whether a sum of strides, each as often as its range allows, lies in
+// [from, to].  Strides descend, so that what the later ones reach leaves each
+// of them a few counts; true where those would be too many to go through.
+struct Step {
+  int64_t stride, lo, hi;
+};
+bool reaches(const std::vector<Step>& steps, size_t k, int64_t from, int64_t to, int* budget) {
+  if (k == steps.size()) return from <= 0 && 0 <= to;
+  int64_t least = 0, most = 0;
+  for (size_t i = k + 1; i < steps.size(); ++i) {
+    least += steps[i].stride * steps[i].lo;
+    most += steps[i].stride * steps[i].hi;
+  }
+  const Step& s = steps[k];
+  auto floor_div = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };
+  const int64_t x0 = std::max(s.lo, -floor_div(most - from, s.stride)), x1 = std::min(s.hi, floor_div(to - least, s.stride));
+  for (int64_t x = x0; x <= x1; ++x)
+    if (--*budget < 0 || reaches(steps, k + 1, from - x * s.stride, to - x * s.stride, budget)) return true;
+  return false;
+}
+
+// whether the `cols` columns from start[0] of a's heads and those from
+// start[1] of b's share memory
+bool share_memory(const at::Tensor& a, const at::Tensor& b, const int64_t start[2], int64_t cols) {
+  const int64_t es = (int64_t)a.element_size(), size = cols * es;
+  std::vector<Step> steps;
+  auto add = [&](int64_t stride, int64_t lo, int64_t hi) {
+    if (lo == hi) return;
+    for (Step& s : steps)
+      if (s.stride == stride) {
+        s.lo += lo, s.hi += hi;
+        return;
+      }
+    steps.push_back({stride, lo, hi});
+  };
+  for (int64_t i = 0; i + 1 < a.dim(); ++i) add(a.stride(i) * es, 1 - a.size(i), 0);
+  for (int64_t i = 0; i + 1 < b.dim(); ++i) add(b.stride(i) * es, 0, b.size(i) - 1);
+  std::sort(steps.begin(), steps.end(), [](const Step& x, const Step& y) { return x.stride > y.stride; });
+  // b's columns lie this far behind a's, and a sum of steps more
+  const int64_t apart = ((char*)b.data_ptr() + start[1] * es) - ((char*)a.data_ptr() + start[0] * es);
+  int budget = 1000;
+  return reaches(steps, 0, -apart - size + 1, -apart + size - 1, &budget);
+}
+
 struct Rotation {
   int64_t start[2];  // of the query's and the key's rotated columns
   double scale;
@@ -388,7 +432,7 @@ bool rotated(const Rotation& r, const at::Tensor in[2], const at::Tensor& pos, c
     }
     from[i] = t.data_ptr(), to[i] = out[i].data_ptr();
   }
-  if (inplace && from[0] == from[1]) return false;
+  if (inplace && in[1].defined() && (from[0] == from[1] || share_memory(q, in[1], r.start, rot))) return false;
   const int64_t b = r.tnd ? 1 : q.size(0), s = q.size(lead - 1);
   const bool full = pos.dim() == lead && (r.tnd || pos.size(0) == b) && pos.size(lead - 1) == s;
   const bool shared = !r.tnd && pos.dim() == 1 && pos.size(0) == s;

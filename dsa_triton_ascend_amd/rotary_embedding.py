@@ -89,6 +89,36 @@ def _overlaps_itself(t):
     return False
 
 
+def _share_memory(a, a_start, b, b_start, cols):
+    """Whether the columns a_start .. a_start + cols of a's heads and b_start ..
+    of b's share memory (both checked by ``_overlaps_itself``)."""
+    size = a.element_size()
+    counts = {}  # how often each stride may be taken
+    for n, s in zip(a.shape[:-1], a.stride()):
+        lo, hi = counts.get(s * size, (0, 0))
+        counts[s * size] = lo - (n - 1), hi
+    for n, s in zip(b.shape[:-1], b.stride()):
+        lo, hi = counts.get(s * size, (0, 0))
+        counts[s * size] = lo, hi + (n - 1)
+    steps = sorted(((s, lo, hi) for s, (lo, hi) in counts.items() if lo != hi), reverse=True)
+    budget = 1000  # descending strides leave each a few counts; if not, the answer is yes
+
+    def reaches(k, first, last):
+        nonlocal budget
+        if k == len(steps):
+            return first <= 0 <= last
+        s, lo, hi = steps[k]
+        least, most = (sum(x[0] * x[i] for x in steps[k + 1:]) for i in (1, 2))
+        for x in range(max(lo, -((most - first) // s)), min(hi, (last - least) // s) + 1):
+            budget -= 1
+            if budget < 0 or reaches(k + 1, first - x * s, last - x * s):
+                return True
+        return False
+
+    apart = b.data_ptr() + b_start * size - a.data_ptr() - a_start * size
+    return reaches(0, -apart - cols * size + 1, -apart + cols * size - 1)
+
+
 def _side(t, start, inplace):
     """Output and C arguments of one rotated tensor [(B,) S, N, D]."""
     if t._is_zerotensor():  # (a gradient without memory)
@@ -149,7 +179,8 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     by the opposite angles.
 
     Returns ``(query_out, key_out)`` (key_out is None without a key), new
-    contiguous tensors, or with ``inplace`` the inputs themselves.  Strided
+    contiguous tensors, or with ``inplace`` the inputs themselves (views of one
+    projection too, if their rotated columns share no memory).  Strided
     views are read as they are if a head's columns are next to each other.
     Differentiable in query and key, any number of times, in both modes (not
     in place; ``inv_freq`` gets no gradient).
@@ -196,8 +227,10 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
             if t is not None and ((t.stride(-1) != 1 and t.shape[-1] != 1) or _overlaps_itself(t)):
                 raise ValueError(f"inplace needs a {name} whose head columns are next to each other and whose "
                                  "elements do not share memory")
-        if key is not None and key.numel() and query.numel() and key.data_ptr() == query.data_ptr():
-            raise ValueError("inplace needs a key and a query of their own")
+        if key is not None and key.numel() and query.numel() and (
+                key.data_ptr() == query.data_ptr()
+                or _share_memory(query, rotary_offset, key, key_rotary_offset, rot)):
+            raise ValueError("inplace needs a key and a query of their own: they share memory")
     _lib.same_device(query, key, positions, inv_freq)
     if not positions.is_contiguous():
         positions = positions.contiguous()

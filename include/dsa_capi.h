@@ -410,7 +410,7 @@ int dsa_li_scores_paged(const void* query, const void* key_cache, const void* we
  * element strides sb / ss / sh (batch, token, head; a packed [T, heads, d]
  * has batch 1 and s1 = T) and columns next to each other, likewise key and
  * the outputs.  An output is its input exactly, with the same strides, or
- * does not overlap it.  positions: int32, or int64 (positions_64), one per token of
+ * overlaps neither input; the outputs' rotated columns share no memory.  positions: int32, or int64 (positions_64), one per token of
  * every sequence (positions_per_sequence: [B, S1]) or shared by all ([S1]);
  * inv_freq: rotary_dim / 2 doubles on the device.  Angles are formed in 64
  * bits.  dtype BF16, FP16 or FP32; rotary_dim even, up to 1024.

@@ -363,3 +363,54 @@ def test_operators_without_derivatives_refuse_tangents():
                   lambda: _attn(latent=True, key_rope=dual(5, 4, 1, 64, dtype=BF))):
             with pytest.raises(ValueError, match="tangents"):
                 f()
+
+
+# ---- in place: query and key in one piece of memory ----
+
+def _views(rng, flat):
+    """A query and a key as strided views of one buffer, often apart, often not:
+    (query, its rotated columns' start, key, start, columns)."""
+    B, S, cols = rng.randint(1, 3), rng.randint(1, 4), 2 * rng.randint(1, 3)
+    heads = [rng.randint(1, 3), rng.randint(1, 3)]
+    pitch = rng.choice([cols, cols + 1, 2 * cols, 3 * cols])
+    row = rng.choice([sum(heads) * pitch, (sum(heads) + 2) * pitch, max(heads) * pitch])
+    seq = rng.choice([S * row, S * row + 3, (S + 1) * row])
+    out = []
+    for h, at in zip(heads, (rng.randint(0, 5), rng.choice([heads[0] * pitch, rng.randint(0, 4 * row), B * seq]))):
+        d = rng.randint(cols, pitch)
+        step = (seq, row) if rng.random() < 0.7 else (row, B * row)
+        t = torch.as_strided(flat, (B, S, h, d), (*step, pitch, 1), at)
+        out += [t, rng.randint(0, d - cols)]
+    return (*out, cols)
+
+
+def _shared(q, qs, k, ks, cols):
+    at = torch.arange(1 << 14)
+    a, b = (torch.as_strided(at, (*t.shape[:-1], cols), t.stride(), t.storage_offset() + s) for t, s in ((q, qs), (k, ks)))
+    return bool(set(a.flatten().tolist()) & set(b.flatten().tolist()))
+
+
+def test_views_that_share_memory_are_told_from_those_that_do_not():
+    import random
+
+    from dsa_triton_ascend_amd.rotary_embedding import _overlaps_itself, _share_memory
+    rng, flat, seen = random.Random(0), torch.zeros(1 << 14), [0, 0]
+    for _ in range(3000):
+        q, qs, k, ks, cols = _views(rng, flat)
+        if not _overlaps_itself(q) and not _overlaps_itself(k):
+            want = _shared(q, qs, k, ks, cols)
+            assert _share_memory(q, qs, k, ks, cols) == want, (q.shape, q.stride(), qs, k.shape, k.stride(), ks, cols)
+            seen[want] += 1
+    assert min(seen) > 300, seen
+
+
+def test_rotary_in_place_refuses_views_that_share_columns():
+    proj = torch.zeros(2, 3, 6, 64, dtype=BF)
+    with pytest.raises(ValueError, match="share memory"):
+        _rope(query=proj[:, :, :4], key=proj[:, :, 3:], inplace=True)
+    with pytest.raises(ValueError, match="share memory"):  # columns 32 .. 63 of one, 24 .. 55 of the other
+        _rope(query=proj[:, :, :4], key=proj[..., 8:][:, :, :1], rotary_offset=32, key_rotary_offset=16, inplace=True)
+    for q, k in ((proj[:, :, :4], proj[:, :, 4:]),          # heads of their own
+                 (proj[..., :40], proj[:, :, :1, 32:])):    # columns 0 .. 31 and 32 .. 63
+        with pytest.raises(ValueError, match="ROCm GPU device"):
+            _rope(query=q, key=k, inplace=True)

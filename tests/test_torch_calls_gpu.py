@@ -333,3 +333,36 @@ def test_caches_are_marked_as_changed(monkeypatch, compiled):
     before = caches[0]._version
     dsa.paged_cache_write(views, rows, table, lens)
     assert caches[0]._version == before + 1
+
+
+def test_in_place_views_of_one_buffer():
+    """The module takes what shares no columns, and no other."""
+    import random
+
+    from test_decode_ops_validation import _shared, _views
+
+    import dsa_triton_ascend_amd as dsa
+    from dsa_triton_ascend_amd import _lib
+    from dsa_triton_ascend_amd.rotary_embedding import _overlaps_itself
+    rng, taken = random.Random(1), [0, 0]
+    start = torch.randn(1 << 14, device="cuda")
+    for _ in range(400):
+        flat = start.clone()
+        q, qs, k, ks, cols = _views(rng, flat)
+        if _overlaps_itself(q) or _overlaps_itself(k):
+            continue
+        pos = torch.randint(0, 99, q.shape[:2], device="cuda")
+        inv, _ = dsa.rotary_frequencies(cols)
+        shared = _shared(q, qs, k, ks, cols) or q.data_ptr() == k.data_ptr()
+        want = dsa.rotary_embedding(q, k, pos, inv, rotary_offset=qs, key_rotary_offset=ks)
+        got = _lib.calls().rotate(q, k, pos, inv, False, qs, ks, 1.0, "BSND", False, True)
+        assert (got is None) == shared
+        if shared:
+            with pytest.raises(ValueError, match="share memory"):
+                dsa.rotary_embedding(q, k, pos, inv, rotary_offset=qs, key_rotary_offset=ks, inplace=True)
+            assert torch.equal(flat, start)
+        else:
+            for a, b, s in zip((q, k), want, (qs, ks)):
+                assert torch.equal(a[..., s:s + cols], b[..., s:s + cols])
+        taken[shared] += 1
+    assert min(taken) > 40, taken
