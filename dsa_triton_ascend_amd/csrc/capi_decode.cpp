@@ -25,6 +25,8 @@ int pc_compact_run(int64_t n, void* const* caches, const int64_t* row_bytes, con
                    const int32_t* refs, int32_t* new_table, int32_t* new_refs, int32_t* page_map, int64_t entries,
                    int64_t pages, int64_t page, void* workspace, hipStream_t stream);
 // paged_attn.hip
+bool paged_attn_launchable(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
+                           int64_t max_blocks, int64_t page);
 size_t paged_attn_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
                                   int64_t max_blocks, int64_t page);
 int paged_attn_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
@@ -76,7 +78,8 @@ static bool paged_attn_sizes_ok(int64_t batch, int64_t s1, int64_t n1, int64_t n
          within(s1, n1, 1ll << 24) && within(batch * s1, n1, (1ll << 31) - 1) &&
          (latent ? n2 == 1 && (d == 128 || d == 256 || d == 512) : d == 64 || d == 128 || d == 256) &&
          page >= 1 && page <= (1 << 20) && max_blocks >= 1 && max_blocks <= (1 << 20) &&
-         within(max_blocks, page, 65535ll * 1024) && within(batch, max_blocks * page, kMaxTableTokens);
+         within(max_blocks, page, 65535ll * 1024) && within(batch, max_blocks * page, kMaxTableTokens) &&
+         paged_attn_launchable(batch, s1, n1, n2, d, latent, max_blocks, page);
 }
 
 }  // namespace dsa
@@ -248,6 +251,8 @@ int dsa_paged_attn(const void* query, const void* query_rope, const void* key, c
   if (st != DSA_OK) return st;
   DSA_CHECK_SUPPORTED(within(batch, max_blocks * page_size, kMaxTableTokens),
                       "batch * max_blocks * page size must be <= 2^35");
+  DSA_CHECK_SUPPORTED(paged_attn_launchable(batch, s1, n1, n2, d, latent, max_blocks, page_size),
+                      "too many query rows for one launch");
   // 16-byte loads of rows
   DSA_CHECK_ARG((((uintptr_t)query | (uintptr_t)key | (uintptr_t)value | (uintptr_t)query_rope | (uintptr_t)key_rope |
                   (uintptr_t)attention_out) & 15) == 0, "tensors must be 16-byte aligned");

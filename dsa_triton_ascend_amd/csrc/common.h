@@ -166,6 +166,9 @@ namespace dsa {
 void set_error(const char* fmt, ...);
 void clear_error();
 int hip_fail(hipError_t e, const char* what);
+// whether HIP launches that many blocks of so many threads: the threads of a
+// launch are counted in 32 bits
+inline bool launchable(int64_t blocks, int threads) { return blocks >= 0 && blocks <= 0xffffffffll / threads; }
 // CUs of the current device (cached per device; 256 when it cannot be queried)
 int device_cu_count();
 // Test hooks set by dsa_set_test_flags (0 in normal use).

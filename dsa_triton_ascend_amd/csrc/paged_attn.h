@@ -226,6 +226,7 @@ size_t paged_part_bytes(const PagedShape& s, int64_t d);
 int paged_workers(int64_t slots, int64_t groups, int64_t batch, int64_t tiles, int min_tiles);
 int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream);
 PagedShape paged_latent_shape(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t max_blocks, int64_t page);
+bool paged_latent_launchable(int64_t workers, int64_t row_groups);
 int paged_latent_launch(const PagedAttnParams& p, int64_t d, int32_t dtype, hipStream_t stream);
 
 }  // namespace dsa

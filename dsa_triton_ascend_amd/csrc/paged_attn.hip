@@ -409,11 +409,17 @@ static void paged_combine_d(const PagedAttnParams& p, int tile, int wg_rows, int
   else paged_combine_kernel<T, 512><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
 }
 
+// rows of a workgroup of the join: four, one per wave, unless the average
+// sequence has so many runs that the waves had better share them
+static int paged_combine_rows(int64_t workers, int64_t batch) { return workers > 32 * batch ? 1 : 4; }
+static int64_t paged_combine_grid(int64_t workers, int64_t batch, int64_t s1, int64_t n1) {
+  const int wg_rows = paged_combine_rows(workers, batch);
+  return batch * ((s1 * n1 + wg_rows - 1) / wg_rows);
+}
+
 int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream) {
-  // rows of a workgroup: four, one per wave, unless the average sequence has
-  // so many runs that the waves had better share them
-  const int wg_rows = p.workers > 32ll * p.batch ? 1 : 4;
-  const unsigned grid = (unsigned)(p.batch * (((int64_t)p.n2 * p.rows + wg_rows - 1) / wg_rows));
+  const int wg_rows = paged_combine_rows(p.workers, p.batch);
+  const unsigned grid = (unsigned)paged_combine_grid(p.workers, p.batch, p.s1, p.n1);
   if (dtype == DSA_DTYPE_BF16) paged_combine_d<bf16>(p, tile, wg_rows, d, grid, stream);
   else paged_combine_d<f16>(p, tile, wg_rows, d, grid, stream);
   DSA_HIP(hipGetLastError());
@@ -464,6 +470,18 @@ static PagedShape paged_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2,
                               int64_t max_blocks, int64_t page) {
   return latent ? paged_latent_shape(batch, s1, n1, d, max_blocks, page)
                 : paged_grouped_shape(batch, s1, n1, n2, d, max_blocks, page);
+}
+
+static int64_t paged_grouped_grid(int64_t workers, int64_t groups) {
+  return (workers * groups + kPaThreads / 64 - 1) / (kPaThreads / 64);
+}
+
+bool paged_attn_launchable(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
+                           int64_t max_blocks, int64_t page) {
+  const PagedShape s = paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
+  return (latent ? paged_latent_launchable(s.workers, s.row_groups)
+                 : launchable(paged_grouped_grid(s.workers, s.groups), kPaThreads)) &&
+         launchable(paged_combine_grid(s.workers, batch, s1, n1), 256);
 }
 
 size_t paged_attn_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
@@ -538,8 +556,7 @@ int paged_attn_run(const void* query, const void* query_rope, const void* key, c
     const int st = paged_latent_launch(p, d, dtype, stream);
     if (st != DSA_OK) return st;
   } else {
-    const int64_t waves = (int64_t)s.workers * s.groups;
-    const unsigned grid = (unsigned)((waves + kPaThreads / 64 - 1) / (kPaThreads / 64));
+    const unsigned grid = (unsigned)paged_grouped_grid(s.workers, s.groups);
     // K and V that the caches could hold until the next call are kept there
     // (134 MB: 38 us, streaming 41; 537 MB: 115 us, streaming 104)
     const int64_t tokens = p.kv_rows < batch * max_blocks * page ? p.kv_rows : batch * max_blocks * page;

@@ -633,8 +633,13 @@ static void paged_latent_d(const PagedAttnParams& p, int64_t d, unsigned grid, h
   else paged_latent_hg<512, T, false>(p, grid, stream);
 }
 
+static int64_t paged_latent_grid(int64_t workers, int64_t row_groups) { return 8 * ((workers + 7) / 8) * row_groups; }
+bool paged_latent_launchable(int64_t workers, int64_t row_groups) {
+  return launchable(paged_latent_grid(workers, row_groups), kPlThreads);
+}
+
 int paged_latent_launch(const PagedAttnParams& p, int64_t d, int32_t dtype, hipStream_t stream) {
-  const unsigned grid = (unsigned)(8ll * ((p.workers + 7) / 8) * p.row_groups);
+  const unsigned grid = (unsigned)paged_latent_grid(p.workers, p.row_groups);
   if (dtype == DSA_DTYPE_BF16) paged_latent_d<bf16>(p, d, grid, stream);
   else paged_latent_d<f16>(p, d, grid, stream);
   DSA_HIP(hipGetLastError());

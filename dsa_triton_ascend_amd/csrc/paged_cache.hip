@@ -105,8 +105,19 @@ int pc_write_run(int64_t n, const void* const* rows, void* const* caches, const 
                  const int64_t* row_sb, const int64_t* row_st, const int32_t* table, const int32_t* lens,
                  const int32_t* row_lengths, int64_t batch, int64_t s, int64_t tokens, int64_t max_blocks,
                  int64_t pages, int64_t page, int32_t layout, hipStream_t stream) {
-  for (int64_t c0 = 0; c0 < n; c0 += kPcMaxCaches) {
-    PcWriteParams p = {};
+  PcWriteParams p = {};
+  p.table = table;
+  p.lens = lens;
+  p.rows = row_lengths;
+  p.tokens = tokens;
+  p.pages = pages;
+  p.batch = (int)batch;
+  p.s = (int)s;
+  p.max_blocks = (int)max_blocks;
+  p.page = (int)page;
+  p.tnd = layout == DSA_LAYOUT_TND;
+  // blocks of the launch for the caches from c0 on
+  auto take = [&](int64_t c0) {
     p.n = (int)(n - c0 < kPcMaxCaches ? n - c0 : kPcMaxCaches);
     int64_t units = 0;
     for (int i = 0; i < p.n; ++i) {
@@ -123,19 +134,15 @@ int pc_write_run(int64_t n, const void* const* rows, void* const* caches, const 
       c.unit0 = (int)units;
       units += row_bytes[k] >> c.shift;
     }
-    p.table = table;
-    p.lens = lens;
-    p.rows = row_lengths;
-    p.tokens = tokens;
-    p.pages = pages;
-    p.batch = (int)batch;
-    p.s = (int)s;
-    p.max_blocks = (int)max_blocks;
-    p.page = (int)page;
-    p.tnd = layout == DSA_LAYOUT_TND;
-    p.units = (int)units;
-    const int64_t grid = (tokens * units + kPcThreads - 1) / kPcThreads;
-    DSA_CHECK_SUPPORTED(units < (1ll << 31) && grid < (1ll << 31), "too many rows for one call");
+    p.units = (int)units;  // (at most 32 rows of 2^24 bytes)
+    return (tokens * units + kPcThreads - 1) / kPcThreads;
+  };
+  // (all of them before the first: a call that is refused has written nothing)
+  for (int64_t c0 = n > kPcMaxCaches ? 0 : n; c0 < n; c0 += kPcMaxCaches)
+    DSA_CHECK_SUPPORTED(launchable(take(c0), kPcThreads), "too many rows for one call");
+  for (int64_t c0 = 0; c0 < n; c0 += kPcMaxCaches) {
+    const int64_t grid = take(c0);
+    DSA_CHECK_SUPPORTED(launchable(grid, kPcThreads), "too many rows for one call");
     pc_write_kernel<<<dim3((unsigned)grid), kPcThreads, 0, stream>>>(p);
     DSA_HIP(hipGetLastError());
   }
@@ -415,12 +422,16 @@ int pc_fork_run(int64_t n, void* const* caches, const int64_t* row_bytes, const 
   const int64_t entries = rows * max_blocks > children * new_blocks ? rows * max_blocks : children * new_blocks;
   int64_t tb = (entries + 2 * kPcThreads - 1) / (2 * kPcThreads);
   tb = tb < 1 ? 1 : (tb > 1024 ? 1024 : tb);
+  // (all launches before the first: a call that is refused has changed no cache)
+  for (int64_t c0 = n > kPcMaxCaches ? 0 : n; c0 < n; c0 += kPcMaxCaches)
+    DSA_CHECK_SUPPORTED(launchable(tb + children * pc_copy_set(p.set, c0, n, caches, row_bytes, page), kPcThreads),
+                        "too many rows and pages for one call");
   bool first = true;
   for (int64_t c0 = 0; first || c0 < n; c0 += kPcMaxCaches, first = false) {
-    const int64_t chunks = pc_copy_set(p.set, c0, n, caches, row_bytes, page);
+    const int64_t chunks = pc_copy_set(p.set, c0, n, caches, row_bytes, page);  // (32 pages of 2^31 bytes: below 2^26)
     p.table_blocks = first ? (int)tb : 0;
     const int64_t grid = p.table_blocks + children * chunks;
-    DSA_CHECK_SUPPORTED(chunks < (1ll << 31) && grid < (1ll << 31), "too many rows and pages for one call");
+    DSA_CHECK_SUPPORTED(launchable(grid, kPcThreads), "too many rows and pages for one call");
     if (first) pc_fork_plan_kernel<<<dim3((unsigned)(1 + copy_blocks)), kPcPlanThreads, 0, stream>>>(p);
     if (grid > 0) pc_fork_kernel<<<dim3((unsigned)grid), kPcThreads, 0, stream>>>(p);
     DSA_HIP(hipGetLastError());
@@ -576,7 +587,6 @@ int pc_compact_run(int64_t n, void* const* caches, const int64_t* row_bytes, con
   bool first = true;
   for (int64_t c0 = 0; first || c0 < n; c0 += kPcMaxCaches, first = false) {
     const int64_t chunks = pc_copy_set(p.set, c0, n, caches, row_bytes, page);
-    DSA_CHECK_SUPPORTED(chunks < (1ll << 31), "pages too large for one call");
     p.table_blocks = first ? (int)tb : 0;
     // at most half the pages move; blocks beyond a few rounds of the CUs loop
     const int64_t most = (pages / 2) * chunks;

@@ -270,7 +270,7 @@ int rope_run(const void* const in[2], void* const out[2], const int64_t* const s
   p.per_part = (int)(((units + parts - 1) / parts + kRopeThreads - 1) / kRopeThreads * kRopeThreads);
   p.parts = (int)((units + p.per_part - 1) / p.per_part);
   const int64_t grid = groups * p.parts;
-  DSA_CHECK_SUPPORTED(grid < (1ll << 31), "too many tokens");
+  DSA_CHECK_SUPPORTED(launchable(grid, kRopeThreads), "too many tokens for one launch");
   if (dtype == DSA_DTYPE_BF16) rope_launch<bf16>(p, vec, inplace, streaming, grid, stream);
   else if (dtype == DSA_DTYPE_FP16) rope_launch<f16>(p, vec, inplace, streaming, grid, stream);
   else rope_launch<float>(p, vec, inplace, streaming, grid, stream);

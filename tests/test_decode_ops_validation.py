@@ -414,3 +414,28 @@ def test_rotary_in_place_refuses_views_that_share_columns():
                  (proj[..., :40], proj[:, :, :1, 32:])):    # columns 0 .. 31 and 32 .. 63
         with pytest.raises(ValueError, match="ROCm GPU device"):
             _rope(query=q, key=k, inplace=True)
+
+
+# ---- launches: fewer than 2^32 threads, checked before the first kernel of a call ----
+
+def test_launches_of_too_many_threads_are_refused():
+    lib = _lib()
+    p, n = ctypes.c_void_p, ctypes.c_int64
+    many = dict(b=1, s=1 << 24, qh=64, per=0)                 # 2^24 tokens of 512 pieces of 16 bytes
+    assert lib.dsa_rope(*_c(ROPE, many)) == 2 and b"launch" in lib.dsa_last_error()
+    big = dict(bytes=_list(n, 4096), sb=_list(n, 4096), st=_list(n, 4096), b=1 << 24, s=1, tokens=1 << 24)
+    assert lib.dsa_paged_cache_write(*_wargs(**big)) == 2 and b"too many rows" in lib.dsa_last_error()
+    # the 33rd cache's launch is too large, that of the 32 before it is not
+    wide = dict(n=33, rows=_list(p, *[A] * 33), caches=_list(p, *[A] * 33), sb=_list(n, *[4096] * 33),
+                st=_list(n, *[4096] * 33), bytes=_list(n, *[1] * 32, 4096), b=1 << 24, s=1, tokens=1 << 24)
+    assert lib.dsa_paged_cache_write(*_wargs(**wide)) == 2
+    fork = dict(rows=1 << 24, kids=1 << 24, bytes2=1 << 40)
+    assert lib.dsa_paged_cache_fork(*_fargs(**fork)) == 2 and b"too many rows" in lib.dsa_last_error()
+    fork = dict(n=33, caches=_list(p, *[A] * 33), bytes=_list(n, *[128] * 32, 1 << 20), rows=1 << 18, kids=1 << 18,
+                bytes2=1 << 40)
+    assert lib.dsa_paged_cache_fork(*_fargs(**fork)) == 2
+    for kw in (dict(b=1 << 16, n1=1024, n2=1), dict(b=1 << 16, s1=8, n1=128, n2=1, v=None, qr=A, kr=A, dr=64)):
+        assert lib.dsa_paged_attn(*_c(ATTN, kw)) == 2 and b"launch" in lib.dsa_last_error()
+    size = lib.dsa_paged_attn_workspace_size
+    assert size(1 << 16, 1, 1024, 1, 128, 0, 4, 16) == 0 and size((1 << 16) - 1, 1, 1024, 1, 128, 0, 4, 16) > 0
+    assert size(1 << 16, 8, 128, 1, 512, 1, 4, 16) == 0 and size((1 << 16) - 1, 8, 128, 1, 512, 1, 4, 16) > 0
