@@ -227,7 +227,7 @@ _calls = None
 
 
 class _NoCalls:
-    """In place of ``_torch_calls`` where it is not built: takes no call."""
+    """In place of ``_torch_calls`` where it is not built or does not load: takes no call."""
 
     @staticmethod
     def write(*args):
@@ -242,14 +242,20 @@ def calls():
     call than here), and it returns None for all others."""
     global _calls
     if _calls is None:
+        why = None
         if not (os.path.exists(LIB_PATH) and os.path.exists(CALLS_PATH)):
-            warnings.warn(f"{CALLS_PATH} is not built: calls of the paged decoding operators take longer on the host")
-            _calls = _NoCalls
+            why = "is not built"
         else:
-            from . import _torch_calls
             lib = load()
-            _torch_calls.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ENTRIES))
-            _calls = _torch_calls
+            try:
+                from . import _torch_calls
+                _torch_calls.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ENTRIES))
+                _calls = _torch_calls
+            except (ImportError, TypeError) as e:  # built for another torch, or from other sources
+                why = f"does not load ({e})"
+        if why:
+            warnings.warn(f"{CALLS_PATH} {why}: calls of the paged decoding operators take longer on the host")
+            _calls = _NoCalls
     return _calls
 
 

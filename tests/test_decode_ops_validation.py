@@ -439,3 +439,30 @@ def test_launches_of_too_many_threads_are_refused():
     size = lib.dsa_paged_attn_workspace_size
     assert size(1 << 16, 1, 1024, 1, 128, 0, 4, 16) == 0 and size((1 << 16) - 1, 1, 1024, 1, 128, 0, 4, 16) > 0
     assert size(1 << 16, 8, 128, 1, 512, 1, 4, 16) == 0 and size((1 << 16) - 1, 8, 128, 1, 512, 1, 4, 16) > 0
+
+
+# ---- the compiled calls ----
+
+def test_compiled_calls_that_do_not_load_are_done_without(tmp_path):
+    """In a process of its own, with the package beside a _torch_calls that the
+    loader refuses, as it does one built for another torch."""
+    import subprocess
+    import sys
+    _lib()
+    pkg = os.path.dirname(os.path.abspath(dsa.__file__))
+    (tmp_path / "dsa_triton_ascend_amd").mkdir()
+    for name in os.listdir(pkg):
+        if name not in ("_torch_calls.so", "__pycache__"):
+            os.symlink(os.path.join(pkg, name), tmp_path / "dsa_triton_ascend_amd" / name)
+    (tmp_path / "dsa_triton_ascend_amd" / "_torch_calls.so").write_bytes(b"not a library")
+    code = ("import warnings, torch; warnings.simplefilter('always')\n"
+            "import dsa_triton_ascend_amd as dsa\n"
+            "from dsa_triton_ascend_amd import _lib\n"
+            "print(_lib.calls() is _lib._NoCalls, _lib.calls() is _lib._NoCalls)\n"
+            "try:\n    dsa.paged_cache_compact([], torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))\n"
+            "except ValueError as e:\n    print(e)\n")
+    env = dict(os.environ, PYTHONPATH=str(tmp_path), DSA_HIP_LIB=os.path.join(pkg, "libdsa_hip.so"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env, cwd=tmp_path, timeout=300)
+    assert r.returncode == 0, r.stderr
+    assert r.stdout.startswith("True True\n") and "ROCm GPU device" in r.stdout
+    assert r.stderr.count("does not load") == 1
