@@ -105,7 +105,7 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
     for name, t in others:
         if name != "query_rope" and not t.is_contiguous():
             raise ValueError(f"the {name} cache must be contiguous (a copy of it would be made at every call)")
-    table = block_table if block_table.dtype is torch.int32 else block_table.to(dtype=torch.int32)
+    table = _int32(block_table)
     if not table.is_contiguous():
         table = table.contiguous()
     q = query if query.is_contiguous() else query.contiguous()
@@ -134,9 +134,17 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
     return out, smax, ssum
 
 
+def _int32(t):
+    if t.dtype is torch.int64:  # what 32 bits do not hold is as far outside as they go, not another value inside
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+    return t if t.dtype is torch.int32 else t.to(dtype=torch.int32)
+
+
 def _lengths(x, device):
-    if isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.device == device and x.is_contiguous():
-        return x
+    if isinstance(x, torch.Tensor):
+        x = _int32(x)
+        if x.device == device and x.is_contiguous():
+            return x
     return _seq_tensor(x, device)
 
 

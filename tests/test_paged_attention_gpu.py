@@ -461,3 +461,23 @@ def test_small_columns_beside_a_large_one(latent, N1, D, dt, large, small):
         x *= small
         x[..., 0] = large
     _compare(args, data, lens)
+
+
+@pytest.mark.parametrize("latent", [False, True])
+def test_64_bit_tables_and_lengths(latent):
+    """Entries and lengths that 32 bits do not hold are outside the cache, past the table or below zero."""
+    import dsa_triton_ascend_amd as dsa
+    lens = [128, 100, 64]
+    args, _ = _make(3, 1, 8, 1 if latent else 2, 512 if latent else 128, 64, lens, torch.bfloat16, latent, seed=97)
+    for name in ("key", "value", "key_rope"):
+        if args[name] is not None:
+            args[name].nan_to_num_(0.25)
+    args["block_table"][0, 1] = -1
+    args["actual_seq_lengths_kv"] = torch.tensor([128, 128, 0], dtype=torch.int32, device="cuda")
+    want = dsa.paged_attention(**args)
+    args["actual_seq_lengths_kv"] = torch.tensor([128, 2 ** 32 + 3, -2 ** 32 + 9], device="cuda")
+    page = int(args["block_table"][1, 0])
+    args["block_table"] = args["block_table"].long()
+    for entry in (2 ** 32 + page, -2 ** 32 + page, 2 ** 31, 2 ** 63 - 1, -2 ** 63):
+        args["block_table"][0, 1] = entry
+        assert all(torch.equal(a, b) for a, b in zip(dsa.paged_attention(**args), want)), entry
