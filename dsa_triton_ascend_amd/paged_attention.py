@@ -27,7 +27,8 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
     [pages, page_size, N2, D], D in (64, 128, 256), N1 a multiple of N2, no
     rope parts.  Latent form: ``value`` None, key [pages, page_size, 1, D], D
     in (128, 256, 512), query_rope [B, S1, N1, 64] and key_rope [pages,
-    page_size, 1, 64].  ``block_table`` [B, max_blocks]; entries outside the
+    page_size, 1, 64].  Caches are contiguous and start at a multiple of 16
+    bytes; a query that does not is copied.  ``block_table`` [B, max_blocks]; entries outside the
     cache read as zero rows; all of it may name up to 2^35 tokens.  ``actual_seq_lengths_kv`` [B]: cached tokens, the
     new ones included.  ``actual_seq_lengths_query`` [B]: new tokens (S1 by
     default); later rows give zeros.
@@ -108,10 +109,8 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
     table = _int32(block_table)
     if not table.is_contiguous():
         table = table.contiguous()
-    q = query if query.is_contiguous() else query.contiguous()
-    qr = query_rope
-    if latent and not qr.is_contiguous():
-        qr = qr.contiguous()
+    q = _rows(query)
+    qr = _rows(query_rope) if latent else None
     out = q.new_empty(q_shape)
     smax = torch.empty((B, N2, S1, N1 // N2), dtype=torch.float32, device=dev)
     ssum = torch.empty_like(smax)
@@ -132,6 +131,12 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
     if status:
         _lib.check(status, "dsa_paged_attn")
     return out, smax, ssum
+
+
+def _rows(t):
+    """The tensor as the kernels read it: contiguous, 16 bytes at a time."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def _int32(t):

@@ -481,3 +481,19 @@ def test_64_bit_tables_and_lengths(latent):
     for entry in (2 ** 32 + page, -2 ** 32 + page, 2 ** 31, 2 ** 63 - 1, -2 ** 63):
         args["block_table"][0, 1] = entry
         assert all(torch.equal(a, b) for a, b in zip(dsa.paged_attention(**args), want)), entry
+
+
+@pytest.mark.parametrize("latent", [False, True])
+def test_queries_at_any_address(latent):
+    import dsa_triton_ascend_amd as dsa
+    args, _ = _make(2, 1, 8, 1 if latent else 2, 512 if latent else 128, 64, [128, 100], torch.bfloat16, latent, seed=99)
+    want = dsa.paged_attention(**args)
+    for name in ("query", "query_rope") if latent else ("query",):
+        t = args[name]
+        args[name] = torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+        assert args[name].data_ptr() % 16 and args[name].is_contiguous()
+    assert all(torch.equal(a, b) for a, b in zip(dsa.paged_attention(**args), want))
+    cache = args["key"]
+    args["key"] = torch.cat([cache.new_zeros(1), cache.flatten()])[1:].view(cache.shape)
+    with pytest.raises(ValueError, match="aligned"):
+        dsa.paged_attention(**args)
