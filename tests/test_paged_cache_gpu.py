@@ -337,3 +337,34 @@ def test_fork_of_many_rows(rows, kids):
     t, l, r = dsa.paged_cache_fork(caches, _ints(table), _ints(lens), _ints(refs), parents=_ints(parents), new_tokens=1)
     assert t.tolist() == w_table and l.tolist() == w_lens and r.tolist() == w_refs
     assert all(torch.equal(c, w) for c, w in zip(caches, want))
+
+
+@pytest.mark.parametrize("pages", [16384, 16385, 20480, 40001])
+@pytest.mark.parametrize("live", ["none", "one", "some", "a chunk's end", "half", "most", "all but one", "all"])
+def test_compact_of_many_pages(pages, live):
+    """Around and above the number of pages up to which one launch counts and
+    ranks; the number in use falls on and off the ends of chunks of 1024."""
+    import dsa_triton_ascend_amd as dsa
+    rng = random.Random(pages)
+    n = {"none": 0, "one": 1, "some": 777, "a chunk's end": 5 * 1024, "half": pages // 2, "most": pages - 1500,
+         "all but one": pages - 1, "all": pages}[live]
+    used = sorted(rng.sample(range(pages), n))
+    refs = torch.zeros(pages, dtype=torch.int32)
+    refs[used] = torch.randint(1, 5, (n,), dtype=torch.int32, generator=torch.Generator().manual_seed(n))
+    holes = (refs[:n] == 0).nonzero().flatten()
+    high = torch.tensor([i for i in used if i >= n], dtype=torch.int64)
+    page_map = torch.where(refs > 0, torch.arange(pages, dtype=torch.int32), -1)
+    page_map[high] = holes.int()
+    table = torch.tensor([[rng.choice([rng.randrange(pages), rng.choice(used) if used else 0, -1, pages]) for _ in range(33)]
+                          for _ in range(7)], dtype=torch.int32)
+    inside = (table >= 0) & (table < pages)
+    w_table = torch.where(inside, page_map[table.clamp(0, pages - 1).long()], -1)
+    w_refs = torch.zeros_like(refs)
+    w_refs[page_map[refs > 0].long()] = refs[refs > 0]
+    caches = [torch.arange(pages * 2 * k, device="cuda", dtype=torch.int32).view(pages, 2, 1, k) for k in (1, 4)]
+    want = [c.clone() for c in caches]
+    for w in want:
+        w[holes.cuda()] = w[high.cuda()]
+    t, r, m = dsa.paged_cache_compact(caches, table.cuda(), refs.cuda())
+    assert torch.equal(t.cpu(), w_table) and torch.equal(r.cpu(), w_refs) and torch.equal(m.cpu(), page_map)
+    assert all(torch.equal(c, w) for c, w in zip(caches, want))

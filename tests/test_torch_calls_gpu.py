@@ -366,3 +366,58 @@ def test_in_place_views_of_one_buffer():
                 assert torch.equal(a[..., s:s + cols], b[..., s:s + cols])
         taken[shared] += 1
     assert min(taken) > 40, taken
+
+
+def test_ordinary_calls_are_taken(monkeypatch):
+    """The forms that are compared with Python above do go by the module: each
+    call is recorded, and it returns something."""
+    import dsa_triton_ascend_amd as dsa
+    from dsa_triton_ascend_amd import _lib
+    module, made = _lib.calls(), []
+
+    class Recorder:
+        def __getattr__(self, name):
+            def call(*args):
+                result = getattr(module, name)(*args)
+                made.append((name, result is not None))
+                return result
+            return call
+
+    monkeypatch.setattr(_lib, "_calls", Recorder())
+
+    def taken(name, f):
+        made.clear()
+        f()
+        assert made == [(name, True)], (name, made)
+
+    caches, table, lens, refs = _state()
+    latent, ltable, llens, _ = _state(cols=128)
+    inv, _ = dsa.rotary_frequencies(32)
+    for lead, layout in (((3, 5), "BSND"), ((7,), "TND")):
+        pos = torch.randint(0, 9999, lead, device="cuda", dtype=I32)
+        q = torch.randn(*lead, 6, 96, device="cuda").bfloat16()
+        k = torch.randn(*lead, 2, 64, device="cuda").bfloat16()
+        for kw in (dict(), dict(inplace=True), dict(inverse=True, interleaved=True)):
+            taken("rotate", lambda: dsa.rotary_embedding(q[..., :5, 16:], k, pos, inv, rotary_offset=32, layout=layout, **kw))
+        fused = torch.randn(*lead, 6, 64, device="cuda")
+        taken("rotate", lambda: dsa.rotary_embedding(fused[..., :4, :], fused[..., 4:, :], pos, inv, layout=layout,
+                                                     inplace=True))
+        leaf = fused.clone().requires_grad_()
+        taken("rotate", lambda: dsa.rotary_embedding(leaf, None, pos, inv, layout=layout)[0].sum().backward())
+    rows = [torch.randn(2, 4, 1, 64, device="cuda").bfloat16(), torch.randn(2, 4, 3, 64, device="cuda").bfloat16()[:, :, 1:2]]
+    packed = [torch.randn(9, 1, 64, device="cuda").bfloat16() for _ in range(2)]
+    counts = torch.tensor([3, 8], dtype=I32, device="cuda")
+    taken("write", lambda: dsa.paged_cache_write(caches, rows, table, lens))
+    taken("write", lambda: dsa.paged_cache_write(tuple(caches), rows, table, lens, row_lengths=counts))
+    taken("write", lambda: dsa.paged_cache_write(caches, packed, table, lens, row_lengths=counts, layout="TND"))
+    taken("fork", lambda: dsa.paged_cache_fork(caches, table, lens, refs, torch.tensor([1, 0, 1], dtype=I32, device="cuda"),
+                                               new_tokens=2))
+    taken("fork", lambda: dsa.paged_cache_fork(caches[0], table, lens, refs))
+    taken("compact", lambda: dsa.paged_cache_compact(caches, table, refs))
+    for new in (None, torch.tensor([2, 1], dtype=I32, device="cuda")):
+        q = torch.randn(2, 2, 8, 128, device="cuda").bfloat16()
+        taken("attention", lambda: dsa.paged_attention(q[..., :64].contiguous(), caches[0], caches[1], table.clamp(min=0),
+                                                       lens, actual_seq_lengths_query=new, pre_tokens=30))
+        taken("attention", lambda: dsa.paged_attention(
+            q, latent[0], None, ltable.clamp(min=0), llens, query_rope=q[..., :64].contiguous(), key_rope=latent[1],
+            actual_seq_lengths_query=new, return_softmax_lse=True))
