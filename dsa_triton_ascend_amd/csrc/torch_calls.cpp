@@ -484,8 +484,9 @@ struct RotaryBackward : torch::autograd::Node {
     Rotation back = r;
     back.inverse = !r.inverse;
     for (int i = 0; i < (int)n; ++i)
-      if (grads[i].defined() && !grads[i]._is_zerotensor() && task_should_compute_output(i)) {
-        in[count] = grads[i].stride(-1) == 1 ? grads[i] : grads[i].contiguous();
+      if (grads[i].defined() && task_should_compute_output(i)) {
+        if (grads[i]._is_zerotensor()) in[count] = at::zeros(grads[i].sizes(), grads[i].options());  // (it has no memory)
+        else in[count] = grads[i].stride(-1) == 1 ? grads[i] : grads[i].contiguous();
         back.start[count] = r.start[i];
         place[count++] = i;
       }

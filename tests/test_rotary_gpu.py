@@ -326,3 +326,31 @@ def test_a_gradient_s_tangent_where_the_input_has_none(monkeypatch, compiled):
         g = fwad.unpack_dual(torch.autograd.grad((qo * fwad.make_dual(w, t)).sum(), q)[0])
     assert torch.equal(g.primal, dsa.rotary_embedding(w, None, pos, inv, inverse=True)[0])
     assert torch.equal(g.tangent, dsa.rotary_embedding(t, None, pos, inv, inverse=True)[0])
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_gradients_and_tangents_without_memory(monkeypatch, compiled):
+    """torch's zero tensors, which stand for zeros that nobody has written."""
+    import torch.autograd.forward_ad as fwad
+
+    import dsa_triton_ascend_amd as dsa
+    from dsa_triton_ascend_amd import _lib
+    if not compiled:
+        monkeypatch.setattr(_lib, "_calls", _lib._NoCalls)
+    pos = torch.arange(5, device="cuda")
+    inv, _ = dsa.rotary_frequencies(64)
+    q = torch.randn(1, 5, 2, 64, device="cuda", requires_grad=True)
+    zero = torch._efficientzerotensor(1, 5, 2, 64, device="cuda")
+    out, _ = dsa.rotary_embedding(q, None, pos, inv)
+    (g,) = torch.autograd.grad(out, q, zero)
+    assert g.shape == q.shape and not g.any()
+    t = torch.randn(1, 5, 2, 64, device="cuda")
+    with fwad.dual_level():
+        out, _ = dsa.rotary_embedding(q, None, pos, inv)
+        g = fwad.unpack_dual(torch.autograd.grad(out, q, fwad.make_dual(torch.zeros_like(t), t))[0])
+        assert not g.primal.any() and torch.equal(g.tangent, dsa.rotary_embedding(t, None, pos, inv, inverse=True)[0])
+        y, _ = dsa.rotary_embedding(fwad.make_dual(t, zero), None, pos, inv)
+        y = fwad.unpack_dual(y)
+        assert torch.equal(y.primal, dsa.rotary_embedding(t, None, pos, inv)[0])
+        assert y.tangent is None or not y.tangent.any()
+    torch.cuda.synchronize()
