@@ -94,7 +94,10 @@ def _compile(src, extra):
 
 
 def build_calls():
-    """Compile _torch_calls.so against the installed torch (no device code)."""
+    """Compile _torch_calls.so against the installed torch (no device code).
+    Without NDEBUG pybind11's headers count references in thread-local data;
+    a module that has some and never uses it makes every thread-local access
+    of the process slow with glibc before 2.39."""
     import sysconfig
 
     import torch
@@ -104,7 +107,7 @@ def build_calls():
     includes = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(rocm, "include")]
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = CALLS_OUT + ".tmp"
-    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-DNDEBUG", "-D__HIP_PLATFORM_AMD__=1",
             "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
            + [x for i in includes for x in ("-isystem", i)]
            + [os.path.join(CSRC, "torch_calls.cpp"), "-o", tmp, "-L" + lib, "-ltorch_python", "-ltorch_cpu",

@@ -466,3 +466,19 @@ def test_compiled_calls_that_do_not_load_are_done_without(tmp_path):
     assert r.returncode == 0, r.stderr
     assert r.stdout.startswith("True True\n") and "ROCm GPU device" in r.stdout
     assert r.stderr.count("does not load") == 1
+
+
+def test_compiled_calls_have_no_thread_local_data():
+    """A module loaded after the library whose thread-local data nobody uses
+    makes each such access of the process slow (with glibc before 2.39)."""
+    import struct
+
+    from dsa_triton_ascend_amd import _lib as L
+    if not os.path.exists(L.CALLS_PATH):
+        pytest.skip("_torch_calls.so not built")
+    with open(L.CALLS_PATH, "rb") as f:
+        elf = f.read()
+    assert elf[:6] == b"\x7fELF\x02\x01"
+    at, size, count = struct.unpack_from("<Q", elf, 32)[0], *struct.unpack_from("<HH", elf, 54)
+    types = [struct.unpack_from("<I", elf, at + i * size)[0] for i in range(count)]
+    assert 1 in types and 7 not in types  # PT_LOAD, PT_TLS
