@@ -6,10 +6,10 @@
 // A token of 576 columns is 1152 bytes and 2176 flops a row.  Up to 32 rows
 // the bytes bound it (16 heads, 32 x 32K tokens, 1.2 GB: 191 us, 6.3 TB/s in
 // all and 7.4 TB/s between 16K and 32K); at 64 rows bytes and LDS reads are
-// near each other (231 us); at 128 it is the LDS reads: 416 KB a tile of 32
+// near each other (238 us); at 128 it is the LDS reads: 416 KB a tile of 32
 // tokens (288 of them K, which each of eight waves reads for its 16 rows),
-// 3250 of a tile's 5400 cycles, beside 2180 of MFMAs (346 us, 0.84 PFLOP/s,
-// 40 % of the matrix pipes' cycles at the 2.05 GHz that the card holds).
+// 3250 of a tile's 5400 cycles, beside 2180 of MFMAs (360 us with the join of
+// 14, 0.81 PFLOP/s, 44 % of the matrix pipes' cycles).
 //
 // One workgroup of eight waves per CU owns a run of tokens for HG rows; a
 // token is read from memory once and serves both products and every row
@@ -36,10 +36,15 @@
 //
 // Up to 32 rows P is multiplied as a sum of two values of the input type,
 // which is free where the bytes bound.  With more rows the MFMAs and LDS reads
-// of the second value are not, so P is rounded once there, and the output is
-// divided by the sum of the rounded values: the weights still add up to one,
-// and what is left is the rounding of single weights, below the rounding of
-// the output.
+// of the second value are not (at 128 rows of 512 columns the LDS has no room
+// for it either), so P is rounded once there, at any number of tokens, and the
+// output is divided by the sum of the rounded values, so that the weights still
+// add up to one.  What is left is the rounding of single weights: an output is
+// off by up to eps sum w |v|, and for values that vary from token to token by
+// about half of its own rounding.  Error against 64 bits over the output, both
+// 2-norms, with P as two values and rounded: bf16 1.66e-3 and 1.73e-3 over 32K
+// tokens, 1.66e-3 and 1.90e-3 over 60 to 1000, 1.66e-3 and 1.70e-3 over two;
+// fp16 2.07e-4 and 2.17e-4, 2.38e-4, 2.13e-4.
 #include "paged_attn.h"
 #include "sfa_fwd.h"
 

@@ -267,6 +267,10 @@ constexpr int kPcRowsHere = 4096;  // rows whose first children the plan finds i
 
 // Block 0 plans: which rows need how many pages, and which free ones those
 // are.  The other blocks copy the counts for the second launch to change.
+// One workgroup is enough for the rows of a batch, not for a table of many
+// thousands: whole forks of rows of 32 pages, captured, take 7 to 8 us for 16
+// rows, 8 to 9 for 256, 10 to 11 for 1024, 24 to 28 for 4096 and 400 to 630 for
+// 65536 (rows that continue themselves, and four from one parent).
 __global__ __launch_bounds__(kPcPlanThreads) void pc_fork_plan_kernel(PcForkParams p) {
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
@@ -445,9 +449,10 @@ int pc_fork_run(int64_t n, void* const* caches, const int64_t* row_bytes, const 
 // and written and the moves need no order.
 // ---------------------------------------------------------------------------
 // Up to this many pages every block of the rank kernel counts the live pages by
-// itself: a block's 1024 threads read 16 counts each.  8192 pages: 5.1 us, and
-// 3.3 + 4.2 us with a launch that counts first, which pays where the counts
-// no longer come from the L2 (64 KB of them here, by 16 blocks).
+// itself: a block's 1024 threads read 16 counts each.  Whole calls, captured,
+// without and with a launch that counts first: 8192 pages 9.9 and 11.8 us,
+// 16384 11.4 and 12.3, 24576 13.2 and 13.9, 32768 15.3 and 15.9, 65536 25.4 and
+// 22.6 (each block reads all counts, so what they read grows with the square).
 constexpr int64_t kPcCountsHere = 16384;
 
 struct PcCompactParams {

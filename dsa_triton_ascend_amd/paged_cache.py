@@ -178,7 +178,12 @@ def paged_cache_fork(caches, block_table, seq_lengths, page_refs, parents=None, 
     order.  A row for which they do not last, or that outgrows the table's
     width, gets no pages and the length -1; its sequence is released unless
     another row continues it, so keep the old state until lengths are checked.
-    Pages of the old table past a sequence's last token are released.
+    Pages of the old table past a sequence's last token are released, and what
+    a row needs is taken from those free before the call: a page that it
+    reserved and did not fill is exchanged for another one, so a pool needs one
+    free page for every row in such a state.  Fork when the room is used up, or
+    write into pages reserved earlier without a fork between.  A length below
+    zero, as of a row that got no pages, counts as zero.
     ``caches`` may be empty (tables only, with ``page_size``), which leaves the
     copies to the caller.
 

@@ -414,6 +414,12 @@ int dsa_li_scores_paged(const void* query, const void* key_cache, const void* we
  * every sequence (positions_per_sequence: [B, S1]) or shared by all ([S1]);
  * inv_freq: rotary_dim / 2 doubles on the device.  Angles are formed in 64
  * bits.  dtype BF16, FP16 or FP32; rotary_dim even, up to 1024.
+ *
+ * This and the entry points below refuse sizes whose launches would have 2^32
+ * threads or more (DSA_ERR_UNSUPPORTED, nothing launched): 2^24 tokens here at
+ * the earliest, 2^26 query rows of dsa_paged_attn, 64 GiB of rows of dsa_paged_cache_write (4
+ * where they move byte by byte).  DSA_ERR_HIP may come after a launch: an error
+ * that another HIP call left behind is reported by the next one.
  */
 int dsa_rope(const void* query, void* query_out, int64_t q_in_sb, int64_t q_in_ss, int64_t q_in_sh, int64_t q_out_sb,
              int64_t q_out_ss, int64_t q_out_sh, int64_t q_heads, int64_t q_d, int64_t q_start, const void* key,
