@@ -61,7 +61,10 @@ from .rotary_embedding import (  # noqa: F401
 from .paged_cache import (  # noqa: F401
     paged_cache_compact,
     paged_cache_fork,
+    paged_cache_plan,
+    paged_cache_prefixes,
     paged_cache_write,
+    paged_cache_write_slots,
 )
 
 from .paged_attention import (  # noqa: F401

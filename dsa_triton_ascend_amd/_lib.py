@@ -166,6 +166,14 @@ SIGNATURES = {
         _i64, _i64, _i64,                     # batch, s1, rotary_dim
         _i32, _i32, _i32, _f32, _vp,          # interleaved, inverse, dtype, attention_scale, stream
     ]),
+    "dsa_rope_axes": (_c.c_int, [
+        _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,  # query, out, 6 strides, heads, d, start
+        _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,  # key, likewise
+        _vp, _i32, _i32, _vp,                 # positions, positions_64, positions_per_sequence, inv_freq
+        _i64, _i64, _i64,                     # batch, s1, rotary_dim
+        _i64, _vp, _i32,                      # n_axes, sections, sections_interleaved
+        _i32, _i32, _i32, _f32, _vp,          # interleaved, inverse, dtype, attention_scale, stream
+    ]),
     "dsa_paged_cache_write": (_c.c_int, [
         _i64, _vp, _vp, _vp, _vp, _vp,        # n_caches, rows, caches, row_bytes, row_batch_stride, row_token_stride
         _i32p, _i32p, _i32p,                  # block_table, seq_lengths, row_lengths
@@ -186,6 +194,22 @@ SIGNATURES = {
         _i32p, _i32p, _i32p, _i32p, _i32p,    # block_table, page_refs, new_block_table, new_page_refs, page_map
         _i64, _i64, _i64, _i64,               # rows, max_blocks, num_pages, page_size
         _vp, _sz, _vp,                        # workspace, workspace_bytes, stream
+    ]),
+    "dsa_paged_cache_plan_workspace_size": (_sz, [_i64, _i64]),
+    "dsa_paged_cache_plan": (_c.c_int, [
+        _i32p, _i32p, _i32p, _i32p,           # block_table, seq_lengths, page_refs, new_lengths
+        _i32p, _i32p, _i32p,                  # new_block_table, new_seq_lengths, new_page_refs
+        _i32p, _i32p, _i32p,                  # slots, positions, row_lengths
+        _i64, _i64, _i64, _i64, _i64,         # rows, max_blocks, num_pages, page_size, tokens
+        _vp, _sz, _vp,                        # workspace, workspace_bytes, stream
+    ]),
+    "dsa_paged_cache_write_slots": (_c.c_int, [
+        _i64, _vp, _vp, _vp, _vp, _vp,        # n_caches, rows, caches, row_bytes, row_batch_stride, row_token_stride
+        _i32p, _i64, _i64, _i64, _i64, _vp,   # slots, batch, s1, num_pages, page_size, stream
+    ]),
+    "dsa_paged_cache_prefixes": (_c.c_int, [
+        _i32p, _i32p, _i32p, _i32p,           # block_table, seq_lengths, prefix_groups, prefix_lengths
+        _i64, _i64, _i64, _i64, _vp,          # rows, max_blocks, page_size, min_tokens, stream
     ]),
     "dsa_paged_attn_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i64, _i64]),
     "dsa_paged_attn": (_c.c_int, [
@@ -222,7 +246,8 @@ def load():
 
 _ENTRIES = ("dsa_rope", "dsa_paged_cache_write", "dsa_paged_cache_fork_workspace_size", "dsa_paged_cache_fork",
             "dsa_paged_cache_compact_workspace_size", "dsa_paged_cache_compact", "dsa_paged_attn_workspace_size",
-            "dsa_paged_attn", "dsa_last_error")  # in the order in which _torch_calls takes them
+            "dsa_paged_attn", "dsa_last_error", "dsa_rope_axes", "dsa_paged_cache_plan_workspace_size",
+            "dsa_paged_cache_plan", "dsa_paged_cache_write_slots", "dsa_paged_cache_prefixes")  # in the order in which _torch_calls takes them
 _calls = None
 
 
@@ -233,7 +258,7 @@ class _NoCalls:
     def write(*args):
         return None
 
-    fork = compact = attention = rotate = write
+    fork = compact = attention = rotate = rotate_axes = plan = write_slots = prefixes = write
 
 
 def calls():

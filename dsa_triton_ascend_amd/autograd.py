@@ -136,43 +136,44 @@ class RotaryEmbeddingFunction(torch.autograd.Function):
     is linear, so a tangent turns as its input does."""
 
     @staticmethod
-    def forward(ctx, query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse):
+    def forward(ctx, query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, axes=None):
         ctx.save_for_backward(positions, inv_freq)
         ctx.save_for_forward(positions, inv_freq)
-        ctx.args = (interleaved, q_start, k_start, scale, not inverse)
+        ctx.args = (interleaved, q_start, k_start, scale, not inverse, axes)
         ctx.shapes = query.shape, None if key is None else key.shape
         ctx.set_materialize_grads(False)
-        return _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False)
+        return _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False, axes)
 
     @staticmethod
     def backward(ctx, d_query, d_key):
         positions, inv_freq = ctx.saved_tensors
-        interleaved, q_start, k_start, scale, inverse = ctx.args
+        interleaved, q_start, k_start, scale, inverse, axes = ctx.args
         d_q = d_query if ctx.needs_input_grad[0] else None
         d_k = d_key if ctx.needs_input_grad[1] else None
-        return _rotate_linear(d_q, d_k, positions, inv_freq, interleaved, q_start, k_start, scale, inverse) + (None,) * 7
+        grads = _rotate_linear(d_q, d_k, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, axes)
+        return grads + (None,) * (len(ctx.needs_input_grad) - 2)
 
     @staticmethod
     def jvp(ctx, t_query, t_key, *_):
         positions, inv_freq = ctx.saved_tensors
-        interleaved, q_start, k_start, scale, inverse = ctx.args
-        out = _rotate_linear(t_query, t_key, positions, inv_freq, interleaved, q_start, k_start, scale, not inverse)
+        interleaved, q_start, k_start, scale, inverse, axes = ctx.args
+        out = _rotate_linear(t_query, t_key, positions, inv_freq, interleaved, q_start, k_start, scale, not inverse, axes)
         some = t_key if t_query is None else t_query
         # (an output's tangent may not be absent)
         return tuple(some.new_zeros(shape) if o is None and shape is not None else o for o, shape in zip(out, ctx.shapes))
 
 
-def _rotate_linear(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse):
+def _rotate_linear(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, axes=None):
     """Rotated gradients or tangents, either of which may be absent, with
     whatever derivatives they carry themselves."""
     if query is None and key is None:
         return None, None
     if query is None:
-        return _rotate_linear(key, None, positions, inv_freq, interleaved, k_start, 0, scale, inverse)[::-1]
+        return _rotate_linear(key, None, positions, inv_freq, interleaved, k_start, 0, scale, inverse, axes)[::-1]
     if torch.is_grad_enabled() or any(t is not None and unpack_dual(t).tangent is not None for t in (query, key)):
         return RotaryEmbeddingFunction.apply(query, key, positions, inv_freq, interleaved, q_start, k_start, scale,
-                                             inverse)
-    return _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False)
+                                             inverse, axes)
+    return _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, False, axes)
 
 
 __all__ = ["RotaryEmbeddingFunction", "SparseFlashAttentionFunction", "sparse_flash_attention_train",

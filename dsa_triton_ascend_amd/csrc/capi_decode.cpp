@@ -9,7 +9,8 @@ namespace dsa {
 int rope_run(const void* const in[2], void* const out[2], const int64_t* const strides[2], const int64_t heads[2],
              const int64_t d[2], const int64_t start[2], int n, const void* positions, int32_t pos64,
              int32_t pos_per_seq, const double* inv_freq, int64_t tokens, int64_t s, int64_t rot, int32_t interleaved,
-             int32_t inverse, int32_t dtype, float scale, hipStream_t stream);
+             int32_t inverse, int32_t dtype, float scale, int64_t axes, const int64_t* sections,
+             int32_t axes_interleaved, hipStream_t stream);
 // paged_cache.hip
 int pc_write_run(int64_t n, const void* const* rows, void* const* caches, const int64_t* row_bytes,
                  const int64_t* row_sb, const int64_t* row_st, const int32_t* table, const int32_t* lens,
@@ -20,6 +21,16 @@ int pc_fork_run(int64_t n, void* const* caches, const int64_t* row_bytes, const 
                 const int32_t* refs, const int32_t* parents, int32_t* new_table, int32_t* new_lens,
                 int32_t* new_refs, int64_t rows, int64_t children, int64_t max_blocks, int64_t new_blocks,
                 int64_t pages, int64_t page, int64_t new_tokens, void* workspace, hipStream_t stream);
+size_t pc_plan_workspace_bytes(int64_t rows, int64_t pages);
+int pc_plan_run(const int32_t* table, const int32_t* lens, const int32_t* refs, const int32_t* more,
+                int32_t* new_table, int32_t* new_lens, int32_t* new_refs, int32_t* slots, int32_t* positions,
+                int32_t* ends, int64_t rows, int64_t max_blocks, int64_t pages, int64_t page, int64_t tokens,
+                void* workspace, hipStream_t stream);
+int pc_slots_run(int64_t n, const void* const* rows, void* const* caches, const int64_t* row_bytes,
+                 const int64_t* row_sb, const int64_t* row_st, const int32_t* slots, int64_t batch, int64_t s,
+                 int64_t pages, int64_t page, hipStream_t stream);
+int pc_prefixes_run(const int32_t* table, const int32_t* lens, int32_t* groups, int32_t* lengths, int64_t rows,
+                    int64_t max_blocks, int64_t page, int64_t min_tokens, hipStream_t stream);
 size_t pc_compact_workspace_bytes(int64_t pages);
 int pc_compact_run(int64_t n, void* const* caches, const int64_t* row_bytes, const int32_t* table,
                    const int32_t* refs, int32_t* new_table, int32_t* new_refs, int32_t* page_map, int64_t entries,
@@ -86,16 +97,13 @@ static bool paged_attn_sizes_ok(int64_t batch, int64_t s1, int64_t n1, int64_t n
 
 using namespace dsa;
 
-extern "C" {
-
-int dsa_rope(const void* query, void* query_out, int64_t q_in_sb, int64_t q_in_ss, int64_t q_in_sh, int64_t q_out_sb,
+static int rope_checked(const void* query, void* query_out, int64_t q_in_sb, int64_t q_in_ss, int64_t q_in_sh, int64_t q_out_sb,
              int64_t q_out_ss, int64_t q_out_sh, int64_t q_heads, int64_t q_d, int64_t q_start, const void* key,
              void* key_out, int64_t k_in_sb, int64_t k_in_ss, int64_t k_in_sh, int64_t k_out_sb, int64_t k_out_ss,
              int64_t k_out_sh, int64_t k_heads, int64_t k_d, int64_t k_start, const void* positions,
              int32_t positions_64, int32_t positions_per_sequence, const double* inv_freq, int64_t batch, int64_t s1,
-             int64_t rotary_dim, int32_t interleaved, int32_t inverse, int32_t dtype, float attention_scale,
-             void* stream) {
-  clear_error();
+             int64_t rotary_dim, int64_t axes, const int64_t* sections, int32_t sections_interleaved,
+             int32_t interleaved, int32_t inverse, int32_t dtype, float attention_scale, void* stream) {
   DSA_CHECK_ARG(query && query_out && positions && inv_freq, "null tensor pointer");
   DSA_CHECK_ARG((key == nullptr) == (key_out == nullptr), "key and key_out must be both provided or both omitted");
   DSA_CHECK_SUPPORTED(dtype == DSA_DTYPE_BF16 || dtype == DSA_DTYPE_FP16 || dtype == DSA_DTYPE_FP32,
@@ -121,8 +129,54 @@ int dsa_rope(const void* query, void* query_out, int64_t q_in_sb, int64_t q_in_s
       DSA_CHECK_ARG(strides[i][j] >= 0 && strides[i][j] < (1ll << 48), "strides must be in [0, 2^48)");
   }
   return rope_run(in, out, strides, heads, d, start, n, positions, positions_64, positions_per_sequence, inv_freq,
-                  batch * s1, s1, rotary_dim, interleaved != 0, inverse != 0, dtype, attention_scale,
-                  (hipStream_t)stream);
+                  batch * s1, s1, rotary_dim, interleaved != 0, inverse != 0, dtype, attention_scale, axes, sections,
+                  sections_interleaved != 0, (hipStream_t)stream);
+}
+
+extern "C" {
+
+int dsa_rope(const void* query, void* query_out, int64_t q_in_sb, int64_t q_in_ss, int64_t q_in_sh, int64_t q_out_sb,
+             int64_t q_out_ss, int64_t q_out_sh, int64_t q_heads, int64_t q_d, int64_t q_start, const void* key,
+             void* key_out, int64_t k_in_sb, int64_t k_in_ss, int64_t k_in_sh, int64_t k_out_sb, int64_t k_out_ss,
+             int64_t k_out_sh, int64_t k_heads, int64_t k_d, int64_t k_start, const void* positions,
+             int32_t positions_64, int32_t positions_per_sequence, const double* inv_freq, int64_t batch, int64_t s1,
+             int64_t rotary_dim, int32_t interleaved, int32_t inverse, int32_t dtype, float attention_scale,
+             void* stream) {
+  clear_error();
+  return rope_checked(query, query_out, q_in_sb, q_in_ss, q_in_sh, q_out_sb, q_out_ss, q_out_sh, q_heads, q_d, q_start,
+                      key, key_out, k_in_sb, k_in_ss, k_in_sh, k_out_sb, k_out_ss, k_out_sh, k_heads, k_d, k_start,
+                      positions, positions_64, positions_per_sequence, inv_freq, batch, s1, rotary_dim, 0, nullptr, 0,
+                      interleaved, inverse, dtype, attention_scale, stream);
+}
+
+int dsa_rope_axes(const void* query, void* query_out, int64_t q_in_sb, int64_t q_in_ss, int64_t q_in_sh, int64_t q_out_sb,
+             int64_t q_out_ss, int64_t q_out_sh, int64_t q_heads, int64_t q_d, int64_t q_start, const void* key,
+             void* key_out, int64_t k_in_sb, int64_t k_in_ss, int64_t k_in_sh, int64_t k_out_sb, int64_t k_out_ss,
+             int64_t k_out_sh, int64_t k_heads, int64_t k_d, int64_t k_start, const void* positions,
+             int32_t positions_64, int32_t positions_per_sequence, const double* inv_freq, int64_t batch, int64_t s1,
+             int64_t rotary_dim, int64_t n_axes, const int64_t* sections, int32_t sections_interleaved,
+             int32_t interleaved, int32_t inverse, int32_t dtype, float attention_scale,
+             void* stream) {
+  clear_error();
+  DSA_CHECK_SUPPORTED(n_axes >= 1 && n_axes <= 4, "the number of axes must be in [1, 4], got %lld", (long long)n_axes);
+  DSA_CHECK_ARG(sections, "null sections");
+  DSA_CHECK_ARG(rotary_dim >= 2 && rotary_dim <= 1024, "rotary dim must be even and in [2, 1024], got %lld",
+                (long long)rotary_dim);
+  int64_t pairs = 0;
+  for (int a = 0; a < n_axes; ++a) {
+    DSA_CHECK_ARG(sections[a] >= 0 && sections[a] <= rotary_dim, "sections must be in [0, rotary dim / 2]");
+    pairs += sections[a];
+  }
+  DSA_CHECK_ARG(2 * pairs == rotary_dim, "sections must add up to half of the rotary dim (%lld), got %lld",
+                (long long)(rotary_dim / 2), (long long)pairs);
+  for (int a = 1; sections_interleaved && a < n_axes; ++a)
+    DSA_CHECK_ARG(sections[a] == 0 || a + (sections[a] - 1) * n_axes < pairs,
+                  "interleaved sections: axis %d has no room for %lld pairs", a, (long long)sections[a]);
+  return rope_checked(query, query_out, q_in_sb, q_in_ss, q_in_sh, q_out_sb, q_out_ss, q_out_sh, q_heads, q_d, q_start,
+                      key, key_out, k_in_sb, k_in_ss, k_in_sh, k_out_sb, k_out_ss, k_out_sh, k_heads, k_d, k_start,
+                      positions, positions_64, positions_per_sequence, inv_freq, batch, s1, rotary_dim, n_axes, sections,
+                      sections_interleaved,
+                      interleaved, inverse, dtype, attention_scale, stream);
 }
 
 int dsa_paged_cache_write(int64_t n_caches, const void* const* rows, void* const* caches, const int64_t* row_bytes,
@@ -213,6 +267,72 @@ int dsa_paged_cache_compact(int64_t n_caches, void* const* caches, const int64_t
   if (st != DSA_OK) return st;
   return pc_compact_run(n_caches, caches, row_bytes, block_table, page_refs, new_block_table, new_page_refs, page_map,
                         rows * max_blocks, num_pages, page_size, workspace, (hipStream_t)stream);
+}
+
+size_t dsa_paged_cache_plan_workspace_size(int64_t rows, int64_t num_pages) {
+  if (rows < 1 || rows > (1 << 24) || num_pages < 1 || num_pages >= (1ll << 31)) return 0;
+  return pc_plan_workspace_bytes(rows, num_pages);
+}
+
+int dsa_paged_cache_plan(const int32_t* block_table, const int32_t* seq_lengths, const int32_t* page_refs,
+                         const int32_t* new_lengths, int32_t* new_block_table, int32_t* new_seq_lengths,
+                         int32_t* new_page_refs, int32_t* slots, int32_t* positions, int32_t* row_lengths,
+                         int64_t rows, int64_t max_blocks, int64_t num_pages, int64_t page_size, int64_t tokens,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  DSA_CHECK_ARG(block_table && seq_lengths && page_refs && new_lengths && new_block_table && new_seq_lengths &&
+                    new_page_refs && row_lengths,
+                "null tensor pointer");
+  DSA_CHECK_ARG(tokens >= 0 && tokens <= (1 << 30), "tokens must be in [0, 2^30]");
+  DSA_CHECK_ARG(tokens == 0 || (slots && positions), "null tensor pointer");
+  int st = check_pages(num_pages, page_size, max_blocks);
+  if (st != DSA_OK) return st;
+  DSA_CHECK_ARG(rows >= 1 && rows <= (1 << 24), "rows of the block table must be in [1, 2^24]");
+  DSA_CHECK_ARG(block_table != new_block_table && seq_lengths != new_seq_lengths && page_refs != new_page_refs,
+                "the new tables must not be the old ones");
+  st = check_workspace(workspace, workspace_bytes, pc_plan_workspace_bytes(rows, num_pages));
+  if (st != DSA_OK) return st;
+  return pc_plan_run(block_table, seq_lengths, page_refs, new_lengths, new_block_table, new_seq_lengths, new_page_refs,
+                     slots, positions, row_lengths, rows, max_blocks, num_pages, page_size, tokens, workspace,
+                     (hipStream_t)stream);
+}
+
+int dsa_paged_cache_write_slots(int64_t n_caches, const void* const* rows, void* const* caches,
+                                const int64_t* row_bytes, const int64_t* row_batch_stride,
+                                const int64_t* row_token_stride, const int32_t* slots, int64_t batch, int64_t s1,
+                                int64_t num_pages, int64_t page_size, void* stream) {
+  clear_error();
+  DSA_CHECK_ARG(n_caches >= 1 && rows && row_batch_stride && row_token_stride, "null row list");
+  DSA_CHECK_ARG(slots, "null tensor pointer");
+  int st = check_pages(num_pages, page_size, 1);
+  if (st != DSA_OK) return st;
+  st = check_caches(n_caches, (const void* const*)caches, row_bytes, page_size);
+  if (st != DSA_OK) return st;
+  for (int64_t i = 0; i < n_caches; ++i) {
+    DSA_CHECK_ARG(rows[i], "null row pointer");
+    DSA_CHECK_ARG(row_batch_stride[i] >= 0 && row_token_stride[i] >= 0 && row_batch_stride[i] < (1ll << 48) &&
+                      row_token_stride[i] < (1ll << 48),
+                  "row strides must be in [0, 2^48)");
+  }
+  DSA_CHECK_ARG(batch >= 1 && s1 >= 1 && batch < (1ll << 31) && s1 < (1ll << 31) &&
+                    within(batch, s1, (1ll << 31) - 1),
+                "tokens must be in [1, 2^31)");
+  return pc_slots_run(n_caches, rows, caches, row_bytes, row_batch_stride, row_token_stride, slots, batch, s1,
+                      num_pages, page_size, (hipStream_t)stream);
+}
+
+int dsa_paged_cache_prefixes(const int32_t* block_table, const int32_t* seq_lengths, int32_t* prefix_groups,
+                             int32_t* prefix_lengths, int64_t rows, int64_t max_blocks, int64_t page_size,
+                             int64_t min_tokens, void* stream) {
+  clear_error();
+  DSA_CHECK_ARG(block_table && seq_lengths && prefix_groups && prefix_lengths, "null tensor pointer");
+  int st = check_pages(1, page_size, max_blocks);
+  if (st != DSA_OK) return st;
+  DSA_CHECK_ARG(rows >= 1 && rows <= (1 << 24), "rows of the block table must be in [1, 2^24]");
+  DSA_CHECK_ARG(min_tokens >= 0 && min_tokens < (1ll << 31), "min_tokens must be in [0, 2^31)");
+  DSA_CHECK_ARG(prefix_groups != prefix_lengths, "groups and lengths must be arrays of their own");
+  return pc_prefixes_run(block_table, seq_lengths, prefix_groups, prefix_lengths, rows, max_blocks, page_size,
+                         min_tokens, (hipStream_t)stream);
 }
 
 size_t dsa_paged_attn_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, int32_t latent,

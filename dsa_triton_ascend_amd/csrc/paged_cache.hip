@@ -608,4 +608,388 @@ int pc_compact_run(int64_t n, void* const* caches, const int64_t* row_bytes, con
   return DSA_OK;
 }
 
+// ---------------------------------------------------------------------------
+// plan: rows extended by numbers of tokens of their own, a slot and a position
+// for each of the packed tokens
+// ---------------------------------------------------------------------------
+struct PcPlanParams {
+  const int32_t *table, *lens, *refs, *more;  // more: new tokens of each row, negative: the row has ended
+  int32_t *new_table, *new_lens, *new_refs, *slots, *positions, *ends;
+  int32_t *start, *freelist;                  // workspace
+  int64_t pages, tokens;
+  int rows, max_blocks, page;
+  int table_blocks;                           // blocks of the table in the second launch
+};
+
+// A row: its tokens, the pages that they hold, and the pages wanted with the
+// new ones (-1 where they would outgrow the table, -2 where the row has ended).
+struct PcRow {
+  int len, held, want;
+};
+
+__device__ __forceinline__ PcRow pc_row(const PcPlanParams& p, int len, int more) {
+  PcRow r;
+  // (below 2^26 tokens, 2^31 new ones, 2^20 of a page: the sums fit 32 bits)
+  const unsigned page = (unsigned)p.page, room = (unsigned)(p.max_blocks * p.page);
+  r.len = (int)min((unsigned)max(len, 0), room);
+  r.held = (int)(((unsigned)r.len + page - 1) / page);
+  const unsigned all = (unsigned)r.len + (unsigned)max(more, 0);
+  r.want = more < 0 ? -2 : (all > room ? -1 : (int)((all + page - 1) / page));
+  return r;
+}
+
+// sums that stop at 2^32 - 1
+__device__ __forceinline__ unsigned pc_add_sat(unsigned a, unsigned b) { return a + b < a ? ~0u : a + b; }
+
+// inclusive such sum over the threads of a block of W waves
+template <int W>
+__device__ __forceinline__ unsigned pc_block_scan_sat(unsigned v, unsigned* s_part, unsigned* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const unsigned x = __shfl_up(v, o);
+    v = lane >= o ? pc_add_sat(v, x) : v;
+  }
+  __syncthreads();
+  if (lane == 63) s_part[wave] = v;
+  __syncthreads();
+  unsigned base = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const unsigned q = s_part[w];
+    if (w < wave) base = pc_add_sat(base, q);
+    all = pc_add_sat(all, q);
+  }
+  *total = all;
+  return pc_add_sat(base, v);
+}
+
+// Block 0 plans: the first of each row's new pages among the free ones (-1: it
+// gets none), and which those are; the lengths and the ends of the rows' tokens.
+// The other blocks copy the counts for the second launch to change.
+__global__ __launch_bounds__(kPcPlanThreads) void pc_plan_kernel(PcPlanParams p) {
+  constexpr int W = kPcPlanThreads / 64;
+  const int tid = threadIdx.x;
+  if (blockIdx.x > 0) {
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * kPcPlanThreads + tid; i < p.pages;
+         i += (int64_t)(gridDim.x - 1) * kPcPlanThreads)
+      p.new_refs[i] = p.refs[i];
+    return;
+  }
+  __shared__ int s_part[W];
+  __shared__ unsigned s_part2[W];
+  // (the first counts are on their way beside what follows)
+  int early[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) early[j] = 4 * tid + j < p.pages ? p.refs[4 * tid + j] : 1;
+  int64_t taken = 0;
+  unsigned end = 0;
+  for (int r0 = 0; r0 < p.rows; r0 += kPcPlanThreads) {
+    const int r = r0 + tid;
+    int need = 0;
+    unsigned more = 0;
+    if (r < p.rows) {
+      const int m = p.more[r];
+      const PcRow k = pc_row(p, p.lens[r], m);
+      need = max(k.want - k.held, 0);
+      more = (unsigned)max(m, 0);
+    }
+    int total;
+    const int incl = pc_block_scan<W>(need, s_part, &total);
+    unsigned all;
+    const unsigned to = pc_add_sat(end, pc_block_scan_sat<W>(more, s_part2, &all));
+    if (r < p.rows) {
+      p.start[r] = (int)min(taken + incl - need, (int64_t)0x7fffffff);
+      p.ends[r] = (int)min(to, 0x7fffffffu);
+    }
+    taken += total;
+    end = pc_add_sat(end, all);
+  }
+  // free pages in ascending order until that many are found
+  int64_t found = 0;
+  for (int64_t i0 = 0; i0 < p.pages && found < taken; i0 += 4 * kPcPlanThreads) {
+    int fr[4], n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t i = i0 + 4 * tid + j;
+      fr[j] = i0 == 0 ? early[j] == 0 : (i < p.pages ? p.refs[i] == 0 : 0);
+      n += fr[j];
+    }
+    int total;
+    int64_t at = found + pc_block_scan<W>(n, s_part, &total) - n;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (fr[j]) p.freelist[at++] = (int)(i0 + 4 * tid + j);
+    found += total;
+  }
+  // a row is served if the free pages last for it and all before it (a thread
+  // reads what it wrote itself)
+  for (int r = tid; r < p.rows; r += kPcPlanThreads) {
+    const int m = p.more[r];
+    const PcRow k = pc_row(p, p.lens[r], m);
+    const int need = max(k.want - k.held, 0);
+    const bool served = k.want >= 0 && (need == 0 || (int64_t)p.start[r] + need <= found);
+    if (!served) p.start[r] = -1;
+    p.new_lens[r] = served ? k.len + m : (k.want == -2 ? 0 : k.len);
+  }
+}
+
+constexpr int kPcEndsHere = 4096;  // rows whose ends a block of tokens keeps in LDS
+
+__global__ __launch_bounds__(kPcThreads) void pc_plan_tables_kernel(PcPlanParams p) {
+  __shared__ int s_ends[kPcEndsHere];
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < p.table_blocks) {
+    const int64_t stride = (int64_t)p.table_blocks * kPcThreads, me = (int64_t)blockIdx.x * kPcThreads + tid;
+    for (int64_t i = me; i < (int64_t)p.rows * p.max_blocks; i += stride) {
+      const int r = i >> 32 ? (int)(i / p.max_blocks) : (int)((unsigned)i / (unsigned)p.max_blocks);
+      const int col = (int)(i - (int64_t)r * p.max_blocks);
+      const int old = p.table[i], at = p.start[r];
+      const PcRow k = pc_row(p, p.lens[r], p.more[r]);
+      int e = -1;
+      if (k.want != -2 && col < k.held) {
+        e = old >= 0 && old < p.pages ? old : -1;
+      } else {
+        if (old >= 0 && old < p.pages) atomicSub(p.new_refs + old, 1);
+        if (at >= 0 && col < k.want) {
+          e = p.freelist[at + col - k.held];
+          atomicAdd(p.new_refs + e, 1);
+        }
+      }
+      p.new_table[i] = e;
+    }
+    return;
+  }
+  // a block's tokens find their rows by the ends
+  const bool here = p.rows <= kPcEndsHere;
+  if (here) {
+    for (int i = tid; i < p.rows; i += kPcThreads) s_ends[i] = p.ends[i];
+    __syncthreads();
+  }
+  const int64_t t = ((int64_t)blockIdx.x - p.table_blocks) * kPcThreads + tid;
+  if (t >= p.tokens) return;
+  int lo = 0, hi = p.rows;  // first r with ends[r] > t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if ((here ? s_ends[mid] : p.ends[mid]) > t) hi = mid; else lo = mid + 1;
+  }
+  int slot = -1, pos = 0;
+  if (lo < p.rows) {
+    const int r = lo, first = r ? (here ? s_ends[r - 1] : p.ends[r - 1]) : 0;
+    const int at = p.start[r];
+    const PcRow k = pc_row(p, p.lens[r], p.more[r]);
+    pos = k.len + (int)(t - first);
+    if (at >= 0) {
+      const int col = (int)((unsigned)pos / (unsigned)p.page);
+      const int blk = col < k.held ? p.table[(int64_t)r * p.max_blocks + col] : p.freelist[at + col - k.held];
+      if (blk >= 0 && blk < p.pages) slot = blk * p.page + (pos - col * p.page);
+    }
+  }
+  p.slots[t] = slot;
+  p.positions[t] = pos;
+}
+
+size_t pc_plan_workspace_bytes(int64_t rows, int64_t pages) { return (size_t)(rows + pages) * sizeof(int32_t); }
+
+int pc_plan_run(const int32_t* table, const int32_t* lens, const int32_t* refs, const int32_t* more,
+                int32_t* new_table, int32_t* new_lens, int32_t* new_refs, int32_t* slots, int32_t* positions,
+                int32_t* ends, int64_t rows, int64_t max_blocks, int64_t pages, int64_t page, int64_t tokens,
+                void* workspace, hipStream_t stream) {
+  PcPlanParams p = {};
+  p.table = table;
+  p.lens = lens;
+  p.refs = refs;
+  p.more = more;
+  p.new_table = new_table;
+  p.new_lens = new_lens;
+  p.new_refs = new_refs;
+  p.slots = slots;
+  p.positions = positions;
+  p.ends = ends;
+  p.start = (int32_t*)workspace;
+  p.freelist = p.start + rows;
+  p.pages = pages;
+  p.tokens = tokens;
+  p.rows = (int)rows;
+  p.max_blocks = (int)max_blocks;
+  p.page = (int)page;
+  int64_t copy_blocks = (pages + 4 * kPcPlanThreads - 1) / (4 * kPcPlanThreads);
+  copy_blocks = copy_blocks > 64 ? 64 : copy_blocks;
+  int64_t tb = (rows * max_blocks + 2 * kPcThreads - 1) / (2 * kPcThreads);
+  tb = tb > 1024 ? 1024 : tb;
+  p.table_blocks = (int)tb;
+  const int64_t grid = tb + (tokens + kPcThreads - 1) / kPcThreads;
+  DSA_CHECK_SUPPORTED(launchable(grid, kPcThreads), "too many tokens for one call");
+  pc_plan_kernel<<<dim3((unsigned)(1 + copy_blocks)), kPcPlanThreads, 0, stream>>>(p);
+  pc_plan_tables_kernel<<<dim3((unsigned)grid), kPcThreads, 0, stream>>>(p);
+  DSA_HIP(hipGetLastError());
+  return DSA_OK;
+}
+
+// ---------------------------------------------------------------------------
+// write to slots: one thread per unit of a token's rows
+// ---------------------------------------------------------------------------
+struct PcSlotParams {
+  PcCache c[kPcMaxCaches];
+  const int32_t* at;
+  int64_t tokens, slots;
+  int n, s, units;
+};
+
+__global__ __launch_bounds__(kPcThreads) void pc_slots_kernel(PcSlotParams p) {
+  const int64_t i = (int64_t)blockIdx.x * kPcThreads + threadIdx.x;
+  const int64_t t = i >> 32 ? i / p.units : (int64_t)((unsigned)i / (unsigned)p.units);
+  if (t >= p.tokens) return;
+  const int u = (int)(i - t * p.units);
+  int ci = 0;
+  while (ci + 1 < p.n && u >= p.c[ci + 1].unit0) ++ci;
+  const PcCache& c = p.c[ci];
+  const int64_t off = (int64_t)(u - c.unit0) << c.shift;
+  const int64_t b = p.s == p.tokens ? 0 : t / p.s;
+  const unsigned char* src = c.src + b * c.src_sb + (t - b * p.s) * c.src_st + off;
+  // (the row is read beside its slot, not behind it)
+  const u32x4 wide = c.shift == 4 ? *(const u32x4*)src : u32x4{0, 0, 0, 0};
+  const int slot = p.at[t];
+  if (slot < 0 || slot >= p.slots) return;
+  unsigned char* dst = c.dst + (int64_t)slot * c.row_bytes + off;
+  if (c.shift == 4) *(u32x4*)dst = wide;
+  else pc_move(dst, src, c.shift);
+}
+
+int pc_slots_run(int64_t n, const void* const* rows, void* const* caches, const int64_t* row_bytes,
+                 const int64_t* row_sb, const int64_t* row_st, const int32_t* slots, int64_t batch, int64_t s,
+                 int64_t pages, int64_t page, hipStream_t stream) {
+  PcSlotParams p = {};
+  p.at = slots;
+  p.tokens = batch * s;
+  p.slots = pages * page;
+  p.s = (int)s;
+  // blocks of the launch for the caches from c0 on
+  auto take = [&](int64_t c0) {
+    p.n = (int)(n - c0 < kPcMaxCaches ? n - c0 : kPcMaxCaches);
+    int64_t units = 0;
+    for (int i = 0; i < p.n; ++i) {
+      PcCache& c = p.c[i];
+      const int64_t k = c0 + i;
+      c.src = (const unsigned char*)rows[k];
+      c.dst = (unsigned char*)caches[k];
+      c.src_sb = row_sb[k];
+      c.src_st = row_st[k];
+      c.row_bytes = (int)row_bytes[k];
+      c.shift = pc_shift((uint64_t)(uintptr_t)c.src | (uintptr_t)c.dst | (uint64_t)row_bytes[k] |
+                         (uint64_t)row_sb[k] | (uint64_t)row_st[k]);
+      c.unit0 = (int)units;
+      units += row_bytes[k] >> c.shift;
+    }
+    p.units = (int)units;  // (at most 32 rows of 2^24 bytes)
+    return (p.tokens * units + kPcThreads - 1) / kPcThreads;
+  };
+  // (all of them before the first: a call that is refused has written nothing)
+  for (int64_t c0 = n > kPcMaxCaches ? 0 : n; c0 < n; c0 += kPcMaxCaches)
+    DSA_CHECK_SUPPORTED(launchable(take(c0), kPcThreads), "too many rows for one call");
+  for (int64_t c0 = 0; c0 < n; c0 += kPcMaxCaches) {
+    const int64_t grid = take(c0);
+    DSA_CHECK_SUPPORTED(launchable(grid, kPcThreads), "too many rows for one call");
+    pc_slots_kernel<<<dim3((unsigned)grid), kPcThreads, 0, stream>>>(p);
+    DSA_HIP(hipGetLastError());
+  }
+  return DSA_OK;
+}
+
+// ---------------------------------------------------------------------------
+// prefixes: neighbouring rows that begin with the same full pages
+// ---------------------------------------------------------------------------
+struct PcPrefixParams {
+  const int32_t *table, *lens;
+  int32_t *groups, *lengths;
+  int rows, max_blocks, page, min_pages;
+};
+
+// Leading full pages that row b has in common with the row before it, the same
+// on all lanes of the wave; 0 if they are too few to count.
+__device__ __forceinline__ int pc_common(const PcPrefixParams& p, int b, int lane) {
+  const int tokens = min(p.lens[b], p.lens[b - 1]);
+  const int whole = min(max(tokens, 0) / p.page, p.max_blocks);
+  const int32_t *x = p.table + (int64_t)b * p.max_blocks, *y = x - p.max_blocks;
+  constexpr int kAhead = 8;  // columns of a lane on their way at a time
+  for (int c0 = 0; c0 < whole; c0 += 64 * kAhead) {
+    int e[kAhead], f[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int c = min(c0 + j * 64 + lane, p.max_blocks - 1);
+      e[j] = x[c];
+      f[j] = y[c];
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int c = c0 + j * 64 + lane;
+      const unsigned long long apart = __ballot(c >= whole || e[j] != f[j] || e[j] < 0);
+      if (apart) {
+        const int n = c0 + j * 64 + __ffsll(apart) - 1;
+        return n >= p.min_pages ? n : 0;
+      }
+    }
+  }
+  return whole >= p.min_pages ? whole : 0;
+}
+
+// a wave per row: common pages to groups
+__global__ __launch_bounds__(kPcThreads) void pc_common_kernel(PcPrefixParams p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t b = (int64_t)blockIdx.x * (kPcThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (b >= p.rows) return;
+  const int n = b ? pc_common(p, (int)b, lane) : 0;
+  if (lane == 0) p.groups[b] = n;
+}
+
+// One workgroup: runs of linked rows and the least that they share.
+__global__ __launch_bounds__(kPcPlanThreads) void pc_groups_kernel(PcPrefixParams p) {
+  constexpr int W = kPcPlanThreads / 64;
+  __shared__ int s_last[W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int b = tid; b < p.rows; b += kPcPlanThreads)
+    __hip_atomic_store(p.lengths + b, 0x7fffffff, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  int before = 0;  // first row of the group that the chunk's first rows may belong to
+  for (int b0 = 0; b0 < p.rows; b0 += kPcPlanThreads) {
+    const int b = b0 + tid;
+    const int common = b < p.rows ? p.groups[b] : 0;
+    // first row of the group: the last row up to b that is not linked
+    const unsigned long long starts = __ballot(common == 0);
+    __syncthreads();
+    if (lane == 0) s_last[wave] = starts ? b0 + wave * 64 + 63 - __clzll(starts) : -1;
+    __syncthreads();
+    const unsigned long long mine = starts & (~0ull >> (63 - lane));
+    int first = -1, last = before;
+    for (int w = 0; w < W; ++w) {
+      const int x = s_last[w];
+      if (w == wave) first = mine ? b0 + wave * 64 + 63 - __clzll(mine) : last;
+      if (x >= 0) last = x;
+    }
+    before = last;
+    if (b < p.rows) {
+      if (common) atomicMin(p.lengths + first, common * p.page);
+      p.groups[b] = first;
+    }
+  }
+  __syncthreads();
+  for (int b = tid; b < p.rows; b += kPcPlanThreads) {
+    const int first = p.groups[b];
+    const int n = __hip_atomic_load(p.lengths + first, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // (a row alone writes its own; the others of a group write what its first row has)
+    __hip_atomic_store(p.lengths + b, n == 0x7fffffff ? 0 : n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+}
+
+int pc_prefixes_run(const int32_t* table, const int32_t* lens, int32_t* groups, int32_t* lengths, int64_t rows,
+                    int64_t max_blocks, int64_t page, int64_t min_tokens, hipStream_t stream) {
+  PcPrefixParams p = {table, lens, groups, lengths, (int)rows, (int)max_blocks, (int)page, 1};
+  const int64_t pages = (min_tokens + page - 1) / page;
+  p.min_pages = (int)(pages < 1 ? 1 : pages);
+  pc_common_kernel<<<dim3((unsigned)((rows + kPcThreads / 64 - 1) / (kPcThreads / 64))), kPcThreads, 0, stream>>>(p);
+  pc_groups_kernel<<<dim3(1), kPcPlanThreads, 0, stream>>>(p);
+  DSA_HIP(hipGetLastError());
+  return DSA_OK;
+}
+
 }  // namespace dsa

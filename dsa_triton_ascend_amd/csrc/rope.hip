@@ -11,6 +11,12 @@
 // are taken in 32 bits, once per token and frequency, into LDS; all heads of
 // the token share them.  No table of positions is read or kept.
 //
+// With several axes (time, height, width) a token has a position on each, and
+// every pair of columns belongs to one axis: contiguous sections of pairs, or
+// pair i to axis i % A while that axis has pairs left and to the first after.
+// Which axis that is takes a few comparisons where the angles are made, once
+// per token and frequency.
+//
 // Bound by memory (3 flops per element), or by the launch for one decoding
 // step.  A thread moves 16 bytes (two times 16 for pairs in the half layout),
 // neighbouring threads neighbouring chunks of a head; heads and tokens are
@@ -42,7 +48,18 @@ struct RopeParams {
   int rot, rot_units, interleaved;
   int tok_wg, parts, per_part;     // tokens of a workgroup; unit ranges they are cut into
   float scale, sign;
+  int axes, axes_interleaved;      // axes: 0 where a token has one position
+  int sec[4];                      // pairs of each axis (interleaved), or the pairs up to its end
+  int64_t axis_stride;             // positions of an axis
 };
+
+// axis of pair f
+__device__ __forceinline__ int rope_axis(const RopeParams& p, int f) {
+  if (!p.axes_interleaved) return (f >= p.sec[0]) + (f >= p.sec[1]) + (f >= p.sec[2]);
+  const int a = (int)((unsigned)f % (unsigned)p.axes);
+  const int n = a == 0 ? p.sec[0] : (a == 1 ? p.sec[1] : (a == 2 ? p.sec[2] : p.sec[3]));
+  return f < p.axes * n ? a : 0;
+}
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeDeep = 3;
@@ -87,7 +104,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeParams p) {
   for (int i = threadIdx.x; i < ntok * half; i += kRopeThreads) {
     const int tk = i / half, f = i - tk * half;
     const int64_t t = tok0 + tk;
-    const int64_t pi = p.pos_per_seq ? t : t % p.s;
+    int64_t pi = p.pos_per_seq ? t : t % p.s;
+    if (p.axes) pi += rope_axis(p, f) * p.axis_stride;
     const double pos = p.pos64 ? (double)((const int64_t*)p.pos)[pi] : (double)((const int32_t*)p.pos)[pi];
     const double turns = pos * (p.inv_freq[f] * 0.15915494309189533577);  // 1 / (2 pi)
     float sn, cs;
@@ -204,11 +222,12 @@ static void rope_launch(const RopeParams& p, int vec, bool inplace, bool streami
   else rope_kernel<T, VEC, false, false><<<g, kRopeThreads, 0, stream>>>(p);
 }
 
-// strides: in (batch, token, head) then out, in elements
+// strides: in (batch, token, head) then out, in elements; axes 0 or 1 to 4 with their pairs
 int rope_run(const void* const in[2], void* const out[2], const int64_t* const strides[2], const int64_t heads[2],
              const int64_t d[2], const int64_t start[2], int n, const void* positions, int32_t pos64,
              int32_t pos_per_seq, const double* inv_freq, int64_t tokens, int64_t s, int64_t rot, int32_t interleaved,
-             int32_t inverse, int32_t dtype, float scale, hipStream_t stream) {
+             int32_t inverse, int32_t dtype, float scale, int64_t axes, const int64_t* sections,
+             int32_t axes_interleaved, hipStream_t stream) {
   const int es = dtype == DSA_DTYPE_FP32 ? 4 : 2;
   const int full = 16 / es;
   // 16-byte chunks: every column count, offset, stride and address a whole
@@ -253,6 +272,14 @@ int rope_run(const void* const in[2], void* const out[2], const int64_t* const s
   p.pos_per_seq = pos_per_seq;
   p.scale = scale;
   p.sign = inverse ? -1.f : 1.f;
+  p.axes = (int)axes;
+  p.axes_interleaved = axes_interleaved;
+  p.axis_stride = pos_per_seq ? tokens : s;
+  for (int a = 0, end = 0; a < 4; ++a) {
+    const int n = a < axes ? (int)sections[a] : 0;
+    end += n;
+    p.sec[a] = axes_interleaved ? n : end;
+  }
   // tokens of few units share a workgroup; tokens of many are cut into parts
   // where they alone would not give every CU a few workgroups
   p.tok_wg = 1;

@@ -45,6 +45,11 @@ struct Entries {
   decltype(&dsa_paged_attn_workspace_size) attn_bytes;
   decltype(&dsa_paged_attn) attn;
   decltype(&dsa_last_error) error;
+  decltype(&dsa_rope_axes) rope_axes;
+  decltype(&dsa_paged_cache_plan_workspace_size) plan_bytes;
+  decltype(&dsa_paged_cache_plan) plan;
+  decltype(&dsa_paged_cache_write_slots) write_slots;
+  decltype(&dsa_paged_cache_prefixes) prefixes;
 } entry;
 
 // the HIP runtime reported an error at or before a launch
@@ -335,6 +340,86 @@ PyObject* attention(PyObject* const* a) {
   return triple(std::move(out), std::move(mx), std::move(sm));
 }
 
+// (block_table, seq_lengths, page_refs, new_lengths, page_size, tokens) -> six tensors
+PyObject* plan(PyObject* const* a) {
+  int index = -1;
+  int64_t page, tokens;
+  const at::Tensor *table = ints(a[0], &index, 2), *lens = ints(a[1], &index, 1), *refs = ints(a[2], &index, 1);
+  const at::Tensor* more = ints(a[3], &index, 1);
+  if (!table || !lens || !refs || !more || !current(index)) return nullptr;
+  if (!integer(a[4], &page) || !integer(a[5], &tokens) || tokens < 1 || tokens > (1 << 30)) return nullptr;
+  const int64_t rows = table->size(0), pages = refs->size(0);
+  if (lens->size(0) != rows || more->size(0) != rows) return nullptr;
+  at::Tensor t[6] = {fresh(table->sizes(), *table), fresh({rows}, *table),   fresh({pages}, *table),
+                     fresh({tokens}, *table),       fresh({tokens}, *table), fresh({rows}, *table)};
+  const size_t bytes = entry.plan_bytes(rows, pages);
+  c10::DataPtr ws = workspace(bytes);
+  auto at = [&](int i) { return (int32_t*)t[i].data_ptr(); };
+  if (!launched(entry.plan, data(table), data(lens), data(refs), data(more), at(0), at(1), at(2), at(3), at(4), at(5),
+                rows, table->size(1), pages, page, tokens, ws.get(), bytes, stream_of(index)))
+    return nullptr;
+  PyObject* r = PyTuple_New(6);
+  if (!r) return nullptr;
+  for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(std::move(t[i])));
+  return r;
+}
+
+// (caches, rows, slots) -> True
+PyObject* write_slots(PyObject* const* a) {
+  int index = -1;
+  Caches c;
+  if (!c.read(a[0], &index) || c.t.empty()) return nullptr;
+  const at::Tensor* slots = tensor(a[2], &index);
+  if (!slots || !current(index) || slots->scalar_type() != at::kInt || !slots->is_contiguous() || slots->numel() == 0)
+    return nullptr;
+  const int64_t lead = slots->dim();
+  PyObject **list, *self;
+  int64_t n;
+  if ((lead != 1 && lead != 2) || !items(a[1], &list, &self, &n) || n != (int64_t)c.t.size()) return nullptr;
+  std::vector<const void*> src(n);
+  std::vector<int64_t> sb(n), st(n);
+  for (int64_t i = 0; i < n; ++i) {
+    const at::Tensor* r = tensor(list[i], &index);
+    const at::Tensor& k = *c.t[i];
+    if (!r || r->dim() != lead + k.dim() - 2 || r->scalar_type() != k.scalar_type() || differentiable(*r)) return nullptr;
+    for (int64_t d = 0; d < lead; ++d)
+      if (r->size(d) != slots->size(d)) return nullptr;
+    int64_t step = 1;
+    for (int64_t d = r->dim() - 1; d >= lead; --d) {
+      if (r->size(d) != k.size(d - lead + 2) || (r->stride(d) != step && r->size(d) != 1)) return nullptr;
+      step *= r->size(d);
+    }
+    const int64_t es = (int64_t)r->element_size();
+    src[i] = r->data_ptr();
+    sb[i] = lead == 1 ? 0 : r->stride(0) * es;
+    st[i] = r->stride(lead - 1) * es;
+  }
+  changed(c);
+  if (!launched(entry.write_slots, n, src.data(), c.at.data(), c.row_bytes.data(), sb.data(), st.data(), data(slots),
+                lead == 1 ? (int64_t)1 : slots->size(0), slots->size(lead - 1), c.pages, c.page, stream_of(index)))
+    return nullptr;
+  Py_RETURN_TRUE;
+}
+
+// (block_table, seq_lengths, page_size, min_tokens) -> pair
+PyObject* prefixes(PyObject* const* a) {
+  int index = -1;
+  int64_t page, least;
+  const at::Tensor *table = ints(a[0], &index, 2), *lens = ints(a[1], &index, 1);
+  if (!table || !lens || !current(index) || !integer(a[2], &page) || !integer(a[3], &least)) return nullptr;
+  const int64_t rows = table->size(0);
+  if (lens->size(0) != rows) return nullptr;
+  at::Tensor groups = fresh({rows}, *table), lengths = fresh({rows}, *table);
+  if (!launched(entry.prefixes, data(table), data(lens), (int32_t*)groups.data_ptr(), (int32_t*)lengths.data_ptr(),
+                rows, table->size(1), page, least, stream_of(index)))
+    return nullptr;
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(groups)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(lengths)));
+  return pair;
+}
+
 // whether two elements of a strided tensor may share an address
 bool overlaps_itself(const at::Tensor& t) {
   std::vector<std::pair<int64_t, int64_t>> d;  // stride, size
@@ -397,6 +482,9 @@ struct Rotation {
   int64_t start[2];  // of the query's and the key's rotated columns
   double scale;
   bool tnd, interleaved, inverse;
+  int64_t axes = 0;  // of the positions: 0, or as many as there are sections
+  int64_t sections[4] = {};
+  bool sections_interleaved = false;
 };
 
 // Rotates in[0] and, if defined, in[1] into out; false if the call is not an
@@ -434,9 +522,22 @@ bool rotated(const Rotation& r, const at::Tensor in[2], const at::Tensor& pos, c
   }
   if (inplace && in[1].defined() && (from[0] == from[1] || share_memory(q, in[1], r.start, rot))) return false;
   const int64_t b = r.tnd ? 1 : q.size(0), s = q.size(lead - 1);
-  const bool full = pos.dim() == lead && (r.tnd || pos.size(0) == b) && pos.size(lead - 1) == s;
-  const bool shared = !r.tnd && pos.dim() == 1 && pos.size(0) == s;
+  const int64_t first = r.axes > 0;  // dimension of the axes before the others
+  if (first && (pos.dim() < 1 || pos.size(0) != r.axes)) return false;
+  const bool full = pos.dim() == first + lead && (r.tnd || pos.size(first) == b) && pos.size(first + lead - 1) == s;
+  const bool shared = !r.tnd && pos.dim() == first + 1 && pos.size(first) == s;
   if (!full && !shared) return false;
+  if (r.axes) {
+    int64_t pairs = 0;
+    for (int64_t a = 0; a < r.axes; ++a) pairs += r.sections[a];
+    if (pairs != freq.size(0)) return false;
+    return launched(entry.rope_axes, from[0], to[0], si[0][0], si[0][1], si[0][2], so[0][0], so[0][1], so[0][2],
+                    heads[0], cols[0], r.start[0], from[1], to[1], si[1][0], si[1][1], si[1][2], so[1][0], so[1][1],
+                    so[1][2], heads[1], cols[1], in[1].defined() ? r.start[1] : 0, pos.data_ptr(),
+                    pos.scalar_type() == at::kLong, full, (const double*)freq.data_ptr(), b, s, rot, r.axes,
+                    (const int64_t*)r.sections, (int32_t)r.sections_interleaved, r.interleaved, r.inverse, dtype,
+                    (float)r.scale, stream_of((int)q.get_device()));
+  }
   return launched(entry.rope, from[0], to[0], si[0][0], si[0][1], si[0][2], so[0][0], so[0][1], so[0][2], heads[0],
                   cols[0], r.start[0], from[1], to[1], si[1][0], si[1][1], si[1][2], so[1][0], so[1][1], so[1][2],
                   heads[1], cols[1], in[1].defined() ? r.start[1] : 0, pos.data_ptr(), pos.scalar_type() == at::kLong,
@@ -519,7 +620,8 @@ bool rotated_with_gradient(const Rotation& r, const at::Tensor in[2], const at::
 }
 
 // (query, key, positions, inv_freq, interleaved, rotary_offset, key_rotary_offset, attention_scale, layout,
-// inverse, inplace) -> (query_out, key_out)
+// inverse, inplace[, sections, sections_interleaved]) -> (query_out, key_out)
+template <bool AXES>
 PyObject* rotate(PyObject* const* a) {
   const int tnd = layout(a[8]);
   int index = -1;
@@ -533,6 +635,14 @@ PyObject* rotate(PyObject* const* a) {
   if (!flag(a[4], &r.interleaved) || !integer(a[5], &r.start[0]) || !number(a[7], &r.scale) ||
       !flag(a[9], &r.inverse) || !flag(a[10], &inplace))
     return nullptr;
+  if (AXES) {
+    if ((!PyTuple_CheckExact(a[11]) && !PyList_CheckExact(a[11])) || !flag(a[12], &r.sections_interleaved)) return nullptr;
+    r.axes = PySequence_Fast_GET_SIZE(a[11]);
+    if (r.axes < 1 || r.axes > 4) return nullptr;
+    for (int64_t i = 0; i < r.axes; ++i)
+      if (!integer(PySequence_Fast_ITEMS(a[11])[i], &r.sections[i]) || r.sections[i] < 0 || r.sections[i] > 512)
+        return nullptr;
+  }
   r.start[1] = r.start[0];
   if (a[6] != Py_None && !integer(a[6], &r.start[1])) return nullptr;
   const bool grad = c10::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()));
@@ -600,7 +710,11 @@ PyMethodDef methods[] = {
     {"fork", FAST((call<fork, 7>)), METH_FASTCALL, nullptr},
     {"compact", FAST((call<compact, 4>)), METH_FASTCALL, nullptr},
     {"attention", FAST((call<attention, 13>)), METH_FASTCALL, nullptr},
-    {"rotate", FAST((call<rotate, 11>)), METH_FASTCALL, nullptr},
+    {"rotate", FAST((call<rotate<false>, 11>)), METH_FASTCALL, nullptr},
+    {"rotate_axes", FAST((call<rotate<true>, 13>)), METH_FASTCALL, nullptr},
+    {"plan", FAST((call<plan, 6>)), METH_FASTCALL, nullptr},
+    {"write_slots", FAST((call<write_slots, 3>)), METH_FASTCALL, nullptr},
+    {"prefixes", FAST((call<prefixes, 4>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, methods};
 

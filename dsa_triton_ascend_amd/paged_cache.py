@@ -1,5 +1,6 @@
 """Pages of a cache on MI355X: writing new tokens, forking, releasing and
-extending sequences, and compaction.
+extending sequences, planning a step of requests of many lengths, finding the
+prefixes that sequences share, and compaction.
 
 The attention and indexer operators read caches in the PA_BSND layout,
 ``[pages, page_size, heads, columns]``, through a block table ``[B,
@@ -21,6 +22,13 @@ One decoding step:
     paged_cache_write([latent, k_rope, k_index], [...], table, lens)                         # per layer
     out, _, _ = paged_attention(q, latent_cache, None, table, lens + 1, ...)                 # per layer
     lens = lens + 1                                                                          # of rows in use
+
+One step of requests with new tokens of their own number each, packed:
+
+    table, lens, refs, slots, positions, ends = paged_cache_plan(table, lens, refs, new, page, tokens)   # once
+    groups, shared = paged_cache_prefixes(table, lens, page)                                             # once
+    paged_cache_write_slots([latent, k_rope, k_index], [...], slots)                                     # per layer
+    out, _, _ = paged_prefix_attention(q, latent_cache, None, table, lens, groups, shared, ...)          # per layer
 """
 from array import array
 
@@ -90,6 +98,34 @@ def _longs(*lists):
     return a, out
 
 
+def _sources(rows, caches, lead):
+    """Addresses and byte strides (batch, token) of the new rows, whose first
+    ``lead`` dimensions are tokens, and the tensors that hold them."""
+    sources, sb, st, kept = [], [], [], []
+    tokens = rows[0].shape[:lead]
+    for r, c in zip(rows, caches):
+        shape, inner = r.shape, c.shape[2:]
+        if shape[lead:] != inner:
+            raise ValueError(f"rows {tuple(shape)} do not fit a cache {tuple(c.shape)}")
+        if shape[:lead] != tokens:
+            raise ValueError(f"rows must have the same tokens for all caches, got {tuple(tokens)} and {tuple(shape)}")
+        if r.dtype != c.dtype:
+            raise ValueError(f"rows dtype {r.dtype} differs from cache dtype {c.dtype}")
+        stride, step = r.stride(), 1
+        for i in range(len(shape) - 1, lead - 1, -1):  # a token's row has to be in one piece
+            if stride[i] != step and shape[i] != 1:
+                r = r.contiguous()
+                stride = r.stride()
+                break
+            step *= shape[i]
+        es = r.element_size()
+        kept.append(r)
+        sources.append(r.data_ptr())
+        sb.append(stride[0] * es if lead == 2 else 0)
+        st.append(stride[lead - 1] * es)
+    return sources, sb, st, kept
+
+
 def paged_cache_write(caches, rows, block_table, seq_lengths, row_lengths=None, layout="BSND"):
     """Write new tokens' rows into the pages of their sequences, in place.
 
@@ -129,27 +165,7 @@ def paged_cache_write(caches, rows, block_table, seq_lengths, row_lengths=None, 
     tokens = rows[0].shape[:lead]
     if lead == 2 and tokens and tokens[0] != batch:
         raise ValueError(f"rows must be [B={batch}, S, ...], got {tuple(rows[0].shape)}")
-    sources, sb, st, kept = [], [], [], []
-    for r, c in zip(rows, caches):
-        shape, inner = r.shape, c.shape[2:]
-        if shape[lead:] != inner:
-            raise ValueError(f"rows {tuple(shape)} do not fit a cache {tuple(c.shape)}")
-        if shape[:lead] != tokens:
-            raise ValueError(f"rows must have the same tokens for all caches, got {tuple(tokens)} and {tuple(shape)}")
-        if r.dtype != c.dtype:
-            raise ValueError(f"rows dtype {r.dtype} differs from cache dtype {c.dtype}")
-        stride, step = r.stride(), 1
-        for i in range(len(shape) - 1, lead - 1, -1):  # a token's row has to be in one piece
-            if stride[i] != step and shape[i] != 1:
-                r = r.contiguous()
-                stride = r.stride()
-                break
-            step *= shape[i]
-        es = r.element_size()
-        kept.append(r)
-        sources.append(r.data_ptr())
-        sb.append(stride[0] * es if lead == 2 else 0)
-        st.append(stride[lead - 1] * es)
+    sources, sb, st, kept = _sources(rows, caches, lead)
     _lib.no_derivatives("paged_cache_write", *caches, *rows)
     index = _lib.same_device(table, lens, row_lengths, *caches, *kept)
     n_tok = tokens[0] if lead == 1 else tokens[0] * tokens[1]
@@ -233,6 +249,136 @@ def paged_cache_fork(caches, block_table, seq_lengths, page_refs, parents=None, 
         _lib.check(status, "dsa_paged_cache_fork")
     _lib.changed(*caches)
     return new_table, new_lens, new_refs
+
+
+def paged_cache_plan(block_table, seq_lengths, page_refs, new_lengths, page_size, tokens):
+    """Tables, slots and positions of a step that adds ``new_lengths[r]`` tokens
+    to row r (int32 [R], a number of its own for each row; negative: the
+    request has ended and its row is released).
+
+    Row r gets pages for its new tokens, lowest free ones first, to rows in
+    order.  A row for which they do not last, every later row that needs any,
+    and a row that would outgrow the table are refused: they keep their pages
+    and their length, and get no new tokens (the length shows it), so that they
+    can wait in place.  Pages freed by the call are not handed out in it.
+    Pages of the old table past a row's last token are released, as by
+    ``paged_cache_fork``.  A partly filled last page that rows share is not to
+    be written: fork first.  A length below zero counts as zero.
+
+    The step's new tokens lie packed, row after row: ``tokens`` places (at least
+    as many as there are new tokens; an integer, known without reading the
+    device; more, as padding, are allowed).
+
+    Returns ``(block_table, seq_lengths, page_refs, slots, positions,
+    row_lengths)``, all int32: the state with the new tokens in it (an ended
+    row: length 0, no pages); each token's place for ``paged_cache_write_slots``
+    (-1: a refused row's, or padding) and its position for ``rotary_embedding``
+    (0 for padding), [tokens]; and the cumulative numbers of new tokens [R], as
+    the packed layouts ("TND") take them (those of refused rows are counted).
+    """
+    state = _lib.calls().plan(block_table, seq_lengths, page_refs, new_lengths, page_size, tokens)
+    if state is not None:
+        return state
+    table = _ints(block_table, "block_table", 2)
+    rows, wide = table.shape
+    lens = _ints(seq_lengths, "seq_lengths", 1)
+    more = _ints(new_lengths, "new_lengths", 1)
+    refs = _ints(page_refs, "page_refs", 1)
+    for name, t in (("seq_lengths", lens), ("new_lengths", more)):
+        if t.shape[0] != rows:
+            raise ValueError(f"{name} must have one entry per row of block_table ({rows}), got {t.shape[0]}")
+    if int(page_size) != page_size or page_size < 1:
+        raise ValueError(f"page_size must be a positive integer, got {page_size}")
+    if int(tokens) != tokens or not 0 <= tokens <= 2 ** 30:
+        raise ValueError(f"tokens must be an integer in [0, 2^30], got {tokens}")
+    index = _lib.same_device(table, lens, more, refs)
+    tokens, pages = int(tokens), refs.shape[0]
+    new_table, new_lens, new_refs = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
+    slots, positions, ends = lens.new_empty(tokens), lens.new_empty(tokens), torch.empty_like(lens)
+    lib = _lib.load()
+    nbytes = lib.dsa_paged_cache_plan_workspace_size(rows, pages)
+    ws = refs.new_empty((nbytes + 3) // 4)
+    status = _lib.call_on(
+        index, lib.dsa_paged_cache_plan, table.data_ptr(), lens.data_ptr(), refs.data_ptr(), more.data_ptr(),
+        new_table.data_ptr(), new_lens.data_ptr(), new_refs.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+        ends.data_ptr(), rows, wide, pages, int(page_size), tokens, ws.data_ptr(), nbytes, _lib.raw_stream(index))
+    if status:
+        _lib.check(status, "dsa_paged_cache_plan")
+    return new_table, new_lens, new_refs, slots, positions, ends
+
+
+def paged_cache_write_slots(caches, rows, slots):
+    """Write packed rows into the slots of a plan, in place.
+
+    ``rows[i]`` [T, ...] or [B, S, ...] holds rows of ``caches[i]`` [pages,
+    page_size, ...], of its dtype and trailing sizes, outside the caches; batch
+    and token strides are free.  ``slots`` (int32 [T] or [B, S]) names each
+    token's place, ``page * page_size + offset``; a token whose place lies
+    outside the caches (-1) is not written.  No place may be given twice.
+    Without a search of tables and lengths in it, this is the form for many
+    layers that share one plan.  Returns None.
+    """
+    if _lib.calls().write_slots(caches, rows, slots):
+        return
+    caches, rows = _list(caches, "caches"), _list(rows, "rows")
+    if len(caches) != len(rows) or not caches:
+        raise ValueError(f"one tensor of rows per cache is needed, got {len(rows)} for {len(caches)}")
+    pages, page, addresses, sizes = _check_caches(caches)
+    if slots.dtype != _INT:
+        raise ValueError(f"slots must be int32, got {slots.dtype}")
+    lead = slots.dim()
+    if lead not in (1, 2):
+        raise ValueError(f"slots must be [T] or [B, S], got {tuple(slots.shape)}")
+    slots = slots if slots.is_contiguous() else slots.contiguous()
+    sources, sb, st, kept = _sources(rows, caches, lead)
+    if rows[0].shape[:lead] != slots.shape:
+        raise ValueError(f"rows must have the tokens of slots {tuple(slots.shape)}, got {tuple(rows[0].shape)}")
+    _lib.no_derivatives("paged_cache_write_slots", *caches, *rows)
+    index = _lib.same_device(slots, *caches, *kept)
+    if slots.numel() == 0:
+        return
+    owner, (a_src, a_dst, a_size, a_sb, a_st) = _longs(sources, addresses, sizes, sb, st)
+    status = _lib.call_on(
+        index, _lib.load().dsa_paged_cache_write_slots, len(caches), a_src, a_dst, a_size, a_sb, a_st,
+        slots.data_ptr(), 1 if lead == 1 else slots.shape[0], slots.shape[-1], pages, page, _lib.raw_stream(index))
+    if status:
+        _lib.check(status, "dsa_paged_cache_write_slots")
+    _lib.changed(*caches)
+
+
+def paged_cache_prefixes(block_table, seq_lengths, page_size, min_tokens=1):
+    """Which neighbouring sequences begin with the same pages, for
+    ``paged_prefix_attention``: of beams, after a fork, or of requests behind a
+    common prompt.
+
+    Row b is linked to the row before it if both sequences begin with the same
+    full pages, one page and ``min_tokens`` tokens at least.  Returns
+    ``(prefix_groups, prefix_lengths)``, int32 [R]: for each row the first row
+    of its run of linked rows, and the tokens that all of the run share: the
+    least that two neighbours in it do (whole pages; 0 for a row without links).
+    Put rows that share much next to each other; where one neighbour shares
+    little of a long common prefix, a ``min_tokens`` above that keeps it apart.
+    """
+    result = _lib.calls().prefixes(block_table, seq_lengths, page_size, min_tokens)
+    if result is not None:
+        return result
+    table = _ints(block_table, "block_table", 2)
+    rows, wide = table.shape
+    lens = _ints(seq_lengths, "seq_lengths", 1)
+    if lens.shape[0] != rows:
+        raise ValueError(f"seq_lengths must have one entry per row of block_table ({rows}), got {lens.shape[0]}")
+    if int(page_size) != page_size or page_size < 1:
+        raise ValueError(f"page_size must be a positive integer, got {page_size}")
+    if int(min_tokens) != min_tokens or not 0 <= min_tokens < 2 ** 31:
+        raise ValueError(f"min_tokens must be an integer in [0, 2^31), got {min_tokens}")
+    index = _lib.same_device(table, lens)
+    groups, lengths = torch.empty_like(lens), torch.empty_like(lens)
+    status = _lib.call_on(
+        index, _lib.load().dsa_paged_cache_prefixes, table.data_ptr(), lens.data_ptr(), groups.data_ptr(),
+        lengths.data_ptr(), rows, wide, int(page_size), int(min_tokens), _lib.raw_stream(index))
+    if status:
+        _lib.check(status, "dsa_paged_cache_prefixes")
+    return groups, lengths
 
 
 def paged_cache_compact(caches, block_table, page_refs, page_size=None):

@@ -3,12 +3,14 @@ the attention operators and rotates the indexer's queries and keys.
 
 ``rotary_embedding`` turns a slice of every head of a query and, in the same
 launch, of a key; ``rotary_frequencies`` gives its frequencies, plain or
-scaled for contexts longer than the trained one.  The reference has no such
-operator: it takes rotated inputs.
+scaled for contexts longer than the trained one.  Tokens of images and video
+may have a position on each of several axes (``sections``).  The reference has
+no such operator: it takes rotated inputs.
 
 Angles ``position * inv_freq`` are formed in 64 bits inside the kernel, so
 positions up to 2^31 are exact to fp32 and no table is kept.
 """
+import ctypes
 import math
 
 import torch
@@ -138,10 +140,12 @@ def _side(t, start, inplace):
 _NO_KEY = (None, None) + (0,) * 9
 
 
-def _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, inplace):
-    """Launch on checked arguments; returns the rotated query and key."""
-    result = _lib.calls().rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale,
-                                 "BSND" if query.dim() == 4 else "TND", inverse, inplace)
+def _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scale, inverse, inplace, axes=None):
+    """Launch on checked arguments; returns the rotated query and key.
+    ``axes``: None, or the pairs of each axis and whether they are interleaved."""
+    args = (query, key, positions, inv_freq, interleaved, q_start, k_start, scale,
+            "BSND" if query.dim() == 4 else "TND", inverse, inplace)
+    result = _lib.calls().rotate(*args) if axes is None else _lib.calls().rotate_axes(*args, *axes)
     if result is not None:
         return result
     query, q_out, q_args = _side(query, q_start, inplace)
@@ -153,19 +157,25 @@ def _rotate(query, key, positions, inv_freq, interleaved, q_start, k_start, scal
     if b == 0 or s == 0:
         return q_out, k_out
     index = query.get_device()
+    lib = _lib.load()
+    fn, extra, rank = lib.dsa_rope, (), positions.dim()
+    if axes is not None:
+        fn, rank = lib.dsa_rope_axes, rank - 1
+        extra = len(axes[0]), (ctypes.c_int64 * len(axes[0]))(*axes[0]), axes[1]
     status = _lib.call_on(
-        index, _lib.load().dsa_rope, *q_args, *k_args, positions.data_ptr(), positions.dtype == torch.int64,
-        len(shape) == 3 or positions.dim() == 2, inv_freq.data_ptr(), b, s, 2 * inv_freq.shape[0], interleaved, inverse,
+        index, fn, *q_args, *k_args, positions.data_ptr(), positions.dtype == torch.int64,
+        len(shape) == 3 or rank == 2, inv_freq.data_ptr(), b, s, 2 * inv_freq.shape[0], *extra, interleaved, inverse,
         _DTYPE[query.dtype], scale, _lib.raw_stream(index))
     if status:
-        _lib.check(status, "dsa_rope")
+        _lib.check(status, "dsa_rope" if axes is None else "dsa_rope_axes")
     if inplace:
         _lib.changed(*(t for t in (q_out, k_out) if t is not None))
     return q_out, k_out
 
 
 def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved=False, rotary_offset=0,
-                     key_rotary_offset=None, attention_scale=1.0, layout="BSND", inverse=False, inplace=False):
+                     key_rotary_offset=None, attention_scale=1.0, layout="BSND", inverse=False, inplace=False,
+                     sections=None, sections_interleaved=False):
     """Rotary positions of ``query`` and, if given, ``key``.
 
     query [B, S, N, D] (layout "BSND") or [T, N, D] ("TND"), bfloat16, float16
@@ -178,6 +188,13 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     Rotated columns are multiplied by ``attention_scale``.  ``inverse`` rotates
     by the opposite angles.
 
+    ``sections`` (up to four numbers, R / 2 in all) gives a token a position on
+    each of as many axes, such as time, height and width: ``positions`` then has
+    the axis as one more leading dimension ([A, B, S], [A, S] or [A, T]), and
+    pair i turns by the position on its axis: the first ``sections[0]`` pairs
+    on axis 0, the next on axis 1, and so on, or (``sections_interleaved``) pair
+    i on axis ``i % A`` while that axis has pairs left, else on axis 0.
+
     Returns ``(query_out, key_out)`` (key_out is None without a key), new
     contiguous tensors, or with ``inplace`` the inputs themselves (views of one
     projection too, if their rotated columns share no memory).  Strided
@@ -185,8 +202,13 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     Differentiable in query and key, any number of times, in both modes (not
     in place; ``inv_freq`` gets no gradient).
     """
-    result = _lib.calls().rotate(query, key, positions, inv_freq, interleaved, rotary_offset, key_rotary_offset,
-                                 attention_scale, layout, inverse, inplace)
+    if sections is None:
+        result = _lib.calls().rotate(query, key, positions, inv_freq, interleaved, rotary_offset, key_rotary_offset,
+                                     attention_scale, layout, inverse, inplace)
+    else:
+        result = _lib.calls().rotate_axes(query, key, positions, inv_freq, interleaved, rotary_offset,
+                                          key_rotary_offset, attention_scale, layout, inverse, inplace, sections,
+                                          sections_interleaved)
     if result is not None:
         return result
     rank = _RANK.get(layout)
@@ -205,9 +227,13 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
     if inv_freq.dim() != 1 or inv_freq.shape[0] < 1:
         raise ValueError(f"inv_freq must be a vector, got {tuple(inv_freq.shape)}")
     rot = 2 * inv_freq.shape[0]
-    if positions.shape != lead and positions.shape != lead[-1:]:
-        raise ValueError(f"positions must have shape {tuple(lead)}, or {tuple(lead[-1:])} for all sequences, "
-                         f"got {tuple(positions.shape)}")
+    axes, first = None, ()
+    if sections is not None:
+        axes = _check_sections(sections, rot // 2, sections_interleaved), bool(sections_interleaved)
+        first = (len(axes[0]),)
+    if positions.shape != first + lead and positions.shape != first + lead[-1:]:
+        raise ValueError(f"positions must have shape {tuple(first + lead)}, or {tuple(first + lead[-1:])} for all "
+                         f"sequences, got {tuple(positions.shape)}")
     if key_rotary_offset is None:
         key_rotary_offset = rotary_offset
     if key is not None:
@@ -240,8 +266,22 @@ def rotary_embedding(query, key=None, positions=None, inv_freq=None, interleaved
             float(attention_scale), bool(inverse))
     if grad:
         from .autograd import RotaryEmbeddingFunction
-        return RotaryEmbeddingFunction.apply(query, key, *args)
-    return _rotate(query, key, *args, inplace)
+        return RotaryEmbeddingFunction.apply(query, key, *args, axes)
+    return _rotate(query, key, *args, inplace, axes)
+
+
+def _check_sections(sections, pairs, interleaved):
+    """The sections as a tuple of integers."""
+    out = tuple(int(n) for n in sections)
+    if not 1 <= len(out) <= 4 or any(n < 0 or n != x for n, x in zip(out, sections)):
+        raise ValueError(f"sections must be one to four numbers of pairs, got {tuple(sections)}")
+    if sum(out) != pairs:
+        raise ValueError(f"sections must add up to the {pairs} pairs of inv_freq, got {out}")
+    if interleaved:
+        for a, n in enumerate(out):
+            if a and n and a + (n - 1) * len(out) >= pairs:
+                raise ValueError(f"interleaved sections: axis {a} has no room for {n} of {pairs} pairs")
+    return out
 
 
 class RotaryEmbedding(torch.nn.Module):
@@ -250,7 +290,7 @@ class RotaryEmbedding(torch.nn.Module):
 
     def __init__(self, dim, base=10000.0, scaling="none", factor=1.0, original_max_position=4096, beta_fast=32.0,
                  beta_slow=1.0, mscale=1.0, mscale_all_dim=0.0, interleaved=False, rotary_offset=0,
-                 key_rotary_offset=None, layout="BSND", device=None):
+                 key_rotary_offset=None, layout="BSND", device=None, sections=None, sections_interleaved=False):
         super().__init__()
         inv_freq, self.attention_scale = rotary_frequencies(
             dim, base, scaling, factor, original_max_position, beta_fast, beta_slow, mscale, mscale_all_dim, device)
@@ -259,6 +299,8 @@ class RotaryEmbedding(torch.nn.Module):
         self.rotary_offset = rotary_offset
         self.key_rotary_offset = key_rotary_offset
         self.layout = layout
+        self.sections = sections
+        self.sections_interleaved = sections_interleaved
 
     def _apply(self, fn, recurse=True):
         # a cast of the module (half(), bfloat16()) leaves the frequencies in 64 bits
@@ -271,6 +313,7 @@ class RotaryEmbedding(torch.nn.Module):
     def forward(self, query, key=None, positions=None):
         return rotary_embedding(query, key, positions, self.inv_freq, interleaved=self.interleaved,
                                 rotary_offset=self.rotary_offset, key_rotary_offset=self.key_rotary_offset,
-                                attention_scale=self.attention_scale, layout=self.layout)
+                                attention_scale=self.attention_scale, layout=self.layout, sections=self.sections,
+                                sections_interleaved=self.sections_interleaved)
 
     construct = forward

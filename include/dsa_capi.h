@@ -430,6 +430,23 @@ int dsa_rope(const void* query, void* query_out, int64_t q_in_sb, int64_t q_in_s
              void* stream);
 
 /*
+ * dsa_rope with positions on several axes (time, height, width of images and
+ * video): positions [n_axes, B, S1] (positions_per_sequence) or [n_axes, S1],
+ * n_axes 1 to 4; pair i turns by the position on its axis.  sections (host
+ * array) has the pairs of each axis, rotary_dim / 2 in all: one section after
+ * the other, or (sections_interleaved) pair i on axis i % n_axes where
+ * i < n_axes * sections[i % n_axes], else on axis 0.
+ */
+int dsa_rope_axes(const void* query, void* query_out, int64_t q_in_sb, int64_t q_in_ss, int64_t q_in_sh,
+                  int64_t q_out_sb, int64_t q_out_ss, int64_t q_out_sh, int64_t q_heads, int64_t q_d, int64_t q_start,
+                  const void* key, void* key_out, int64_t k_in_sb, int64_t k_in_ss, int64_t k_in_sh, int64_t k_out_sb,
+                  int64_t k_out_ss, int64_t k_out_sh, int64_t k_heads, int64_t k_d, int64_t k_start,
+                  const void* positions, int32_t positions_64, int32_t positions_per_sequence, const double* inv_freq,
+                  int64_t batch, int64_t s1, int64_t rotary_dim, int64_t n_axes, const int64_t* sections,
+                  int32_t sections_interleaved, int32_t interleaved, int32_t inverse, int32_t dtype,
+                  float attention_scale, void* stream);
+
+/*
  * Pages of a cache.  A cache is [num_pages, page_size, row] with rows of
  * row_bytes[i] bytes next to each other; the n_caches caches of a call (host
  * arrays of device pointers) share block_table, int32 [rows, max_blocks].
@@ -484,6 +501,47 @@ int dsa_paged_cache_compact(int64_t n_caches, void* const* caches, const int64_t
                             int32_t* new_page_refs, int32_t* page_map, int64_t rows, int64_t max_blocks,
                             int64_t num_pages, int64_t page_size, void* workspace, size_t workspace_bytes,
                             void* stream);
+
+/*
+ * Plan: the state of a pool for a step that adds new_lengths[r] tokens to row r
+ * (its own number for each; negative: the row has ended and is released).  Row r
+ * gets pages for its new tokens, lowest free ones (page_refs 0 before the call)
+ * first, to rows in ascending order; a row for which they do not last, and every
+ * later one that needs any, keeps its pages and length and gets no tokens, and so
+ * does a row that would outgrow the table.  Entries of the old table past a row's
+ * last token are released.  new_seq_lengths: with the new tokens (0 for an ended
+ * row).  The new tokens of all rows lie end to end, row_lengths [rows] their
+ * cumulative counts (refused ones too; at most 2^31 - 1); slots and positions
+ * [tokens] get each token's cache row (page * page_size + offset; -1 for a refused
+ * row's and behind the last) and its position in the sequence (0 behind the last).
+ */
+size_t dsa_paged_cache_plan_workspace_size(int64_t rows, int64_t num_pages);
+int dsa_paged_cache_plan(const int32_t* block_table, const int32_t* seq_lengths, const int32_t* page_refs,
+                         const int32_t* new_lengths, int32_t* new_block_table, int32_t* new_seq_lengths,
+                         int32_t* new_page_refs, int32_t* slots, int32_t* positions, int32_t* row_lengths,
+                         int64_t rows, int64_t max_blocks, int64_t num_pages, int64_t page_size, int64_t tokens,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Write to slots: token s of row b (byte strides as in dsa_paged_cache_write;
+ * packed rows: batch 1) goes to the cache row slots[b * s1 + s] of every cache,
+ * or nowhere where that is outside the caches.  No slot may be given twice.
+ */
+int dsa_paged_cache_write_slots(int64_t n_caches, const void* const* rows, void* const* caches,
+                                const int64_t* row_bytes, const int64_t* row_batch_stride,
+                                const int64_t* row_token_stride, const int32_t* slots, int64_t batch, int64_t s1,
+                                int64_t num_pages, int64_t page_size, void* stream);
+
+/*
+ * Prefixes: row b is linked to row b - 1 if the two begin with the same full
+ * pages of their tokens, of min_tokens tokens at least (and one page).
+ * prefix_groups [rows]: the first row of each run of linked rows;
+ * prefix_lengths [rows]: the least number of tokens (whole pages) that two
+ * neighbours of the run share, 0 for a row without links.
+ */
+int dsa_paged_cache_prefixes(const int32_t* block_table, const int32_t* seq_lengths, int32_t* prefix_groups,
+                             int32_t* prefix_lengths, int64_t rows, int64_t max_blocks, int64_t page_size,
+                             int64_t min_tokens, void* stream);
 
 /*
  * Attention of the newest tokens of each sequence over every cached token
