@@ -69,7 +69,9 @@ from .paged_cache import (  # noqa: F401
 
 from .paged_attention import (  # noqa: F401
     PagedAttention,
+    PagedPrefixAttention,
     paged_attention,
+    paged_prefix_attention,
 )
 
 sparse_flash_attention = sparse_flash_attention_triton

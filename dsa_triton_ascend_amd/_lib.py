@@ -221,6 +221,16 @@ SIGNATURES = {
         _i32, _i64, _i64, _i32, _f32, _i32,   # sparse_mode, pre_tokens, next_tokens, dtype, scale_value, return_lse
         _vp, _sz, _vp,                        # workspace, workspace_bytes, stream
     ]),
+    "dsa_paged_prefix_attn_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i64, _i64]),
+    "dsa_paged_prefix_attn": (_c.c_int, [
+        _vp, _vp, _vp, _vp, _vp,              # query, query_rope, key, key_rope, value
+        _vp, _vp, _vp,                        # attention_out, softmax_max, softmax_sum
+        _i32p, _i32p, _i32p, _i32p, _i32p,    # actual_seq_q, actual_seq_kv, block_table, prefix_groups, prefix_lengths
+        _i64, _i64, _i64, _i64, _i64, _i64,   # batch, s1, n1, n2, d, d_rope
+        _i64, _i64, _i64,                     # num_blocks, page_size, max_blocks
+        _i32, _i64, _i64, _i32, _f32, _i32,   # sparse_mode, pre_tokens, next_tokens, dtype, scale_value, return_lse
+        _vp, _sz, _vp,                        # workspace, workspace_bytes, stream
+    ]),
 }
 
 _lib = None
@@ -247,7 +257,8 @@ def load():
 _ENTRIES = ("dsa_rope", "dsa_paged_cache_write", "dsa_paged_cache_fork_workspace_size", "dsa_paged_cache_fork",
             "dsa_paged_cache_compact_workspace_size", "dsa_paged_cache_compact", "dsa_paged_attn_workspace_size",
             "dsa_paged_attn", "dsa_last_error", "dsa_rope_axes", "dsa_paged_cache_plan_workspace_size",
-            "dsa_paged_cache_plan", "dsa_paged_cache_write_slots", "dsa_paged_cache_prefixes")  # in the order in which _torch_calls takes them
+            "dsa_paged_cache_plan", "dsa_paged_cache_write_slots", "dsa_paged_cache_prefixes",
+            "dsa_paged_prefix_attn_workspace_size", "dsa_paged_prefix_attn")  # in the order in which _torch_calls takes them
 _calls = None
 
 
@@ -258,7 +269,7 @@ class _NoCalls:
     def write(*args):
         return None
 
-    fork = compact = attention = rotate = rotate_axes = plan = write_slots = prefixes = write
+    fork = compact = attention = rotate = rotate_axes = plan = write_slots = prefixes = prefix_attention = write
 
 
 def calls():

@@ -35,6 +35,9 @@ SOURCES = [
     "paged_cache.hip",
     "paged_attn.hip",
     "paged_attn_latent.hip",
+    "capi_serving.cpp",
+    "paged_prefix.hip",
+    "paged_prefix_latent.hip",
 ]
 
 ARCH = os.environ.get("DSA_OFFLOAD_ARCH", "gfx950")
@@ -72,6 +75,8 @@ PER_SOURCE_FLAGS = {
     "li_fwd.hip": VGPR_FORM,
     "paged_attn.hip": VGPR_FORM,
     "paged_attn_latent.hip": VGPR_FORM,
+    "paged_prefix.hip": VGPR_FORM,
+    "paged_prefix_latent.hip": VGPR_FORM,
 }
 
 

@@ -26,6 +26,8 @@
 
 #include "sfa_common.h"
 
+#include <type_traits>
+
 namespace dsa {
 
 constexpr float kPaBelow = 8.f;   // ref is set this far below the largest score
@@ -52,6 +54,29 @@ struct PagedAttnParams {
   float scale_log2;
 };
 
+// With a prefix that sequences share (paged_prefix.h): these kernels take what
+// is behind it, and the join takes its parts too.
+struct PagedPrefixParams : PagedAttnParams {
+  const int32_t *ids, *shared;  // per sequence: its family and the tokens that it shares
+  i32x4* where;                 // per sequence: first job of its family, blocks of rows, parts, place in the family
+  // rows of part_o / part_ml: behind those of the runs come, for each sequence,
+  // one for what a run has of it if that is all of it, then those of the jobs
+  int64_t whole0, part0;
+  int prefix_workers;           // jobs of one key head aimed at
+  int job_rows;                 // rows of a block
+};
+
+template <typename P> constexpr bool kPrefixed = std::is_same<P, PagedPrefixParams>::value;
+
+// Tokens that sequence b shares with the one before or behind it.
+__device__ __forceinline__ int paged_shared(const PagedPrefixParams& p, int b) {
+  const int before = max(b - 1, 0), behind = min(b + 1, p.batch - 1);
+  const int id = p.ids[b], n = p.shared[b];
+  const int id0 = p.ids[before], n0 = p.shared[before], id1 = p.ids[behind], n1 = p.shared[behind];
+  const bool links = (b > 0 && id0 == id && n0 == n) || (b + 1 < p.batch && id1 == id && n1 == n);
+  return id >= 0 && n > 0 && links ? min(n, p.max_blocks * p.page) : 0;
+}
+
 // page and offset of a token.  t * magic / 2^32 is at most t / 2^32 below
 // t / page, so its integer part is off by one at most.
 __device__ __forceinline__ unsigned paged_split(const PagedAttnParams& p, unsigned t, unsigned* off) {
@@ -66,8 +91,15 @@ __device__ __forceinline__ unsigned paged_split(const PagedAttnParams& p, unsign
 }
 
 struct PagedSeq {
-  int act_q, act_k, lo, hi;  // lo <= t < hi: tokens that any row sees
+  int act_q, act_k, lo, hi;  // lo <= t < hi: tokens that any row sees (with a prefix: behind it)
 };
+struct PagedSeqBehind : PagedSeq {
+  int shared;  // tokens of the prefix
+};
+template <typename P> using PagedSeqOf = std::conditional_t<kPrefixed<P>, PagedSeqBehind, PagedSeq>;
+// whether a sequence has a prefix before it
+__device__ __forceinline__ bool paged_behind(const PagedSeq&) { return false; }
+__device__ __forceinline__ bool paged_behind(const PagedSeqBehind& s) { return s.shared != 0; }
 
 // A row's output times the factor f, which is 0 where the row saw no token of
 // the run: then the output is 0 too, also where another row's value beside it
@@ -87,20 +119,26 @@ __device__ __forceinline__ void paged_bounds(const PagedAttnParams& p, int act_q
   *lo = (int)min(max(l, (int64_t)0), (int64_t)0x7fffffff);
 }
 
-__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
-  PagedSeq s;
+template <typename P>
+__device__ __forceinline__ PagedSeqOf<P> paged_seq(const P& p, int b) {
+  PagedSeqOf<P> s;
   s.act_k = min(max(p.act_k[b], 0), p.max_blocks * p.page);
   s.act_q = p.act_q ? min(max(p.act_q[b], 0), p.s1) : p.s1;
   int l, h;
   paged_bounds(p, s.act_q, s.act_k, 0, &s.lo, &h);
   paged_bounds(p, s.act_q, s.act_k, max(s.act_q - 1, 0), &l, &s.hi);
+  if constexpr (kPrefixed<P>) {
+    s.shared = paged_shared(p, b);
+    s.lo = max(s.lo, s.shared);
+  }
   if (s.hi < s.lo) s.hi = s.lo;
   return s;
 }
 
 // sequence b, the same on all lanes (nothing past the last)
-__device__ __forceinline__ PagedSeq paged_seq_uniform(const PagedAttnParams& p, int b) {
-  PagedSeq s = paged_seq(p, min(b, p.batch - 1));
+template <typename P>
+__device__ __forceinline__ PagedSeqOf<P> paged_seq_uniform(const P& p, int b) {
+  PagedSeqOf<P> s = paged_seq(p, min(b, p.batch - 1));
   s.lo = __builtin_amdgcn_readfirstlane(s.lo);
   s.hi = b < p.batch ? __builtin_amdgcn_readfirstlane(s.hi) : s.lo;
   return s;
@@ -127,17 +165,18 @@ constexpr int kPaSlack = 2;
 // 19.2 with 4, 23.4 with 8; of 8192: 27.5, 22.1, 21.4, 26.5; grouped heads alike).
 constexpr int kPaMinTiles = 2;
 
+template <typename P>
 struct PagedPlan {
   int total, per;   // tiles, tiles of a worker
   int grain;
-  PagedSeq seq;     // of this lane
+  PagedSeqOf<P> seq;  // of this lane
   int tiles, incl;  // its tiles, and those of the lanes up to it
 
   __device__ __forceinline__ int padded(int n) const {
     return grain == 1 ? n : (int)((unsigned)(n + grain - 1) / (unsigned)grain) * grain;
   }
 
-  __device__ __forceinline__ void make(const PagedAttnParams& p, int tile, int lane) {
+  __device__ __forceinline__ void make(const P& p, int tile, int lane) {
     tiles = 0;
     if (lane < p.batch) {
       seq = paged_seq(p, lane);
@@ -171,7 +210,7 @@ struct PagedPlan {
   }
 
   // sequence that holds tile `at` (< total), and the tiles before it
-  __device__ __forceinline__ int find(const PagedAttnParams& p, int tile, int lane, int at, int* before) const {
+  __device__ __forceinline__ int find(const P& p, int tile, int lane, int at, int* before) const {
     int base = 0, n = tiles, in = incl;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
       const int b = b0 + 64 + lane;
@@ -191,13 +230,14 @@ struct PagedPlan {
   }
 
   // sequence b (the same on all lanes)
-  __device__ __forceinline__ PagedSeq sequence(const PagedAttnParams& p, int b) const {
-    PagedSeq s;
+  __device__ __forceinline__ PagedSeqOf<P> sequence(const P& p, int b) const {
+    PagedSeqOf<P> s;
     if (b < 64) {
       s.act_q = __builtin_amdgcn_readlane(seq.act_q, b);
       s.act_k = __builtin_amdgcn_readlane(seq.act_k, b);
       s.lo = __builtin_amdgcn_readlane(seq.lo, b);
       s.hi = __builtin_amdgcn_readlane(seq.hi, b);
+      if constexpr (kPrefixed<P>) s.shared = __builtin_amdgcn_readlane(seq.shared, b);
     } else {
       s = paged_seq(p, b);
       s.lo = __builtin_amdgcn_readfirstlane(s.lo);
@@ -209,7 +249,7 @@ struct PagedPlan {
   __device__ __forceinline__ int worker_of(int at) const { return (int)((unsigned)at / (unsigned)per); }
 
   // tiles before sequence b
-  __device__ __forceinline__ int start(const PagedAttnParams& p, int tile, int lane, int b) const {
+  __device__ __forceinline__ int start(const P& p, int tile, int lane, int b) const {
     if (b < 64) return b ? __builtin_amdgcn_readlane(incl, b - 1) : 0;
     int n = 0;
 #pragma unroll 4
@@ -218,6 +258,14 @@ struct PagedPlan {
   }
 };
 
+// Row of part_o where a run that has all tokens of sequence b leaves its output
+// for lane group g, if there is a prefix before them (a run may have several
+// such sequences, where it has two parts of sequences at most).
+__device__ __forceinline__ int64_t paged_whole_slot(const PagedAttnParams&, int, int) { return 0; }
+__device__ __forceinline__ int64_t paged_whole_slot(const PagedPrefixParams& p, int b, int g) {
+  return p.whole0 + ((int64_t)b * p.groups + g) * p.group_rows;
+}
+
 // workspace and launches of the two kernels (paged_attn.hip, paged_attn_latent.hip)
 struct PagedShape {
   int workers, min_tiles, groups, row_groups, group_rows, tile;
@@ -225,8 +273,20 @@ struct PagedShape {
 size_t paged_part_bytes(const PagedShape& s, int64_t d);
 int paged_workers(int64_t slots, int64_t groups, int64_t batch, int64_t tiles, int min_tiles);
 int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream);
+bool paged_combine_launchable(int64_t workers, int64_t batch, int64_t s1, int64_t n1);
+int paged_combine_launch(const PagedPrefixParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream);
+// of either kind of work: its shape, its parameters, and the launch of all but the join
+PagedShape paged_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent, int64_t max_blocks,
+                       int64_t page);
+void paged_fill(PagedAttnParams& p, const PagedShape& s, const void* query, const void* query_rope, const void* key,
+                const void* key_rope, const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
+                const int32_t* act_k, const int32_t* table, int64_t batch, int64_t s1, int64_t n1, int64_t n2,
+                int64_t num_blocks, int64_t page, int64_t max_blocks, int32_t mode, int64_t pre_tokens,
+                int64_t next_tokens, float scale, int32_t return_lse);
+int paged_grouped_launch(const PagedPrefixParams& p, int64_t d, int32_t dtype, hipStream_t stream);
 PagedShape paged_latent_shape(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t max_blocks, int64_t page);
 bool paged_latent_launchable(int64_t workers, int64_t row_groups);
 int paged_latent_launch(const PagedAttnParams& p, int64_t d, int32_t dtype, hipStream_t stream);
+int paged_latent_launch(const PagedPrefixParams& p, int64_t d, int32_t dtype, hipStream_t stream);
 
 }  // namespace dsa

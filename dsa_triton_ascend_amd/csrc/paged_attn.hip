@@ -42,8 +42,8 @@ constexpr int pa_waves(int d, int mt) { return d <= 128 && mt <= 2 ? 2 : 1; }
 
 // STREAM: loads that keep nothing in the caches, for more K and V than the
 // caches hold from one call to the next.
-template <typename T, int D, int MT, bool STREAM>
-__global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel(PagedAttnParams p) {
+template <typename T, int D, int MT, bool STREAM, typename P>
+__global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel(P p) {
   using E = Elem<T>;
   using V8 = typename E::v8;
   constexpr int KS = D / 32;   // k-steps of the scores
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
   if (worker >= p.workers) return;
   const int kvh = ng / p.row_groups, rg = ng - kvh * p.row_groups;
 
-  PagedPlan plan;
+  PagedPlan<P> plan;
   plan.make(p, kPaTile, lane);
   if (worker >= (plan.total + plan.per - 1) / plan.per) return;
   int at = worker * plan.per;
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
 
   bool first_segment = true;
   b = __builtin_amdgcn_readfirstlane(b);
-  PagedSeq seq = plan.sequence(p, b);  // (later ones are read again: the plan's do not stay in registers)
+  PagedSeqOf<P> seq = plan.sequence(p, b);  // (later ones are read again: the plan's do not stay in registers)
   while (at < end) {
     const int nt = paged_tiles(seq, kPaTile);
     if (nt == 0) {
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
 
     // MFMA j, register r of lane group g: column 8 (4 g + r) + j % 8 of piece
     // j / 8 (4 (4 g + r) + j at D = 64), so a lane holds whole chunks
-    const bool whole = t0 == 0 && t1 == nt;
+    const bool all = t0 == 0 && t1 == nt, whole = all && !paged_behind(seq);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const float l = xgroup_sum(sum[mt]);
@@ -255,8 +255,8 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
           }
         }
       } else {
-        const int64_t slot = (((int64_t)worker * 2 + (first_segment ? 0 : 1)) * p.groups + ng) * p.group_rows +
-                             mt * 16 + li;
+        int64_t slot = (((int64_t)worker * 2 + (first_segment ? 0 : 1)) * p.groups + ng) * p.group_rows + mt * 16 + li;
+        if constexpr (kPrefixed<P>) slot = all ? paged_whole_slot(p, b, ng) + mt * 16 + li : slot;
         float* dst = p.part_o + slot * D;
         const float seen = l != 0.f ? 1.f : 0.f;
 #pragma unroll
@@ -290,8 +290,8 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
 // ---------------------------------------------------------------------------
 constexpr int kPcFewRuns = 64;
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, int tile, int wg_rows) {
+template <typename T, int D, typename P>
+__global__ __launch_bounds__(256) void paged_combine_kernel(P p, int tile, int wg_rows) {
   using E = Elem<T>;
   constexpr int EPL = D / 64;
   typedef T TV __attribute__((ext_vector_type(EPL)));
@@ -302,13 +302,19 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, i
   const int per_seq = p.n2 * p.rows, groups = (per_seq + wg_rows - 1) / wg_rows;
   const int b = blockIdx.x / groups, row0 = (blockIdx.x - b * groups) * wg_rows;
 
-  PagedPlan plan;
+  PagedPlan<P> plan;
   plan.make(p, tile, lane);
-  const int nt = paged_tiles(plan.sequence(p, b), tile);
+  const PagedSeqOf<P> seq = plan.sequence(p, b);
+  const int nt = paged_tiles(seq, tile);
   const int first = plan.start(p, tile, lane, b), last = first + nt - 1;
   const int w0 = nt ? plan.worker_of(first) : 0;
-  const int runs = nt ? plan.worker_of(last) - w0 + 1 : 0;
-  if (runs == 1) return;  // written whole by its worker
+  const int own = nt ? plan.worker_of(last) - w0 + 1 : 0;
+  int runs = own;
+  i32x4 where = {0, 0, 0, 0};
+  if constexpr (kPrefixed<P>) {  // behind the runs: the parts of the prefix
+    if (seq.shared) where = p.where[b], runs += where[2];
+  }
+  if (runs == 1 && !paged_behind(seq)) return;  // written whole by its worker
   const int slot0 = first != w0 * plan.per ? 1 : 0;  // of the first worker; the others' is 0
 
   // the runs i0 .. i1 of a row, summed relative to the largest reference of all
@@ -317,7 +323,20 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, i
     const int rg = rr / p.group_rows;
     const int64_t in_group = (int64_t)(kvh * p.row_groups + rg) * p.group_rows + (rr - rg * p.group_rows);
     const int64_t span = (int64_t)p.groups * p.group_rows;
-    auto slot = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i == 0 ? slot0 : 0)) * span + in_group; };
+    int block = 0, in_block = 0;
+    if constexpr (kPrefixed<P>) {
+      const int64_t r = (int64_t)where[3] * p.rows + rr;  // among the family's
+      block = where[0] + (int)(r / p.job_rows), in_block = (int)(r % p.job_rows);
+    }
+    auto slot = [&](int i) {
+      const int64_t s = ((int64_t)(w0 + i) * 2 + (i == 0 ? slot0 : 0)) * span + in_group;
+      if constexpr (kPrefixed<P>) {
+        const int64_t job = block + (int64_t)(i - own) * where[1];
+        if (own == 1 && i == 0) return paged_whole_slot(p, b, kvh * p.row_groups + rg) + (rr - rg * p.group_rows);
+        return i < own ? s : p.part0 + (job * p.n2 + kvh) * p.job_rows + in_block;
+      }
+      return s;
+    };
     float m = -INFINITY, t = -INFINITY;
     for (int i = lane; i < runs; i += 64) {
       const f32x4 ml = p.part_ml[slot(i)];
@@ -401,8 +420,8 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnParams p, i
   }
 }
 
-template <typename T>
-static void paged_combine_d(const PagedAttnParams& p, int tile, int wg_rows, int64_t d, unsigned grid, hipStream_t stream) {
+template <typename T, typename P>
+static void paged_combine_d(const P& p, int tile, int wg_rows, int64_t d, unsigned grid, hipStream_t stream) {
   if (d == 64) paged_combine_kernel<T, 64><<<grid, 256, 0, stream>>>(p, tile, wg_rows);  // grouped form only
   else if (d == 128) paged_combine_kernel<T, 128><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
   else if (d == 256) paged_combine_kernel<T, 256><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
@@ -417,13 +436,25 @@ static int64_t paged_combine_grid(int64_t workers, int64_t batch, int64_t s1, in
   return batch * ((s1 * n1 + wg_rows - 1) / wg_rows);
 }
 
-int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream) {
+bool paged_combine_launchable(int64_t workers, int64_t batch, int64_t s1, int64_t n1) {
+  return launchable(paged_combine_grid(workers, batch, s1, n1), 256);
+}
+
+template <typename P>
+static int paged_combine(const P& p, int tile, int64_t d, int32_t dtype, hipStream_t stream) {
   const int wg_rows = paged_combine_rows(p.workers, p.batch);
   const unsigned grid = (unsigned)paged_combine_grid(p.workers, p.batch, p.s1, p.n1);
   if (dtype == DSA_DTYPE_BF16) paged_combine_d<bf16>(p, tile, wg_rows, d, grid, stream);
   else paged_combine_d<f16>(p, tile, wg_rows, d, grid, stream);
   DSA_HIP(hipGetLastError());
   return DSA_OK;
+}
+
+int paged_combine_launch(const PagedAttnParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream) {
+  return paged_combine(p, tile, d, dtype, stream);
+}
+int paged_combine_launch(const PagedPrefixParams& p, int tile, int64_t d, int32_t dtype, hipStream_t stream) {
+  return paged_combine(p, tile, d, dtype, stream);
 }
 
 size_t paged_part_bytes(const PagedShape& s, int64_t d) {
@@ -466,8 +497,8 @@ static PagedShape paged_grouped_shape(int64_t batch, int64_t s1, int64_t n1, int
   return s;
 }
 
-static PagedShape paged_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
-                              int64_t max_blocks, int64_t page) {
+PagedShape paged_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent, int64_t max_blocks,
+                       int64_t page) {
   return latent ? paged_latent_shape(batch, s1, n1, d, max_blocks, page)
                 : paged_grouped_shape(batch, s1, n1, n2, d, max_blocks, page);
 }
@@ -481,7 +512,7 @@ bool paged_attn_launchable(int64_t batch, int64_t s1, int64_t n1, int64_t n2, in
   const PagedShape s = paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
   return (latent ? paged_latent_launchable(s.workers, s.row_groups)
                  : launchable(paged_grouped_grid(s.workers, s.groups), kPaThreads)) &&
-         launchable(paged_combine_grid(s.workers, batch, s1, n1), 256);
+         paged_combine_launchable(s.workers, batch, s1, n1);
 }
 
 size_t paged_attn_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
@@ -489,35 +520,49 @@ size_t paged_attn_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t
   return paged_part_bytes(paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page), d);
 }
 
-template <typename T, int D, int MT>
-static void paged_launch_one(const PagedAttnParams& p, bool streaming, unsigned grid, hipStream_t stream) {
+template <typename T, int D, int MT, typename P>
+static void paged_launch_one(const P& p, bool streaming, unsigned grid, hipStream_t stream) {
   if (streaming) paged_attn_kernel<T, D, MT, true><<<grid, kPaThreads, 0, stream>>>(p);
   else paged_attn_kernel<T, D, MT, false><<<grid, kPaThreads, 0, stream>>>(p);
 }
 
-template <typename T, int D>
-static void paged_launch_mt(const PagedAttnParams& p, bool streaming, unsigned grid, hipStream_t stream) {
+template <typename T, int D, typename P>
+static void paged_launch_mt(const P& p, bool streaming, unsigned grid, hipStream_t stream) {
   if (p.group_rows == 16) paged_launch_one<T, D, 1>(p, streaming, grid, stream);
   else if (p.group_rows == 32) paged_launch_one<T, D, 2>(p, streaming, grid, stream);
   else if constexpr (D <= 128) paged_launch_one<T, D, 4>(p, streaming, grid, stream);
 }
 
-template <typename T>
-static void paged_launch(const PagedAttnParams& p, int64_t d, bool streaming, unsigned grid, hipStream_t stream) {
+template <typename T, typename P>
+static void paged_launch(const P& p, int64_t d, bool streaming, unsigned grid, hipStream_t stream) {
   if (d == 64) paged_launch_mt<T, 64>(p, streaming, grid, stream);
   else if (d == 128) paged_launch_mt<T, 128>(p, streaming, grid, stream);
   else paged_launch_mt<T, 256>(p, streaming, grid, stream);
 }
 
-int paged_attn_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
-                   const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
-                   const int32_t* act_k, const int32_t* table, int64_t batch, int64_t s1, int64_t n1, int64_t n2,
-                   int64_t d, int64_t num_blocks, int64_t page, int64_t max_blocks, int32_t mode, int64_t pre_tokens,
-                   int64_t next_tokens, int32_t dtype, float scale, int32_t return_lse, void* workspace,
-                   hipStream_t stream) {
-  const bool latent = value == nullptr;
-  const PagedShape s = paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
-  PagedAttnParams p = {};
+template <typename P>
+static int paged_grouped(const P& p, int64_t d, int32_t dtype, hipStream_t stream) {
+  const unsigned grid = (unsigned)paged_grouped_grid(p.workers, p.groups);
+  // K and V that the caches could hold until the next call are kept there
+  // (134 MB: 38 us, streaming 41; 537 MB: 115 us, streaming 104)
+  const int64_t all = (int64_t)p.batch * p.max_blocks * p.page;
+  const int64_t tokens = p.kv_rows < all ? p.kv_rows : all;
+  const bool streaming = tokens * p.n2 * d * 4 > (256ll << 20);
+  if (dtype == DSA_DTYPE_BF16) paged_launch<bf16>(p, d, streaming, grid, stream);
+  else paged_launch<f16>(p, d, streaming, grid, stream);
+  DSA_HIP(hipGetLastError());
+  return DSA_OK;
+}
+
+int paged_grouped_launch(const PagedPrefixParams& p, int64_t d, int32_t dtype, hipStream_t stream) {
+  return paged_grouped(p, d, dtype, stream);
+}
+
+void paged_fill(PagedAttnParams& p, const PagedShape& s, const void* query, const void* query_rope, const void* key,
+                const void* key_rope, const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
+                const int32_t* act_k, const int32_t* table, int64_t batch, int64_t s1, int64_t n1, int64_t n2,
+                int64_t num_blocks, int64_t page, int64_t max_blocks, int32_t mode, int64_t pre_tokens,
+                int64_t next_tokens, float scale, int32_t return_lse) {
   p.q = query;
   p.qr = query_rope;
   p.k = key;
@@ -529,9 +574,6 @@ int paged_attn_run(const void* query, const void* query_rope, const void* key, c
   p.act_q = act_q;
   p.act_k = act_k;
   p.table = table;
-  const int64_t part_rows = (int64_t)s.workers * 2 * s.groups * s.group_rows;
-  p.part_ml = (f32x4*)workspace;
-  p.part_o = (float*)(p.part_ml + part_rows);
   p.kv_rows = num_blocks * page;
   p.band_pre = band_clamp(pre_tokens);
   p.band_next = band_clamp(next_tokens);
@@ -552,19 +594,24 @@ int paged_attn_run(const void* query, const void* query_rope, const void* key, c
   p.group_rows = s.group_rows;
   p.page_magic = 0xffffffffu / (unsigned)page;
   p.scale_log2 = scale * kLog2e;
-  if (latent) {
-    const int st = paged_latent_launch(p, d, dtype, stream);
-    if (st != DSA_OK) return st;
-  } else {
-    const unsigned grid = (unsigned)paged_grouped_grid(s.workers, s.groups);
-    // K and V that the caches could hold until the next call are kept there
-    // (134 MB: 38 us, streaming 41; 537 MB: 115 us, streaming 104)
-    const int64_t tokens = p.kv_rows < batch * max_blocks * page ? p.kv_rows : batch * max_blocks * page;
-    const bool streaming = tokens * n2 * d * 4 > (256ll << 20);
-    if (dtype == DSA_DTYPE_BF16) paged_launch<bf16>(p, d, streaming, grid, stream);
-    else paged_launch<f16>(p, d, streaming, grid, stream);
-    DSA_HIP(hipGetLastError());
-  }
+}
+
+int paged_attn_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
+                   const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
+                   const int32_t* act_k, const int32_t* table, int64_t batch, int64_t s1, int64_t n1, int64_t n2,
+                   int64_t d, int64_t num_blocks, int64_t page, int64_t max_blocks, int32_t mode, int64_t pre_tokens,
+                   int64_t next_tokens, int32_t dtype, float scale, int32_t return_lse, void* workspace,
+                   hipStream_t stream) {
+  const bool latent = value == nullptr;
+  const PagedShape s = paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
+  PagedAttnParams p = {};
+  paged_fill(p, s, query, query_rope, key, key_rope, value, out, smax, ssum, act_q, act_k, table, batch, s1, n1, n2,
+             num_blocks, page, max_blocks, mode, pre_tokens, next_tokens, scale, return_lse);
+  const int64_t part_rows = (int64_t)s.workers * 2 * s.groups * s.group_rows;
+  p.part_ml = (f32x4*)workspace;
+  p.part_o = (float*)(p.part_ml + part_rows);
+  const int st = latent ? paged_latent_launch(p, d, dtype, stream) : paged_grouped(p, d, dtype, stream);
+  if (st != DSA_OK) return st;
   return paged_combine_launch(p, s.tile, d, dtype, stream);
 }
 

@@ -48,8 +48,6 @@
 #include "paged_attn.h"
 #include "sfa_fwd.h"
 
-#include <type_traits>
-
 namespace dsa {
 
 __device__ __attribute__((aligned(16))) unsigned char g_latent_zero_row[1024];
@@ -75,8 +73,8 @@ __device__ __forceinline__ void pl_dma_glb(unsigned lds_base, const void* gaddr)
 constexpr int kPlThreads = 512;
 constexpr int kPlPages = 512;  // block-table entries held in LDS
 
-template <int D, typename T, int HG, bool STREAM>
-__global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnParams p) {
+template <int D, typename T, int HG, bool STREAM, typename P>
+__global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(P p) {
   using E = Elem<T>;
   using V8 = typename E::v8;
   typedef T T4 __attribute__((ext_vector_type(4)));
@@ -130,7 +128,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   const int rg = jj % p.row_groups;
   const int worker = (jj / p.row_groups) * 8 + (blockIdx.x & 7);
   if (worker >= p.workers) return;
-  PagedPlan plan;
+  PagedPlan<P> plan;
   plan.make(p, TILE, lane);
   if (worker >= (plan.total + plan.per - 1) / plan.per) return;
   int at = worker * plan.per;
@@ -172,7 +170,7 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
   // (what the plan keeps of the sequences does not stay in the registers
   // through the tiles: later ones are read again)
   b = __builtin_amdgcn_readfirstlane(b);
-  PagedSeq seq = plan.sequence(p, b);
+  PagedSeqOf<P> seq = plan.sequence(p, b);
   while (at < end) {
     const int ln = fresh_lane(), li = ln & 15, lg = ln >> 4, tid = wave * 64 + ln;
     const int nt = paged_tiles(seq, TILE);
@@ -512,9 +510,10 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(PagedAttnPa
     // (a scope of its own: the lane's numbers are made anew here)
     [&](int ln) __attribute__((always_inline)) {
     const int li = ln & 15, lg = ln >> 4;
-    const bool whole = t0 == 0 && t1 == nt;
-    const int64_t slot0 =
+    const bool all = t0 == 0 && t1 == nt, whole = all && !paged_behind(seq);
+    int64_t slot0 =
         (((int64_t)worker * 2 + (first_segment ? 0 : 1)) * p.groups + rg) * p.group_rows;
+    if constexpr (kPrefixed<P>) slot0 = all ? paged_whole_slot(p, b, rg) : slot0;
     {
       const float l = xgroup_sum(sum), n = xgroup_sum(kLo ? sum : sum_p);
       const int r = wave * 16 + li, rr = rg * HG + r;
@@ -616,16 +615,16 @@ PagedShape paged_latent_shape(int64_t batch, int64_t s1, int64_t n1, int64_t d, 
   return s;
 }
 
-template <int D, typename T, bool STREAM>
-static void paged_latent_hg(const PagedAttnParams& p, unsigned grid, hipStream_t stream) {
+template <int D, typename T, bool STREAM, typename P>
+static void paged_latent_hg(const P& p, unsigned grid, hipStream_t stream) {
   if (p.group_rows == 16) paged_latent_kernel<D, T, 16, STREAM><<<grid, kPlThreads, 0, stream>>>(p);
   else if (p.group_rows == 32) paged_latent_kernel<D, T, 32, STREAM><<<grid, kPlThreads, 0, stream>>>(p);
   else if (p.group_rows == 64) paged_latent_kernel<D, T, 64, STREAM><<<grid, kPlThreads, 0, stream>>>(p);
   else paged_latent_kernel<D, T, 128, STREAM><<<grid, kPlThreads, 0, stream>>>(p);
 }
 
-template <typename T>
-static void paged_latent_d(const PagedAttnParams& p, int64_t d, unsigned grid, hipStream_t stream) {
+template <typename T, typename P>
+static void paged_latent_d(const P& p, int64_t d, unsigned grid, hipStream_t stream) {
   // rows that the caches cannot hold until the next call, read by one row
   // group only, are not kept there (512 columns; 1.2 GB at 16 heads: 222 us,
   // streaming 192; 300 MB at 32 rows: 85 and 79; 75 MB at 16: 28 and 29)
@@ -643,12 +642,20 @@ bool paged_latent_launchable(int64_t workers, int64_t row_groups) {
   return launchable(paged_latent_grid(workers, row_groups), kPlThreads);
 }
 
-int paged_latent_launch(const PagedAttnParams& p, int64_t d, int32_t dtype, hipStream_t stream) {
+template <typename P>
+static int paged_latent(const P& p, int64_t d, int32_t dtype, hipStream_t stream) {
   const unsigned grid = (unsigned)paged_latent_grid(p.workers, p.row_groups);
   if (dtype == DSA_DTYPE_BF16) paged_latent_d<bf16>(p, d, grid, stream);
   else paged_latent_d<f16>(p, d, grid, stream);
   DSA_HIP(hipGetLastError());
   return DSA_OK;
+}
+
+int paged_latent_launch(const PagedAttnParams& p, int64_t d, int32_t dtype, hipStream_t stream) {
+  return paged_latent(p, d, dtype, stream);
+}
+int paged_latent_launch(const PagedPrefixParams& p, int64_t d, int32_t dtype, hipStream_t stream) {
+  return paged_latent(p, d, dtype, stream);
 }
 
 }  // namespace dsa

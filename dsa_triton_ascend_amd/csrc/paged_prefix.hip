@@ -1,0 +1,508 @@
+// Attention over a prefix that sequences share, grouped heads (described in
+// paged_prefix.h), and the launches of the whole operator.
+//
+//   S^T = K Q^T,  P = 2^(S - ref),  O^T = V^T P^T
+//
+// A family of 32 sequences with eight query heads per key head has 256 rows a
+// key head, and a token of the prefix serves them all: 4 * 256 flops per byte of
+// K and V, so the matrix instructions bound it, and beside them the vector
+// unit, which has a softmax weight to make for every 4 D flops.
+//
+// A workgroup has up to 16 NW MR rows: wave w the 16 MR from 16 MR w on, in MR
+// tiles of 16.  K and V come in tiles of 32 tokens by LDS-DMA into a ring,
+// chunks of 16 bytes swizzled so that both products read them without bank
+// conflicts; every wave reads the whole tile, so the rows of a wave set what the
+// LDS has to give (16 KB per 2048 MFMA cycles of a CU at 64 rows of 128 columns).
+// S^T leaves a token's weight where the second product wants it: token 16 tt +
+// 4 g + r is k slot 8 g + 4 tt + r of lane group g, and V^T is read transposed
+// in that order, so P stays in its lanes.
+//
+// A step computes the scores of tile t + 1 with the second half of the softmax
+// of tile t between its MFMAs, then the output of tile t with the first half of
+// that of tile t + 1.  One barrier a step.
+//
+// P is rounded once to the input type, and the output is divided by the sum of
+// the rounded weights, which one more row of ones beside V gives; the sum that
+// is returned is that of the weights in 32 bits.
+#include "paged_prefix.h"
+#include "sfa_fwd.h"
+
+namespace dsa {
+
+__device__ __attribute__((aligned(16))) unsigned char g_prefix_zero_row[1024];
+
+constexpr int kPrefixPages = 1024;  // block-table entries held in LDS
+
+template <int D> constexpr int kPrefixRing = D == 256 ? 4 : (D == 128 ? 6 : 8);
+
+template <typename T, int D, int NW, int MR>
+__global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixParams p) {
+  using E = Elem<T>;
+  using V8 = typename E::v8;
+  constexpr int R = NW * 16 * MR, NT = NW * 64, TILE = kPrefixTile;
+  constexpr int KS = D / 32;                // k-steps of the scores
+  constexpr int ND = D / 16;                // output tiles
+  constexpr int ROW = D * 2;
+  constexpr int CPT = D / 8;                // 16-byte chunks of a token
+  constexpr int TPI = 64 / CPT;             // tokens of one DMA
+  constexpr int NL = TILE / TPI < NW ? TILE / TPI : NW;  // waves that fetch
+  constexpr int NI = TILE / TPI / NL;       // their DMAs per tile of K, and of V
+  constexpr int TILE_BYTES = TILE * ROW, STAGE = 2 * TILE_BYTES, NB = kPrefixRing<D>;
+  constexpr int kSteps = 64 / NI;           // tiles whose rows a register holds
+  constexpr int HR = MR / 2;                // row tiles of the first half of a softmax
+  static_assert(NI * NL * TPI == TILE && MR % 2 == 0, "tile split");
+  __shared__ __attribute__((aligned(16))) unsigned char smem[NB * STAGE];
+  __shared__ int s_tab[kPrefixPages];
+  __shared__ int s_span[2];
+
+  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto swz_k = [](int t) { return D == 64 ? rope_swz(t) : nope_swz(t); };
+  auto swz_v = [](int t) { return D == 64 ? ((t >> 1) & 3) << 1 : nope_swz(t); };
+
+  const int64_t row_bytes = (int64_t)p.n2 * ROW;
+  const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  const unsigned flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
+  const unsigned smem_base = (unsigned)(uintptr_t)smem;
+  // a DMA lies in one page, at an offset that 32 bits hold
+  const bool one_page = p.page % TPI == 0 && row_bytes * TPI < (1ll << 31);
+  // where a lane reads and the wave's DMAs take from
+  const int k_at = li * ROW + ((lg ^ swz_k(li)) * 16);
+  const int v_tok = lg * 4 + (li >> 2);
+  const int v_at = v_tok * ROW + ((((li & 3) >> 1) ^ swz_v(v_tok)) * 16) + (li & 1) * 8;
+  int k_from[NI], v_from[NI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int tk = (j * NL + wave) * TPI + lane / CPT;
+    k_from[j] = (int)((lane / CPT) * row_bytes) + ((lane % CPT) ^ swz_k(tk)) * 16;
+    v_from[j] = (int)((lane / CPT) * row_bytes) + ((lane % CPT) ^ swz_v(tk)) * 16;
+  }
+  V8 ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = E::from_f32(1.f);
+
+  PrefixPlan<R> plan;
+  int head;
+  int job = prefix_job_of(blockIdx.x, gridDim.x, 0, p.n2, &head);
+  typename PrefixPlan<R>::Job jb = plan.make(p, lane, job);
+  for (int round = 0; job < plan.jobs;) {
+    const int part = (job - jb.job0) / jb.blocks, block = (job - jb.job0) - part * jb.blocks;
+    const int all_tiles = (jb.f.tokens + TILE - 1) / TILE, per = (all_tiles + jb.parts - 1) / jb.parts;
+    const int first = jb.f.first, n_rows = min(jb.f.count * p.rows - block * R, R);
+    if (job == jb.job0 && head == 0)
+      for (int i = tid; i < jb.f.count; i += NT) p.where[first + i] = i32x4{jb.job0, jb.blocks, jb.parts, i};
+
+    // rows of this lane's MFMA columns, and the tokens that they see
+    V8 qf[MR][KS];
+    int lo[MR], hi[MR];
+    int span_lo = 0x7fffffff, span_hi = 0, all_lo = 0, all_hi = 0x7fffffff;
+#pragma unroll
+    for (int rt = 0; rt < MR; ++rt) {
+      const int r = wave * 16 * MR + rt * 16 + li;
+      const bool live = r < n_rows;
+      const int vr = block * R + (live ? r : 0), i = vr / p.rows, rr = vr - i * p.rows;
+      const int s = rr / p.group, b = first + i;
+      const int act_k = min(max(p.act_k[b], 0), p.max_blocks * p.page);
+      const int act_q = p.act_q ? min(max(p.act_q[b], 0), p.s1) : p.s1;
+      paged_bounds(p, act_q, act_k, s, &lo[rt], &hi[rt]);
+      hi[rt] = live ? min(hi[rt], jb.f.tokens) : 0;
+      if (live && hi[rt] > lo[rt]) {
+        span_lo = min(span_lo, lo[rt]);
+        span_hi = max(span_hi, hi[rt]);
+      }
+      if (live) {
+        all_lo = max(all_lo, lo[rt]);
+        all_hi = min(all_hi, hi[rt]);
+      }
+      const int64_t row = ((int64_t)b * p.s1 + s) * p.n1 + head * p.group + (rr - s * p.group);
+      const u32x4 z = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 x = live ? *(const u32x4*)((const T*)p.q + row * D + ks * 32 + lg * 8) : z;
+        qf[rt][ks] = as_v8<V8>((x & keep) ^ flip);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) {
+      span_lo = min(span_lo, __shfl_xor(span_lo, o));
+      span_hi = max(span_hi, __shfl_xor(span_hi, o));
+      all_lo = max(all_lo, __shfl_xor(all_lo, o));
+      all_hi = min(all_hi, __shfl_xor(all_hi, o));
+    }
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    const bool active = wave * 16 * MR < n_rows;
+    __syncthreads();
+    if (tid == 0) s_span[0] = 0x7fffffff, s_span[1] = 0;
+    __syncthreads();
+    if (lane == 0) {
+      atomicMin(&s_span[0], span_lo);
+      atomicMax(&s_span[1], span_hi);
+    }
+    __syncthreads();
+    span_lo = __builtin_amdgcn_readfirstlane(s_span[0]);
+    span_hi = __builtin_amdgcn_readfirstlane(s_span[1]);
+    const int tok1 = min(min((part + 1) * per * TILE, jb.f.tokens), span_hi);
+    const int tok0 = max(part * per * TILE, span_lo / TILE * TILE);
+
+    f32x4 acc[ND][MR], accn[MR];
+    float ref[MR], top[MR], sum[MR];
+#pragma unroll
+    for (int rt = 0; rt < MR; ++rt) {
+      ref[rt] = top[rt] = -INFINITY;
+      sum[rt] = 0.f;
+      accn[rt] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < ND; ++j) acc[j][rt] = {0.f, 0.f, 0.f, 0.f};
+    }
+    const unsigned char* const kbase = (const unsigned char*)p.k + (int64_t)head * ROW;
+    const unsigned char* const vbase = (const unsigned char*)p.v + (int64_t)head * ROW;
+    const int32_t* const tab = p.table + (int64_t)first * p.max_blocks;
+
+    for (int ta = tok0; ta < tok1;) {
+      // the pages of as many tokens as the LDS holds entries for, in whole tiles
+      unsigned off0;
+      const int pg0 = (int)paged_split(p, (unsigned)ta, &off0);
+      const int64_t reach = (int64_t)(pg0 + kPrefixPages) * p.page;
+      const int tb = reach >= tok1 ? tok1 : (int)(reach / TILE * TILE);
+      const int npg = (int)paged_split(p, (unsigned)tb - 1u, &off0) - pg0 + 1;
+      lds_barrier();  // the entries and tiles before are read
+      for (int i = tid; i < npg; i += NT) s_tab[i] = tab[pg0 + i];
+#pragma unroll
+      for (int rt = 0; rt < MR; ++rt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[rt][ks]));  // (Q's loads end here)
+      lds_barrier();
+      const int n_tiles = (tb - ta + TILE - 1) / TILE;
+
+      // cache row of a token, -1 outside the span or without a page (read as zeros)
+      auto row_of = [&](int tok) -> int {
+        if (tok >= tb || tok < span_lo) return -1;
+        unsigned off;
+        const unsigned pg = paged_split(p, (unsigned)tok, &off);
+        const int blk = s_tab[(int)pg - pg0];
+        const int64_t r = (int64_t)blk * p.page + (int)off;
+        return blk < 0 || r >= p.kv_rows ? -1 : (int)r;
+      };
+      int rows = -1;  // lane e: first cache row of DMA e % NI of tile f0 + e / NI
+      auto fetch = [&](int f) {
+        if (NL < NW && wave >= NL) return;
+        const int stage = f % NB;
+        const int tok = ta + f * TILE;
+        if (one_page && (tok >= span_lo || tok >= tb)) {
+          if (f % kSteps == 0 || f == 0 || tok - TILE < span_lo) {
+            const int f0 = f - f % kSteps;
+            rows = row_of(ta + (f0 + lane / NI) * TILE + ((lane % NI) * NL + wave) * TPI);
+          }
+#pragma unroll
+          for (int j = 0; j < NI; ++j) {
+            const int r = __builtin_amdgcn_readlane(rows, (f % kSteps) * NI + j);
+            const int here = tok + (j * NL + wave) * TPI;
+            const int bytes = r < 0 ? 0 : min(tb - here, TPI) * (int)row_bytes;
+            const int64_t at = (int64_t)(r < 0 ? 0 : r) * row_bytes;
+            const unsigned dst = smem_base + stage * STAGE + (j * NL + wave) * 1024;
+            dma_buf16(dst, k_from[j], __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + at), (short)0, bytes, 0x00020000));
+            dma_buf16(dst + TILE_BYTES, v_from[j],
+                      __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + at), (short)0, bytes, 0x00020000));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < NI; ++j) {
+            const int tk = (j * NL + wave) * TPI + lane / CPT;
+            const int r = row_of(tok + tk);
+            const int kc = ((lane % CPT) ^ swz_k(tk)) * 16, vc = ((lane % CPT) ^ swz_v(tk)) * 16;
+            const unsigned dst = smem_base + stage * STAGE + (j * NL + wave) * 1024;
+            dma_glb16(dst, r >= 0 ? kbase + r * row_bytes + kc : g_prefix_zero_row + kc);
+            dma_glb16(dst + TILE_BYTES, r >= 0 ? vbase + r * row_bytes + vc : g_prefix_zero_row + vc);
+          }
+        }
+      };
+
+      float f_moved[MR];
+      bool moved = false;
+      // the first half of the softmax of tile t, in 2 + 2 HR slices
+      auto soft_a = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR], int t) {
+        if (k == 0) {
+          const int tk = ta + t * TILE;
+          if (tk < all_lo || tk + TILE > min(all_hi, tb)) {
+#pragma unroll
+            for (int rt = 0; rt < MR; ++rt)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int tok = tk + (i >> 2) * 16 + lg * 4 + (i & 3);
+                s[i >> 2][rt][i & 3] = tok >= lo[rt] && tok < min(hi[rt], tb) ? s[i >> 2][rt][i & 3] : -INFINITY;
+              }
+          }
+        } else if (k == 1) {
+          float m[MR];
+          bool moves = false;
+#pragma unroll
+          for (int rt = 0; rt < MR; ++rt) {
+            m[rt] = s[0][rt][0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) m[rt] = fmaxf(m[rt], s[i >> 2][rt][i & 3]);
+            top[rt] = fmaxf(top[rt], m[rt]);
+            moves |= m[rt] * scale > ref[rt] + kPaAbove;
+          }
+          moved = __any(moves);
+          if (moved) {
+#pragma unroll
+            for (int rt = 0; rt < MR; ++rt) {
+              const float mx = xgroup_max(m[rt]) * scale;
+              const float nref = mx > ref[rt] + kPaAbove ? mx - kPaBelow : ref[rt];
+              const float f = ref[rt] == -INFINITY ? 0.f : fast_exp2(ref[rt] - nref);
+              ref[rt] = nref;
+              sum[rt] *= f;
+              f_moved[rt] = f;
+            }
+          }
+        } else if (k < 2 + 2 * HR) {
+          const int rt = (k - 2) >> 1, tt = (k - 2) & 1;
+          const float from = ref[rt] == -INFINITY ? 0.f : ref[rt];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = fast_exp2(__builtin_fmaf(s[tt][rt][i], scale, -from));
+            sum[rt] += e;
+            ph[rt][tt * 4 + i] = E::from_f32(e);
+          }
+        }
+      };
+      // the second half, in 2 HR slices
+      auto soft_b = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR]) {
+        if (k < 2 * HR) {
+          const int rt = HR + (k >> 1), tt = k & 1;
+          const float from = ref[rt] == -INFINITY ? 0.f : ref[rt];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = fast_exp2(__builtin_fmaf(s[tt][rt][i], scale, -from));
+            sum[rt] += e;
+            ph[rt][tt * 4 + i] = E::from_f32(e);
+          }
+        }
+      };
+      // scores of a stage's tile
+      auto gemm1 = [&](int stage, f32x4 (&s)[2][MR], auto&& between) {
+        const unsigned char* at = smem + stage * STAGE;
+        const int base = k_at;
+        auto read = [&](int ks, int tt) {
+          return as_v8<V8>(*(const u32x4*)(at + ((base ^ ((ks & 3) << 6)) + tt * 16 * ROW + (ks >> 2) * 256)));
+        };
+        constexpr int PF = 2;
+        V8 fa[PF][2];
+#pragma unroll
+        for (int i = 0; i < PF; ++i)
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) fa[i][tt] = read(i, tt);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) {
+            const V8 f = fa[ks % PF][tt];
+            if (ks + PF < KS) fa[ks % PF][tt] = read(ks + PF, tt);
+#pragma unroll
+            for (int rt = 0; rt < MR; ++rt) {
+              const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+              s[tt][rt] = E::mfma(f, qf[rt][ks], ks == 0 ? z : s[tt][rt]);
+            }
+            between(ks * 2 + tt);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      };
+      // output of a stage's tile
+      auto gemm2 = [&](int stage, V8 (&ph)[MR], auto&& between) {
+        const unsigned char* at = smem + stage * STAGE + TILE_BYTES;
+        auto read = [&](int dt) -> V8 {
+          const unsigned char* pp = at + ((v_at ^ ((dt & 7) << 5)) + (dt >> 3) * 256);
+          const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)pp);
+          const bf16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(pp + 16 * ROW));
+          const i16x4 w1 = __builtin_bit_cast(i16x4, v1), w2 = __builtin_bit_cast(i16x4, v2);
+          const i16x8 w = {w1[0], w1[1], w1[2], w1[3], w2[0], w2[1], w2[2], w2[3]};
+          return __builtin_bit_cast(V8, w);
+        };
+        constexpr int PF = 3;
+        V8 va[PF];
+#pragma unroll
+        for (int i = 0; i < PF; ++i) va[i] = read(i);
+#pragma unroll
+        for (int rt = 0; rt < MR; ++rt) accn[rt] = E::mfma(ones, ph[rt], accn[rt]);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          const V8 f = va[dt % PF];
+          if (dt + PF < ND) va[dt % PF] = read(dt + PF);
+#pragma unroll
+          for (int rt = 0; rt < MR; ++rt) acc[dt][rt] = E::mfma(f, ph[rt], acc[dt][rt]);
+          between(dt);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      auto rescale = [&]() {
+        if (moved) {
+#pragma unroll
+          for (int rt = 0; rt < MR; ++rt) {
+            accn[rt] *= f_moved[rt];
+#pragma unroll
+            for (int j = 0; j < ND; ++j) acc[j][rt] *= f_moved[rt];
+          }
+        }
+      };
+      constexpr int NA = 2 + 2 * HR, NBH = 2 * HR;  // slices of the halves
+      f32x4 s0[2][MR], s1[2][MR];
+      V8 p0[MR], p1[MR];
+      auto step = [&](int t, f32x4 (&s)[2][MR], f32x4 (&sn)[2][MR], V8 (&ph)[MR], V8 (&pn)[MR]) {
+        // tile t + 1 has landed: all but the NB - 3 tiles asked for after it
+        wait_vmcnt<(NB - 3) * 2 * NI>();
+        lds_barrier();
+        fetch(t + NB - 1);
+        if (!active) return;
+        if (t + 1 < n_tiles) {
+          gemm1((t + 1) % NB, sn, [&](int i) {
+            // 2 KS places for NBH slices
+#pragma unroll
+            for (int k = i * NBH / (2 * KS); k < (i + 1) * NBH / (2 * KS); ++k) soft_b(k, s, ph);
+          });
+          gemm2(t % NB, ph, [&](int i) {
+#pragma unroll
+            for (int k = i * NA / ND; k < (i + 1) * NA / ND; ++k) soft_a(k, sn, pn, t + 1);
+          });
+          rescale();
+        } else {
+#pragma unroll
+          for (int k = 0; k < NBH; ++k) soft_b(k, s, ph);
+          gemm2(t % NB, ph, [](int) {});
+        }
+      };
+
+      // the first tiles (those past the end, here and below, read zeros, so
+      // that the number of DMAs in flight is known)
+#pragma unroll 1
+      for (int f = 0; f < NB - 1; ++f) fetch(f);
+      wait_vmcnt<(NB - 2) * 2 * NI>();
+      lds_barrier();
+      if (active) {
+        gemm1(0, s0, [](int) {});
+#pragma unroll
+        for (int k = 0; k < NA; ++k) soft_a(k, s0, p0, 0);
+        rescale();
+      }
+      for (int t = 0; t < n_tiles; t += 2) {
+        step(t, s0, s1, p0, p1);
+        if (t + 1 < n_tiles) step(t + 1, s1, s0, p1, p0);
+      }
+      wait_vmcnt<0>();  // of the DMAs past the end too: the ring is theirs until then
+      ta = tb;
+    }
+
+    // the job's output
+    const int64_t slot0 = p.part0 + ((int64_t)job * p.n2 + head) * R;
+#pragma unroll
+    for (int rt = 0; rt < MR; ++rt) {
+      const int r = wave * 16 * MR + rt * 16 + li;
+      const float l = xgroup_sum(sum[rt]), t = xgroup_max(top[rt]) * scale;
+      if (r >= n_rows) continue;
+      const float seen = l != 0.f ? 1.f : 0.f;
+      float* dst = p.part_o + (slot0 + r) * D + lg * 4;
+#pragma unroll
+      for (int j = 0; j < ND; ++j) *(f32x4*)(dst + j * 16) = paged_scaled(acc[j][rt], seen);
+      if (lg == 0) p.part_ml[slot0 + r] = {ref[rt], l, t, accn[rt][0]};
+    }
+    job = prefix_job_of(blockIdx.x, gridDim.x, ++round, p.n2, &head);
+    if (job < plan.jobs) jb = plan.next(p, lane, job);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the operator: the prefixes, what is behind them, and the join
+// ---------------------------------------------------------------------------
+struct PrefixShape {
+  PagedShape behind;
+  int workers, rows;   // jobs of one key head aimed at; rows of a block
+  int64_t jobs, grid;  // at most
+};
+
+static int prefix_rows(int64_t d, bool latent) { return latent ? kPrefixLatentRows : (d == 256 ? 128 : 256); }
+
+static PrefixShape prefix_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
+                                int64_t max_blocks, int64_t page) {
+  PrefixShape s;
+  s.behind = paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
+  s.rows = prefix_rows(d, latent);
+  const int64_t cus = device_cu_count();
+  s.workers = (int)(cus / n2 < 1 ? 1 : cus / n2);
+  const int64_t blocks = batch * s1 * (n1 / n2) / s.rows + batch / 2 + 1;
+  s.jobs = blocks >= (1ll << 30) ? 1ll << 31 : prefix_jobs((int)blocks, s.workers);
+  s.grid = (cus + 7) / 8 * 8;
+  return s;
+}
+
+bool paged_prefix_launchable(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
+                             int64_t max_blocks, int64_t page) {
+  const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
+  // (jobs, their places over all key heads, and the tiles of all blocks of rows are counted in 32 bits)
+  return s.jobs < (1ll << 26) && s.jobs * n2 + s.grid < (1ll << 31) &&
+         (batch * s1 * (n1 / n2) / s.rows + batch) * ((max_blocks * page + kPrefixTile - 1) / kPrefixTile) < (1ll << 31);
+}
+
+// rows of the outputs of runs, of sequences that a run has whole, and of jobs
+static int64_t prefix_run_rows(const PrefixShape& s) {
+  return (int64_t)s.behind.workers * 2 * s.behind.groups * s.behind.group_rows;
+}
+static int64_t prefix_whole_rows(const PrefixShape& s, int64_t batch) {
+  return batch * s.behind.groups * s.behind.group_rows;
+}
+static size_t prefix_part_rows(const PrefixShape& s, int64_t batch, int64_t n2) {
+  return (size_t)prefix_run_rows(s) + (size_t)prefix_whole_rows(s, batch) + (size_t)s.jobs * n2 * s.rows;
+}
+
+size_t paged_prefix_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
+                                    int64_t max_blocks, int64_t page) {
+  const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
+  return prefix_part_rows(s, batch, n2) * (sizeof(f32x4) + d * sizeof(float)) + (size_t)batch * sizeof(i32x4);
+}
+
+template <typename T>
+static void prefix_grouped_d(const PagedPrefixParams& p, int64_t d, unsigned grid, hipStream_t stream) {
+  if (d == 64) prefix_grouped_kernel<T, 64, 8, 2><<<grid, 512, 0, stream>>>(p);
+  else if (d == 128) prefix_grouped_kernel<T, 128, 8, 2><<<grid, 512, 0, stream>>>(p);
+  else prefix_grouped_kernel<T, 256, 4, 2><<<grid, 256, 0, stream>>>(p);
+}
+
+int paged_prefix_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
+                     const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
+                     const int32_t* act_k, const int32_t* table, const int32_t* ids, const int32_t* shared,
+                     int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, int64_t num_blocks, int64_t page,
+                     int64_t max_blocks, int32_t mode, int64_t pre_tokens, int64_t next_tokens, int32_t dtype,
+                     float scale, int32_t return_lse, void* workspace, hipStream_t stream) {
+  const bool latent = value == nullptr;
+  const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
+  PagedPrefixParams p = {};
+  paged_fill(p, s.behind, query, query_rope, key, key_rope, value, out, smax, ssum, act_q, act_k, table, batch, s1, n1,
+             n2, num_blocks, page, max_blocks, mode, pre_tokens, next_tokens, scale, return_lse);
+  const size_t rows = prefix_part_rows(s, batch, n2);
+  p.part_ml = (f32x4*)workspace;
+  p.part_o = (float*)(p.part_ml + rows);
+  p.where = (i32x4*)(p.part_o + rows * d);
+  p.whole0 = prefix_run_rows(s);
+  p.part0 = p.whole0 + prefix_whole_rows(s, batch);
+  p.ids = ids;
+  p.shared = shared;
+  p.prefix_workers = s.workers;
+  p.job_rows = s.rows;
+  const int64_t most = (s.jobs * n2 + 7) / 8 * 8;
+  const unsigned grid = (unsigned)(most < s.grid ? most : s.grid);
+  int st;
+  if (latent) {
+    st = prefix_latent_launch(p, d, dtype, grid, stream);
+    if (st != DSA_OK) return st;
+    st = paged_latent_launch(p, d, dtype, stream);
+  } else {
+    if (dtype == DSA_DTYPE_BF16) prefix_grouped_d<bf16>(p, d, grid, stream);
+    else prefix_grouped_d<f16>(p, d, grid, stream);
+    DSA_HIP(hipGetLastError());
+    st = paged_grouped_launch(p, d, dtype, stream);
+  }
+  if (st != DSA_OK) return st;
+  return paged_combine_launch(p, s.behind.tile, d, dtype, stream);
+}
+
+}  // namespace dsa

@@ -50,6 +50,8 @@ struct Entries {
   decltype(&dsa_paged_cache_plan) plan;
   decltype(&dsa_paged_cache_write_slots) write_slots;
   decltype(&dsa_paged_cache_prefixes) prefixes;
+  decltype(&dsa_paged_prefix_attn_workspace_size) prefix_attn_bytes;
+  decltype(&dsa_paged_prefix_attn) prefix_attn;
 } entry;
 
 // the HIP runtime reported an error at or before a launch
@@ -294,7 +296,9 @@ PyObject* compact(PyObject* const* a) {
 }
 
 // (query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
-// actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse) -> triple
+// actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse
+// [, prefix_groups, prefix_lengths]) -> triple
+template <bool PREFIX>
 PyObject* attention(PyObject* const* a) {
   int index = -1;
   const at::Tensor *q = tensor(a[0], &index), *k = tensor(a[1], &index), *v = nullptr, *qr = nullptr, *kr = nullptr;
@@ -325,13 +329,26 @@ PyObject* attention(PyObject* const* a) {
     if (!cache(v) || a[6] != Py_None || a[7] != Py_None || v->sizes() != k->sizes()) return nullptr;
   }
   if (a[8] != Py_None && (!(act_q = ints(a[8], &index, 1)) || act_q->size(0) != b)) return nullptr;
+  const at::Tensor *groups = nullptr, *shared = nullptr;
+  if (PREFIX) {
+    groups = ints(a[13], &index, 1), shared = ints(a[14], &index, 1);
+    if (!groups || !shared || groups->size(0) != b || shared->size(0) != b) return nullptr;
+  }
   const int64_t wide = table->size(1);
-  const size_t bytes = entry.attn_bytes(b, s1, n1, n2, d, latent, wide, page);
+  const size_t bytes = (PREFIX ? entry.prefix_attn_bytes : entry.attn_bytes)(b, s1, n1, n2, d, latent, wide, page);
   if (!bytes) return nullptr;
   at::Tensor out = fresh(q->sizes(), *q), mx = fresh({b, n2, s1, n1 / n2}, *q, at::kFloat);
   at::Tensor sm = fresh({b, n2, s1, n1 / n2}, *q, at::kFloat);
   c10::DataPtr ws = workspace(bytes);
-  if (!launched(entry.attn, q->data_ptr(), latent ? qr->data_ptr() : nullptr, k->data_ptr(), latent ? kr->data_ptr() : nullptr,
+  if (PREFIX) {
+    if (!launched(entry.prefix_attn, q->data_ptr(), latent ? qr->data_ptr() : nullptr, k->data_ptr(),
+                  latent ? kr->data_ptr() : nullptr, latent ? nullptr : v->data_ptr(), out.data_ptr(),
+                  (float*)mx.data_ptr(), (float*)sm.data_ptr(), data(act_q), data(act_k), data(table), data(groups),
+                  data(shared), b, s1, n1, n2, d, latent ? 64 : 0, pages, page, wide, (int32_t)mode, pre, next,
+                  kind == at::kHalf ? DSA_DTYPE_FP16 : DSA_DTYPE_BF16, (float)scale, lse, ws.get(), bytes,
+                  stream_of(index)))
+      return nullptr;
+  } else if (!launched(entry.attn, q->data_ptr(), latent ? qr->data_ptr() : nullptr, k->data_ptr(), latent ? kr->data_ptr() : nullptr,
                  latent ? nullptr : v->data_ptr(), out.data_ptr(), (float*)mx.data_ptr(), (float*)sm.data_ptr(),
                  data(act_q), data(act_k), data(table), b, s1, n1, n2, d, latent ? 64 : 0, pages, page, wide,
                  (int32_t)mode, pre, next, kind == at::kHalf ? DSA_DTYPE_FP16 : DSA_DTYPE_BF16, (float)scale, lse,
@@ -709,7 +726,8 @@ PyMethodDef methods[] = {
     {"write", FAST((call<write, 6>)), METH_FASTCALL, nullptr},
     {"fork", FAST((call<fork, 7>)), METH_FASTCALL, nullptr},
     {"compact", FAST((call<compact, 4>)), METH_FASTCALL, nullptr},
-    {"attention", FAST((call<attention, 13>)), METH_FASTCALL, nullptr},
+    {"attention", FAST((call<attention<false>, 13>)), METH_FASTCALL, nullptr},
+    {"prefix_attention", FAST((call<attention<true>, 15>)), METH_FASTCALL, nullptr},
     {"rotate", FAST((call<rotate<false>, 11>)), METH_FASTCALL, nullptr},
     {"rotate_axes", FAST((call<rotate<true>, 13>)), METH_FASTCALL, nullptr},
     {"plan", FAST((call<plan, 6>)), METH_FASTCALL, nullptr},

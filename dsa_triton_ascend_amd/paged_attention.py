@@ -4,7 +4,8 @@ and contexts where every cached token is attended.
 
 Two forms: grouped heads over key and value caches, and the MLA-absorb form
 over the latent cache of the sparse operators (value = key[..., :D], one key
-head, rope parts of 64 columns).  The reference has no such operator; argument
+head, rope parts of 64 columns).  ``paged_prefix_attention`` reads a prefix
+that sequences share once for all of them.  The reference has no such operator; argument
 names, masks, zero rows and the return triple are those of
 ``sparse_flash_attention``.
 """
@@ -50,6 +51,48 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
                                     return_softmax_lse)
     if result is not None:
         return result
+    return _attend(query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
+                   actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse)
+
+
+def paged_prefix_attention(query, key, value, block_table, actual_seq_lengths_kv, prefix_groups, prefix_lengths,
+                           scale_value=1.0, query_rope=None, key_rope=None, actual_seq_lengths_query=None,
+                           sparse_mode=3, pre_tokens=INT64_MAX, next_tokens=INT64_MAX, return_softmax_lse=False):
+    """``paged_attention`` of sequences that share a prefix (a system prompt, a
+    common document or image, the beams of a fork), which is read once for all
+    of them.
+
+    Neighbouring sequences with the same ``prefix_groups`` entry and the same
+    ``prefix_lengths`` entry are a family (int32 [B], as from
+    ``paged_cache_prefixes``): the first ``prefix_lengths`` tokens of each are
+    those in the pages of the family's first sequence; what follows is in the
+    pages of each sequence.  A negative group, a length of 0 and a sequence
+    alone share nothing.  The prefix may end inside a page and may be longer
+    than some of the sequences.  Results are those of ``paged_attention`` where the
+    sequences' rows of the table name the same pages for the prefix, rounded
+    once more in the weights: the numerators of a prefix are rounded to the
+    input type in both forms.  A value of the prefix that one row of a family
+    sees and another does not must be finite.
+
+    Everything else as in ``paged_attention``.
+    """
+    result = _lib.calls().prefix_attention(
+        query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
+        actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse, prefix_groups,
+        prefix_lengths)
+    if result is not None:
+        return result
+    if prefix_groups is None or prefix_lengths is None:
+        raise ValueError("prefix_groups and prefix_lengths are required")
+    return _attend(query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
+                   actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse,
+                   (prefix_groups, prefix_lengths))
+
+
+def _attend(query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
+            actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse, prefix=None):
+    """The call on arguments of any kind that may be converted; ``prefix``:
+    None, or the groups and lengths of shared prefixes."""
     pre_tokens, next_tokens = _band_args(pre_tokens, next_tokens)
     if sparse_mode not in (0, 3):
         raise ValueError("Only sparse_mode 0 (full) / 3 (rightDownCausal) supported")
@@ -96,13 +139,19 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
         raise ValueError("block_table and actual_seq_lengths_kv are required")
     if block_table.dim() != 2 or block_table.shape[0] < B:
         raise ValueError(f"block_table must be [B, max_blocks] with B={B} rows, got {tuple(block_table.shape)}")
-    _lib.no_derivatives("paged_attention", query, *(t for _, t in others))
+    what = "paged_attention" if prefix is None else "paged_prefix_attention"
+    _lib.no_derivatives(what, query, *(t for _, t in others))
     index = _lib.same_device(query, key, value, query_rope, key_rope, block_table)
     dev = query.device
     act_k = _lengths(actual_seq_lengths_kv, dev)
     act_q = None if actual_seq_lengths_query is None else _lengths(actual_seq_lengths_query, dev)
     if act_k.numel() != B or (act_q is not None and act_q.numel() != B):
         raise ValueError("actual sequence length arrays must have one entry per batch")
+    families = ()
+    if prefix is not None:
+        families = tuple(_lengths(x, dev) for x in prefix)
+        if any(x.numel() != B for x in families):
+            raise ValueError(f"prefix_groups and prefix_lengths must have one entry per sequence ({B})")
     for name, t in others:
         if name != "query_rope" and not t.is_contiguous():
             raise ValueError(f"the {name} cache must be contiguous (a copy of it would be made at every call)")
@@ -120,16 +169,18 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
     if key.numel() == 0 or wide == 0:  # no page at all: no row sees a token
         return out.zero_(), smax.zero_(), ssum.zero_()
     lib = _lib.load()
-    nbytes = _lib.call_on(index, lib.dsa_paged_attn_workspace_size, B, S1, N1, N2, D, latent, wide, page)
+    entry, size = ((lib.dsa_paged_attn, lib.dsa_paged_attn_workspace_size) if prefix is None else
+                   (lib.dsa_paged_prefix_attn, lib.dsa_paged_prefix_attn_workspace_size))
+    nbytes = _lib.call_on(index, size, B, S1, N1, N2, D, latent, wide, page)
     ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
     status = _lib.call_on(
-        index, lib.dsa_paged_attn, q.data_ptr(), qr.data_ptr() if latent else None, key.data_ptr(),
+        index, entry, q.data_ptr(), qr.data_ptr() if latent else None, key.data_ptr(),
         key_rope.data_ptr() if latent else None, None if latent else value.data_ptr(), out.data_ptr(),
         smax.data_ptr(), ssum.data_ptr(), None if act_q is None else act_q.data_ptr(), act_k.data_ptr(),
-        table.data_ptr(), B, S1, N1, N2, D, _D_ROPE if latent else 0, pages, page, wide, sparse_mode, pre_tokens,
+        table.data_ptr(), *(x.data_ptr() for x in families), B, S1, N1, N2, D, _D_ROPE if latent else 0, pages, page, wide, sparse_mode, pre_tokens,
         next_tokens, code, float(scale_value), bool(return_softmax_lse), ws.data_ptr(), nbytes, _lib.raw_stream(index))
     if status:
-        _lib.check(status, "dsa_paged_attn")
+        _lib.check(status, "dsa_" + what.replace("attention", "attn"))
     return out, smax, ssum
 
 
@@ -173,5 +224,19 @@ class PagedAttention(torch.nn.Module):
             query_rope=query_rope, key_rope=key_rope, actual_seq_lengths_query=actual_seq_lengths_query,
             sparse_mode=self.sparse_mode, pre_tokens=self.pre_tokens, next_tokens=self.next_tokens,
             return_softmax_lse=self.return_softmax_lse)
+
+    construct = forward
+
+
+class PagedPrefixAttention(PagedAttention):
+    """Module wrapper of ``paged_prefix_attention``."""
+
+    def forward(self, query, key, value, block_table, actual_seq_lengths_kv, prefix_groups, prefix_lengths,
+                query_rope=None, key_rope=None, actual_seq_lengths_query=None):
+        return paged_prefix_attention(
+            query, key, value, block_table, actual_seq_lengths_kv, prefix_groups, prefix_lengths,
+            scale_value=self.scale_value, query_rope=query_rope, key_rope=key_rope,
+            actual_seq_lengths_query=actual_seq_lengths_query, sparse_mode=self.sparse_mode,
+            pre_tokens=self.pre_tokens, next_tokens=self.next_tokens, return_softmax_lse=self.return_softmax_lse)
 
     construct = forward

@@ -574,6 +574,29 @@ int dsa_paged_attn(const void* query, const void* query_rope, const void* key, c
                    int64_t next_tokens, int32_t dtype, float scale_value, int32_t return_lse, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/*
+ * dsa_paged_attn for sequences that share a prefix.  A family is a run of
+ * neighbouring sequences with the same prefix_groups entry (at least 0) and the
+ * same prefix_lengths entry (at least 1): their first prefix_lengths tokens are
+ * those of the family's first sequence, whose pages alone are read for them, once
+ * for all; tokens from there on are each sequence's own.  Sequences of their own
+ * share nothing, whatever their length says.  Results are those of dsa_paged_attn
+ * where the sequences' tables name the same pages for the prefix.  A value of the
+ * prefix that one row of a family sees and another does not must be finite.
+ * Everything else as dsa_paged_attn; the query rows and the tiles of 32 tokens of a
+ * table row are fewer than 2^31 as a product.
+ */
+size_t dsa_paged_prefix_attn_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d,
+                                            int32_t latent, int64_t max_blocks, int64_t page_size);
+int dsa_paged_prefix_attn(const void* query, const void* query_rope, const void* key, const void* key_rope,
+                          const void* value, void* attention_out, float* softmax_max, float* softmax_sum,
+                          const int32_t* actual_seq_q, const int32_t* actual_seq_kv, const int32_t* block_table,
+                          const int32_t* prefix_groups, const int32_t* prefix_lengths, int64_t batch, int64_t s1,
+                          int64_t n1, int64_t n2, int64_t d, int64_t d_rope, int64_t num_blocks, int64_t page_size,
+                          int64_t max_blocks, int32_t sparse_mode, int64_t pre_tokens, int64_t next_tokens,
+                          int32_t dtype, float scale_value, int32_t return_lse, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
