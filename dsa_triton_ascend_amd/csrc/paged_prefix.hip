@@ -33,7 +33,9 @@ __device__ __attribute__((aligned(16))) unsigned char g_prefix_zero_row[1024];
 
 constexpr int kPrefixPages = 1024;  // block-table entries held in LDS
 
-template <int D> constexpr int kPrefixRing = D == 256 ? 4 : (D == 128 ? 6 : 8);
+// tiles of a stage of the ring, and stages
+template <int D> constexpr int kPrefixSub = D == 256 ? 1 : 2;
+template <int D> constexpr int kPrefixRing = D == 64 ? 6 : 4;
 
 template <typename T, int D, int NW, int MR>
 __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixParams p) {
@@ -45,14 +47,15 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
   constexpr int ROW = D * 2;
   constexpr int CPT = D / 8;                // 16-byte chunks of a token
   constexpr int TPI = 64 / CPT;             // tokens of one DMA
-  constexpr int NL = TILE / TPI < NW ? TILE / TPI : NW;  // waves that fetch
-  constexpr int NI = TILE / TPI / NL;       // their DMAs per tile of K, and of V
-  constexpr int TILE_BYTES = TILE * ROW, STAGE = 2 * TILE_BYTES, NB = kPrefixRing<D>;
-  constexpr int kSteps = 64 / NI;           // tiles whose rows a register holds
+  constexpr int SUB = kPrefixSub<D>, FETCH = TILE * SUB;   // tokens of a stage
+  constexpr int NI = FETCH / TPI / NW;      // DMAs of a wave per stage of K, and of V
+  constexpr int K_BYTES = FETCH * ROW, STAGE = 2 * K_BYTES, NB = kPrefixRing<D>;
+  constexpr int kStages = 64 / NI;          // stages whose rows a register holds
   constexpr int HR = MR / 2;                // row tiles of the first half of a softmax
-  static_assert(NI * NL * TPI == TILE && MR % 2 == 0, "tile split");
+  static_assert(NI * NW * TPI == FETCH && MR % 2 == 0 && NB * STAGE <= 131072, "tile split");
   __shared__ __attribute__((aligned(16))) unsigned char smem[NB * STAGE];
   __shared__ int s_tab[kPrefixPages];
+  __shared__ int s_lo[R], s_hi[R];  // tokens that the rows see
   __shared__ int s_span[2];
 
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
@@ -66,14 +69,14 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
   const unsigned smem_base = (unsigned)(uintptr_t)smem;
   // a DMA lies in one page, at an offset that 32 bits hold
   const bool one_page = p.page % TPI == 0 && row_bytes * TPI < (1ll << 31);
-  // where a lane reads and the wave's DMAs take from
+  // where a lane reads, and the wave's DMAs take from
   const int k_at = li * ROW + ((lg ^ swz_k(li)) * 16);
   const int v_tok = lg * 4 + (li >> 2);
-  const int v_at = v_tok * ROW + ((((li & 3) >> 1) ^ swz_v(v_tok)) * 16) + (li & 1) * 8;
+  const int v_at = K_BYTES + v_tok * ROW + ((((li & 3) >> 1) ^ swz_v(v_tok)) * 16) + (li & 1) * 8;
   int k_from[NI], v_from[NI];
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
-    const int tk = (j * NL + wave) * TPI + lane / CPT;
+    const int tk = (j * NW + wave) * TPI + lane / CPT;
     k_from[j] = (int)((lane / CPT) * row_bytes) + ((lane % CPT) ^ swz_k(tk)) * 16;
     v_from[j] = (int)((lane / CPT) * row_bytes) + ((lane % CPT) ^ swz_v(tk)) * 16;
   }
@@ -94,7 +97,8 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
 
     // rows of this lane's MFMA columns, and the tokens that they see
     V8 qf[MR][KS];
-    int lo[MR], hi[MR];
+    __syncthreads();  // (the job before has read what it left)
+    if (tid == 0) s_span[0] = 0x7fffffff, s_span[1] = 0;
     int span_lo = 0x7fffffff, span_hi = 0, all_lo = 0, all_hi = 0x7fffffff;
 #pragma unroll
     for (int rt = 0; rt < MR; ++rt) {
@@ -104,15 +108,17 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
       const int s = rr / p.group, b = first + i;
       const int act_k = min(max(p.act_k[b], 0), p.max_blocks * p.page);
       const int act_q = p.act_q ? min(max(p.act_q[b], 0), p.s1) : p.s1;
-      paged_bounds(p, act_q, act_k, s, &lo[rt], &hi[rt]);
-      hi[rt] = live ? min(hi[rt], jb.f.tokens) : 0;
-      if (live && hi[rt] > lo[rt]) {
-        span_lo = min(span_lo, lo[rt]);
-        span_hi = max(span_hi, hi[rt]);
+      int lo, hi;
+      paged_bounds(p, act_q, act_k, s, &lo, &hi);
+      hi = live ? min(hi, jb.f.tokens) : 0;
+      if (lg == 0) s_lo[r] = lo, s_hi[r] = hi;
+      if (live && hi > lo) {
+        span_lo = min(span_lo, lo);
+        span_hi = max(span_hi, hi);
       }
       if (live) {
-        all_lo = max(all_lo, lo[rt]);
-        all_hi = min(all_hi, hi[rt]);
+        all_lo = max(all_lo, lo);
+        all_hi = min(all_hi, hi);
       }
       const int64_t row = ((int64_t)b * p.s1 + s) * p.n1 + head * p.group + (rr - s * p.group);
       const u32x4 z = {0u, 0u, 0u, 0u};
@@ -132,8 +138,6 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
     all_lo = __builtin_amdgcn_readfirstlane(all_lo);
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
     const bool active = wave * 16 * MR < n_rows;
-    __syncthreads();
-    if (tid == 0) s_span[0] = 0x7fffffff, s_span[1] = 0;
     __syncthreads();
     if (lane == 0) {
       atomicMin(&s_span[0], span_lo);
@@ -184,54 +188,64 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
         const int64_t r = (int64_t)blk * p.page + (int)off;
         return blk < 0 || r >= p.kv_rows ? -1 : (int)r;
       };
-      int rows = -1;  // lane e: first cache row of DMA e % NI of tile f0 + e / NI
-      auto fetch = [&](int f) {
-        if (NL < NW && wave >= NL) return;
-        const int stage = f % NB;
-        const int tok = ta + f * TILE;
+      int rows = -1;  // lane e: first cache row of DMA e % NI of stage f0 + e / NI
+      // the f-th stage's tokens into the ring at `at`
+      auto fetch = [&](int f, int at) {
+        const int tok = ta + f * FETCH;
+        const unsigned dst = smem_base + at + wave * 1024;
         if (one_page && (tok >= span_lo || tok >= tb)) {
-          if (f % kSteps == 0 || f == 0 || tok - TILE < span_lo) {
-            const int f0 = f - f % kSteps;
-            rows = row_of(ta + (f0 + lane / NI) * TILE + ((lane % NI) * NL + wave) * TPI);
-          }
+          if (f % kStages == 0 || tok - FETCH < span_lo)
+            rows = row_of(ta + (f - f % kStages + lane / NI) * FETCH + ((lane % NI) * NW + wave) * TPI);
 #pragma unroll
           for (int j = 0; j < NI; ++j) {
-            const int r = __builtin_amdgcn_readlane(rows, (f % kSteps) * NI + j);
-            const int here = tok + (j * NL + wave) * TPI;
+            const int r = __builtin_amdgcn_readlane(rows, (f % kStages) * NI + j);
+            const int here = tok + (j * NW + wave) * TPI;
             const int bytes = r < 0 ? 0 : min(tb - here, TPI) * (int)row_bytes;
-            const int64_t at = (int64_t)(r < 0 ? 0 : r) * row_bytes;
-            const unsigned dst = smem_base + stage * STAGE + (j * NL + wave) * 1024;
-            dma_buf16(dst, k_from[j], __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + at), (short)0, bytes, 0x00020000));
-            dma_buf16(dst + TILE_BYTES, v_from[j],
-                      __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + at), (short)0, bytes, 0x00020000));
+            const int64_t from = (int64_t)(r < 0 ? 0 : r) * row_bytes;
+            dma_buf16(dst + j * NW * 1024, k_from[j],
+                      __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + from), (short)0, bytes, 0x00020000));
+            dma_buf16(dst + j * NW * 1024 + K_BYTES, v_from[j],
+                      __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + from), (short)0, bytes, 0x00020000));
           }
         } else {
 #pragma unroll
           for (int j = 0; j < NI; ++j) {
-            const int tk = (j * NL + wave) * TPI + lane / CPT;
+            const int tk = (j * NW + wave) * TPI + lane / CPT;
             const int r = row_of(tok + tk);
             const int kc = ((lane % CPT) ^ swz_k(tk)) * 16, vc = ((lane % CPT) ^ swz_v(tk)) * 16;
-            const unsigned dst = smem_base + stage * STAGE + (j * NL + wave) * 1024;
-            dma_glb16(dst, r >= 0 ? kbase + r * row_bytes + kc : g_prefix_zero_row + kc);
-            dma_glb16(dst + TILE_BYTES, r >= 0 ? vbase + r * row_bytes + vc : g_prefix_zero_row + vc);
+            dma_glb16(dst + j * NW * 1024, r >= 0 ? kbase + r * row_bytes + kc : g_prefix_zero_row + kc);
+            dma_glb16(dst + j * NW * 1024 + K_BYTES, r >= 0 ? vbase + r * row_bytes + vc : g_prefix_zero_row + vc);
           }
         }
       };
 
       float f_moved[MR];
       bool moved = false;
-      // the first half of the softmax of tile t, in 2 + 2 HR slices
+      auto weights = [&](int rt, int tt, f32x4 (&s)[2][MR], V8 (&ph)[MR]) {
+        const float from = ref[rt] == -INFINITY ? 0.f : ref[rt];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = fast_exp2(__builtin_fmaf(s[tt][rt][i], scale, -from));
+          sum[rt] += e;
+          ph[rt][tt * 4 + i] = E::from_f32(e);
+        }
+      };
+      // the first half of the softmax of tile t, in NA slices
+      constexpr int NA = 2 + 2 * HR, NBH = 2 * HR;
       auto soft_a = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR], int t) {
         if (k == 0) {
           const int tk = ta + t * TILE;
           if (tk < all_lo || tk + TILE > min(all_hi, tb)) {
+            const int mine = tk + lg * 4;
 #pragma unroll
-            for (int rt = 0; rt < MR; ++rt)
+            for (int rt = 0; rt < MR; ++rt) {
+              const int r = wave * 16 * MR + rt * 16 + li, lo = s_lo[r], hi = min(s_hi[r], tb);
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const int tok = tk + (i >> 2) * 16 + lg * 4 + (i & 3);
-                s[i >> 2][rt][i & 3] = tok >= lo[rt] && tok < min(hi[rt], tb) ? s[i >> 2][rt][i & 3] : -INFINITY;
+                const int tok = mine + (i >> 2) * 16 + (i & 3);
+                s[i >> 2][rt][i & 3] = tok >= lo && tok < hi ? s[i >> 2][rt][i & 3] : -INFINITY;
               }
+            }
           }
         } else if (k == 1) {
           float m[MR];
@@ -256,49 +270,46 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
               f_moved[rt] = f;
             }
           }
-        } else if (k < 2 + 2 * HR) {
-          const int rt = (k - 2) >> 1, tt = (k - 2) & 1;
-          const float from = ref[rt] == -INFINITY ? 0.f : ref[rt];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = fast_exp2(__builtin_fmaf(s[tt][rt][i], scale, -from));
-            sum[rt] += e;
-            ph[rt][tt * 4 + i] = E::from_f32(e);
-          }
+        } else if (k < NA) {
+          weights((k - 2) >> 1, (k - 2) & 1, s, ph);
         }
       };
-      // the second half, in 2 HR slices
-      auto soft_b = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR]) {
-        if (k < 2 * HR) {
-          const int rt = HR + (k >> 1), tt = k & 1;
-          const float from = ref[rt] == -INFINITY ? 0.f : ref[rt];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = fast_exp2(__builtin_fmaf(s[tt][rt][i], scale, -from));
-            sum[rt] += e;
-            ph[rt][tt * 4 + i] = E::from_f32(e);
-          }
-        }
+      // the second half, in NBH slices
+      auto soft_b = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR]) { weights(HR + (k >> 1), k & 1, s, ph); };
+      // The first fragments of a product are read while the one before it ends:
+      // both tiles have landed by then.
+      constexpr int PK = 2, PV = 2;
+      V8 ka[PK][2], va[PV];
+      auto read_k = [&](int base, int ks, int tt) {
+        return as_v8<V8>(*(const u32x4*)(smem + (base ^ ((ks & 3) << 6)) + tt * 16 * ROW + (ks >> 2) * 256));
       };
-      // scores of a stage's tile
-      auto gemm1 = [&](int stage, f32x4 (&s)[2][MR], auto&& between) {
-        const unsigned char* at = smem + stage * STAGE;
-        const int base = k_at;
-        auto read = [&](int ks, int tt) {
-          return as_v8<V8>(*(const u32x4*)(at + ((base ^ ((ks & 3) << 6)) + tt * 16 * ROW + (ks >> 2) * 256)));
-        };
-        constexpr int PF = 2;
-        V8 fa[PF][2];
+      auto read_v = [&](int base, int dt) -> V8 {
+        const unsigned char* pp = smem + (base ^ ((dt & 7) << 5)) + (dt >> 3) * 256;
+        const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)pp);
+        const bf16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(pp + 16 * ROW));
+        const i16x4 w1 = __builtin_bit_cast(i16x4, v1), w2 = __builtin_bit_cast(i16x4, v2);
+        const i16x8 w = {w1[0], w1[1], w1[2], w1[3], w2[0], w2[1], w2[2], w2[3]};
+        return __builtin_bit_cast(V8, w);
+      };
+      auto first_k = [&](int at) {
 #pragma unroll
-        for (int i = 0; i < PF; ++i)
+        for (int i = 0; i < PK; ++i)
 #pragma unroll
-          for (int tt = 0; tt < 2; ++tt) fa[i][tt] = read(i, tt);
+          for (int tt = 0; tt < 2; ++tt) ka[i][tt] = read_k(at + k_at, i, tt);
+      };
+      auto first_v = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < PV; ++i) va[i] = read_v(at + v_at, i);
+      };
+      // scores of the tile at `at`; behind them the tile at `then` is multiplied
+      auto gemm1 = [&](int at, int then, f32x4 (&s)[2][MR], auto&& between) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) {
-            const V8 f = fa[ks % PF][tt];
-            if (ks + PF < KS) fa[ks % PF][tt] = read(ks + PF, tt);
+            const V8 f = ka[ks % PK][tt];
+            if (ks + PK < KS) ka[ks % PK][tt] = read_k(at + k_at, ks + PK, tt);
+            else if (ks + 1 == KS && tt == 0) first_v(then);
 #pragma unroll
             for (int rt = 0; rt < MR; ++rt) {
               const f32x4 z = {0.f, 0.f, 0.f, 0.f};
@@ -309,35 +320,21 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
           }
         }
       };
-      // output of a stage's tile
-      auto gemm2 = [&](int stage, V8 (&ph)[MR], auto&& between) {
-        const unsigned char* at = smem + stage * STAGE + TILE_BYTES;
-        auto read = [&](int dt) -> V8 {
-          const unsigned char* pp = at + ((v_at ^ ((dt & 7) << 5)) + (dt >> 3) * 256);
-          const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)pp);
-          const bf16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(pp + 16 * ROW));
-          const i16x4 w1 = __builtin_bit_cast(i16x4, v1), w2 = __builtin_bit_cast(i16x4, v2);
-          const i16x8 w = {w1[0], w1[1], w1[2], w1[3], w2[0], w2[1], w2[2], w2[3]};
-          return __builtin_bit_cast(V8, w);
-        };
-        constexpr int PF = 3;
-        V8 va[PF];
-#pragma unroll
-        for (int i = 0; i < PF; ++i) va[i] = read(i);
+      // output of the tile at `at`; behind it come the scores of the tile at `then`
+      auto gemm2 = [&](int at, int then, V8 (&ph)[MR], auto&& between) {
 #pragma unroll
         for (int rt = 0; rt < MR; ++rt) accn[rt] = E::mfma(ones, ph[rt], accn[rt]);
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) {
-          const V8 f = va[dt % PF];
-          if (dt + PF < ND) va[dt % PF] = read(dt + PF);
+          const V8 f = va[dt % PV];
+          if (dt + PV < ND) va[dt % PV] = read_v(at + v_at, dt + PV);
+          else if (SUB == 2 && dt + 1 == ND) first_k(then);
 #pragma unroll
           for (int rt = 0; rt < MR; ++rt) acc[dt][rt] = E::mfma(f, ph[rt], acc[dt][rt]);
           between(dt);
           __builtin_amdgcn_sched_barrier(0);
         }
-      };
-      auto rescale = [&]() {
-        if (moved) {
+        if (moved) {  // for the tile after this one
 #pragma unroll
           for (int rt = 0; rt < MR; ++rt) {
             accn[rt] *= f_moved[rt];
@@ -346,48 +343,84 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
           }
         }
       };
-      constexpr int NA = 2 + 2 * HR, NBH = 2 * HR;  // slices of the halves
-      f32x4 s0[2][MR], s1[2][MR];
-      V8 p0[MR], p1[MR];
-      auto step = [&](int t, f32x4 (&s)[2][MR], f32x4 (&sn)[2][MR], V8 (&ph)[MR], V8 (&pn)[MR]) {
-        // tile t + 1 has landed: all but the NB - 3 tiles asked for after it
-        wait_vmcnt<(NB - 3) * 2 * NI>();
-        lds_barrier();
-        fetch(t + NB - 1);
-        if (!active) return;
-        if (t + 1 < n_tiles) {
-          gemm1((t + 1) % NB, sn, [&](int i) {
-            // 2 KS places for NBH slices
-#pragma unroll
-            for (int k = i * NBH / (2 * KS); k < (i + 1) * NBH / (2 * KS); ++k) soft_b(k, s, ph);
-          });
-          gemm2(t % NB, ph, [&](int i) {
-#pragma unroll
-            for (int k = i * NA / ND; k < (i + 1) * NA / ND; ++k) soft_a(k, sn, pn, t + 1);
-          });
-          rescale();
-        } else {
-#pragma unroll
-          for (int k = 0; k < NBH; ++k) soft_b(k, s, ph);
-          gemm2(t % NB, ph, [](int) {});
-        }
-      };
 
       // the first tiles (those past the end, here and below, read zeros, so
       // that the number of DMAs in flight is known)
 #pragma unroll 1
-      for (int f = 0; f < NB - 1; ++f) fetch(f);
+      for (int f = 0; f < NB - 1; ++f) fetch(f, f * STAGE);
       wait_vmcnt<(NB - 2) * 2 * NI>();
       lds_barrier();
+      // step t: scores of tile t + 1 (of no visible token after the last) with the
+      // second half of the softmax of tile t, then the output of tile t with the
+      // first half of that of tile t + 1
+      int at = 0;  // of the stage of tile t
+      const int n_stages = (n_tiles + SUB - 1) / SUB;
+      auto next_stage = [&](int x) { return x == (NB - 1) * STAGE ? 0 : x + STAGE; };
+      auto open_stage = [&](int f) {
+        wait_vmcnt<(NB - 3) * 2 * NI>();  // the stage after it has landed
+        lds_barrier();
+        fetch(f + NB - 1, at == 0 ? (NB - 1) * STAGE : at - STAGE);
+      };
       if (active) {
-        gemm1(0, s0, [](int) {});
+        f32x4 s0[2][MR], s1[2][MR];
+        V8 p0[MR], p1[MR];
+        first_k(0);
+        gemm1(0, 0, s0, [](int) {});
 #pragma unroll
         for (int k = 0; k < NA; ++k) soft_a(k, s0, p0, 0);
-        rescale();
-      }
-      for (int t = 0; t < n_tiles; t += 2) {
-        step(t, s0, s1, p0, p1);
-        if (t + 1 < n_tiles) step(t + 1, s1, s0, p1, p0);
+        if (moved) {
+#pragma unroll
+          for (int rt = 0; rt < MR; ++rt) {
+            accn[rt] *= f_moved[rt];
+#pragma unroll
+            for (int j = 0; j < ND; ++j) acc[j][rt] *= f_moved[rt];
+          }
+        }
+        // tiles t, t + 1 and t + 2 lie at `cur`, `next` and `then`
+        auto step = [&](int t, int cur, int next, int then, f32x4 (&s)[2][MR], f32x4 (&sn)[2][MR], V8 (&ph)[MR],
+                        V8 (&pn)[MR]) {
+          gemm1(next, cur, sn, [&](int i) {
+            // 2 KS places for NBH slices
+#pragma unroll
+            for (int k = i * NBH / (2 * KS); k < (i + 1) * NBH / (2 * KS); ++k) soft_b(k, s, ph);
+          });
+          gemm2(cur, then, ph, [&](int i) {
+#pragma unroll
+            for (int k = i * NA / ND; k < (i + 1) * NA / ND; ++k) soft_a(k, sn, pn, t + 1);
+          });
+        };
+        // (the first fragments of tile 1's scores: its stage has landed)
+        if constexpr (SUB == 2) first_k(TILE * ROW);
+        for (int t = 0;;) {
+          open_stage(t / SUB);
+          int next = next_stage(at);
+          asm volatile("" : "+s"(next));  // (so that each stage's offsets fit the instructions)
+          if constexpr (SUB == 2) {
+            step(t, at, at + TILE * ROW, next, s0, s1, p0, p1);
+            at = next;  // (of tile t + 2)
+            if (++t >= n_tiles) break;
+            const int here = next == 0 ? (NB - 1) * STAGE : next - STAGE;
+            step(t, here + TILE * ROW, next, next + TILE * ROW, s1, s0, p1, p0);
+            if (++t >= n_tiles) break;
+          } else {
+            int then = next_stage(next);
+            asm volatile("" : "+s"(then));
+            first_k(next);
+            step(t, at, next, next, s0, s1, p0, p1);
+            at = next;
+            if (++t >= n_tiles) break;
+            open_stage(t);
+            first_k(then);
+            step(t, at, then, then, s1, s0, p1, p0);
+            at = then;
+            if (++t >= n_tiles) break;
+          }
+        }
+      } else {
+        for (int f = 0; f < n_stages; ++f) {
+          open_stage(f);
+          at = next_stage(at);
+        }
       }
       wait_vmcnt<0>();  // of the DMAs past the end too: the ring is theirs until then
       ta = tb;
