@@ -64,6 +64,7 @@ struct PagedPrefixParams : PagedAttnParams {
   int64_t whole0, part0;
   int prefix_workers;           // jobs of one key head aimed at
   int job_rows;                 // rows of a block
+  unsigned rows_magic, group_magic;  // floor((2^32 - 1) / rows), of group
 };
 
 template <typename P> constexpr bool kPrefixed = std::is_same<P, PagedPrefixParams>::value;

@@ -37,7 +37,9 @@ constexpr int kPrefixPages = 1024;  // block-table entries held in LDS
 template <int D> constexpr int kPrefixSub = D == 256 ? 1 : 2;
 template <int D> constexpr int kPrefixRing = D == 64 ? 6 : 4;
 
-template <typename T, int D, int NW, int MR>
+// FAST: no DMA lies in two pages, none of its rows' offsets needs more than 32
+// bits, and there is no band whose lower end could lie inside a tile.
+template <typename T, int D, int NW, int MR, bool FAST>
 __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixParams p) {
   using E = Elem<T>;
   using V8 = typename E::v8;
@@ -56,7 +58,7 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
   __shared__ __attribute__((aligned(16))) unsigned char smem[NB * STAGE];
   __shared__ int s_tab[kPrefixPages];
   __shared__ int s_lo[R], s_hi[R];  // tokens that the rows see
-  __shared__ int s_span[2];
+  __shared__ int s_span[2], s_all[NW][2];  // tokens that any row sees, and that all rows of a wave do
 
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -67,8 +69,6 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
   const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
   const unsigned flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
   const unsigned smem_base = (unsigned)(uintptr_t)smem;
-  // a DMA lies in one page, at an offset that 32 bits hold
-  const bool one_page = p.page % TPI == 0 && row_bytes * TPI < (1ll << 31);
   // where a lane reads, and the wave's DMAs take from
   const int k_at = li * ROW + ((lg ^ swz_k(li)) * 16);
   const int v_tok = lg * 4 + (li >> 2);
@@ -84,68 +84,63 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = E::from_f32(1.f);
 
+  PrefixLengths lengths;
+  lengths.load(p, lane);
   PrefixPlan<R> plan;
   int head;
   int job = prefix_job_of(blockIdx.x, gridDim.x, 0, p.n2, &head);
-  typename PrefixPlan<R>::Job jb = plan.make(p, lane, job);
+  plan.make(p, lane);
   for (int round = 0; job < plan.jobs;) {
+    const typename PrefixPlan<R>::Job jb = plan.find(p, lane, job);
     const int part = (job - jb.job0) / jb.blocks, block = (job - jb.job0) - part * jb.blocks;
     const int all_tiles = (jb.f.tokens + TILE - 1) / TILE, per = (all_tiles + jb.parts - 1) / jb.parts;
     const int first = jb.f.first, n_rows = min(jb.f.count * p.rows - block * R, R);
     if (job == jb.job0 && head == 0)
       for (int i = tid; i < jb.f.count; i += NT) p.where[first + i] = i32x4{jb.job0, jb.blocks, jb.parts, i};
 
-    // rows of this lane's MFMA columns, and the tokens that they see
-    V8 qf[MR][KS];
-    __syncthreads();  // (the job before has read what it left)
-    if (tid == 0) s_span[0] = 0x7fffffff, s_span[1] = 0;
-    int span_lo = 0x7fffffff, span_hi = 0, all_lo = 0, all_hi = 0x7fffffff;
-#pragma unroll
-    for (int rt = 0; rt < MR; ++rt) {
-      const int r = wave * 16 * MR + rt * 16 + li;
-      const bool live = r < n_rows;
-      const int vr = block * R + (live ? r : 0), i = vr / p.rows, rr = vr - i * p.rows;
-      const int s = rr / p.group, b = first + i;
-      const int act_k = min(max(p.act_k[b], 0), p.max_blocks * p.page);
-      const int act_q = p.act_q ? min(max(p.act_q[b], 0), p.s1) : p.s1;
+    // the tokens that the rows see
+    lds_barrier();  // (the job before has read what it left)
+    if (tid < 2) s_span[tid] = tid ? 0 : 0x7fffffff;
+    if (tid < 2 * NW) s_all[tid >> 1][tid & 1] = tid & 1 ? 0x7fffffff : 0;
+    lds_barrier();
+    for (int r0 = wave * 64; r0 < n_rows; r0 += NT) {
+      const int r = min(r0 + lane, n_rows - 1);  // (all lanes go along: they have the lengths)
+      const unsigned vr = block * R + r, i = prefix_div(vr, p.rows, p.rows_magic);
+      const int s = prefix_div(vr - i * p.rows, p.group, p.group_magic);
       int lo, hi;
-      paged_bounds(p, act_q, act_k, s, &lo, &hi);
-      hi = live ? min(hi, jb.f.tokens) : 0;
-      if (lg == 0) s_lo[r] = lo, s_hi[r] = hi;
-      if (live && hi > lo) {
-        span_lo = min(span_lo, lo);
-        span_hi = max(span_hi, hi);
+      lengths.bounds(p, first + i, s, jb.f.tokens, &lo, &hi);
+      s_lo[r] = lo, s_hi[r] = hi;
+      if (hi > lo) {
+        atomicMin(&s_span[0], lo);
+        atomicMax(&s_span[1], hi);
       }
-      if (live) {
-        all_lo = max(all_lo, lo);
-        all_hi = min(all_hi, hi);
-      }
-      const int64_t row = ((int64_t)b * p.s1 + s) * p.n1 + head * p.group + (rr - s * p.group);
-      const u32x4 z = {0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 x = live ? *(const u32x4*)((const T*)p.q + row * D + ks * 32 + lg * 8) : z;
-        qf[rt][ks] = as_v8<V8>((x & keep) ^ flip);
-      }
+      atomicMax(&s_all[r / (16 * MR)][0], lo);
+      atomicMin(&s_all[r / (16 * MR)][1], hi);
     }
-#pragma unroll
-    for (int o = 1; o < 16; o *= 2) {
-      span_lo = min(span_lo, __shfl_xor(span_lo, o));
-      span_hi = max(span_hi, __shfl_xor(span_hi, o));
-      all_lo = max(all_lo, __shfl_xor(all_lo, o));
-      all_hi = min(all_hi, __shfl_xor(all_hi, o));
-    }
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    lds_barrier();
+    const int span_lo = __builtin_amdgcn_readfirstlane(s_span[0]), span_hi = __builtin_amdgcn_readfirstlane(s_span[1]);
+    const int all_lo = __builtin_amdgcn_readfirstlane(s_all[wave][0]);
+    const int all_hi = __builtin_amdgcn_readfirstlane(s_all[wave][1]);
     const bool active = wave * 16 * MR < n_rows;
-    __syncthreads();
-    if (lane == 0) {
-      atomicMin(&s_span[0], span_lo);
-      atomicMax(&s_span[1], span_hi);
-    }
-    __syncthreads();
-    span_lo = __builtin_amdgcn_readfirstlane(s_span[0]);
-    span_hi = __builtin_amdgcn_readfirstlane(s_span[1]);
+    V8 qf[MR][KS];
+    auto load_q = [&]() {
+      u32x4 x[MR][KS];
+#pragma unroll
+      for (int rt = 0; rt < MR; ++rt) {
+        const int r = wave * 16 * MR + rt * 16 + li;
+        const bool live = r < n_rows;
+        const unsigned vr = block * R + (live ? r : 0), i = prefix_div(vr, p.rows, p.rows_magic);
+        const unsigned rr = vr - i * p.rows, s = prefix_div(rr, p.group, p.group_magic);
+        const int64_t row = ((int64_t)(first + i) * p.s1 + s) * p.n1 + head * p.group + (rr - s * p.group);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          x[rt][ks] = live ? *(const u32x4*)((const T*)p.q + row * D + ks * 32 + lg * 8) : u32x4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int rt = 0; rt < MR; ++rt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = as_v8<V8>((x[rt][ks] & keep) ^ flip);
+    };
     const int tok1 = min(min((part + 1) * per * TILE, jb.f.tokens), span_hi);
     const int tok0 = max(part * per * TILE, span_lo / TILE * TILE);
 
@@ -172,10 +167,6 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
       const int npg = (int)paged_split(p, (unsigned)tb - 1u, &off0) - pg0 + 1;
       lds_barrier();  // the entries and tiles before are read
       for (int i = tid; i < npg; i += NT) s_tab[i] = tab[pg0 + i];
-#pragma unroll
-      for (int rt = 0; rt < MR; ++rt)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[rt][ks]));  // (Q's loads end here)
       lds_barrier();
       const int n_tiles = (tb - ta + TILE - 1) / TILE;
 
@@ -188,28 +179,24 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
         const int64_t r = (int64_t)blk * p.page + (int)off;
         return blk < 0 || r >= p.kv_rows ? -1 : (int)r;
       };
-      int rows = -1;  // lane e: first cache row of DMA e % NI of stage f0 + e / NI
       // the f-th stage's tokens into the ring at `at`
+      int rows = -1;  // lane e: first cache row of DMA e % NI of stage f0 + e / NI
       auto fetch = [&](int f, int at) {
         const int tok = ta + f * FETCH;
         const unsigned dst = smem_base + at + wave * 1024;
-        if (one_page && (tok >= span_lo || tok >= tb)) {
-          if (f % kStages == 0 || tok - FETCH < span_lo)
-            rows = row_of(ta + (f - f % kStages + lane / NI) * FETCH + ((lane % NI) * NW + wave) * TPI);
+        if (FAST && f % kStages == 0) rows = row_of(tok + lane / NI * FETCH + ((lane % NI) * NW + wave) * TPI);
 #pragma unroll
-          for (int j = 0; j < NI; ++j) {
+        for (int j = 0; j < NI; ++j) {
+          if constexpr (FAST) {
+            // (a row of -1: no bytes)
             const int r = __builtin_amdgcn_readlane(rows, (f % kStages) * NI + j);
-            const int here = tok + (j * NW + wave) * TPI;
-            const int bytes = r < 0 ? 0 : min(tb - here, TPI) * (int)row_bytes;
-            const int64_t from = (int64_t)(r < 0 ? 0 : r) * row_bytes;
+            const int bytes = min(tb - tok - (j * NW + wave) * TPI, TPI) * (int)row_bytes & ~(r >> 31);
+            const int64_t from = (int64_t)max(r, 0) * row_bytes;
             dma_buf16(dst + j * NW * 1024, k_from[j],
                       __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + from), (short)0, bytes, 0x00020000));
             dma_buf16(dst + j * NW * 1024 + K_BYTES, v_from[j],
                       __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + from), (short)0, bytes, 0x00020000));
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < NI; ++j) {
+          } else {
             const int tk = (j * NW + wave) * TPI + lane / CPT;
             const int r = row_of(tok + tk);
             const int kc = ((lane % CPT) ^ swz_k(tk)) * 16, vc = ((lane % CPT) ^ swz_v(tk)) * 16;
@@ -344,11 +331,18 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
         }
       };
 
-      // the first tiles (those past the end, here and below, read zeros, so
-      // that the number of DMAs in flight is known)
+      // the first stage comes beside Q, whose loads end here, the others behind
+      // (those past the end, here and below, read zeros, so that the number of
+      // DMAs in flight is known)
+      fetch(0, 0);
+      if (ta == tok0) load_q();
+      wait_vmcnt<0>();
+#pragma unroll
+      for (int rt = 0; rt < MR; ++rt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[rt][ks]));
 #pragma unroll 1
-      for (int f = 0; f < NB - 1; ++f) fetch(f, f * STAGE);
-      wait_vmcnt<(NB - 2) * 2 * NI>();
+      for (int f = 1; f < NB - 1; ++f) fetch(f, f * STAGE);
       lds_barrier();
       // step t: scores of tile t + 1 (of no visible token after the last) with the
       // second half of the softmax of tile t, then the output of tile t with the
@@ -396,20 +390,20 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
           int next = next_stage(at);
           asm volatile("" : "+s"(next));  // (so that each stage's offsets fit the instructions)
           if constexpr (SUB == 2) {
-            step(t, at, at + TILE * ROW, next, s0, s1, p0, p1);
+            const int here = at;
+            step(t, here, here + TILE * ROW, next, s0, s1, p0, p1);
             at = next;  // (of tile t + 2)
             if (++t >= n_tiles) break;
-            const int here = next == 0 ? (NB - 1) * STAGE : next - STAGE;
             step(t, here + TILE * ROW, next, next + TILE * ROW, s1, s0, p1, p0);
             if (++t >= n_tiles) break;
           } else {
-            int then = next_stage(next);
-            asm volatile("" : "+s"(then));
             first_k(next);
             step(t, at, next, next, s0, s1, p0, p1);
             at = next;
             if (++t >= n_tiles) break;
             open_stage(t);
+            int then = next_stage(next);
+            asm volatile("" : "+s"(then));
             first_k(then);
             step(t, at, then, then, s1, s0, p1, p0);
             at = then;
@@ -440,7 +434,6 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
       if (lg == 0) p.part_ml[slot0 + r] = {ref[rt], l, t, accn[rt][0]};
     }
     job = prefix_job_of(blockIdx.x, gridDim.x, ++round, p.n2, &head);
-    if (job < plan.jobs) jb = plan.next(p, lane, job);
   }
 }
 
@@ -493,11 +486,18 @@ size_t paged_prefix_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64
   return prefix_part_rows(s, batch, n2) * (sizeof(f32x4) + d * sizeof(float)) + (size_t)batch * sizeof(i32x4);
 }
 
-template <typename T>
+template <typename T, bool FAST>
 static void prefix_grouped_d(const PagedPrefixParams& p, int64_t d, unsigned grid, hipStream_t stream) {
-  if (d == 64) prefix_grouped_kernel<T, 64, 8, 2><<<grid, 512, 0, stream>>>(p);
-  else if (d == 128) prefix_grouped_kernel<T, 128, 8, 2><<<grid, 512, 0, stream>>>(p);
-  else prefix_grouped_kernel<T, 256, 4, 2><<<grid, 256, 0, stream>>>(p);
+  if (d == 64) prefix_grouped_kernel<T, 64, 8, 2, FAST><<<grid, 512, 0, stream>>>(p);
+  else if (d == 128) prefix_grouped_kernel<T, 128, 8, 2, FAST><<<grid, 512, 0, stream>>>(p);
+  else prefix_grouped_kernel<T, 256, 4, 2, FAST><<<grid, 256, 0, stream>>>(p);
+}
+
+static void prefix_grouped_launch(const PagedPrefixParams& p, int64_t d, int32_t dtype, unsigned grid, hipStream_t stream) {
+  const int tokens = (int)(512 / d);  // of a DMA
+  const bool fast = p.page % tokens == 0 && (int64_t)p.n2 * d * 2 * tokens < (1ll << 31) && p.band_pre >= (1ll << 31);
+  if (dtype == DSA_DTYPE_BF16) fast ? prefix_grouped_d<bf16, true>(p, d, grid, stream) : prefix_grouped_d<bf16, false>(p, d, grid, stream);
+  else fast ? prefix_grouped_d<f16, true>(p, d, grid, stream) : prefix_grouped_d<f16, false>(p, d, grid, stream);
 }
 
 int paged_prefix_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
@@ -521,6 +521,8 @@ int paged_prefix_run(const void* query, const void* query_rope, const void* key,
   p.shared = shared;
   p.prefix_workers = s.workers;
   p.job_rows = s.rows;
+  p.rows_magic = 0xffffffffu / (unsigned)p.rows;
+  p.group_magic = 0xffffffffu / (unsigned)p.group;
   const int64_t most = (s.jobs * n2 + 7) / 8 * 8;
   const unsigned grid = (unsigned)(most < s.grid ? most : s.grid);
   int st;
@@ -529,8 +531,7 @@ int paged_prefix_run(const void* query, const void* query_rope, const void* key,
     if (st != DSA_OK) return st;
     st = paged_latent_launch(p, d, dtype, stream);
   } else {
-    if (dtype == DSA_DTYPE_BF16) prefix_grouped_d<bf16>(p, d, grid, stream);
-    else prefix_grouped_d<f16>(p, d, grid, stream);
+    prefix_grouped_launch(p, d, dtype, grid, stream);
     DSA_HIP(hipGetLastError());
     st = paged_grouped_launch(p, d, dtype, stream);
   }

@@ -55,10 +55,12 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool rope_wave = wave < 4;
 
+  PrefixLengths lengths;
+  lengths.load(p, lane);
   PrefixPlan<HG> plan;
   int head;
   int job = prefix_job_of(blockIdx.x, gridDim.x, 0, 1, &head);
-  typename PrefixPlan<HG>::Job jb = plan.make(p, lane, job);
+  plan.make(p, lane);
 
   // scores in log2 units are s * scale - ref, one operation each; for that
   // the scale is positive: Q takes its sign, and is zero where it is
@@ -91,6 +93,7 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
   using Off = std::integral_constant<bool, false>;
 
   for (int round = 0; job < plan.jobs;) {
+    const typename PrefixPlan<HG>::Job jb = plan.find(p, fresh_lane(), job);
     const int ln = fresh_lane(), li = ln & 15, lg = ln >> 4, tid = wave * 64 + ln;
     int all_lo, all_hi, tok0, tok1;
     const int part = (job - jb.job0) / jb.blocks, block = (job - jb.job0) - part * jb.blocks;
@@ -100,17 +103,16 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
       if (job == jb.job0)
         for (int i = tid; i < jb.f.count; i += kPxThreads) p.where[first + i] = i32x4{jb.job0, jb.blocks, jb.parts, i};
       // what the rows see of the prefix, and what any and all of the block's do
-      __syncthreads();  // (the job before has read what it left)
+      lds_barrier();  // (the job before has read what it left)
       if (tid == 0) s_span[0] = 0x7fffffff, s_span[1] = 0;
-      __syncthreads();
+      lds_barrier();
       const int r = wave * 16 + li;
       const bool live = r < n_rows;
-      const int vr = block * HG + (live ? r : 0), i = vr / p.rows, s = (vr - i * p.rows) / p.n1;
-      const int act_k = min(max(p.act_k[first + i], 0), p.max_blocks * p.page);
-      const int act_q = p.act_q ? min(max(p.act_q[first + i], 0), p.s1) : p.s1;
+      const unsigned vr = block * HG + (live ? r : 0), i = prefix_div(vr, p.rows, p.rows_magic);
+      const int s = prefix_div(vr - i * p.rows, p.group, p.group_magic);
       int lo, hi;
-      paged_bounds(p, act_q, act_k, s, &lo, &hi);
-      hi = live ? min(hi, jb.f.tokens) : 0;
+      lengths.bounds(p, first + i, s, jb.f.tokens, &lo, &hi);
+      hi = live ? hi : 0;
       if (lg == 0) s_lo[r] = lo, s_hi[r] = hi;
       if (lg == 0 && hi > lo) {
         atomicMin(&s_span[0], lo);
@@ -125,7 +127,7 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
       }
       all_lo = __builtin_amdgcn_readfirstlane(all_lo);
       all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-      __syncthreads();
+      lds_barrier();
       const int per = ((jb.f.tokens + TILE - 1) / TILE + jb.parts - 1) / jb.parts * TILE;
       tok0 = max(part * per, __builtin_amdgcn_readfirstlane(s_span[0]));
       tok1 = min(min((part + 1) * per, jb.f.tokens), __builtin_amdgcn_readfirstlane(s_span[1]));
@@ -135,7 +137,6 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
         for (int c = tid; c < rows_here * (D / 4); c += kPxThreads)
           *((f32x4*)(p.part_o + slot0 * D) + c) = f32x4{0.f, 0.f, 0.f, 0.f};
         job = prefix_job_of(blockIdx.x, gridDim.x, ++round, 1, &head);
-        if (job < plan.jobs) jb = plan.next(p, lane, job);
         continue;
       }
     }
@@ -488,7 +489,6 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
     put(0.f, p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht]; });
     }(fresh_lane());
     job = prefix_job_of(blockIdx.x, gridDim.x, ++round, 1, &head);
-    if (job < plan.jobs) jb = plan.next(p, fresh_lane(), job);
   }
 }
 
