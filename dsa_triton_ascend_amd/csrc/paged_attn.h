@@ -55,16 +55,28 @@ struct PagedAttnParams {
 };
 
 // With a prefix that sequences share (paged_prefix.h): these kernels take what
-// is behind it, and the join takes its parts too.
+// is behind it, plan the work on the prefixes meanwhile, and the join takes
+// both's parts.
+struct PagedWhere {  // of a sequence, for the join
+  int job0, blocks, parts, place;  // first job of its family, blocks of rows, parts (0: no family), its place there
+  int run0, runs, slot0, unused;   // its runs and the slot of the first
+};
+struct PagedJob {  // rows of a family, and tokens tok0 .. tok1 of its prefix
+  int first, row0, rows, unused;   // first sequence; rows from row0 on, of the family
+  int tok0, tok1;
+  int all_lo, all_hi;              // tokens that all rows of the family see
+};
 struct PagedPrefixParams : PagedAttnParams {
   const int32_t *ids, *shared;  // per sequence: its family and the tokens that it shares
-  i32x4* where;                 // per sequence: first job of its family, blocks of rows, parts, place in the family
+  PagedWhere* where;
+  PagedJob* job;
+  int* n_jobs;
   // rows of part_o / part_ml: behind those of the runs come, for each sequence,
   // one for what a run has of it if that is all of it, then those of the jobs
   int64_t whole0, part0;
   int prefix_workers;           // jobs of one key head aimed at
-  int job_rows;                 // rows of a block
-  unsigned rows_magic, group_magic;  // floor((2^32 - 1) / rows), of group
+  int job_shift;                // log2 of the rows of a block
+  unsigned rows_magic, group_magic, heads_magic;  // floor((2^32 - 1) / rows), of group, of n2
 };
 
 template <typename P> constexpr bool kPrefixed = std::is_same<P, PagedPrefixParams>::value;

@@ -24,7 +24,7 @@
 //
 // P is multiplied as a sum of two values of the input type (the MFMAs are
 // idle otherwise), so the weights keep 16 bits and more.
-#include "paged_attn.h"
+#include "paged_prefix.h"
 
 namespace dsa {
 
@@ -52,6 +52,13 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
   constexpr int EPL = D / 16;  // V columns of a lane
   const int lane = threadIdx.x & 63;
   const int li = lane & 15, lg = lane >> 4;
+  if constexpr (kPrefixed<P>) {
+    // the last workgroup plans the work on the prefixes
+    if (blockIdx.x == gridDim.x - 1) {
+      if (threadIdx.x < 64) prefix_plan(p, kPaTile, lane);
+      return;
+    }
+  }
   const int64_t wid = (int64_t)blockIdx.x * (kPaThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int worker = (int)(wid / p.groups), ng = (int)(wid - (int64_t)worker * p.groups);
   if (worker >= p.workers) return;
@@ -302,20 +309,23 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(P p, int tile, int w
   const int per_seq = p.n2 * p.rows, groups = (per_seq + wg_rows - 1) / wg_rows;
   const int b = blockIdx.x / groups, row0 = (blockIdx.x - b * groups) * wg_rows;
 
-  PagedPlan<P> plan;
-  plan.make(p, tile, lane);
-  const PagedSeqOf<P> seq = plan.sequence(p, b);
-  const int nt = paged_tiles(seq, tile);
-  const int first = plan.start(p, tile, lane, b), last = first + nt - 1;
-  const int w0 = nt ? plan.worker_of(first) : 0;
-  const int own = nt ? plan.worker_of(last) - w0 + 1 : 0;
-  int runs = own;
-  i32x4 where = {0, 0, 0, 0};
-  if constexpr (kPrefixed<P>) {  // behind the runs: the parts of the prefix
-    if (seq.shared) where = p.where[b], runs += where[2];
+  int w0, own, slot0;
+  PagedWhere where;
+  if constexpr (kPrefixed<P>) {
+    where = p.where[b];
+    w0 = where.run0, own = where.runs, slot0 = where.slot0;
+  } else {
+    PagedPlan<P> plan;
+    plan.make(p, tile, lane);
+    const int nt = paged_tiles(plan.sequence(p, b), tile);
+    const int first = plan.start(p, tile, lane, b), last = first + nt - 1;
+    w0 = nt ? plan.worker_of(first) : 0;
+    own = nt ? plan.worker_of(last) - w0 + 1 : 0;
+    slot0 = first != w0 * plan.per ? 1 : 0;  // of the first worker; the others' is 0
   }
-  if (runs == 1 && !paged_behind(seq)) return;  // written whole by its worker
-  const int slot0 = first != w0 * plan.per ? 1 : 0;  // of the first worker; the others' is 0
+  const bool behind = kPrefixed<P> && where.parts;
+  const int runs = behind ? own + where.parts : own;  // behind the runs: the parts of the prefix
+  if (runs == 1 && !behind) return;  // written whole by its worker
 
   // the runs i0 .. i1 of a row, summed relative to the largest reference of all
   auto row_of = [&](int row, int i0, int i1, float* big, float* top, FV* o, float* l, float* n) {
@@ -325,15 +335,15 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(P p, int tile, int w
     const int64_t span = (int64_t)p.groups * p.group_rows;
     int block = 0, in_block = 0;
     if constexpr (kPrefixed<P>) {
-      const int64_t r = (int64_t)where[3] * p.rows + rr;  // among the family's
-      block = where[0] + (int)(r / p.job_rows), in_block = (int)(r % p.job_rows);
+      const int r = where.place * p.rows + rr;  // among the family's
+      block = where.job0 + (r >> p.job_shift), in_block = r & ((1 << p.job_shift) - 1);
     }
     auto slot = [&](int i) {
       const int64_t s = ((int64_t)(w0 + i) * 2 + (i == 0 ? slot0 : 0)) * span + in_group;
       if constexpr (kPrefixed<P>) {
-        const int64_t job = block + (int64_t)(i - own) * where[1];
+        const int64_t job = block + (int64_t)(i - own) * where.blocks;
         if (own == 1 && i == 0) return paged_whole_slot(p, b, kvh * p.row_groups + rg) + (rr - rg * p.group_rows);
-        return i < own ? s : p.part0 + (job * p.n2 + kvh) * p.job_rows + in_block;
+        return i < own ? s : p.part0 + ((job * p.n2 + kvh) << p.job_shift) + in_block;
       }
       return s;
     };
@@ -542,7 +552,7 @@ static void paged_launch(const P& p, int64_t d, bool streaming, unsigned grid, h
 
 template <typename P>
 static int paged_grouped(const P& p, int64_t d, int32_t dtype, hipStream_t stream) {
-  const unsigned grid = (unsigned)paged_grouped_grid(p.workers, p.groups);
+  const unsigned grid = (unsigned)paged_grouped_grid(p.workers, p.groups) + (kPrefixed<P> ? 1 : 0);
   // K and V that the caches could hold until the next call are kept there
   // (134 MB: 38 us, streaming 41; 537 MB: 115 us, streaming 104)
   const int64_t all = (int64_t)p.batch * p.max_blocks * p.page;

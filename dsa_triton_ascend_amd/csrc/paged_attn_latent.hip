@@ -45,7 +45,7 @@
 // 2-norms, with P as two values and rounded: bf16 1.66e-3 and 1.73e-3 over 32K
 // tokens, 1.66e-3 and 1.90e-3 over 60 to 1000, 1.66e-3 and 1.70e-3 over two;
 // fp16 2.07e-4 and 2.17e-4, 2.38e-4, 2.13e-4.
-#include "paged_attn.h"
+#include "paged_prefix.h"
 #include "sfa_fwd.h"
 
 namespace dsa {
@@ -123,6 +123,13 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(P p) {
   const int lw = wave - (NW - NL);  // among the fetching waves
   const bool rope_wave = lw >= 0 && lw < 4;
 
+  if constexpr (kPrefixed<P>) {
+    // the last workgroup plans the work on the prefixes
+    if (blockIdx.x == gridDim.x - 1) {
+      if (wave == 0) prefix_plan(p, TILE, lane);
+      return;
+    }
+  }
   // the row groups of a worker read the same tokens: they share an XCD
   const int jj = blockIdx.x >> 3;
   const int rg = jj % p.row_groups;
@@ -644,7 +651,7 @@ bool paged_latent_launchable(int64_t workers, int64_t row_groups) {
 
 template <typename P>
 static int paged_latent(const P& p, int64_t d, int32_t dtype, hipStream_t stream) {
-  const unsigned grid = (unsigned)paged_latent_grid(p.workers, p.row_groups);
+  const unsigned grid = (unsigned)paged_latent_grid(p.workers, p.row_groups) + (kPrefixed<P> ? 1 : 0);
   if (dtype == DSA_DTYPE_BF16) paged_latent_d<bf16>(p, d, grid, stream);
   else paged_latent_d<f16>(p, d, grid, stream);
   DSA_HIP(hipGetLastError());

@@ -9,12 +9,14 @@
 // paged_attn.h.  paged_combine_kernel joins both: every part of a row comes as
 // a reference, a sum and an unnormalised output, as the runs there.
 //
-// Work.  A job is up to R rows of a family (over its sequences, new tokens and
-// the query heads of one key head) and a part of its prefix.  Parts are as long
-// as gives as many jobs as there are workgroups, whatever the families' sizes
-// and lengths; the jobs of the same part, for other rows and key heads, run
-// next to each other on one XCD, whose L2 they share.  All of it is found on
-// the device from the ids and lengths, by every wave for itself.
+// Work.  A job is a block of up to R rows of a family (over its sequences, new
+// tokens and the query heads of one key head) and a part of its prefix.  Parts
+// are as long as gives as many jobs as there are workgroups, whatever the
+// families' sizes and lengths; the jobs of the same part, for other rows and key
+// heads, run next to each other on one XCD, whose L2 they share.  All of it is
+// found on the device from the ids and lengths, by one wave beside the kernel of
+// paged_attn.h, which runs first: found by every workgroup for itself it took
+// 8 us of each (most of it instructions that had to be fetched first).
 #pragma once
 
 #include "paged_attn.h"
@@ -65,49 +67,31 @@ __device__ __forceinline__ PrefixFamily prefix_families(const PagedPrefixParams&
   return f;
 }
 
-// New and cached tokens of the sequences of a family's rows.  Lane l keeps
-// those of sequence l, so that up to 64 sequences are read once, beside the
-// families, and not behind them.
-struct PrefixLengths {
-  int act_q, act_k;
-  __device__ __forceinline__ void load(const PagedPrefixParams& p, int lane) {
-    const int b = min(lane, p.batch - 1);
-    act_k = p.act_k[b];
-    act_q = p.act_q ? p.act_q[b] : p.s1;
-  }
-  // the tokens of the family's prefix that new token s of sequence b sees
-  __device__ __forceinline__ void bounds(const PagedPrefixParams& p, int b, int s, int tokens, int* lo, int* hi) const {
-    int k, q;
-    if (p.batch <= 64) {
-      k = __shfl(act_k, b);
-      q = __shfl(act_q, b);
-    } else {
-      k = p.act_k[b];
-      q = p.act_q ? p.act_q[b] : p.s1;
-    }
-    paged_bounds(p, min(max(q, 0), p.s1), min(max(k, 0), p.max_blocks * p.page), s, lo, hi);
-    *hi = min(*hi, tokens);
-  }
-};
+// n / d with magic = floor((2^32 - 1) / d): n * magic / 2^32 is at most
+// n / 2^32 below n / d, so its integer part is off by one at most
+__device__ __forceinline__ unsigned prefix_div(unsigned n, unsigned d, unsigned magic) {
+  const unsigned q = __umulhi(n, magic);
+  return q + (n - q * d >= d);
+}
 
-// Jobs of one key head for blocks of R rows.
-template <int R>
+__device__ __forceinline__ int prefix_div_up(int a, int b) { return (int)((unsigned)(a + b - 1) / (unsigned)b); }
+
+__device__ __forceinline__ int wave_min_int(int v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = min(v, __shfl_xor(v, o));
+  return v;
+}
+
+// The jobs of one key head, where the join finds a sequence's parts.  One wave.
 struct PrefixPlan {
-  int per;           // tiles of a part, at most
-  int jobs;          // in all
-  PrefixFamily f;    // of this lane among the first 64 sequences,
-  int m, t;          // its blocks of rows and tiles
-
-  struct Job {
-    PrefixFamily f;
-    int job0, blocks, parts;  // of the family: its first job, blocks of rows, parts of its prefix
-  };
-
-  static __device__ __forceinline__ int div_up(int a, int b) { return (int)((unsigned)(a + b - 1) / (unsigned)b); }
+  int per;         // tiles of a part, at most
+  int jobs;        // in all
+  PrefixFamily f;  // of this lane among 64 sequences,
+  int m, t;        // its blocks of rows and tiles
 
   __device__ __forceinline__ void families(const PagedPrefixParams& p, int c0, int lane) {
     f = prefix_families(p, c0, lane);
-    m = f.count ? (int)(((int64_t)f.count * p.rows + R - 1) / R) : 0;
+    m = (int)(((int64_t)f.count * p.rows + (1 << p.job_shift) - 1) >> p.job_shift);
     t = (f.tokens + kPrefixTile - 1) / kPrefixTile;
   }
 
@@ -119,9 +103,9 @@ struct PrefixPlan {
     families(p, 0, lane);
     if (p.batch <= 64) {
       const int work = wave_total(m * t), most = prefix_jobs(wave_total(m), p.prefix_workers);
-      per = max(div_up(work, most), kPrefixMinTiles);
+      per = max(prefix_div_up(work, most), kPrefixMinTiles);
       for (;;) {
-        jobs = wave_total(m * div_up(t, per));
+        jobs = wave_total(m * prefix_div_up(t, per));
         if (jobs <= most) return;
         per += max(per >> 4, 1);
       }
@@ -136,57 +120,133 @@ struct PrefixPlan {
     rows = wave_total(rows);
     const int most = prefix_jobs(rows, p.prefix_workers);
     for (int room = 0;; room = rows) {
-      per = max(div_up(work, most - room), kPrefixMinTiles);
+      per = max(prefix_div_up(work, most - room), kPrefixMinTiles);
       int n = 0;
       for (int c0 = 0; c0 < p.batch; c0 += 64) {
         families(p, c0, lane);
-        n += m * div_up(t, per);
+        n += m * prefix_div_up(t, per);
       }
       jobs = wave_total(n);
       if (jobs <= most) return;
     }
   }
 
-  // job number `job` (below `jobs`)
-  __device__ __forceinline__ Job find(const PagedPrefixParams& p, int lane, int job) {
-    Job j = {{0, 0, 0}, 0, 1, 1};
-    int base = 0;
+  // Writes the jobs, and for every sequence where its parts are; `runs` is the
+  // plan of what is behind the prefixes.
+  __device__ __forceinline__ void write(const PagedPrefixParams& p, const PagedPlan<PagedPrefixParams>& runs, int tile,
+                                        int lane) {
+    if (lane == 0) *p.n_jobs = jobs;
+    int job_base = 0, run_base = 0;
     for (int c0 = 0; c0 < p.batch; c0 += 64) {
       if (p.batch > 64) families(p, c0, lane);
-      const int parts = div_up(t, per), n = m * parts;
-      const int incl = wave_scan(n);
-      const unsigned long long hit = __ballot(base + incl > job);
-      if (hit) {
-        const int l = __ffsll(hit) - 1;
-        j.f.first = __builtin_amdgcn_readlane(f.first, l);
-        j.f.count = __builtin_amdgcn_readlane(f.count, l);
-        j.f.tokens = __builtin_amdgcn_readlane(f.tokens, l);
-        j.job0 = base + __builtin_amdgcn_readlane(incl - n, l);
-        j.blocks = __builtin_amdgcn_readlane(m, l);
-        j.parts = __builtin_amdgcn_readlane(parts, l);
-        break;
+      // the sequences' runs
+      const int b = c0 + lane;
+      PagedSeqBehind seq = {};
+      int nt = 0, padded = 0;
+      if (b < p.batch) {
+        seq = paged_seq(p, b);
+        nt = paged_tiles(seq, tile);
+        padded = runs.padded(nt);
       }
-      base += __builtin_amdgcn_readlane(incl, 63);
+      const int upto = wave_scan(padded);
+      PagedWhere w = {};
+      if (nt) {
+        const int first = run_base + upto - padded;
+        w.run0 = runs.worker_of(first);
+        w.runs = runs.worker_of(first + nt - 1) - w.run0 + 1;
+        w.slot0 = first != w.run0 * runs.per;
+      }
+      if (b < p.batch) {  // (of a family's sequences the first half comes with the family)
+        int* at = (int*)(p.where + b);
+        at[4] = w.run0, at[5] = w.runs, at[6] = w.slot0;
+        if (!seq.shared) at[0] = at[1] = at[2] = at[3] = 0;
+      }
+      run_base += __builtin_amdgcn_readlane(upto, 63);
+      // what the rows of a sequence see: they rise with its new token
+      int lo0, hi0, lo1, hi1;
+      paged_bounds(p, seq.act_q, seq.act_k, 0, &lo0, &hi0);
+      paged_bounds(p, seq.act_q, seq.act_k, max(p.s1 - 1, 0), &lo1, &hi1);
+      int seen_lo = 0x7fffffff, seen_hi = 0;  // any of its rows
+      if (seq.act_q > 0) {
+        seen_lo = lo0;
+        int l;
+        paged_bounds(p, seq.act_q, seq.act_k, seq.act_q - 1, &l, &seen_hi);
+      }
+      const int all_lo = lo1, all_hi = seq.act_q == p.s1 ? hi0 : 0;
+      // the families that start here
+      const int parts = prefix_div_up(t, per), n = m * parts, incl = wave_scan(n);
+      for (unsigned long long todo = __ballot(n > 0); todo; todo &= todo - 1) {
+        const int l = __ffsll(todo) - 1;
+        const int first = __builtin_amdgcn_readlane(f.first, l), count = __builtin_amdgcn_readlane(f.count, l);
+        const int tokens = __builtin_amdgcn_readlane(f.tokens, l), blocks = __builtin_amdgcn_readlane(m, l);
+        const int np = __builtin_amdgcn_readlane(parts, l), nj = __builtin_amdgcn_readlane(n, l);
+        const int job0 = job_base + __builtin_amdgcn_readlane(incl, l) - nj;
+        const bool in = lane >= l && lane < l + count;
+        int lo = in ? seen_lo : 0x7fffffff, hi = in ? seen_hi : 0, alo = in ? all_lo : 0, ahi = in ? all_hi : 0x7fffffff;
+        for (int e = c0 + 64 + lane; e < first + count; e += 64) {  // (sequences of the next 64s)
+          const PagedSeqBehind s = paged_seq(p, e);
+          int l0, h0, l1, h1;
+          paged_bounds(p, s.act_q, s.act_k, 0, &l0, &h0);
+          paged_bounds(p, s.act_q, s.act_k, max(s.act_q - 1, 0), &l1, &h1);
+          if (s.act_q > 0) lo = min(lo, l0), hi = max(hi, h1);
+          alo = max(alo, l1);  // (a row behind the last new token sees nothing: all_hi is 0 then)
+          ahi = min(ahi, s.act_q == p.s1 ? h0 : 0);
+        }
+        lo = wave_min_int(lo);
+        hi = min(-wave_min_int(-hi), tokens);
+        alo = -wave_min_int(-alo);
+        ahi = wave_min_int(ahi);
+        // parts of equal numbers of whole tiles, cut to what is seen
+        const int each = prefix_div_up((tokens + kPrefixTile - 1) / kPrefixTile, np) * kPrefixTile;
+        for (int j = lane; j < nj; j += 64) {
+          const int part = (int)((unsigned)j / (unsigned)blocks), block = j - part * blocks;
+          PagedJob q;
+          q.first = first;
+          q.row0 = block << p.job_shift;
+          q.rows = min(count * p.rows - q.row0, 1 << p.job_shift);
+          q.unused = 0;
+          q.tok0 = max(part * each, lo);
+          q.tok1 = min(part * each + each, hi);
+          q.all_lo = alo;
+          q.all_hi = ahi;
+          p.job[job0 + j] = q;
+        }
+        for (int i = lane; i < count; i += 64) {
+          int* at = (int*)(p.where + first + i);
+          at[0] = job0, at[1] = blocks, at[2] = np, at[3] = i;
+        }
+      }
+      job_base += __builtin_amdgcn_readlane(incl, 63);
     }
-    return j;
   }
 };
 
-// n / d with magic = floor((2^32 - 1) / d): n * magic / 2^32 is at most
-// n / 2^32 below n / d, so its integer part is off by one at most
-__device__ __forceinline__ unsigned prefix_div(unsigned n, unsigned d, unsigned magic) {
-  const unsigned q = __umulhi(n, magic);
-  return q + (n - q * d >= d);
+// A wave beside the runs plans the prefixes.
+__device__ __forceinline__ void prefix_plan(const PagedPrefixParams& p, int tile, int lane) {
+  PagedPlan<PagedPrefixParams> runs;
+  runs.make(p, tile, lane);
+  PrefixPlan plan;
+  plan.make(p, lane);
+  plan.write(p, runs, tile, lane);
 }
 
-// Which job, of which key head, workgroup `block` of `grid` has in round `round`
-// (-1: none): the jobs lie end to end over the XCDs (workgroup x runs on XCD
-// x % 8), key head by key head.
-__device__ __forceinline__ int prefix_job_of(int block, int grid, int round, int heads, int* head) {
+// Which job, of which key head, workgroup `block` of `grid` has in round `round`:
+// the jobs lie end to end over the XCDs (workgroup x runs on XCD x % 8), key
+// heads next to each other.
+__device__ __forceinline__ int prefix_job_of(const PagedPrefixParams& p, int block, int grid, int round, int* head) {
   const int at = round * grid + (block & 7) * (grid >> 3) + (block >> 3);
-  const int job = at / heads;
-  *head = at - job * heads;
+  const int job = p.n2 == 1 ? at : (int)prefix_div(at, p.n2, p.heads_magic);
+  *head = at - job * p.n2;
   return job;
+}
+
+// The tokens that row `row` of a job sees of the prefix.
+__device__ __forceinline__ void prefix_bounds(const PagedPrefixParams& p, const PagedJob& j, int row, int* lo, int* hi) {
+  const unsigned vr = j.row0 + row, i = prefix_div(vr, p.rows, p.rows_magic);
+  const int s = (int)prefix_div(vr - i * p.rows, p.group, p.group_magic), b = j.first + (int)i;
+  const int act_k = min(max(p.act_k[b], 0), p.max_blocks * p.page);
+  paged_bounds(p, p.act_q ? min(max(p.act_q[b], 0), p.s1) : p.s1, act_k, s, lo, hi);
+  *hi = min(*hi, j.tok1);
 }
 
 // kernels of the two forms (paged_prefix.hip, paged_prefix_latent.hip)

@@ -37,8 +37,8 @@ constexpr int kPrefixPages = 1024;  // block-table entries held in LDS
 template <int D> constexpr int kPrefixSub = D == 256 ? 1 : 2;
 template <int D> constexpr int kPrefixRing = D == 64 ? 6 : 4;
 
-// FAST: no DMA lies in two pages, none of its rows' offsets needs more than 32
-// bits, and there is no band whose lower end could lie inside a tile.
+// FAST: no DMA lies in two pages (jobs start at whole tiles: there is no band),
+// and none of its rows' offsets needs more than 32 bits.
 template <typename T, int D, int NW, int MR, bool FAST>
 __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixParams p) {
   using E = Elem<T>;
@@ -58,7 +58,6 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
   __shared__ __attribute__((aligned(16))) unsigned char smem[NB * STAGE];
   __shared__ int s_tab[kPrefixPages];
   __shared__ int s_lo[R], s_hi[R];  // tokens that the rows see
-  __shared__ int s_span[2], s_all[NW][2];  // tokens that any row sees, and that all rows of a wave do
 
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -84,43 +83,17 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = E::from_f32(1.f);
 
-  PrefixLengths lengths;
-  lengths.load(p, lane);
-  PrefixPlan<R> plan;
   int head;
-  int job = prefix_job_of(blockIdx.x, gridDim.x, 0, p.n2, &head);
-  plan.make(p, lane);
-  for (int round = 0; job < plan.jobs;) {
-    const typename PrefixPlan<R>::Job jb = plan.find(p, lane, job);
-    const int part = (job - jb.job0) / jb.blocks, block = (job - jb.job0) - part * jb.blocks;
-    const int all_tiles = (jb.f.tokens + TILE - 1) / TILE, per = (all_tiles + jb.parts - 1) / jb.parts;
-    const int first = jb.f.first, n_rows = min(jb.f.count * p.rows - block * R, R);
-    if (job == jb.job0 && head == 0)
-      for (int i = tid; i < jb.f.count; i += NT) p.where[first + i] = i32x4{jb.job0, jb.blocks, jb.parts, i};
-
-    // the tokens that the rows see
-    lds_barrier();  // (the job before has read what it left)
-    if (tid < 2) s_span[tid] = tid ? 0 : 0x7fffffff;
-    if (tid < 2 * NW) s_all[tid >> 1][tid & 1] = tid & 1 ? 0x7fffffff : 0;
-    lds_barrier();
-    for (int r0 = wave * 64; r0 < n_rows; r0 += NT) {
-      const int r = min(r0 + lane, n_rows - 1);  // (all lanes go along: they have the lengths)
-      const unsigned vr = block * R + r, i = prefix_div(vr, p.rows, p.rows_magic);
-      const int s = prefix_div(vr - i * p.rows, p.group, p.group_magic);
-      int lo, hi;
-      lengths.bounds(p, first + i, s, jb.f.tokens, &lo, &hi);
-      s_lo[r] = lo, s_hi[r] = hi;
-      if (hi > lo) {
-        atomicMin(&s_span[0], lo);
-        atomicMax(&s_span[1], hi);
-      }
-      atomicMax(&s_all[r / (16 * MR)][0], lo);
-      atomicMin(&s_all[r / (16 * MR)][1], hi);
+  int job = prefix_job_of(p, blockIdx.x, gridDim.x, 0, &head);
+  const int jobs = *p.n_jobs;
+  for (int round = 0; job < jobs;) {
+    const PagedJob jb = p.job[job];
+    const int first = jb.first, n_rows = jb.rows, tok0 = jb.tok0, tok1 = jb.tok1;
+    const bool masked = tok0 < jb.all_lo || tok1 > jb.all_hi;
+    if (masked) {  // what the rows see, where it is not all of it
+      lds_barrier();  // (the job before has read what it left)
+      for (int r = tid; r < n_rows; r += NT) prefix_bounds(p, jb, r, s_lo + r, s_hi + r);
     }
-    lds_barrier();
-    const int span_lo = __builtin_amdgcn_readfirstlane(s_span[0]), span_hi = __builtin_amdgcn_readfirstlane(s_span[1]);
-    const int all_lo = __builtin_amdgcn_readfirstlane(s_all[wave][0]);
-    const int all_hi = __builtin_amdgcn_readfirstlane(s_all[wave][1]);
     const bool active = wave * 16 * MR < n_rows;
     V8 qf[MR][KS];
     auto load_q = [&]() {
@@ -129,7 +102,7 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
       for (int rt = 0; rt < MR; ++rt) {
         const int r = wave * 16 * MR + rt * 16 + li;
         const bool live = r < n_rows;
-        const unsigned vr = block * R + (live ? r : 0), i = prefix_div(vr, p.rows, p.rows_magic);
+        const unsigned vr = jb.row0 + (live ? r : 0), i = prefix_div(vr, p.rows, p.rows_magic);
         const unsigned rr = vr - i * p.rows, s = prefix_div(rr, p.group, p.group_magic);
         const int64_t row = ((int64_t)(first + i) * p.s1 + s) * p.n1 + head * p.group + (rr - s * p.group);
 #pragma unroll
@@ -141,9 +114,6 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = as_v8<V8>((x[rt][ks] & keep) ^ flip);
     };
-    const int tok1 = min(min((part + 1) * per * TILE, jb.f.tokens), span_hi);
-    const int tok0 = max(part * per * TILE, span_lo / TILE * TILE);
-
     f32x4 acc[ND][MR], accn[MR];
     float ref[MR], top[MR], sum[MR];
 #pragma unroll
@@ -172,7 +142,7 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
 
       // cache row of a token, -1 outside the span or without a page (read as zeros)
       auto row_of = [&](int tok) -> int {
-        if (tok >= tb || tok < span_lo) return -1;
+        if (tok >= tb) return -1;
         unsigned off;
         const unsigned pg = paged_split(p, (unsigned)tok, &off);
         const int blk = s_tab[(int)pg - pg0];
@@ -222,11 +192,12 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
       auto soft_a = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR], int t) {
         if (k == 0) {
           const int tk = ta + t * TILE;
-          if (tk < all_lo || tk + TILE > min(all_hi, tb)) {
+          if (masked || tk + TILE > tb) {
             const int mine = tk + lg * 4;
 #pragma unroll
             for (int rt = 0; rt < MR; ++rt) {
-              const int r = wave * 16 * MR + rt * 16 + li, lo = s_lo[r], hi = min(s_hi[r], tb);
+              const int r = min(wave * 16 * MR + rt * 16 + li, n_rows - 1);
+              const int lo = masked ? s_lo[r] : 0, hi = masked ? min(s_hi[r], tb) : tb;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const int tok = mine + (i >> 2) * 16 + (i & 3);
@@ -433,7 +404,7 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
       for (int j = 0; j < ND; ++j) *(f32x4*)(dst + j * 16) = paged_scaled(acc[j][rt], seen);
       if (lg == 0) p.part_ml[slot0 + r] = {ref[rt], l, t, accn[rt][0]};
     }
-    job = prefix_job_of(blockIdx.x, gridDim.x, ++round, p.n2, &head);
+    job = prefix_job_of(p, blockIdx.x, gridDim.x, ++round, &head);
   }
 }
 
@@ -442,20 +413,20 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
 // ---------------------------------------------------------------------------
 struct PrefixShape {
   PagedShape behind;
-  int workers, rows;   // jobs of one key head aimed at; rows of a block
+  int workers, shift;  // jobs of one key head aimed at; log2 of the rows of a block
   int64_t jobs, grid;  // at most
 };
 
-static int prefix_rows(int64_t d, bool latent) { return latent ? kPrefixLatentRows : (d == 256 ? 128 : 256); }
+static int prefix_shift(int64_t d, bool latent) { return latent || d == 256 ? 7 : 8; }
 
 static PrefixShape prefix_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
                                 int64_t max_blocks, int64_t page) {
   PrefixShape s;
   s.behind = paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
-  s.rows = prefix_rows(d, latent);
+  s.shift = prefix_shift(d, latent);
   const int64_t cus = device_cu_count();
   s.workers = (int)(cus / n2 < 1 ? 1 : cus / n2);
-  const int64_t blocks = batch * s1 * (n1 / n2) / s.rows + batch / 2 + 1;
+  const int64_t blocks = (batch * s1 * (n1 / n2) >> s.shift) + batch / 2 + 1;
   s.jobs = blocks >= (1ll << 30) ? 1ll << 31 : prefix_jobs((int)blocks, s.workers);
   s.grid = (cus + 7) / 8 * 8;
   return s;
@@ -466,7 +437,7 @@ bool paged_prefix_launchable(int64_t batch, int64_t s1, int64_t n1, int64_t n2, 
   const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
   // (jobs, their places over all key heads, and the tiles of all blocks of rows are counted in 32 bits)
   return s.jobs < (1ll << 26) && s.jobs * n2 + s.grid < (1ll << 31) &&
-         (batch * s1 * (n1 / n2) / s.rows + batch) * ((max_blocks * page + kPrefixTile - 1) / kPrefixTile) < (1ll << 31);
+         ((batch * s1 * (n1 / n2) >> s.shift) + batch) * ((max_blocks * page + kPrefixTile - 1) / kPrefixTile) < (1ll << 31);
 }
 
 // rows of the outputs of runs, of sequences that a run has whole, and of jobs
@@ -477,13 +448,14 @@ static int64_t prefix_whole_rows(const PrefixShape& s, int64_t batch) {
   return batch * s.behind.groups * s.behind.group_rows;
 }
 static size_t prefix_part_rows(const PrefixShape& s, int64_t batch, int64_t n2) {
-  return (size_t)prefix_run_rows(s) + (size_t)prefix_whole_rows(s, batch) + (size_t)s.jobs * n2 * s.rows;
+  return (size_t)prefix_run_rows(s) + (size_t)prefix_whole_rows(s, batch) + ((size_t)s.jobs * n2 << s.shift);
 }
 
 size_t paged_prefix_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
                                     int64_t max_blocks, int64_t page) {
   const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
-  return prefix_part_rows(s, batch, n2) * (sizeof(f32x4) + d * sizeof(float)) + (size_t)batch * sizeof(i32x4);
+  return prefix_part_rows(s, batch, n2) * (sizeof(f32x4) + d * sizeof(float)) + (size_t)batch * sizeof(PagedWhere) +
+         (size_t)s.jobs * sizeof(PagedJob) + 16;
 }
 
 template <typename T, bool FAST>
@@ -493,11 +465,15 @@ static void prefix_grouped_d(const PagedPrefixParams& p, int64_t d, unsigned gri
   else prefix_grouped_kernel<T, 256, 4, 2, FAST><<<grid, 256, 0, stream>>>(p);
 }
 
-static void prefix_grouped_launch(const PagedPrefixParams& p, int64_t d, int32_t dtype, unsigned grid, hipStream_t stream) {
+static int prefix_grouped_launch(const PagedPrefixParams& p, int64_t d, int32_t dtype, unsigned grid, hipStream_t stream) {
   const int tokens = (int)(512 / d);  // of a DMA
   const bool fast = p.page % tokens == 0 && (int64_t)p.n2 * d * 2 * tokens < (1ll << 31) && p.band_pre >= (1ll << 31);
-  if (dtype == DSA_DTYPE_BF16) fast ? prefix_grouped_d<bf16, true>(p, d, grid, stream) : prefix_grouped_d<bf16, false>(p, d, grid, stream);
-  else fast ? prefix_grouped_d<f16, true>(p, d, grid, stream) : prefix_grouped_d<f16, false>(p, d, grid, stream);
+  if (dtype == DSA_DTYPE_BF16 && fast) prefix_grouped_d<bf16, true>(p, d, grid, stream);
+  else if (dtype == DSA_DTYPE_BF16) prefix_grouped_d<bf16, false>(p, d, grid, stream);
+  else if (fast) prefix_grouped_d<f16, true>(p, d, grid, stream);
+  else prefix_grouped_d<f16, false>(p, d, grid, stream);
+  DSA_HIP(hipGetLastError());
+  return DSA_OK;
 }
 
 int paged_prefix_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
@@ -514,27 +490,22 @@ int paged_prefix_run(const void* query, const void* query_rope, const void* key,
   const size_t rows = prefix_part_rows(s, batch, n2);
   p.part_ml = (f32x4*)workspace;
   p.part_o = (float*)(p.part_ml + rows);
-  p.where = (i32x4*)(p.part_o + rows * d);
+  p.where = (PagedWhere*)(p.part_o + rows * d);
+  p.job = (PagedJob*)(p.where + batch);
+  p.n_jobs = (int*)(p.job + s.jobs);
   p.whole0 = prefix_run_rows(s);
   p.part0 = p.whole0 + prefix_whole_rows(s, batch);
   p.ids = ids;
   p.shared = shared;
   p.prefix_workers = s.workers;
-  p.job_rows = s.rows;
+  p.job_shift = s.shift;
   p.rows_magic = 0xffffffffu / (unsigned)p.rows;
   p.group_magic = 0xffffffffu / (unsigned)p.group;
+  p.heads_magic = 0xffffffffu / (unsigned)p.n2;
   const int64_t most = (s.jobs * n2 + 7) / 8 * 8;
   const unsigned grid = (unsigned)(most < s.grid ? most : s.grid);
-  int st;
-  if (latent) {
-    st = prefix_latent_launch(p, d, dtype, grid, stream);
-    if (st != DSA_OK) return st;
-    st = paged_latent_launch(p, d, dtype, stream);
-  } else {
-    prefix_grouped_launch(p, d, dtype, grid, stream);
-    DSA_HIP(hipGetLastError());
-    st = paged_grouped_launch(p, d, dtype, stream);
-  }
+  int st = latent ? paged_latent_launch(p, d, dtype, stream) : paged_grouped_launch(p, d, dtype, stream);
+  if (st == DSA_OK) st = latent ? prefix_latent_launch(p, d, dtype, grid, stream) : prefix_grouped_launch(p, d, dtype, grid, stream);
   if (st != DSA_OK) return st;
   return paged_combine_launch(p, s.behind.tile, d, dtype, stream);
 }

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
   __shared__ __attribute__((aligned(16))) unsigned char s_p[2 * HG * PROW];
   __shared__ __attribute__((aligned(16))) unsigned char s_q[QL ? HG * QL * 64 : 16];
   __shared__ int s_tab[kPxPages];
-  __shared__ int s_lo[HG], s_hi[HG], s_span[2];
+  __shared__ int s_lo[HG], s_hi[HG];
   __shared__ float s_f[2 * HG];  // by a tile's parity: factors of the rows whose reference moved
   __shared__ int s_flag[3];  // by a tile's number modulo 3: bits of the waves whose rows moved
   float* const s_n = (float*)s_p;  // of a finished run, in place of P: the rows' divisors
@@ -55,12 +55,9 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool rope_wave = wave < 4;
 
-  PrefixLengths lengths;
-  lengths.load(p, lane);
-  PrefixPlan<HG> plan;
   int head;
-  int job = prefix_job_of(blockIdx.x, gridDim.x, 0, 1, &head);
-  plan.make(p, lane);
+  int job = prefix_job_of(p, blockIdx.x, gridDim.x, 0, &head);
+  const int jobs = *p.n_jobs;
 
   // scores in log2 units are s * scale - ref, one operation each; for that
   // the scale is positive: Q takes its sign, and is zero where it is
@@ -92,51 +89,22 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
   };
   using Off = std::integral_constant<bool, false>;
 
-  for (int round = 0; job < plan.jobs;) {
-    const typename PrefixPlan<HG>::Job jb = plan.find(p, fresh_lane(), job);
+  for (int round = 0; job < jobs;) {
+    const PagedJob jb = p.job[job];
     const int ln = fresh_lane(), li = ln & 15, lg = ln >> 4, tid = wave * 64 + ln;
-    int all_lo, all_hi, tok0, tok1;
-    const int part = (job - jb.job0) / jb.blocks, block = (job - jb.job0) - part * jb.blocks;
-    const int first = jb.f.first, n_rows = jb.f.count * p.rows - block * HG;  // (of the block and those after it)
+    const int first = jb.first, n_rows = jb.rows, tok0 = jb.tok0, tok1 = jb.tok1;
     const int64_t slot0 = p.part0 + (int64_t)job * HG;
-    {
-      if (job == jb.job0)
-        for (int i = tid; i < jb.f.count; i += kPxThreads) p.where[first + i] = i32x4{jb.job0, jb.blocks, jb.parts, i};
-      // what the rows see of the prefix, and what any and all of the block's do
+    const bool masked = tok0 < jb.all_lo || tok1 > jb.all_hi;
+    if (masked) {  // what the rows see, where it is not all of it
       lds_barrier();  // (the job before has read what it left)
-      if (tid == 0) s_span[0] = 0x7fffffff, s_span[1] = 0;
-      lds_barrier();
-      const int r = wave * 16 + li;
-      const bool live = r < n_rows;
-      const unsigned vr = block * HG + (live ? r : 0), i = prefix_div(vr, p.rows, p.rows_magic);
-      const int s = prefix_div(vr - i * p.rows, p.group, p.group_magic);
-      int lo, hi;
-      lengths.bounds(p, first + i, s, jb.f.tokens, &lo, &hi);
-      hi = live ? hi : 0;
-      if (lg == 0) s_lo[r] = lo, s_hi[r] = hi;
-      if (lg == 0 && hi > lo) {
-        atomicMin(&s_span[0], lo);
-        atomicMax(&s_span[1], hi);
-      }
-      all_lo = live ? lo : 0;
-      all_hi = live ? hi : 0x7fffffff;
-#pragma unroll
-      for (int o = 1; o < 16; o *= 2) {
-        all_lo = max(all_lo, __shfl_xor(all_lo, o));
-        all_hi = min(all_hi, __shfl_xor(all_hi, o));
-      }
-      all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-      all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-      lds_barrier();
-      const int per = ((jb.f.tokens + TILE - 1) / TILE + jb.parts - 1) / jb.parts * TILE;
-      tok0 = max(part * per, __builtin_amdgcn_readfirstlane(s_span[0]));
-      tok1 = min(min((part + 1) * per, jb.f.tokens), __builtin_amdgcn_readfirstlane(s_span[1]));
+      for (int r = tid; r < n_rows; r += kPxThreads) prefix_bounds(p, jb, r, s_lo + r, s_hi + r);
+    }
+    {
       if (tok1 <= tok0) {  // none of the block's rows sees any of it
-        const int rows_here = min(n_rows, HG);
-        for (int r = tid; r < rows_here; r += kPxThreads) p.part_ml[slot0 + r] = {-INFINITY, 0.f, -INFINITY, 0.f};
-        for (int c = tid; c < rows_here * (D / 4); c += kPxThreads)
+        for (int r = tid; r < n_rows; r += kPxThreads) p.part_ml[slot0 + r] = {-INFINITY, 0.f, -INFINITY, 0.f};
+        for (int c = tid; c < n_rows * (D / 4); c += kPxThreads)
           *((f32x4*)(p.part_o + slot0 * D) + c) = f32x4{0.f, 0.f, 0.f, 0.f};
-        job = prefix_job_of(blockIdx.x, gridDim.x, ++round, 1, &head);
+        job = prefix_job_of(p, blockIdx.x, gridDim.x, ++round, &head);
         continue;
       }
     }
@@ -157,12 +125,11 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
     u32x4 ql_in[QL ? QL : 1];
     {
       // (bounds in the descriptors: rows that do not exist read zeros)
-      const int rows_here = min(n_rows, HG);
-      const int64_t row0 = (int64_t)first * p.rows + block * HG;
+            const int64_t row0 = (int64_t)first * p.rows + jb.row0;
       const __amdgpu_buffer_rsrc_t q_src =
-          __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)p.q + row0 * D), (short)0, rows_here * D * 2, 0x00020000);
+          __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)p.q + row0 * D), (short)0, n_rows * D * 2, 0x00020000);
       const __amdgpu_buffer_rsrc_t qr_src = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)((const T*)p.qr + row0 * DR), (short)0, rows_here * DR * 2, 0x00020000);
+          (void*)((const T*)p.qr + row0 * DR), (short)0, n_rows * DR * 2, 0x00020000);
       const int r = wave * 16 + li;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -299,11 +266,10 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
       auto stage = [&](int k, int t, int flag) {
         if (k == 0) {
           const int tk = ta + t * TILE;
-          if (tk < all_lo || tk + TILE > min(all_hi, tb)) {
+          if (masked || tk + TILE > tb) {
             const int ln = fresh_lane();
-            const int lo = s_lo[wave * 16 + (ln & 15)];
-            int hi = s_hi[wave * 16 + (ln & 15)];
-            hi = min(hi, tb);
+            const int r = min(wave * 16 + (ln & 15), n_rows - 1);
+            const int lo = masked ? s_lo[r] : 0, hi = masked ? min(s_hi[r], tb) : tb;
 #pragma unroll
             for (int i = 0; i < NTT * 4; ++i) {
               const int tok = tk + (i >> 2) * 16 + (ln >> 4) * 4 + (i & 3);
@@ -488,7 +454,7 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
     }
     put(0.f, p.part_o + slot0 * D, [&](int ht, int j) { return acc[j][ht]; });
     }(fresh_lane());
-    job = prefix_job_of(blockIdx.x, gridDim.x, ++round, 1, &head);
+    job = prefix_job_of(p, blockIdx.x, gridDim.x, ++round, &head);
   }
 }
 
