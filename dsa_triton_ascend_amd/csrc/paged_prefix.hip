@@ -149,31 +149,28 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
         const int64_t r = (int64_t)blk * p.page + (int)off;
         return blk < 0 || r >= p.kv_rows ? -1 : (int)r;
       };
-      // the f-th stage's tokens into the ring at `at`
-      int rows = -1;  // lane e: first cache row of DMA e % NI of stage f0 + e / NI
-      auto fetch = [&](int f, int at) {
-        const int tok = ta + f * FETCH;
-        const unsigned dst = smem_base + at + wave * 1024;
-        if (FAST && f % kStages == 0) rows = row_of(tok + lane / NI * FETCH + ((lane % NI) * NW + wave) * TPI);
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          if constexpr (FAST) {
-            // (a row of -1: no bytes)
-            const int r = __builtin_amdgcn_readlane(rows, (f % kStages) * NI + j);
-            const int bytes = min(tb - tok - (j * NW + wave) * TPI, TPI) * (int)row_bytes & ~(r >> 31);
-            const int64_t from = (int64_t)max(r, 0) * row_bytes;
-            dma_buf16(dst + j * NW * 1024, k_from[j],
-                      __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + from), (short)0, bytes, 0x00020000));
-            dma_buf16(dst + j * NW * 1024 + K_BYTES, v_from[j],
-                      __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + from), (short)0, bytes, 0x00020000));
-          } else {
-            const int tk = (j * NW + wave) * TPI + lane / CPT;
-            const int r = row_of(tok + tk);
-            const int kc = ((lane % CPT) ^ swz_k(tk)) * 16, vc = ((lane % CPT) ^ swz_v(tk)) * 16;
-            dma_glb16(dst + j * NW * 1024, r >= 0 ? kbase + r * row_bytes + kc : g_prefix_zero_row + kc);
-            dma_glb16(dst + j * NW * 1024 + K_BYTES, r >= 0 ? vbase + r * row_bytes + vc : g_prefix_zero_row + vc);
-          }
+      // DMA i (K and V in turn) of the f-th stage's tokens into the ring at `at`
+      int rows = -1;  // lane e: first cache row of DMA pair e % NI of stage f0 + e / NI
+      auto dma = [&](int f, int i, int at) {
+        const int j = i >> 1, tok = ta + f * FETCH;
+        const unsigned dst = smem_base + at + (j * NW + wave) * 1024 + (i & 1 ? K_BYTES : 0);
+        if constexpr (FAST) {
+          if (i == 0 && f % kStages == 0) rows = row_of(tok + lane / NI * FETCH + ((lane % NI) * NW + wave) * TPI);
+          // (a row of -1: no bytes)
+          const int r = __builtin_amdgcn_readlane(rows, (f % kStages) * NI + j);
+          const int bytes = min(tb - tok - (j * NW + wave) * TPI, TPI) * (int)row_bytes & ~(r >> 31);
+          const int64_t from = (int64_t)max(r, 0) * row_bytes;
+          dma_buf16(dst, i & 1 ? v_from[j] : k_from[j],
+                    __builtin_amdgcn_make_buffer_rsrc((void*)((i & 1 ? vbase : kbase) + from), (short)0, bytes, 0x00020000));
+        } else {
+          const int tk = (j * NW + wave) * TPI + lane / CPT;
+          const int r = row_of(tok + tk), ch = ((lane % CPT) ^ (i & 1 ? swz_v(tk) : swz_k(tk))) * 16;
+          dma_glb16(dst, r >= 0 ? (i & 1 ? vbase : kbase) + r * row_bytes + ch : g_prefix_zero_row + ch);
         }
+      };
+      auto fetch = [&](int f, int at) {
+#pragma unroll
+        for (int i = 0; i < 2 * NI; ++i) dma(f, i, at);
       };
 
       float f_moved[MR];
@@ -321,11 +318,11 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
       int at = 0;  // of the stage of tile t
       const int n_stages = (n_tiles + SUB - 1) / SUB;
       auto next_stage = [&](int x) { return x == (NB - 1) * STAGE ? 0 : x + STAGE; };
-      auto open_stage = [&](int f) {
+      auto open_stage = [&]() {
         wait_vmcnt<(NB - 3) * 2 * NI>();  // the stage after it has landed
         lds_barrier();
-        fetch(f + NB - 1, at == 0 ? (NB - 1) * STAGE : at - STAGE);
       };
+      auto free_stage = [&]() { return at == 0 ? (NB - 1) * STAGE : at - STAGE; };
       if (active) {
         f32x4 s0[2][MR], s1[2][MR];
         V8 p0[MR], p1[MR];
@@ -341,13 +338,19 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
             for (int j = 0; j < ND; ++j) acc[j][rt] *= f_moved[rt];
           }
         }
-        // tiles t, t + 1 and t + 2 lie at `cur`, `next` and `then`
+        // Tiles t, t + 1 and t + 2 lie at `cur`, `next` and `then`.  DMAs d0 .. d1 of
+        // stage f go into the ring at `to`, between the scores: one after the
+        // other they hold up the wave that asks for them (43 cycles each, when
+        // all waves do).
         auto step = [&](int t, int cur, int next, int then, f32x4 (&s)[2][MR], f32x4 (&sn)[2][MR], V8 (&ph)[MR],
-                        V8 (&pn)[MR]) {
+                        V8 (&pn)[MR], auto d0, auto d1, int f, int to) {
           gemm1(next, cur, sn, [&](int i) {
-            // 2 KS places for NBH slices
+            // 2 KS places for NBH slices and the DMAs
 #pragma unroll
             for (int k = i * NBH / (2 * KS); k < (i + 1) * NBH / (2 * KS); ++k) soft_b(k, s, ph);
+            constexpr int n = decltype(d1)::value - decltype(d0)::value;
+#pragma unroll
+            for (int k = i * n / (2 * KS); k < (i + 1) * n / (2 * KS); ++k) dma(f, decltype(d0)::value + k, to);
           });
           gemm2(cur, then, ph, [&](int i) {
 #pragma unroll
@@ -356,34 +359,38 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
         };
         // (the first fragments of tile 1's scores: its stage has landed)
         if constexpr (SUB == 2) first_k(TILE * ROW);
+        std::integral_constant<int, 0> none;
+        std::integral_constant<int, NI> half;
+        std::integral_constant<int, 2 * NI> all;
         for (int t = 0;;) {
-          open_stage(t / SUB);
+          open_stage();
           int next = next_stage(at);
           asm volatile("" : "+s"(next));  // (so that each stage's offsets fit the instructions)
           if constexpr (SUB == 2) {
-            const int here = at;
-            step(t, here, here + TILE * ROW, next, s0, s1, p0, p1);
+            const int here = at, to = free_stage(), f = t / 2 + NB - 1;
+            step(t, here, here + TILE * ROW, next, s0, s1, p0, p1, none, half, f, to);
             at = next;  // (of tile t + 2)
             if (++t >= n_tiles) break;
-            step(t, here + TILE * ROW, next, next + TILE * ROW, s1, s0, p1, p0);
+            step(t, here + TILE * ROW, next, next + TILE * ROW, s1, s0, p1, p0, half, all, f, to);
             if (++t >= n_tiles) break;
           } else {
             first_k(next);
-            step(t, at, next, next, s0, s1, p0, p1);
+            step(t, at, next, next, s0, s1, p0, p1, none, all, t + NB - 1, free_stage());
             at = next;
             if (++t >= n_tiles) break;
-            open_stage(t);
+            open_stage();
             int then = next_stage(next);
             asm volatile("" : "+s"(then));
             first_k(then);
-            step(t, at, then, then, s1, s0, p1, p0);
+            step(t, at, then, then, s1, s0, p1, p0, none, all, t + NB - 1, free_stage());
             at = then;
             if (++t >= n_tiles) break;
           }
         }
       } else {
         for (int f = 0; f < n_stages; ++f) {
-          open_stage(f);
+          open_stage();
+          fetch(f + NB - 1, free_stage());
           at = next_stage(at);
         }
       }
