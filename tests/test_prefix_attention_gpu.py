@@ -64,8 +64,6 @@ def _make(families, S1, N1, N2, D, page, dtype, latent, seed=0, act_q=None, mode
         return lo, hi
 
     def put(b, t0, t1, rows):
-        for t in range(t0, t1, page):
-            pass
         t = t0
         while t < t1:
             z = min(t1, (t // page + 1) * page)
@@ -411,3 +409,41 @@ def test_empty_caches_and_batches():
     i = torch.zeros(2, dtype=torch.int32, device="cuda")
     out, mx, sm = dsa.paged_prefix_attention(q, none, none, torch.zeros(2, 1, dtype=torch.int32, device="cuda"), i, i, i)
     assert not out.any() and not mx.any() and not sm.any()
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(prefix_groups=2), "one entry per sequence"), (dict(prefix_lengths=4), "one entry per sequence"),
+    (dict(actual_seq_lengths_kv=2), "one entry per batch"), (dict(actual_seq_lengths_query=5), "one entry per batch")])
+def test_refuses_lengths_of_other_batches(change, match):
+    import dsa_triton_ascend_amd as dsa
+    args, _, _ = _make([(0, 96, [100, 150, 130])], 1, page=16, dtype=torch.float16, latent=False, N1=8, N2=2, D=128)
+    for name, n in change.items():
+        with pytest.raises(ValueError, match=match):
+            dsa.paged_prefix_attention(**dict(args, **{name: torch.zeros(n, dtype=torch.int32, device="cuda")}))
+        with pytest.raises(ValueError, match=match):
+            dsa.paged_prefix_attention(**dict(args, **{name: [0] * n}))
+
+
+def test_refuses_strided_caches():
+    import dsa_triton_ascend_amd as dsa
+    args, _, _ = _make([(0, 96, [100, 150, 130])], 1, page=16, dtype=torch.float16, latent=False, N1=8, N2=2, D=128)
+    for name in ("key", "value"):
+        wide = torch.zeros(*args[name].shape[:2], 4, 128, dtype=torch.float16, device="cuda")
+        with pytest.raises(ValueError, match="contiguous"):
+            dsa.paged_prefix_attention(**dict(args, **{name: wide[:, :, ::2]}))
+
+
+@pytest.mark.parametrize("latent", [False, True])
+def test_strided_queries_and_other_tables(latent):
+    """Heads of a wider projection, tables of more rows and of 64 bits, a batch of one."""
+    import dsa_triton_ascend_amd as dsa
+    for families in ([(0, 96, [100, 150, 130])], [(0, 50, [75])]):
+        args, data, lens = _make(families, 1, page=16, dtype=torch.bfloat16, seed=2, **_form(latent))
+        want = _compare(args, data, lens)
+        q = args["query"]
+        wide = torch.randn(*q.shape[:2], q.shape[2] + 3, q.shape[3], device="cuda").to(q.dtype)
+        wide[:, :, 2:-1] = q
+        table = torch.cat([args["block_table"], args["block_table"][:1] * 0 - 7])
+        got = dsa.paged_prefix_attention(**dict(args, query=wide[:, :, 2:-1], block_table=table.long()))
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)

@@ -188,3 +188,86 @@ def test_rope_axes_entry_refuses(change, message):
     for i, x in change.items():
         a[i] = x
     _c("dsa_rope_axes", a, message)
+
+
+# ---- paged_prefix_attention ----
+
+def _attn(latent=False, **kw):
+    """Arguments of a call with three sequences, four pages of 16 tokens."""
+    a = dict(query=torch.zeros(3, 1, 8, 512 if latent else 128, dtype=BF),
+             key=torch.zeros(4, 16, 1, 512, dtype=BF) if latent else torch.zeros(4, 16, 2, 128, dtype=BF),
+             value=None if latent else torch.zeros(4, 16, 2, 128, dtype=BF), block_table=_i(3, 2),
+             actual_seq_lengths_kv=_i(3), prefix_groups=_i(3), prefix_lengths=_i(3))
+    if latent:
+        a.update(query_rope=torch.zeros(3, 1, 8, 64, dtype=BF), key_rope=torch.zeros(4, 16, 1, 64, dtype=BF))
+    a.update(kw)
+    return dsa.paged_prefix_attention(**a)
+
+
+@pytest.mark.parametrize("latent", [False, True])
+@pytest.mark.parametrize("kw,match", [
+    (dict(prefix_groups=None), "prefix_groups and prefix_lengths are required"),
+    (dict(prefix_lengths=None), "prefix_groups and prefix_lengths are required"),
+    (dict(actual_seq_lengths_kv=None), "are required"),
+    (dict(block_table=_i(2, 2)), "block_table"),
+    (dict(sparse_mode=2), "sparse_mode"),
+    (dict(query=torch.zeros(3, 1, 8, 96, dtype=BF)), "columns"),
+    (dict(query=torch.zeros(3, 1, 8, 128)), "columns|dtype|must be"),
+    (dict(query=torch.zeros(3, 8, 128, dtype=BF)), "query must be"),
+    (dict(pre_tokens="x"), "pre_tokens|invalid literal"),
+    (dict(), "ROCm GPU device"),
+])
+def test_prefix_attention_refuses(latent, kw, match):
+    with pytest.raises(ValueError, match=match):
+        _attn(latent, **kw)
+
+
+@pytest.mark.parametrize("latent,kw,match", [
+    (False, dict(value=None), "query_rope and key_rope"),
+    (False, dict(query_rope=torch.zeros(3, 1, 8, 64, dtype=BF)), "no rope parts"),
+    (False, dict(query=torch.zeros(3, 1, 7, 128, dtype=BF)), "multiple"),
+    (False, dict(value=torch.zeros(4, 16, 2, 64, dtype=BF)), "value"),
+    (False, dict(value=torch.zeros(4, 16, 2, 128)), "dtype"),
+    (True, dict(query_rope=torch.zeros(3, 1, 8, 32, dtype=BF)), "query_rope"),
+    (True, dict(key=torch.zeros(4, 16, 2, 512, dtype=BF), key_rope=torch.zeros(4, 16, 2, 64, dtype=BF)), "one key head"),
+])
+def test_prefix_attention_forms_refuse(latent, kw, match):
+    with pytest.raises(ValueError, match=match):
+        _attn(latent, **kw)
+
+
+@pytest.mark.parametrize("name", ["query", "key", "value"])
+def test_prefix_attention_has_no_backward(name):
+    t = torch.zeros(3, 1, 8, 128, dtype=BF) if name == "query" else torch.zeros(4, 16, 2, 128, dtype=BF)
+    with pytest.raises(ValueError, match="paged_prefix_attention has no backward"):
+        _attn(**{name: t.requires_grad_()})
+
+
+@pytest.mark.parametrize("change,message", [
+    ({0: None}, "null"), ({2: None}, "null"), ({5: None}, "null"), ({9: None}, "null"), ({10: None}, "null"),
+    ({11: None}, "null"), ({12: None}, "null"), ({1: P}, "no rope parts"), ({4: None}, "query_rope and key_rope"),
+    ({7: None}, "softmax_max and softmax_sum"), ({13: 0}, "batch"), ({13: 2 ** 24 + 1}, "batch"), ({14: 0}, "S1"),
+    ({15: 7}, "divisible"), ({17: 96}, "D must be"), ({19: 0}, "at least one"), ({20: 0}, "page"),
+    ({21: 2 ** 20 + 1}, "max_blocks"), ({14: 2 ** 22}, "query rows"), ({22: 1}, "sparse_mode"), ({25: 2}, "dtype"),
+    ({28: None}, "workspace"), ({29: 100}, "workspace"), ({28: P + 8}, "16-byte"), ({0: P + 2}, "16-byte")])
+def test_prefix_attention_entry_refuses(change, message):
+    a = [P, None, P, None, P, P, P, P, None, P, P, P, P, 3, 1, 8, 2, 128, 0, 8, 16, 4, 3, 2 ** 62, 2 ** 62, 0, 0.1, 1,
+         P, 1 << 40, None]
+    for i, x in change.items():
+        a[i] = x
+    _c("dsa_paged_prefix_attn", a, message)
+
+
+@pytest.mark.parametrize("change", [
+    {0: 0}, {0: 2 ** 24 + 1}, {1: 0}, {2: 7}, {3: 0}, {4: 96}, {4: 512}, {5: 1}, {6: 0}, {6: 2 ** 20 + 1}, {7: 0},
+    {7: 2 ** 20 + 1}, {1: 2 ** 62}, {6: 2 ** 62}])
+def test_prefix_attention_workspace_of_no_call_is_zero(change):
+    from dsa_triton_ascend_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    a = [3, 1, 8, 2, 128, 0, 4, 16]
+    size = _lib.load().dsa_paged_prefix_attn_workspace_size
+    assert size(*a) > 0
+    for i, x in change.items():
+        a[i] = x
+    assert size(*a) == 0
