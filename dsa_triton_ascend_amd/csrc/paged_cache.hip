@@ -919,30 +919,16 @@ struct PcPrefixParams {
   int rows, max_blocks, page, min_pages;
 };
 
-// A workgroup per row: leading full pages that it has in common with the row
-// before it, to groups; 0 if they are too few to count.  Its waves look at a
-// quarter of the columns each (256 rows of 2000 pages: 3.4 us, one wave a row
-// 6.7), and do not wait for the lengths to know how many there are.
-__global__ __launch_bounds__(kPcThreads) void pc_common_kernel(PcPrefixParams p) {
-  constexpr int W = kPcThreads / 64;
-  __shared__ int s_apart[W];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.x;
-  if (b == 0) {
-    if (threadIdx.x == 0) p.groups[0] = 0;
-    return;
-  }
-  const int l0 = p.lens[b - 1], l1 = p.lens[b];
-  const int32_t *x = p.table + (int64_t)b * p.max_blocks, *y = x - p.max_blocks;
-  const int part = (p.max_blocks + 64 * W - 1) / (64 * W) * 64;
-  const int c1 = min((wave + 1) * part, p.max_blocks);
-  int apart = 0x7fffffff;  // first column of the wave's where the rows differ
+// First column in [c0, c1) where rows x and y of the table differ or name no
+// page, 0x7fffffff if none does.  One wave; rows of `wide` columns.
+__device__ __forceinline__ int pc_apart(const int32_t* x, const int32_t* y, int c0, int c1, int wide, int lane) {
   constexpr int kAhead = 8;  // columns of a lane on their way at a time
-  for (int c0 = wave * part; c0 < c1 && apart == 0x7fffffff; c0 += 64 * kAhead) {
+  int apart = 0x7fffffff;
+  for (; c0 < c1 && apart == 0x7fffffff; c0 += 64 * kAhead) {
     int e[kAhead], f[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      const int c = min(c0 + j * 64 + lane, p.max_blocks - 1);
+      const int c = min(c0 + j * 64 + lane, wide - 1);
       e[j] = x[c];
       f[j] = y[c];
     }
@@ -953,21 +939,56 @@ __global__ __launch_bounds__(kPcThreads) void pc_common_kernel(PcPrefixParams p)
       if (m) apart = c0 + j * 64 + __ffsll(m) - 1;
     }
   }
-  if (lane == 0) s_apart[wave] = apart;
+  return apart;
+}
+
+// the full pages that row b shares, of those before column `apart`; 0 if too few to count
+__device__ __forceinline__ int pc_shared(const PcPrefixParams& p, int l0, int l1, int apart) {
+  const int n = min(min(max(min(l0, l1), 0) / p.page, p.max_blocks), apart);
+  return n >= p.min_pages ? n : 0;
+}
+
+// A workgroup per row: leading full pages that it has in common with the row
+// before it, to groups.  Its waves look at a quarter of the columns each (256
+// rows of 2000 pages: 3.4 us, one wave a row 6.7), and do not wait for the
+// lengths to know how many there are.
+__global__ __launch_bounds__(kPcThreads) void pc_common_kernel(PcPrefixParams p) {
+  constexpr int W = kPcThreads / 64;
+  __shared__ int s_apart[W];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.x;
+  if (b == 0) {
+    if (threadIdx.x == 0) p.groups[0] = 0;
+    return;
+  }
+  const int l0 = p.lens[b - 1], l1 = p.lens[b];
+  const int32_t* x = p.table + (int64_t)b * p.max_blocks;
+  const int part = (p.max_blocks + 64 * W - 1) / (64 * W) * 64, c0 = wave * part;
+  const int mine = pc_apart(x, x - p.max_blocks, c0, min(c0 + part, p.max_blocks), p.max_blocks, threadIdx.x & 63);
+  if ((threadIdx.x & 63) == 0) s_apart[wave] = mine;
   __syncthreads();
   if (threadIdx.x == 0) {
-    int n = min(max(min(l0, l1), 0) / p.page, p.max_blocks);
+    int apart = s_apart[0];
 #pragma unroll
-    for (int w = 0; w < W; ++w) n = min(n, s_apart[w]);
-    p.groups[b] = n >= p.min_pages ? n : 0;
+    for (int w = 1; w < W; ++w) apart = min(apart, s_apart[w]);
+    p.groups[b] = pc_shared(p, l0, l1, apart);
   }
 }
 
-// One workgroup: runs of linked rows and the least that they share.
+// One workgroup: runs of linked rows and the least that they share.  ALL: it
+// looks for what they have in common too, a wave a row.
+template <bool ALL>
 __global__ __launch_bounds__(kPcPlanThreads) void pc_groups_kernel(PcPrefixParams p) {
   constexpr int W = kPcPlanThreads / 64;
   __shared__ int s_last[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (ALL) {
+    for (int b = __builtin_amdgcn_readfirstlane(wave); b < p.rows; b += W) {
+      const int32_t* x = p.table + (int64_t)b * p.max_blocks;
+      const int l0 = p.lens[max(b - 1, 0)], l1 = p.lens[b];
+      const int apart = b ? pc_apart(x, x - p.max_blocks, 0, p.max_blocks, p.max_blocks, lane) : 0;
+      if (lane == 0) p.groups[b] = pc_shared(p, l0, l1, apart);
+    }
+  }
   for (int b = tid; b < p.rows; b += kPcPlanThreads)
     __hip_atomic_store(p.lengths + b, 0x7fffffff, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
@@ -1008,8 +1029,15 @@ int pc_prefixes_run(const int32_t* table, const int32_t* lens, int32_t* groups, 
   const int64_t pages = (min_tokens + page - 1) / page;
   p.min_pages = (int)(pages < 1 ? 1 : pages);
   DSA_CHECK_SUPPORTED(launchable(rows, kPcThreads), "too many rows for one call");
-  pc_common_kernel<<<dim3((unsigned)rows), kPcThreads, 0, stream>>>(p);
-  pc_groups_kernel<<<dim3(1), kPcPlanThreads, 0, stream>>>(p);
+  // In one launch where a wave has a row and looks at it once (a call for 16 rows
+  // of 512 columns takes 3.9 us, replayed 3.7; in two launches 6.5, replayed 4.5;
+  // for 32 rows, two a wave, 5.0 and 4.9 against 6.6 and 4.7).
+  if (rows <= kPcPlanThreads / 64 && max_blocks <= 512) {
+    pc_groups_kernel<true><<<dim3(1), kPcPlanThreads, 0, stream>>>(p);
+  } else {
+    pc_common_kernel<<<dim3((unsigned)rows), kPcThreads, 0, stream>>>(p);
+    pc_groups_kernel<false><<<dim3(1), kPcPlanThreads, 0, stream>>>(p);
+  }
   DSA_HIP(hipGetLastError());
   return DSA_OK;
 }

@@ -257,8 +257,9 @@ def _prefixes(table, lens, page, least=1):
     return groups, shared
 
 
-@pytest.mark.parametrize("rows,page,wide", [(1, 16, 3), (2, 1, 1), (5, 16, 9), (64, 4, 70), (70, 16, 600), (1030, 8, 5),
-                                            (3000, 16, 3)])
+@pytest.mark.parametrize("rows,page,wide", [(1, 16, 3), (2, 1, 1), (5, 16, 9), (16, 8, 512),
+                                            (17, 8, 512), (16, 8, 513), (3, 1, 1200), (64, 4, 70), (70, 16, 600),
+                                            (1030, 8, 5), (3000, 16, 3)])
 @pytest.mark.parametrize("least", [0, 1, 40])
 def test_prefixes(rows, page, wide, least):
     import dsa_triton_ascend_amd as dsa
