@@ -228,7 +228,8 @@ SIGNATURES = {
         _i32p, _i32p, _i32p, _i32p, _i32p,    # actual_seq_q, actual_seq_kv, block_table, prefix_groups, prefix_lengths
         _i64, _i64, _i64, _i64, _i64, _i64,   # batch, s1, n1, n2, d, d_rope
         _i64, _i64, _i64,                     # num_blocks, page_size, max_blocks
-        _i32, _i64, _i64, _i32, _f32, _i32,   # sparse_mode, pre_tokens, next_tokens, dtype, scale_value, return_lse
+        _i32, _i64, _i64, _i64, _i32, _f32,   # sparse_mode, pre_tokens, next_tokens, min_tokens, dtype, scale_value
+        _i32,                                 # return_lse
         _vp, _sz, _vp,                        # workspace, workspace_bytes, stream
     ]),
 }

@@ -13,8 +13,8 @@ int paged_prefix_run(const void* query, const void* query_rope, const void* key,
                      const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
                      const int32_t* act_k, const int32_t* table, const int32_t* ids, const int32_t* shared,
                      int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, int64_t num_blocks, int64_t page,
-                     int64_t max_blocks, int32_t mode, int64_t pre_tokens, int64_t next_tokens, int32_t dtype,
-                     float scale, int32_t return_lse, void* workspace, hipStream_t stream);
+                     int64_t max_blocks, int32_t mode, int64_t pre_tokens, int64_t next_tokens, int64_t min_tokens,
+                     int32_t dtype, float scale, int32_t return_lse, void* workspace, hipStream_t stream);
 
 }  // namespace dsa
 
@@ -36,7 +36,7 @@ int dsa_paged_prefix_attn(const void* query, const void* query_rope, const void*
                           const int32_t* prefix_groups, const int32_t* prefix_lengths, int64_t batch, int64_t s1,
                           int64_t n1, int64_t n2, int64_t d, int64_t d_rope, int64_t num_blocks, int64_t page_size,
                           int64_t max_blocks, int32_t sparse_mode, int64_t pre_tokens, int64_t next_tokens,
-                          int32_t dtype, float scale_value, int32_t return_lse, void* workspace,
+                          int64_t min_tokens, int32_t dtype, float scale_value, int32_t return_lse, void* workspace,
                           size_t workspace_bytes, void* stream) {
   clear_error();
   const bool latent = value == nullptr;
@@ -53,7 +53,8 @@ int dsa_paged_prefix_attn(const void* query, const void* query_rope, const void*
   DSA_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
   return paged_prefix_run(query, query_rope, key, key_rope, value, attention_out, softmax_max, softmax_sum,
                           actual_seq_q, actual_seq_kv, block_table, prefix_groups, prefix_lengths, batch, s1, n1, n2, d,
-                          num_blocks, page_size, max_blocks, sparse_mode, pre_tokens, next_tokens, dtype, scale_value,
+                          num_blocks, page_size, max_blocks, sparse_mode, pre_tokens, next_tokens, min_tokens, dtype,
+                          scale_value,
                           return_lse, workspace, (hipStream_t)stream);
 }
 

@@ -56,7 +56,8 @@ struct PagedAttnParams {
 
 // With a prefix that sequences share (paged_prefix.h): these kernels take what
 // is behind it, plan the work on the prefixes meanwhile, and the join takes
-// both's parts.
+// both's parts.  A short prefix they take too, for each sequence, from the pages
+// of its family's first.
 struct PagedWhere {  // of a sequence, for the join
   int job0, blocks, parts, place;  // first job of its family, blocks of rows, parts (0: no family), its place there
   int run0, runs, slot0, unused;   // its runs and the slot of the first
@@ -74,12 +75,27 @@ struct PagedPrefixParams : PagedAttnParams {
   // rows of part_o / part_ml: behind those of the runs come, for each sequence,
   // one for what a run has of it if that is all of it, then those of the jobs
   int64_t whole0, part0;
+  int least;                    // tokens of a prefix from which on it is worked on for its family together
   int prefix_workers;           // jobs of one key head aimed at
   int job_shift;                // log2 of the rows of a block
   unsigned rows_magic, group_magic, heads_magic;  // floor((2^32 - 1) / rows), of group, of n2
 };
 
 template <typename P> constexpr bool kPrefixed = std::is_same<P, PagedPrefixParams>::value;
+
+// whether sequence b has the family of the one before it
+__device__ __forceinline__ bool paged_linked(const PagedPrefixParams& p, int b) {
+  const int before = max(b - 1, 0), id = p.ids[b], n = p.shared[b];
+  return b > 0 && id >= 0 && n > 0 && p.ids[before] == id && p.shared[before] == n;
+}
+
+// the first sequence of the family that b is in, for a b that is the same on all lanes
+__device__ __forceinline__ int paged_leader(const PagedPrefixParams& p, int b, int lane) {
+  for (;; b -= 64) {
+    const unsigned long long apart = ~__ballot(paged_linked(p, max(b - lane, 0)));
+    if (apart) return b - (__ffsll(apart) - 1);
+  }
+}
 
 // Tokens that sequence b shares with the one before or behind it.
 __device__ __forceinline__ int paged_shared(const PagedPrefixParams& p, int b) {
@@ -107,7 +123,8 @@ struct PagedSeq {
   int act_q, act_k, lo, hi;  // lo <= t < hi: tokens that any row sees (with a prefix: behind it)
 };
 struct PagedSeqBehind : PagedSeq {
-  int shared;  // tokens of the prefix
+  int shared;  // tokens of the prefix before it
+  int given;   // tokens of its own that are in the pages of its family's first sequence
 };
 template <typename P> using PagedSeqOf = std::conditional_t<kPrefixed<P>, PagedSeqBehind, PagedSeq>;
 // whether a sequence has a prefix before it
@@ -141,7 +158,9 @@ __device__ __forceinline__ PagedSeqOf<P> paged_seq(const P& p, int b) {
   paged_bounds(p, s.act_q, s.act_k, 0, &s.lo, &h);
   paged_bounds(p, s.act_q, s.act_k, max(s.act_q - 1, 0), &l, &s.hi);
   if constexpr (kPrefixed<P>) {
-    s.shared = paged_shared(p, b);
+    s.given = paged_shared(p, b);
+    s.shared = s.given >= p.least ? s.given : 0;
+    s.given -= s.shared;
     s.lo = max(s.lo, s.shared);
   }
   if (s.hi < s.lo) s.hi = s.lo;
@@ -250,7 +269,10 @@ struct PagedPlan {
       s.act_k = __builtin_amdgcn_readlane(seq.act_k, b);
       s.lo = __builtin_amdgcn_readlane(seq.lo, b);
       s.hi = __builtin_amdgcn_readlane(seq.hi, b);
-      if constexpr (kPrefixed<P>) s.shared = __builtin_amdgcn_readlane(seq.shared, b);
+      if constexpr (kPrefixed<P>) {
+        s.shared = __builtin_amdgcn_readlane(seq.shared, b);
+        s.given = __builtin_amdgcn_readlane(seq.given, b);
+      }
     } else {
       s = paged_seq(p, b);
       s.lo = __builtin_amdgcn_readfirstlane(s.lo);

@@ -87,7 +87,9 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
     }
     const int t0 = at - before, t1 = min(end - before, nt);
     const int tok0 = seq.lo + t0 * kPaTile, tok1 = min(seq.hi, seq.lo + t1 * kPaTile);
-    const int32_t* tab = p.table + (int64_t)b * p.max_blocks;
+    const int32_t *tab = p.table + (int64_t)b * p.max_blocks, *lead = tab;
+    if constexpr (kPrefixed<P>)
+      if (__any(seq.given)) lead = p.table + (int64_t)paged_leader(p, b, lane) * p.max_blocks;
 
     // rows of this lane's MFMA column: query head kvh * group + r % group of
     // token r / group
@@ -123,7 +125,9 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
     auto page_of = [&](int tile0) {
       const int t = tile0 + (lane & 31);
       unsigned off;
-      return t < tok1 ? tab[paged_split(p, (unsigned)t, &off)] : -1;
+      const int32_t* from = tab;
+      if constexpr (kPrefixed<P>) from = t < seq.given ? lead : tab;
+      return t < tok1 ? from[paged_split(p, (unsigned)t, &off)] : -1;
     };
     auto row_of = [&](int tile0, int blk) {
       unsigned off;
@@ -297,6 +301,12 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
 // ---------------------------------------------------------------------------
 constexpr int kPcFewRuns = 64;
 
+// rows of a workgroup of the join: four, one per wave, unless the average
+// sequence has so many runs that the waves had better share them
+__host__ __device__ __forceinline__ int paged_combine_rows(int64_t workers, int64_t batch) {
+  return workers > 32 * batch ? 1 : 4;
+}
+
 template <typename T, int D, typename P>
 __global__ __launch_bounds__(256) void paged_combine_kernel(P p, int tile, int wg_rows) {
   using E = Elem<T>;
@@ -404,8 +414,12 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(P p, int tile, int w
   };
   FV o;
   float big, top, l, n;
-  if (runs <= kPcFewRuns && wg_rows > 1) {
-    if (row0 + wave < per_seq) {
+  bool wave_rows = wg_rows > 1;
+  if constexpr (kPrefixed<P>) {  // (without a prefix as without this argument)
+    if (!behind) wave_rows = paged_combine_rows(p.workers, p.batch) > 1;
+  }
+  if (runs <= kPcFewRuns && wave_rows) {
+    if (row0 + wave < per_seq && (!kPrefixed<P> || wave < wg_rows)) {
       row_of(row0 + wave, 0, runs, &big, &top, &o, &l, &n);
       write(row0 + wave, o, big, top, l, n);
     }
@@ -438,9 +452,6 @@ static void paged_combine_d(const P& p, int tile, int wg_rows, int64_t d, unsign
   else paged_combine_kernel<T, 512><<<grid, 256, 0, stream>>>(p, tile, wg_rows);
 }
 
-// rows of a workgroup of the join: four, one per wave, unless the average
-// sequence has so many runs that the waves had better share them
-static int paged_combine_rows(int64_t workers, int64_t batch) { return workers > 32 * batch ? 1 : 4; }
 static int64_t paged_combine_grid(int64_t workers, int64_t batch, int64_t s1, int64_t n1) {
   const int wg_rows = paged_combine_rows(workers, batch);
   return batch * ((s1 * n1 + wg_rows - 1) / wg_rows);
@@ -452,8 +463,15 @@ bool paged_combine_launchable(int64_t workers, int64_t batch, int64_t s1, int64_
 
 template <typename P>
 static int paged_combine(const P& p, int tile, int64_t d, int32_t dtype, hipStream_t stream) {
-  const int wg_rows = paged_combine_rows(p.workers, p.batch);
-  const unsigned grid = (unsigned)paged_combine_grid(p.workers, p.batch, p.s1, p.n1);
+  int wg_rows = paged_combine_rows(p.workers, p.batch);
+  if constexpr (kPrefixed<P>) {
+    // or a family so many parts (16 latent heads, 8 sequences behind 32K tokens,
+    // 256 parts: 59 us with a wave a row, 19 with four)
+    const int blocks = (int)(((int64_t)p.batch * p.rows >> p.job_shift) + 1);
+    if (p.prefix_workers >= 32 * blocks) wg_rows = 1;
+  }
+  const int64_t per_seq = (int64_t)p.s1 * p.n1;
+  const unsigned grid = (unsigned)(p.batch * ((per_seq + wg_rows - 1) / wg_rows));
   if (dtype == DSA_DTYPE_BF16) paged_combine_d<bf16>(p, tile, wg_rows, d, grid, stream);
   else paged_combine_d<f16>(p, tile, wg_rows, d, grid, stream);
   DSA_HIP(hipGetLastError());

@@ -188,7 +188,9 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(P p) {
     }
     const int t0 = at - before, t1 = min(end - before, nt);
     const int tok0 = seq.lo + t0 * TILE, tok1 = min(seq.hi, seq.lo + t1 * TILE);
-    const int32_t* tab = p.table + (int64_t)b * p.max_blocks;
+    const int32_t *tab = p.table + (int64_t)b * p.max_blocks, *lead = tab;
+    if constexpr (kPrefixed<P>)
+      if (__any(seq.given)) lead = p.table + (int64_t)paged_leader(p, b, ln) * p.max_blocks;
 
     // the run's pages, as many as the LDS holds at a time, a thread's each
     int ta = tok0, tb, pg0, page_entry;
@@ -196,8 +198,11 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(P p) {
       unsigned off0;
       pg0 = (int)paged_split(p, (unsigned)ta, &off0);
       tb = (int)min((int64_t)tok1, (int64_t)(pg0 + kPlPages) * p.page);
+      const int32_t* from = tab;
+      if constexpr (kPrefixed<P>)
+        if (ta < seq.given) from = lead, tb = min(tb, seq.given);
       const int npg = (int)paged_split(p, (unsigned)tb - 1u, &off0) - pg0 + 1;
-      page_entry = tid < npg ? tab[pg0 + tid] : 0;
+      page_entry = tid < npg ? from[pg0 + tid] : 0;
     };
     read_pages();
 

@@ -25,6 +25,7 @@ namespace dsa {
 
 constexpr int kPrefixTile = 32;  // tokens
 constexpr int kPrefixMinTiles = 2;  // fewest tiles of a part
+constexpr float kPrefixPartTiles = 18.f;
 
 // jobs of one key head for `m` blocks of rows: as many as there are workers, or
 // (where the blocks alone are more than half of them) whole rounds of workers,
@@ -44,7 +45,8 @@ __device__ __forceinline__ PrefixFamily prefix_families(const PagedPrefixParams&
   const int i0 = min(max(b - 1, 0), last), i1 = min(b, last), i2 = min(b + 1, last);
   const int id0 = p.ids[i0], id1 = p.ids[i1], id2 = p.ids[i2];
   const int n0 = p.shared[i0], n1 = p.shared[i1], n2 = p.shared[i2];
-  const bool shares = id1 >= 0 && n1 > 0;
+  const int room = p.max_blocks * p.page;
+  const bool shares = id1 >= 0 && min(n1, room) >= p.least;
   const bool mine = shares && b > 0 && b <= last && id0 == id1 && n0 == n1;  // linked to the sequence before it
   const bool next = shares && b < last && id1 == id2 && n1 == n2;
   const unsigned long long links = __ballot(mine);
@@ -52,13 +54,14 @@ __device__ __forceinline__ PrefixFamily prefix_families(const PagedPrefixParams&
   if (next && !mine) {
     const unsigned long long after = lane == 63 ? 0ull : links >> (lane + 1);
     f.count = __ffsll(~after);  // the links that follow, and the first sequence
-    f.tokens = min(n1, p.max_blocks * p.page);
+    f.tokens = min(n1, room);
   }
   // a family that goes on behind these
   bool open = f.count > 0 && lane + f.count == 64 && b + f.count < p.batch;
   for (int e = c0 + 64; __any(open); e += 64) {
     const int j = min(e + lane, last), id = p.ids[j], n = p.shared[j];
-    const bool linked = e + lane <= last && id >= 0 && n > 0 && id == p.ids[j - 1] && n == p.shared[j - 1];
+    const bool linked = e + lane <= last && id >= 0 && min(n, room) >= p.least && id == p.ids[j - 1] &&
+                        n == p.shared[j - 1];
     const unsigned long long more = __ballot(linked);
     const int k = ~more ? __ffsll(~more) - 1 : 64;
     if (open) f.count += k;
@@ -95,6 +98,13 @@ struct PrefixPlan {
     t = (f.tokens + kPrefixTile - 1) / kPrefixTile;
   }
 
+  // Fewest tiles of a part.  A part more costs the writing and joining of its
+  // output, so long as PREFIX_TILES tiles take: J jobs cost J + 18 W / J of that for W tiles in all.
+  __device__ __forceinline__ int least(const PagedPrefixParams& p, int work, int blocks, int rows) const {
+    const float fill = (float)rows / (float)(max(blocks, 1) << p.job_shift);
+    return max((int)__builtin_sqrtf((float)work * (float)p.n2 * fill * (1.f / kPrefixPartTiles) + 0.5f), kPrefixMinTiles);
+  }
+
   // sum m ceil(t / per) may be `most` jobs.  Up to 64 sequences the length of
   // the parts is fitted to the families; with more, which would be read again
   // for it, it is the shortest that has room for every rounding up, unless one
@@ -102,25 +112,26 @@ struct PrefixPlan {
   __device__ __forceinline__ void make(const PagedPrefixParams& p, int lane) {
     families(p, 0, lane);
     if (p.batch <= 64) {
-      const int work = wave_total(m * t), most = prefix_jobs(wave_total(m), p.prefix_workers);
-      per = max(prefix_div_up(work, most), kPrefixMinTiles);
+      const int work = wave_total(m * t), blocks = wave_total(m), most = prefix_jobs(blocks, p.prefix_workers);
+      per = max(prefix_div_up(work, most), least(p, work, blocks, wave_total(f.count * p.rows)));
       for (;;) {
         jobs = wave_total(m * prefix_div_up(t, per));
         if (jobs <= most) return;
         per += max(per >> 4, 1);
       }
     }
-    int work = 0, rows = 0;
+    int work = 0, rows = 0, all = 0;
     for (int c0 = 0; c0 < p.batch; c0 += 64) {
       families(p, c0, lane);
       work += m * t;
       rows += m;
+      all += f.count * p.rows;
     }
     work = wave_total(work);
     rows = wave_total(rows);
-    const int most = prefix_jobs(rows, p.prefix_workers);
+    const int most = prefix_jobs(rows, p.prefix_workers), fewest = least(p, work, rows, wave_total(all));
     for (int room = 0;; room = rows) {
-      per = max(prefix_div_up(work, most - room), kPrefixMinTiles);
+      per = max(prefix_div_up(work, most - room), fewest);
       int n = 0;
       for (int c0 = 0; c0 < p.batch; c0 += 64) {
         families(p, c0, lane);

@@ -483,12 +483,18 @@ static int prefix_grouped_launch(const PagedPrefixParams& p, int64_t d, int32_t 
   return DSA_OK;
 }
 
+// Tokens of a prefix from which on it is worked on for its family together.
+static int prefix_least(int64_t min_tokens) {
+  if (min_tokens >= 0) return (int)(min_tokens < 1 ? 1 : (min_tokens > 0x7fffffff ? 0x7fffffff : min_tokens));
+  return 1;
+}
+
 int paged_prefix_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
                      const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
                      const int32_t* act_k, const int32_t* table, const int32_t* ids, const int32_t* shared,
                      int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, int64_t num_blocks, int64_t page,
-                     int64_t max_blocks, int32_t mode, int64_t pre_tokens, int64_t next_tokens, int32_t dtype,
-                     float scale, int32_t return_lse, void* workspace, hipStream_t stream) {
+                     int64_t max_blocks, int32_t mode, int64_t pre_tokens, int64_t next_tokens, int64_t min_tokens,
+                     int32_t dtype, float scale, int32_t return_lse, void* workspace, hipStream_t stream) {
   const bool latent = value == nullptr;
   const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
   PagedPrefixParams p = {};
@@ -504,6 +510,7 @@ int paged_prefix_run(const void* query, const void* query_rope, const void* key,
   p.part0 = p.whole0 + prefix_whole_rows(s, batch);
   p.ids = ids;
   p.shared = shared;
+  p.least = prefix_least(min_tokens);
   p.prefix_workers = s.workers;
   p.job_shift = s.shift;
   p.rows_magic = 0xffffffffu / (unsigned)p.rows;
@@ -512,7 +519,8 @@ int paged_prefix_run(const void* query, const void* query_rope, const void* key,
   const int64_t most = (s.jobs * n2 + 7) / 8 * 8;
   const unsigned grid = (unsigned)(most < s.grid ? most : s.grid);
   int st = latent ? paged_latent_launch(p, d, dtype, stream) : paged_grouped_launch(p, d, dtype, stream);
-  if (st == DSA_OK) st = latent ? prefix_latent_launch(p, d, dtype, grid, stream) : prefix_grouped_launch(p, d, dtype, grid, stream);
+  if (st == DSA_OK && p.least <= max_blocks * page)
+    st = latent ? prefix_latent_launch(p, d, dtype, grid, stream) : prefix_grouped_launch(p, d, dtype, grid, stream);
   if (st != DSA_OK) return st;
   return paged_combine_launch(p, s.behind.tile, d, dtype, stream);
 }

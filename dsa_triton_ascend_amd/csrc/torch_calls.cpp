@@ -297,7 +297,7 @@ PyObject* compact(PyObject* const* a) {
 
 // (query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
 // actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse
-// [, prefix_groups, prefix_lengths]) -> triple
+// [, prefix_groups, prefix_lengths, min_tokens]) -> triple
 template <bool PREFIX>
 PyObject* attention(PyObject* const* a) {
   int index = -1;
@@ -330,8 +330,10 @@ PyObject* attention(PyObject* const* a) {
   }
   if (a[8] != Py_None && (!(act_q = ints(a[8], &index, 1)) || act_q->size(0) != b)) return nullptr;
   const at::Tensor *groups = nullptr, *shared = nullptr;
+  int64_t least = -1;
   if (PREFIX) {
     groups = ints(a[13], &index, 1), shared = ints(a[14], &index, 1);
+    if (a[15] != Py_None && (!integer(a[15], &least) || least < 0)) return nullptr;
     if (!groups || !shared || groups->size(0) != b || shared->size(0) != b) return nullptr;
   }
   const int64_t wide = table->size(1);
@@ -345,7 +347,7 @@ PyObject* attention(PyObject* const* a) {
                   latent ? kr->data_ptr() : nullptr, latent ? nullptr : v->data_ptr(), out.data_ptr(),
                   (float*)mx.data_ptr(), (float*)sm.data_ptr(), data(act_q), data(act_k), data(table), data(groups),
                   data(shared), b, s1, n1, n2, d, latent ? 64 : 0, pages, page, wide, (int32_t)mode, pre, next,
-                  kind == at::kHalf ? DSA_DTYPE_FP16 : DSA_DTYPE_BF16, (float)scale, lse, ws.get(), bytes,
+                  least, kind == at::kHalf ? DSA_DTYPE_FP16 : DSA_DTYPE_BF16, (float)scale, lse, ws.get(), bytes,
                   stream_of(index)))
       return nullptr;
   } else if (!launched(entry.attn, q->data_ptr(), latent ? qr->data_ptr() : nullptr, k->data_ptr(), latent ? kr->data_ptr() : nullptr,
@@ -727,7 +729,7 @@ PyMethodDef methods[] = {
     {"fork", FAST((call<fork, 7>)), METH_FASTCALL, nullptr},
     {"compact", FAST((call<compact, 4>)), METH_FASTCALL, nullptr},
     {"attention", FAST((call<attention<false>, 13>)), METH_FASTCALL, nullptr},
-    {"prefix_attention", FAST((call<attention<true>, 15>)), METH_FASTCALL, nullptr},
+    {"prefix_attention", FAST((call<attention<true>, 16>)), METH_FASTCALL, nullptr},
     {"rotate", FAST((call<rotate<false>, 11>)), METH_FASTCALL, nullptr},
     {"rotate_axes", FAST((call<rotate<true>, 13>)), METH_FASTCALL, nullptr},
     {"plan", FAST((call<plan, 6>)), METH_FASTCALL, nullptr},

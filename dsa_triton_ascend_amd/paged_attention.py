@@ -57,7 +57,8 @@ def paged_attention(query, key, value, block_table, actual_seq_lengths_kv, scale
 
 def paged_prefix_attention(query, key, value, block_table, actual_seq_lengths_kv, prefix_groups, prefix_lengths,
                            scale_value=1.0, query_rope=None, key_rope=None, actual_seq_lengths_query=None,
-                           sparse_mode=3, pre_tokens=INT64_MAX, next_tokens=INT64_MAX, return_softmax_lse=False):
+                           sparse_mode=3, pre_tokens=INT64_MAX, next_tokens=INT64_MAX, return_softmax_lse=False,
+                           min_tokens=None):
     """``paged_attention`` of sequences that share a prefix (a system prompt, a
     common document or image, the beams of a fork), which is read once for all
     of them.
@@ -79,18 +80,21 @@ def paged_prefix_attention(query, key, value, block_table, actual_seq_lengths_kv
     result = _lib.calls().prefix_attention(
         query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
         actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse, prefix_groups,
-        prefix_lengths)
+        prefix_lengths, min_tokens)
     if result is not None:
         return result
     if prefix_groups is None or prefix_lengths is None:
         raise ValueError("prefix_groups and prefix_lengths are required")
+    if min_tokens is not None and (int(min_tokens) != min_tokens or not 0 <= min_tokens < 2 ** 63):
+        raise ValueError(f"min_tokens must be None or an integer in [0, 2^63), got {min_tokens}")
     return _attend(query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
                    actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse,
-                   (prefix_groups, prefix_lengths))
+                   (prefix_groups, prefix_lengths), -1 if min_tokens is None else int(min_tokens))
 
 
 def _attend(query, key, value, block_table, actual_seq_lengths_kv, scale_value, query_rope, key_rope,
-            actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse, prefix=None):
+            actual_seq_lengths_query, sparse_mode, pre_tokens, next_tokens, return_softmax_lse, prefix=None,
+            min_tokens=-1):
     """The call on arguments of any kind that may be converted; ``prefix``:
     None, or the groups and lengths of shared prefixes."""
     pre_tokens, next_tokens = _band_args(pre_tokens, next_tokens)
@@ -177,8 +181,9 @@ def _attend(query, key, value, block_table, actual_seq_lengths_kv, scale_value, 
         index, entry, q.data_ptr(), qr.data_ptr() if latent else None, key.data_ptr(),
         key_rope.data_ptr() if latent else None, None if latent else value.data_ptr(), out.data_ptr(),
         smax.data_ptr(), ssum.data_ptr(), None if act_q is None else act_q.data_ptr(), act_k.data_ptr(),
-        table.data_ptr(), *(x.data_ptr() for x in families), B, S1, N1, N2, D, _D_ROPE if latent else 0, pages, page, wide, sparse_mode, pre_tokens,
-        next_tokens, code, float(scale_value), bool(return_softmax_lse), ws.data_ptr(), nbytes, _lib.raw_stream(index))
+        table.data_ptr(), *(x.data_ptr() for x in families), B, S1, N1, N2, D, _D_ROPE if latent else 0, pages, page,
+        wide, sparse_mode, pre_tokens, next_tokens, *(() if prefix is None else (min_tokens,)), code,
+        float(scale_value), bool(return_softmax_lse), ws.data_ptr(), nbytes, _lib.raw_stream(index))
     if status:
         _lib.check(status, "dsa_" + what.replace("attention", "attn"))
     return out, smax, ssum
@@ -231,12 +236,18 @@ class PagedAttention(torch.nn.Module):
 class PagedPrefixAttention(PagedAttention):
     """Module wrapper of ``paged_prefix_attention``."""
 
+    def __init__(self, scale_value=1.0, sparse_mode=3, return_softmax_lse=False, pre_tokens=INT64_MAX,
+                 next_tokens=INT64_MAX, min_tokens=None):
+        super().__init__(scale_value, sparse_mode, return_softmax_lse, pre_tokens, next_tokens)
+        self.min_tokens = min_tokens
+
     def forward(self, query, key, value, block_table, actual_seq_lengths_kv, prefix_groups, prefix_lengths,
                 query_rope=None, key_rope=None, actual_seq_lengths_query=None):
         return paged_prefix_attention(
             query, key, value, block_table, actual_seq_lengths_kv, prefix_groups, prefix_lengths,
             scale_value=self.scale_value, query_rope=query_rope, key_rope=key_rope,
             actual_seq_lengths_query=actual_seq_lengths_query, sparse_mode=self.sparse_mode,
-            pre_tokens=self.pre_tokens, next_tokens=self.next_tokens, return_softmax_lse=self.return_softmax_lse)
+            pre_tokens=self.pre_tokens, next_tokens=self.next_tokens, return_softmax_lse=self.return_softmax_lse,
+            min_tokens=self.min_tokens)
 
     construct = forward

@@ -594,7 +594,7 @@ int dsa_paged_prefix_attn(const void* query, const void* query_rope, const void*
                           const int32_t* prefix_groups, const int32_t* prefix_lengths, int64_t batch, int64_t s1,
                           int64_t n1, int64_t n2, int64_t d, int64_t d_rope, int64_t num_blocks, int64_t page_size,
                           int64_t max_blocks, int32_t sparse_mode, int64_t pre_tokens, int64_t next_tokens,
-                          int32_t dtype, float scale_value, int32_t return_lse, void* workspace,
+                          int64_t min_tokens, int32_t dtype, float scale_value, int32_t return_lse, void* workspace,
                           size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

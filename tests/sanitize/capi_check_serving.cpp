@@ -109,15 +109,15 @@ int main() {
     if (latent) opt.insert(4);
     else opt.insert({1, 3});
     sweep(latent ? "paged_prefix_attn latent" : "paged_prefix_attn grouped", 14, opt,
-          {2, 1, 8, latent ? 1 : 2, latent ? 512 : 128, latent ? 64 : 0, 8, 16, 4, 3, 1ll << 62, 1ll << 62, 0, 1,
-           1ll << 40},
+          {2, 1, 8, latent ? 1 : 2, latent ? 512 : 128, latent ? 64 : 0, 8, 16, 4, 3, 1ll << 62, 1ll << 62, -1, 0,
+           1, 1ll << 40},
           [latent](Ps p, Is v) {
             return dsa_paged_prefix_attn(p[0], latent ? p[1] : nullptr, p[2], latent ? p[3] : nullptr,
                                          latent ? nullptr : p[4], (void*)p[5], (float*)p[6], (float*)p[7],
                                          (const int32_t*)p[8], (const int32_t*)p[9], (const int32_t*)p[10],
                                          (const int32_t*)p[11], (const int32_t*)p[12], v[0], v[1], v[2], v[3], v[4],
-                                         v[5], v[6], v[7], v[8], (int32_t)v[9], v[10], v[11], (int32_t)v[12], 0.1f,
-                                         (int32_t)v[13], (void*)p[13], (size_t)v[14], nullptr);
+                                         v[5], v[6], v[7], v[8], (int32_t)v[9], v[10], v[11], v[12],
+                                         (int32_t)v[13], 0.1f, (int32_t)v[14], (void*)p[13], (size_t)v[15], nullptr);
           });
   }
   for (int latent = 0; latent < 2; ++latent) {

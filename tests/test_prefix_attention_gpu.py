@@ -101,7 +101,7 @@ def _make(families, S1, N1, N2, D, page, dtype, latent, seed=0, act_q=None, mode
                 actual_seq_lengths_kv=ints(lens), prefix_groups=ints(ids), prefix_lengths=ints(shared),
                 scale_value=1.0 / math.sqrt(D + 64 if latent else D), query_rope=qr, key_rope=caches[1] if latent else None,
                 actual_seq_lengths_query=None if act_q is None else ints(act_q), sparse_mode=mode, pre_tokens=pre,
-                next_tokens=nxt, return_softmax_lse=True)
+                next_tokens=nxt, return_softmax_lse=True, min_tokens=1)
     return args, data, lens
 
 
@@ -312,7 +312,7 @@ def test_equals_paged_attention_of_the_same_pages(latent):
     a = dsa.paged_prefix_attention(**args)
     table = args["block_table"].clone()
     table[1:3, :20] = table[0, :20]
-    plain = {k: v for k, v in args.items() if not k.startswith("prefix")}
+    plain = {k: v for k, v in args.items() if not k.startswith("prefix") and k != "min_tokens"}
     plain["block_table"] = table
     b = dsa.paged_attention(**plain)
     for x, y in zip(a, b):
@@ -394,7 +394,7 @@ def test_compiled_and_python_calls_agree(monkeypatch):
         lists = dict(args, prefix_groups=[0, 0, 0], prefix_lengths=[96, 96, 96], actual_seq_lengths_kv=lens,
                      block_table=args["block_table"].long())
         c = dsa.paged_prefix_attention(**lists)
-        m = dsa.PagedPrefixAttention(scale_value=args["scale_value"], return_softmax_lse=True)
+        m = dsa.PagedPrefixAttention(scale_value=args["scale_value"], return_softmax_lse=True, min_tokens=1)
         d = m(args["query"], args["key"], args["value"], args["block_table"], args["actual_seq_lengths_kv"],
               args["prefix_groups"], args["prefix_lengths"], args["query_rope"], args["key_rope"])
         monkeypatch.undo()
@@ -447,3 +447,46 @@ def test_strided_queries_and_other_tables(latent):
         got = dsa.paged_prefix_attention(**dict(args, query=wide[:, :, 2:-1], block_table=table.long()))
         for x, y in zip(got, want):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("i", range(len(GROUPED) + len(LATENT)))
+def test_short_prefixes_sequence_by_sequence(i):
+    """Families below min_tokens: each sequence for itself, the prefix from the pages of the family's first."""
+    latent = i >= len(GROUPED)
+    if latent:
+        N1, D, S1, page, dtype, families = LATENT[i - len(GROUPED)]
+        N2 = 1
+    else:
+        N1, N2, D, S1, page, dtype, families = GROUPED[i]
+    args, data, lens = _make(families, S1, N1, N2, D, page, DTYPES[dtype], latent, seed=i)
+    for least in (2 ** 40, 50):  # none together; some
+        _compare(dict(args, min_tokens=least), data, lens)
+
+
+@pytest.mark.parametrize("latent", [False, True])
+@pytest.mark.parametrize("shared", [64, 75])
+def test_sequence_by_sequence_is_paged_attention(latent, shared):
+    """Bit for bit where the tables name the same pages, and whatever the tables of the others name there."""
+    import dsa_triton_ascend_amd as dsa
+    families = [(0, shared, [330, 400, 20]), (1, 0, [500]), (2, shared, [77, 300])]
+    args, data, lens = _make(families, 1, page=16, dtype=torch.bfloat16, seed=8, **_form(latent))
+    a = dsa.paged_prefix_attention(**dict(args, min_tokens=1000))
+    if shared % 16:
+        _compare(args, data, lens, got=a)
+        return
+    table = args["block_table"].clone()
+    table[1:3, :shared // 16], table[5, :shared // 16] = table[0, :shared // 16], table[4, :shared // 16]
+    plain = {k: v for k, v in args.items() if not k.startswith("prefix") and k != "min_tokens"}
+    b = dsa.paged_attention(**dict(plain, block_table=table))
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+def test_prefixes_longer_than_the_table_and_min_tokens():
+    """A shared length past the table's room counts as the room, also against min_tokens."""
+    for latent in (False, True):
+        args, data, lens = _make([(0, 96, [96, 80, 50])], 1, page=16, dtype=torch.float16, seed=3, **_form(latent))
+        assert args["block_table"].shape[1] == 6
+        args["prefix_lengths"].fill_(2 ** 31 - 1)
+        for least in (1, 96, 97, 10 ** 6, None):
+            _compare(dict(args, min_tokens=least), data, lens)

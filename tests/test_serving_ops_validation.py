@@ -215,6 +215,9 @@ def _attn(latent=False, **kw):
     (dict(query=torch.zeros(3, 1, 8, 128)), "columns|dtype|must be"),
     (dict(query=torch.zeros(3, 8, 128, dtype=BF)), "query must be"),
     (dict(pre_tokens="x"), "pre_tokens|invalid literal"),
+    (dict(min_tokens=-1), "min_tokens"),
+    (dict(min_tokens=0.5), "min_tokens"),
+    (dict(min_tokens=2 ** 63), "min_tokens"),
     (dict(), "ROCm GPU device"),
 ])
 def test_prefix_attention_refuses(latent, kw, match):
@@ -248,11 +251,11 @@ def test_prefix_attention_has_no_backward(name):
     ({11: None}, "null"), ({12: None}, "null"), ({1: P}, "no rope parts"), ({4: None}, "query_rope and key_rope"),
     ({7: None}, "softmax_max and softmax_sum"), ({13: 0}, "batch"), ({13: 2 ** 24 + 1}, "batch"), ({14: 0}, "S1"),
     ({15: 7}, "divisible"), ({17: 96}, "D must be"), ({19: 0}, "at least one"), ({20: 0}, "page"),
-    ({21: 2 ** 20 + 1}, "max_blocks"), ({14: 2 ** 22}, "query rows"), ({22: 1}, "sparse_mode"), ({25: 2}, "dtype"),
-    ({28: None}, "workspace"), ({29: 100}, "workspace"), ({28: P + 8}, "16-byte"), ({0: P + 2}, "16-byte")])
+    ({21: 2 ** 20 + 1}, "max_blocks"), ({14: 2 ** 22}, "query rows"), ({22: 1}, "sparse_mode"), ({26: 2}, "dtype"),
+    ({29: None}, "workspace"), ({30: 100}, "workspace"), ({29: P + 8}, "16-byte"), ({0: P + 2}, "16-byte")])
 def test_prefix_attention_entry_refuses(change, message):
-    a = [P, None, P, None, P, P, P, P, None, P, P, P, P, 3, 1, 8, 2, 128, 0, 8, 16, 4, 3, 2 ** 62, 2 ** 62, 0, 0.1, 1,
-         P, 1 << 40, None]
+    a = [P, None, P, None, P, P, P, P, None, P, P, P, P, 3, 1, 8, 2, 128, 0, 8, 16, 4, 3, 2 ** 62, 2 ** 62, -1, 0, 0.1,
+         1, P, 1 << 40, None]
     for i, x in change.items():
         a[i] = x
     _c("dsa_paged_prefix_attn", a, message)
