@@ -63,7 +63,7 @@ struct PagedWhere {  // of a sequence, for the join
   int run0, runs, slot0, unused;   // its runs and the slot of the first
 };
 struct PagedJob {  // rows of a family, and tokens tok0 .. tok1 of its prefix
-  int first, row0, rows, unused;   // first sequence; rows from row0 on, of the family
+  int first, row0, rows, lead;     // first sequence; rows from row0 on; the sequence whose pages hold the prefix
   int tok0, tok1;
   int all_lo, all_hi;              // tokens that all rows of the family see
 };
@@ -75,7 +75,9 @@ struct PagedPrefixParams : PagedAttnParams {
   // rows of part_o / part_ml: behind those of the runs come, for each sequence,
   // one for what a run has of it if that is all of it, then those of the jobs
   int64_t whole0, part0;
-  int least;                    // tokens of a prefix from which on it is worked on for its family together
+  // tokens of a prefix, and sequences for a block of their rows, from which on a
+  // prefix is worked on for its family together
+  int least, worth;
   int prefix_workers;           // jobs of one key head aimed at
   int job_shift;                // log2 of the rows of a block
   unsigned rows_magic, group_magic, heads_magic;  // floor((2^32 - 1) / rows), of group, of n2
@@ -85,8 +87,8 @@ template <typename P> constexpr bool kPrefixed = std::is_same<P, PagedPrefixPara
 
 // whether sequence b has the family of the one before it
 __device__ __forceinline__ bool paged_linked(const PagedPrefixParams& p, int b) {
-  const int before = max(b - 1, 0), id = p.ids[b], n = p.shared[b];
-  return b > 0 && id >= 0 && n > 0 && p.ids[before] == id && p.shared[before] == n;
+  const int here = min(b, p.batch - 1), before = max(here - 1, 0), id = p.ids[here], n = p.shared[here];
+  return b == here && b > 0 && id >= 0 && n > 0 && p.ids[before] == id && p.shared[before] == n;
 }
 
 // the first sequence of the family that b is in, for a b that is the same on all lanes
@@ -97,13 +99,30 @@ __device__ __forceinline__ int paged_leader(const PagedPrefixParams& p, int b, i
   }
 }
 
-// Tokens that sequence b shares with the one before or behind it.
-__device__ __forceinline__ int paged_shared(const PagedPrefixParams& p, int b) {
-  const int before = max(b - 1, 0), behind = min(b + 1, p.batch - 1);
-  const int id = p.ids[b], n = p.shared[b];
-  const int id0 = p.ids[before], n0 = p.shared[before], id1 = p.ids[behind], n1 = p.shared[behind];
-  const bool links = (b > 0 && id0 == id && n0 == n) || (b + 1 < p.batch && id1 == id && n1 == n);
-  return id >= 0 && n > 0 && links ? min(n, p.max_blocks * p.page) : 0;
+// Whether the prefix of `tokens` tokens of a family of `count` sequences is worked on for all of them
+// together.
+__device__ __forceinline__ bool paged_together(const PagedPrefixParams& p, int tokens, int count) {
+  const int blocks = (count * p.rows + (1 << p.job_shift) - 1) >> p.job_shift;
+  return count > 1 && tokens >= p.least && count >= p.worth * blocks;
+}
+
+// Sequence b's family among the 64 sequences from a multiple of 64 on: where it
+// starts and how many they are.  What is worked on together is cut there, so
+// that a wave sees all of it at once.  b: the same on all lanes, or lane l's is
+// the l-th of the 64.
+struct PagedFamily {
+  int first, count;
+  bool linked;  // with any other, also of another 64
+};
+__device__ __forceinline__ PagedFamily paged_family(const PagedPrefixParams& p, int b) {
+  const int c0 = b & ~63, l = b & 63;
+  const unsigned long long all = __ballot(paged_linked(p, c0 + (int)(threadIdx.x & 63))), links = all & ~1ull;
+  PagedFamily f;
+  f.first = c0 + 63 - __clzll(~links & (~0ull >> (63 - l)));
+  const unsigned long long after = l == 63 ? 0ull : links >> (l + 1);
+  f.count = b - f.first + __ffsll(~after);
+  f.linked = f.count > 1 || (l == 0 && (all & 1)) || (l == 63 && paged_linked(p, b + 1));
+  return f;
 }
 
 // page and offset of a token.  t * magic / 2^32 is at most t / 2^32 below
@@ -158,8 +177,9 @@ __device__ __forceinline__ PagedSeqOf<P> paged_seq(const P& p, int b) {
   paged_bounds(p, s.act_q, s.act_k, 0, &s.lo, &h);
   paged_bounds(p, s.act_q, s.act_k, max(s.act_q - 1, 0), &l, &s.hi);
   if constexpr (kPrefixed<P>) {
-    s.given = paged_shared(p, b);
-    s.shared = s.given >= p.least ? s.given : 0;
+    const PagedFamily f = paged_family(p, b);
+    s.given = f.linked ? min(p.shared[b], p.max_blocks * p.page) : 0;
+    s.shared = paged_together(p, s.given, f.count) ? s.given : 0;
     s.given -= s.shared;
     s.lo = max(s.lo, s.shared);
   }

@@ -38,36 +38,13 @@ struct PrefixFamily {
   int first, count, tokens;  // sequences and shared tokens (0: none starts here)
 };
 
-// the families that start at sequences c0 .. c0 + 63, one per lane (all loads of
-// a lane at once: one after the other they take a microsecond each)
+// the families worked on together that start at sequences c0 .. c0 + 63, one per lane
 __device__ __forceinline__ PrefixFamily prefix_families(const PagedPrefixParams& p, int c0, int lane) {
-  const int last = p.batch - 1, b = c0 + lane;
-  const int i0 = min(max(b - 1, 0), last), i1 = min(b, last), i2 = min(b + 1, last);
-  const int id0 = p.ids[i0], id1 = p.ids[i1], id2 = p.ids[i2];
-  const int n0 = p.shared[i0], n1 = p.shared[i1], n2 = p.shared[i2];
-  const int room = p.max_blocks * p.page;
-  const bool shares = id1 >= 0 && min(n1, room) >= p.least;
-  const bool mine = shares && b > 0 && b <= last && id0 == id1 && n0 == n1;  // linked to the sequence before it
-  const bool next = shares && b < last && id1 == id2 && n1 == n2;
-  const unsigned long long links = __ballot(mine);
-  PrefixFamily f = {b, 0, 0};
-  if (next && !mine) {
-    const unsigned long long after = lane == 63 ? 0ull : links >> (lane + 1);
-    f.count = __ffsll(~after);  // the links that follow, and the first sequence
-    f.tokens = min(n1, room);
-  }
-  // a family that goes on behind these
-  bool open = f.count > 0 && lane + f.count == 64 && b + f.count < p.batch;
-  for (int e = c0 + 64; __any(open); e += 64) {
-    const int j = min(e + lane, last), id = p.ids[j], n = p.shared[j];
-    const bool linked = e + lane <= last && id >= 0 && min(n, room) >= p.least && id == p.ids[j - 1] &&
-                        n == p.shared[j - 1];
-    const unsigned long long more = __ballot(linked);
-    const int k = ~more ? __ffsll(~more) - 1 : 64;
-    if (open) f.count += k;
-    open = open && k == 64;
-  }
-  return f;
+  const int b = c0 + lane;
+  const PagedFamily f = paged_family(p, b);
+  const int tokens = min(p.shared[min(b, p.batch - 1)], p.max_blocks * p.page);
+  const bool here = f.first == b && paged_together(p, tokens, f.count);
+  return {b, here ? f.count : 0, here ? tokens : 0};
 }
 
 // n / d with magic = floor((2^32 - 1) / d): n * magic / 2^32 is at most
@@ -193,20 +170,9 @@ struct PrefixPlan {
         const int np = __builtin_amdgcn_readlane(parts, l), nj = __builtin_amdgcn_readlane(n, l);
         const int job0 = job_base + __builtin_amdgcn_readlane(incl, l) - nj;
         const bool in = lane >= l && lane < l + count;
-        int lo = in ? seen_lo : 0x7fffffff, hi = in ? seen_hi : 0, alo = in ? all_lo : 0, ahi = in ? all_hi : 0x7fffffff;
-        for (int e = c0 + 64 + lane; e < first + count; e += 64) {  // (sequences of the next 64s)
-          const PagedSeqBehind s = paged_seq(p, e);
-          int l0, h0, l1, h1;
-          paged_bounds(p, s.act_q, s.act_k, 0, &l0, &h0);
-          paged_bounds(p, s.act_q, s.act_k, max(s.act_q - 1, 0), &l1, &h1);
-          if (s.act_q > 0) lo = min(lo, l0), hi = max(hi, h1);
-          alo = max(alo, l1);  // (a row behind the last new token sees nothing: all_hi is 0 then)
-          ahi = min(ahi, s.act_q == p.s1 ? h0 : 0);
-        }
-        lo = wave_min_int(lo);
-        hi = min(-wave_min_int(-hi), tokens);
-        alo = -wave_min_int(-alo);
-        ahi = wave_min_int(ahi);
+        const int lo = wave_min_int(in ? seen_lo : 0x7fffffff), hi = min(-wave_min_int(in ? -seen_hi : 0), tokens);
+        const int alo = -wave_min_int(in ? -all_lo : 0), ahi = wave_min_int(in ? all_hi : 0x7fffffff);
+        const int lead = first == c0 ? paged_leader(p, first, lane) : first;
         // parts of equal numbers of whole tiles, cut to what is seen
         const int each = prefix_div_up((tokens + kPrefixTile - 1) / kPrefixTile, np) * kPrefixTile;
         for (int j = lane; j < nj; j += 64) {
@@ -215,7 +181,7 @@ struct PrefixPlan {
           q.first = first;
           q.row0 = block << p.job_shift;
           q.rows = min(count * p.rows - q.row0, 1 << p.job_shift);
-          q.unused = 0;
+          q.lead = lead;
           q.tok0 = max(part * each, lo);
           q.tok1 = min(part * each + each, hi);
           q.all_lo = alo;

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
     }
     const unsigned char* const kbase = (const unsigned char*)p.k + (int64_t)head * ROW;
     const unsigned char* const vbase = (const unsigned char*)p.v + (int64_t)head * ROW;
-    const int32_t* const tab = p.table + (int64_t)first * p.max_blocks;
+    const int32_t* const tab = p.table + (int64_t)jb.lead * p.max_blocks;
 
     for (int ta = tok0; ta < tok1;) {
       // the pages of as many tokens as the LDS holds entries for, in whole tiles
@@ -484,9 +484,13 @@ static int prefix_grouped_launch(const PagedPrefixParams& p, int64_t d, int32_t 
 }
 
 // Tokens of a prefix from which on it is worked on for its family together.
-static int prefix_least(int64_t min_tokens) {
-  if (min_tokens >= 0) return (int)(min_tokens < 1 ? 1 : (min_tokens > 0x7fffffff ? 0x7fffffff : min_tokens));
-  return 1;
+static int prefix_least(int64_t min_tokens, int64_t batch, int64_t rows, int64_t token_bytes, bool latent) {
+  constexpr int64_t never = 0x7fffffff;
+  if (min_tokens < 0) {
+    if (latent && rows >= 64) return (int)never;
+    min_tokens = (latent ? 320ll << 20 : 256ll << 20) / (batch * token_bytes);
+  }
+  return (int)(min_tokens < 1 ? 1 : (min_tokens < never ? min_tokens : never));
 }
 
 int paged_prefix_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
@@ -510,7 +514,8 @@ int paged_prefix_run(const void* query, const void* query_rope, const void* key,
   p.part0 = p.whole0 + prefix_whole_rows(s, batch);
   p.ids = ids;
   p.shared = shared;
-  p.least = prefix_least(min_tokens);
+  p.least = prefix_least(min_tokens, batch, p.rows, (int64_t)(latent ? d + 64 : 2 * n2 * d) * 2, latent);
+  p.worth = min_tokens >= 0 ? 0 : (latent ? 2 : 4);
   p.prefix_workers = s.workers;
   p.job_shift = s.shift;
   p.rows_magic = 0xffffffffu / (unsigned)p.rows;

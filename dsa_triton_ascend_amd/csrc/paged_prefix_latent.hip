@@ -108,7 +108,7 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
         continue;
       }
     }
-    const int32_t* tab = p.table + (int64_t)first * p.max_blocks;
+    const int32_t* tab = p.table + (int64_t)jb.lead * p.max_blocks;
 
     // the run's pages, as many as the LDS holds at a time, a thread's each
     int ta = tok0, tb, pg0, page_entry;

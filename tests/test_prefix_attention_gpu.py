@@ -490,3 +490,25 @@ def test_prefixes_longer_than_the_table_and_min_tokens():
         args["prefix_lengths"].fill_(2 ** 31 - 1)
         for least in (1, 96, 97, 10 ** 6, None):
             _compare(dict(args, min_tokens=least), data, lens)
+
+
+@pytest.mark.parametrize("latent,N1,N2,D", [(False, 32, 8, 128), (True, 16, 1, 512), (True, 64, 1, 512)])
+def test_families_chosen_by_size(latent, N1, N2, D):
+    """Without min_tokens: long prefixes of many, of few and of two, short ones, and sequences alone, in one batch."""
+    P = 4800 if latent else 2400
+    families = [(0, P, [P + 17 * i for i in range(33)]), (1, P + 16, [P + 20, P + 90]), (2, 160, [170 + i for i in range(20)]),
+                (-1, 50, [300]), (3, P - 16, [P, P + 3, P + 100, P - 500, P + 40])]
+    args, data, lens = _make(families, 1, N1, N2, D, 16, torch.bfloat16, latent, seed=4)
+    _compare(dict(args, min_tokens=None), data, lens)
+
+
+@pytest.mark.parametrize("latent", [False, True])
+@pytest.mark.parametrize("before", [0, 1, 40, 62, 63, 64])
+@pytest.mark.parametrize("least", [1, 1000])
+def test_families_across_64s(latent, before, least):
+    """Together in parts of 64 sequences, and for each, the prefix in the pages of the first of all."""
+    families = [(-1, 0, [10 + i % 3 for i in range(before)]), (0, 48, [50 + i % 40 for i in range(90)]),
+                (1, 32, [33, 40])]
+    form = dict(latent=latent, D=128, N1=2, N2=1)
+    args, data, lens = _make([f for f in families if f[2]], 1, page=16, dtype=torch.bfloat16, seed=6, **form)
+    _compare(dict(args, min_tokens=least), data, lens)

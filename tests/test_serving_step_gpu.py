@@ -156,11 +156,13 @@ def _loop(dsa, latent, dtype, heads):
                     x[r, :n] = y[ends[r]:ends[r] + n]
         args = m.attend(pad[0], pad[1], table, lens, groups, shared, _ints(counts))
         _compare(args, history, after, act_q=counts)
+        _compare(dict(args, min_tokens=1), history, after, act_q=counts)
     assert waited  # some request was refused and waited in place
 
 
 @pytest.mark.parametrize("latent,dtype,heads", [(False, torch.bfloat16, 8), (True, torch.float16, 16)])
-def test_captured_decoding_step(latent, dtype, heads):
+@pytest.mark.parametrize("least", [None, 1])
+def test_captured_decoding_step(latent, dtype, heads, least):
     """A decoding step whose state stays on the device, replayed beside the same steps made eagerly."""
     import dsa_triton_ascend_amd as dsa
     pages, wide, rows = 40, 8, 4
@@ -182,7 +184,7 @@ def test_captured_decoding_step(latent, dtype, heads):
         dsa.paged_cache_write_slots(m.caches, rows_, slots)
         groups, shared = dsa.paged_cache_prefixes(state[0], state[1], PAGE)
         return dsa.paged_prefix_attention(**m.attend(a[:, None], None if b is None else b[:, None], state[0], state[1],
-                                                     groups, shared))
+                                                     groups, shared), min_tokens=least)
 
     inputs = [[torch.randn_like(x.float()).to(dtype) for x in (q, qr, *kv) if x is not None] for _ in range(12)]
 
