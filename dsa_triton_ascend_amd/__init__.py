@@ -14,6 +14,10 @@ Public API, mirroring the reference's operator modules:
 * around one decoding step: ``rotary_embedding`` / ``RotaryEmbedding``
   (with ``rotary_frequencies``), ``paged_cache_write`` / ``paged_cache_fork`` /
   ``paged_cache_compact``, and ``paged_attention`` / ``PagedAttention``
+* for requests of many lengths: ``paged_cache_plan`` and
+  ``paged_cache_write_slots``; for those that share a prefix:
+  ``paged_cache_prefixes`` and ``paged_prefix_attention`` /
+  ``PagedPrefixAttention``
 
 and the autograd pairing for training (``autograd.py``):
 ``sparse_flash_attention_train`` / ``SparseFlashAttentionFunction`` and

@@ -99,8 +99,8 @@ __device__ __forceinline__ int paged_leader(const PagedPrefixParams& p, int b, i
   }
 }
 
-// Whether the prefix of `tokens` tokens of a family of `count` sequences is worked on for all of them
-// together.
+// Whether the prefix of a family of `count` sequences is worked on for all of
+// them together (paged_prefix.h).
 __device__ __forceinline__ bool paged_together(const PagedPrefixParams& p, int tokens, int count) {
   const int blocks = (count * p.rows + (1 << p.job_shift) - 1) >> p.job_shift;
   return count > 1 && tokens >= p.least && count >= p.worth * blocks;
@@ -238,7 +238,7 @@ struct PagedPlan {
     total = __builtin_amdgcn_readlane(incl, 63);
     if (p.batch > 64) {
       int n = 0;
-#pragma unroll 4
+#pragma unroll (kPrefixed<P> ? 1 : 4)
       for (int b = 64 + lane; b < p.batch; b += 64) n += paged_tiles(paged_seq(p, b), tile);
       total += wave_total(n);
     }
@@ -247,7 +247,7 @@ struct PagedPlan {
     if (p.batch > p.workers) return;
     for (int g = per; g <= per + kPaSlack; g += kPaSlack) {
       int n = (int)((unsigned)(tiles + g - 1) / (unsigned)g);
-#pragma unroll 4
+#pragma unroll (kPrefixed<P> ? 1 : 4)
       for (int b = 64 + lane; b < p.batch; b += 64)
         n += (int)((unsigned)(paged_tiles(paged_seq(p, b), tile) + g - 1) / (unsigned)g);
       const int runs = wave_total(n);
@@ -307,7 +307,7 @@ struct PagedPlan {
   __device__ __forceinline__ int start(const P& p, int tile, int lane, int b) const {
     if (b < 64) return b ? __builtin_amdgcn_readlane(incl, b - 1) : 0;
     int n = 0;
-#pragma unroll 4
+#pragma unroll (kPrefixed<P> ? 1 : 4)
     for (int i = lane; i < b; i += 64) n += padded(paged_tiles(paged_seq(p, i), tile));
     return wave_total(n);
   }

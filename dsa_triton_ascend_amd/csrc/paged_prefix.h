@@ -6,8 +6,31 @@
 // queries of all of a family's sequences attend over the prefix together, so
 // that a token of it is read once for all of them and the products have
 // hundreds of rows; what each sequence has behind the prefix goes the way of
-// paged_attn.h.  paged_combine_kernel joins both: every part of a row comes as
-// a reference, a sum and an unnormalised output, as the runs there.
+// paged_attn.h.  paged_combine_kernel joins both: every part i of a row comes as
+// a reference, a sum and an unnormalised output, as the runs there,
+//
+//   O = (sum_i 2^(ref_i - m) O_i) / (sum_i 2^(ref_i - m) n_i),  m = max_i ref_i
+//
+// all in 32 bits (the parts in memory too).
+//
+// Which families.  Together costs a launch more, and outputs of 32 bits that are
+// written and joined: 6 to 10 us with grouped heads, 15 to 20 over the latent
+// cache.  Apart costs the reading of the prefix by every sequence, from the
+// caches for the most part, at some 13 TB/s.  So a prefix has to be so long
+// that all sequences of the batch would read 256 MB (latent: 320 MB) of it.  Measured
+// with one family, us, apart and together, at 8 key heads of 128 columns and
+// eight query heads on each: 32 sequences behind 2048 tokens 38.7 and 40.6,
+// behind 8192 94 and 48, behind 32768 322 and 69; 8 behind 2048 24 and 28,
+// behind 8192 41 and 33.  16 latent heads: 32 sequences behind 8192 tokens 57
+// and 60, behind 32768 162 and 81; 64 behind 8192 94 and 72.
+// With many families what counts is the rows: a block of 256 rows takes
+// 1.3 ns a token over the whole device, a sequence alone 0.3 (latent: 128 rows 0.3, 16 to 32
+// heads 0.15), so a family needs four (two) sequences for each of its blocks.
+// From 64 latent rows of a sequence on its own products bound it, and together
+// is never faster (128 heads, 32 sequences behind 32768 tokens: 301 and 312; 64 heads 188
+// and 178).  The caller may set the length instead.
+// What is not worked on together each sequence reads for itself (paged_attn.h),
+// from the pages of the family's first, 1 to 4 us slower than paged_attention.
 //
 // Work.  A job is a block of up to R rows of a family (over its sequences, new
 // tokens and the query heads of one key head) and a part of its prefix.  Parts
@@ -17,6 +40,7 @@
 // found on the device from the ids and lengths, by one wave beside the kernel of
 // paged_attn.h, which runs first: found by every workgroup for itself it took
 // 8 us of each (most of it instructions that had to be fetched first).
+// Families are cut at multiples of 64 sequences, so that a wave sees them whole.
 #pragma once
 
 #include "paged_attn.h"
@@ -25,7 +49,7 @@ namespace dsa {
 
 constexpr int kPrefixTile = 32;  // tokens
 constexpr int kPrefixMinTiles = 2;  // fewest tiles of a part
-constexpr float kPrefixPartTiles = 18.f;
+constexpr float kPrefixPartTiles = 18.f;  // jobs whose outputs cost what a tile of all of them does
 
 // jobs of one key head for `m` blocks of rows: as many as there are workers, or
 // (where the blocks alone are more than half of them) whole rounds of workers,
@@ -75,11 +99,14 @@ struct PrefixPlan {
     t = (f.tokens + kPrefixTile - 1) / kPrefixTile;
   }
 
-  // Fewest tiles of a part.  A part more costs the writing and joining of its
-  // output, so long as PREFIX_TILES tiles take: J jobs cost J + 18 W / J of that for W tiles in all.
+  // Fewest tiles of a part.  J jobs of W tiles in all take about W / J tiles'
+  // time, and the writing and joining of their outputs J / 18 of it (full
+  // blocks): least for J = sqrt(18 W).  (16 latent heads, 8 sequences behind 8192
+  // tokens: 51 us with 64 jobs, 57 with 128.)
   __device__ __forceinline__ int least(const PagedPrefixParams& p, int work, int blocks, int rows) const {
     const float fill = (float)rows / (float)(max(blocks, 1) << p.job_shift);
-    return max((int)__builtin_sqrtf((float)work * (float)p.n2 * fill * (1.f / kPrefixPartTiles) + 0.5f), kPrefixMinTiles);
+    const float tiles = __builtin_sqrtf((float)work * (float)p.n2 * fill * (1.f / kPrefixPartTiles) + 0.5f);
+    return max((int)tiles, kPrefixMinTiles);
   }
 
   // sum m ceil(t / per) may be `most` jobs.  Up to 64 sequences the length of

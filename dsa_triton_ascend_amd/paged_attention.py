@@ -70,10 +70,16 @@ def paged_prefix_attention(query, key, value, block_table, actual_seq_lengths_kv
     pages of each sequence.  A negative group, a length of 0 and a sequence
     alone share nothing.  The prefix may end inside a page and may be longer
     than some of the sequences.  Results are those of ``paged_attention`` where the
-    sequences' rows of the table name the same pages for the prefix, rounded
-    once more in the weights: the numerators of a prefix are rounded to the
-    input type in both forms.  A value of the prefix that one row of a family
-    sees and another does not must be finite.
+    sequences' rows of the table name the same pages for the prefix, up to the
+    rounding of the softmax's numerators to the input type, which prefixes that
+    are worked on together have in both forms.  A value of the prefix that one
+    row of a family sees and another does not must be finite.
+
+    ``min_tokens``: the shortest prefix that is worked on for its family
+    together; shorter ones each sequence reads for itself, which is faster for
+    short prefixes and small families.  None: chosen from the sizes (32 sequences
+    of eight key heads of 128 columns from 2048 tokens on, of 16 latent heads
+    from 9102; with 64 latent heads and more, never: their products bound it).
 
     Everything else as in ``paged_attention``.
     """

@@ -583,6 +583,8 @@ int dsa_paged_attn(const void* query, const void* query_rope, const void* key, c
  * share nothing, whatever their length says.  Results are those of dsa_paged_attn
  * where the sequences' tables name the same pages for the prefix.  A value of the
  * prefix that one row of a family sees and another does not must be finite.
+ * min_tokens: prefixes of fewer tokens are read by each sequence for itself;
+ * negative: chosen from the sizes.
  * Everything else as dsa_paged_attn; the query rows and the tiles of 32 tokens of a
  * table row are fewer than 2^31 as a product.
  */
