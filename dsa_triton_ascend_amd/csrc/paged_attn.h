@@ -75,9 +75,7 @@ struct PagedPrefixParams : PagedAttnParams {
   // rows of part_o / part_ml: behind those of the runs come, for each sequence,
   // one for what a run has of it if that is all of it, then those of the jobs
   int64_t whole0, part0;
-  // tokens of a prefix, and sequences for a block of their rows, from which on a
-  // prefix is worked on for its family together
-  int least, worth;
+  int least;  // tokens of a prefix from which on it is worked on for its family together
   int prefix_workers;           // jobs of one key head aimed at
   int job_shift;                // log2 of the rows of a block
   unsigned rows_magic, group_magic, heads_magic;  // floor((2^32 - 1) / rows), of group, of n2
@@ -102,8 +100,7 @@ __device__ __forceinline__ int paged_leader(const PagedPrefixParams& p, int b, i
 // Whether the prefix of a family of `count` sequences is worked on for all of
 // them together (paged_prefix.h).
 __device__ __forceinline__ bool paged_together(const PagedPrefixParams& p, int tokens, int count) {
-  const int blocks = (count * p.rows + (1 << p.job_shift) - 1) >> p.job_shift;
-  return count > 1 && tokens >= p.least && count >= p.worth * blocks;
+  return count > 1 && tokens >= p.least;
 }
 
 // Sequence b's family among the 64 sequences from a multiple of 64 on: where it

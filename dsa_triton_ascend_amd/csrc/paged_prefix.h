@@ -15,20 +15,19 @@
 //
 // Which families.  Together costs a launch more, and outputs of 32 bits that are
 // written and joined: 6 to 10 us with grouped heads, 15 to 20 over the latent
-// cache.  Apart costs the reading of the prefix by every sequence, from the
-// caches for the most part, at some 13 TB/s.  So a prefix has to be so long
-// that all sequences of the batch would read 256 MB (latent: 320 MB) of it.  Measured
-// with one family, us, apart and together, at 8 key heads of 128 columns and
-// eight query heads on each: 32 sequences behind 2048 tokens 38.7 and 40.6,
-// behind 8192 94 and 48, behind 32768 322 and 69; 8 behind 2048 24 and 28,
-// behind 8192 41 and 33.  16 latent heads: 32 sequences behind 8192 tokens 57
-// and 60, behind 32768 162 and 81; 64 behind 8192 94 and 72.
-// With many families what counts is the rows: a block of 256 rows takes
-// 1.3 ns a token over the whole device, a sequence alone 0.3 (latent: 128 rows 0.3, 16 to 32
-// heads 0.15), so a family needs four (two) sequences for each of its blocks.
+// cache.  Apart costs the reading of the prefix by every sequence (and every
+// row group of one), from the caches for the most part.  So a prefix has to be
+// so long that the whole batch would read 256 MB (latent: 320 MB) of it.
+// Measured, us, apart and together, 8 key heads of 128 columns and eight query
+// heads on each: 32 sequences behind 2048 tokens 38.7 and 40.6, behind 8192 94
+// and 48, behind 32768 322 and 69; 8 behind 2048 24 and 28, behind 8192 41 and 33;
+// 16 families of two behind 4096 94 and 77, behind 16384 313 and 225; 16 new tokens of
+// 16 sequences behind 2048 85 and 76.  16 latent heads: 32 sequences behind 8192 tokens
+// 57 and 60, behind 32768 162 and 81; 64 behind 8192 94 and 72; 16 families of
+// two behind 16384 96 and 103.
 // From 64 latent rows of a sequence on its own products bound it, and together
-// is never faster (128 heads, 32 sequences behind 32768 tokens: 301 and 312; 64 heads 188
-// and 178).  The caller may set the length instead.
+// is hardly faster or slower (128 heads, 32 sequences behind 32768 tokens: 301
+// and 312; 64 heads 188 and 178).  The caller may set the length instead.
 // What is not worked on together each sequence reads for itself (paged_attn.h),
 // from the pages of the family's first, 1 to 4 us slower than paged_attention.
 //

@@ -504,12 +504,10 @@ static int prefix_grouped_launch(const PagedPrefixParams& p, int64_t d, int32_t 
 
 // Tokens of a prefix from which on it is worked on for its family together
 // (described in paged_prefix.h).
-static int prefix_least(int64_t min_tokens, int64_t batch, int64_t rows, int64_t token_bytes, bool latent) {
+static int prefix_least(int64_t min_tokens, int64_t rows, int64_t readers, int64_t token_bytes, bool latent) {
   constexpr int64_t never = 0x7fffffff;
-  if (min_tokens < 0) {
-    if (latent && rows >= 64) return (int)never;
-    min_tokens = (latent ? 320ll << 20 : 256ll << 20) / (batch * token_bytes);
-  }
+  if (min_tokens < 0)
+    min_tokens = latent && rows >= 64 ? never : (latent ? 320 << 20 : 256 << 20) / (readers * token_bytes);
   return (int)(min_tokens < 1 ? 1 : (min_tokens < never ? min_tokens : never));
 }
 
@@ -534,8 +532,7 @@ int paged_prefix_run(const void* query, const void* query_rope, const void* key,
   p.part0 = p.whole0 + prefix_whole_rows(s, batch);
   p.ids = ids;
   p.shared = shared;
-  p.least = prefix_least(min_tokens, batch, p.rows, (int64_t)(latent ? d + 64 : 2 * n2 * d) * 2, latent);
-  p.worth = min_tokens >= 0 ? 0 : (latent ? 2 : 4);
+  p.least = prefix_least(min_tokens, p.rows, batch * p.row_groups, (latent ? d + 64 : 2 * n2 * d) * 2, latent);
   p.prefix_workers = s.workers;
   p.job_shift = s.shift;
   p.rows_magic = 0xffffffffu / (unsigned)p.rows;
