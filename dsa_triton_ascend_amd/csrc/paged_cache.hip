@@ -1,5 +1,6 @@
 // Pages of a cache: writing new tokens' rows, forking / releasing / extending
-// the block table's rows, and compaction.
+// the block table's rows, planning a step of rows of many lengths, finding the
+// prefixes that rows share, and compaction.
 //
 // A cache is [pages, page_size, row]; several caches (latent, rope, indexer
 // keys, of several layers) share one block table, and one call moves the rows
@@ -14,7 +15,9 @@
 // Bound by the launches for one step's tables (a fork of 16 rows: 3.8 + 4.8 us
 // for its two kernels, a write of 32 rows 3.9, of 8192 rows 8.4), by memory
 // where pages move (half of a 740 MB pool in use: 369 MB read and written in
-// 76.5 us, 4.8 TB/s; a large copy reaches 4.9).
+// 76.5 us, 4.8 TB/s; a large copy reaches 4.9).  A plan of 256 rows over 85000
+// pages takes 5.5 + 3.6 us, writing 8192 rows of a plan 6.9 (22 MB; one
+// dependent read less than a write that searches the tables, 8.4).
 #include "common.h"
 
 namespace dsa {

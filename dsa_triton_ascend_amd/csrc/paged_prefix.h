@@ -20,11 +20,11 @@
 // so long that the whole batch would read 256 MB (latent: 320 MB) of it.
 // Measured, us, apart and together, 8 key heads of 128 columns and eight query
 // heads on each: 32 sequences behind 2048 tokens 38.7 and 40.6, behind 8192 94
-// and 48, behind 32768 322 and 69; 8 behind 2048 24 and 28, behind 8192 41 and 33;
-// 16 families of two behind 4096 94 and 77, behind 16384 313 and 225; 16 new tokens of
-// 16 sequences behind 2048 85 and 76.  16 latent heads: 32 sequences behind 8192 tokens
-// 57 and 60, behind 32768 162 and 81; 64 behind 8192 94 and 72; 16 families of
-// two behind 16384 96 and 103.
+// and 48, behind 32768 322 and 69; 8 behind 2048 24 and 28, behind 8192 41 and
+// 33; 16 families of two behind 4096 94 and 77, behind 16384 313 and 225; 16 new
+// tokens of 16 sequences behind 2048 85 and 76.  16 latent heads: 32 sequences
+// behind 8192 tokens 57 and 60, behind 32768 162 and 81; 64 behind 8192 94 and
+// 72; 16 families of two behind 16384 96 and 103.
 // From 64 latent rows of a sequence on its own products bound it, and together
 // is hardly faster or slower (128 heads, 32 sequences behind 32768 tokens: 301
 // and 312; 64 heads 188 and 178).  The caller may set the length instead.

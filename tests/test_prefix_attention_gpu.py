@@ -512,3 +512,14 @@ def test_families_across_64s(latent, before, least):
     form = dict(latent=latent, D=128, N1=2, N2=1)
     args, data, lens = _make([f for f in families if f[2]], 1, page=16, dtype=torch.bfloat16, seed=6, **form)
     _compare(dict(args, min_tokens=least), data, lens)
+
+
+def test_families_chosen_by_size_of_large_batches():
+    """More sequences than a wave has lanes, families that go on behind the 64th, prefixes just long enough and not."""
+    B, token_bytes = 130, 4096
+    least = (256 << 20) // (B * token_bytes)
+    families = [(0, least + 8, [least + 10 + i for i in range(70)]), (1, least - 8, [least + i for i in range(20)]),
+                (2, least + 1, [least + 40 - 3 * i for i in range(38)]), (3, 2 * least, [2 * least + 5] * 2)]
+    assert sum(len(m) for _, _, m in families) == B
+    args, data, lens = _make(families, 1, 16, 8, 128, 16, torch.bfloat16, False, seed=9)
+    _compare(dict(args, min_tokens=None), data, lens)
