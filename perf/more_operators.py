@@ -267,8 +267,8 @@ def prepare(case, seed):
         wide = max(total)
         st["table"] = _ints([r + [-1] * (wide - len(r)) for r in table])
         st["lens"], st["lens_host"] = _ints(lens), lens
-        # what the plan of a step gives: each sequence's family and the tokens of the full pages that it shares
-        st["groups"], st["shared"] = _ints(leader), _ints([n // page * page for n in shared])
+        # what the plan of a step gives: each sequence's family and the tokens it shares
+        st["groups"], st["shared"] = _ints(leader), _ints(shared)
         # queries of twice the keys' spread: the softmax settles on a few hundred of 32K tokens
         st["q"] = normal(len(lens), case["q"], case["heads"], d) * 2
         st["k"] = normal(pool, page, n2, d)
