@@ -135,12 +135,37 @@ __device__ __forceinline__ unsigned paged_split(const PagedAttnParams& p, unsign
   return q;
 }
 
+// The tokens of a prefix that are worked on together: its whole pages, since a
+// sequence may have the page in which it ends for itself; all of one that ends in
+// its first page.
+__device__ __forceinline__ int paged_whole_pages(const PagedAttnParams& p, int tokens) {
+  if (tokens <= p.page) return tokens;
+  unsigned off;
+  paged_split(p, (unsigned)tokens, &off);
+  return tokens - (int)off;
+}
+
+// How many of a prefix's tokens a sequence has in the pages of its family's first:
+// all but those of the page in which the prefix ends, where its own row of the table
+// (`own`) names the same page as the first's for the last whole one.  Then it has a
+// page of its own there, as after a fork, which copies a page that is partly filled;
+// rows that leave the prefix out hold anything else.
+__device__ __forceinline__ int paged_given(const PagedAttnParams& p, int tokens, const int32_t* own,
+                                           const int32_t* first) {
+  const int whole = paged_whole_pages(p, tokens);
+  if (whole == tokens) return tokens;
+  unsigned off;
+  const unsigned last = paged_split(p, (unsigned)whole, &off) - 1;
+  const int e = own[last];
+  return e == first[last] && e >= 0 && (int64_t)e * p.page < p.kv_rows ? whole : tokens;
+}
+
 struct PagedSeq {
   int act_q, act_k, lo, hi;  // lo <= t < hi: tokens that any row sees (with a prefix: behind it)
 };
 struct PagedSeqBehind : PagedSeq {
   int shared;  // tokens of the prefix before it
-  int given;   // tokens of its own that are in the pages of its family's first sequence
+  int given;   // where it reads some of the prefix itself: the prefix's tokens (paged_given)
 };
 template <typename P> using PagedSeqOf = std::conditional_t<kPrefixed<P>, PagedSeqBehind, PagedSeq>;
 // whether a sequence has a prefix before it
@@ -175,9 +200,10 @@ __device__ __forceinline__ PagedSeqOf<P> paged_seq(const P& p, int b) {
   paged_bounds(p, s.act_q, s.act_k, max(s.act_q - 1, 0), &l, &s.hi);
   if constexpr (kPrefixed<P>) {
     const PagedFamily f = paged_family(p, b);
-    s.given = f.linked ? min(p.shared[b], p.max_blocks * p.page) : 0;
-    s.shared = paged_together(p, s.given, f.count) ? s.given : 0;
-    s.given -= s.shared;
+    const int tokens = f.linked ? min(p.shared[b], p.max_blocks * p.page) : 0;
+    const int whole = paged_whole_pages(p, tokens);
+    s.shared = paged_together(p, whole, f.count) ? whole : 0;
+    s.given = s.shared == tokens ? 0 : tokens;
     s.lo = max(s.lo, s.shared);
   }
   if (s.hi < s.lo) s.hi = s.lo;

@@ -89,7 +89,10 @@ __global__ __launch_bounds__(kPaThreads, pa_waves(D, MT)) void paged_attn_kernel
     const int tok0 = seq.lo + t0 * kPaTile, tok1 = min(seq.hi, seq.lo + t1 * kPaTile);
     const int32_t *tab = p.table + (int64_t)b * p.max_blocks, *lead = tab;
     if constexpr (kPrefixed<P>)
-      if (__any(seq.given)) lead = p.table + (int64_t)paged_leader(p, b, lane) * p.max_blocks;
+      if (__any(seq.given)) {
+        lead = p.table + (int64_t)paged_leader(p, b, lane) * p.max_blocks;
+        seq.given = paged_given(p, seq.given, tab, lead);
+      }
 
     // rows of this lane's MFMA column: query head kvh * group + r % group of
     // token r / group

@@ -190,7 +190,10 @@ __global__ __launch_bounds__(kPlThreads, 1) void paged_latent_kernel(P p) {
     const int tok0 = seq.lo + t0 * TILE, tok1 = min(seq.hi, seq.lo + t1 * TILE);
     const int32_t *tab = p.table + (int64_t)b * p.max_blocks, *lead = tab;
     if constexpr (kPrefixed<P>)
-      if (__any(seq.given)) lead = p.table + (int64_t)paged_leader(p, b, ln) * p.max_blocks;
+      if (__any(seq.given)) {
+        lead = p.table + (int64_t)paged_leader(p, b, ln) * p.max_blocks;
+        seq.given = paged_given(p, seq.given, tab, lead);
+      }
 
     // the run's pages, as many as the LDS holds at a time, a thread's each
     int ta = tok0, tb, pg0, page_entry;

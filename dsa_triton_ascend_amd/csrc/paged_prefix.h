@@ -2,7 +2,8 @@
 // grouped-head and the shared-latent kernels have in common.
 //
 // A family is a run of neighbouring sequences with the same id and the same
-// shared length; its prefix lies in the pages of its first sequence.  The
+// shared length; its prefix lies in the pages of its first sequence, but for the
+// page in which it ends, which each sequence may have for itself (paged_given).  The
 // queries of all of a family's sequences attend over the prefix together, so
 // that a token of it is read once for all of them and the products have
 // hundreds of rows; what each sequence has behind the prefix goes the way of
@@ -65,7 +66,7 @@ struct PrefixFamily {
 __device__ __forceinline__ PrefixFamily prefix_families(const PagedPrefixParams& p, int c0, int lane) {
   const int b = c0 + lane;
   const PagedFamily f = paged_family(p, b);
-  const int tokens = min(p.shared[min(b, p.batch - 1)], p.max_blocks * p.page);
+  const int tokens = paged_whole_pages(p, min(p.shared[min(b, p.batch - 1)], p.max_blocks * p.page));
   const bool here = f.first == b && paged_together(p, tokens, f.count);
   return {b, here ? f.count : 0, here ? tokens : 0};
 }

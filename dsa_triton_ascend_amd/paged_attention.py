@@ -68,8 +68,12 @@ def paged_prefix_attention(query, key, value, block_table, actual_seq_lengths_kv
     ``paged_cache_prefixes``): the first ``prefix_lengths`` tokens of each are
     those in the pages of the family's first sequence; what follows is in the
     pages of each sequence.  A negative group, a length of 0 and a sequence
-    alone share nothing.  The prefix may end inside a page and may be longer
-    than some of the sequences.  Results are those of ``paged_attention`` where the
+    alone share nothing.  The prefix may be longer than some of the sequences,
+    and may end inside a page: a sequence whose row of the table names the same
+    page as the first's for the prefix's last whole page has what is in the page
+    behind it in its own (as after a fork, which copies a page that is partly
+    filled), every other one, and all where the prefix ends in its first page,
+    in the first's.  Results are those of ``paged_attention`` where the
     sequences' rows of the table name the same pages for the prefix, up to the
     rounding of the softmax's numerators to the input type, which prefixes that
     are worked on together have in both forms.  A value of the prefix that one

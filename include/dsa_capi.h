@@ -579,7 +579,10 @@ int dsa_paged_attn(const void* query, const void* query_rope, const void* key, c
  * neighbouring sequences with the same prefix_groups entry (at least 0) and the
  * same prefix_lengths entry (at least 1): their first prefix_lengths tokens are
  * those of the family's first sequence, whose pages alone are read for them, once
- * for all; tokens from there on are each sequence's own.  Sequences of their own
+ * for all; tokens from there on are each sequence's own.  Where the prefix ends
+ * inside a page, behind a whole one, its tokens in that page are a sequence's own
+ * too if its row of block_table has the same entry as the first's (a page of the
+ * cache) for the page before.  Sequences of their own
  * share nothing, whatever their length says.  Results are those of dsa_paged_attn
  * where the sequences' tables name the same pages for the prefix.  A value of the
  * prefix that one row of a family sees and another does not must be finite.
