@@ -65,7 +65,8 @@ def paged_prefix_attention(query, key, value, block_table, actual_seq_lengths_kv
 
     Neighbouring sequences with the same ``prefix_groups`` entry and the same
     ``prefix_lengths`` entry are a family (int32 [B], as from
-    ``paged_cache_prefixes``): the first ``prefix_lengths`` tokens of each are
+    ``paged_cache_prefixes``; ids of any integer type, such as hashes of the
+    prompts): the first ``prefix_lengths`` tokens of each are
     those in the pages of the family's first sequence; what follows is in the
     pages of each sequence.  A negative group, a length of 0 and a sequence
     alone share nothing.  The prefix may be longer than some of the sequences,
@@ -163,7 +164,7 @@ def _attend(query, key, value, block_table, actual_seq_lengths_kv, scale_value, 
         raise ValueError("actual sequence length arrays must have one entry per batch")
     families = ()
     if prefix is not None:
-        families = tuple(_lengths(x, dev) for x in prefix)
+        families = _groups(prefix[0], dev), _lengths(prefix[1], dev)
         if any(x.numel() != B for x in families):
             raise ValueError(f"prefix_groups and prefix_lengths must have one entry per sequence ({B})")
     for name, t in others:
@@ -217,6 +218,29 @@ def _lengths(x, device):
         if x.device == device and x.is_contiguous():
             return x
     return _seq_tensor(x, device)
+
+
+def _groups(x, device):
+    """Ids of families as the kernels compare them: in 32 bits, equal between
+    neighbours exactly where the given ones are, and negative where those are."""
+    if not isinstance(x, torch.Tensor):
+        ids, runs = list(x), []
+        if any(int(v) != v for v in ids):
+            raise ValueError("prefix_groups must be integers")
+        for i, v in enumerate(ids):
+            runs.append(-1 if v < 0 else runs[-1] if i and v == ids[i - 1] else i)
+        return _seq_tensor(runs, device)
+    if x.is_floating_point() or x.is_complex():
+        raise ValueError(f"prefix_groups must be integers, got {x.dtype}")
+    if x.dtype not in (torch.int64, torch.uint64, torch.uint32) or x.numel() == 0:
+        return _lengths(x, device)
+    # ids that 32 bits may not hold: the index of the first of each run of equal ones
+    x = x.to(device).reshape(-1)
+    signed = x.dtype is torch.int64
+    x = x.to(torch.int64) if x.dtype is torch.uint32 else x.view(torch.int64)
+    first = torch.arange(x.numel(), device=device)
+    first = torch.where(x == x.roll(1), 0, first).cummax(0).values
+    return (torch.where(x < 0, -1, first) if signed else first).to(torch.int32)
 
 
 class PagedAttention(torch.nn.Module):
