@@ -222,6 +222,7 @@ SIGNATURES = {
         _vp, _sz, _vp,                        # workspace, workspace_bytes, stream
     ]),
     "dsa_paged_prefix_attn_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i64, _i64]),
+    "dsa_paged_prefix_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i64, _i64, _i64]),
     "dsa_paged_prefix_attn": (_c.c_int, [
         _vp, _vp, _vp, _vp, _vp,              # query, query_rope, key, key_rope, value
         _vp, _vp, _vp,                        # attention_out, softmax_max, softmax_sum
@@ -259,7 +260,7 @@ _ENTRIES = ("dsa_rope", "dsa_paged_cache_write", "dsa_paged_cache_fork_workspace
             "dsa_paged_cache_compact_workspace_size", "dsa_paged_cache_compact", "dsa_paged_attn_workspace_size",
             "dsa_paged_attn", "dsa_last_error", "dsa_rope_axes", "dsa_paged_cache_plan_workspace_size",
             "dsa_paged_cache_plan", "dsa_paged_cache_write_slots", "dsa_paged_cache_prefixes",
-            "dsa_paged_prefix_attn_workspace_size", "dsa_paged_prefix_attn")  # in the order in which _torch_calls takes them
+            "dsa_paged_prefix_attn_workspace_bytes", "dsa_paged_prefix_attn")  # in the order in which _torch_calls takes them
 _calls = None
 
 

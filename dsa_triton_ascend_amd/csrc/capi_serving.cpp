@@ -8,7 +8,7 @@ namespace dsa {
 bool paged_prefix_launchable(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
                              int64_t max_blocks, int64_t page);
 size_t paged_prefix_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
-                                    int64_t max_blocks, int64_t page);
+                                    int64_t max_blocks, int64_t page, int64_t min_tokens);
 int paged_prefix_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
                      const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
                      const int32_t* act_k, const int32_t* table, const int32_t* ids, const int32_t* shared,
@@ -24,10 +24,16 @@ extern "C" {
 
 size_t dsa_paged_prefix_attn_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d,
                                             int32_t latent, int64_t max_blocks, int64_t page_size) {
+  return dsa_paged_prefix_attn_workspace_bytes(batch, s1, n1, n2, d, latent, max_blocks, page_size, 0);
+}
+
+size_t dsa_paged_prefix_attn_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d,
+                                             int32_t latent, int64_t max_blocks, int64_t page_size,
+                                             int64_t min_tokens) {
   if (!paged_attn_sizes_ok(batch, s1, n1, n2, d, latent != 0, max_blocks, page_size) ||
       !paged_prefix_launchable(batch, s1, n1, n2, d, latent != 0, max_blocks, page_size))
     return 0;
-  return paged_prefix_workspace_bytes(batch, s1, n1, n2, d, latent != 0, max_blocks, page_size);
+  return paged_prefix_workspace_bytes(batch, s1, n1, n2, d, latent != 0, max_blocks, page_size, min_tokens);
 }
 
 int dsa_paged_prefix_attn(const void* query, const void* query_rope, const void* key, const void* key_rope,
@@ -48,14 +54,13 @@ int dsa_paged_prefix_attn(const void* query, const void* query_rope, const void*
   DSA_CHECK_SUPPORTED(paged_prefix_launchable(batch, s1, n1, n2, d, latent, max_blocks, page_size),
                       "too many query rows, or too many for so wide a block table");
   st = check_workspace(workspace, workspace_bytes,
-                       paged_prefix_workspace_bytes(batch, s1, n1, n2, d, latent, max_blocks, page_size));
+                       paged_prefix_workspace_bytes(batch, s1, n1, n2, d, latent, max_blocks, page_size, min_tokens));
   if (st != DSA_OK) return st;
   DSA_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
   return paged_prefix_run(query, query_rope, key, key_rope, value, attention_out, softmax_max, softmax_sum,
                           actual_seq_q, actual_seq_kv, block_table, prefix_groups, prefix_lengths, batch, s1, n1, n2, d,
                           num_blocks, page_size, max_blocks, sparse_mode, pre_tokens, next_tokens, min_tokens, dtype,
-                          scale_value,
-                          return_lse, workspace, (hipStream_t)stream);
+                          scale_value, return_lse, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

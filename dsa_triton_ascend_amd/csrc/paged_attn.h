@@ -69,6 +69,7 @@ struct PagedJob {  // rows of a family, and tokens tok0 .. tok1 of its prefix
 };
 struct PagedPrefixParams : PagedAttnParams {
   const int32_t *ids, *shared;  // per sequence: its family and the tokens that it shares
+  int before;  // sequences of the call that come before this launch's, in all arrays (-before .. -1)
   PagedWhere* where;
   PagedJob* job;
   int* n_jobs;
@@ -85,14 +86,14 @@ template <typename P> constexpr bool kPrefixed = std::is_same<P, PagedPrefixPara
 
 // whether sequence b has the family of the one before it
 __device__ __forceinline__ bool paged_linked(const PagedPrefixParams& p, int b) {
-  const int here = min(b, p.batch - 1), before = max(here - 1, 0), id = p.ids[here], n = p.shared[here];
-  return b == here && b > 0 && id >= 0 && n > 0 && p.ids[before] == id && p.shared[before] == n;
+  const int here = min(b, p.batch - 1), before = max(here - 1, -p.before), id = p.ids[here], n = p.shared[here];
+  return b == here && b > -p.before && id >= 0 && n > 0 && p.ids[before] == id && p.shared[before] == n;
 }
 
-// the first sequence of the family that b is in, for a b that is the same on all lanes
+// the first sequence of the family that b is in, for a b that is the same on all lanes (all of them active)
 __device__ __forceinline__ int paged_leader(const PagedPrefixParams& p, int b, int lane) {
   for (;; b -= 64) {
-    const unsigned long long apart = ~__ballot(paged_linked(p, max(b - lane, 0)));
+    const unsigned long long apart = ~__ballot(paged_linked(p, max(b - lane, -p.before)));
     if (apart) return b - (__ffsll(apart) - 1);
   }
 }

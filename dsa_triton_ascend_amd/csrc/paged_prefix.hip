@@ -444,12 +444,14 @@ struct PrefixShape {
   PagedShape behind;
   int workers, shift;  // jobs of one key head aimed at; log2 of the rows of a block
   int64_t jobs, grid;  // at most
+  int64_t run_rows, whole_rows, job_rows;  // of outputs: of runs, of sequences that a run has whole, of jobs
 };
 
 static int prefix_shift(int64_t d, bool latent) { return latent || d == 256 ? 7 : 8; }
 
+// together: whether there may be jobs
 static PrefixShape prefix_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
-                                int64_t max_blocks, int64_t page) {
+                                int64_t max_blocks, int64_t page, bool together) {
   PrefixShape s;
   s.behind = paged_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
   s.shift = prefix_shift(d, latent);
@@ -458,33 +460,76 @@ static PrefixShape prefix_shape(int64_t batch, int64_t s1, int64_t n1, int64_t n
   const int64_t blocks = (batch * s1 * (n1 / n2) >> s.shift) + batch / 2 + 1;
   s.jobs = blocks >= (1ll << 30) ? 1ll << 31 : prefix_jobs((int)blocks, s.workers);
   s.grid = (cus + 7) / 8 * 8;
+  if (!together) s.jobs = 0;
+  s.run_rows = (int64_t)s.behind.workers * 2 * s.behind.groups * s.behind.group_rows;
+  s.whole_rows = together ? batch * s.behind.groups * s.behind.group_rows : 0;
+  s.job_rows = s.jobs * n2 << s.shift;
   return s;
 }
 
 bool paged_prefix_launchable(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
                              int64_t max_blocks, int64_t page) {
-  const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
+  const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page, true);
   // (jobs, their places over all key heads, and the tiles of all blocks of rows are counted in 32 bits)
   return s.jobs < (1ll << 26) && s.jobs * n2 + s.grid < (1ll << 31) &&
          ((batch * s1 * (n1 / n2) >> s.shift) + batch) * ((max_blocks * page + kPrefixTile - 1) / kPrefixTile) < (1ll << 31);
 }
 
-// rows of the outputs of runs, of sequences that a run has whole, and of jobs
-static int64_t prefix_run_rows(const PrefixShape& s) {
-  return (int64_t)s.behind.workers * 2 * s.behind.groups * s.behind.group_rows;
+// Tokens of a prefix from which on it is worked on for its family together
+// (described in paged_prefix.h).
+static int prefix_least(int64_t min_tokens, int64_t rows, int64_t readers, int64_t token_bytes, bool latent) {
+  constexpr int64_t never = 0x7fffffff;
+  if (min_tokens < 0)
+    min_tokens = latent && rows >= 64 ? never : (latent ? 320 << 20 : 256 << 20) / (readers * token_bytes);
+  return (int)(min_tokens < 1 ? 1 : (min_tokens < never ? min_tokens : never));
 }
-static int64_t prefix_whole_rows(const PrefixShape& s, int64_t batch) {
-  return batch * s.behind.groups * s.behind.group_rows;
-}
-static size_t prefix_part_rows(const PrefixShape& s, int64_t batch, int64_t n2) {
-  return (size_t)prefix_run_rows(s) + (size_t)prefix_whole_rows(s, batch) + ((size_t)s.jobs * n2 << s.shift);
+
+// How a call is worked on: which prefixes for their families together, and the
+// sequences of a launch.  Together takes some three times the rows of the queries
+// in 32 bits: up to 512 MB of it for all sequences at once, else for as many at a
+// time (families that go on in the next launch are cut there, as at multiples of
+// 64 sequences; with so many rows each has blocks of its own anyway), and for none
+// where two would be too many.
+constexpr int64_t kPrefixBytes = 1 << 29;
+
+struct PrefixCall {
+  int least;      // tokens, more than the table has where nothing is worked on together
+  int64_t batch;  // sequences of a launch
+  PrefixShape shape;
+  size_t part_rows() const { return (size_t)(shape.run_rows + shape.whole_rows + shape.job_rows); }
+};
+
+static PrefixCall prefix_call(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
+                              int64_t max_blocks, int64_t page, int64_t min_tokens) {
+  PrefixCall c;
+  const int64_t room = max_blocks * page;
+  auto shape = [&](int64_t n, bool together) { return prefix_shape(n, s1, n1, n2, d, latent, max_blocks, page, together); };
+  c.batch = batch;
+  c.shape = shape(batch, true);
+  c.least = prefix_least(min_tokens, s1 * (n1 / n2), batch * c.shape.behind.row_groups, (latent ? d + 64 : 2 * n2 * d) * 2,
+                         latent);
+  auto fits = [&](const PrefixShape& s) {
+    return (s.whole_rows + s.job_rows) * (int64_t)(sizeof(f32x4) + d * sizeof(float)) <= kPrefixBytes;
+  };
+  if (c.least <= room && !fits(c.shape)) {
+    int64_t most = 1, over = batch;
+    while (over - most > 1) {
+      const int64_t n = (most + over) / 2;
+      (fits(shape(n, true)) ? most : over) = n;
+    }
+    if (most == 1) c.least = 0x7fffffff;
+    const int64_t launches = (batch + most - 1) / most;
+    if (most > 1) c.batch = (batch + launches - 1) / launches;
+  }
+  if (c.least > room || c.batch < batch) c.shape = shape(c.batch, c.least <= room);
+  return c;
 }
 
 size_t paged_prefix_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d, bool latent,
-                                    int64_t max_blocks, int64_t page) {
-  const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
-  return prefix_part_rows(s, batch, n2) * (sizeof(f32x4) + d * sizeof(float)) + (size_t)batch * sizeof(PagedWhere) +
-         (size_t)s.jobs * sizeof(PagedJob) + 16;
+                                    int64_t max_blocks, int64_t page, int64_t min_tokens) {
+  const PrefixCall c = prefix_call(batch, s1, n1, n2, d, latent, max_blocks, page, min_tokens);
+  return c.part_rows() * (sizeof(f32x4) + d * sizeof(float)) + (size_t)c.batch * sizeof(PagedWhere) +
+         (size_t)c.shape.jobs * sizeof(PagedJob) + 16;
 }
 
 template <typename T, bool FAST>
@@ -505,15 +550,6 @@ static int prefix_grouped_launch(const PagedPrefixParams& p, int64_t d, int32_t 
   return DSA_OK;
 }
 
-// Tokens of a prefix from which on it is worked on for its family together
-// (described in paged_prefix.h).
-static int prefix_least(int64_t min_tokens, int64_t rows, int64_t readers, int64_t token_bytes, bool latent) {
-  constexpr int64_t never = 0x7fffffff;
-  if (min_tokens < 0)
-    min_tokens = latent && rows >= 64 ? never : (latent ? 320 << 20 : 256 << 20) / (readers * token_bytes);
-  return (int)(min_tokens < 1 ? 1 : (min_tokens < never ? min_tokens : never));
-}
-
 int paged_prefix_run(const void* query, const void* query_rope, const void* key, const void* key_rope,
                      const void* value, void* out, float* smax, float* ssum, const int32_t* act_q,
                      const int32_t* act_k, const int32_t* table, const int32_t* ids, const int32_t* shared,
@@ -521,33 +557,44 @@ int paged_prefix_run(const void* query, const void* query_rope, const void* key,
                      int64_t max_blocks, int32_t mode, int64_t pre_tokens, int64_t next_tokens, int64_t min_tokens,
                      int32_t dtype, float scale, int32_t return_lse, void* workspace, hipStream_t stream) {
   const bool latent = value == nullptr;
-  const PrefixShape s = prefix_shape(batch, s1, n1, n2, d, latent, max_blocks, page);
-  PagedPrefixParams p = {};
-  paged_fill(p, s.behind, query, query_rope, key, key_rope, value, out, smax, ssum, act_q, act_k, table, batch, s1, n1,
-             n2, num_blocks, page, max_blocks, mode, pre_tokens, next_tokens, scale, return_lse);
-  const size_t rows = prefix_part_rows(s, batch, n2);
-  p.part_ml = (f32x4*)workspace;
-  p.part_o = (float*)(p.part_ml + rows);
-  p.where = (PagedWhere*)(p.part_o + rows * d);
-  p.job = (PagedJob*)(p.where + batch);
-  p.n_jobs = (int*)(p.job + s.jobs);
-  p.whole0 = prefix_run_rows(s);
-  p.part0 = p.whole0 + prefix_whole_rows(s, batch);
-  p.ids = ids;
-  p.shared = shared;
-  p.least = prefix_least(min_tokens, p.rows, batch * p.row_groups, (latent ? d + 64 : 2 * n2 * d) * 2, latent);
-  p.prefix_workers = s.workers;
-  p.job_shift = s.shift;
-  p.rows_magic = 0xffffffffu / (unsigned)p.rows;
-  p.group_magic = 0xffffffffu / (unsigned)p.group;
-  p.heads_magic = 0xffffffffu / (unsigned)p.n2;
-  const int64_t most = (s.jobs * n2 + 7) / 8 * 8;
-  const unsigned grid = (unsigned)(most < s.grid ? most : s.grid);
-  int st = latent ? paged_latent_launch(p, d, dtype, stream) : paged_grouped_launch(p, d, dtype, stream);
-  if (st == DSA_OK && p.least <= max_blocks * page)
-    st = latent ? prefix_latent_launch(p, d, dtype, grid, stream) : prefix_grouped_launch(p, d, dtype, grid, stream);
-  if (st != DSA_OK) return st;
-  return paged_combine_launch(p, s.behind.tile, d, dtype, stream);
+  const PrefixCall c = prefix_call(batch, s1, n1, n2, d, latent, max_blocks, page, min_tokens);
+  const bool together = c.least <= max_blocks * page;
+  auto at = [](const void* x, int64_t bytes) { return x ? (const unsigned char*)x + bytes : nullptr; };
+  for (int64_t b0 = 0; b0 < batch; b0 += c.batch) {
+    const int64_t n = batch - b0 < c.batch ? batch - b0 : c.batch, rows0 = b0 * s1 * n1;
+    const PrefixShape s =
+        n == c.batch ? c.shape : prefix_shape(n, s1, n1, n2, d, latent, max_blocks, page, together);
+    PagedPrefixParams p = {};
+    paged_fill(p, s.behind, at(query, rows0 * d * 2), at(query_rope, rows0 * 64 * 2), key, key_rope, value,
+               (void*)at(out, rows0 * d * 2), (float*)at(smax, rows0 * 4), (float*)at(ssum, rows0 * 4),
+               (const int32_t*)at(act_q, b0 * 4), act_k + b0, table + b0 * max_blocks, n, s1, n1, n2, num_blocks, page,
+               max_blocks, mode, pre_tokens, next_tokens, scale, return_lse);
+    const int64_t rows = s.run_rows + s.whole_rows + s.job_rows;
+    p.part_ml = (f32x4*)workspace;
+    p.part_o = (float*)(p.part_ml + rows);
+    p.where = (PagedWhere*)(p.part_o + rows * d);
+    p.job = (PagedJob*)(p.where + n);
+    p.n_jobs = (int*)(p.job + s.jobs);
+    p.whole0 = s.run_rows;
+    p.part0 = p.whole0 + s.whole_rows;
+    p.ids = ids + b0;
+    p.shared = shared + b0;
+    p.before = (int)b0;
+    p.least = c.least;
+    p.prefix_workers = s.workers;
+    p.job_shift = s.shift;
+    p.rows_magic = 0xffffffffu / (unsigned)p.rows;
+    p.group_magic = 0xffffffffu / (unsigned)p.group;
+    p.heads_magic = 0xffffffffu / (unsigned)p.n2;
+    const int64_t most = (s.jobs * n2 + 7) / 8 * 8;
+    const unsigned grid = (unsigned)(most < s.grid ? most : s.grid);
+    int st = latent ? paged_latent_launch(p, d, dtype, stream) : paged_grouped_launch(p, d, dtype, stream);
+    if (st == DSA_OK && together)
+      st = latent ? prefix_latent_launch(p, d, dtype, grid, stream) : prefix_grouped_launch(p, d, dtype, grid, stream);
+    if (st == DSA_OK) st = paged_combine_launch(p, s.behind.tile, d, dtype, stream);
+    if (st != DSA_OK) return st;
+  }
+  return DSA_OK;
 }
 
 }  // namespace dsa

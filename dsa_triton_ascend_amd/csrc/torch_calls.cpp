@@ -50,7 +50,7 @@ struct Entries {
   decltype(&dsa_paged_cache_plan) plan;
   decltype(&dsa_paged_cache_write_slots) write_slots;
   decltype(&dsa_paged_cache_prefixes) prefixes;
-  decltype(&dsa_paged_prefix_attn_workspace_size) prefix_attn_bytes;
+  decltype(&dsa_paged_prefix_attn_workspace_bytes) prefix_attn_bytes;
   decltype(&dsa_paged_prefix_attn) prefix_attn;
 } entry;
 
@@ -337,7 +337,8 @@ PyObject* attention(PyObject* const* a) {
     if (!groups || !shared || groups->size(0) != b || shared->size(0) != b) return nullptr;
   }
   const int64_t wide = table->size(1);
-  const size_t bytes = (PREFIX ? entry.prefix_attn_bytes : entry.attn_bytes)(b, s1, n1, n2, d, latent, wide, page);
+  const size_t bytes = PREFIX ? entry.prefix_attn_bytes(b, s1, n1, n2, d, latent, wide, page, least)
+                              : entry.attn_bytes(b, s1, n1, n2, d, latent, wide, page);
   if (!bytes) return nullptr;
   at::Tensor out = fresh(q->sizes(), *q), mx = fresh({b, n2, s1, n1 / n2}, *q, at::kFloat);
   at::Tensor sm = fresh({b, n2, s1, n1 / n2}, *q, at::kFloat);

@@ -184,16 +184,16 @@ def _attend(query, key, value, block_table, actual_seq_lengths_kv, scale_value, 
     if key.numel() == 0 or wide == 0:  # no page at all: no row sees a token
         return out.zero_(), smax.zero_(), ssum.zero_()
     lib = _lib.load()
-    entry, size = ((lib.dsa_paged_attn, lib.dsa_paged_attn_workspace_size) if prefix is None else
-                   (lib.dsa_paged_prefix_attn, lib.dsa_paged_prefix_attn_workspace_size))
-    nbytes = _lib.call_on(index, size, B, S1, N1, N2, D, latent, wide, page)
+    entry, size, least = ((lib.dsa_paged_attn, lib.dsa_paged_attn_workspace_size, ()) if prefix is None else
+                          (lib.dsa_paged_prefix_attn, lib.dsa_paged_prefix_attn_workspace_bytes, (min_tokens,)))
+    nbytes = _lib.call_on(index, size, B, S1, N1, N2, D, latent, wide, page, *least)
     ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
     status = _lib.call_on(
         index, entry, q.data_ptr(), qr.data_ptr() if latent else None, key.data_ptr(),
         key_rope.data_ptr() if latent else None, None if latent else value.data_ptr(), out.data_ptr(),
         smax.data_ptr(), ssum.data_ptr(), None if act_q is None else act_q.data_ptr(), act_k.data_ptr(),
         table.data_ptr(), *(x.data_ptr() for x in families), B, S1, N1, N2, D, _D_ROPE if latent else 0, pages, page,
-        wide, sparse_mode, pre_tokens, next_tokens, *(() if prefix is None else (min_tokens,)), code,
+        wide, sparse_mode, pre_tokens, next_tokens, *least, code,
         float(scale_value), bool(return_softmax_lse), ws.data_ptr(), nbytes, _lib.raw_stream(index))
     if status:
         _lib.check(status, "dsa_" + what.replace("attention", "attn"))

@@ -588,11 +588,19 @@ int dsa_paged_attn(const void* query, const void* query_rope, const void* key, c
  * prefix that one row of a family sees and another does not must be finite.
  * min_tokens: prefixes of fewer tokens are read by each sequence for itself;
  * negative: chosen from the sizes.
+ * The workspace of a call with that min_tokens comes from
+ * dsa_paged_prefix_attn_workspace_bytes, for whatever min_tokens from
+ * dsa_paged_prefix_attn_workspace_size.  It is little more than dsa_paged_attn's where no
+ * prefix can be worked on together, and at most 512 MB more where some can: beyond
+ * that the sequences are worked on so many at a time.
  * Everything else as dsa_paged_attn; the query rows and the tiles of 32 tokens of a
  * table row are fewer than 2^31 as a product.
  */
 size_t dsa_paged_prefix_attn_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d,
                                             int32_t latent, int64_t max_blocks, int64_t page_size);
+size_t dsa_paged_prefix_attn_workspace_bytes(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d,
+                                             int32_t latent, int64_t max_blocks, int64_t page_size,
+                                             int64_t min_tokens);
 int dsa_paged_prefix_attn(const void* query, const void* query_rope, const void* key, const void* key_rope,
                           const void* value, void* attention_out, float* softmax_max, float* softmax_sum,
                           const int32_t* actual_seq_q, const int32_t* actual_seq_kv, const int32_t* block_table,
