@@ -361,23 +361,29 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(P p, int tile, int w
       return s;
     };
     float m = -INFINITY, t = -INFINITY;
-    bool bad = false;  // scores that are not numbers set no reference: their sums show them
     for (int i = lane; i < runs; i += 64) {
       const f32x4 ml = p.part_ml[slot(i)];
       m = fmaxf(m, ml[0]);
       t = fmaxf(t, ml[2]);
-      bad |= ml[1] != ml[1];
     }
     *big = m = wave_max(m);
     *top = wave_max(t);
     FV acc = {};
     float la = 0.f, na = 0.f;
-    if (m == -INFINITY && __any(bad)) {
-      la = na = __builtin_nanf("");
+    if (m == -INFINITY) {
+      // no token seen, or scores that are not numbers, which set no reference:
+      // the sums show them
+      bool bad = false;
+      for (int i = lane; i < runs; i += 64) {
+        const float l = p.part_ml[slot(i)][1];
+        bad |= l != l;
+      }
+      if (__any(bad)) {
+        la = na = __builtin_nanf("");
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) acc[e] = la;
-    }
-    if (m != -INFINITY)
+        for (int e = 0; e < EPL; ++e) acc[e] = la;
+      }
+    } else {
       for (int c = i0; c < i1; c += 64) {
         const int mine = c + lane;
         float f = 0.f;
@@ -402,6 +408,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(P p, int tile, int w
           }
         }
       }
+    }
     *o = acc;
     *l = wave_sum(la);
     *n = wave_sum(na);
