@@ -23,12 +23,21 @@ One decoding step:
     out, _, _ = paged_attention(q, latent_cache, None, table, lens + 1, ...)                 # per layer
     lens = lens + 1                                                                          # of rows in use
 
-One step of requests with new tokens of their own number each, packed:
+One step of requests with new tokens of their own number each: ``new[r]`` of
+row r, S1 at most (a number known on the host), packed in ``tokens`` places for
+rotation and writes.  Attention takes each row's own tokens, padded to S1:
 
+    old = lens.clamp(min=0)
     table, lens, refs, slots, positions, ends = paged_cache_plan(table, lens, refs, new, page, tokens)   # once
     groups, shared = paged_cache_prefixes(table, lens, page)                                             # once
+    counts = (lens - old).clamp(min=0)     # tokens taken, 0 for rows that were refused or have ended      once
+    at = ((ends - new.clamp(min=0))[:, None] + torch.arange(S1, device=ends.device)).clamp(max=tokens - 1)  # once
     paged_cache_write_slots([latent, k_rope, k_index], [...], slots)                                     # per layer
-    out, _, _ = paged_prefix_attention(q, latent_cache, None, table, lens, groups, shared, ...)          # per layer
+    out, _, _ = paged_prefix_attention(q[at], latent_cache, None, table, lens, groups, shared,           # per layer
+                                       query_rope=q_rope[at], key_rope=k_rope_cache, actual_seq_lengths_query=counts)
+
+and token t of the packed ones has its output at ``out[r, t - (ends - new)[r]]``
+with ``r = torch.searchsorted(ends, t, right=True)`` (tokens of refused rows: zeros).
 """
 from array import array
 
