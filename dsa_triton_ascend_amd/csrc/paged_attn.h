@@ -107,7 +107,7 @@ __device__ __forceinline__ bool paged_together(const PagedPrefixParams& p, int t
 // Sequence b's family among the 64 sequences from a multiple of 64 on: where it
 // starts and how many they are.  What is worked on together is cut there, so
 // that a wave sees all of it at once.  b: the same on all lanes, or lane l's is
-// the l-th of the 64.
+// the l-th of the 64; lanes may be missing only where no sequence is theirs.
 struct PagedFamily {
   int first, count;
   bool linked;  // with any other, also of another 64
@@ -329,9 +329,10 @@ struct PagedPlan {
 
   // tiles before sequence b
   __device__ __forceinline__ int start(const P& p, int tile, int lane, int b) const {
+    static_assert(!kPrefixed<P>, "the lanes from b on stay away from the loop, so that families would end at b");
     if (b < 64) return b ? __builtin_amdgcn_readlane(incl, b - 1) : 0;
     int n = 0;
-#pragma unroll (kPrefixed<P> ? 1 : 4)
+#pragma unroll 4
     for (int i = lane; i < b; i += 64) n += padded(paged_tiles(paged_seq(p, i), tile));
     return wave_total(n);
   }
