@@ -15,22 +15,34 @@
 // all in 32 bits (the parts in memory too).
 //
 // Which families.  Together costs a launch more, and outputs of 32 bits that are
-// written and joined: 6 to 10 us with grouped heads, 15 to 20 over the latent
+// written and joined: 5 to 10 us with grouped heads, 15 to 20 over the latent
 // cache.  Apart costs the reading of the prefix by every sequence (and every
 // row group of one), from the caches for the most part.  So a prefix has to be
 // so long that the whole batch would read 256 MB (latent: 320 MB) of it.
-// Measured, us, apart and together, 8 key heads of 128 columns and eight query
-// heads on each: 32 sequences behind 2048 tokens 38.7 and 40.6, behind 8192 94
-// and 48, behind 32768 322 and 69; 8 behind 2048 24 and 28, behind 8192 41 and
-// 33; 16 families of two behind 4096 94 and 77, behind 16384 313 and 225; 16 new
-// tokens of 16 sequences behind 2048 85 and 76.  16 latent heads: 32 sequences
-// behind 8192 tokens 57 and 60, behind 32768 162 and 81; 64 behind 8192 94 and
-// 72; 16 families of two behind 16384 96 and 103.
+// Measured, us, apart and together, 200 tokens behind the prefix, 8 key heads of
+// 128 columns and eight query heads on each: 32 sequences behind 2048 tokens 40
+// and 43, behind 8192 95 and 52, behind 32768 324 and 83; 8 behind 2048 25 and 29,
+// behind 8192 41 and 35; 16 families of two behind 4096 95 and 87, behind 16384
+// 318 and 240; 16 new tokens of 16 sequences behind 2048 84 and 81.  16 latent
+// heads: 32 sequences behind 8192 tokens 60 and 61, behind 32768 179 and 83; 64
+// behind 8192 101 and 72; 16 families of two behind 16384 100 and 105.
 // From 64 latent rows of a sequence on its own products bound it, and together
-// is hardly faster or slower (128 heads, 32 sequences behind 32768 tokens: 301
-// and 312; 64 heads 188 and 178).  The caller may set the length instead.
+// is hardly faster or slower (32 sequences behind 32768 tokens: 128 heads 311 and
+// 325; 64 heads 194 and 184).  The caller may set the length instead.
+//
+// The rule counts the batch, not what each family saves: near its border it takes
+// the slower way by up to 8 % (the first of the grouped cases, the last of the
+// latent ones), and one pair among many unrelated sequences may be worked on
+// together for less than the launch costs.  Pools and tables of more than 256 MB of cache are loaded past the
+// caches, as by paged_attention; prefixes that sequences read apart are then read
+// from memory by each (32 behind 1024 tokens with 1024 of their own: 53 us, 40
+// with loads that are kept, which take 202 in place of 182 for 32 unrelated
+// sequences of 8000 tokens).
 // What is not worked on together each sequence reads for itself (paged_attn.h),
-// from the pages of the family's first, 1 to 4 us slower than paged_attention.
+// from the pages of the family's first: up to 2 us slower than paged_attention
+// with grouped heads, 2 to 13 % over the latent cache (16 heads, 64 sequences
+// behind 8192 tokens: 89 and 101 us; 128 heads, 32 behind 32768: 304 and 311), for
+// the search for families in every worker.
 //
 // Work.  A job is a block of up to R rows of a family (over its sequences, new
 // tokens and the query heads of one key head) and a part of its prefix.  Parts

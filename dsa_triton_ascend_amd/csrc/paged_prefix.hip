@@ -4,15 +4,16 @@
 //   S^T = K Q^T,  P = 2^(S - ref),  O^T = V^T P^T
 //
 // A family of 32 sequences with eight query heads per key head has 256 rows a
-// key head, and a token of the prefix serves them all: 4 * 256 flops per byte of
-// K and V, so the matrix instructions bound it, and beside them the vector
-// unit, which has a softmax weight to make for every 4 D flops.
+// key head, and a token of the prefix serves them all: 256 flops per byte of K
+// and V, so the matrix instructions bound it, and beside them the vector unit,
+// which has a softmax weight to make for every 4 D flops.
 //
 // A workgroup has up to 16 NW MR rows: wave w the 16 MR from 16 MR w on, in MR
 // tiles of 16.  K and V come in tiles of 32 tokens by LDS-DMA into a ring,
 // chunks of 16 bytes swizzled so that both products read them without bank
 // conflicts; every wave reads the whole tile, so the rows of a wave set what the
-// LDS has to give (16 KB per 2048 MFMA cycles of a CU at 64 rows of 128 columns).
+// LDS has to give (at 32 rows a wave 128 KB a tile of 128 columns, 512 cycles of
+// a CU's LDS beside 1536 of its MFMAs).
 // S^T leaves a token's weight where the second product wants it: token 16 tt +
 // 4 g + r is k slot 8 g + 4 tt + r of lane group g, and V^T is read transposed
 // in that order, so P stays in its lanes.
@@ -21,21 +22,20 @@
 // of tile t between its MFMAs, then the output of tile t with the first half of
 // that of tile t + 1.  One barrier a step.
 //
-// P is rounded once to the input type, and the output is divided by the sum of
-// the rounded weights, which one more row of ones beside V gives, so that they
-// still add up to one; the sum that is returned is that of the weights in 32
-// bits.  (Two values of the input type, as paged_attn.hip has them, would cost
-// half as many matrix instructions again, which are not free here.)  Error
-// against 64 bits, both 2-norms, 32 sequences behind 32768 tokens: bf16 2.1e-3,
-// rounding of the output included (1.7e-3 alone).
+// P is multiplied as a sum of two values of the input type, as paged_attn.hip has
+// it: half as many matrix instructions again, and the error of a call does not
+// depend on which way its sizes choose.  Rounded once the kernel took 50 us in
+// place of 63 behind 32768 tokens, and the error against 64 bits, both 2-norms,
+// was 2.1e-3 with bf16 where the rounding of the output alone is 1.7e-3, as now.
 //
 // Measured, 8 key heads of 128 columns with eight query heads each, 32
-// sequences: behind 32768 tokens 50 us, 0.71 PFLOP/s, behind 131072 174 us,
-// 0.81 (a large product of the library: 1.3 to 1.4).  LDS reads (16 KB of 64
-// rows' MFMAs at about 256 bytes a clock), the softmax and the MFMAs take about
-// as long each, and what does not overlap is left: the matrix pipes work 38 to
-// 46 % of the cycles.  10 us of a launch are its start and the 32-bit outputs
-// of 256 jobs (34 MB).
+// sequences: behind 32768 tokens 63 us, 0.55 PFLOP/s without counting weights
+// twice, behind 131072 215 us, 0.64 (a large product of the library: 1.3 to 1.4).
+// In the latter the matrix pipes work 49 % of the cycles, the vector units 46 %
+// beside the issue of the MFMAs, the LDS 16 %; two waves of a SIMD overlap the
+// two only in part.  10 us of a launch are its start and the 32-bit outputs of
+// 256 jobs (34 MB).
+// Steps, measured with weights in one value:
 //  * All DMAs of a stage at once, where all waves wait for the issue: 200 us
 //    behind 131072 tokens; one by one between the scores' MFMAs: 174; between
 //    the output's: 184.
@@ -59,8 +59,8 @@ template <int D> constexpr int kPrefixRing = D == 64 ? 6 : 4;
 // FAST: no DMA lies in two pages (jobs start at whole tiles: there is no band),
 // and none of its rows' offsets needs more than 32 bits, so that one descriptor
 // serves a DMA in place of an address per lane (32 sequences behind 32768
-// tokens: 50.7 us against 60.5 at 8 key heads of 128 columns, 36.6 against 38.5
-// at 8 of 64, 57.8 against 88.8 at 4 of 256).
+// tokens: 63 us against 75 at 8 key heads of 128 columns, 44.6 against 46.6
+// at 8 of 64, 69 against 98 at 4 of 256).
 template <typename T, int D, int NW, int MR, bool FAST>
 __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixParams p) {
   using E = Elem<T>;
@@ -101,9 +101,6 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
     k_from[j] = (int)((lane / CPT) * row_bytes) + ((lane % CPT) ^ swz_k(tk)) * 16;
     v_from[j] = (int)((lane / CPT) * row_bytes) + ((lane % CPT) ^ swz_v(tk)) * 16;
   }
-  V8 ones;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = E::from_f32(1.f);
 
   int head;
   int job = prefix_job_of(p, blockIdx.x, gridDim.x, 0, &head);
@@ -136,13 +133,12 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = as_v8<V8>((x[rt][ks] & keep) ^ flip);
     };
-    f32x4 acc[ND][MR], accn[MR];
+    f32x4 acc[ND][MR];
     float ref[MR], top[MR], sum[MR];
 #pragma unroll
     for (int rt = 0; rt < MR; ++rt) {
       ref[rt] = top[rt] = -INFINITY;
       sum[rt] = 0.f;
-      accn[rt] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < ND; ++j) acc[j][rt] = {0.f, 0.f, 0.f, 0.f};
     }
@@ -197,18 +193,19 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
 
       float f_moved[MR];
       bool moved = false;
-      auto weights = [&](int rt, int tt, f32x4 (&s)[2][MR], V8 (&ph)[MR]) {
+      auto weights = [&](int rt, int tt, f32x4 (&s)[2][MR], V8 (&ph)[MR], V8 (&pl)[MR]) {
         const float from = ref[rt] == -INFINITY ? 0.f : ref[rt];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float e = fast_exp2(__builtin_fmaf(s[tt][rt][i], scale, -from));
           sum[rt] += e;
           ph[rt][tt * 4 + i] = E::from_f32(e);
+          pl[rt][tt * 4 + i] = E::from_f32(e - E::to_f32(ph[rt][tt * 4 + i]));
         }
       };
       // the first half of the softmax of tile t, in NA slices
       constexpr int NA = 2 + 2 * HR, NBH = 2 * HR;
-      auto soft_a = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR], int t) {
+      auto soft_a = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR], V8 (&pl)[MR], int t) {
         if (k == 0) {
           const int tk = ta + t * TILE;
           if (masked || tk + TILE > tb) {
@@ -248,11 +245,11 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
             }
           }
         } else if (k < NA) {
-          weights((k - 2) >> 1, (k - 2) & 1, s, ph);
+          weights((k - 2) >> 1, (k - 2) & 1, s, ph, pl);
         }
       };
       // the second half, in NBH slices
-      auto soft_b = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR]) { weights(HR + (k >> 1), k & 1, s, ph); };
+      auto soft_b = [&](int k, f32x4 (&s)[2][MR], V8 (&ph)[MR], V8 (&pl)[MR]) { weights(HR + (k >> 1), k & 1, s, ph, pl); };
       // The first fragments of a product are read while the one before it ends:
       // both tiles have landed by then.
       constexpr int PK = 2, PV = 2;
@@ -298,9 +295,7 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
         }
       };
       // output of the tile at `at`; behind it come the scores of the tile at `then`
-      auto gemm2 = [&](int at, int then, V8 (&ph)[MR], auto&& between) {
-#pragma unroll
-        for (int rt = 0; rt < MR; ++rt) accn[rt] = E::mfma(ones, ph[rt], accn[rt]);
+      auto gemm2 = [&](int at, int then, V8 (&ph)[MR], V8 (&pl)[MR], auto&& between) {
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) {
           const V8 f = va[dt % PV];
@@ -308,13 +303,14 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
           else if (SUB == 2 && dt + 1 == ND) first_k(then);
 #pragma unroll
           for (int rt = 0; rt < MR; ++rt) acc[dt][rt] = E::mfma(f, ph[rt], acc[dt][rt]);
+#pragma unroll
+          for (int rt = 0; rt < MR; ++rt) acc[dt][rt] = E::mfma(f, pl[rt], acc[dt][rt]);
           between(dt);
           __builtin_amdgcn_sched_barrier(0);
         }
         if (moved) {  // for the tile after this one
 #pragma unroll
           for (int rt = 0; rt < MR; ++rt) {
-            accn[rt] *= f_moved[rt];
 #pragma unroll
             for (int j = 0; j < ND; ++j) acc[j][rt] *= f_moved[rt];
           }
@@ -347,15 +343,14 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
       auto free_stage = [&]() { return at == 0 ? (NB - 1) * STAGE : at - STAGE; };
       if (active) {
         f32x4 s0[2][MR], s1[2][MR];
-        V8 p0[MR], p1[MR];
+        V8 p0[MR], p1[MR], l0[MR], l1[MR];
         first_k(0);
         gemm1(0, 0, s0, [](int) {});
 #pragma unroll
-        for (int k = 0; k < NA; ++k) soft_a(k, s0, p0, 0);
+        for (int k = 0; k < NA; ++k) soft_a(k, s0, p0, l0, 0);
         if (moved) {
 #pragma unroll
           for (int rt = 0; rt < MR; ++rt) {
-            accn[rt] *= f_moved[rt];
 #pragma unroll
             for (int j = 0; j < ND; ++j) acc[j][rt] *= f_moved[rt];
           }
@@ -365,18 +360,18 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
         // other they hold up the wave that asks for them (43 cycles each, when
         // all waves do).
         auto step = [&](int t, int cur, int next, int then, f32x4 (&s)[2][MR], f32x4 (&sn)[2][MR], V8 (&ph)[MR],
-                        V8 (&pn)[MR], auto d0, auto d1, int f, int to) {
+                        V8 (&pl)[MR], V8 (&pn)[MR], V8 (&ln)[MR], auto d0, auto d1, int f, int to) {
           gemm1(next, cur, sn, [&](int i) {
             // 2 KS places for NBH slices and the DMAs
 #pragma unroll
-            for (int k = i * NBH / (2 * KS); k < (i + 1) * NBH / (2 * KS); ++k) soft_b(k, s, ph);
+            for (int k = i * NBH / (2 * KS); k < (i + 1) * NBH / (2 * KS); ++k) soft_b(k, s, ph, pl);
             constexpr int n = decltype(d1)::value - decltype(d0)::value;
 #pragma unroll
             for (int k = i * n / (2 * KS); k < (i + 1) * n / (2 * KS); ++k) dma(f, decltype(d0)::value + k, to);
           });
-          gemm2(cur, then, ph, [&](int i) {
+          gemm2(cur, then, ph, pl, [&](int i) {
 #pragma unroll
-            for (int k = i * NA / ND; k < (i + 1) * NA / ND; ++k) soft_a(k, sn, pn, t + 1);
+            for (int k = i * NA / ND; k < (i + 1) * NA / ND; ++k) soft_a(k, sn, pn, ln, t + 1);
           });
         };
         // (the first fragments of tile 1's scores: its stage has landed)
@@ -390,21 +385,21 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
           asm volatile("" : "+s"(next));  // (so that each stage's offsets fit the instructions)
           if constexpr (SUB == 2) {
             const int here = at, to = free_stage(), f = t / 2 + NB - 1;
-            step(t, here, here + TILE * ROW, next, s0, s1, p0, p1, none, half, f, to);
+            step(t, here, here + TILE * ROW, next, s0, s1, p0, l0, p1, l1, none, half, f, to);
             at = next;  // (of tile t + 2)
             if (++t >= n_tiles) break;
-            step(t, here + TILE * ROW, next, next + TILE * ROW, s1, s0, p1, p0, half, all, f, to);
+            step(t, here + TILE * ROW, next, next + TILE * ROW, s1, s0, p1, l1, p0, l0, half, all, f, to);
             if (++t >= n_tiles) break;
           } else {
             first_k(next);
-            step(t, at, next, next, s0, s1, p0, p1, none, all, t + NB - 1, free_stage());
+            step(t, at, next, next, s0, s1, p0, l0, p1, l1, none, all, t + NB - 1, free_stage());
             at = next;
             if (++t >= n_tiles) break;
             open_stage();
             int then = next_stage(next);
             asm volatile("" : "+s"(then));
             first_k(then);
-            step(t, at, then, then, s1, s0, p1, p0, none, all, t + NB - 1, free_stage());
+            step(t, at, then, then, s1, s0, p1, l1, p0, l0, none, all, t + NB - 1, free_stage());
             at = then;
             if (++t >= n_tiles) break;
           }
@@ -431,7 +426,7 @@ __global__ __launch_bounds__(NW * 64, 1) void prefix_grouped_kernel(PagedPrefixP
       float* dst = p.part_o + (slot0 + r) * D + lg * 4;
 #pragma unroll
       for (int j = 0; j < ND; ++j) *(f32x4*)(dst + j * 16) = paged_scaled(acc[j][rt], seen);
-      if (lg == 0) p.part_ml[slot0 + r] = {ref[rt], l, t, accn[rt][0]};
+      if (lg == 0) p.part_ml[slot0 + r] = {ref[rt], l, t, l};
     }
     job = prefix_job_of(p, blockIdx.x, gridDim.x, ++round, &head);
   }

@@ -4,16 +4,20 @@
 //   S^T = K Q^T,  P = 2^(S - ref),  O^T = V^T P^T,  V = K[:, :D]
 //
 // At 16 heads a sequence alone has 2 * 1088 * 16 flops for the 1152 bytes of a
-// token; the rows of eight sequences together are 128, and the LDS reads bound
-// it: each of eight waves reads all of K for its 16 rows.  The split of the work in
-// a workgroup is that of paged_attn_latent.hip at 128 rows: wave w has the
+// token; the rows of eight sequences together are 128, whose products bound it,
+// and beside them the LDS, from which each of eight waves reads all of K for its
+// 16 rows.  The split of the work in a workgroup is that of paged_attn_latent.hip at 128 rows: wave w has the
 // scores and the softmax of rows 16 w on, P goes through LDS, and each wave has
 // D / 8 columns of all rows' outputs.  What is a row's sequence, new token and
 // head, and what it sees, differs from row to row here.
 //
 // P is rounded once, and the output divided by the sum of the rounded values,
-// as there.  Measured, 512 columns: 2.3 us for a tile of 32 tokens of every CU's
-// 128 rows (0.9 PFLOP/s), and 20 us for the start and the 32-bit outputs of 256
+// as there at 128 rows (with up to 32 it keeps two values there; 2-norms of the
+// error, bf16, 1.66e-3 with two and 1.75e-3 with one, of which 1.66e-3 is the
+// output's own rounding).  Measured, 512 columns: 2.3 us for a tile of 32 tokens of
+// every CU's 128 rows (0.9 PFLOP/s; the matrix pipes, the LDS and the vector units
+// each work 33 to 36 % of the cycles of a launch of some 25 tiles: what is lost is
+// overlap), and 20 us for the start and the 32-bit outputs of 256
 // jobs (67 MB): 16 heads, 32 sequences behind 32768 tokens 56 us, with what is
 // behind the prefix and the join 81 (each sequence for itself 162).
 #include "paged_prefix.h"
@@ -141,7 +145,7 @@ __global__ __launch_bounds__(kPxThreads, 1) void prefix_latent_kernel(PagedPrefi
     u32x4 ql_in[QL ? QL : 1];
     {
       // (bounds in the descriptors: rows that do not exist read zeros)
-            const int64_t row0 = (int64_t)first * p.rows + jb.row0;
+      const int64_t row0 = (int64_t)first * p.rows + jb.row0;
       const __amdgpu_buffer_rsrc_t q_src =
           __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)p.q + row0 * D), (short)0, n_rows * D * 2, 0x00020000);
       const __amdgpu_buffer_rsrc_t qr_src = __builtin_amdgcn_make_buffer_rsrc(

@@ -75,9 +75,9 @@ def paged_prefix_attention(query, key, value, block_table, actual_seq_lengths_kv
     behind it in its own (as after a fork, which copies a page that is partly
     filled), every other one, and all where the prefix ends in its first page,
     in the first's.  Results are those of ``paged_attention`` where the
-    sequences' rows of the table name the same pages for the prefix, up to the
-    rounding of the softmax's numerators to the input type, which prefixes that
-    are worked on together have in both forms.  A value of the prefix that one
+    sequences' rows of the table name the same pages for the prefix; in the latent
+    form up to the rounding of the softmax's numerators to the input type, which
+    prefixes that are worked on together have at all numbers of heads.  A value of the prefix that one
     row of a family sees and another does not must be finite.
 
     ``min_tokens``: the shortest prefix that is worked on for its family

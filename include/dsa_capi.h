@@ -593,8 +593,9 @@ int dsa_paged_attn(const void* query, const void* query_rope, const void* key, c
  * dsa_paged_prefix_attn_workspace_size.  It is little more than dsa_paged_attn's where no
  * prefix can be worked on together, and at most 512 MB more where some can: beyond
  * that the sequences are worked on so many at a time.
- * Everything else as dsa_paged_attn; the query rows and the tiles of 32 tokens of a
- * table row are fewer than 2^31 as a product.
+ * Everything else as dsa_paged_attn; the blocks of query rows of a key head (256 a
+ * block; 128 in the latent form and at d = 256) and of all sequences, times the tiles
+ * of 32 tokens of a table row, must be fewer than 2^31.
  */
 size_t dsa_paged_prefix_attn_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t n2, int64_t d,
                                             int32_t latent, int64_t max_blocks, int64_t page_size);
