@@ -151,14 +151,17 @@ __device__ __forceinline__ int paged_whole_pages(const PagedAttnParams& p, int t
 // (`own`) names the same page as the first's for the last whole one.  Then it has a
 // page of its own there, as after a fork, which copies a page that is partly filled;
 // rows that leave the prefix out hold anything else.
+// The same on all lanes: the numbers of tiles come from it.
 __device__ __forceinline__ int paged_given(const PagedAttnParams& p, int tokens, const int32_t* own,
                                            const int32_t* first) {
+  tokens = __builtin_amdgcn_readfirstlane(tokens);
   const int whole = paged_whole_pages(p, tokens);
   if (whole == tokens) return tokens;
   unsigned off;
   const unsigned last = paged_split(p, (unsigned)whole, &off) - 1;
-  const int e = own[last];
-  return e == first[last] && e >= 0 && (int64_t)e * p.page < p.kv_rows ? whole : tokens;
+  const int e = __builtin_amdgcn_readfirstlane(own[last]);
+  const bool named = e == __builtin_amdgcn_readfirstlane(first[last]) && e >= 0 && (int64_t)e * p.page < p.kv_rows;
+  return named ? whole : tokens;
 }
 
 struct PagedSeq {
