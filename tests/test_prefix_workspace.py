@@ -86,3 +86,15 @@ def test_prompts_that_would_take_too_much_together(latent):
     same = {k: v for k, v in args.items() if not k.startswith("prefix") and k != "min_tokens"}
     for x, y in zip(got, dsa.paged_attention(**dict(same, block_table=table))):
         assert torch.equal(x, y)
+
+
+def test_any_min_tokens_and_sizes_of_no_call():
+    from dsa_triton_ascend_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    size = _lib.load().dsa_paged_prefix_attn_workspace_bytes
+    a = (32, 64, 64, 8, 128, 0, 512, 64)
+    assert size(*a, -2 ** 63) == size(*a, -1) > size(*a, 2 ** 63 - 1) > 0
+    assert size(*a, 0) == size(*a, 1) == size(*a, 512 * 64) > size(*a, 512 * 64 + 1) == size(*a, 2 ** 31)
+    for i, x in ((0, 0), (0, -1), (1, 2 ** 62), (3, 7), (4, 96), (6, 0), (7, 2 ** 20 + 1)):
+        assert size(*a[:i], x, *a[i + 1:], 1) == 0
