@@ -24,11 +24,11 @@
 // and 43, behind 8192 95 and 52, behind 32768 324 and 83; 8 behind 2048 25 and 29,
 // behind 8192 41 and 35; 16 families of two behind 4096 95 and 87, behind 16384
 // 318 and 240; 16 new tokens of 16 sequences behind 2048 84 and 81.  16 latent
-// heads: 32 sequences behind 8192 tokens 60 and 61, behind 32768 179 and 83; 64
-// behind 8192 101 and 72; 16 families of two behind 16384 100 and 105.
+// heads: 32 sequences behind 8192 tokens 58 and 61, behind 32768 171 and 83; 64
+// behind 8192 97 and 72; 16 families of two behind 16384 96 and 104.
 // From 64 latent rows of a sequence on its own products bound it, and together
-// is hardly faster or slower (32 sequences behind 32768 tokens: 128 heads 311 and
-// 325; 64 heads 194 and 184).  The caller may set the length instead.
+// is hardly faster or slower (32 sequences behind 32768 tokens: 128 heads 310 and
+// 322; 64 heads 194 and 183).  The caller may set the length instead.
 //
 // The rule counts the batch, not what each family saves: near its border it takes
 // the slower way by up to 8 % (the first of the grouped cases, the last of the
@@ -40,8 +40,8 @@
 // sequences of 8000 tokens).
 // What is not worked on together each sequence reads for itself (paged_attn.h),
 // from the pages of the family's first: up to 2 us slower than paged_attention
-// with grouped heads, 2 to 13 % over the latent cache (16 heads, 64 sequences
-// behind 8192 tokens: 89 and 101 us; 128 heads, 32 behind 32768: 304 and 311), for
+// with grouped heads, 2 to 9 % over the latent cache (16 heads, 64 sequences
+// behind 8192 tokens: 89 and 97 us; 128 heads, 32 behind 32768: 301 and 310), for
 // the search for families in every worker.
 //
 // Work.  A job is a block of up to R rows of a family (over its sequences, new
